@@ -149,6 +149,14 @@ SIGNATURES = {
                               _c_int, _c_i64, _c_int, _c_int, _c_int, _c_f, _p, _p]),
     "sla2h_bwd_dkdv": (_c_int, [_p, _p, _p, _p, _p, _p, _p, _p, _c_int, _c_int, _c_int, _c_i64,
                                 _c_int, _c_int, _c_f, _p, _p, _p]),
+    "sla2h_dense_attn_fwd_workspace_bytes": (ctypes.c_size_t, [_c_int, _c_int, _c_int, _c_i64,
+                                                               _c_i64]),
+    "sla2h_dense_attn_fwd": (_c_int, [_p, _p, _p, _p, _p, _p, _c_int, _c_int, _c_int, _c_int,
+                                      _c_i64, _c_i64, _c_int, _c_f, _p, _p, _p, _p]),
+    "sla2h_dense_attn_bwd_workspace_bytes": (ctypes.c_size_t, [_c_int, _c_int, _c_int, _c_int,
+                                                               _c_i64, _c_i64]),
+    "sla2h_dense_attn_bwd": (_c_int, [_p, _p, _p, _p, _p, _p, _p, _p, _p, _c_int, _c_int, _c_int,
+                                      _c_int, _c_i64, _c_i64, _c_int, _c_f, _p, _p, _p, _p, _p]),
 }
 
 _LIB = None

@@ -30,6 +30,8 @@ SOURCES = {
     "attn_train.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1",
                        "-mllvm", "-structurizecfg-skip-uniform-regions=true"],
     "attn_bwd.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
+    "dense_attn.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
+    "dense_attn_bwd.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
     "mla_glue.hip": [],
     "block_train.hip": [],
     "linear_bwd.hip": [],

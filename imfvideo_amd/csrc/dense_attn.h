@@ -1,0 +1,114 @@
+// Shared pieces of the dense attention kernels (forward and backward), gfx950:
+// 32 x 32 x 16 MFMA tiles on 64-channel heads, tiles of 64 rows in LDS.
+//
+// Operand layout of a 32 x 32 x 16 product, lane l = 32 h + r:
+//   A (rows) and B (columns): row / column r, contracted slots 8 h .. 8 h + 7;
+//   C: column r, rows 8 g + 4 h + i in register 4 g + i (g, i = 0 .. 3).
+// A C tile is therefore the B operand of a product that contracts its rows: step s
+// (16 rows) takes registers 8 s .. 8 s + 7, slot j holding row 16 s + 8 (j / 4) + 4 h + j % 4.
+// The A operand of that product reads the other matrix transposed from its row-major tile
+// in LDS (ds_read_b64_tr_b16), rows in the same order.  Probabilities never leave
+// the registers.
+//
+// LDS tile: 64 rows x 128 bytes, the 16-byte chunk c of row r at chunk c ^ (r & 7), so that
+// the 32 rows of an operand read and the 8 rows x 64 bytes of a transposing read
+// spread over all banks.  The tiles are loaded straight into LDS (buffer_load ... lds): the
+// swizzle is applied to the chunk each lane fetches, and rows past the end of a sequence come
+// back as zeros from the buffer's range check, whatever memory holds there.
+#pragma once
+
+#include "common.h"
+
+namespace sla2h {
+
+typedef __attribute__((ext_vector_type(16))) float f32x16;
+
+constexpr int kDD = 64;         // head width
+constexpr int kRowB = 2 * kDD;  // bytes of a row of a head
+constexpr int kTileRows = 64;
+constexpr int kTileB = kTileRows * kRowB;
+
+template <typename T16>
+__device__ inline f32x16 mfma_32x32x16(u32x4 a, u32x4 b, f32x16 c);
+template <>
+__device__ inline f32x16 mfma_32x32x16<BF16>(u32x4 a, u32x4 b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a),
+                                                 __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+template <>
+__device__ inline f32x16 mfma_32x32x16<F16>(u32x4 a, u32x4 b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a),
+                                                __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+
+__device__ inline f32x16 zero16() {
+  f32x16 z;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) z[i] = 0.f;
+  return z;
+}
+
+__device__ inline void dma16(__amdgpu_buffer_rsrc_t rs, void* dst, int voff) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (__attribute__((address_space(3))) void*)dst, 16,
+                                           voff, 0, 0, 0);
+}
+
+// Rows [row0, row0 + n) of a (rows, 64) 16-bit matrix with row stride `ld` bytes as
+// a buffer resource whose range check ends with the last row; n <= 0: empty.
+__device__ inline __amdgpu_buffer_rsrc_t rows_rsrc(const uint16_t* base, int64_t row0, int64_t n,
+                                                   int64_t ld) {
+  const char* p = reinterpret_cast<const char*>(base) + row0 * ld;
+  const int64_t rows = n < kTileRows ? n : kTileRows;
+  return make_rsrc(p, n <= 0 ? 0 : (rows - 1) * ld + kRowB);
+}
+
+// Byte address (within a tile) of the 16-byte chunk c of row r.
+__device__ inline int chunk_addr(int r, int c) { return r * kRowB + ((c ^ (r & 7)) << 4); }
+
+// Row operand (A or B) of rows r0 + (l & 31): step s contracts channels 16 s .. 16 s + 15.
+__device__ inline u32x4 row_frag(const unsigned char* tile, int r0, int s, int l) {
+  return *reinterpret_cast<const u32x4*>(tile + chunk_addr(r0 + (l & 31), 2 * s + (l >> 5)));
+}
+
+// Transposed operand: row = channel 32 mb + (l & 31), contracted over the tile's rows
+// r0 .. r0 + 15 in the order of a C tile's registers (see above).
+__device__ inline u32x4 col_frag(const unsigned char* tile, int r0, int mb, int l) {
+  const int h = l >> 5, gs = (l >> 4) & 1, r = r0 + 4 * h + ((l & 15) >> 2);
+  const int c = 4 * mb + 2 * gs + ((l & 3) >> 1), o = 8 * (l & 1);
+  const u32x2 lo = lds_read_tr16(tile + chunk_addr(r, c) + o);
+  const u32x2 hi = lds_read_tr16(tile + chunk_addr(r + 8, c) + o);
+  return u32x4{lo.x, lo.y, hi.x, hi.y};
+}
+
+// The B operand of step s from a C tile's registers, rounded to 16 bits.
+template <typename T16>
+__device__ inline u32x4 pack_step(const f32x16& p, int s) {
+  return u32x4{pack_pair<T16>(p[8 * s], p[8 * s + 1]), pack_pair<T16>(p[8 * s + 2], p[8 * s + 3]),
+               pack_pair<T16>(p[8 * s + 4], p[8 * s + 5]),
+               pack_pair<T16>(p[8 * s + 6], p[8 * s + 7])};
+}
+
+__device__ inline float swap32_max(float v) {
+  const float2 a = swap32(v);
+  return fmaxf(a.x, a.y);
+}
+__device__ inline float swap32_sum(float v) {
+  const float2 a = swap32(v);
+  return a.x + a.y;
+}
+
+// s_waitcnt vmcnt(n) lgkmcnt(0)
+constexpr int wait_vm_lgkm0(int n) { return (n & 15) | ((n >> 4) << 14) | 0x70; }
+
+// Sequence lengths of batch b, clamped into [0, L]; L without an array.
+__device__ inline int seq_len(const int32_t* lens, int b, int64_t L) {
+  if (!lens) return (int)L;
+  const int n = __builtin_amdgcn_readfirstlane(lens[b]);
+  return n < 0 ? 0 : (n > L ? (int)L : n);
+}
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+constexpr int kNoLimit = 0x7fffffff;
+
+}  // namespace sla2h

@@ -1,0 +1,525 @@
+// Dense softmax attention on 64-channel heads, forward, gfx950.
+//
+//   S = c q k^T over the keys j < k_len (causal: j <= i + k_len - q_len),
+//   o = softmax(S) v,  lse = log sum exp S;  a row without a key: o = 0, lse = -inf.
+//
+// One pass over the keys: O^T += V^T P^T with P = exp2(S - m), row sums beside it, m a
+// running row bound in log2 units.  m moves only when a tile's maximum exceeds it by more
+// than kSlack (a wave-uniform, rarely taken branch rescales the accumulators): the
+// result does not depend on m beyond rounding, and the common path needs no
+// exchange between lanes.  P is rounded to the operands' 16-bit type for the product (an
+// error of half a unit in its last place per term, as the inputs themselves carry); row sums
+// add the fp32 values, so that lse, which the backward builds on, is exact to fp32.
+#include "dense_attn.h"
+
+#include <initializer_list>
+
+namespace sla2h {
+
+namespace {
+
+// Probabilities are held as exp2(S - m + shift) <= 2^(shift + slack).  fp16 spends its
+// exponent range on the small ones (2^-24 to 2^15); bf16 has fp32's range.
+template <typename T16>
+struct Range;
+template <>
+struct Range<BF16> {
+  static constexpr float shift = 0.f, slack = 10.f;
+};
+template <>
+struct Range<F16> {
+  static constexpr float shift = 9.f, slack = 6.f;
+};
+constexpr float kFloor = -1e30f;  // m before the first key (finite: -inf - m stays -inf)
+
+struct DenseFwdArgs {
+  const uint16_t *q, *k, *v;
+  uint16_t* o;
+  float* lse;
+  const int32_t *q_lens, *k_lens;
+  int64_t qb, qh, ql, kb, kh, kl, vb, vh, vl, ob, oh, ol;  // strides in elements
+  int64_t Lq, Lk;
+  int H, Hkv, rep;
+  int causal;
+  float c;  // scale * log2(e)
+  int qtiles;  // query tiles of a head
+  int nwork, per_xcd;
+  // split form
+  float* part;   // [split][B * H * Lq][64] unnormalised sums
+  float2* ml;    // [split][B * H * Lq] (m, l)
+  int splits, units;  // 32-key units of a split
+  int64_t nrows;      // B * H * Lq
+};
+
+// One 32-key x 32-query score tile: mask, running bound, probabilities.  Returns the
+// packed operands of the two product steps.  acc: the O^T tiles to rescale.
+template <typename T16>
+__device__ inline void softmax_tile(f32x16& s, float c, float& m, float& mthr, float& lsum,
+                                    f32x16 (&acc)[2], u32x4 (&p)[2]) {
+  float mx = fmaxf(fmaxf(s[0], s[1]), s[2]);
+#pragma unroll
+  for (int i = 3; i < 15; i += 2) mx = fmaxf(fmaxf(mx, s[i]), s[i + 1]);
+  mx = fmaxf(mx, s[15]);
+  if (__builtin_amdgcn_ballot_w64(mx > mthr)) {
+    const float mn = fmaxf(m, swap32_max(mx) * c);
+    const float f = fast_exp2(m - mn);
+    m = mn;
+    mthr = (mn + Range<T16>::slack) / c;
+    lsum *= f;
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) acc[b][i] *= f;
+  }
+  const float off = Range<T16>::shift - m;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) s[i] = fast_exp2(__builtin_fmaf(s[i], c, off));
+#pragma unroll
+  for (int t = 0; t < 2; ++t) p[t] = pack_step<T16>(s, t);
+  float r[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) r[i] = (s[i] + s[4 + i]) + (s[8 + i] + s[12 + i]);
+  lsum += (r[0] + r[1]) + (r[2] + r[3]);
+}
+
+// scores of keys at or past a lane's limit -> -inf; lim counts from the tile's first key
+__device__ inline void mask_tile(f32x16& s, int lim, int h) {
+  const int x = lim - 4 * h;
+#pragma unroll
+  for (int i = 0; i < 16; ++i)
+    s[i] = 8 * (i >> 2) + (i & 3) < x ? s[i] : -__builtin_inff();
+}
+
+// Keys that query i sees: [0, limit).
+__device__ inline int key_limit(int i, int qlen, int klen, int causal) {
+  if (i >= qlen) return 0;
+  if (!causal) return klen;
+  const int64_t e = (int64_t)i + klen - qlen + 1;
+  return e < 0 ? 0 : (e < klen ? (int)e : klen);
+}
+
+// Workgroup = 4 waves x (32 NQ) query rows of one head; all waves read the key and value
+// tiles of 64 rows from LDS, loaded three slots ahead with one barrier per tile.
+template <typename T16, int NQ>
+__global__ __launch_bounds__(256, 2) void dense_fwd_kernel(DenseFwdArgs a) {
+  __shared__ __align__(16) unsigned char k0[kTileB], k1[kTileB], k2[kTileB];
+  __shared__ __align__(16) unsigned char v0[kTileB], v1[kTileB], v2[kTileB];
+  const int logical = (blockIdx.x & 7) * a.per_xcd + (blockIdx.x >> 3);
+  if (logical >= a.nwork) return;
+  const int bh = __builtin_amdgcn_readfirstlane(logical / a.qtiles);
+  // causal: the longest rows first
+  int qt = __builtin_amdgcn_readfirstlane(logical - bh * a.qtiles);
+  if (a.causal) qt = a.qtiles - 1 - qt;
+  const int b = bh / a.H, hq = bh - b * a.H, hk = hq / a.rep;
+  const int tid = threadIdx.x, l = tid & 63, h = l >> 5;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int qlen = seq_len(a.q_lens, b, a.Lq), klen = seq_len(a.k_lens, b, a.Lk);
+
+  const int q0 = qt * (128 * NQ);           // first row of the workgroup
+  const int qw = q0 + w * (32 * NQ);        // ... of the wave
+  const int qend = min(q0 + 128 * NQ, qlen);
+  const int kmax = qend > q0 ? key_limit(qend - 1, qlen, klen, a.causal) : 0;
+  const int nt = (kmax + kTileRows - 1) / kTileRows;
+
+  const uint16_t* kp = a.k + b * a.kb + hk * a.kh;
+  const uint16_t* vp = a.v + b * a.vb + hk * a.vh;
+  const int64_t kld = a.kl * 2, vld = a.vl * 2;
+  const int lrow = l >> 3, lch = ((l & 7) ^ lrow) << 4;
+  auto load_tile = [&](int t, unsigned char* kt, unsigned char* vt) {
+    const int64_t n = (int64_t)klen - (int64_t)t * kTileRows;
+    const auto rk = rows_rsrc(kp, (int64_t)t * kTileRows, n, kld);
+    const auto rv = rows_rsrc(vp, (int64_t)t * kTileRows, n, vld);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int r = 16 * w + 8 * i;
+      dma16(rk, kt + r * kRowB, (r + lrow) * (int)kld + lch);
+      dma16(rv, vt + r * kRowB, (r + lrow) * (int)vld + lch);
+    }
+  };
+
+  u32x4 qf[NQ][4];
+  int lim[NQ];
+  {
+    const uint16_t* qp = a.q + b * a.qb + hq * a.qh;
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) {
+      const int i = qw + 32 * n + (l & 31);
+      lim[n] = key_limit(i, qlen, klen, a.causal);
+#pragma unroll
+      for (int s = 0; s < 4; ++s)
+        qf[n][s] = i < qlen ? *reinterpret_cast<const u32x4*>(qp + i * a.ql + 16 * s + 8 * h)
+                            : u32x4{0, 0, 0, 0};
+    }
+  }
+  // keys that every query of the wave sees, and that any of them sees
+  const int wlast = min(qw + 32 * NQ, qlen) - 1;
+  const int wany = wlast >= qw ? key_limit(wlast, qlen, klen, a.causal) : 0;
+  const int wall = wlast >= qw ? key_limit(qw, qlen, klen, a.causal) : 0;
+
+  f32x16 acc[NQ][2];
+  float m[NQ], mthr[NQ], lsum[NQ];
+#pragma unroll
+  for (int n = 0; n < NQ; ++n) {
+    acc[n][0] = zero16();
+    acc[n][1] = zero16();
+    m[n] = kFloor;
+    mthr[n] = kFloor;
+    lsum[n] = 0.f;
+  }
+
+  auto compute = [&](int t, const unsigned char* kt, const unsigned char* vt) {
+    const int base = t * kTileRows;
+    if (base >= wany) return;
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb) {
+      u32x4 kf[4];
+#pragma unroll
+      for (int s = 0; s < 4; ++s) kf[s] = row_frag(kt, 32 * kb, s, l);
+      u32x4 p[NQ][2];
+#pragma unroll
+      for (int n = 0; n < NQ; ++n) {
+        f32x16 sc = zero16();
+#pragma unroll
+        for (int s = 0; s < 4; ++s) sc = mfma_32x32x16<T16>(kf[s], qf[n][s], sc);
+        if (base + kTileRows > wall) mask_tile(sc, lim[n] - base - 32 * kb, h);
+        softmax_tile<T16>(sc, a.c, m[n], mthr[n], lsum[n], acc[n], p[n]);
+      }
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+#pragma unroll
+        for (int mb = 0; mb < 2; ++mb) {
+          const u32x4 vf = col_frag(vt, 32 * kb + 16 * s, mb, l);
+#pragma unroll
+          for (int n = 0; n < NQ; ++n) acc[n][mb] = mfma_32x32x16<T16>(vf, p[n][s], acc[n][mb]);
+        }
+    }
+  };
+
+  // Tile t lives in slot t % 3; tiles loaded past the last one are empty (zeros).
+  load_tile(0, k0, v0);
+  load_tile(1, k1, v1);
+  for (int t = 0; t < nt; t += 3) {
+    __builtin_amdgcn_s_waitcnt(wait_vm_lgkm0(4));
+    __builtin_amdgcn_s_barrier();  // tile t has landed, tile t - 1 is read
+    load_tile(t + 2, k2, v2);
+    compute(t, k0, v0);
+    if (t + 1 >= nt) break;
+    __builtin_amdgcn_s_waitcnt(wait_vm_lgkm0(4));
+    __builtin_amdgcn_s_barrier();
+    load_tile(t + 3, k0, v0);
+    compute(t + 1, k1, v1);
+    if (t + 2 >= nt) break;
+    __builtin_amdgcn_s_waitcnt(wait_vm_lgkm0(4));
+    __builtin_amdgcn_s_barrier();
+    load_tile(t + 4, k1, v1);
+    compute(t + 2, k2, v2);
+  }
+  __builtin_amdgcn_s_waitcnt(wait_vm_lgkm0(0));  // no load into this LDS outlives the workgroup
+
+  uint16_t* op = a.o + b * a.ob + hq * a.oh;
+#pragma unroll
+  for (int n = 0; n < NQ; ++n) {
+    const int i = qw + 32 * n + (l & 31);
+    if (i >= a.Lq) continue;
+    const float ls = swap32_sum(lsum[n]);
+    const float inv = ls > 0.f ? 1.f / ls : (ls == 0.f ? 0.f : ls);
+#pragma unroll
+    for (int mb = 0; mb < 2; ++mb)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const u32x2 x{pack_pair<T16>(acc[n][mb][4 * g] * inv, acc[n][mb][4 * g + 1] * inv),
+                      pack_pair<T16>(acc[n][mb][4 * g + 2] * inv, acc[n][mb][4 * g + 3] * inv)};
+        *reinterpret_cast<u32x2*>(op + i * a.ol + 32 * mb + 8 * g + 4 * h) =
+            lim[n] > 0 ? x : u32x2{0, 0};
+      }
+    if (a.lse && h == 0)
+      a.lse[(int64_t)bh * a.Lq + i] =
+          lim[n] > 0 ? (m[n] - Range<T16>::shift + __log2f(ls)) * kLn2 : -__builtin_inff();
+  }
+}
+
+// Few queries: workgroup = 32 rows (of the `rep` query heads that share a key head) over one
+// range of keys; its waves take the 32-key units in turn, each with LDS slots of its own (no
+// barrier in the loop), and their sums are joined in LDS.  With one range the result is final,
+// else a second kernel adds the ranges in order.
+template <typename T16>
+__global__ __launch_bounds__(256, 2) void dense_fwd_split_kernel(DenseFwdArgs a) {
+  constexpr int kUnitB = 32 * kRowB;
+  __shared__ __align__(16) unsigned char kv0[4][2 * kUnitB], kv1[4][2 * kUnitB];
+  __shared__ float mls[4][2][32];
+  const int blk = blockIdx.x / a.splits, sp = blockIdx.x - blk * a.splits;
+  const int bk = __builtin_amdgcn_readfirstlane(blk / a.qtiles);
+  const int qt = __builtin_amdgcn_readfirstlane(blk - bk * a.qtiles);
+  const int b = bk / a.Hkv, hk = bk - b * a.Hkv;
+  const int tid = threadIdx.x, l = tid & 63, h = l >> 5;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int qlen = seq_len(a.q_lens, b, a.Lq), klen = seq_len(a.k_lens, b, a.Lk);
+
+  // row of the group: head hk rep + row / Lq, query row % Lq
+  const int64_t row = (int64_t)qt * 32 + (l & 31);
+  const bool live = row < (int64_t)a.rep * a.Lq;
+  const int hq = hk * a.rep + (live ? (int)(row / a.Lq) : 0);
+  const int i = live ? (int)(row % a.Lq) : 0;
+  const int lim = live ? key_limit(i, qlen, klen, a.causal) : 0;
+  int kmax = lim, kmin = lim;
+#pragma unroll
+  for (int s = 16; s >= 1; s >>= 1) {
+    kmax = max(kmax, __shfl_xor(kmax, s, 64));
+    kmin = min(kmin, __shfl_xor(kmin, s, 64));
+  }
+  kmax = __builtin_amdgcn_readfirstlane(kmax);
+  kmin = __builtin_amdgcn_readfirstlane(kmin);
+
+  const uint16_t* kp = a.k + b * a.kb + hk * a.kh;
+  const uint16_t* vp = a.v + b * a.vb + hk * a.vh;
+  const int64_t kld = a.kl * 2, vld = a.vl * 2;
+  const int lrow = l >> 3, lch = ((l & 7) ^ lrow) << 4;
+  const int64_t u0 = (int64_t)sp * a.units;
+  const int64_t uend = min(u0 + a.units, ((int64_t)kmax + 31) / 32);
+  auto load_unit = [&](int64_t u, unsigned char* kv) {
+    const int64_t n = u < uend ? min((int64_t)klen - u * 32, (int64_t)32) : 0;
+    const auto rk = rows_rsrc(kp, u * 32, n, kld);
+    const auto rv = rows_rsrc(vp, u * 32, n, vld);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      dma16(rk, kv + 8 * j * kRowB, (8 * j + lrow) * (int)kld + lch);
+      dma16(rv, kv + kUnitB + 8 * j * kRowB, (8 * j + lrow) * (int)vld + lch);
+    }
+  };
+
+  u32x4 qf[4];
+  {
+    const uint16_t* qp = a.q + b * a.qb + hq * a.qh + i * a.ql;
+#pragma unroll
+    for (int s = 0; s < 4; ++s)
+      qf[s] = lim > 0 ? *reinterpret_cast<const u32x4*>(qp + 16 * s + 8 * h) : u32x4{0, 0, 0, 0};
+  }
+  f32x16 acc[2] = {zero16(), zero16()};
+  float m = kFloor, mthr = kFloor, lsum = 0.f;
+  auto compute = [&](int64_t u, const unsigned char* kv) {
+    f32x16 sc = zero16();
+#pragma unroll
+    for (int s = 0; s < 4; ++s) sc = mfma_32x32x16<T16>(row_frag(kv, 0, s, l), qf[s], sc);
+    if (u * 32 + 32 > kmin) mask_tile(sc, (int)(lim - u * 32), h);
+    u32x4 p[2];
+    softmax_tile<T16>(sc, a.c, m, mthr, lsum, acc, p);
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+      for (int mb = 0; mb < 2; ++mb)
+        acc[mb] = mfma_32x32x16<T16>(col_frag(kv + kUnitB, 16 * s, mb, l), p[s], acc[mb]);
+  };
+  int64_t u = u0 + w;
+  load_unit(u, kv0[w]);
+  for (; u < uend; u += 8) {
+    load_unit(u + 4, kv1[w]);
+    __builtin_amdgcn_s_waitcnt(wait_vm_lgkm0(8));
+    compute(u, kv0[w]);
+    if (u + 4 >= uend) break;
+    __builtin_amdgcn_s_waitcnt(wait_vm_lgkm0(8));
+    load_unit(u + 8, kv0[w]);
+    __builtin_amdgcn_s_waitcnt(wait_vm_lgkm0(8));
+    compute(u + 4, kv1[w]);
+    __builtin_amdgcn_s_waitcnt(wait_vm_lgkm0(8));
+  }
+  __builtin_amdgcn_s_waitcnt(wait_vm_lgkm0(0));
+
+  // join the four waves: fp32 O^T tiles [channel][row] in the slots' memory
+  lsum = swap32_sum(lsum);
+  if (h == 0) {
+    mls[w][0][l] = m;
+    mls[w][1][l] = lsum;
+  }
+  float* ot = reinterpret_cast<float*>(w < 2 ? kv0[2 * w] : kv1[2 * (w - 2)]);
+  __syncthreads();
+#pragma unroll
+  for (int mb = 0; mb < 2; ++mb)
+#pragma unroll
+    for (int r = 0; r < 16; ++r)
+      ot[(32 * mb + 8 * (r >> 2) + 4 * h + (r & 3)) * 32 + (l & 31)] = acc[mb][r];
+  __syncthreads();
+  // thread: row tid % 32, channels 8 (tid / 32) ..
+  const int r = tid & 31, c0 = (tid >> 5) * 8;
+  float mm = fmaxf(fmaxf(mls[0][0][r], mls[1][0][r]), fmaxf(mls[2][0][r], mls[3][0][r]));
+  float f[4], ll = 0.f, x[8];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    f[j] = fast_exp2(mls[j][0][r] - mm);
+    ll += f[j] * mls[j][1][r];
+  }
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    x[e] = 0.f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float* src = reinterpret_cast<const float*>(j < 2 ? kv0[2 * j] : kv1[2 * (j - 2)]);
+      x[e] += f[j] * src[(c0 + e) * 32 + r];
+    }
+  }
+  const int64_t orow = (int64_t)qt * 32 + r;
+  if (orow >= (int64_t)a.rep * a.Lq) return;
+  const int oh = hk * a.rep + (int)(orow / a.Lq), oi = (int)(orow % a.Lq);
+  const int64_t flat = ((int64_t)b * a.H + oh) * a.Lq + oi;
+  if (a.splits > 1) {
+    float* d = a.part + (sp * a.nrows + flat) * kDD + c0;
+    *reinterpret_cast<f32x4*>(d) = f32x4{x[0], x[1], x[2], x[3]};
+    *reinterpret_cast<f32x4*>(d + 4) = f32x4{x[4], x[5], x[6], x[7]};
+    if (c0 == 0) a.ml[sp * a.nrows + flat] = make_float2(mm, ll);
+    return;
+  }
+  const bool some = key_limit(oi, qlen, klen, a.causal) > 0;
+  const float inv = 1.f / ll;
+  u32x4 y;
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    y[e] = some ? pack_pair<T16>(x[2 * e] * inv, x[2 * e + 1] * inv) : 0u;
+  *reinterpret_cast<u32x4*>(a.o + b * a.ob + oh * a.oh + oi * a.ol + c0) = y;
+  if (a.lse && c0 == 0)
+    a.lse[flat] = some ? (mm - Range<T16>::shift + __log2f(ll)) * kLn2 : -__builtin_inff();
+}
+
+// Adds the key ranges of a row in order; 16 lanes per row, four channels each.
+template <typename T16>
+__global__ __launch_bounds__(256) void dense_join_kernel(DenseFwdArgs a) {
+  const int64_t flat = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
+  if (flat >= a.nrows) return;
+  const int c0 = (threadIdx.x & 15) * 4;
+  const int64_t bh = flat / a.Lq;
+  const int i = (int)(flat - bh * a.Lq), b = (int)(bh / a.H), hq = (int)(bh - (int64_t)b * a.H);
+  const int qlen = a.q_lens ? max(0, (int)min((int64_t)a.q_lens[b], a.Lq)) : (int)a.Lq;
+  const int klen = a.k_lens ? max(0, (int)min((int64_t)a.k_lens[b], a.Lk)) : (int)a.Lk;
+  float mm = kFloor;
+  for (int s = 0; s < a.splits; ++s) mm = fmaxf(mm, a.ml[s * a.nrows + flat].x);
+  float ll = 0.f;
+  f32x4 x{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int s = 0; s < a.splits; ++s) {
+    const float2 ml = a.ml[s * a.nrows + flat];
+    const float f = fast_exp2(ml.x - mm);
+    ll += f * ml.y;
+    x += f * *reinterpret_cast<const f32x4*>(a.part + (s * a.nrows + flat) * kDD + c0);
+  }
+  const bool some = key_limit(i, qlen, klen, a.causal) > 0;
+  const float inv = 1.f / ll;
+  const u32x2 y{some ? pack_pair<T16>(x[0] * inv, x[1] * inv) : 0u,
+                some ? pack_pair<T16>(x[2] * inv, x[3] * inv) : 0u};
+  *reinterpret_cast<u32x2*>(a.o + b * a.ob + hq * a.oh + i * a.ol + c0) = y;
+  if (a.lse && c0 == 0)
+    a.lse[flat] = some ? (mm - Range<T16>::shift + __log2f(ll)) * kLn2 : -__builtin_inff();
+}
+
+// The form of a call: query blocks of 256 or 128 rows with all keys, or the split form.
+struct FwdPlan {
+  int nq;  // 2, 1: dense_fwd_kernel<NQ>; 0: split form
+  int64_t qtiles, nwork;
+  int splits;
+  int64_t units;
+};
+
+FwdPlan fwd_plan(int B, int H, int Hkv, int64_t Lq, int64_t Lk) {
+  FwdPlan p{};
+  const int64_t bh = (int64_t)B * H;
+  for (int nq = 2; nq >= 1; --nq) {
+    p.nq = nq;
+    p.qtiles = (Lq + 128 * nq - 1) / (128 * nq);
+    p.nwork = bh * p.qtiles;
+    p.splits = 1;
+    if (p.nwork >= 256) return p;
+  }
+  p.nq = 0;
+  p.qtiles = ((H / Hkv) * Lq + 31) / 32;
+  const int64_t blocks = (int64_t)B * Hkv * p.qtiles, units = (Lk + 31) / 32;
+  int64_t s = (512 + blocks - 1) / blocks;
+  const int64_t most = units / 8;  // two units per wave and range at least
+  s = s < most ? s : most;
+  p.splits = s < 1 ? 1 : (int)s;
+  p.units = (units + p.splits - 1) / p.splits;
+  p.splits = (int)((units + p.units - 1) / p.units);
+  p.nwork = blocks * p.splits;
+  return p;
+}
+
+bool sizes_ok(int B, int H, int Hkv, int64_t Lq, int64_t Lk) {
+  return B > 0 && H > 0 && Hkv > 0 && H % Hkv == 0 && Lq > 0 && Lk > 0 &&
+         Lq < ((int64_t)1 << 30) && Lk < ((int64_t)1 << 30) &&
+         (int64_t)B * H < ((int64_t)1 << 20) && (H / Hkv) * Lq < ((int64_t)1 << 31);
+}
+
+}  // namespace
+
+}  // namespace sla2h
+
+using namespace sla2h;
+
+extern "C" size_t sla2h_dense_attn_fwd_workspace_bytes(int B, int H, int Hkv, int64_t Lq,
+                                                       int64_t Lk) {
+  if (!sizes_ok(B, H, Hkv, Lq, Lk)) return 0;
+  const FwdPlan p = fwd_plan(B, H, Hkv, Lq, Lk);
+  return p.splits > 1 ? (size_t)p.splits * B * H * Lq * (kDD * 4 + 8) : 0;
+}
+
+extern "C" int sla2h_dense_attn_fwd(const void* q, const void* k, const void* v,
+                                    const int64_t* strides, const int32_t* q_lens,
+                                    const int32_t* k_lens, int dtype, int B, int H, int Hkv,
+                                    int64_t Lq, int64_t Lk, int causal, float scale,
+                                    void* workspace, void* o, float* lse, void* stream) {
+  SLA2H_CHECK_ARG(q && k && v && strides && o);
+  SLA2H_CHECK_ARG(dtype == SLA2H_DTYPE_F16 || dtype == SLA2H_DTYPE_BF16);
+  SLA2H_CHECK_ARG(sizes_ok(B, H, Hkv, Lq, Lk));
+  SLA2H_CHECK_ARG(scale > 0.f && scale < 1e30f);
+  SLA2H_CHECK_ARG(((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)o |
+                   (uintptr_t)workspace) % 16 == 0);
+  SLA2H_CHECK_ARG(((uintptr_t)lse | (uintptr_t)q_lens | (uintptr_t)k_lens) % 4 == 0);
+  for (int i = 0; i < 12; ++i) SLA2H_CHECK_ARG(strides[i] >= 0 && strides[i] % 8 == 0);
+  // rows apart from each other: the range check of a tile's load tells them by their offset
+  for (int i : {2, 5, 8, 11}) SLA2H_CHECK_ARG(strides[i] >= kDD);
+  // 32-bit byte offsets within a tile of 64 rows
+  SLA2H_CHECK_ARG(strides[5] < ((int64_t)1 << 23) && strides[8] < ((int64_t)1 << 23));
+  const FwdPlan p = fwd_plan(B, H, Hkv, Lq, Lk);
+  SLA2H_CHECK_ARG(p.splits == 1 || workspace);
+  SLA2H_CHECK_ARG(p.nwork < ((int64_t)1 << 30));
+  DenseFwdArgs a{};
+  a.q = static_cast<const uint16_t*>(q);
+  a.k = static_cast<const uint16_t*>(k);
+  a.v = static_cast<const uint16_t*>(v);
+  a.o = static_cast<uint16_t*>(o);
+  a.lse = lse;
+  a.q_lens = q_lens;
+  a.k_lens = k_lens;
+  a.qb = strides[0], a.qh = strides[1], a.ql = strides[2];
+  a.kb = strides[3], a.kh = strides[4], a.kl = strides[5];
+  a.vb = strides[6], a.vh = strides[7], a.vl = strides[8];
+  a.ob = strides[9], a.oh = strides[10], a.ol = strides[11];
+  a.Lq = Lq;
+  a.Lk = Lk;
+  a.H = H;
+  a.Hkv = Hkv;
+  a.rep = H / Hkv;
+  a.causal = causal != 0;
+  a.c = scale * kLog2e;
+  a.qtiles = (int)p.qtiles;
+  a.nwork = (int)p.nwork;
+  a.per_xcd = (int)((p.nwork + 7) / 8);
+  a.splits = p.splits;
+  a.units = (int)p.units;
+  a.nrows = (int64_t)B * H * Lq;
+  if (p.splits > 1) {
+    a.part = static_cast<float*>(workspace);
+    a.ml = reinterpret_cast<float2*>(a.part + (int64_t)p.splits * a.nrows * kDD);
+  }
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  auto go = [&](auto tag) -> int {
+    using T16 = decltype(tag);
+    if (p.nq == 2)
+      dense_fwd_kernel<T16, 2><<<8 * a.per_xcd, 256, 0, st>>>(a);
+    else if (p.nq == 1)
+      dense_fwd_kernel<T16, 1><<<8 * a.per_xcd, 256, 0, st>>>(a);
+    else
+      dense_fwd_split_kernel<T16><<<a.nwork, 256, 0, st>>>(a);
+    const int err = (int)hipGetLastError();
+    if (err || p.splits == 1) return err;
+    dense_join_kernel<T16><<<(unsigned)((a.nrows + 15) / 16), 256, 0, st>>>(a);
+    return (int)hipGetLastError();
+  };
+  return dtype == SLA2H_DTYPE_BF16 ? go(BF16{}) : go(F16{});
+}

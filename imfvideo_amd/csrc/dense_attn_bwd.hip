@@ -1,0 +1,656 @@
+// Backward of dense softmax attention on 64-channel heads, gfx950.  The probabilities
+// are recomputed from the rows' log-sum-exp:
+//
+//   P_ij = exp(S_ij - lse_i),  delta_i = do_i . o_i,  dP = do v^T,  dS = P (dP - delta),
+//   dq = scale dS k,  dk = scale dS^T q,  dv = P^T do   (summed over a key head's queries).
+//
+// Three kernels: the rows' delta; dq with a workgroup per query block (keys streamed
+// through LDS); dk and dv with a workgroup per key block (queries streamed through LDS).
+// Seven tile products instead of the five of one fused pass, but no sum goes through
+// atomics or memory: the result does not depend on the order of dispatch.
+//
+// fp16 operands: P (down to 1 / length) and dS would fall below fp16's normal range, so the
+// exponent takes + kShift and dP - delta a power of two from the bound
+// |dP - delta| <= 2 max|do_i| max|v_j| (row norms, per key head), which brings |dS| below
+// 2^kShift; both are taken out of the fp32 sums again.  bf16 has fp32's range and needs
+// neither.
+#include "dense_attn.h"
+
+#include <initializer_list>
+
+namespace sla2h {
+
+namespace {
+
+template <typename T16>
+struct Shift {
+  static constexpr bool scaled = false;
+  static constexpr float p = 0.f;
+};
+template <>
+struct Shift<F16> {
+  static constexpr bool scaled = true;
+  static constexpr float p = 15.f;
+};
+
+constexpr int kNormRows = 256;  // rows of a partial maximum of the norms
+
+struct DenseBwdArgs {
+  const uint16_t *q, *k, *v, *o, *dout;
+  const float* lse;
+  uint16_t *dq, *dk, *dv;
+  const int32_t *q_lens, *k_lens;
+  int64_t qb, qh, ql, kb, kh, kl, vb, vh, vl, ob, oh, ol, gb, gh, gl;
+  int64_t dqb, dqh, dql, dkb, dkh, dkl, dvb, dvh, dvl;
+  int64_t Lq, Lk;
+  int H, Hkv, rep, nbh, nbk;
+  int causal;
+  float c, inv_c, scale;
+  float *nlse, *ndelta;  // (B, H, Lq): -(lse log2e - shift) / c and -delta
+  float *gmax, *vmax;    // (B, H, nqb), (B, Hkv, nkb): largest row norms (fp16)
+  int nqb, nkb;
+  // dq
+  int qtiles, dq_splits, dq_nwork, dq_per_xcd;
+  // dk, dv
+  int ktiles, kv_splits, kv_nwork, kv_per_xcd;
+  float* part;
+};
+
+// Queries [first, qlen) see a key.
+__device__ inline int first_query(int qlen, int klen, int causal) {
+  if (klen == 0) return qlen;
+  return causal && qlen > klen ? qlen - klen : 0;
+}
+
+// delta of 256 rows of a head (8 lanes per row), and for fp16 the largest row norm of
+// do; the workgroups behind them take the norms of v.
+template <typename T16>
+__global__ __launch_bounds__(256) void dense_bwd_prep_kernel(DenseBwdArgs a, int64_t nq) {
+  __shared__ float red[4];
+  const int tid = threadIdx.x, c0 = (tid & 7) * 8;
+  const bool is_v = blockIdx.x >= nq;
+  const int64_t blk = is_v ? blockIdx.x - nq : blockIdx.x;
+  const int nb = is_v ? a.nkb : a.nqb, heads = is_v ? a.Hkv : a.H;
+  const int64_t bh = blk / nb;
+  const int t = (int)(blk - bh * nb), b = (int)(bh / heads), hh = (int)(bh - (int64_t)b * heads);
+  const int qlen = seq_len(a.q_lens, b, a.Lq), klen = seq_len(a.k_lens, b, a.Lk);
+  const int len = is_v ? klen : qlen;
+  const int first = is_v ? 0 : first_query(qlen, klen, a.causal);
+  float top = 0.f;
+#pragma unroll 2
+  for (int j = 0; j < kNormRows / 32; ++j) {
+    const int64_t i = (int64_t)t * kNormRows + 32 * j + (tid >> 3);
+    float dot = 0.f, nrm = 0.f;
+    if (i >= first && i < len) {
+      const u32x4 g = *reinterpret_cast<const u32x4*>(
+          is_v ? a.v + b * a.vb + hh * a.vh + i * a.vl + c0
+               : a.dout + b * a.gb + hh * a.gh + i * a.gl + c0);
+      u32x4 o{0, 0, 0, 0};
+      if (!is_v) o = *reinterpret_cast<const u32x4*>(a.o + b * a.ob + hh * a.oh + i * a.ol + c0);
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          const float gv = T16::to_f32((uint16_t)(g[e] >> (16 * x)));
+          dot += gv * T16::to_f32((uint16_t)(o[e] >> (16 * x)));
+          nrm += gv * gv;
+        }
+    }
+#pragma unroll
+    for (int s = 4; s >= 1; s >>= 1) {
+      dot += __shfl_xor(dot, s, 64);
+      if (Shift<T16>::scaled) nrm += __shfl_xor(nrm, s, 64);
+    }
+    top = fmaxf(top, nrm);
+    if (!is_v && c0 == 0 && i < a.Lq) {
+      const bool live = i >= first && i < len;
+      const int64_t f = bh * a.Lq + i;
+      a.ndelta[f] = live ? -dot : 0.f;
+      a.nlse[f] = live ? (Shift<T16>::p - a.lse[f] * kLog2e) * a.inv_c : -__builtin_inff();
+    }
+  }
+  if (Shift<T16>::scaled) {
+    top = wave_max(top);
+    if ((tid & 63) == 0) red[tid >> 6] = top;
+    __syncthreads();
+    if (tid == 0)
+      (is_v ? a.vmax : a.gmax)[blk] =
+          sqrtf(fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3])));
+  }
+}
+
+// fp16: the power of two m with 2 max|do| max|v| m <= 1 for a key head's group.
+__device__ inline float ds_scale(const DenseBwdArgs& a, int b, int hk) {
+  const int tid = threadIdx.x, l = tid & 63;
+  const int64_t ng = (int64_t)a.rep * a.nqb;
+  const float* g = a.gmax + ((int64_t)b * a.H + (int64_t)hk * a.rep) * a.nqb;
+  const float* v = a.vmax + ((int64_t)b * a.Hkv + hk) * a.nkb;
+  float mg = 0.f, mv = 0.f;
+  for (int64_t i = l; i < ng; i += 64) mg = fmaxf(mg, g[i]);
+  for (int i = l; i < a.nkb; i += 64) mv = fmaxf(mv, v[i]);
+  const float bound = 2.f * wave_max(mg) * wave_max(mv);
+  if (!(bound > 0.f) || !(bound < 1e38f)) return 1.f;
+  int e;
+  (void)frexpf(bound, &e);  // bound < 2^e
+  e = e < -100 ? -100 : e;
+  return __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane((127 - e) << 23));
+}
+
+// A C tile pair (dO^T-like, [channel][row]) of a lane's row, 16-bit or fp32 parts.
+template <typename T16>
+__device__ inline void store_row(uint16_t* p, const f32x16 (&x)[2], float f, int h, bool keep) {
+#pragma unroll
+  for (int mb = 0; mb < 2; ++mb)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const u32x2 y{pack_pair<T16>(x[mb][4 * g] * f, x[mb][4 * g + 1] * f),
+                    pack_pair<T16>(x[mb][4 * g + 2] * f, x[mb][4 * g + 3] * f)};
+      *reinterpret_cast<u32x2*>(p + 32 * mb + 8 * g + 4 * h) = keep ? y : u32x2{0, 0};
+    }
+}
+__device__ inline void store_part(float* p, const f32x16 (&x)[2], float f, int h, bool keep) {
+#pragma unroll
+  for (int mb = 0; mb < 2; ++mb)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      f32x4 y;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) y[i] = keep ? x[mb][4 * g + i] * f : 0.f;
+      *reinterpret_cast<f32x4*>(p + 32 * mb + 8 * g + 4 * h) = y;
+    }
+}
+
+// dq: workgroup = 4 waves x (32 NQ) query rows; keys and values as in the forward.
+// dQ^T += K^T dS^T with dS^T straight from the score tile's registers.
+template <typename T16, int NQ>
+__global__ __launch_bounds__(256, 2) void dense_bwd_dq_kernel(DenseBwdArgs a) {
+  __shared__ __align__(16) unsigned char k0[kTileB], k1[kTileB], k2[kTileB];
+  __shared__ __align__(16) unsigned char v0[kTileB], v1[kTileB], v2[kTileB];
+  const int logical = (blockIdx.x & 7) * a.dq_per_xcd + (blockIdx.x >> 3);
+  if (logical >= a.dq_nwork) return;
+  const int per_bh = a.qtiles * a.dq_splits;
+  const int bh = __builtin_amdgcn_readfirstlane(logical / per_bh);
+  const int rest = __builtin_amdgcn_readfirstlane(logical - bh * per_bh);
+  int qt = rest / a.dq_splits;
+  const int sp = rest - qt * a.dq_splits;
+  if (a.causal) qt = a.qtiles - 1 - qt;
+  const int b = bh / a.H, hq = bh - b * a.H, hk = hq / a.rep;
+  const int tid = threadIdx.x, l = tid & 63, h = l >> 5;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int qlen = seq_len(a.q_lens, b, a.Lq), klen = seq_len(a.k_lens, b, a.Lk);
+
+  const int q0 = qt * (128 * NQ), qw = q0 + w * (32 * NQ);
+  const int qend = min(q0 + 128 * NQ, qlen);
+  auto limit = [&](int i) {
+    if (i >= qlen) return 0;
+    if (!a.causal) return klen;
+    const int64_t e = (int64_t)i + klen - qlen + 1;
+    return e < 0 ? 0 : (e < klen ? (int)e : klen);
+  };
+  const int kmax = qend > q0 ? limit(qend - 1) : 0;
+  const int ntile = (kmax + kTileRows - 1) / kTileRows;
+  const int per = (ntile + a.dq_splits - 1) / a.dq_splits;
+  const int t0 = sp * per, nt = min(ntile, t0 + per);
+
+  const uint16_t* kp = a.k + b * a.kb + hk * a.kh;
+  const uint16_t* vp = a.v + b * a.vb + hk * a.vh;
+  const int64_t kld = a.kl * 2, vld = a.vl * 2;
+  const int lrow = l >> 3, lch = ((l & 7) ^ lrow) << 4;
+  auto load_tile = [&](int t, unsigned char* kt, unsigned char* vt) {
+    const int64_t n = (int64_t)klen - (int64_t)t * kTileRows;
+    const auto rk = rows_rsrc(kp, (int64_t)t * kTileRows, n, kld);
+    const auto rv = rows_rsrc(vp, (int64_t)t * kTileRows, n, vld);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int r = 16 * w + 8 * i;
+      dma16(rk, kt + r * kRowB, (r + lrow) * (int)kld + lch);
+      dma16(rv, vt + r * kRowB, (r + lrow) * (int)vld + lch);
+    }
+  };
+
+  float mul = 1.f;
+  if (Shift<T16>::scaled) mul = ds_scale(a, b, hk);
+  u32x4 qf[NQ][4], gf[NQ][4];
+  int lim[NQ];
+  float nl[NQ], nd[NQ];  // shift - lse log2e, -delta (times mul)
+  {
+    const uint16_t* qp = a.q + b * a.qb + hq * a.qh;
+    const uint16_t* gp = a.dout + b * a.gb + hq * a.gh;
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) {
+      const int i = qw + 32 * n + (l & 31);
+      lim[n] = limit(i);
+      const bool live = lim[n] > 0;
+      nl[n] = live ? a.nlse[(int64_t)bh * a.Lq + i] * a.c : -__builtin_inff();
+      nd[n] = live ? a.ndelta[(int64_t)bh * a.Lq + i] * mul : 0.f;
+#pragma unroll
+      for (int s = 0; s < 4; ++s) {
+        qf[n][s] = live ? *reinterpret_cast<const u32x4*>(qp + i * a.ql + 16 * s + 8 * h)
+                        : u32x4{0, 0, 0, 0};
+        gf[n][s] = live ? *reinterpret_cast<const u32x4*>(gp + i * a.gl + 16 * s + 8 * h)
+                        : u32x4{0, 0, 0, 0};
+      }
+    }
+  }
+  const int wlast = min(qw + 32 * NQ, qlen) - 1;
+  const int wany = wlast >= qw ? limit(wlast) : 0;
+  const int wall = wlast >= qw ? limit(qw) : 0;
+
+  f32x16 acc[NQ][2];
+#pragma unroll
+  for (int n = 0; n < NQ; ++n) acc[n][0] = acc[n][1] = zero16();
+
+  auto compute = [&](int t, const unsigned char* kt, const unsigned char* vt) {
+    const int base = t * kTileRows;
+    if (base >= wany) return;
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb) {
+      u32x4 kf[4], vf[4];
+#pragma unroll
+      for (int s = 0; s < 4; ++s) {
+        kf[s] = row_frag(kt, 32 * kb, s, l);
+        vf[s] = row_frag(vt, 32 * kb, s, l);
+      }
+      u32x4 ds[NQ][2];
+#pragma unroll
+      for (int n = 0; n < NQ; ++n) {
+        f32x16 sc = zero16(), dp = zero16();
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+          sc = mfma_32x32x16<T16>(kf[s], qf[n][s], sc);
+          dp = mfma_32x32x16<T16>(vf[s], gf[n][s], dp);
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const float p = fast_exp2(__builtin_fmaf(sc[i], a.c, nl[n]));
+          dp[i] = p * (Shift<T16>::scaled ? __builtin_fmaf(dp[i], mul, nd[n]) : dp[i] + nd[n]);
+        }
+        if (base + kTileRows > wall) {
+          const int x = lim[n] - base - 32 * kb - 4 * h;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) dp[i] = 8 * (i >> 2) + (i & 3) < x ? dp[i] : 0.f;
+        }
+        ds[n][0] = pack_step<T16>(dp, 0);
+        ds[n][1] = pack_step<T16>(dp, 1);
+      }
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+#pragma unroll
+        for (int mb = 0; mb < 2; ++mb) {
+          const u32x4 kc = col_frag(kt, 32 * kb + 16 * s, mb, l);
+#pragma unroll
+          for (int n = 0; n < NQ; ++n) acc[n][mb] = mfma_32x32x16<T16>(kc, ds[n][s], acc[n][mb]);
+        }
+    }
+  };
+
+  load_tile(t0, k0, v0);
+  load_tile(t0 + 1, k1, v1);
+  for (int t = t0; t < nt; t += 3) {
+    __builtin_amdgcn_s_waitcnt(wait_vm_lgkm0(4));
+    __builtin_amdgcn_s_barrier();
+    load_tile(t + 2, k2, v2);
+    compute(t, k0, v0);
+    if (t + 1 >= nt) break;
+    __builtin_amdgcn_s_waitcnt(wait_vm_lgkm0(4));
+    __builtin_amdgcn_s_barrier();
+    load_tile(t + 3, k0, v0);
+    compute(t + 1, k1, v1);
+    if (t + 2 >= nt) break;
+    __builtin_amdgcn_s_waitcnt(wait_vm_lgkm0(4));
+    __builtin_amdgcn_s_barrier();
+    load_tile(t + 4, k1, v1);
+    compute(t + 2, k2, v2);
+  }
+  __builtin_amdgcn_s_waitcnt(wait_vm_lgkm0(0));
+
+  const float f = Shift<T16>::scaled ? a.scale * (1.f / 32768.f) / mul : a.scale;
+#pragma unroll
+  for (int n = 0; n < NQ; ++n) {
+    const int i = qw + 32 * n + (l & 31);
+    if (i >= a.Lq) continue;
+    if (a.dq_splits == 1)
+      store_row<T16>(a.dq + b * a.dqb + hq * a.dqh + i * a.dql, acc[n], f, h, lim[n] > 0);
+    else
+      store_part(a.part + (((int64_t)sp * a.nbh + bh) * a.Lq + i) * kDD, acc[n], f, h,
+                 lim[n] > 0);
+  }
+}
+
+// dk, dv: workgroup = 4 waves x (32 NK) keys of one key head; the query rows of the heads
+// that read it are streamed through LDS in tiles of 64 with their -lse and -delta,
+// which start the accumulators of S and dP.
+template <typename T16, int NK>
+__global__ __launch_bounds__(256, NK == 1 ? 2 : 1) void dense_bwd_dkdv_kernel(DenseBwdArgs a) {
+  __shared__ __align__(16) unsigned char q0_[kTileB], q1_[kTileB], q2_[kTileB];
+  __shared__ __align__(16) unsigned char g0_[kTileB], g1_[kTileB], g2_[kTileB];
+  __shared__ __align__(16) float s0_[2][64], s1_[2][64], s2_[2][64];
+  const int logical = (blockIdx.x & 7) * a.kv_per_xcd + (blockIdx.x >> 3);
+  if (logical >= a.kv_nwork) return;
+  const int per_bk = a.ktiles * a.kv_splits;
+  const int bk = __builtin_amdgcn_readfirstlane(logical / per_bk);
+  const int rest = __builtin_amdgcn_readfirstlane(logical - bk * per_bk);
+  const int ktile = rest / a.kv_splits, sp = rest - ktile * a.kv_splits;
+  const int b = bk / a.Hkv, hk = bk - b * a.Hkv;
+  const int tid = threadIdx.x, l = tid & 63, h = l >> 5;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int qlen = seq_len(a.q_lens, b, a.Lq), klen = seq_len(a.k_lens, b, a.Lk);
+
+  const int key0 = ktile * (128 * NK), kw = key0 + w * (32 * NK);
+  // first query that sees a key of the workgroup (causal: i >= j - off)
+  const int off = klen - qlen;
+  int first = first_query(qlen, klen, a.causal);
+  if (a.causal) first = max(first, key0 - off);
+  const int nq = key0 < klen && first < qlen ? (qlen - first + kTileRows - 1) / kTileRows : 0;
+  const int total = nq * a.rep;  // (head, query tile) pairs
+  const int per = (total + a.kv_splits - 1) / a.kv_splits;
+  const int u0 = sp * per, u1 = min(total, u0 + per);
+
+  const int64_t qld = a.ql * 2, gld = a.gl * 2;
+  const int lrow = l >> 3, lch = ((l & 7) ^ lrow) << 4;
+  auto load_tile = [&](int u, unsigned char* qt, unsigned char* gt, float (*st)[64]) {
+    const int r = u < u1 ? u / nq : 0;
+    const int hq = hk * a.rep + r;
+    const int row = first + (u - r * nq) * kTileRows;
+    const int64_t n = u < u1 ? (int64_t)qlen - row : 0;
+    const auto rq = rows_rsrc(a.q + b * a.qb + hq * a.qh, row, n, qld);
+    const auto rg = rows_rsrc(a.dout + b * a.gb + hq * a.gh, row, n, gld);
+    const float* stat = (w & 1) ? a.ndelta : a.nlse;
+    const auto rs = make_rsrc(stat + ((int64_t)b * a.H + hq) * a.Lq + row,
+                              n <= 0 ? 0 : (n < 64 ? n : 64) * 4);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int rr = 16 * w + 8 * i;
+      dma16(rq, qt + rr * kRowB, (rr + lrow) * (int)qld + lch);
+      dma16(rg, gt + rr * kRowB, (rr + lrow) * (int)gld + lch);
+    }
+    // waves 0 and 2 bring -lse, 1 and 3 -delta (the same values twice)
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(
+        rs, (__attribute__((address_space(3))) void*)&st[w & 1][0], 4, 4 * l, 0, 0, 0);
+  };
+
+  float mul = 1.f;
+  if (Shift<T16>::scaled) mul = ds_scale(a, b, hk);
+  u32x4 kf[NK][4], vf[NK][4];
+#pragma unroll
+  for (int n = 0; n < NK; ++n) {
+    const int j = kw + 32 * n + (l & 31);
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      const bool live = j < klen;
+      kf[n][s] = live ? *reinterpret_cast<const u32x4*>(a.k + b * a.kb + hk * a.kh + j * a.kl +
+                                                        16 * s + 8 * h)
+                      : u32x4{0, 0, 0, 0};
+      vf[n][s] = live ? *reinterpret_cast<const u32x4*>(a.v + b * a.vb + hk * a.vh + j * a.vl +
+                                                        16 * s + 8 * h)
+                      : u32x4{0, 0, 0, 0};
+    }
+  }
+  f32x16 ak[NK][2], av[NK][2];
+#pragma unroll
+  for (int n = 0; n < NK; ++n) ak[n][0] = ak[n][1] = av[n][0] = av[n][1] = zero16();
+
+  auto compute = [&](int u, const unsigned char* qt, const unsigned char* gt,
+                     const float (*st)[64]) {
+    const int row = first + (u % nq) * kTileRows;
+    if (kw >= klen) return;
+#pragma unroll
+    for (int qb = 0; qb < 2; ++qb) {
+      u32x4 qa[4], ga[4];
+#pragma unroll
+      for (int s = 0; s < 4; ++s) {
+        qa[s] = row_frag(qt, 32 * qb, s, l);
+        ga[s] = row_frag(gt, 32 * qb, s, l);
+      }
+      u32x4 p[NK][2], ds[NK][2];
+#pragma unroll
+      for (int n = 0; n < NK; ++n) {
+        f32x16 sc, dp;
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const f32x4 x = *reinterpret_cast<const f32x4*>(&st[0][32 * qb + 8 * g + 4 * h]);
+          const f32x4 y = *reinterpret_cast<const f32x4*>(&st[1][32 * qb + 8 * g + 4 * h]);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            sc[4 * g + i] = x[i];
+            dp[4 * g + i] = y[i];
+          }
+        }
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+          sc = mfma_32x32x16<T16>(qa[s], kf[n][s], sc);
+          dp = mfma_32x32x16<T16>(ga[s], vf[n][s], dp);
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) sc[i] = fast_exp2(sc[i] * a.c);
+        if (a.causal && row + 32 * qb < kw + 32 * n + 31 - off) {
+          const int x = kw + 32 * n + (l & 31) - off - row - 32 * qb - 4 * h;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) sc[i] = 8 * (i >> 2) + (i & 3) >= x ? sc[i] : 0.f;
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          dp[i] = (Shift<T16>::scaled ? sc[i] * mul : sc[i]) * dp[i];
+        p[n][0] = pack_step<T16>(sc, 0);
+        p[n][1] = pack_step<T16>(sc, 1);
+        ds[n][0] = pack_step<T16>(dp, 0);
+        ds[n][1] = pack_step<T16>(dp, 1);
+      }
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+#pragma unroll
+        for (int mb = 0; mb < 2; ++mb) {
+          const u32x4 gc = col_frag(gt, 32 * qb + 16 * s, mb, l);
+          const u32x4 qc = col_frag(qt, 32 * qb + 16 * s, mb, l);
+#pragma unroll
+          for (int n = 0; n < NK; ++n) {
+            av[n][mb] = mfma_32x32x16<T16>(gc, p[n][s], av[n][mb]);
+            ak[n][mb] = mfma_32x32x16<T16>(qc, ds[n][s], ak[n][mb]);
+          }
+        }
+    }
+  };
+
+  load_tile(u0, q0_, g0_, s0_);
+  load_tile(u0 + 1, q1_, g1_, s1_);
+  for (int u = u0; u < u1; u += 3) {
+    __builtin_amdgcn_s_waitcnt(wait_vm_lgkm0(5));
+    __builtin_amdgcn_s_barrier();
+    load_tile(u + 2, q2_, g2_, s2_);
+    compute(u, q0_, g0_, s0_);
+    if (u + 1 >= u1) break;
+    __builtin_amdgcn_s_waitcnt(wait_vm_lgkm0(5));
+    __builtin_amdgcn_s_barrier();
+    load_tile(u + 3, q0_, g0_, s0_);
+    compute(u + 1, q1_, g1_, s1_);
+    if (u + 2 >= u1) break;
+    __builtin_amdgcn_s_waitcnt(wait_vm_lgkm0(5));
+    __builtin_amdgcn_s_barrier();
+    load_tile(u + 4, q1_, g1_, s1_);
+    compute(u + 2, q2_, g2_, s2_);
+  }
+  __builtin_amdgcn_s_waitcnt(wait_vm_lgkm0(0));
+
+  const float fv = Shift<T16>::scaled ? 1.f / 32768.f : 1.f;
+  const float fk = Shift<T16>::scaled ? a.scale * (1.f / 32768.f) / mul : a.scale;
+#pragma unroll
+  for (int n = 0; n < NK; ++n) {
+    const int j = kw + 32 * n + (l & 31);
+    if (j >= a.Lk) continue;
+    const bool keep = j < klen;
+    if (a.kv_splits == 1) {
+      store_row<T16>(a.dk + b * a.dkb + hk * a.dkh + j * a.dkl, ak[n], fk, h, keep);
+      store_row<T16>(a.dv + b * a.dvb + hk * a.dvh + j * a.dvl, av[n], fv, h, keep);
+    } else {
+      float* d = a.part + (((int64_t)sp * a.nbk + bk) * a.Lk + j) * (2 * kDD);
+      store_part(d, ak[n], fk, h, keep);
+      store_part(d + kDD, av[n], fv, h, keep);
+    }
+  }
+}
+
+// Adds the parts of a row of W = 64 (dq) or 128 (dk | dv) channels in order.
+template <typename T16, int W>
+__global__ __launch_bounds__(256) void dense_bwd_join_kernel(const float* __restrict__ part,
+                                                             int splits, int64_t nrows, int64_t L,
+                                                             int heads, uint16_t* y0, int64_t b0,
+                                                             int64_t h0, int64_t l0, uint16_t* y1,
+                                                             int64_t b1, int64_t h1, int64_t l1) {
+  const int64_t e = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+  if (e >= nrows * W) return;
+  const int64_t row = e / W, bh = row / L, i = row - bh * L;
+  const int c = (int)(e - row * W);
+  const int64_t b = bh / heads, hh = bh - b * heads;
+  f32x4 x{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int s = 0; s < splits; ++s)
+    x += *reinterpret_cast<const f32x4*>(part + (s * nrows + row) * W + c);
+  const u32x2 y{pack_pair<T16>(x[0], x[1]), pack_pair<T16>(x[2], x[3])};
+  uint16_t* d = W == 64 || c < 64 ? y0 + b * b0 + hh * h0 + i * l0 + c
+                                  : y1 + b * b1 + hh * h1 + i * l1 + (c - 64);
+  *reinterpret_cast<u32x2*>(d) = y;
+}
+
+struct BwdPlan {
+  int nq;  // query rows of a dq workgroup: 128 nq
+  int64_t qtiles, dq_nwork, ktiles, kv_nwork;
+  int dq_splits, kv_splits;
+  int64_t nqb, nkb;
+  size_t stats, parts;  // floats
+};
+
+BwdPlan bwd_plan(int dtype, int B, int H, int Hkv, int64_t Lq, int64_t Lk) {
+  BwdPlan p{};
+  const int64_t bh = (int64_t)B * H, bk = (int64_t)B * Hkv, rep = H / Hkv;
+  p.nq = bh * ((Lq + 255) / 256) >= 256 ? 2 : 1;
+  p.qtiles = (Lq + 128 * p.nq - 1) / (128 * p.nq);
+  auto split = [](int64_t blocks, int64_t tiles) {
+    if (blocks >= 256) return 1;
+    const int64_t s = (512 + blocks - 1) / blocks, most = tiles / 2;
+    return (int)(s < most ? s : (most < 1 ? 1 : most));
+  };
+  p.dq_splits = split(bh * p.qtiles, (Lk + 63) / 64);
+  p.dq_nwork = bh * p.qtiles * p.dq_splits;
+  p.ktiles = (Lk + 127) / 128;
+  p.kv_splits = split(bk * p.ktiles, rep * ((Lq + 63) / 64));
+  p.kv_nwork = bk * p.ktiles * p.kv_splits;
+  p.nqb = (Lq + kNormRows - 1) / kNormRows;
+  p.nkb = (Lk + kNormRows - 1) / kNormRows;
+  p.stats = 2 * bh * Lq + (dtype == SLA2H_DTYPE_F16 ? bh * p.nqb + bk * p.nkb : 0);
+  p.stats = (p.stats + 3) & ~(size_t)3;
+  const size_t pq = p.dq_splits > 1 ? (size_t)p.dq_splits * bh * Lq * kDD : 0;
+  const size_t pk = p.kv_splits > 1 ? (size_t)p.kv_splits * bk * Lk * 2 * kDD : 0;
+  p.parts = pq > pk ? pq : pk;
+  return p;
+}
+
+bool sizes_ok(int B, int H, int Hkv, int64_t Lq, int64_t Lk) {
+  return B > 0 && H > 0 && Hkv > 0 && H % Hkv == 0 && Lq > 0 && Lk > 0 &&
+         Lq < ((int64_t)1 << 30) && Lk < ((int64_t)1 << 30) && (int64_t)B * H < 65536 &&
+         (H / Hkv) * ((Lq + 63) / 64) < ((int64_t)1 << 30);
+}
+
+}  // namespace
+
+}  // namespace sla2h
+
+using namespace sla2h;
+
+extern "C" size_t sla2h_dense_attn_bwd_workspace_bytes(int dtype, int B, int H, int Hkv,
+                                                       int64_t Lq, int64_t Lk) {
+  if (!sizes_ok(B, H, Hkv, Lq, Lk)) return 0;
+  const BwdPlan p = bwd_plan(dtype, B, H, Hkv, Lq, Lk);
+  return (p.stats + p.parts) * 4;
+}
+
+extern "C" int sla2h_dense_attn_bwd(const void* q, const void* k, const void* v, const void* o,
+                                    const void* dout, const float* lse, const int64_t* strides,
+                                    const int32_t* q_lens, const int32_t* k_lens, int dtype,
+                                    int B, int H, int Hkv, int64_t Lq, int64_t Lk, int causal,
+                                    float scale, void* workspace, void* dq, void* dk, void* dv,
+                                    void* stream) {
+  SLA2H_CHECK_ARG(q && k && v && o && dout && lse && strides && workspace && dq && dk && dv);
+  SLA2H_CHECK_ARG(dtype == SLA2H_DTYPE_F16 || dtype == SLA2H_DTYPE_BF16);
+  SLA2H_CHECK_ARG(sizes_ok(B, H, Hkv, Lq, Lk));
+  SLA2H_CHECK_ARG(scale > 0.f && scale < 1e30f);
+  SLA2H_CHECK_ARG(((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)o | (uintptr_t)dout |
+                   (uintptr_t)workspace | (uintptr_t)dq | (uintptr_t)dk | (uintptr_t)dv) % 16 == 0);
+  SLA2H_CHECK_ARG(((uintptr_t)lse | (uintptr_t)q_lens | (uintptr_t)k_lens) % 4 == 0);
+  for (int i = 0; i < 24; ++i) SLA2H_CHECK_ARG(strides[i] >= 0 && strides[i] % 8 == 0);
+  // rows apart from each other: the range check of a tile's load tells them by their offset
+  for (int i : {2, 5, 8, 11, 14, 17, 20, 23}) SLA2H_CHECK_ARG(strides[i] >= kDD);
+  // 32-bit byte offsets within a tile of 64 rows
+  for (int i : {2, 5, 8, 14}) SLA2H_CHECK_ARG(strides[i] < ((int64_t)1 << 23));
+  const BwdPlan p = bwd_plan(dtype, B, H, Hkv, Lq, Lk);
+  SLA2H_CHECK_ARG(p.dq_nwork < ((int64_t)1 << 30) && p.kv_nwork < ((int64_t)1 << 30));
+  const int64_t bh = (int64_t)B * H, bk = (int64_t)B * Hkv;
+  const int64_t pq = bh * p.nqb, pv = dtype == SLA2H_DTYPE_F16 ? bk * p.nkb : 0;
+  SLA2H_CHECK_ARG(pq + pv < ((int64_t)1 << 31));
+  DenseBwdArgs a{};
+  a.q = static_cast<const uint16_t*>(q);
+  a.k = static_cast<const uint16_t*>(k);
+  a.v = static_cast<const uint16_t*>(v);
+  a.o = static_cast<const uint16_t*>(o);
+  a.dout = static_cast<const uint16_t*>(dout);
+  a.lse = lse;
+  a.dq = static_cast<uint16_t*>(dq);
+  a.dk = static_cast<uint16_t*>(dk);
+  a.dv = static_cast<uint16_t*>(dv);
+  a.q_lens = q_lens;
+  a.k_lens = k_lens;
+  int64_t* dst[24] = {&a.qb,  &a.qh,  &a.ql,  &a.kb,  &a.kh,  &a.kl,  &a.vb,  &a.vh,
+                      &a.vl,  &a.ob,  &a.oh,  &a.ol,  &a.gb,  &a.gh,  &a.gl,  &a.dqb,
+                      &a.dqh, &a.dql, &a.dkb, &a.dkh, &a.dkl, &a.dvb, &a.dvh, &a.dvl};
+  for (int i = 0; i < 24; ++i) *dst[i] = strides[i];
+  a.Lq = Lq;
+  a.Lk = Lk;
+  a.H = H;
+  a.Hkv = Hkv;
+  a.rep = H / Hkv;
+  a.nbh = (int)bh;
+  a.nbk = (int)bk;
+  a.causal = causal != 0;
+  a.c = scale * kLog2e;
+  a.inv_c = 1.f / a.c;
+  a.scale = scale;
+  a.nlse = static_cast<float*>(workspace);
+  a.ndelta = a.nlse + bh * Lq;
+  a.gmax = a.ndelta + bh * Lq;
+  a.vmax = a.gmax + bh * p.nqb;
+  a.nqb = (int)p.nqb;
+  a.nkb = (int)p.nkb;
+  a.part = a.nlse + p.stats;
+  a.qtiles = (int)p.qtiles;
+  a.dq_splits = p.dq_splits;
+  a.dq_nwork = (int)p.dq_nwork;
+  a.dq_per_xcd = (int)((p.dq_nwork + 7) / 8);
+  a.ktiles = (int)p.ktiles;
+  a.kv_splits = p.kv_splits;
+  a.kv_nwork = (int)p.kv_nwork;
+  a.kv_per_xcd = (int)((p.kv_nwork + 7) / 8);
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  auto go = [&](auto tag) -> int {
+    using T16 = decltype(tag);
+    int err;
+    dense_bwd_prep_kernel<T16><<<(unsigned)(pq + pv), 256, 0, st>>>(a, pq);
+    if ((err = (int)hipGetLastError())) return err;
+    if (p.nq == 2)
+      dense_bwd_dq_kernel<T16, 2><<<8 * a.dq_per_xcd, 256, 0, st>>>(a);
+    else
+      dense_bwd_dq_kernel<T16, 1><<<8 * a.dq_per_xcd, 256, 0, st>>>(a);
+    if ((err = (int)hipGetLastError())) return err;
+    if (p.dq_splits > 1) {
+      dense_bwd_join_kernel<T16, kDD><<<(unsigned)((bh * Lq * kDD / 4 + 255) / 256), 256, 0, st>>>(
+          a.part, p.dq_splits, bh * Lq, Lq, H, a.dq, a.dqb, a.dqh, a.dql, nullptr, 0, 0, 0);
+      if ((err = (int)hipGetLastError())) return err;
+    }
+    dense_bwd_dkdv_kernel<T16, 1><<<8 * a.kv_per_xcd, 256, 0, st>>>(a);
+    if ((err = (int)hipGetLastError()) || p.kv_splits == 1) return err;
+    dense_bwd_join_kernel<T16, 2 * kDD>
+        <<<(unsigned)((bk * Lk * 2 * kDD / 4 + 255) / 256), 256, 0, st>>>(
+            a.part, p.kv_splits, bk * Lk, Lk, Hkv, a.dk, a.dkb, a.dkh, a.dkl, a.dv, a.dvb, a.dvh,
+            a.dvl);
+    return (int)hipGetLastError();
+  };
+  return dtype == SLA2H_DTYPE_BF16 ? go(BF16{}) : go(F16{});
+}

@@ -15,10 +15,11 @@ from functools import partial
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
+from torch.autograd.function import once_differentiable
 
 __all__ = ["RMSNorm", "SituAndMul", "SwiGLUMlp", "MLAAttention", "TransformerBlock",
            "apply_rotary_pos_emb", "precompute_axial_rope_3d", "scaled_variance_linear",
-           "sdpa_math_attention"]
+           "dense_attention", "sdpa_math_attention"]
 
 
 class _CastOf(torch.autograd.Function):
@@ -115,6 +116,58 @@ def scaled_variance_linear(in_features, out_features, bias=True, init_constant=1
 def sdpa_math_attention(q, k, v):
     """Dense softmax attention on (b, l, H, hd) tensors (the default attn_impl)."""
     o = F.scaled_dot_product_attention(q.transpose(1, 2), k.transpose(1, 2), v.transpose(1, 2))
+    return o.transpose(1, 2)
+
+
+class _DenseAttentionFunction(torch.autograd.Function):
+    """Dense attention of (B, H, L, 64) operands on the HIP kernels; saves the operands,
+    the output and the rows' log-sum-exp, and recomputes the probabilities."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, causal, q_lens, k_lens, scale):
+        from . import ops
+        o, lse = ops.dense_attn_fwd(q, k, v, causal, q_lens, k_lens, scale)
+        ctx.args = causal, scale
+        ctx.save_for_backward(q, k, v, o, lse, q_lens, k_lens)
+        return o
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, do):
+        from . import ops
+        if ops.batched(do):
+            raise RuntimeError("dense_attention: its backward takes one gradient at a time "
+                               "(no vmap or is_grads_batched)")
+        q, k, v, o, lse, q_lens, k_lens = ctx.saved_tensors
+        causal, scale = ctx.args
+        return (*ops.dense_attn_bwd(do, q, k, v, o, lse, causal, q_lens, k_lens, scale),
+                None, None, None, None)
+
+
+def dense_attention(q, k, v, causal=False, q_lens=None, k_lens=None, scale=None):
+    """Dense softmax attention on the gfx950 kernels, forward and backward: q
+    (b, l, H, 64) over k, v (b, lk, Hkv, 64) of one 16-bit dtype (under a 16-bit
+    autocast any floating dtype, cast to it), H a multiple of Hkv; usable as an
+    attn_impl.  q_lens, k_lens (b,): the clips' lengths in a padded batch; rows
+    behind them, and rows without a key, are zero and take no gradient.  causal:
+    query i sees the keys j <= i + k_len - q_len.  scale: 64^-1/2 by default.
+
+    Memory is linear in l (the probabilities are recomputed in the backward), and
+    results do not depend on the order of execution.  GPU tensors only; one
+    reverse-mode derivative (no double backward, forward mode or vmap)."""
+    if torch.is_autocast_enabled("cuda"):
+        dt = torch.get_autocast_dtype("cuda")
+        q, k, v = (t.to(dt) if t.is_floating_point() else t for t in (q, k, v))
+    from . import ops
+    for t, name in ((q, "q"), (k, "k"), (v, "v")):
+        if t.dim() != 4:
+            raise ValueError(f"{name}: expected (b, l, H, 64), got {tuple(t.shape)}")
+    q, k, v = (t.transpose(1, 2) for t in (q, k, v))
+    q_lens, k_lens = (ops.attn_lens(n, q, s) for n, s in ((q_lens, "q_lens"), (k_lens, "k_lens")))
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        o = _DenseAttentionFunction.apply(q, k, v, causal, q_lens, k_lens, scale)
+    else:
+        o, _ = ops.dense_attn_fwd(q, k, v, causal, q_lens, k_lens, scale, with_lse=False)
     return o.transpose(1, 2)
 
 

@@ -5,6 +5,7 @@ with torch's caching allocator on the inputs' device and launches on torch's
 current HIP stream.  Inputs must already live on a GPU: there is no CPU path.
 """
 
+import ctypes
 import math
 
 import torch
@@ -1476,3 +1477,139 @@ def _rows16(t):
         v = v.clone(memory_format=torch.contiguous_format)
         s = F
     return v, F, s
+
+
+# ---------------------------------------------------------------------------
+# Dense softmax attention (sla2h_dense_attn_fwd / _bwd)
+# ---------------------------------------------------------------------------
+def _launch(dev, name, *args):
+    """A library call with the tensors' device current and its current stream."""
+    fn = getattr(_lib.load(), name)
+    if dev.index is None or dev.index == torch.cuda.current_device():
+        _lib.check(fn(*args, _stream(dev)), name)
+    else:
+        with torch.cuda.device(dev):
+            _lib.check(fn(*args, _stream(dev)), name)
+
+
+_ATTN_ROW_SPAN = 1 << 23  # row strides below it (32-bit offsets within 64 rows)
+
+
+def _attn_strides(t):
+    """(batch, head, row) strides of a (B, H, L, 64) tensor; of a size of one 0, for
+    the rows 64."""
+    return [s if n > 1 else d for n, s, d in zip(t.shape[:3], t.stride()[:3], (0, 0, E_TILE))]
+
+
+def _attn_operand(t):
+    """t with a unit channel stride, 16-byte aligned rows and row strides that the
+    kernels take, copied where it has not."""
+    if (t.stride(3) == 1 and t.data_ptr() % 16 == 0
+            and all(s % 8 == 0 for s in _attn_strides(t))
+            and E_TILE <= _attn_strides(t)[2] < _ATTN_ROW_SPAN):
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
+
+
+def _attn_like(t, shape=None, dtype=None):
+    """Empty (B, H, L, 64), token-major in memory where t's rows are further apart
+    than its heads (a permuted (B, L, H, 64))."""
+    B, H, L, D = shape or t.shape
+    dtype = dtype or t.dtype
+    if t.stride(2) > t.stride(1):
+        return torch.empty(B, L, H, D, device=t.device, dtype=dtype).transpose(1, 2)
+    return torch.empty(B, H, L, D, device=t.device, dtype=dtype)
+
+
+def attn_lens(lens, q, name):
+    """Sequence lengths (whole numbers, one per batch entry of q) as contiguous int32 on
+    q's device, or None."""
+    if lens is None:
+        return None
+    lens = torch.as_tensor(lens)
+    if (lens.dtype.is_floating_point or lens.dtype.is_complex or lens.dtype == torch.bool
+            or tuple(lens.shape) != tuple(q.shape[:1])):
+        raise ValueError(f"{name}: expected {q.shape[0]} whole numbers, got "
+                         f"{tuple(lens.shape)} {lens.dtype}")
+    if lens.dtype != torch.int32:  # values past 32 bits are past any length
+        lens = lens.clamp(0, 2 ** 31 - 1)
+    return lens.to(q.device, torch.int32).contiguous()
+
+
+def _attn_args(q, k, v, scale):
+    """Checks of dense attention's operands; returns (dtype code, B, H, Hkv, Lq, Lk, scale)."""
+    _need_gpu(q, k, v)
+    for t, name in ((q, "q"), (k, "k"), (v, "v")):
+        if t.dim() != 4 or t.shape[-1] != E_TILE:
+            raise ValueError(f"{name}: expected (B, H, L, 64), got {tuple(t.shape)}")
+        if t.dtype != q.dtype or t.device != q.device:
+            raise ValueError("q, k and v must share dtype and device: "
+                             f"q {q.dtype} {q.device}, {name} {t.dtype} {t.device}")
+    code = _dtype_code(q)
+    B, H, Lq, D = q.shape
+    Hkv, Lk = k.shape[1:3]
+    if k.shape != v.shape or k.shape[0] != B or (H and (Hkv == 0 or H % Hkv)):
+        raise ValueError("k and v must share their shape, q's batch and a number of heads that "
+                         f"divides q's: {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
+    scale = D ** -0.5 if scale is None else float(scale)
+    if not 0.0 < scale < 1e30:
+        raise ValueError(f"scale must be positive, got {scale}")
+    return code, B, H, Hkv, Lq, Lk, scale
+
+
+def _strides_arg(*ts):
+    s = [x for t in ts for x in _attn_strides(t)]
+    return (ctypes.c_int64 * len(s))(*s)
+
+
+def dense_attn_fwd(q, k, v, causal=False, q_lens=None, k_lens=None, scale=None, with_lse=True):
+    """Dense softmax attention of q (B, H, Lq, 64) over k, v (B, Hkv, Lk, 64), 16-bit,
+    any strides with a unit channel stride -> (o in q's layout, lse (B, H, Lq) fp32
+    or None).  H a multiple of Hkv; q_lens, k_lens (B,): the sequences' lengths
+    (values outside [0, L] are clamped); causal: query i sees the keys
+    j <= i + k_len - q_len.  Rows past a length and rows without a key are 0, their
+    lse -inf."""
+    code, B, H, Hkv, Lq, Lk, scale = _attn_args(q, k, v, scale)
+    dev = q.device
+    q_lens, k_lens = attn_lens(q_lens, q, "q_lens"), attn_lens(k_lens, q, "k_lens")
+    q, k, v = _attn_operand(q), _attn_operand(k), _attn_operand(v)
+    o = _attn_like(q)
+    lse = torch.empty(B, H, Lq, device=dev, dtype=torch.float32) if with_lse else None
+    if o.numel() == 0 or Lk == 0:
+        o.zero_()
+        if lse is not None:
+            lse.fill_(float("-inf"))
+        return o, lse
+    need = _lib.load().sla2h_dense_attn_fwd_workspace_bytes(B, H, Hkv, Lq, Lk)
+    ws = _scratch(need, dev) if need else None
+    _launch(dev, "sla2h_dense_attn_fwd", q.data_ptr(), k.data_ptr(), v.data_ptr(),
+            _strides_arg(q, k, v, o), _ptr(q_lens), _ptr(k_lens), code, B, H, Hkv, Lq, Lk,
+            int(bool(causal)), scale, _ptr(ws), o.data_ptr(), _ptr(lse))
+    return o, lse
+
+
+def dense_attn_bwd(do, q, k, v, o, lse, causal=False, q_lens=None, k_lens=None, scale=None):
+    """Gradients (dq, dk, dv) of dense_attn_fwd for the output gradient do, from its
+    operands, its output o and lse (recomputed probabilities); dk and dv summed
+    over the query heads of a key head, zero behind the sequences."""
+    code, B, H, Hkv, Lq, Lk, scale = _attn_args(q, k, v, scale)
+    dev = q.device
+    for t, name in ((do, "do"), (o, "o")):
+        if t.shape != q.shape or t.dtype != q.dtype or t.device != dev:
+            raise ValueError(f"{name}: expected {tuple(q.shape)} {q.dtype} on {dev}, got "
+                             f"{tuple(t.shape)} {t.dtype} on {t.device}")
+    if tuple(lse.shape) != (B, H, Lq) or lse.dtype != torch.float32 or lse.device != dev:
+        raise ValueError(f"lse: expected ({B}, {H}, {Lq}) float32 on {dev}, got "
+                         f"{tuple(lse.shape)} {lse.dtype} on {lse.device}")
+    q_lens, k_lens = attn_lens(q_lens, q, "q_lens"), attn_lens(k_lens, q, "k_lens")
+    q, k, v, o, do = (_attn_operand(t) for t in (q, k, v, o, do))
+    lse = lse.contiguous()
+    dq, dk, dv = _attn_like(q), _attn_like(k), _attn_like(v)
+    if q.numel() == 0 or k.numel() == 0:
+        return dq.zero_(), dk.zero_(), dv.zero_()
+    ws = _scratch(_lib.load().sla2h_dense_attn_bwd_workspace_bytes(code, B, H, Hkv, Lq, Lk), dev)
+    _launch(dev, "sla2h_dense_attn_bwd", q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(),
+            do.data_ptr(), lse.data_ptr(), _strides_arg(q, k, v, o, do, dq, dk, dv),
+            _ptr(q_lens), _ptr(k_lens), code, B, H, Hkv, Lq, Lk, int(bool(causal)), scale,
+            ws.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr())
+    return dq, dk, dv

@@ -840,6 +840,47 @@ int sla2h_sla2_infer_in(const void* q, const void* k, const void* v, int dtype, 
                         int64_t L, int bq, const float* proj_q, const float* proj_k,
                         void* workspace, float* qpool, float* kpool_t, void* stream);
 
+/*
+ * Dense softmax attention on 64-channel heads, forward:
+ *   S = scale q k^T over the keys j < k_len of a batch's sequence, with causal only
+ *   j <= i + k_len - q_len (the last query sees the last key); o = softmax(S) v,
+ *   lse = log sum exp S (natural log).  Rows at or past q_len and rows without a key: o = 0,
+ *   lse = -inf.  Whatever memory holds behind a sequence (NaN too) is not used.
+ * q (B, H, Lq, 64), k, v (B, Hkv, Lk, 64), o like q, of one 16-bit dtype, H a multiple of
+ * Hkv (query head h reads key head h / (H / Hkv)).  strides: host array of 12 int64, the
+ * (batch, head, row) strides of q, k, v, o in elements, multiples of 8 (batch and head strides
+ * 0 for broadcast inputs; row strides at least 64, k's and v's below 2^23); unit channel stride, 16-byte aligned pointers.  q_lens, k_lens (B)
+ * int32 on the device or NULL (all Lq / Lk); values are clamped into [0, Lq] / [0, Lk].
+ * lse (B, H, Lq) fp32 contiguous or NULL.  fp32 accumulation; probabilities are rounded
+ * to dtype for their product with v.  Calls with few query rows split the keys over
+ * workgroups and join the parts in order (a workspace of
+ * sla2h_dense_attn_fwd_workspace_bytes, 0 for most calls).
+ * The attn_impl of the reference's MLAAttention (models/imf_dit_video.py:323-467).
+ */
+size_t sla2h_dense_attn_fwd_workspace_bytes(int B, int H, int Hkv, int64_t Lq, int64_t Lk);
+int sla2h_dense_attn_fwd(const void* q, const void* k, const void* v, const int64_t* strides,
+                         const int32_t* q_lens, const int32_t* k_lens, int dtype, int B, int H,
+                         int Hkv, int64_t Lq, int64_t Lk, int causal, float scale,
+                         void* workspace, void* o, float* lse, void* stream);
+
+/*
+ * Its backward, the probabilities recomputed from lse:
+ *   delta = rowsum(dout o), dS = P (dout v^T - delta), dq = scale dS k, dk = scale dS^T q,
+ *   dv = P^T dout, dk and dv summed over the query heads of a key head.
+ * q, k, v, lse, lens, sizes, causal and scale as in the forward, o its output, dout like o;
+ * dq like q, dk and dv like k.  strides: host array of 24 int64, the (batch, head, row)
+ * strides of q, k, v, o, dout, dq, dk, dv in elements (the same conditions; row strides of q, k, v and
+ * dout below 2^23).  Gradients of rows behind a sequence and of rows without a key are 0; dout is
+ * not read there.  No atomics: results are reproducible bit for bit.
+ */
+size_t sla2h_dense_attn_bwd_workspace_bytes(int dtype, int B, int H, int Hkv, int64_t Lq,
+                                            int64_t Lk);
+int sla2h_dense_attn_bwd(const void* q, const void* k, const void* v, const void* o,
+                         const void* dout, const float* lse, const int64_t* strides,
+                         const int32_t* q_lens, const int32_t* k_lens, int dtype, int B, int H,
+                         int Hkv, int64_t Lq, int64_t Lk, int causal, float scale,
+                         void* workspace, void* dq, void* dk, void* dv, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
