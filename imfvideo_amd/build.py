@@ -32,6 +32,7 @@ SOURCES = {
     "attn_bwd.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
     "dense_attn.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
     "dense_attn_bwd.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
+    "act8.hip": [],
     "mla_glue.hip": [],
     "block_train.hip": [],
     "linear_bwd.hip": [],

@@ -181,6 +181,9 @@ __device__ inline u32x2 lds_read_tr16(const void* p) {
   return __builtin_bit_cast(u32x2, v);
 }
 
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+
 // 2^x on the hardware exp unit (v_exp_f32); inputs here are <= 0 or -inf.
 __device__ inline float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 

@@ -107,8 +107,6 @@ __device__ inline int seq_len(const int32_t* lens, int b, int64_t L) {
   return n < 0 ? 0 : (n > L ? (int)L : n);
 }
 
-constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kLn2 = 0.6931471805599453f;
 constexpr int kNoLimit = 0x7fffffff;
 
 }  // namespace sla2h

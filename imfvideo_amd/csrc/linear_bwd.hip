@@ -10,6 +10,7 @@
 // as well: grid = output tiles x ranges, fp32 partial tiles, then one pass
 // that adds the ranges in order (no atomics: the result does not depend on
 // the dispatch order).
+#include "act8.h"
 #include "common.h"
 
 namespace sla2h {
@@ -171,6 +172,220 @@ __global__ __launch_bounds__(256) void wgrad_sum_kernel(const f32x4* __restrict_
   dw[i] = s;
 }
 
+// --- dW = dY^T X with X in 8 bits (act8.h) -----------------------------------
+//
+// dW_mn = sum over row tiles t of s_t,n (sum over the tile's rows dY_rm code_rn): the codes are
+// whole numbers up to 127 and exact in either 16-bit type, so the products of a tile of 64 rows
+// are exact in fp32 and the tile's scale is applied to the sum, in fp32.  X is never
+// rounded to 16 bits again.
+struct Wgrad8Args {
+  const uint16_t* dy;
+  const int8_t* codes;
+  const float* scales;
+  float* out;  // [range][M][N]
+  int64_t rows, ldy;
+  int M, N, cb;
+  int tn, tiles;
+  int64_t per_split;  // row tiles of a range
+  int nwork, per_xcd;
+};
+
+constexpr int kAStage = kAct * kWT * 2;  // bytes of one operand's stage: 64 rows x 256 B
+
+// sixteen codes as 16-bit numbers, exactly
+template <typename T16>
+__device__ inline void widen16(u32x4 c, u32x4& lo, u32x4& hi) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const uint32_t a = pack_pair<T16>(code_f32<0>(c[e]), code_f32<1>(c[e]));
+    const uint32_t b = pack_pair<T16>(code_f32<2>(c[e]), code_f32<3>(c[e]));
+    if (e < 2)
+      lo[2 * e] = a, lo[2 * e + 1] = b;
+    else
+      hi[2 * e - 4] = a, hi[2 * e - 3] = b;
+  }
+}
+
+// Workgroup = one 128 x 128 tile of dW over one range of row tiles, wave (wm, wn) 64 x 64 of it
+// (one code tile wide, so its scale is one number per stage).  A stage is 64 rows: dY goes to
+// LDS as it is (DMA: buffer loads straight into LDS, for 16-byte aligned rows; else through
+// registers), the codes are widened on their way, two slots each, and the fragments are
+// read transposed as in wgrad_kernel.
+template <typename T16, bool DMA>
+__global__ __launch_bounds__(256, 2) void wgrad8_kernel(Wgrad8Args a) {
+  __shared__ __align__(16) unsigned char ly[2 * kAStage];
+  __shared__ __align__(16) unsigned char lx[2 * kAStage];
+  const int logical = (blockIdx.x & 7) * a.per_xcd + (blockIdx.x >> 3);
+  if (logical >= a.nwork) return;
+  const int sp = __builtin_amdgcn_readfirstlane(logical / a.tiles);
+  const int tile = __builtin_amdgcn_readfirstlane(logical - sp * a.tiles);
+  const int m0 = (tile / a.tn) * kWT, n0 = (tile % a.tn) * kWT;
+  const int64_t rts = (a.rows + kAct - 1) / kAct;
+  const int64_t t0 = sp * a.per_split;
+  const int nst = (int)(min(rts, t0 + a.per_split) - t0);
+  const int tid = threadIdx.x;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int l = tid & 63, r = l & 15, g = l >> 4;
+  const int wm = w >> 1, wn = w & 1;
+
+  // dY: rows past the last one read as zero
+  const int64_t ld2 = a.ldy * 2;
+  const int lrow = 4 * w + (l >> 4);
+  const int col = ((((l & 15) >> 1) ^ (lrow & 7)) << 5) + (l & 1) * 16;
+  const int voff = lrow * (int)ld2 + m0 * 2 + col;
+  auto dma_y = [&](int s) {
+    const int64_t row = (t0 + s) * kAct;
+    const int64_t left = s < nst ? a.rows - row : 0;
+    const auto ry = make_rsrc(reinterpret_cast<const char*>(a.dy) + row * ld2,
+                              left <= 0 ? 0 : ((left < kAct ? left : kAct) - 1) * ld2 + a.M * 2);
+    unsigned char* p = ly + (s & 1) * kAStage + w * 1024;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) dma16(ry, p + 4096 * k, voff + 16 * k * (int)ld2);
+  };
+  // ... or element groups of any alignment through registers: row 16 k + tid / 16
+  const int yr = tid >> 4, yc = m0 + (tid & 15) * 8;
+  auto load_y = [&](int s, u32x4 (&v)[4]) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int64_t row = (t0 + s) * kAct + 16 * k + yr;
+      v[k] = s < nst && row < a.rows ? load_row8(a.dy + row * a.ldy, yc, a.M) : u32x4{0, 0, 0, 0};
+    }
+  };
+  auto put_y = [&](int s, const u32x4 (&v)[4]) {
+    unsigned char* p = ly + (s & 1) * kAStage + yr * 256 +
+                       ((((tid & 15) >> 1) ^ (yr & 7)) << 5) + (tid & 1) * 16;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) *reinterpret_cast<u32x4*>(p + 4096 * k) = v[k];
+  };
+  // codes: threads 0 .. 127 the first tile's 4 KB, the others the second's, 16 bytes each twice
+  // (always two loads, zeros past the last tile: the loop counts them)
+  const int ct = n0 / kAct, xi = tid & 127;
+  const int xoff = (tid >> 7) * kActBytes + xi * 16;
+  auto load_x = [&](int s, u32x4 (&v)[2]) {
+    const auto rx = make_rsrc(a.codes + ((t0 + s) * a.cb + ct) * kActBytes,
+                              s < nst ? (a.cb - ct < 2 ? 1 : 2) * kActBytes : 0);
+    v[0] = buf_load16(rx, xoff, 0);
+    v[1] = buf_load16(rx, xoff + 2048, 0);
+  };
+  auto put_x = [&](int s, const u32x4 (&v)[2]) {
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const int row = (xi >> 2) + 32 * k, c = 4 * (tid >> 7) + (xi & 3);
+      u32x4 lo, hi;
+      widen16<T16>(v[k], lo, hi);
+      u32x4* p = reinterpret_cast<u32x4*>(lx + (s & 1) * kAStage + row * 256 +
+                                          ((c ^ (row & 7)) << 5));
+      p[0] = lo;
+      p[1] = hi;
+    }
+  };
+  const int st = n0 / kAct + wn;  // this wave's code tile
+  auto scale_of = [&](int s) {
+    return s < nst && st < a.cb ? a.scales[(t0 + s) * a.cb + st] : 0.f;
+  };
+
+  const int rho = 4 * g + (r >> 2);
+  const uint32_t by = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)ly;
+  const uint32_t bx = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)lx;
+  uint32_t fy[4], fx[4];
+#pragma unroll
+  for (int t = 0; t < 4; ++t) {
+    fy[t] = by + rho * 256 + (((4 * wm + t) ^ (rho & 7)) << 5) + (r & 3) * 8;
+    fx[t] = bx + rho * 256 + (((4 * wn + t) ^ (rho & 7)) << 5) + (r & 3) * 8;
+  }
+  f32x4 acc[4][4];  // [n sub-tile][m sub-tile]: lane holds dW[m = r][n = 4 g + i]
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+  u32x4 xv[2], yv[4];
+  load_x(0, xv);
+  if (DMA) {
+    dma_y(0);
+  } else {
+    load_y(0, yv);
+    put_y(0, yv);
+    load_y(1, yv);
+  }
+  put_x(0, xv);
+  load_x(1, xv);
+  float sc = scale_of(0);
+  for (int s = 0; s < nst; ++s) {
+    // this wave's part of stage s is in LDS (the two loads of codes behind it may be
+    // in flight), then everyone's, and stage s - 1 is read
+    __builtin_amdgcn_s_waitcnt(DMA ? 0x0072 : 0xC07F);
+    __builtin_amdgcn_s_barrier();
+    if (DMA) {
+      dma_y(s + 1);
+    } else {
+      put_y(s + 1, yv);
+      load_y(s + 2, yv);
+    }
+    put_x(s + 1, xv);
+    load_x(s + 2, xv);
+    const float scn = scale_of(s + 1);
+    u32x4 fm[2][4], fn[2][4];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const uint32_t slot = (s & 1) * kAStage + k * 8192;
+      read_frags(fy, slot, fm[k]);
+      read_frags(fx, slot, fn[k]);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        f32x4 t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int k = 0; k < 2; ++k) t = mfma_16x16x32<T16>(fn[k][i], fm[k][j], t);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[i][j][e] = __builtin_fmaf(sc, t[e], acc[i][j][e]);
+      }
+    sc = scn;
+  }
+  __builtin_amdgcn_s_waitcnt(0x0070);  // no load into this workgroup's LDS outlives it
+
+  float* out = a.out + (int64_t)sp * a.M * a.N;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int m = m0 + 64 * wm + 16 * j + r;
+    if (m >= a.M) continue;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int n = n0 + 64 * wn + 16 * i + 4 * g;
+      float* o = out + (int64_t)m * a.N + n;
+      if (a.N % 4 == 0) {
+        if (n < a.N) *reinterpret_cast<f32x4*>(o) = acc[i][j];
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (n + e < a.N) o[e] = acc[i][j][e];
+      }
+    }
+  }
+}
+
+// the ranges' sum for a weight whose size is no multiple of four
+__global__ __launch_bounds__(256) void wgrad_sum1_kernel(const float* __restrict__ part, int splits,
+                                                        int64_t n, float* __restrict__ dw) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= n) return;
+  float s = part[i];
+#pragma unroll 8
+  for (int j = 1; j < splits; ++j) s += part[j * n + i];
+  dw[i] = s;
+}
+
+// Ranges of row tiles: about two workgroups per CU, at least four stages each.
+int wgrad8_splits(int64_t rows, int M, int N) {
+  const int64_t tiles = (int64_t)((M + kWT - 1) / kWT) * ((N + kWT - 1) / kWT);
+  int64_t s = 512 / tiles;
+  const int64_t most = (rows + kAct - 1) / kAct / 4;
+  s = s < most ? s : most;
+  return s < 1 ? 1 : (int)s;
+}
+
 // Ranges of rows: enough workgroups for two on each of the 256 CUs, and at
 // least eight stages per range.
 int wgrad_splits(int64_t rows, int M, int N) {
@@ -236,5 +451,66 @@ extern "C" int sla2h_linear_wgrad(const void* dy, int64_t ldy, const void* x, in
   const int64_t n4 = (int64_t)M * N / 4;
   wgrad_sum_kernel<<<(unsigned)((n4 + 255) / 256), 256, 0, st>>>(
       static_cast<const f32x4*>(workspace), used, n4, reinterpret_cast<f32x4*>(dw));
+  return (int)hipGetLastError();
+}
+
+extern "C" size_t sla2h_linear_wgrad8_workspace_bytes(int64_t rows, int M, int N) {
+  if (rows <= 0 || M <= 0 || N <= 0) return 0;
+  const int s = wgrad8_splits(rows, M, N);
+  return s > 1 ? (size_t)s * M * N * 4 : 0;
+}
+
+extern "C" int sla2h_linear_wgrad8(const void* dy, int64_t ldy, const int8_t* codes,
+                                   const float* scales, int dtype, int64_t rows, int M, int N,
+                                   void* workspace, float* dw, void* stream) {
+  SLA2H_CHECK_ARG(dy && codes && scales && dw);
+  SLA2H_CHECK_ARG(dtype == SLA2H_DTYPE_F16 || dtype == SLA2H_DTYPE_BF16);
+  SLA2H_CHECK_ARG(rows > 0 && M > 0 && N > 0 && ldy >= M && ldy < ((int64_t)1 << 23));
+  SLA2H_CHECK_ARG(((uintptr_t)codes | (uintptr_t)dw | (uintptr_t)workspace) % 16 == 0 &&
+                  (uintptr_t)scales % 4 == 0 && (uintptr_t)dy % 2 == 0);
+  const int splits = wgrad8_splits(rows, M, N);
+  SLA2H_CHECK_ARG(splits == 1 || workspace);
+  const int64_t tm = ((int64_t)M + kWT - 1) / kWT, tn = ((int64_t)N + kWT - 1) / kWT;
+  const int64_t rts = (rows + kAct - 1) / kAct, per = (rts + splits - 1) / splits;
+  const int64_t used = (rts + per - 1) / per;  // ranges that hold a row
+  SLA2H_CHECK_ARG(tm * tn * used < ((int64_t)1 << 28) && per < ((int64_t)1 << 30));
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  Wgrad8Args a;
+  a.dy = static_cast<const uint16_t*>(dy);
+  a.codes = codes;
+  a.scales = scales;
+  a.out = used > 1 ? static_cast<float*>(workspace) : dw;
+  a.rows = rows;
+  a.ldy = ldy;
+  a.M = M;
+  a.N = N;
+  a.cb = (N + kAct - 1) / kAct;
+  a.tn = (int)tn;
+  a.tiles = (int)(tm * tn);
+  a.per_split = per;
+  a.nwork = (int)(tm * tn * used);
+  a.per_xcd = (a.nwork + 7) / 8;
+  const bool dma = (uintptr_t)dy % 16 == 0 && ldy % 8 == 0 && M % 8 == 0;
+  const unsigned grid = 8u * a.per_xcd;
+  auto go = [&](auto tag) {
+    using T16 = decltype(tag);
+    if (dma)
+      wgrad8_kernel<T16, true><<<grid, 256, 0, st>>>(a);
+    else
+      wgrad8_kernel<T16, false><<<grid, 256, 0, st>>>(a);
+  };
+  if (dtype == SLA2H_DTYPE_BF16)
+    go(BF16{});
+  else
+    go(F16{});
+  const int err = (int)hipGetLastError();
+  if (err || used == 1) return err;
+  const int64_t n = (int64_t)M * N;
+  if (n % 4 == 0)
+    wgrad_sum_kernel<<<(unsigned)((n / 4 + 255) / 256), 256, 0, st>>>(
+        static_cast<const f32x4*>(workspace), (int)used, n / 4, reinterpret_cast<f32x4*>(dw));
+  else
+    wgrad_sum1_kernel<<<(unsigned)((n + 255) / 256), 256, 0, st>>>(
+        static_cast<const float*>(workspace), (int)used, n, dw);
   return (int)hipGetLastError();
 }

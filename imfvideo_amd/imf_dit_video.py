@@ -119,6 +119,14 @@ def sdpa_math_attention(q, k, v):
     return o.transpose(1, 2)
 
 
+def _no_batched(d, what):
+    """RuntimeError for gradients under vmap: the kernels take one at a time."""
+    from . import ops
+    if ops.batched(d):
+        raise RuntimeError(f"{what}: the backward takes one gradient at a time "
+                           "(no vmap or is_grads_batched)")
+
+
 class _DenseAttentionFunction(torch.autograd.Function):
     """Dense attention of (B, H, L, 64) operands on the HIP kernels; saves the operands,
     the output and the rows' log-sum-exp, and recomputes the probabilities."""
@@ -135,9 +143,7 @@ class _DenseAttentionFunction(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, do):
         from . import ops
-        if ops.batched(do):
-            raise RuntimeError("dense_attention: its backward takes one gradient at a time "
-                               "(no vmap or is_grads_batched)")
+        _no_batched(do, "dense_attention")
         q, k, v, o, lse, q_lens, k_lens = ctx.saved_tensors
         causal, scale = ctx.args
         return (*ops.dense_attn_bwd(do, q, k, v, o, lse, causal, q_lens, k_lens, scale),
@@ -299,17 +305,45 @@ class _SituMulFunction(torch.autograd.Function):
         return dgate, dup, None, None
 
 
+class _Situ8Function(torch.autograd.Function):
+    """SituAndMul on the GPU with gate and up kept in 8 bits for the backward: one
+    kernel forward that packs them beside h, one backward that reads them."""
+
+    @staticmethod
+    def forward(ctx, gate, up, beta, linear_beta):
+        from . import ops
+        h, g8, u8 = ops.situ8_fwd(gate, up, beta, linear_beta)
+        ctx.args = beta, linear_beta, g8.rows, g8.cols
+        ctx.save_for_backward(g8.codes, g8.scales, u8.codes, u8.scales)
+        return h
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dh):
+        from . import ops
+        _no_batched(dh, "SituAndMul(act8=True)")
+        gc, gs, uc, us = ctx.saved_tensors
+        beta, linear_beta, *shape = ctx.args
+        return (*ops.situ8_bwd(dh, ops.Act8(gc, gs, *shape), ops.Act8(uc, us, *shape), beta,
+                               linear_beta), None, None)
+
+
 class SituAndMul(nn.Module):
     """situ(g) * up with situ(g) = beta tanh(g / beta) sigmoid(g); with
     linear_beta the up branch is soft-clamped to linear_beta tanh(up / linear_beta).
     GPU tensors of one 16-bit or fp32 dtype run the fused kernels
     (sla2h_situ_mul_fwd / _bwd); anything else (CPU tensors, mixed or other
-    dtypes) the eager fp32 expression, each branch cast to fp32 on its own."""
+    dtypes) the eager fp32 expression, each branch cast to fp32 on its own.
 
-    def __init__(self, beta=1.0, linear_beta=None):
+    act8: where gradients of 16-bit GPU tensors are recorded, keep gate and up in 8
+    bits for the backward (ops.act8_pack's tiles) instead of the tensors
+    themselves; the gradients are those at the kept values."""
+
+    def __init__(self, beta=1.0, linear_beta=None, act8=False):
         super().__init__()
         self.beta = beta
         self.linear_beta = linear_beta
+        self.act8 = act8
 
     def forward(self, x, up=None):
         if up is None:
@@ -319,6 +353,12 @@ class SituAndMul(nn.Module):
             gate = x
         if (gate.is_cuda and up.is_cuda and up.dtype == gate.dtype
                 and gate.dtype in (torch.float16, torch.bfloat16, torch.float32)):
+            if (self.act8 and gate.dtype != torch.float32 and gate.numel()
+                    and gate.shape == up.shape and gate.device == up.device
+                    and torch.is_grad_enabled() and (gate.requires_grad or up.requires_grad)):
+                return _Situ8Function.apply(gate, up, float(self.beta),
+                                            None if self.linear_beta is None
+                                            else float(self.linear_beta))
             return _SituMulFunction.apply(gate, up, float(self.beta),
                                           None if self.linear_beta is None
                                           else float(self.linear_beta))
@@ -330,23 +370,107 @@ class SituAndMul(nn.Module):
         return (act * u).to(dtype)
 
 
+def _wgrad(dy, x, weight_dtype):
+    """dY^T X for a 16-bit x in the weight's dtype, by the rule of _LinearFunction."""
+    from . import ops
+    M, N = dy.shape[-1], x.shape[-1]
+    if (-(-M // 128) * -(-N // 128) <= _WGRAD_MAX_TILES
+            and ops.linear_wgrad_ok(x.numel() // N, M, N)):
+        return ops.linear_wgrad(dy, x).to(weight_dtype)
+    return (dy.reshape(-1, M).t() @ x.reshape(-1, N)).to(weight_dtype)
+
+
+class _Mlp8Function(torch.autograd.Function):
+    """SwiGLUMlp whose backward works from 8-bit activations: kept are the input (for
+    the weight gradients of w1 and w3, read from the codes), gate and up; the hidden
+    activation of w2's weight gradient is computed again.  x1 and x3 hold the same
+    values (one output per consumer of the norm before)."""
+
+    @staticmethod
+    def forward(ctx, x1, x3, w1, w3, w2, beta, linear_beta):
+        from . import ops
+        h1, h3, h2 = (w.to(x1.dtype) for w in (w1, w3, w2))
+        h, g8, u8 = ops.situ8_fwd(F.linear(x1, h1), F.linear(x1, h3), beta, linear_beta)
+        x8 = ops.act8_pack(x1)
+        ctx.args = beta, linear_beta
+        ctx.shapes = [(a.rows, a.cols) for a in (x8, g8, u8)]
+        ctx.dtypes = [w.dtype for w in (w1, w3, w2)]
+        ctx.save_for_backward(h1, h3, h2, *(t for a in (x8, g8, u8) for t in a[:2]))
+        return F.linear(h, h2)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        from . import ops
+        _no_batched(dy, "SwiGLUMlp(act8=True)")
+        h1, h3, h2, *ts = ctx.saved_tensors
+        x8, g8, u8 = (ops.Act8(*ts[2 * i:2 * i + 2], *n) for i, n in enumerate(ctx.shapes))
+        n1, n3, nw1, nw3, nw2 = ctx.needs_input_grad[:5]
+        d1, d3, d2 = ctx.dtypes
+        dg, du, *h = ops.situ8_bwd(dy @ h2, g8, u8, *ctx.args, with_h=nw2)
+        return (dg @ h1 if n1 else None, du @ h3 if n3 else None,
+                ops.linear_wgrad8(dg, x8).to(d1) if nw1 else None,
+                ops.linear_wgrad8(du, x8).to(d3) if nw3 else None,
+                _wgrad(dy, h[0], d2) if nw2 else None, None, None)
+
+
+def _plain_module(m, kind):
+    """m is a `kind` whose call is its forward and nothing else."""
+    return (type(m) is kind and "forward" not in m.__dict__ and not m._forward_hooks
+            and not m._forward_pre_hooks and not m._backward_hooks
+            and not m._backward_pre_hooks)
+
+
 class SwiGLUMlp(nn.Module):
-    """Gated MLP w2(situ(w1 x) * w3 x)."""
+    """Gated MLP w2(situ(w1 x) * w3 x).
+
+    act8: where gradients are recorded for 16-bit GPU activations (a 16-bit autocast,
+    or 16-bit inputs and weights), keep the input, gate and up in 8 bits for
+    the backward and compute the hidden activation again (_Mlp8Function): per token
+    in_features + 2 hidden_features bytes instead of 2 in_features + 6
+    hidden_features.  Otherwise (no gradients, CPU tensors, transforms of torch.func,
+    hooked submodules) the same MLP with unpacked activations."""
 
     def __init__(self, in_features, hidden_features, weight_init_constant=1.0, situ_beta=1.0,
-                 situ_linear_beta=None):
+                 situ_linear_beta=None, act8=False):
         super().__init__()
         linear = partial(scaled_variance_linear, bias=False, init_constant=weight_init_constant)
         self.w1 = linear(in_features, hidden_features)
         self.w3 = linear(in_features, hidden_features)
         self.w2 = linear(hidden_features, in_features)
-        self.act = SituAndMul(beta=situ_beta, linear_beta=situ_linear_beta)
+        self.act = SituAndMul(beta=situ_beta, linear_beta=situ_linear_beta, act8=act8)
+        self.act8 = act8
 
     def forward(self, x):
         return self._forward(x, x)
 
+    def _mlp8_dtype(self, x1, x3):
+        """The 16-bit dtype in which _Mlp8Function takes this call, or None."""
+        ws = (self.w1.weight, self.w3.weight, self.w2.weight)
+        if not (self.act8 and x1.is_cuda and x1.numel() and torch.is_grad_enabled()
+                and any(t.requires_grad for t in (x1, x3, *ws)) and x1.is_floating_point()):
+            return None
+        auto = torch.is_autocast_enabled("cuda")
+        dt = torch.get_autocast_dtype("cuda") if auto else x1.dtype
+        half = (torch.float16, torch.bfloat16)
+        if dt not in half or any(w.dtype not in (half + (torch.float32,) if auto else (dt,))
+                                 or w.device != x1.device for w in ws):
+            return None
+        from . import ops
+        plain = (all(_plain_module(m, _Linear) and m.bias is None
+                     for m in (self.w1, self.w3, self.w2))
+                 and _plain_module(self.act, SituAndMul) and self.act.act8
+                 and not nn.modules.module._has_any_global_hook())
+        return dt if plain and ops.plain_eager(x1, x3, *ws) else None
+
     def _forward(self, x1, x3):
         """The MLP with w1 reading x1 and w3 reading x3 (the same values)."""
+        dt = self._mlp8_dtype(x1, x3)
+        if dt is not None:
+            lb = self.act.linear_beta
+            return _Mlp8Function.apply(x1.to(dt), x3.to(dt), self.w1.weight, self.w3.weight,
+                                       self.w2.weight, float(self.act.beta),
+                                       None if lb is None else float(lb))
         return self.w2(self.act(self.w1(x1), self.w3(x3)))
 
 
@@ -646,12 +770,13 @@ def _residual(x, a, scale):
 
 class TransformerBlock(nn.Module):
     """x += attn(norm1(x)) * attn_scale;  x += mlp(norm2(x)) * mlp_scale
-    (vector gates initialised to zero)."""
+    (vector gates initialised to zero).  act8: the MLP keeps its activations in 8
+    bits for the backward (SwiGLUMlp)."""
 
     def __init__(self, hidden_size, num_heads, q_lora_rank, kv_lora_rank, qk_nope_head_dim,
                  qk_rope_head_dim, v_head_dim, mlp_ratio=8 / 3, weight_init_constant=1.0,
                  norm_eps=1e-6, attn_impl=sdpa_math_attention, use_attn_res=False, situ_beta=4.0,
-                 situ_linear_beta=25.0, mla_use_output_gate=True):
+                 situ_linear_beta=25.0, mla_use_output_gate=True, act8=False):
         super().__init__()
         self.norm1 = RMSNorm(hidden_size, eps=norm_eps)
         self.attn = MLAAttention(hidden_size, num_heads=num_heads, q_lora_rank=q_lora_rank,
@@ -662,7 +787,7 @@ class TransformerBlock(nn.Module):
         self.norm2 = RMSNorm(hidden_size, eps=norm_eps)
         self.mlp = SwiGLUMlp(hidden_size, int(hidden_size * mlp_ratio),
                              weight_init_constant=weight_init_constant, situ_beta=situ_beta,
-                             situ_linear_beta=situ_linear_beta)
+                             situ_linear_beta=situ_linear_beta, act8=act8)
         self.attn_scale = nn.Parameter(torch.zeros(hidden_size))
         self.mlp_scale = nn.Parameter(torch.zeros(hidden_size))
         if use_attn_res:

@@ -7,6 +7,7 @@ current HIP stream.  Inputs must already live on a GPU: there is no CPU path.
 
 import ctypes
 import math
+from typing import NamedTuple
 
 import torch
 
@@ -1613,3 +1614,127 @@ def dense_attn_bwd(do, q, k, v, o, lse, causal=False, q_lens=None, k_lens=None, 
             _ptr(q_lens), _ptr(k_lens), code, B, H, Hkv, Lq, Lk, int(bool(causal)), scale,
             ws.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr())
     return dq, dk, dv
+
+
+# ---------------------------------------------------------------------------
+# Activations kept in 8 bits for the backward pass (sla2h_act8_* / situ8 / wgrad8)
+# ---------------------------------------------------------------------------
+class Act8(NamedTuple):
+    """An activation of `rows` x `cols` kept in 8 bits: int8 codes by 64 x 64 tiles and
+    a scale per tile (act8_pack)."""
+    codes: torch.Tensor   # (ceil(rows / 64), ceil(cols / 64), 64, 64) int8
+    scales: torch.Tensor  # (ceil(rows / 64), ceil(cols / 64)) fp32
+    rows: int
+    cols: int
+
+
+def _act8_empty(rows, cols, dev):
+    rb, cb = -(-rows // E_TILE), -(-cols // E_TILE)
+    return Act8(torch.empty(rb, cb, E_TILE, E_TILE, device=dev, dtype=torch.int8),
+                torch.empty(rb, cb, device=dev, dtype=torch.float32), rows, cols)
+
+
+def _act8_check(a, name):
+    rb, cb = -(-a.rows // E_TILE), -(-a.cols // E_TILE)
+    if (tuple(a.codes.shape) != (rb, cb, E_TILE, E_TILE) or a.codes.dtype != torch.int8
+            or tuple(a.scales.shape) != (rb, cb) or a.scales.dtype != torch.float32
+            or not a.codes.is_contiguous() or not a.scales.is_contiguous()
+            or a.codes.data_ptr() % 16 or a.codes.device != a.scales.device):
+        raise ValueError(f"{name}: not the 8-bit tiles of {a.rows} x {a.cols}")
+    _need_gpu(a.codes, a.scales)
+
+
+def act8_pack(x):
+    """x (..., cols) 16-bit -> Act8 of its rows: per 64 x 64 tile s = max|x| / 127 + 1e-12,
+    codes round_half_away(x / s).  A tile with an infinity or a NaN comes back as NaN."""
+    _need_gpu(x)
+    code = _dtype_code(x)
+    if x.dim() == 0 or x.numel() == 0:
+        raise ValueError(f"act8_pack: nothing to pack in {tuple(x.shape)}")
+    x2, cols, ld = _rows_view(x)
+    a = _act8_empty(x2.shape[0], cols, x.device)
+    _launch(x.device, "sla2h_act8_pack", x2.data_ptr(), ld, code, a.rows, cols,
+            a.codes.data_ptr(), a.scales.data_ptr())
+    return a
+
+
+def act8_unpack(a, dtype):
+    """The values that a holds, code * scale rounded to the 16-bit dtype: (rows, cols)."""
+    _act8_check(a, "act8_unpack")
+    x = torch.empty(a.rows, a.cols, device=a.codes.device, dtype=dtype)
+    _launch(x.device, "sla2h_act8_unpack", a.codes.data_ptr(), a.scales.data_ptr(),
+            _dtype_code(x), a.rows, a.cols, x.data_ptr())
+    return x
+
+
+def _gate_args(beta, linear_beta):
+    beta, lb = float(beta), float(linear_beta or 0.0)
+    if not (0.0 < beta < 1e30 and 0.0 <= lb < 1e30):
+        raise ValueError(f"situ8: beta must be positive and linear_beta not negative, got "
+                         f"{beta}, {linear_beta}")
+    return beta, lb
+
+
+def situ8_fwd(gate, up, beta, linear_beta=None):
+    """situ_mul_fwd that also keeps gate and up in 8 bits -> (h, gate Act8, up Act8).
+    h is computed from the 16-bit inputs."""
+    _need_gpu(gate, up)
+    if gate.shape != up.shape or gate.dtype != up.dtype or gate.device != up.device:
+        raise ValueError("situ8: gate and up must share shape, dtype and device")
+    code = _dtype_code(gate)
+    beta, lb = _gate_args(beta, linear_beta)
+    if gate.dim() == 0 or gate.numel() == 0:
+        raise ValueError(f"situ8: nothing to compute in {tuple(gate.shape)}")
+    g2, F, sg = _rows_view(gate)
+    u2, _, su = _rows_view(up)
+    dev = gate.device
+    h = torch.empty(gate.shape, device=dev, dtype=gate.dtype)
+    g8, u8 = _act8_empty(g2.shape[0], F, dev), _act8_empty(g2.shape[0], F, dev)
+    _launch(dev, "sla2h_situ8_fwd", g2.data_ptr(), u2.data_ptr(), code, g8.rows, F, sg, su, beta,
+            lb, h.data_ptr(), g8.codes.data_ptr(), g8.scales.data_ptr(), u8.codes.data_ptr(),
+            u8.scales.data_ptr())
+    return h, g8, u8
+
+
+def situ8_bwd(dh, g8, u8, beta, linear_beta=None, with_h=False):
+    """Gradients (dgate, dup) of situ8_fwd for dh (..., cols) at the kept values, in dh's
+    dtype and shape; with_h also h of the kept values (the next layer's input again)."""
+    _need_gpu(dh)
+    code = _dtype_code(dh)
+    beta, lb = _gate_args(beta, linear_beta)
+    _act8_check(g8, "situ8_bwd gate")
+    _act8_check(u8, "situ8_bwd up")
+    if (g8.rows, g8.cols) != (u8.rows, u8.cols) or dh.shape[-1:] != (g8.cols,) or (
+            dh.numel() != g8.rows * g8.cols) or not dh.device == g8.codes.device == u8.codes.device:
+        raise ValueError(f"situ8_bwd: dh {tuple(dh.shape)} on {dh.device} does not fit "
+                         f"{g8.rows} x {g8.cols} and {u8.rows} x {u8.cols} on {g8.codes.device}")
+    d2, F, sd = _rows_view(dh)
+    out = [torch.empty(dh.shape, device=dh.device, dtype=dh.dtype) for _ in range(2 + with_h)]
+    _launch(dh.device, "sla2h_situ8_bwd", d2.data_ptr(), sd, g8.codes.data_ptr(),
+            g8.scales.data_ptr(), u8.codes.data_ptr(), u8.scales.data_ptr(), code, g8.rows, F,
+            beta, lb, F, out[0].data_ptr(), out[1].data_ptr(),
+            out[2].data_ptr() if with_h else None)
+    return tuple(out)
+
+
+def linear_wgrad8(dy, a):
+    """dW = dY^T X (M, cols) fp32 from dy (..., M) 16-bit and X as Act8: the products with
+    the codes are exact, their tile's scale is applied in fp32."""
+    _need_gpu(dy)
+    code = _dtype_code(dy)
+    _act8_check(a, "linear_wgrad8")
+    M = dy.shape[-1] if dy.dim() else 0
+    if M == 0 or dy.numel() != a.rows * M or dy.device != a.codes.device:
+        raise ValueError(f"linear_wgrad8: dy {tuple(dy.shape)} on {dy.device} has not the "
+                         f"{a.rows} rows of X on {a.codes.device}")
+    d2, _, ld = _rows_view(dy)
+    if ld >= _ATTN_ROW_SPAN:
+        d2 = d2.contiguous()
+        ld = M
+    lib = _lib.load()
+    dw = torch.empty(M, a.cols, device=dy.device, dtype=torch.float32)
+    need = lib.sla2h_linear_wgrad8_workspace_bytes(a.rows, M, a.cols)
+    ws = _scratch(need, dy.device) if need else None
+    _launch(dy.device, "sla2h_linear_wgrad8", d2.data_ptr(), ld, a.codes.data_ptr(),
+            a.scales.data_ptr(), code, a.rows, M, a.cols, _ptr(ws), dw.data_ptr())
+    return dw

@@ -881,6 +881,44 @@ int sla2h_dense_attn_bwd(const void* q, const void* k, const void* v, const void
                          int Hkv, int64_t Lq, int64_t Lk, int causal, float scale,
                          void* workspace, void* dq, void* dk, void* dv, void* stream);
 
+/*
+ * Activations kept in 8 bits for the backward pass.  x (rows, F) 16-bit with row stride ld
+ * elements -> codes (ceil(rows / 64), ceil(F / 64), 64, 64) int8, 16-byte aligned, one 64 x 64
+ * tile after the other, zeros past the edges; scales (ceil(rows / 64), ceil(F / 64)) fp32.
+ *   s = fl32(fl32(max|x|) / 127) + fl32(1e-12) per tile,  code = round_half_away(fl32(x / s)),
+ * the value it holds is fl32(code s).  A tile with an infinity or a NaN has a NaN scale: all of it
+ * comes back as NaN.  unpack writes the values rounded to dtype, (rows, F) contiguous.
+ */
+int sla2h_act8_pack(const void* x, int64_t ld, int dtype, int64_t rows, int F, int8_t* codes,
+                    float* scales, void* stream);
+int sla2h_act8_unpack(const int8_t* codes, const float* scales, int dtype, int64_t rows, int F,
+                      void* x, void* stream);
+
+/*
+ * sla2h_situ_mul_fwd that also packs gate and up (the arithmetic of h is on the 16-bit inputs,
+ * h (rows, F) contiguous), and the backward at the packed values: dh (rows, F) with row
+ * stride sd -> dgate, dup and, unless NULL, h again (that of the packed values), rows of stride so
+ * elements, columns up to F written.  16-bit dtypes.
+ */
+int sla2h_situ8_fwd(const void* gate, const void* up, int dtype, int64_t rows, int F, int64_t sg,
+                    int64_t su, float beta, float lb, void* h, int8_t* gate_codes,
+                    float* gate_scales, int8_t* up_codes, float* up_scales, void* stream);
+int sla2h_situ8_bwd(const void* dh, int64_t sd, const int8_t* gate_codes,
+                    const float* gate_scales, const int8_t* up_codes, const float* up_scales,
+                    int dtype, int64_t rows, int F, float beta, float lb, int64_t so,
+                    void* dgate, void* dup, void* h, void* stream);
+
+/*
+ * Weight gradient dw (M, N) = dY^T X fp32 from dy (rows, M) 16-bit with row stride ldy < 2^23 and
+ * X (rows, N) as sla2h_act8_pack leaves it.  Exact products, fp32 sums: X is not rounded
+ * again.  Any M and N; 16-byte aligned rows of dy with M a multiple of 8 load straight into
+ * LDS.  Workspace of sla2h_linear_wgrad8_workspace_bytes (may be 0).  Reproducible.
+ */
+size_t sla2h_linear_wgrad8_workspace_bytes(int64_t rows, int M, int N);
+int sla2h_linear_wgrad8(const void* dy, int64_t ldy, const int8_t* codes, const float* scales,
+                        int dtype, int64_t rows, int M, int N, void* workspace, float* dw,
+                        void* stream);
+
 #ifdef __cplusplus
 }
 #endif
