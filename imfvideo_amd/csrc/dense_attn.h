@@ -10,9 +10,12 @@
 // in LDS (ds_read_b64_tr_b16), rows in the same order.  Probabilities never leave
 // the registers.
 //
-// LDS tile: 64 rows x 128 bytes, the 16-byte chunk c of row r at chunk c ^ (r & 7), so that
-// the 32 rows of an operand read and the 8 rows x 64 bytes of a transposing read
-// spread over all banks.  The tiles are loaded straight into LDS (buffer_load ... lds): the
+// LDS tile: 64 rows x 128 bytes, the 16-byte chunk c of row r at chunk c ^ key(r), key(r) the
+// bits 1, 2, 3 of r reversed.  The 64 banks serve 256 bytes a cycle: 16 lanes of an operand read
+// (one chunk of 16 rows: rows of one parity share 32 banks and have eight different keys) and 32
+// lanes of a transposing read (64 bytes of four rows: the rows of one parity differ in the
+// key's top bit, so their chunk quads do not meet).  Without conflicts for both; with r & 7 as
+// the key both take twice the cycles.  The tiles are loaded straight into LDS (buffer_load ... lds): the
 // swizzle is applied to the chunk each lane fetches, and rows past the end of a sequence come
 // back as zeros from the buffer's range check, whatever memory holds there.
 #pragma once
@@ -63,20 +66,48 @@ __device__ inline __amdgpu_buffer_rsrc_t rows_rsrc(const uint16_t* base, int64_t
 }
 
 // Byte address (within a tile) of the 16-byte chunk c of row r.
-__device__ inline int chunk_addr(int r, int c) { return r * kRowB + ((c ^ (r & 7)) << 4); }
+__device__ inline int row_key(int r) {
+  return ((r << 1) & 4) | ((r >> 1) & 2) | ((r >> 3) & 1);
+}
+__device__ inline int chunk_addr(int r, int c) { return r * kRowB + ((c ^ row_key(r)) << 4); }
 
-// Row operand (A or B) of rows r0 + (l & 31): step s contracts channels 16 s .. 16 s + 15.
-__device__ inline u32x4 row_frag(const unsigned char* tile, int r0, int s, int l) {
-  return *reinterpret_cast<const u32x4*>(tile + chunk_addr(r0 + (l & 31), 2 * s + (l >> 5)));
+// Loads eight rows (8 j .. 8 j + 7 of a tile) straight into LDS: lane l brings the chunk of
+// row 8 j + l / 8 that belongs at its place.
+__device__ inline void dma_rows8(__amdgpu_buffer_rsrc_t rs, unsigned char* tile, int j, int ld,
+                                 int l) {
+  const int r = 8 * j + (l >> 3);
+  dma16(rs, tile + 8 * j * kRowB, r * ld + (((l & 7) ^ row_key(r)) << 4));
+}
+
+// A lane's byte offsets in a tile, for the operand reads below: eight registers, everything
+// else is an immediate of the read.
+struct LaneOff {
+  int row[4];     // chunk 2 s + h of row l & 31
+  int col[2][2];  // channels 32 mb .. of rows 4 h + .., and of the rows eight further on
+  __device__ explicit LaneOff(int l) {
+    const int h = l >> 5;
+#pragma unroll
+    for (int s = 0; s < 4; ++s) row[s] = chunk_addr(l & 31, 2 * s + h);
+    const int r = 4 * h + ((l & 15) >> 2), c = 2 * ((l >> 4) & 1) + ((l & 3) >> 1);
+#pragma unroll
+    for (int mb = 0; mb < 2; ++mb)
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
+        col[mb][x] = chunk_addr(r + 8 * x, 4 * mb + c) + 8 * (l & 1);
+  }
+};
+
+// Row operand (A or B) of rows r0 + (l & 31), r0 a multiple of 32: step s contracts channels
+// 16 s .. 16 s + 15.
+__device__ inline u32x4 row_frag(const unsigned char* tile, int r0, int s, const LaneOff& o) {
+  return *reinterpret_cast<const u32x4*>(tile + o.row[s] + r0 * kRowB);
 }
 
 // Transposed operand: row = channel 32 mb + (l & 31), contracted over the tile's rows
-// r0 .. r0 + 15 in the order of a C tile's registers (see above).
-__device__ inline u32x4 col_frag(const unsigned char* tile, int r0, int mb, int l) {
-  const int h = l >> 5, gs = (l >> 4) & 1, r = r0 + 4 * h + ((l & 15) >> 2);
-  const int c = 4 * mb + 2 * gs + ((l & 3) >> 1), o = 8 * (l & 1);
-  const u32x2 lo = lds_read_tr16(tile + chunk_addr(r, c) + o);
-  const u32x2 hi = lds_read_tr16(tile + chunk_addr(r + 8, c) + o);
+// r0 .. r0 + 15 (r0 a multiple of 16) in the order of a C tile's registers (see above).
+__device__ inline u32x4 col_frag(const unsigned char* tile, int r0, int mb, const LaneOff& o) {
+  const u32x2 lo = lds_read_tr16(tile + o.col[mb][0] + r0 * kRowB);
+  const u32x2 hi = lds_read_tr16(tile + o.col[mb][1] + r0 * kRowB);
   return u32x4{lo.x, lo.y, hi.x, hi.y};
 }
 

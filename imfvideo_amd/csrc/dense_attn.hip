@@ -4,10 +4,10 @@
 //   o = softmax(S) v,  lse = log sum exp S;  a row without a key: o = 0, lse = -inf.
 //
 // One pass over the keys: O^T += V^T P^T with P = exp2(S - m), row sums beside it, m a
-// running row bound in log2 units.  m moves only when a tile's maximum exceeds it by more
-// than kSlack (a wave-uniform, rarely taken branch rescales the accumulators): the
-// result does not depend on m beyond rounding, and the common path needs no
-// exchange between lanes.  P is rounded to the operands' 16-bit type for the product (an
+// row bound in log2 units, the maximum of the first keys.  It moves only when a tile's sums
+// show that its probabilities have outgrown the range set aside for them (a wave-uniform,
+// rarely taken branch computes the tile again and rescales the accumulators): the result
+// does not depend on m beyond rounding, and the common path computes no maximum.  P is rounded to the operands' 16-bit type for the product (an
 // error of half a unit in its last place per term, as the inputs themselves carry); row sums
 // add the fp32 values, so that lse, which the backward builds on, is exact to fp32.
 #include "dense_attn.h"
@@ -18,17 +18,17 @@ namespace sla2h {
 
 namespace {
 
-// Probabilities are held as exp2(S - m + shift) <= 2^(shift + slack).  fp16 spends its
-// exponent range on the small ones (2^-24 to 2^15); bf16 has fp32's range.
+// Probabilities are held as exp2(S - m + shift); a lane's sum of 16 stays at or below `most`.
+// fp16 spends its exponent range on the small ones (2^-24 to 2^15); bf16 has fp32's range.
 template <typename T16>
 struct Range;
 template <>
 struct Range<BF16> {
-  static constexpr float shift = 0.f, slack = 10.f;
+  static constexpr float shift = 0.f, most = 1024.f;
 };
 template <>
 struct Range<F16> {
-  static constexpr float shift = 9.f, slack = 6.f;
+  static constexpr float shift = 9.f, most = 32768.f;
 };
 constexpr float kFloor = -1e30f;  // m before the first key (finite: -inf - m stays -inf)
 
@@ -51,35 +51,40 @@ struct DenseFwdArgs {
   int64_t nrows;      // B * H * Lq
 };
 
-// One 32-key x 32-query score tile: mask, running bound, probabilities.  Returns the
-// packed operands of the two product steps.  acc: the O^T tiles to rescale.
-template <typename T16>
-__device__ inline void softmax_tile(f32x16& s, float c, float& m, float& mthr, float& lsum,
-                                    f32x16 (&acc)[2], u32x4 (&p)[2]) {
+// Largest of a lane's 16 scores.
+__device__ inline float lane_max(const f32x16& s) {
   float mx = fmaxf(fmaxf(s[0], s[1]), s[2]);
 #pragma unroll
   for (int i = 3; i < 15; i += 2) mx = fmaxf(fmaxf(mx, s[i]), s[i + 1]);
-  mx = fmaxf(mx, s[15]);
-  if (__builtin_amdgcn_ballot_w64(mx > mthr)) {
-    const float mn = fmaxf(m, swap32_max(mx) * c);
-    const float f = fast_exp2(m - mn);
-    m = mn;
-    mthr = (mn + Range<T16>::slack) / c;
-    lsum *= f;
+  return fmaxf(mx, s[15]);
+}
+
+// Moves the bound of a 32-key x 32-query tile to its maximum and rescales what the old
+// bound weighed.
+__device__ inline void raise_bound(float mx, float c, float& m, float& lsum, f32x16 (&acc)[2]) {
+  const float mn = fmaxf(m, swap32_max(mx) * c);
+  const float f = fast_exp2(m - mn);
+  m = mn;
+  lsum *= f;
 #pragma unroll
-    for (int b = 0; b < 2; ++b)
+  for (int b = 0; b < 2; ++b)
 #pragma unroll
-      for (int i = 0; i < 16; ++i) acc[b][i] *= f;
-  }
+    for (int i = 0; i < 16; ++i) acc[b][i] *= f;
+}
+
+// Probabilities of a tile, packed as the operands of the two product steps; their sum.
+template <typename T16>
+__device__ inline float probabilities(const f32x16& s, float c, float m, u32x4 (&p)[2]) {
   const float off = Range<T16>::shift - m;
+  f32x16 e;
 #pragma unroll
-  for (int i = 0; i < 16; ++i) s[i] = fast_exp2(__builtin_fmaf(s[i], c, off));
+  for (int i = 0; i < 16; ++i) e[i] = fast_exp2(__builtin_fmaf(s[i], c, off));
 #pragma unroll
-  for (int t = 0; t < 2; ++t) p[t] = pack_step<T16>(s, t);
+  for (int t = 0; t < 2; ++t) p[t] = pack_step<T16>(e, t);
   float r[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) r[i] = (s[i] + s[4 + i]) + (s[8 + i] + s[12 + i]);
-  lsum += (r[0] + r[1]) + (r[2] + r[3]);
+  for (int i = 0; i < 4; ++i) r[i] = (e[i] + e[4 + i]) + (e[8 + i] + e[12 + i]);
+  return (r[0] + r[1]) + (r[2] + r[3]);
 }
 
 // scores of keys at or past a lane's limit -> -inf; lim counts from the tile's first key
@@ -99,11 +104,14 @@ __device__ inline int key_limit(int i, int qlen, int klen, int causal) {
 }
 
 // Workgroup = 4 waves x (32 NQ) query rows of one head; all waves read the key and value
-// tiles of 64 rows from LDS, loaded three slots ahead with one barrier per tile.
+// tiles of 64 rows from LDS, loaded three tiles ahead into four slots with one barrier per tile.
+// The step of 32 keys is software-pipelined: its scores were computed one step earlier, so
+// that the score products of the next step, which depend on nothing here, run on the matrix
+// cores under this step's exponentials; operands of the step after are read from LDS meanwhile.
 template <typename T16, int NQ>
 __global__ __launch_bounds__(256, 2) void dense_fwd_kernel(DenseFwdArgs a) {
-  __shared__ __align__(16) unsigned char k0[kTileB], k1[kTileB], k2[kTileB];
-  __shared__ __align__(16) unsigned char v0[kTileB], v1[kTileB], v2[kTileB];
+  __shared__ __align__(16) unsigned char k0[kTileB], k1[kTileB], k2[kTileB], k3[kTileB];
+  __shared__ __align__(16) unsigned char v0[kTileB], v1[kTileB], v2[kTileB], v3[kTileB];
   const int logical = (blockIdx.x & 7) * a.per_xcd + (blockIdx.x >> 3);
   if (logical >= a.nwork) return;
   const int bh = __builtin_amdgcn_readfirstlane(logical / a.qtiles);
@@ -113,6 +121,7 @@ __global__ __launch_bounds__(256, 2) void dense_fwd_kernel(DenseFwdArgs a) {
   const int b = bh / a.H, hq = bh - b * a.H, hk = hq / a.rep;
   const int tid = threadIdx.x, l = tid & 63, h = l >> 5;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const LaneOff lo(l);
   const int qlen = seq_len(a.q_lens, b, a.Lq), klen = seq_len(a.k_lens, b, a.Lk);
 
   const int q0 = qt * (128 * NQ);           // first row of the workgroup
@@ -124,16 +133,14 @@ __global__ __launch_bounds__(256, 2) void dense_fwd_kernel(DenseFwdArgs a) {
   const uint16_t* kp = a.k + b * a.kb + hk * a.kh;
   const uint16_t* vp = a.v + b * a.vb + hk * a.vh;
   const int64_t kld = a.kl * 2, vld = a.vl * 2;
-  const int lrow = l >> 3, lch = ((l & 7) ^ lrow) << 4;
-  auto load_tile = [&](int t, unsigned char* kt, unsigned char* vt) {
+  auto load_tile = [&](int t, unsigned char* kt, unsigned char* vt) __attribute__((always_inline)) {
     const int64_t n = (int64_t)klen - (int64_t)t * kTileRows;
     const auto rk = rows_rsrc(kp, (int64_t)t * kTileRows, n, kld);
     const auto rv = rows_rsrc(vp, (int64_t)t * kTileRows, n, vld);
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const int r = 16 * w + 8 * i;
-      dma16(rk, kt + r * kRowB, (r + lrow) * (int)kld + lch);
-      dma16(rv, vt + r * kRowB, (r + lrow) * (int)vld + lch);
+      dma_rows8(rk, kt, 2 * w + i, (int)kld, l);
+      dma_rows8(rv, vt, 2 * w + i, (int)vld, l);
     }
   };
 
@@ -157,62 +164,106 @@ __global__ __launch_bounds__(256, 2) void dense_fwd_kernel(DenseFwdArgs a) {
   const int wall = wlast >= qw ? key_limit(qw, qlen, klen, a.causal) : 0;
 
   f32x16 acc[NQ][2];
-  float m[NQ], mthr[NQ], lsum[NQ];
+  float m[NQ], lsum[NQ];
 #pragma unroll
   for (int n = 0; n < NQ; ++n) {
     acc[n][0] = zero16();
     acc[n][1] = zero16();
     m[n] = kFloor;
-    mthr[n] = kFloor;
     lsum[n] = 0.f;
   }
 
-  auto compute = [&](int t, const unsigned char* kt, const unsigned char* vt) {
-    const int base = t * kTileRows;
-    if (base >= wany) return;
+  f32x16 sc[2][NQ];
+  u32x4 kf[4];
+  auto read_k = [&](const unsigned char* kt, int kb) __attribute__((always_inline)) {
 #pragma unroll
-    for (int kb = 0; kb < 2; ++kb) {
-      u32x4 kf[4];
+    for (int s = 0; s < 4; ++s) kf[s] = row_frag(kt, 32 * kb, s, lo);
+  };
+  auto scores = [&](int kb) __attribute__((always_inline)) {
 #pragma unroll
-      for (int s = 0; s < 4; ++s) kf[s] = row_frag(kt, 32 * kb, s, l);
-      u32x4 p[NQ][2];
+    for (int n = 0; n < NQ; ++n) sc[kb][n] = zero16();
 #pragma unroll
-      for (int n = 0; n < NQ; ++n) {
-        f32x16 sc = zero16();
+    for (int s = 0; s < 4; ++s)
 #pragma unroll
-        for (int s = 0; s < 4; ++s) sc = mfma_32x32x16<T16>(kf[s], qf[n][s], sc);
-        if (base + kTileRows > wall) mask_tile(sc, lim[n] - base - 32 * kb, h);
-        softmax_tile<T16>(sc, a.c, m[n], mthr[n], lsum[n], acc[n], p[n]);
-      }
+      for (int n = 0; n < NQ; ++n) sc[kb][n] = mfma_32x32x16<T16>(kf[s], qf[n][s], sc[kb][n]);
+  };
+  auto mask = [&](int kb, int base) __attribute__((always_inline)) {
+    if (base + 32 > wall) {
+      asm volatile("");  // a branch: rare, and 64 selects when speculated
 #pragma unroll
-      for (int s = 0; s < 2; ++s)
-#pragma unroll
-        for (int mb = 0; mb < 2; ++mb) {
-          const u32x4 vf = col_frag(vt, 32 * kb + 16 * s, mb, l);
-#pragma unroll
-          for (int n = 0; n < NQ; ++n) acc[n][mb] = mfma_32x32x16<T16>(vf, p[n][s], acc[n][mb]);
-        }
+      for (int n = 0; n < NQ; ++n) mask_tile(sc[kb][n], lim[n] - base, h);
     }
   };
-
-  // Tile t lives in slot t % 3; tiles loaded past the last one are empty (zeros).
+  auto raise = [&](int kb) __attribute__((always_inline)) {
+#pragma unroll
+    for (int n = 0; n < NQ; ++n)
+      raise_bound(lane_max(sc[kb][n]), a.c, m[n], lsum[n], acc[n]);
+  };
+  // one step: keys 32 kb .. of tile t; kn, kb: the step after next
+  auto step = [&](int t, int kb, const unsigned char* kt, const unsigned char* vt,
+                  const unsigned char* kn) __attribute__((always_inline)) {
+    const int base = t * kTileRows + 32 * kb;
+    u32x4 vf[2][2], p[NQ][2];
+    float r[NQ];
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+      for (int mb = 0; mb < 2; ++mb) vf[s][mb] = col_frag(vt, 32 * kb + 16 * s, mb, lo);
+    mask(kb, base);
+    scores(kb ^ 1);
+    read_k(kn, kb);
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) r[n] = probabilities<T16>(sc[kb][n], a.c, m[n], p[n]);
+    bool over = r[0] > Range<T16>::most;
+    if (NQ == 2) over = over || r[NQ - 1] > Range<T16>::most;
+    if (__builtin_amdgcn_ballot_w64(over)) {  // the step's scores again, under a new bound
+      read_k(kt, kb);
+      scores(kb);
+      mask(kb, base);
+      raise(kb);
+#pragma unroll
+      for (int n = 0; n < NQ; ++n) r[n] = probabilities<T16>(sc[kb][n], a.c, m[n], p[n]);
+      read_k(kn, kb);
+    }
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) lsum[n] += r[n];
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+      for (int mb = 0; mb < 2; ++mb)
+#pragma unroll
+        for (int n = 0; n < NQ; ++n)
+          acc[n][mb] = mfma_32x32x16<T16>(vf[s][mb], p[n][s], acc[n][mb]);
+  };
+  // Tile t lives in slot t % 4; tiles past the last one are empty (zeros).  At the top of
+  // tile t the tiles up to t + 1 have landed and tile t - 1 is read.
+  auto tile = [&](int t, const unsigned char* kt, const unsigned char* vt,
+                  const unsigned char* kt1, unsigned char* kl, unsigned char* vl) __attribute__((always_inline)) {
+    __builtin_amdgcn_s_waitcnt(wait_vm_lgkm0(4));
+    __builtin_amdgcn_s_barrier();
+    load_tile(t + 3, kl, vl);
+    if (t * kTileRows >= wany) return;
+    step(t, 0, kt, vt, kt1);
+    step(t, 1, kt, vt, kt1);
+  };
   load_tile(0, k0, v0);
   load_tile(1, k1, v1);
-  for (int t = 0; t < nt; t += 3) {
-    __builtin_amdgcn_s_waitcnt(wait_vm_lgkm0(4));
-    __builtin_amdgcn_s_barrier();  // tile t has landed, tile t - 1 is read
-    load_tile(t + 2, k2, v2);
-    compute(t, k0, v0);
+  load_tile(2, k2, v2);
+  __builtin_amdgcn_s_waitcnt(wait_vm_lgkm0(8));
+  __builtin_amdgcn_s_barrier();
+  read_k(k0, 0);
+  scores(0);
+  mask(0, 0);
+  raise(0);
+  read_k(k0, 1);
+  for (int t = 0; t < nt; t += 4) {
+    tile(t, k0, v0, k1, k3, v3);
     if (t + 1 >= nt) break;
-    __builtin_amdgcn_s_waitcnt(wait_vm_lgkm0(4));
-    __builtin_amdgcn_s_barrier();
-    load_tile(t + 3, k0, v0);
-    compute(t + 1, k1, v1);
+    tile(t + 1, k1, v1, k2, k0, v0);
     if (t + 2 >= nt) break;
-    __builtin_amdgcn_s_waitcnt(wait_vm_lgkm0(4));
-    __builtin_amdgcn_s_barrier();
-    load_tile(t + 4, k1, v1);
-    compute(t + 2, k2, v2);
+    tile(t + 2, k2, v2, k3, k1, v1);
+    if (t + 3 >= nt) break;
+    tile(t + 3, k3, v3, k0, k2, v2);
   }
   __builtin_amdgcn_s_waitcnt(wait_vm_lgkm0(0));  // no load into this LDS outlives the workgroup
 
@@ -253,6 +304,7 @@ __global__ __launch_bounds__(256, 2) void dense_fwd_split_kernel(DenseFwdArgs a)
   const int b = bk / a.Hkv, hk = bk - b * a.Hkv;
   const int tid = threadIdx.x, l = tid & 63, h = l >> 5;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const LaneOff lo(l);
   const int qlen = seq_len(a.q_lens, b, a.Lq), klen = seq_len(a.k_lens, b, a.Lk);
 
   // row of the group: head hk rep + row / Lq, query row % Lq
@@ -273,17 +325,16 @@ __global__ __launch_bounds__(256, 2) void dense_fwd_split_kernel(DenseFwdArgs a)
   const uint16_t* kp = a.k + b * a.kb + hk * a.kh;
   const uint16_t* vp = a.v + b * a.vb + hk * a.vh;
   const int64_t kld = a.kl * 2, vld = a.vl * 2;
-  const int lrow = l >> 3, lch = ((l & 7) ^ lrow) << 4;
   const int64_t u0 = (int64_t)sp * a.units;
   const int64_t uend = min(u0 + a.units, ((int64_t)kmax + 31) / 32);
-  auto load_unit = [&](int64_t u, unsigned char* kv) {
+  auto load_unit = [&](int64_t u, unsigned char* kv) __attribute__((always_inline)) {
     const int64_t n = u < uend ? min((int64_t)klen - u * 32, (int64_t)32) : 0;
     const auto rk = rows_rsrc(kp, u * 32, n, kld);
     const auto rv = rows_rsrc(vp, u * 32, n, vld);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      dma16(rk, kv + 8 * j * kRowB, (8 * j + lrow) * (int)kld + lch);
-      dma16(rv, kv + kUnitB + 8 * j * kRowB, (8 * j + lrow) * (int)vld + lch);
+      dma_rows8(rk, kv, j, (int)kld, l);
+      dma_rows8(rv, kv + kUnitB, j, (int)vld, l);
     }
   };
 
@@ -295,19 +346,25 @@ __global__ __launch_bounds__(256, 2) void dense_fwd_split_kernel(DenseFwdArgs a)
       qf[s] = lim > 0 ? *reinterpret_cast<const u32x4*>(qp + 16 * s + 8 * h) : u32x4{0, 0, 0, 0};
   }
   f32x16 acc[2] = {zero16(), zero16()};
-  float m = kFloor, mthr = kFloor, lsum = 0.f;
-  auto compute = [&](int64_t u, const unsigned char* kv) {
+  float m = kFloor, lsum = 0.f;
+  auto compute = [&](int64_t u, const unsigned char* kv) __attribute__((always_inline)) {
     f32x16 sc = zero16();
 #pragma unroll
-    for (int s = 0; s < 4; ++s) sc = mfma_32x32x16<T16>(row_frag(kv, 0, s, l), qf[s], sc);
+    for (int s = 0; s < 4; ++s) sc = mfma_32x32x16<T16>(row_frag(kv, 0, s, lo), qf[s], sc);
     if (u * 32 + 32 > kmin) mask_tile(sc, (int)(lim - u * 32), h);
+    // the wave's first unit sets the bound of the rows that see a key of it
     u32x4 p[2];
-    softmax_tile<T16>(sc, a.c, m, mthr, lsum, acc, p);
+    float r = probabilities<T16>(sc, a.c, m, p);
+    if (__builtin_amdgcn_ballot_w64(r > Range<T16>::most)) {
+      raise_bound(lane_max(sc), a.c, m, lsum, acc);
+      r = probabilities<T16>(sc, a.c, m, p);
+    }
+    lsum += r;
 #pragma unroll
     for (int s = 0; s < 2; ++s)
 #pragma unroll
       for (int mb = 0; mb < 2; ++mb)
-        acc[mb] = mfma_32x32x16<T16>(col_frag(kv + kUnitB, 16 * s, mb, l), p[s], acc[mb]);
+        acc[mb] = mfma_32x32x16<T16>(col_frag(kv + kUnitB, 16 * s, mb, lo), p[s], acc[mb]);
   };
   int64_t u = u0 + w;
   load_unit(u, kv0[w]);

@@ -177,11 +177,12 @@ __global__ __launch_bounds__(256, 2) void dense_bwd_dq_kernel(DenseBwdArgs a) {
   const int b = bh / a.H, hq = bh - b * a.H, hk = hq / a.rep;
   const int tid = threadIdx.x, l = tid & 63, h = l >> 5;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const LaneOff lo(l);
   const int qlen = seq_len(a.q_lens, b, a.Lq), klen = seq_len(a.k_lens, b, a.Lk);
 
   const int q0 = qt * (128 * NQ), qw = q0 + w * (32 * NQ);
   const int qend = min(q0 + 128 * NQ, qlen);
-  auto limit = [&](int i) {
+  auto limit = [&](int i) __attribute__((always_inline)) {
     if (i >= qlen) return 0;
     if (!a.causal) return klen;
     const int64_t e = (int64_t)i + klen - qlen + 1;
@@ -195,16 +196,14 @@ __global__ __launch_bounds__(256, 2) void dense_bwd_dq_kernel(DenseBwdArgs a) {
   const uint16_t* kp = a.k + b * a.kb + hk * a.kh;
   const uint16_t* vp = a.v + b * a.vb + hk * a.vh;
   const int64_t kld = a.kl * 2, vld = a.vl * 2;
-  const int lrow = l >> 3, lch = ((l & 7) ^ lrow) << 4;
-  auto load_tile = [&](int t, unsigned char* kt, unsigned char* vt) {
+  auto load_tile = [&](int t, unsigned char* kt, unsigned char* vt) __attribute__((always_inline)) {
     const int64_t n = (int64_t)klen - (int64_t)t * kTileRows;
     const auto rk = rows_rsrc(kp, (int64_t)t * kTileRows, n, kld);
     const auto rv = rows_rsrc(vp, (int64_t)t * kTileRows, n, vld);
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const int r = 16 * w + 8 * i;
-      dma16(rk, kt + r * kRowB, (r + lrow) * (int)kld + lch);
-      dma16(rv, vt + r * kRowB, (r + lrow) * (int)vld + lch);
+      dma_rows8(rk, kt, 2 * w + i, (int)kld, l);
+      dma_rows8(rv, vt, 2 * w + i, (int)vld, l);
     }
   };
 
@@ -240,7 +239,7 @@ __global__ __launch_bounds__(256, 2) void dense_bwd_dq_kernel(DenseBwdArgs a) {
 #pragma unroll
   for (int n = 0; n < NQ; ++n) acc[n][0] = acc[n][1] = zero16();
 
-  auto compute = [&](int t, const unsigned char* kt, const unsigned char* vt) {
+  auto compute = [&](int t, const unsigned char* kt, const unsigned char* vt) __attribute__((always_inline)) {
     const int base = t * kTileRows;
     if (base >= wany) return;
 #pragma unroll
@@ -248,8 +247,8 @@ __global__ __launch_bounds__(256, 2) void dense_bwd_dq_kernel(DenseBwdArgs a) {
       u32x4 kf[4], vf[4];
 #pragma unroll
       for (int s = 0; s < 4; ++s) {
-        kf[s] = row_frag(kt, 32 * kb, s, l);
-        vf[s] = row_frag(vt, 32 * kb, s, l);
+        kf[s] = row_frag(kt, 32 * kb, s, lo);
+        vf[s] = row_frag(vt, 32 * kb, s, lo);
       }
       u32x4 ds[NQ][2];
 #pragma unroll
@@ -277,7 +276,7 @@ __global__ __launch_bounds__(256, 2) void dense_bwd_dq_kernel(DenseBwdArgs a) {
       for (int s = 0; s < 2; ++s)
 #pragma unroll
         for (int mb = 0; mb < 2; ++mb) {
-          const u32x4 kc = col_frag(kt, 32 * kb + 16 * s, mb, l);
+          const u32x4 kc = col_frag(kt, 32 * kb + 16 * s, mb, lo);
 #pragma unroll
           for (int n = 0; n < NQ; ++n) acc[n][mb] = mfma_32x32x16<T16>(kc, ds[n][s], acc[n][mb]);
         }
@@ -334,6 +333,7 @@ __global__ __launch_bounds__(256, NK == 1 ? 2 : 1) void dense_bwd_dkdv_kernel(De
   const int b = bk / a.Hkv, hk = bk - b * a.Hkv;
   const int tid = threadIdx.x, l = tid & 63, h = l >> 5;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const LaneOff lo(l);
   const int qlen = seq_len(a.q_lens, b, a.Lq), klen = seq_len(a.k_lens, b, a.Lk);
 
   const int key0 = ktile * (128 * NK), kw = key0 + w * (32 * NK);
@@ -347,8 +347,7 @@ __global__ __launch_bounds__(256, NK == 1 ? 2 : 1) void dense_bwd_dkdv_kernel(De
   const int u0 = sp * per, u1 = min(total, u0 + per);
 
   const int64_t qld = a.ql * 2, gld = a.gl * 2;
-  const int lrow = l >> 3, lch = ((l & 7) ^ lrow) << 4;
-  auto load_tile = [&](int u, unsigned char* qt, unsigned char* gt, float (*st)[64]) {
+  auto load_tile = [&](int u, unsigned char* qt, unsigned char* gt, float (*st)[64]) __attribute__((always_inline)) {
     const int r = u < u1 ? u / nq : 0;
     const int hq = hk * a.rep + r;
     const int row = first + (u - r * nq) * kTileRows;
@@ -360,9 +359,8 @@ __global__ __launch_bounds__(256, NK == 1 ? 2 : 1) void dense_bwd_dkdv_kernel(De
                               n <= 0 ? 0 : (n < 64 ? n : 64) * 4);
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const int rr = 16 * w + 8 * i;
-      dma16(rq, qt + rr * kRowB, (rr + lrow) * (int)qld + lch);
-      dma16(rg, gt + rr * kRowB, (rr + lrow) * (int)gld + lch);
+      dma_rows8(rq, qt, 2 * w + i, (int)qld, l);
+      dma_rows8(rg, gt, 2 * w + i, (int)gld, l);
     }
     // waves 0 and 2 bring -lse, 1 and 3 -delta (the same values twice)
     __builtin_amdgcn_raw_ptr_buffer_load_lds(
@@ -391,7 +389,7 @@ __global__ __launch_bounds__(256, NK == 1 ? 2 : 1) void dense_bwd_dkdv_kernel(De
   for (int n = 0; n < NK; ++n) ak[n][0] = ak[n][1] = av[n][0] = av[n][1] = zero16();
 
   auto compute = [&](int u, const unsigned char* qt, const unsigned char* gt,
-                     const float (*st)[64]) {
+                     const float (*st)[64]) __attribute__((always_inline)) {
     const int row = first + (u % nq) * kTileRows;
     if (kw >= klen) return;
 #pragma unroll
@@ -399,8 +397,8 @@ __global__ __launch_bounds__(256, NK == 1 ? 2 : 1) void dense_bwd_dkdv_kernel(De
       u32x4 qa[4], ga[4];
 #pragma unroll
       for (int s = 0; s < 4; ++s) {
-        qa[s] = row_frag(qt, 32 * qb, s, l);
-        ga[s] = row_frag(gt, 32 * qb, s, l);
+        qa[s] = row_frag(qt, 32 * qb, s, lo);
+        ga[s] = row_frag(gt, 32 * qb, s, lo);
       }
       u32x4 p[NK][2], ds[NK][2];
 #pragma unroll
@@ -440,8 +438,8 @@ __global__ __launch_bounds__(256, NK == 1 ? 2 : 1) void dense_bwd_dkdv_kernel(De
       for (int s = 0; s < 2; ++s)
 #pragma unroll
         for (int mb = 0; mb < 2; ++mb) {
-          const u32x4 gc = col_frag(gt, 32 * qb + 16 * s, mb, l);
-          const u32x4 qc = col_frag(qt, 32 * qb + 16 * s, mb, l);
+          const u32x4 gc = col_frag(gt, 32 * qb + 16 * s, mb, lo);
+          const u32x4 qc = col_frag(qt, 32 * qb + 16 * s, mb, lo);
 #pragma unroll
           for (int n = 0; n < NK; ++n) {
             av[n][mb] = mfma_32x32x16<T16>(gc, p[n][s], av[n][mb]);

@@ -207,14 +207,15 @@ __device__ inline void widen16(u32x4 c, u32x4& lo, u32x4& hi) {
 }
 
 // Workgroup = one 128 x 128 tile of dW over one range of row tiles, wave (wm, wn) 64 x 64 of it
-// (one code tile wide, so its scale is one number per stage).  A stage is 64 rows: dY goes to
-// LDS as it is (DMA: buffer loads straight into LDS, for 16-byte aligned rows; else through
-// registers), the codes are widened on their way, two slots each, and the fragments are
-// read transposed as in wgrad_kernel.
+// (one code tile wide, so its scale is one number per stage).  A stage is 64 rows in one of two
+// LDS slots: dY goes there as it is (DMA: buffer loads straight into LDS, for 16-byte
+// aligned rows; else through registers, as aligned dwords funnelled to the row's start), the
+// codes are widened on their way, and the fragments are read transposed.  A slot is an array
+// of its own: LDS reads of one then need not wait for the loads into the other.
 template <typename T16, bool DMA>
 __global__ __launch_bounds__(256, 2) void wgrad8_kernel(Wgrad8Args a) {
-  __shared__ __align__(16) unsigned char ly[2 * kAStage];
-  __shared__ __align__(16) unsigned char lx[2 * kAStage];
+  __shared__ __align__(16) unsigned char ly0[kAStage], ly1[kAStage];
+  __shared__ __align__(16) unsigned char lx0[kAStage], lx1[kAStage];
   const int logical = (blockIdx.x & 7) * a.per_xcd + (blockIdx.x >> 3);
   if (logical >= a.nwork) return;
   const int sp = __builtin_amdgcn_readfirstlane(logical / a.tiles);
@@ -228,53 +229,70 @@ __global__ __launch_bounds__(256, 2) void wgrad8_kernel(Wgrad8Args a) {
   const int l = tid & 63, r = l & 15, g = l >> 4;
   const int wm = w >> 1, wn = w & 1;
 
-  // dY: rows past the last one read as zero
+  // dY rows of stage s as a buffer from the dword that holds its first element, rows past the
+  // last one read as zero; a column past M reads the next row's and only ever feeds an
+  // output that is not stored.
   const int64_t ld2 = a.ldy * 2;
-  const int lrow = 4 * w + (l >> 4);
-  const int col = ((((l & 15) >> 1) ^ (lrow & 7)) << 5) + (l & 1) * 16;
-  const int voff = lrow * (int)ld2 + m0 * 2 + col;
-  auto dma_y = [&](int s) {
-    const int64_t row = (t0 + s) * kAct;
-    const int64_t left = s < nst ? a.rows - row : 0;
-    const auto ry = make_rsrc(reinterpret_cast<const char*>(a.dy) + row * ld2,
-                              left <= 0 ? 0 : ((left < kAct ? left : kAct) - 1) * ld2 + a.M * 2);
-    unsigned char* p = ly + (s & 1) * kAStage + w * 1024;
-#pragma unroll
-    for (int k = 0; k < 4; ++k) dma16(ry, p + 4096 * k, voff + 16 * k * (int)ld2);
+  const int odd = (int)((uintptr_t)a.dy & 2);
+  auto rows_of = [&](int s) __attribute__((always_inline)) {
+    const int64_t row = (t0 + s) * kAct, left = s < nst ? a.rows - row : 0;
+    const uintptr_t p = (uintptr_t)a.dy + row * ld2;
+    const int64_t n = ((left < kAct ? left : kAct) - 1) * ld2 + a.M * 2 + (p & 2);
+    return make_rsrc(reinterpret_cast<const void*>(p & ~(uintptr_t)3),
+                     left <= 0 ? 0 : (n + 3) & ~(int64_t)3);
   };
-  // ... or element groups of any alignment through registers: row 16 k + tid / 16
-  const int yr = tid >> 4, yc = m0 + (tid & 15) * 8;
-  auto load_y = [&](int s, u32x4 (&v)[4]) {
+  const int lrow = 4 * w + (l >> 4);
+  const int voff = lrow * (int)ld2 + m0 * 2 + ((((l & 15) >> 1) ^ (lrow & 7)) << 5) + (l & 1) * 16;
+  auto dma_y = [&](int s, unsigned char* ly) __attribute__((always_inline)) {
+    const auto ry = rows_of(s);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) dma16(ry, ly + w * 1024 + 4096 * k, voff + 16 * k * (int)ld2);
+  };
+  // thread: row 16 k + tid / 16, eight elements; a stage's first row is an even number of
+  // elements past dy's, so its alignment is dy's
+  const int yr = tid >> 4;
+  auto y_off = [&](int k) { return (16 * k + yr) * (int)ld2 + m0 * 2 + (tid & 15) * 16 + odd; };
+  auto load_y = [&](int s, u32x4 (&v)[4], uint32_t (&x)[4]) __attribute__((always_inline)) {
+    const auto ry = rows_of(s);
+    // the range ends with a whole dword: the row behind the last one may begin in it
+    const int64_t left = a.rows - (t0 + s) * kAct;
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-      const int64_t row = (t0 + s) * kAct + 16 * k + yr;
-      v[k] = s < nst && row < a.rows ? load_row8(a.dy + row * a.ldy, yc, a.M) : u32x4{0, 0, 0, 0};
+      const int o = 16 * k + yr < left ? y_off(k) & ~3 : 0x7ffffff0;
+      v[k] = buf_load16(ry, o, 0);
+      x[k] = __builtin_amdgcn_raw_buffer_load_b32(ry, o + 16, 0, 0);
     }
   };
-  auto put_y = [&](int s, const u32x4 (&v)[4]) {
-    unsigned char* p = ly + (s & 1) * kAStage + yr * 256 +
-                       ((((tid & 15) >> 1) ^ (yr & 7)) << 5) + (tid & 1) * 16;
+  auto put_y = [&](unsigned char* ly, const u32x4 (&v)[4], const uint32_t (&x)[4])
+      __attribute__((always_inline)) {
+    unsigned char* p = ly + yr * 256 + ((((tid & 15) >> 1) ^ (yr & 7)) << 5) + (tid & 1) * 16;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) *reinterpret_cast<u32x4*>(p + 4096 * k) = v[k];
+    for (int k = 0; k < 4; ++k) {
+      const uint32_t sh = y_off(k) & 2;
+      *reinterpret_cast<u32x4*>(p + 4096 * k) =
+          u32x4{__builtin_amdgcn_alignbyte(v[k][1], v[k][0], sh),
+                __builtin_amdgcn_alignbyte(v[k][2], v[k][1], sh),
+                __builtin_amdgcn_alignbyte(v[k][3], v[k][2], sh),
+                __builtin_amdgcn_alignbyte(x[k], v[k][3], sh)};
+    }
   };
   // codes: threads 0 .. 127 the first tile's 4 KB, the others the second's, 16 bytes each twice
   // (always two loads, zeros past the last tile: the loop counts them)
   const int ct = n0 / kAct, xi = tid & 127;
   const int xoff = (tid >> 7) * kActBytes + xi * 16;
-  auto load_x = [&](int s, u32x4 (&v)[2]) {
+  auto load_x = [&](int s, u32x4 (&v)[2]) __attribute__((always_inline)) {
     const auto rx = make_rsrc(a.codes + ((t0 + s) * a.cb + ct) * kActBytes,
                               s < nst ? (a.cb - ct < 2 ? 1 : 2) * kActBytes : 0);
     v[0] = buf_load16(rx, xoff, 0);
     v[1] = buf_load16(rx, xoff + 2048, 0);
   };
-  auto put_x = [&](int s, const u32x4 (&v)[2]) {
+  auto put_x = [&](unsigned char* lx, const u32x4 (&v)[2]) __attribute__((always_inline)) {
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
       const int row = (xi >> 2) + 32 * k, c = 4 * (tid >> 7) + (xi & 3);
       u32x4 lo, hi;
       widen16<T16>(v[k], lo, hi);
-      u32x4* p = reinterpret_cast<u32x4*>(lx + (s & 1) * kAStage + row * 256 +
-                                          ((c ^ (row & 7)) << 5));
+      u32x4* p = reinterpret_cast<u32x4*>(lx + row * 256 + ((c ^ (row & 7)) << 5));
       p[0] = lo;
       p[1] = hi;
     }
@@ -284,15 +302,18 @@ __global__ __launch_bounds__(256, 2) void wgrad8_kernel(Wgrad8Args a) {
     return s < nst && st < a.cb ? a.scales[(t0 + s) * a.cb + st] : 0.f;
   };
 
+  // fragment reads: row 4 g + r / 4 (and + 16) of each half stage, chunk = 16-column sub-tile
   const int rho = 4 * g + (r >> 2);
-  const uint32_t by = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)ly;
-  const uint32_t bx = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)lx;
-  uint32_t fy[4], fx[4];
+  int fy[4], fx[4];
 #pragma unroll
   for (int t = 0; t < 4; ++t) {
-    fy[t] = by + rho * 256 + (((4 * wm + t) ^ (rho & 7)) << 5) + (r & 3) * 8;
-    fx[t] = bx + rho * 256 + (((4 * wn + t) ^ (rho & 7)) << 5) + (r & 3) * 8;
+    fy[t] = rho * 256 + (((4 * wm + t) ^ (rho & 7)) << 5) + (r & 3) * 8;
+    fx[t] = rho * 256 + (((4 * wn + t) ^ (rho & 7)) << 5) + (r & 3) * 8;
   }
+  auto frag = [&](const unsigned char* p) __attribute__((always_inline)) {
+    const u32x2 lo = lds_read_tr16(p), hi = lds_read_tr16(p + 4096);
+    return u32x4{lo.x, lo.y, hi.x, hi.y};
+  };
   f32x4 acc[4][4];  // [n sub-tile][m sub-tile]: lane holds dW[m = r][n = 4 g + i]
 #pragma unroll
   for (int i = 0; i < 4; ++i)
@@ -300,49 +321,59 @@ __global__ __launch_bounds__(256, 2) void wgrad8_kernel(Wgrad8Args a) {
     for (int j = 0; j < 4; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
 
   u32x4 xv[2], yv[4];
-  load_x(0, xv);
-  if (DMA) {
-    dma_y(0);
-  } else {
-    load_y(0, yv);
-    put_y(0, yv);
-    load_y(1, yv);
-  }
-  put_x(0, xv);
-  load_x(1, xv);
+  uint32_t ye[4];
   float sc = scale_of(0);
-  for (int s = 0; s < nst; ++s) {
+  // one stage: everything of stage s + 1 moves into the other slot meanwhile
+  auto stage = [&](int s, const unsigned char* ly, const unsigned char* lx, unsigned char* ny,
+                   unsigned char* nx) __attribute__((always_inline)) {
     // this wave's part of stage s is in LDS (the two loads of codes behind it may be
     // in flight), then everyone's, and stage s - 1 is read
     __builtin_amdgcn_s_waitcnt(DMA ? 0x0072 : 0xC07F);
     __builtin_amdgcn_s_barrier();
     if (DMA) {
-      dma_y(s + 1);
+      dma_y(s + 1, ny);
     } else {
-      put_y(s + 1, yv);
-      load_y(s + 2, yv);
+      put_y(ny, yv, ye);
+      load_y(s + 2, yv, ye);
     }
-    put_x(s + 1, xv);
+    put_x(nx, xv);
     load_x(s + 2, xv);
     const float scn = scale_of(s + 1);
-    u32x4 fm[2][4], fn[2][4];
+    u32x4 fm[2][4];
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      const uint32_t slot = (s & 1) * kAStage + k * 8192;
-      read_frags(fy, slot, fm[k]);
-      read_frags(fx, slot, fn[k]);
-    }
+    for (int k = 0; k < 2; ++k)
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+      for (int j = 0; j < 4; ++j) fm[k][j] = frag(ly + 8192 * k + fy[j]);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      u32x4 fn[2];
+#pragma unroll
+      for (int k = 0; k < 2; ++k) fn[k] = frag(lx + 8192 * k + fx[i]);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         f32x4 t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int k = 0; k < 2; ++k) t = mfma_16x16x32<T16>(fn[k][i], fm[k][j], t);
+        for (int k = 0; k < 2; ++k) t = mfma_16x16x32<T16>(fn[k], fm[k][j], t);
 #pragma unroll
         for (int e = 0; e < 4; ++e) acc[i][j][e] = __builtin_fmaf(sc, t[e], acc[i][j][e]);
       }
+    }
     sc = scn;
+  };
+  load_x(0, xv);
+  if (DMA) {
+    dma_y(0, ly0);
+  } else {
+    load_y(0, yv, ye);
+    put_y(ly0, yv, ye);
+    load_y(1, yv, ye);
+  }
+  put_x(lx0, xv);
+  load_x(1, xv);
+  for (int s = 0; s < nst; s += 2) {
+    stage(s, ly0, lx0, ly1, lx1);
+    if (s + 1 >= nst) break;
+    stage(s + 1, ly1, lx1, ly0, lx0);
   }
   __builtin_amdgcn_s_waitcnt(0x0070);  // no load into this workgroup's LDS outlives it
 

@@ -211,6 +211,10 @@ def test_weight_gradient(shape, dt):
         wide = torch.full((rows, M + 40), float("nan"), device="cuda", dtype=dt)
         wide[:, lo:lo + M] = dy.cuda()
         assert torch.equal(ops.linear_wgrad8(wide[:, lo:lo + M], a), dw), lo
+    # NaN right behind the last row
+    more = torch.full((rows * M + 64,), float("nan"), device="cuda", dtype=dt)
+    more[:rows * M] = dy.cuda().reshape(-1)
+    assert torch.equal(ops.linear_wgrad8(more[:rows * M].view(rows, M), a), dw)
 
 
 def test_module_keeps_8_bits_and_its_gradients():
