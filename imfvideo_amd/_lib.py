@@ -152,11 +152,11 @@ SIGNATURES = {
     "sla2h_dense_attn_fwd_workspace_bytes": (ctypes.c_size_t, [_c_int, _c_int, _c_int, _c_i64,
                                                                _c_i64]),
     "sla2h_dense_attn_fwd": (_c_int, [_p, _p, _p, _p, _p, _p, _c_int, _c_int, _c_int, _c_int,
-                                      _c_i64, _c_i64, _c_int, _c_f, _p, _p, _p, _p]),
+                                      _c_i64, _c_i64, _c_int, _c_f, _p, _p, _p, _p, _p]),
     "sla2h_dense_attn_bwd_workspace_bytes": (ctypes.c_size_t, [_c_int, _c_int, _c_int, _c_int,
                                                                _c_i64, _c_i64]),
-    "sla2h_dense_attn_bwd": (_c_int, [_p, _p, _p, _p, _p, _p, _p, _p, _p, _c_int, _c_int, _c_int,
-                                      _c_int, _c_i64, _c_i64, _c_int, _c_f, _p, _p, _p, _p, _p]),
+    "sla2h_dense_attn_bwd": (_c_int, [_p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _c_int, _c_int,
+                                      _c_int, _c_int, _c_i64, _c_i64, _c_int, _c_f, _p, _p, _p, _p, _p]),
     "sla2h_act8_pack": (_c_int, [_p, _c_i64, _c_int, _c_i64, _c_int, _p, _p, _p]),
     "sla2h_act8_unpack": (_c_int, [_p, _p, _c_int, _c_i64, _c_int, _p, _p]),
     "sla2h_situ8_fwd": (_c_int, [_p, _p, _c_int, _c_i64, _c_int, _c_i64, _c_i64, _c_f, _c_f, _p,

@@ -34,7 +34,7 @@ constexpr float kFloor = -1e30f;  // m before the first key (finite: -inf - m st
 
 struct DenseFwdArgs {
   const uint16_t *q, *k, *v;
-  uint16_t* o;
+  uint16_t *o, *lo;  // lo: (B, Lq, H, 64) or null
   float* lse;
   const int32_t *q_lens, *k_lens;
   int64_t qb, qh, ql, kb, kh, kl, vb, vh, vl, ob, oh, ol;  // strides in elements
@@ -93,6 +93,16 @@ __device__ inline void mask_tile(f32x16& s, int lim, int h) {
 #pragma unroll
   for (int i = 0; i < 16; ++i)
     s[i] = 8 * (i >> 2) + (i & 3) < x ? s[i] : -__builtin_inff();
+}
+
+// Two values as 16 bits, and what the rounding lost as 16 bits again (0 past the type's range).
+template <typename T16>
+__device__ inline uint32_t round_pair(float x, float y, uint32_t& lost) {
+  const uint32_t p = pack_pair<T16>(x, y);
+  const float ex = x - T16::to_f32((uint16_t)(p & 0xffff)), ey = y - T16::to_f32((uint16_t)(p >> 16));
+  lost = pack_pair<T16>(__builtin_fabsf(ex) < __builtin_inff() ? ex : 0.f,
+                        __builtin_fabsf(ey) < __builtin_inff() ? ey : 0.f);
+  return p;
 }
 
 // Keys that query i sees: [0, limit).
@@ -278,10 +288,19 @@ __global__ __launch_bounds__(256, 2) void dense_fwd_kernel(DenseFwdArgs a) {
     for (int mb = 0; mb < 2; ++mb)
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
-        const u32x2 x{pack_pair<T16>(acc[n][mb][4 * g] * inv, acc[n][mb][4 * g + 1] * inv),
-                      pack_pair<T16>(acc[n][mb][4 * g + 2] * inv, acc[n][mb][4 * g + 3] * inv)};
-        *reinterpret_cast<u32x2*>(op + i * a.ol + 32 * mb + 8 * g + 4 * h) =
-            lim[n] > 0 ? x : u32x2{0, 0};
+        u32x2 x, y;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          uint32_t lost;
+          x[e] = round_pair<T16>(acc[n][mb][4 * g + 2 * e] * inv,
+                                 acc[n][mb][4 * g + 2 * e + 1] * inv, lost);
+          y[e] = lost;
+        }
+        const int c = 32 * mb + 8 * g + 4 * h;
+        *reinterpret_cast<u32x2*>(op + i * a.ol + c) = lim[n] > 0 ? x : u32x2{0, 0};
+        if (a.lo)
+          *reinterpret_cast<u32x2*>(a.lo + (((int64_t)b * a.Lq + i) * a.H + hq) * kDD + c) =
+              lim[n] > 0 ? y : u32x2{0, 0};
       }
     if (a.lse && h == 0)
       a.lse[(int64_t)bh * a.Lq + i] =
@@ -426,41 +445,70 @@ __global__ __launch_bounds__(256, 2) void dense_fwd_split_kernel(DenseFwdArgs a)
   }
   const bool some = key_limit(oi, qlen, klen, a.causal) > 0;
   const float inv = 1.f / ll;
-  u32x4 y;
+  u32x4 y, z;
 #pragma unroll
-  for (int e = 0; e < 4; ++e)
-    y[e] = some ? pack_pair<T16>(x[2 * e] * inv, x[2 * e + 1] * inv) : 0u;
+  for (int e = 0; e < 4; ++e) {
+    uint32_t lost;
+    const uint32_t p = round_pair<T16>(x[2 * e] * inv, x[2 * e + 1] * inv, lost);
+    y[e] = some ? p : 0u;
+    z[e] = some ? lost : 0u;
+  }
   *reinterpret_cast<u32x4*>(a.o + b * a.ob + oh * a.oh + oi * a.ol + c0) = y;
+  if (a.lo)
+    *reinterpret_cast<u32x4*>(a.lo + (((int64_t)b * a.Lq + oi) * a.H + oh) * kDD + c0) = z;
   if (a.lse && c0 == 0)
     a.lse[flat] = some ? (mm - Range<T16>::shift + __log2f(ll)) * kLn2 : -__builtin_inff();
 }
 
-// Adds the key ranges of a row in order; 16 lanes per row, four channels each.
+// Joins the key ranges of a row: a workgroup's 16 groups of 16 lanes (four channels each) take
+// the ranges in turn, and their sums are added in order (the ranges come in the tens
+// where rows are few, so that one group alone would wait for one load after the other).
 template <typename T16>
 __global__ __launch_bounds__(256) void dense_join_kernel(DenseFwdArgs a) {
-  const int64_t flat = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
-  if (flat >= a.nrows) return;
-  const int c0 = (threadIdx.x & 15) * 4;
+  __shared__ float sm[16], sl[16];
+  __shared__ f32x4 sx[16][16];
+  const int64_t flat = blockIdx.x;
+  const int grp = threadIdx.x >> 4, c0 = (threadIdx.x & 15) * 4;
   const int64_t bh = flat / a.Lq;
   const int i = (int)(flat - bh * a.Lq), b = (int)(bh / a.H), hq = (int)(bh - (int64_t)b * a.H);
-  const int qlen = a.q_lens ? max(0, (int)min((int64_t)a.q_lens[b], a.Lq)) : (int)a.Lq;
-  const int klen = a.k_lens ? max(0, (int)min((int64_t)a.k_lens[b], a.Lk)) : (int)a.Lk;
-  float mm = kFloor;
-  for (int s = 0; s < a.splits; ++s) mm = fmaxf(mm, a.ml[s * a.nrows + flat].x);
-  float ll = 0.f;
+  const int qlen = seq_len(a.q_lens, b, a.Lq), klen = seq_len(a.k_lens, b, a.Lk);
+  float mm = kFloor, ll = 0.f;
   f32x4 x{0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-  for (int s = 0; s < a.splits; ++s) {
+  for (int s = grp; s < a.splits; s += 16) {
     const float2 ml = a.ml[s * a.nrows + flat];
-    const float f = fast_exp2(ml.x - mm);
-    ll += f * ml.y;
-    x += f * *reinterpret_cast<const f32x4*>(a.part + (s * a.nrows + flat) * kDD + c0);
+    const f32x4 y = *reinterpret_cast<const f32x4*>(a.part + (s * a.nrows + flat) * kDD + c0);
+    const float mn = fmaxf(mm, ml.x), f = fast_exp2(mm - mn), g = fast_exp2(ml.x - mn);
+    mm = mn;
+    ll = ll * f + g * ml.y;
+    x = x * f + g * y;
+  }
+  sx[grp][threadIdx.x & 15] = x;
+  if (c0 == 0) sm[grp] = mm, sl[grp] = ll;
+  __syncthreads();
+  if (grp) return;
+#pragma unroll
+  for (int j = 0; j < 16; ++j) mm = fmaxf(mm, sm[j]);
+  ll = 0.f;
+  x = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int j = 0; j < 16; ++j) {
+    const float f = fast_exp2(sm[j] - mm);
+    ll += f * sl[j];
+    x += f * sx[j][threadIdx.x & 15];
   }
   const bool some = key_limit(i, qlen, klen, a.causal) > 0;
   const float inv = 1.f / ll;
-  const u32x2 y{some ? pack_pair<T16>(x[0] * inv, x[1] * inv) : 0u,
-                some ? pack_pair<T16>(x[2] * inv, x[3] * inv) : 0u};
+  u32x2 y, z;
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    uint32_t lost;
+    const uint32_t p = round_pair<T16>(x[2 * e] * inv, x[2 * e + 1] * inv, lost);
+    y[e] = some ? p : 0u;
+    z[e] = some ? lost : 0u;
+  }
   *reinterpret_cast<u32x2*>(a.o + b * a.ob + hq * a.oh + i * a.ol + c0) = y;
+  if (a.lo)
+    *reinterpret_cast<u32x2*>(a.lo + (((int64_t)b * a.Lq + i) * a.H + hq) * kDD + c0) = z;
   if (a.lse && c0 == 0)
     a.lse[flat] = some ? (mm - Range<T16>::shift + __log2f(ll)) * kLn2 : -__builtin_inff();
 }
@@ -519,13 +567,14 @@ extern "C" int sla2h_dense_attn_fwd(const void* q, const void* k, const void* v,
                                     const int64_t* strides, const int32_t* q_lens,
                                     const int32_t* k_lens, int dtype, int B, int H, int Hkv,
                                     int64_t Lq, int64_t Lk, int causal, float scale,
-                                    void* workspace, void* o, float* lse, void* stream) {
+                                    void* workspace, void* o, float* lse, void* o_lo,
+                                    void* stream) {
   SLA2H_CHECK_ARG(q && k && v && strides && o);
   SLA2H_CHECK_ARG(dtype == SLA2H_DTYPE_F16 || dtype == SLA2H_DTYPE_BF16);
   SLA2H_CHECK_ARG(sizes_ok(B, H, Hkv, Lq, Lk));
   SLA2H_CHECK_ARG(scale > 0.f && scale < 1e30f);
   SLA2H_CHECK_ARG(((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)o |
-                   (uintptr_t)workspace) % 16 == 0);
+                   (uintptr_t)o_lo | (uintptr_t)workspace) % 16 == 0);
   SLA2H_CHECK_ARG(((uintptr_t)lse | (uintptr_t)q_lens | (uintptr_t)k_lens) % 4 == 0);
   for (int i = 0; i < 12; ++i) SLA2H_CHECK_ARG(strides[i] >= 0 && strides[i] % 8 == 0);
   // rows apart from each other: the range check of a tile's load tells them by their offset
@@ -540,6 +589,7 @@ extern "C" int sla2h_dense_attn_fwd(const void* q, const void* k, const void* v,
   a.k = static_cast<const uint16_t*>(k);
   a.v = static_cast<const uint16_t*>(v);
   a.o = static_cast<uint16_t*>(o);
+  a.lo = static_cast<uint16_t*>(o_lo);
   a.lse = lse;
   a.q_lens = q_lens;
   a.k_lens = k_lens;
@@ -575,7 +625,7 @@ extern "C" int sla2h_dense_attn_fwd(const void* q, const void* k, const void* v,
       dense_fwd_split_kernel<T16><<<a.nwork, 256, 0, st>>>(a);
     const int err = (int)hipGetLastError();
     if (err || p.splits == 1) return err;
-    dense_join_kernel<T16><<<(unsigned)((a.nrows + 15) / 16), 256, 0, st>>>(a);
+    dense_join_kernel<T16><<<(unsigned)a.nrows, 256, 0, st>>>(a);
     return (int)hipGetLastError();
   };
   return dtype == SLA2H_DTYPE_BF16 ? go(BF16{}) : go(F16{});

@@ -36,7 +36,7 @@ struct Shift<F16> {
 constexpr int kNormRows = 256;  // rows of a partial maximum of the norms
 
 struct DenseBwdArgs {
-  const uint16_t *q, *k, *v, *o, *dout;
+  const uint16_t *q, *k, *v, *o, *o_lo, *dout;
   const float* lse;
   uint16_t *dq, *dk, *dv;
   const int32_t *q_lens, *k_lens;
@@ -85,14 +85,20 @@ __global__ __launch_bounds__(256) void dense_bwd_prep_kernel(DenseBwdArgs a, int
       const u32x4 g = *reinterpret_cast<const u32x4*>(
           is_v ? a.v + b * a.vb + hh * a.vh + i * a.vl + c0
                : a.dout + b * a.gb + hh * a.gh + i * a.gl + c0);
-      u32x4 o{0, 0, 0, 0};
-      if (!is_v) o = *reinterpret_cast<const u32x4*>(a.o + b * a.ob + hh * a.oh + i * a.ol + c0);
+      u32x4 o{0, 0, 0, 0}, ol{0, 0, 0, 0};
+      if (!is_v) {
+        o = *reinterpret_cast<const u32x4*>(a.o + b * a.ob + hh * a.oh + i * a.ol + c0);
+        if (a.o_lo)
+          ol = *reinterpret_cast<const u32x4*>(
+              a.o_lo + (((int64_t)b * a.Lq + i) * a.H + hh) * kDD + c0);
+      }
 #pragma unroll
       for (int e = 0; e < 4; ++e)
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
           const float gv = T16::to_f32((uint16_t)(g[e] >> (16 * x)));
-          dot += gv * T16::to_f32((uint16_t)(o[e] >> (16 * x)));
+          dot += gv * (T16::to_f32((uint16_t)(o[e] >> (16 * x))) +
+                       T16::to_f32((uint16_t)(ol[e] >> (16 * x))));
           nrm += gv * gv;
         }
     }
@@ -524,7 +530,7 @@ BwdPlan bwd_plan(int dtype, int B, int H, int Hkv, int64_t Lq, int64_t Lk) {
   p.qtiles = (Lq + 128 * p.nq - 1) / (128 * p.nq);
   auto split = [](int64_t blocks, int64_t tiles) {
     if (blocks >= 256) return 1;
-    const int64_t s = (512 + blocks - 1) / blocks, most = tiles / 2;
+    const int64_t s = (512 + blocks - 1) / blocks, most = tiles / 4;
     return (int)(s < most ? s : (most < 1 ? 1 : most));
   };
   p.dq_splits = split(bh * p.qtiles, (Lk + 63) / 64);
@@ -562,7 +568,7 @@ extern "C" size_t sla2h_dense_attn_bwd_workspace_bytes(int dtype, int B, int H, 
 }
 
 extern "C" int sla2h_dense_attn_bwd(const void* q, const void* k, const void* v, const void* o,
-                                    const void* dout, const float* lse, const int64_t* strides,
+                                    const void* o_lo, const void* dout, const float* lse, const int64_t* strides,
                                     const int32_t* q_lens, const int32_t* k_lens, int dtype,
                                     int B, int H, int Hkv, int64_t Lq, int64_t Lk, int causal,
                                     float scale, void* workspace, void* dq, void* dk, void* dv,
@@ -572,7 +578,7 @@ extern "C" int sla2h_dense_attn_bwd(const void* q, const void* k, const void* v,
   SLA2H_CHECK_ARG(sizes_ok(B, H, Hkv, Lq, Lk));
   SLA2H_CHECK_ARG(scale > 0.f && scale < 1e30f);
   SLA2H_CHECK_ARG(((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)o | (uintptr_t)dout |
-                   (uintptr_t)workspace | (uintptr_t)dq | (uintptr_t)dk | (uintptr_t)dv) % 16 == 0);
+                   (uintptr_t)o_lo | (uintptr_t)workspace | (uintptr_t)dq | (uintptr_t)dk | (uintptr_t)dv) % 16 == 0);
   SLA2H_CHECK_ARG(((uintptr_t)lse | (uintptr_t)q_lens | (uintptr_t)k_lens) % 4 == 0);
   for (int i = 0; i < 24; ++i) SLA2H_CHECK_ARG(strides[i] >= 0 && strides[i] % 8 == 0);
   // rows apart from each other: the range check of a tile's load tells them by their offset
@@ -589,6 +595,7 @@ extern "C" int sla2h_dense_attn_bwd(const void* q, const void* k, const void* v,
   a.k = static_cast<const uint16_t*>(k);
   a.v = static_cast<const uint16_t*>(v);
   a.o = static_cast<const uint16_t*>(o);
+  a.o_lo = static_cast<const uint16_t*>(o_lo);
   a.dout = static_cast<const uint16_t*>(dout);
   a.lse = lse;
   a.dq = static_cast<uint16_t*>(dq);

@@ -128,15 +128,18 @@ def _no_batched(d, what):
 
 
 class _DenseAttentionFunction(torch.autograd.Function):
-    """Dense attention of (B, H, L, 64) operands on the HIP kernels; saves the operands,
-    the output and the rows' log-sum-exp, and recomputes the probabilities."""
+    """Dense attention of (b, l, H, 64) operands on the HIP kernels; saves the operands,
+    the output with what its rounding lost, and the rows' log-sum-exp, and recomputes
+    the probabilities."""
 
     @staticmethod
     def forward(ctx, q, k, v, causal, q_lens, k_lens, scale):
         from . import ops
-        o, lse = ops.dense_attn_fwd(q, k, v, causal, q_lens, k_lens, scale)
+        o, lse, o_lo = ops.dense_attn_fwd(q.transpose(1, 2), k.transpose(1, 2), v.transpose(1, 2),
+                                          causal, q_lens, k_lens, scale, with_lo=True)
+        o = o.transpose(1, 2)
         ctx.args = causal, scale
-        ctx.save_for_backward(q, k, v, o, lse, q_lens, k_lens)
+        ctx.save_for_backward(q, k, v, o, lse, o_lo, q_lens, k_lens)
         return o
 
     @staticmethod
@@ -144,10 +147,12 @@ class _DenseAttentionFunction(torch.autograd.Function):
     def backward(ctx, do):
         from . import ops
         _no_batched(do, "dense_attention")
-        q, k, v, o, lse, q_lens, k_lens = ctx.saved_tensors
+        q, k, v, o, lse, o_lo, q_lens, k_lens = ctx.saved_tensors
         causal, scale = ctx.args
-        return (*ops.dense_attn_bwd(do, q, k, v, o, lse, causal, q_lens, k_lens, scale),
-                None, None, None, None)
+        dq, dk, dv = ops.dense_attn_bwd(*(t.transpose(1, 2) for t in (do, q, k, v, o)), lse,
+                                        causal, q_lens, k_lens, scale, o_lo)
+        return (dq.transpose(1, 2), dk.transpose(1, 2), dv.transpose(1, 2), None, None, None,
+                None)
 
 
 def dense_attention(q, k, v, causal=False, q_lens=None, k_lens=None, scale=None):
@@ -165,15 +170,17 @@ def dense_attention(q, k, v, causal=False, q_lens=None, k_lens=None, scale=None)
         dt = torch.get_autocast_dtype("cuda")
         q, k, v = (t.to(dt) if t.is_floating_point() else t for t in (q, k, v))
     from . import ops
-    for t, name in ((q, "q"), (k, "k"), (v, "v")):
-        if t.dim() != 4:
-            raise ValueError(f"{name}: expected (b, l, H, 64), got {tuple(t.shape)}")
-    q, k, v = (t.transpose(1, 2) for t in (q, k, v))
-    q_lens, k_lens = (ops.attn_lens(n, q, s) for n, s in ((q_lens, "q_lens"), (k_lens, "k_lens")))
+    if not q.dim() == k.dim() == v.dim() == 4:
+        raise ValueError("q, k, v: expected (b, l, H, 64), got "
+                         f"{tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
+    if q_lens is not None:
+        q_lens = ops.attn_lens(q_lens, q, "q_lens")
+    if k_lens is not None:
+        k_lens = ops.attn_lens(k_lens, q, "k_lens")
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
-        o = _DenseAttentionFunction.apply(q, k, v, causal, q_lens, k_lens, scale)
-    else:
-        o, _ = ops.dense_attn_fwd(q, k, v, causal, q_lens, k_lens, scale, with_lse=False)
+        return _DenseAttentionFunction.apply(q, k, v, causal, q_lens, k_lens, scale)
+    o, _ = ops.dense_attn_fwd(q.transpose(1, 2), k.transpose(1, 2), v.transpose(1, 2), causal,
+                              q_lens, k_lens, scale, with_lse=False)
     return o.transpose(1, 2)
 
 

@@ -6,6 +6,7 @@ current HIP stream.  Inputs must already live on a GPU: there is no CPU path.
 """
 
 import ctypes
+import functools
 import math
 from typing import NamedTuple
 
@@ -1485,41 +1486,52 @@ def _rows16(t):
 # ---------------------------------------------------------------------------
 def _launch(dev, name, *args):
     """A library call with the tensors' device current and its current stream."""
-    fn = getattr(_lib.load(), name)
-    if dev.index is None or dev.index == torch.cuda.current_device():
-        _lib.check(fn(*args, _stream(dev)), name)
+    fn = getattr(_lib._LIB or _lib.load(), name)
+    index = dev.index
+    if index is None or index == torch._C._cuda_getDevice():
+        code = fn(*args, _stream(dev))
     else:
         with torch.cuda.device(dev):
-            _lib.check(fn(*args, _stream(dev)), name)
+            code = fn(*args, _stream(dev))
+    if code:
+        _lib.check(code, name)
 
 
 _ATTN_ROW_SPAN = 1 << 23  # row strides below it (32-bit offsets within 64 rows)
 
 
-def _attn_strides(t):
-    """(batch, head, row) strides of a (B, H, L, 64) tensor; of a size of one 0, for
-    the rows 64."""
-    return [s if n > 1 else d for n, s, d in zip(t.shape[:3], t.stride()[:3], (0, 0, E_TILE))]
+@functools.lru_cache(maxsize=512)
+def _attn_layout(shape, stride):
+    """What the kernels need of a (B, H, L, 64) operand's layout: its (batch, head, row)
+    strides (of a size of one 0, of a single row 64), or None where they do not take
+    it, and whether its memory is token-major (rows further apart than heads)."""
+    s = tuple(s if n > 1 else d for n, s, d in zip(shape, stride, (0, 0, E_TILE)))
+    ok = (stride[3] == 1 and all(x % 8 == 0 for x in s) and E_TILE <= s[2] < _ATTN_ROW_SPAN)
+    return (s if ok else None), stride[2] > stride[1]
 
 
 def _attn_operand(t):
-    """t with a unit channel stride, 16-byte aligned rows and row strides that the
-    kernels take, copied where it has not."""
-    if (t.stride(3) == 1 and t.data_ptr() % 16 == 0
-            and all(s % 8 == 0 for s in _attn_strides(t))
-            and E_TILE <= _attn_strides(t)[2] < _ATTN_ROW_SPAN):
-        return t
-    return t.clone(memory_format=torch.contiguous_format)
+    """(t, its strides, token-major): t as it is, or a copy where the kernels cannot take
+    its strides or its alignment."""
+    s, token = _attn_layout(t.shape, t.stride())
+    if s is None or t.data_ptr() % 16:
+        t = t.clone(memory_format=torch.contiguous_format)
+        s, token = _attn_layout(t.shape, t.stride())
+    return t, s, token
 
 
-def _attn_like(t, shape=None, dtype=None):
-    """Empty (B, H, L, 64), token-major in memory where t's rows are further apart
-    than its heads (a permuted (B, L, H, 64))."""
-    B, H, L, D = shape or t.shape
-    dtype = dtype or t.dtype
-    if t.stride(2) > t.stride(1):
-        return torch.empty(B, L, H, D, device=t.device, dtype=dtype).transpose(1, 2)
-    return torch.empty(B, H, L, D, device=t.device, dtype=dtype)
+def _attn_like(t, token):
+    """An empty tensor like t (B, H, L, 64) and its strides, token-major in memory for
+    `token` (a permuted (B, L, H, 64))."""
+    B, H, L, D = t.shape
+    if token:
+        e = torch.empty((B, L, H, D), device=t.device, dtype=t.dtype).transpose(1, 2)
+    else:
+        e = torch.empty((B, H, L, D), device=t.device, dtype=t.dtype)
+    return e, _attn_layout(e.shape, e.stride())[0]
+
+
+_I64x12, _I64x24 = ctypes.c_int64 * 12, ctypes.c_int64 * 24
 
 
 def attn_lens(lens, q, name):
@@ -1528,6 +1540,9 @@ def attn_lens(lens, q, name):
     if lens is None:
         return None
     lens = torch.as_tensor(lens)
+    if (lens.dtype == torch.int32 and lens.shape == q.shape[:1] and lens.device == q.device
+            and lens.is_contiguous()):
+        return lens
     if (lens.dtype.is_floating_point or lens.dtype.is_complex or lens.dtype == torch.bool
             or tuple(lens.shape) != tuple(q.shape[:1])):
         raise ValueError(f"{name}: expected {q.shape[0]} whole numbers, got "
@@ -1540,59 +1555,72 @@ def attn_lens(lens, q, name):
 def _attn_args(q, k, v, scale):
     """Checks of dense attention's operands; returns (dtype code, B, H, Hkv, Lq, Lk, scale)."""
     _need_gpu(q, k, v)
-    for t, name in ((q, "q"), (k, "k"), (v, "v")):
-        if t.dim() != 4 or t.shape[-1] != E_TILE:
-            raise ValueError(f"{name}: expected (B, H, L, 64), got {tuple(t.shape)}")
-        if t.dtype != q.dtype or t.device != q.device:
-            raise ValueError("q, k and v must share dtype and device: "
-                             f"q {q.dtype} {q.device}, {name} {t.dtype} {t.device}")
+    if not q.dtype == k.dtype == v.dtype or not q.device == k.device == v.device:
+        raise ValueError("q, k and v must share dtype and device: "
+                         f"{q.dtype} {q.device}, {k.dtype} {k.device}, {v.dtype} {v.device}")
     code = _dtype_code(q)
-    B, H, Lq, D = q.shape
-    Hkv, Lk = k.shape[1:3]
-    if k.shape != v.shape or k.shape[0] != B or (H and (Hkv == 0 or H % Hkv)):
+    qs, ks, vs = q.shape, k.shape, v.shape
+    for s, name in ((qs, "q"), (ks, "k"), (vs, "v")):
+        if len(s) != 4 or s[3] != E_TILE:
+            raise ValueError(f"{name}: expected (B, H, L, 64), got {tuple(s)}")
+    B, H, Lq, D = qs
+    Hkv, Lk = ks[1:3]
+    if ks != vs or ks[0] != B or (H and (Hkv == 0 or H % Hkv)):
         raise ValueError("k and v must share their shape, q's batch and a number of heads that "
-                         f"divides q's: {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
+                         f"divides q's: {tuple(qs)}, {tuple(ks)}, {tuple(vs)}")
     scale = D ** -0.5 if scale is None else float(scale)
     if not 0.0 < scale < 1e30:
         raise ValueError(f"scale must be positive, got {scale}")
     return code, B, H, Hkv, Lq, Lk, scale
 
 
-def _strides_arg(*ts):
-    s = [x for t in ts for x in _attn_strides(t)]
-    return (ctypes.c_int64 * len(s))(*s)
+@functools.lru_cache(maxsize=512)
+def _attn_fwd_workspace(*sizes):
+    return _lib.load().sla2h_dense_attn_fwd_workspace_bytes(*sizes)
 
 
-def dense_attn_fwd(q, k, v, causal=False, q_lens=None, k_lens=None, scale=None, with_lse=True):
+@functools.lru_cache(maxsize=512)
+def _attn_bwd_workspace(*sizes):
+    return _lib.load().sla2h_dense_attn_bwd_workspace_bytes(*sizes)
+
+
+def dense_attn_fwd(q, k, v, causal=False, q_lens=None, k_lens=None, scale=None, with_lse=True,
+                   with_lo=False):
     """Dense softmax attention of q (B, H, Lq, 64) over k, v (B, Hkv, Lk, 64), 16-bit,
     any strides with a unit channel stride -> (o in q's layout, lse (B, H, Lq) fp32
     or None).  H a multiple of Hkv; q_lens, k_lens (B,): the sequences' lengths
     (values outside [0, L] are clamped); causal: query i sees the keys
     j <= i + k_len - q_len.  Rows past a length and rows without a key are 0, their
-    lse -inf."""
+    lse -inf.  with_lo: also o_lo (B, Lq, H, 64), o's dtype, what o's rounding lost (o +
+    o_lo has about twice o's digits): the backward's row sums then do not carry it."""
     code, B, H, Hkv, Lq, Lk, scale = _attn_args(q, k, v, scale)
     dev = q.device
     q_lens, k_lens = attn_lens(q_lens, q, "q_lens"), attn_lens(k_lens, q, "k_lens")
-    q, k, v = _attn_operand(q), _attn_operand(k), _attn_operand(v)
-    o = _attn_like(q)
-    lse = torch.empty(B, H, Lq, device=dev, dtype=torch.float32) if with_lse else None
-    if o.numel() == 0 or Lk == 0:
+    (q, sq, token), (k, sk, _), (v, sv, _) = _attn_operand(q), _attn_operand(k), _attn_operand(v)
+    o, so = _attn_like(q, token)
+    lse = torch.empty((B, H, Lq), device=dev, dtype=torch.float32) if with_lse else None
+    lo = torch.empty((B, Lq, H, E_TILE), device=dev, dtype=q.dtype) if with_lo else None
+    if B * H * Lq * Lk == 0:
         o.zero_()
         if lse is not None:
             lse.fill_(float("-inf"))
-        return o, lse
-    need = _lib.load().sla2h_dense_attn_fwd_workspace_bytes(B, H, Hkv, Lq, Lk)
-    ws = _scratch(need, dev) if need else None
-    _launch(dev, "sla2h_dense_attn_fwd", q.data_ptr(), k.data_ptr(), v.data_ptr(),
-            _strides_arg(q, k, v, o), _ptr(q_lens), _ptr(k_lens), code, B, H, Hkv, Lq, Lk,
-            int(bool(causal)), scale, _ptr(ws), o.data_ptr(), _ptr(lse))
-    return o, lse
+        if lo is not None:
+            lo.zero_()
+    else:
+        need = _attn_fwd_workspace(B, H, Hkv, Lq, Lk)
+        ws = _scratch(need, dev) if need else None
+        _launch(dev, "sla2h_dense_attn_fwd", q.data_ptr(), k.data_ptr(), v.data_ptr(),
+                _I64x12(*sq, *sk, *sv, *so), _ptr(q_lens), _ptr(k_lens), code, B, H, Hkv, Lq, Lk,
+                1 if causal else 0, scale, _ptr(ws), o.data_ptr(), _ptr(lse), _ptr(lo))
+    return (o, lse, lo) if with_lo else (o, lse)
 
 
-def dense_attn_bwd(do, q, k, v, o, lse, causal=False, q_lens=None, k_lens=None, scale=None):
+def dense_attn_bwd(do, q, k, v, o, lse, causal=False, q_lens=None, k_lens=None, scale=None,
+                   o_lo=None):
     """Gradients (dq, dk, dv) of dense_attn_fwd for the output gradient do, from its
-    operands, its output o and lse (recomputed probabilities); dk and dv summed
-    over the query heads of a key head, zero behind the sequences."""
+    operands, its output o (with o_lo where it was asked for) and lse, the
+    probabilities recomputed; dk and dv summed over the query heads of a key head, zero
+    behind the sequences."""
     code, B, H, Hkv, Lq, Lk, scale = _attn_args(q, k, v, scale)
     dev = q.device
     for t, name in ((do, "do"), (o, "o")):
@@ -1602,17 +1630,24 @@ def dense_attn_bwd(do, q, k, v, o, lse, causal=False, q_lens=None, k_lens=None, 
     if tuple(lse.shape) != (B, H, Lq) or lse.dtype != torch.float32 or lse.device != dev:
         raise ValueError(f"lse: expected ({B}, {H}, {Lq}) float32 on {dev}, got "
                          f"{tuple(lse.shape)} {lse.dtype} on {lse.device}")
+    if o_lo is not None:
+        if tuple(o_lo.shape) != (B, Lq, H, E_TILE) or o_lo.dtype != q.dtype or o_lo.device != dev:
+            raise ValueError(f"o_lo: expected ({B}, {Lq}, {H}, 64) {q.dtype} on {dev}, got "
+                             f"{tuple(o_lo.shape)} {o_lo.dtype} on {o_lo.device}")
+        o_lo = aligned(o_lo.contiguous(), 16)
     q_lens, k_lens = attn_lens(q_lens, q, "q_lens"), attn_lens(k_lens, q, "k_lens")
-    q, k, v, o, do = (_attn_operand(t) for t in (q, k, v, o, do))
+    (q, sq, tq), (k, sk, tk), (v, sv, tv) = _attn_operand(q), _attn_operand(k), _attn_operand(v)
+    (o, so, _), (do, sg, _) = _attn_operand(o), _attn_operand(do)
     lse = lse.contiguous()
-    dq, dk, dv = _attn_like(q), _attn_like(k), _attn_like(v)
-    if q.numel() == 0 or k.numel() == 0:
+    (dq, s1), (dk, s2), (dv, s3) = _attn_like(q, tq), _attn_like(k, tk), _attn_like(v, tv)
+    if B * H * Lq * Lk == 0:
         return dq.zero_(), dk.zero_(), dv.zero_()
-    ws = _scratch(_lib.load().sla2h_dense_attn_bwd_workspace_bytes(code, B, H, Hkv, Lq, Lk), dev)
+    ws = _scratch(_attn_bwd_workspace(code, B, H, Hkv, Lq, Lk), dev)
     _launch(dev, "sla2h_dense_attn_bwd", q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(),
-            do.data_ptr(), lse.data_ptr(), _strides_arg(q, k, v, o, do, dq, dk, dv),
-            _ptr(q_lens), _ptr(k_lens), code, B, H, Hkv, Lq, Lk, int(bool(causal)), scale,
-            ws.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr())
+            _ptr(o_lo), do.data_ptr(), lse.data_ptr(),
+            _I64x24(*sq, *sk, *sv, *so, *sg, *s1, *s2, *s3), _ptr(q_lens), _ptr(k_lens), code, B,
+            H, Hkv, Lq, Lk, 1 if causal else 0, scale, ws.data_ptr(), dq.data_ptr(),
+            dk.data_ptr(), dv.data_ptr())
     return dq, dk, dv
 
 

@@ -852,7 +852,9 @@ int sla2h_sla2_infer_in(const void* q, const void* k, const void* v, int dtype, 
  * 0 for broadcast inputs; row strides at least 64, k's and v's below 2^23); unit channel stride, 16-byte aligned pointers.  q_lens, k_lens (B)
  * int32 on the device or NULL (all Lq / Lk); values are clamped into [0, Lq] / [0, Lk].
  * lse (B, H, Lq) fp32 contiguous or NULL.  fp32 accumulation; probabilities are rounded
- * to dtype for their product with v.  Calls with few query rows split the keys over
+ * to dtype for their product with v.  o_lo: NULL, or (B, Lq, H, 64) contiguous in dtype, what
+ * the rounding of o to dtype lost (the exact row sums of the backward are taken from o + o_lo;
+ * without it delta carries o's rounding).  Calls with few query rows split the keys over
  * workgroups and join the parts in order (a workspace of
  * sla2h_dense_attn_fwd_workspace_bytes, 0 for most calls).
  * The attn_impl of the reference's MLAAttention (models/imf_dit_video.py:323-467).
@@ -861,13 +863,14 @@ size_t sla2h_dense_attn_fwd_workspace_bytes(int B, int H, int Hkv, int64_t Lq, i
 int sla2h_dense_attn_fwd(const void* q, const void* k, const void* v, const int64_t* strides,
                          const int32_t* q_lens, const int32_t* k_lens, int dtype, int B, int H,
                          int Hkv, int64_t Lq, int64_t Lk, int causal, float scale,
-                         void* workspace, void* o, float* lse, void* stream);
+                         void* workspace, void* o, float* lse, void* o_lo, void* stream);
 
 /*
  * Its backward, the probabilities recomputed from lse:
- *   delta = rowsum(dout o), dS = P (dout v^T - delta), dq = scale dS k, dk = scale dS^T q,
+ *   delta = rowsum(dout (o + o_lo)), dS = P (dout v^T - delta), dq = scale dS k, dk = scale dS^T q,
  *   dv = P^T dout, dk and dv summed over the query heads of a key head.
- * q, k, v, lse, lens, sizes, causal and scale as in the forward, o its output, dout like o;
+ * q, k, v, lse, lens, sizes, causal and scale as in the forward, o its output (o_lo its
+ * second half or NULL), dout like o;
  * dq like q, dk and dv like k.  strides: host array of 24 int64, the (batch, head, row)
  * strides of q, k, v, o, dout, dq, dk, dv in elements (the same conditions; row strides of q, k, v and
  * dout below 2^23).  Gradients of rows behind a sequence and of rows without a key are 0; dout is
@@ -876,7 +879,7 @@ int sla2h_dense_attn_fwd(const void* q, const void* k, const void* v, const int6
 size_t sla2h_dense_attn_bwd_workspace_bytes(int dtype, int B, int H, int Hkv, int64_t Lq,
                                             int64_t Lk);
 int sla2h_dense_attn_bwd(const void* q, const void* k, const void* v, const void* o,
-                         const void* dout, const float* lse, const int64_t* strides,
+                         const void* o_lo, const void* dout, const float* lse, const int64_t* strides,
                          const int32_t* q_lens, const int32_t* k_lens, int dtype, int B, int H,
                          int Hkv, int64_t Lq, int64_t Lk, int causal, float scale,
                          void* workspace, void* dq, void* dk, void* dv, void* stream);

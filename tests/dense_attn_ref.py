@@ -4,7 +4,8 @@ rounding errors that the 16-bit kernels may make.
 With u half a unit in the last place of the operands' type (eps / 2) and t a bound for fp32
 arithmetic (products, hardware exp2 and log2, log-sum-exp, sums):
   P is rounded to 16 bits for P v:           |do| <= u |o| + (u + t) P |v|
-  delta is taken from the rounded o:         |ddelta| <= |dout| . |do| + t |dout| . P|v|
+  delta is taken from the rounded o, or, with its second half, from one that carries
+  the errors before that rounding only: |ddelta| <= |dout| . (|do| (- u |o|)) + t |dout| . P|v|
   P and dS are rounded before the products:  |ddv| <= u |dv| + (u + t) P^T |dout|
     |ddS| <= (u + t) |dS| + P (|ddelta| + t |dout| |v|^T + t |delta|)
   |ddq| <= u |dq| + scale |ddS| |k| + t scale |dS| |k|,  dk alike.
@@ -28,7 +29,8 @@ def visible(B, Lq, Lk, causal, ql, kl):
     return out
 
 
-def attention(q, k, v, causal=False, ql=None, kl=None, scale=None, do=None, dev="cpu"):
+def attention(q, k, v, causal=False, ql=None, kl=None, scale=None, do=None, dev="cpu",
+              lo=False):
     """(B, H, L, 64) operands -> dict of name -> (value, bound), float64 on dev; lse
     without a bound (-inf where no key is seen)."""
     B, H, Lq, D = q.shape
@@ -57,6 +59,7 @@ def attention(q, k, v, causal=False, ql=None, kl=None, scale=None, do=None, dev=
     delta = (g * o).sum(-1, keepdim=True)
     dP = g @ V.transpose(-1, -2)
     dS = P * (dP - delta)
+    eo = eo - u * (1 - u) * o.abs() if lo else eo
     ed = (g.abs() * eo).sum(-1, keepdim=True) + T32 * (g.abs() * PV).sum(-1, keepdim=True)
     mag = g.abs() @ V.abs().transpose(-1, -2) + delta.abs()
     eS = (u + T32) * dS.abs() + P * (ed + T32 * mag) + 2.0 ** -36 * see * mag.amax((-1, -2),

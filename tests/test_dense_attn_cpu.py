@@ -53,6 +53,8 @@ def test_types_scale_and_lengths():
             ops.dense_attn_fwd(q, q, q, k_lens=bad)
     with pytest.raises(ValueError, match="lse"):
         ops.dense_attn_bwd(q, q, q, q, q, torch.zeros(2, 2, 5))
+    with pytest.raises(ValueError, match="o_lo"):
+        ops.dense_attn_bwd(q, q, q, q, q, torch.zeros(2, 2, 4), o_lo=fake(2, 2, 4, 64))
     with pytest.raises(ValueError, match="do"):
         ops.dense_attn_bwd(fake(2, 2, 5, 64), q, q, q, q, torch.zeros(2, 2, 4))
 
@@ -63,12 +65,13 @@ def test_c_entries_check_their_arguments():
     st = lambda **kw: (ctypes.c_int64 * 24)(*[kw.get(f"s{i}", 64) for i in range(24)])
 
     def fwd(q=16, k=16, v=16, s=st(), dtype=1, B=1, H=2, Hkv=2, Lq=4, Lk=4, scale=0.125, o=16,
-            lse=4, ws=None):
+            lse=4, ws=None, lo=None):
         return lib.sla2h_dense_attn_fwd(q, k, v, s, None, None, dtype, B, H, Hkv, Lq, Lk, 0,
-                                        scale, ws, o, lse, None)
+                                        scale, ws, o, lse, lo, None)
 
-    def bwd(q=16, lse=4, s=st(), dtype=1, B=1, H=2, Hkv=2, Lq=4, Lk=4, scale=0.125, ws=16):
-        return lib.sla2h_dense_attn_bwd(q, 16, 16, 16, 16, lse, s, None, None, dtype, B, H, Hkv,
+    def bwd(q=16, lse=4, s=st(), dtype=1, B=1, H=2, Hkv=2, Lq=4, Lk=4, scale=0.125, ws=16,
+            lo=None):
+        return lib.sla2h_dense_attn_bwd(q, 16, 16, 16, lo, 16, lse, s, None, None, dtype, B, H, Hkv,
                                         Lq, Lk, 0, scale, ws, 16, 16, 16, None)
 
     for f in (fwd, bwd):
@@ -79,7 +82,7 @@ def test_c_entries_check_their_arguments():
         assert f(s=st(s1=4)) == bad and f(s=st(s4=-64)) == bad   # rows off 16 bytes, negative
         assert f(s=st(s5=1 << 23)) == bad                        # a row stride past 32-bit offsets
         assert f(s=st(s2=0)) == bad                              # rows on top of each other
-        assert f(lse=2) == bad
+        assert f(lse=2) == bad and f(lo=8) == bad
     assert bwd(lse=None) == bad and bwd(ws=None) == bad
     # few queries over many keys: the split form needs its workspace
     assert lib.sla2h_dense_attn_fwd_workspace_bytes(1, 1, 1, 1, 100_000) > 0

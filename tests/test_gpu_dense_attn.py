@@ -21,9 +21,12 @@ def inputs(seed, B, H, Hkv, Lq, Lk, dt, gain=1.5):
                                rn(B, Hkv, Lk, 64), 0.3 * rn(B, H, Lq, 64))]
 
 
-def run(q, k, v, do, **kw):
+def run(q, k, v, do, lo=True, **kw):
     from imfvideo_amd import ops
-    o, lse = ops.dense_attn_fwd(q, k, v, **kw)
+    o, lse, *o_lo = ops.dense_attn_fwd(q, k, v, with_lo=lo, **kw)
+    if lo:
+        assert torch.equal(o, ops.dense_attn_fwd(q, k, v, **kw)[0])
+        kw["o_lo"], = o_lo
     return dict(zip(("o", "lse", "dq", "dk", "dv"),
                     (o, lse, *ops.dense_attn_bwd(do, q, k, v, o, lse, **kw))))
 
@@ -60,11 +63,27 @@ def test_forward_and_gradients(shape, mask, dt):
         kl = torch.randint(0, Lk + 1, (B,), generator=g)
         ql[0], kl[B - 1] = Lq, Lk
     dev = "cuda" if H > 16 else "cpu"
-    want = R.attention(q, k, v, causal, ql, kl, do=do, dev=dev)
     c = lambda t: None if t is None else t.cuda()
-    got = run(c(q), c(k), c(v), c(do), causal=causal, q_lens=c(ql), k_lens=c(kl))
-    torch.cuda.synchronize()
-    check_all(got, want, (shape, mask, dt))
+    for lo in (True, False):
+        want = R.attention(q, k, v, causal, ql, kl, do=do, dev=dev, lo=lo)
+        got = run(c(q), c(k), c(v), c(do), lo, causal=causal, q_lens=c(ql), k_lens=c(kl))
+        torch.cuda.synchronize()
+        check_all(got, want, (shape, mask, dt, lo))
+
+
+@pytest.mark.parametrize("shape", [(1, 2, 2, 70, 90), (1, 2, 1, 3, 900), (2, 64, 64, 200, 70)])
+@pytest.mark.parametrize("dt", DTYPES)
+def test_what_the_rounding_lost(shape, dt):
+    """o + o_lo is o before its rounding, to the rounding of o_lo: within the errors of P."""
+    from imfvideo_amd import ops
+    q, k, v, _ = inputs(7, *shape, dt)
+    o, _, lo = ops.dense_attn_fwd(q.cuda(), k.cuda(), v.cuda(), with_lo=True)
+    val, tol = R.attention(q, k, v, lo=True)["o"]
+    u = torch.finfo(dt).eps / 2
+    both = o.double().cpu() + lo.transpose(1, 2).double().cpu()
+    assert ((both - val).abs() <= tol - u * (1 - u) * val.abs()).all()
+    assert (lo.transpose(1, 2).double().abs().cpu() <= u * 1.01 * o.double().abs().cpu()
+            + torch.finfo(dt).smallest_normal).all()
 
 
 @pytest.mark.parametrize("dt", DTYPES)
