@@ -17,6 +17,8 @@ import torch.nn as nn
 import torch.nn.functional as F
 from torch.autograd.function import once_differentiable
 
+from . import ops
+
 __all__ = ["RMSNorm", "SituAndMul", "SwiGLUMlp", "MLAAttention", "TransformerBlock",
            "apply_rotary_pos_emb", "precompute_axial_rope_3d", "scaled_variance_linear",
            "dense_attention", "sdpa_math_attention"]
@@ -121,7 +123,6 @@ def sdpa_math_attention(q, k, v):
 
 def _no_batched(d, what):
     """RuntimeError for gradients under vmap: the kernels take one at a time."""
-    from . import ops
     if ops.batched(d):
         raise RuntimeError(f"{what}: the backward takes one gradient at a time "
                            "(no vmap or is_grads_batched)")
@@ -134,10 +135,7 @@ class _DenseAttentionFunction(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, v, causal, q_lens, k_lens, scale):
-        from . import ops
-        o, lse, o_lo = ops.dense_attn_fwd(q.transpose(1, 2), k.transpose(1, 2), v.transpose(1, 2),
-                                          causal, q_lens, k_lens, scale, with_lo=True)
-        o = o.transpose(1, 2)
+        o, lse, o_lo = ops.dense_attn_fwd(q, k, v, causal, q_lens, k_lens, scale, True, True, True)
         ctx.args = causal, scale
         ctx.save_for_backward(q, k, v, o, lse, o_lo, q_lens, k_lens)
         return o
@@ -145,14 +143,11 @@ class _DenseAttentionFunction(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, do):
-        from . import ops
         _no_batched(do, "dense_attention")
         q, k, v, o, lse, o_lo, q_lens, k_lens = ctx.saved_tensors
         causal, scale = ctx.args
-        dq, dk, dv = ops.dense_attn_bwd(*(t.transpose(1, 2) for t in (do, q, k, v, o)), lse,
-                                        causal, q_lens, k_lens, scale, o_lo)
-        return (dq.transpose(1, 2), dk.transpose(1, 2), dv.transpose(1, 2), None, None, None,
-                None)
+        return (*ops.dense_attn_bwd(do, q, k, v, o, lse, causal, q_lens, k_lens, scale, o_lo,
+                                    True), None, None, None, None)
 
 
 def dense_attention(q, k, v, causal=False, q_lens=None, k_lens=None, scale=None):
@@ -169,19 +164,13 @@ def dense_attention(q, k, v, causal=False, q_lens=None, k_lens=None, scale=None)
     if torch.is_autocast_enabled("cuda"):
         dt = torch.get_autocast_dtype("cuda")
         q, k, v = (t.to(dt) if t.is_floating_point() else t for t in (q, k, v))
-    from . import ops
-    if not q.dim() == k.dim() == v.dim() == 4:
-        raise ValueError("q, k, v: expected (b, l, H, 64), got "
-                         f"{tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
     if q_lens is not None:
         q_lens = ops.attn_lens(q_lens, q, "q_lens")
     if k_lens is not None:
         k_lens = ops.attn_lens(k_lens, q, "k_lens")
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         return _DenseAttentionFunction.apply(q, k, v, causal, q_lens, k_lens, scale)
-    o, _ = ops.dense_attn_fwd(q.transpose(1, 2), k.transpose(1, 2), v.transpose(1, 2), causal,
-                              q_lens, k_lens, scale, with_lse=False)
-    return o.transpose(1, 2)
+    return ops.dense_attn_fwd(q, k, v, causal, q_lens, k_lens, scale, False, False, True)[0]
 
 
 class _RMSNormFunction(torch.autograd.Function):
@@ -318,7 +307,6 @@ class _Situ8Function(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, gate, up, beta, linear_beta):
-        from . import ops
         h, g8, u8 = ops.situ8_fwd(gate, up, beta, linear_beta)
         ctx.args = beta, linear_beta, g8.rows, g8.cols
         ctx.save_for_backward(g8.codes, g8.scales, u8.codes, u8.scales)
@@ -327,7 +315,6 @@ class _Situ8Function(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dh):
-        from . import ops
         _no_batched(dh, "SituAndMul(act8=True)")
         gc, gs, uc, us = ctx.saved_tensors
         beta, linear_beta, *shape = ctx.args
@@ -379,7 +366,6 @@ class SituAndMul(nn.Module):
 
 def _wgrad(dy, x, weight_dtype):
     """dY^T X for a 16-bit x in the weight's dtype, by the rule of _LinearFunction."""
-    from . import ops
     M, N = dy.shape[-1], x.shape[-1]
     if (-(-M // 128) * -(-N // 128) <= _WGRAD_MAX_TILES
             and ops.linear_wgrad_ok(x.numel() // N, M, N)):
@@ -395,7 +381,6 @@ class _Mlp8Function(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x1, x3, w1, w3, w2, beta, linear_beta):
-        from . import ops
         h1, h3, h2 = (w.to(x1.dtype) for w in (w1, w3, w2))
         h, g8, u8 = ops.situ8_fwd(F.linear(x1, h1), F.linear(x1, h3), beta, linear_beta)
         x8 = ops.act8_pack(x1)
@@ -408,7 +393,6 @@ class _Mlp8Function(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        from . import ops
         _no_batched(dy, "SwiGLUMlp(act8=True)")
         h1, h3, h2, *ts = ctx.saved_tensors
         x8, g8, u8 = (ops.Act8(*ts[2 * i:2 * i + 2], *n) for i, n in enumerate(ctx.shapes))

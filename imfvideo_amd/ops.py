@@ -1500,38 +1500,90 @@ def _launch(dev, name, *args):
 _ATTN_ROW_SPAN = 1 << 23  # row strides below it (32-bit offsets within 64 rows)
 
 
+class _AttnPlan:
+    """What dense attention's calls need of its operands' shapes and strides (q, k, v
+    (B, H, L, 64), or (B, L, H, 64) for tok)."""
+    __slots__ = ("sizes", "copy", "empty", "o_shape", "o_stride", "o_flip", "k_shape", "k_flip",
+                 "v_flip", "fwd", "bwd", "fwd_ws", "bwd_ws", "lse_shape", "lo_shape")
+
+
 @functools.lru_cache(maxsize=512)
-def _attn_layout(shape, stride):
-    """What the kernels need of a (B, H, L, 64) operand's layout: its (batch, head, row)
-    strides (of a size of one 0, of a single row 64), or None where they do not take
-    it, and whether its memory is token-major (rows further apart than heads)."""
-    s = tuple(s if n > 1 else d for n, s, d in zip(shape, stride, (0, 0, E_TILE)))
-    ok = (stride[3] == 1 and all(x % 8 == 0 for x in s) and E_TILE <= s[2] < _ATTN_ROW_SPAN)
-    return (s if ok else None), stride[2] > stride[1]
+def _attn_plan(qs, qt, ks, kt, vs, vt, dtype, tok):
+    for s, name in ((qs, "q"), (ks, "k"), (vs, "v")):
+        if len(s) != 4 or s[3] != E_TILE:
+            raise ValueError(f"{name}: expected (B, {'L, H' if tok else 'H, L'}, 64), got {tuple(s)}")
+    h, r = (2, 1) if tok else (1, 2)  # the heads' and the rows' dimension
+    B, H, Lq, Hkv, Lk = qs[0], qs[h], qs[r], ks[h], ks[r]
+    if ks != vs or ks[0] != B or (H and (Hkv == 0 or H % Hkv)):
+        raise ValueError("k and v must share their shape, q's batch and a number of heads that "
+                         f"divides q's: {tuple(qs)}, {tuple(ks)}, {tuple(vs)}")
+    p = _AttnPlan()
+    p.sizes = B, H, Hkv, Lq, Lk
+    p.empty = B * H * Lq * Lk == 0
+
+    def strides(shape, stride):
+        """(batch, head, row): of a size of one 0, of a single row 64"""
+        return [stride[i] if shape[i] > 1 else d for i, d in ((0, 0), (h, 0), (r, E_TILE))]
+
+    ins = [strides(s, t) for s, t in ((qs, qt), (ks, kt), (vs, vt))]
+    p.copy = [t[3] != 1 or any(x % 8 for x in s) or not E_TILE <= s[2] < _ATTN_ROW_SPAN
+              for s, t in zip(ins, (qt, kt, vt))]
+
+    def out(shape, stride):
+        """Layout of a tensor like this one: (strides, torch's strides, dimensions 1 and 2
+        in the other order in memory), token-major where rows are further apart than heads"""
+        token = stride[r] > stride[h] or (tok and shape[r] * shape[h] <= 1)
+        n, m = (shape[r], shape[h]) if token else (shape[h], shape[r])
+        mem = (n * m * E_TILE, m * E_TILE, E_TILE, 1)
+        flip = token != tok
+        st = (mem[0], mem[2], mem[1], 1) if flip else mem
+        return strides(shape, st), st, flip
+
+    (so, p.o_stride, p.o_flip), (sk, _, p.k_flip), (sv, _, p.v_flip) = (
+        out(s, t) for s, t in ((qs, qt), (ks, kt), (vs, vt)))
+    swap = lambda s, flip: (s[0], s[2], s[1], s[3]) if flip else tuple(s)
+    p.o_shape = swap(qs, p.o_flip)
+    p.k_shape = tuple(ks)
+    p.lse_shape, p.lo_shape = (B, H, Lq), (B, Lq, H, E_TILE)
+    p.fwd = (ctypes.c_int64 * 12)(*sum(ins, []), *so)
+    p.bwd = (ctypes.c_int64 * 24)(*sum(ins, []), *so, *so, *so, *sk, *sv)
+    p.fwd_ws = p.bwd_ws = 0
+    if not p.empty:
+        lib = _lib.load()
+        p.fwd_ws = lib.sla2h_dense_attn_fwd_workspace_bytes(*p.sizes)
+        p.bwd_ws = lib.sla2h_dense_attn_bwd_workspace_bytes(_HALF[dtype], *p.sizes)
+    return p
 
 
-def _attn_operand(t):
-    """(t, its strides, token-major): t as it is, or a copy where the kernels cannot take
-    its strides or its alignment."""
-    s, token = _attn_layout(t.shape, t.stride())
-    if s is None or t.data_ptr() % 16:
-        t = t.clone(memory_format=torch.contiguous_format)
-        s, token = _attn_layout(t.shape, t.stride())
-    return t, s, token
+_HALF = {torch.float16: 0, torch.bfloat16: 1}
 
 
-def _attn_like(t, token):
-    """An empty tensor like t (B, H, L, 64) and its strides, token-major in memory for
-    `token` (a permuted (B, L, H, 64))."""
-    B, H, L, D = t.shape
-    if token:
-        e = torch.empty((B, L, H, D), device=t.device, dtype=t.dtype).transpose(1, 2)
-    else:
-        e = torch.empty((B, H, L, D), device=t.device, dtype=t.dtype)
-    return e, _attn_layout(e.shape, e.stride())[0]
+def _attn_operands(q, k, v, scale, tok):
+    """Checks; returns q, k, v (copied where the kernels do not take their strides or
+    alignment), their plan and the scale."""
+    if not (q.is_cuda and k.is_cuda and v.is_cuda):
+        _need_gpu(q, k, v)
+    if not q.dtype == k.dtype == v.dtype or not q.device == k.device == v.device:
+        raise ValueError("q, k and v must share dtype and device: "
+                         f"{q.dtype} {q.device}, {k.dtype} {k.device}, {v.dtype} {v.device}")
+    if q.dtype not in _HALF:
+        _dtype_code(q)
+    plan = _attn_plan(q.shape, q.stride(), k.shape, k.stride(), v.shape, v.stride(), q.dtype, tok)
+    if any(plan.copy) or (q.data_ptr() | k.data_ptr() | v.data_ptr()) % 16:
+        q, k, v = (t.clone(memory_format=torch.contiguous_format) if c or t.data_ptr() % 16 else t
+                   for t, c in zip((q, k, v), plan.copy))
+        plan = _attn_plan(q.shape, q.stride(), k.shape, k.stride(), v.shape, v.stride(), q.dtype,
+                          tok)
+    if scale is None:
+        scale = E_TILE ** -0.5
+    elif not 0.0 < scale < 1e30:
+        raise ValueError(f"scale must be positive, got {scale}")
+    return q, k, v, plan, float(scale)
 
 
-_I64x12, _I64x24 = ctypes.c_int64 * 12, ctypes.c_int64 * 24
+def _attn_empty(shape, dev, dtype, flip):
+    t = torch.empty(shape, device=dev, dtype=dtype)
+    return t.transpose(1, 2) if flip else t
 
 
 def attn_lens(lens, q, name):
@@ -1552,101 +1604,80 @@ def attn_lens(lens, q, name):
     return lens.to(q.device, torch.int32).contiguous()
 
 
-def _attn_args(q, k, v, scale):
-    """Checks of dense attention's operands; returns (dtype code, B, H, Hkv, Lq, Lk, scale)."""
-    _need_gpu(q, k, v)
-    if not q.dtype == k.dtype == v.dtype or not q.device == k.device == v.device:
-        raise ValueError("q, k and v must share dtype and device: "
-                         f"{q.dtype} {q.device}, {k.dtype} {k.device}, {v.dtype} {v.device}")
-    code = _dtype_code(q)
-    qs, ks, vs = q.shape, k.shape, v.shape
-    for s, name in ((qs, "q"), (ks, "k"), (vs, "v")):
-        if len(s) != 4 or s[3] != E_TILE:
-            raise ValueError(f"{name}: expected (B, H, L, 64), got {tuple(s)}")
-    B, H, Lq, D = qs
-    Hkv, Lk = ks[1:3]
-    if ks != vs or ks[0] != B or (H and (Hkv == 0 or H % Hkv)):
-        raise ValueError("k and v must share their shape, q's batch and a number of heads that "
-                         f"divides q's: {tuple(qs)}, {tuple(ks)}, {tuple(vs)}")
-    scale = D ** -0.5 if scale is None else float(scale)
-    if not 0.0 < scale < 1e30:
-        raise ValueError(f"scale must be positive, got {scale}")
-    return code, B, H, Hkv, Lq, Lk, scale
-
-
-@functools.lru_cache(maxsize=512)
-def _attn_fwd_workspace(*sizes):
-    return _lib.load().sla2h_dense_attn_fwd_workspace_bytes(*sizes)
-
-
-@functools.lru_cache(maxsize=512)
-def _attn_bwd_workspace(*sizes):
-    return _lib.load().sla2h_dense_attn_bwd_workspace_bytes(*sizes)
-
-
 def dense_attn_fwd(q, k, v, causal=False, q_lens=None, k_lens=None, scale=None, with_lse=True,
-                   with_lo=False):
+                   with_lo=False, tok=False):
     """Dense softmax attention of q (B, H, Lq, 64) over k, v (B, Hkv, Lk, 64), 16-bit,
     any strides with a unit channel stride -> (o in q's layout, lse (B, H, Lq) fp32
-    or None).  H a multiple of Hkv; q_lens, k_lens (B,): the sequences' lengths
-    (values outside [0, L] are clamped); causal: query i sees the keys
-    j <= i + k_len - q_len.  Rows past a length and rows without a key are 0, their
+    or None); with tok all of them (B, L, H, 64).  H a multiple of Hkv; q_lens, k_lens (B,):
+    the sequences' lengths (values outside [0, L] are clamped); causal: query i sees the
+    keys j <= i + k_len - q_len.  Rows past a length and rows without a key are 0, their
     lse -inf.  with_lo: also o_lo (B, Lq, H, 64), o's dtype, what o's rounding lost (o +
     o_lo has about twice o's digits): the backward's row sums then do not carry it."""
-    code, B, H, Hkv, Lq, Lk, scale = _attn_args(q, k, v, scale)
-    dev = q.device
-    q_lens, k_lens = attn_lens(q_lens, q, "q_lens"), attn_lens(k_lens, q, "k_lens")
-    (q, sq, token), (k, sk, _), (v, sv, _) = _attn_operand(q), _attn_operand(k), _attn_operand(v)
-    o, so = _attn_like(q, token)
-    lse = torch.empty((B, H, Lq), device=dev, dtype=torch.float32) if with_lse else None
-    lo = torch.empty((B, Lq, H, E_TILE), device=dev, dtype=q.dtype) if with_lo else None
-    if B * H * Lq * Lk == 0:
+    q, k, v, p, scale = _attn_operands(q, k, v, scale, tok)
+    dev, dtype = q.device, q.dtype
+    if q_lens is not None:
+        q_lens = attn_lens(q_lens, q, "q_lens")
+    if k_lens is not None:
+        k_lens = attn_lens(k_lens, q, "k_lens")
+    o = _attn_empty(p.o_shape, dev, dtype, p.o_flip)
+    lse = torch.empty(p.lse_shape, device=dev, dtype=torch.float32) if with_lse else None
+    lo = torch.empty(p.lo_shape, device=dev, dtype=dtype) if with_lo else None
+    if p.empty:
         o.zero_()
         if lse is not None:
             lse.fill_(float("-inf"))
         if lo is not None:
             lo.zero_()
     else:
-        need = _attn_fwd_workspace(B, H, Hkv, Lq, Lk)
-        ws = _scratch(need, dev) if need else None
-        _launch(dev, "sla2h_dense_attn_fwd", q.data_ptr(), k.data_ptr(), v.data_ptr(),
-                _I64x12(*sq, *sk, *sv, *so), _ptr(q_lens), _ptr(k_lens), code, B, H, Hkv, Lq, Lk,
-                1 if causal else 0, scale, _ptr(ws), o.data_ptr(), _ptr(lse), _ptr(lo))
+        ws = _scratch(p.fwd_ws, dev) if p.fwd_ws else None
+        _launch(dev, "sla2h_dense_attn_fwd", q.data_ptr(), k.data_ptr(), v.data_ptr(), p.fwd,
+                _ptr(q_lens), _ptr(k_lens), _HALF[dtype], *p.sizes, 1 if causal else 0, scale,
+                _ptr(ws), o.data_ptr(), _ptr(lse), _ptr(lo))
     return (o, lse, lo) if with_lo else (o, lse)
 
 
 def dense_attn_bwd(do, q, k, v, o, lse, causal=False, q_lens=None, k_lens=None, scale=None,
-                   o_lo=None):
+                   o_lo=None, tok=False):
     """Gradients (dq, dk, dv) of dense_attn_fwd for the output gradient do, from its
     operands, its output o (with o_lo where it was asked for) and lse, the
     probabilities recomputed; dk and dv summed over the query heads of a key head, zero
     behind the sequences."""
-    code, B, H, Hkv, Lq, Lk, scale = _attn_args(q, k, v, scale)
-    dev = q.device
-    for t, name in ((do, "do"), (o, "o")):
-        if t.shape != q.shape or t.dtype != q.dtype or t.device != dev:
-            raise ValueError(f"{name}: expected {tuple(q.shape)} {q.dtype} on {dev}, got "
+    q, k, v, p, scale = _attn_operands(q, k, v, scale, tok)
+    dev, dtype = q.device, q.dtype
+
+    def like_q(t, name):
+        if t.shape != q.shape or t.dtype != dtype or t.device != dev:
+            raise ValueError(f"{name}: expected {tuple(q.shape)} {dtype} on {dev}, got "
                              f"{tuple(t.shape)} {t.dtype} on {t.device}")
-    if tuple(lse.shape) != (B, H, Lq) or lse.dtype != torch.float32 or lse.device != dev:
-        raise ValueError(f"lse: expected ({B}, {H}, {Lq}) float32 on {dev}, got "
+        if t.stride() != p.o_stride or t.data_ptr() % 16:
+            t = _attn_empty(p.o_shape, dev, dtype, p.o_flip).copy_(t)
+        return t
+
+    do, o = like_q(do, "do"), like_q(o, "o")
+    if lse.shape != p.lse_shape or lse.dtype != torch.float32 or lse.device != dev:
+        raise ValueError(f"lse: expected {p.lse_shape} float32 on {dev}, got "
                          f"{tuple(lse.shape)} {lse.dtype} on {lse.device}")
+    lse = lse.contiguous()
     if o_lo is not None:
-        if tuple(o_lo.shape) != (B, Lq, H, E_TILE) or o_lo.dtype != q.dtype or o_lo.device != dev:
-            raise ValueError(f"o_lo: expected ({B}, {Lq}, {H}, 64) {q.dtype} on {dev}, got "
+        if o_lo.shape != p.lo_shape or o_lo.dtype != dtype or o_lo.device != dev:
+            raise ValueError(f"o_lo: expected {p.lo_shape} {dtype} on {dev}, got "
                              f"{tuple(o_lo.shape)} {o_lo.dtype} on {o_lo.device}")
         o_lo = aligned(o_lo.contiguous(), 16)
-    q_lens, k_lens = attn_lens(q_lens, q, "q_lens"), attn_lens(k_lens, q, "k_lens")
-    (q, sq, tq), (k, sk, tk), (v, sv, tv) = _attn_operand(q), _attn_operand(k), _attn_operand(v)
-    (o, so, _), (do, sg, _) = _attn_operand(o), _attn_operand(do)
-    lse = lse.contiguous()
-    (dq, s1), (dk, s2), (dv, s3) = _attn_like(q, tq), _attn_like(k, tk), _attn_like(v, tv)
-    if B * H * Lq * Lk == 0:
+    if q_lens is not None:
+        q_lens = attn_lens(q_lens, q, "q_lens")
+    if k_lens is not None:
+        k_lens = attn_lens(k_lens, q, "k_lens")
+    dq = _attn_empty(p.o_shape, dev, dtype, p.o_flip)
+    ks = p.k_shape
+    kf = (ks[0], ks[2], ks[1], ks[3])
+    dk = _attn_empty(kf if p.k_flip else ks, dev, dtype, p.k_flip)
+    dv = _attn_empty(kf if p.v_flip else ks, dev, dtype, p.v_flip)
+    if p.empty:
         return dq.zero_(), dk.zero_(), dv.zero_()
-    ws = _scratch(_attn_bwd_workspace(code, B, H, Hkv, Lq, Lk), dev)
+    ws = _scratch(p.bwd_ws, dev)
     _launch(dev, "sla2h_dense_attn_bwd", q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(),
-            _ptr(o_lo), do.data_ptr(), lse.data_ptr(),
-            _I64x24(*sq, *sk, *sv, *so, *sg, *s1, *s2, *s3), _ptr(q_lens), _ptr(k_lens), code, B,
-            H, Hkv, Lq, Lk, 1 if causal else 0, scale, ws.data_ptr(), dq.data_ptr(),
+            _ptr(o_lo), do.data_ptr(), lse.data_ptr(), p.bwd, _ptr(q_lens), _ptr(k_lens),
+            _HALF[dtype], *p.sizes, 1 if causal else 0, scale, ws.data_ptr(), dq.data_ptr(),
             dk.data_ptr(), dv.data_ptr())
     return dq, dk, dv
 
