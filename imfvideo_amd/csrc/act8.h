@@ -42,15 +42,16 @@ __device__ inline uint32_t abs_max2(uint32_t a, uint32_t b) {
   return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(x, y));
 }
 
-// Scale of a tile from each lane's packed magnitudes.
+// Largest magnitude of a wave's lanes (infinity for a NaN too), and the scale of a tile.
 template <typename T16>
-__device__ inline float tile_scale(uint32_t top2) {
+__device__ inline float wave_top_of(uint32_t top2) {
   constexpr uint32_t kInf = T16::kDtype == SLA2H_DTYPE_BF16 ? 0x7f80u : 0x7c00u;
   const uint32_t a = top2 & 0xffffu, b = top2 >> 16;
   const uint32_t m = a > b ? a : b;
-  const float f = wave_max(m >= kInf ? __builtin_inff() : T16::to_f32((uint16_t)m));
-  if (f == __builtin_inff()) return __builtin_nanf("");
-  return f / 127.0f + 1e-12f;
+  return wave_max(m >= kInf ? __builtin_inff() : T16::to_f32((uint16_t)m));
+}
+__device__ inline float scale_of_top(float top) {
+  return top == __builtin_inff() ? __builtin_nanf("") : top / 127.0f + 1e-12f;
 }
 
 // Codes of four elements, packed.  r = fl(1 / s): the product with r is within an ulp of

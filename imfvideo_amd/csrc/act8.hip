@@ -5,9 +5,8 @@
 //   situ(g) = beta tanh(g / beta) sigmoid(g),  sat(u) = lb tanh(u / lb) (u for lb = 0)
 //   dg = dh sat(u) situ'(g),  du = dh situ(g) sat'(u)   at the restored g and u.
 //
-// HBM-bound by design (8 bytes per element each way for the gate, against 10 with 16-bit
-// gate and up in the backward): one wave per 64 x 64 tile, so a tile's scale needs no exchange
-// through LDS, and all of a wave's loads (8 or 16 KB) are in flight before it computes.
+// HBM-bound by design: 8 bytes per element each way for the gate (10 with 16-bit gate and
+// up in the backward).
 //
 // With a = e^(-2|x|), tanh|x| = (1 - a) / (1 + a) and sech^2 x = 4 a / (1 + a)^2: one exp
 // gives both without the cancellation of 1 - tanh^2; 1 - a itself cancels for small |x|, where
@@ -18,76 +17,98 @@ namespace sla2h {
 
 namespace {
 
+// Workgroup = one tile, 16 elements of each operand per thread: thread t holds rows
+// t / 8 and 32 + t / 8, columns 8 (t % 8) .. + 7, so a wave's access covers eight rows of 128
+// bytes and its codes 512 bytes in a row.  (A wave per tile needs no exchange for the scale, but four
+// times the registers, which left two waves per SIMD, and four times the latency of a small
+// call: 274 x 1,365 forward 21 us against 9.)
 struct Tile {
-  int64_t row;  // of this lane's first group of eight
+  int64_t row;  // of this thread's first group of eight
   int c;        // its column
   int64_t id;   // tile number
 };
 
-// Wave w of the grid takes tile w; lane l holds row 8 i + l / 8, columns 8 (l % 8) .. + 7.
-__device__ inline bool my_tile(int64_t ntile, int cb, Tile& t) {
-  t.id = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  if (t.id >= ntile) return false;
-  const int l = threadIdx.x & 63;
+__device__ inline Tile my_tile(int cb) {
+  Tile t;
+  t.id = blockIdx.x;
   const int64_t rt = t.id / cb;
-  t.row = rt * kAct + (l >> 3);
-  t.c = (int)(t.id - rt * cb) * kAct + (l & 7) * 8;
-  return true;
+  t.row = rt * kAct + (threadIdx.x >> 3);
+  t.c = (int)(t.id - rt * cb) * kAct + (threadIdx.x & 7) * 8;
+  return t;
 }
 
-template <typename T16>
 __device__ inline void load_tile(const uint16_t* x, int64_t ld, int64_t rows, int F, const Tile& t,
-                                 u32x4 (&v)[8]) {
+                                 u32x4 (&v)[2]) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int64_t r = t.row + 8 * i;
+  for (int i = 0; i < 2; ++i) {
+    const int64_t r = t.row + 32 * i;
     v[i] = r < rows ? load_row8(x + r * ld, t.c, F) : u32x4{0, 0, 0, 0};
   }
 }
 
 template <typename T16>
-__device__ inline void pack_tile(const u32x4 (&v)[8], const Tile& t, int8_t* codes,
-                                 float* scales) {
+__device__ inline uint32_t top_of(const u32x4 (&v)[2]) {
   uint32_t top = 0;
 #pragma unroll
-  for (int i = 0; i < 8; ++i)
+  for (int i = 0; i < 2; ++i)
 #pragma unroll
     for (int e = 0; e < 4; ++e) top = abs_max2(top, v[i][e]);
-  const float s = tile_scale<T16>(top), r = 1.0f / s;
-  const int l = threadIdx.x & 63;
-  u32x2* dst = reinterpret_cast<u32x2*>(codes + t.id * kActBytes) + l;
+  return top;
+}
+
+// Scales of N operands' tiles (one barrier).
+template <typename T16, int N>
+__device__ inline void tile_scales(const u32x4 (*const (&v)[N])[2], float (&s)[N]) {
+  __shared__ float wave_top[N][4];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) dst[64 * i] = codes8<T16>(v[i], s, r);
-  if (l == 0) scales[t.id] = s;
+  for (int n = 0; n < N; ++n) {
+    const float f = wave_top_of<T16>(top_of<T16>(*v[n]));
+    if ((threadIdx.x & 63) == 0) wave_top[n][threadIdx.x >> 6] = f;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int n = 0; n < N; ++n) {
+    const float* w = wave_top[n];
+    s[n] = scale_of_top(fmaxf(fmaxf(w[0], w[1]), fmaxf(w[2], w[3])));
+  }
+}
+
+template <typename T16>
+__device__ inline void store_codes(const u32x4 (&v)[2], float s, const Tile& t, int8_t* codes,
+                                   float* scales) {
+  const float r = 1.0f / s;
+  u32x2* dst = reinterpret_cast<u32x2*>(codes + t.id * kActBytes) + threadIdx.x;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) dst[256 * i] = codes8<T16>(v[i], s, r);
+  if (threadIdx.x == 0) scales[t.id] = s;
 }
 
 template <typename T16>
 __global__ __launch_bounds__(256) void act8_pack_kernel(const uint16_t* __restrict__ x, int64_t ld,
-                                                        int64_t rows, int F, int cb, int64_t ntile,
+                                                        int64_t rows, int F, int cb,
                                                         int8_t* __restrict__ codes,
                                                         float* __restrict__ scales) {
-  Tile t;
-  if (!my_tile(ntile, cb, t)) return;
-  u32x4 v[8];
-  load_tile<T16>(x, ld, rows, F, t, v);
-  pack_tile<T16>(v, t, codes, scales);
+  const Tile t = my_tile(cb);
+  u32x4 v[2];
+  load_tile(x, ld, rows, F, t, v);
+  float s[1];
+  tile_scales<T16, 1>({&v}, s);
+  store_codes<T16>(v, s[0], t, codes, scales);
 }
 
 template <typename T16>
 __global__ __launch_bounds__(256) void act8_unpack_kernel(const int8_t* __restrict__ codes,
                                                           const float* __restrict__ scales,
                                                           int64_t rows, int F, int cb,
-                                                          int64_t ntile,
                                                           uint16_t* __restrict__ x) {
-  Tile t;
-  if (!my_tile(ntile, cb, t)) return;
+  const Tile t = my_tile(cb);
   const float s = scales[t.id];
-  const u32x2* src = reinterpret_cast<const u32x2*>(codes + t.id * kActBytes) + (threadIdx.x & 63);
+  const u32x2* src = reinterpret_cast<const u32x2*>(codes + t.id * kActBytes) + threadIdx.x;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int64_t r = t.row + 8 * i;
+  for (int i = 0; i < 2; ++i) {
+    const int64_t r = t.row + 32 * i;
     float y[8];
-    values8(src[64 * i], s, y);
+    values8(src[256 * i], s, y);
     if (r < rows)
       store_row8(x + r * F, t.c, F,
                  u32x4{pack_pair<T16>(y[0], y[1]), pack_pair<T16>(y[2], y[3]),
@@ -151,16 +172,14 @@ __device__ inline void gate_bwd(float dh, float g, float u, const Gate& p, float
 template <typename T16, bool SAT>
 __global__ __launch_bounds__(256) void situ8_fwd_kernel(
     const uint16_t* __restrict__ G, const uint16_t* __restrict__ U, int64_t sg, int64_t su,
-    int64_t rows, int F, int cb, int64_t ntile, Gate p, uint16_t* __restrict__ H,
-    int8_t* __restrict__ gc, float* __restrict__ gs, int8_t* __restrict__ uc,
-    float* __restrict__ us) {
-  Tile t;
-  if (!my_tile(ntile, cb, t)) return;
-  u32x4 g[8], u[8];
-  load_tile<T16>(G, sg, rows, F, t, g);
-  load_tile<T16>(U, su, rows, F, t, u);
+    int64_t rows, int F, int cb, Gate p, uint16_t* __restrict__ H, int8_t* __restrict__ gc,
+    float* __restrict__ gs, int8_t* __restrict__ uc, float* __restrict__ us) {
+  const Tile t = my_tile(cb);
+  u32x4 g[2], u[2];
+  load_tile(G, sg, rows, F, t, g);
+  load_tile(U, su, rows, F, t, u);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
+  for (int i = 0; i < 2; ++i) {
     u32x4 y;
 #pragma unroll
     for (int e = 0; e < 4; ++e)
@@ -168,35 +187,35 @@ __global__ __launch_bounds__(256) void situ8_fwd_kernel(
                                           T16::to_f32((uint16_t)(u[i][e] & 0xffff)), p),
                             gate_fwd<SAT>(T16::to_f32((uint16_t)(g[i][e] >> 16)),
                                           T16::to_f32((uint16_t)(u[i][e] >> 16)), p));
-    const int64_t r = t.row + 8 * i;
+    const int64_t r = t.row + 32 * i;
     if (r < rows) store_row8(H + r * F, t.c, F, y);
   }
-  pack_tile<T16>(g, t, gc, gs);
-  pack_tile<T16>(u, t, uc, us);
+  float s[2];
+  tile_scales<T16, 2>({&g, &u}, s);
+  store_codes<T16>(g, s[0], t, gc, gs);
+  store_codes<T16>(u, s[1], t, uc, us);
 }
 
 template <typename T16, bool SAT, bool WITH_H>
 __global__ __launch_bounds__(256) void situ8_bwd_kernel(
     const uint16_t* __restrict__ DH, int64_t sd, const int8_t* __restrict__ gc,
     const float* __restrict__ gs, const int8_t* __restrict__ uc, const float* __restrict__ us,
-    int64_t rows, int F, int cb, int64_t ntile, Gate p, int64_t so, uint16_t* __restrict__ DG,
+    int64_t rows, int F, int cb, Gate p, int64_t so, uint16_t* __restrict__ DG,
     uint16_t* __restrict__ DU, uint16_t* __restrict__ H) {
-  Tile t;
-  if (!my_tile(ntile, cb, t)) return;
-  const int l = threadIdx.x & 63;
-  const u32x2* gp = reinterpret_cast<const u32x2*>(gc + t.id * kActBytes) + l;
-  const u32x2* up = reinterpret_cast<const u32x2*>(uc + t.id * kActBytes) + l;
-  u32x4 dh[8];
-  u32x2 g8[8], u8[8];
+  const Tile t = my_tile(cb);
+  const u32x2* gp = reinterpret_cast<const u32x2*>(gc + t.id * kActBytes) + threadIdx.x;
+  const u32x2* up = reinterpret_cast<const u32x2*>(uc + t.id * kActBytes) + threadIdx.x;
+  u32x4 dh[2];
+  u32x2 g8[2], u8[2];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    g8[i] = gp[64 * i];
-    u8[i] = up[64 * i];
+  for (int i = 0; i < 2; ++i) {
+    g8[i] = gp[256 * i];
+    u8[i] = up[256 * i];
   }
-  load_tile<T16>(DH, sd, rows, F, t, dh);
+  load_tile(DH, sd, rows, F, t, dh);
   const float s1 = gs[t.id], s2 = us[t.id];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
+  for (int i = 0; i < 2; ++i) {
     float g[8], u[8], dg[8], du[8], h[8];
     values8(g8[i], s1, g);
     values8(u8[i], s2, u);
@@ -204,7 +223,7 @@ __global__ __launch_bounds__(256) void situ8_bwd_kernel(
     for (int e = 0; e < 8; ++e)
       gate_bwd<SAT>(T16::to_f32((uint16_t)(dh[i][e >> 1] >> (16 * (e & 1)))), g[e], u[e], p,
                     dg[e], du[e], h[e]);
-    const int64_t r = t.row + 8 * i;
+    const int64_t r = t.row + 32 * i;
     if (r >= rows) continue;
     auto put = [&](uint16_t* y, const float (&x)[8]) {
       store_row8(y + r * so, t.c, F,
@@ -221,9 +240,8 @@ bool plan(int64_t rows, int F, int& cb, int64_t& ntile, unsigned& grid) {
   if (rows <= 0 || F <= 0) return false;
   cb = (F + kAct - 1) / kAct;
   ntile = (rows + kAct - 1) / kAct * cb;
-  const int64_t g = (ntile + 3) / 4;
-  grid = (unsigned)g;
-  return g < ((int64_t)1 << 31);
+  grid = (unsigned)ntile;
+  return ntile < ((int64_t)1 << 31);
 }
 
 bool code_ok(const void* c, const void* s) { return c && s && (uintptr_t)c % 16 == 0 && (uintptr_t)s % 4 == 0; }
@@ -246,9 +264,9 @@ extern "C" int sla2h_act8_pack(const void* x, int64_t ld, int dtype, int64_t row
   hipStream_t st = static_cast<hipStream_t>(stream);
   const uint16_t* xp = static_cast<const uint16_t*>(x);
   if (dtype == SLA2H_DTYPE_BF16)
-    act8_pack_kernel<BF16><<<grid, 256, 0, st>>>(xp, ld, rows, F, cb, nt, codes, scales);
+    act8_pack_kernel<BF16><<<grid, 256, 0, st>>>(xp, ld, rows, F, cb, codes, scales);
   else
-    act8_pack_kernel<F16><<<grid, 256, 0, st>>>(xp, ld, rows, F, cb, nt, codes, scales);
+    act8_pack_kernel<F16><<<grid, 256, 0, st>>>(xp, ld, rows, F, cb, codes, scales);
   return (int)hipGetLastError();
 }
 
@@ -262,9 +280,9 @@ extern "C" int sla2h_act8_unpack(const int8_t* codes, const float* scales, int d
   hipStream_t st = static_cast<hipStream_t>(stream);
   uint16_t* xp = static_cast<uint16_t*>(x);
   if (dtype == SLA2H_DTYPE_BF16)
-    act8_unpack_kernel<BF16><<<grid, 256, 0, st>>>(codes, scales, rows, F, cb, nt, xp);
+    act8_unpack_kernel<BF16><<<grid, 256, 0, st>>>(codes, scales, rows, F, cb, xp);
   else
-    act8_unpack_kernel<F16><<<grid, 256, 0, st>>>(codes, scales, rows, F, cb, nt, xp);
+    act8_unpack_kernel<F16><<<grid, 256, 0, st>>>(codes, scales, rows, F, cb, xp);
   return (int)hipGetLastError();
 }
 
@@ -289,7 +307,7 @@ extern "C" int sla2h_situ8_fwd(const void* gate, const void* up, int dtype, int6
     using T16 = decltype(tag);
     situ8_fwd_kernel<T16, decltype(sat)::value><<<grid, 256, 0, st>>>(
         static_cast<const uint16_t*>(gate), static_cast<const uint16_t*>(up), sg, su, rows, F, cb,
-        nt, p, static_cast<uint16_t*>(h), gate_codes, gate_scales, up_codes, up_scales);
+        p, static_cast<uint16_t*>(h), gate_codes, gate_scales, up_codes, up_scales);
     return (int)hipGetLastError();
   };
   if (dtype == SLA2H_DTYPE_BF16)
@@ -315,7 +333,7 @@ extern "C" int sla2h_situ8_bwd(const void* dh, int64_t sd, const int8_t* gate_co
     using T16 = decltype(tag);
     situ8_bwd_kernel<T16, decltype(sat)::value, decltype(wh)::value><<<grid, 256, 0, st>>>(
         static_cast<const uint16_t*>(dh), sd, gate_codes, gate_scales, up_codes, up_scales, rows,
-        F, cb, nt, p, so, static_cast<uint16_t*>(dgate), static_cast<uint16_t*>(dup),
+        F, cb, p, so, static_cast<uint16_t*>(dgate), static_cast<uint16_t*>(dup),
         static_cast<uint16_t*>(h));
     return (int)hipGetLastError();
   };

@@ -138,6 +138,41 @@ __device__ inline int seq_len(const int32_t* lens, int b, int64_t L) {
   return n < 0 ? 0 : (n > L ? (int)L : n);
 }
 
-constexpr int kNoLimit = 0x7fffffff;
+// Which head and tile a workgroup takes.  Workgroups go to the eight XCDs in turn, each with
+// an L2 of its own.
+//   even tiles (no mask, no lengths): an XCD takes a run of neighbouring tiles, so that those of
+//     a head share the streamed operand in its L2;
+//   uneven ones: heads in turn over the XCDs (a multiple of eight heads: each XCD keeps its own),
+//     tile by tile, the longest first where the mask orders them (`last`): runs of
+//     neighbours would leave the XCDs of short sequences idle.
+//     B = 3, H = 8 over 2, L = 4,159, causal, clips of 4,159, 2,703 and 1,247: see the kernels.
+struct WorkMap {
+  int heads, tiles;  // tiles of a head
+  int n;             // heads * tiles
+  int even, last;
+};
+inline WorkMap work_map(int64_t heads, int64_t tiles, bool even, bool last) {
+  return WorkMap{(int)heads, (int)tiles, (int)(heads * tiles), even, last};
+}
+inline unsigned work_grid(const WorkMap& m) { return m.even ? 8u * ((m.n + 7) / 8) : (unsigned)m.n; }
+__device__ inline bool work_item(const WorkMap& m, int& head, int& tile) {
+  const int blk = blockIdx.x;
+  if (m.even) {
+    const int i = (blk & 7) * ((m.n + 7) / 8) + (blk >> 3);
+    if (i >= m.n) return false;
+    head = i / m.tiles;
+    tile = i - head * m.tiles;
+  } else if (m.heads % 8 == 0) {
+    const int per = m.heads / 8, i = blk >> 3;
+    tile = i / per;
+    head = (blk & 7) + 8 * (i - tile * per);
+  } else {
+    tile = blk / m.heads;
+    head = blk - tile * m.heads;
+  }
+  head = __builtin_amdgcn_readfirstlane(head);
+  tile = __builtin_amdgcn_readfirstlane(m.last ? m.tiles - 1 - tile : tile);
+  return true;
+}
 
 }  // namespace sla2h

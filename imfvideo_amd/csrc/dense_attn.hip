@@ -42,8 +42,8 @@ struct DenseFwdArgs {
   int H, Hkv, rep;
   int causal;
   float c;  // scale * log2(e)
-  int qtiles;  // query tiles of a head
-  int nwork, per_xcd;
+  WorkMap map;
+  int qtiles, nwork;  // split form: query tiles of a key head, workgroups
   // split form
   float* part;   // [split][B * H * Lq][64] unnormalised sums
   float2* ml;    // [split][B * H * Lq] (m, l)
@@ -122,12 +122,8 @@ template <typename T16, int NQ>
 __global__ __launch_bounds__(256, 2) void dense_fwd_kernel(DenseFwdArgs a) {
   __shared__ __align__(16) unsigned char k0[kTileB], k1[kTileB], k2[kTileB], k3[kTileB];
   __shared__ __align__(16) unsigned char v0[kTileB], v1[kTileB], v2[kTileB], v3[kTileB];
-  const int logical = (blockIdx.x & 7) * a.per_xcd + (blockIdx.x >> 3);
-  if (logical >= a.nwork) return;
-  const int bh = __builtin_amdgcn_readfirstlane(logical / a.qtiles);
-  // causal: the longest rows first
-  int qt = __builtin_amdgcn_readfirstlane(logical - bh * a.qtiles);
-  if (a.causal) qt = a.qtiles - 1 - qt;
+  int bh, qt;
+  if (!work_item(a.map, bh, qt)) return;
   const int b = bh / a.H, hq = bh - b * a.H, hk = hq / a.rep;
   const int tid = threadIdx.x, l = tid & 63, h = l >> 5;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -521,16 +517,23 @@ struct FwdPlan {
   int64_t units;
 };
 
-FwdPlan fwd_plan(int B, int H, int Hkv, int64_t Lq, int64_t Lk) {
+// even: neither causal nor lengths
+FwdPlan fwd_plan(int B, int H, int Hkv, int64_t Lq, int64_t Lk, bool even) {
   FwdPlan p{};
   const int64_t bh = (int64_t)B * H;
-  for (int nq = 2; nq >= 1; --nq) {
-    p.nq = nq;
-    p.qtiles = (Lq + 128 * nq - 1) / (128 * nq);
-    p.nwork = bh * p.qtiles;
-    p.splits = 1;
-    if (p.nwork >= 256) return p;
-  }
+  p.splits = 1;
+  p.qtiles = (Lq + 255) / 256;
+  p.nwork = bh * p.qtiles;
+  // 64 rows per wave read each operand from LDS half as often, 32 rows make twice as many
+  // workgroups.  us, 256 against 128 rows per workgroup: even tiles B = 1, H = 8, L = 29,952
+  // (936 workgroups) 1,784 : 2,027, L = 8,192 (256) 153 : 154; causal L = 29,952 889 : 951, L = 8,192
+  // 143 : 100; B = 3, L = 4,159 (408) 111 : 83.
+  p.nq = 2;
+  if (p.nwork >= (even ? 256 : 768)) return p;
+  p.nq = 1;
+  p.qtiles = (Lq + 127) / 128;
+  p.nwork = bh * p.qtiles;
+  if (p.nwork >= 256) return p;
   p.nq = 0;
   p.qtiles = ((H / Hkv) * Lq + 31) / 32;
   const int64_t blocks = (int64_t)B * Hkv * p.qtiles, units = (Lk + 31) / 32;
@@ -559,7 +562,7 @@ using namespace sla2h;
 extern "C" size_t sla2h_dense_attn_fwd_workspace_bytes(int B, int H, int Hkv, int64_t Lq,
                                                        int64_t Lk) {
   if (!sizes_ok(B, H, Hkv, Lq, Lk)) return 0;
-  const FwdPlan p = fwd_plan(B, H, Hkv, Lq, Lk);
+  const FwdPlan p = fwd_plan(B, H, Hkv, Lq, Lk, true);  // the split form does not depend on it
   return p.splits > 1 ? (size_t)p.splits * B * H * Lq * (kDD * 4 + 8) : 0;
 }
 
@@ -581,7 +584,8 @@ extern "C" int sla2h_dense_attn_fwd(const void* q, const void* k, const void* v,
   for (int i : {2, 5, 8, 11}) SLA2H_CHECK_ARG(strides[i] >= kDD);
   // 32-bit byte offsets within a tile of 64 rows
   SLA2H_CHECK_ARG(strides[5] < ((int64_t)1 << 23) && strides[8] < ((int64_t)1 << 23));
-  const FwdPlan p = fwd_plan(B, H, Hkv, Lq, Lk);
+  const bool even = !causal && !q_lens && !k_lens;
+  const FwdPlan p = fwd_plan(B, H, Hkv, Lq, Lk, even);
   SLA2H_CHECK_ARG(p.splits == 1 || workspace);
   SLA2H_CHECK_ARG(p.nwork < ((int64_t)1 << 30));
   DenseFwdArgs a{};
@@ -606,7 +610,7 @@ extern "C" int sla2h_dense_attn_fwd(const void* q, const void* k, const void* v,
   a.c = scale * kLog2e;
   a.qtiles = (int)p.qtiles;
   a.nwork = (int)p.nwork;
-  a.per_xcd = (int)((p.nwork + 7) / 8);
+  a.map = work_map((int64_t)B * H, p.qtiles, even, causal);
   a.splits = p.splits;
   a.units = (int)p.units;
   a.nrows = (int64_t)B * H * Lq;
@@ -618,9 +622,9 @@ extern "C" int sla2h_dense_attn_fwd(const void* q, const void* k, const void* v,
   auto go = [&](auto tag) -> int {
     using T16 = decltype(tag);
     if (p.nq == 2)
-      dense_fwd_kernel<T16, 2><<<8 * a.per_xcd, 256, 0, st>>>(a);
+      dense_fwd_kernel<T16, 2><<<work_grid(a.map), 256, 0, st>>>(a);
     else if (p.nq == 1)
-      dense_fwd_kernel<T16, 1><<<8 * a.per_xcd, 256, 0, st>>>(a);
+      dense_fwd_kernel<T16, 1><<<work_grid(a.map), 256, 0, st>>>(a);
     else
       dense_fwd_split_kernel<T16><<<a.nwork, 256, 0, st>>>(a);
     const int err = (int)hipGetLastError();

@@ -49,10 +49,8 @@ struct DenseBwdArgs {
   float *nlse, *ndelta;  // (B, H, Lq): -(lse log2e - shift) / c and -delta
   float *gmax, *vmax;    // (B, H, nqb), (B, Hkv, nkb): largest row norms (fp16)
   int nqb, nkb;
-  // dq
-  int qtiles, dq_splits, dq_nwork, dq_per_xcd;
-  // dk, dv
-  int ktiles, kv_splits, kv_nwork, kv_per_xcd;
+  WorkMap dq_map, kv_map;  // tiles x splits of a query head, of a key head
+  int dq_splits, kv_splits;
   float* part;
 };
 
@@ -172,14 +170,9 @@ template <typename T16, int NQ>
 __global__ __launch_bounds__(256, 2) void dense_bwd_dq_kernel(DenseBwdArgs a) {
   __shared__ __align__(16) unsigned char k0[kTileB], k1[kTileB], k2[kTileB];
   __shared__ __align__(16) unsigned char v0[kTileB], v1[kTileB], v2[kTileB];
-  const int logical = (blockIdx.x & 7) * a.dq_per_xcd + (blockIdx.x >> 3);
-  if (logical >= a.dq_nwork) return;
-  const int per_bh = a.qtiles * a.dq_splits;
-  const int bh = __builtin_amdgcn_readfirstlane(logical / per_bh);
-  const int rest = __builtin_amdgcn_readfirstlane(logical - bh * per_bh);
-  int qt = rest / a.dq_splits;
-  const int sp = rest - qt * a.dq_splits;
-  if (a.causal) qt = a.qtiles - 1 - qt;
+  int bh, item;
+  if (!work_item(a.dq_map, bh, item)) return;
+  const int qt = item / a.dq_splits, sp = item - qt * a.dq_splits;
   const int b = bh / a.H, hq = bh - b * a.H, hk = hq / a.rep;
   const int tid = threadIdx.x, l = tid & 63, h = l >> 5;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -330,12 +323,9 @@ __global__ __launch_bounds__(256, NK == 1 ? 2 : 1) void dense_bwd_dkdv_kernel(De
   __shared__ __align__(16) unsigned char q0_[kTileB], q1_[kTileB], q2_[kTileB];
   __shared__ __align__(16) unsigned char g0_[kTileB], g1_[kTileB], g2_[kTileB];
   __shared__ __align__(16) float s0_[2][64], s1_[2][64], s2_[2][64];
-  const int logical = (blockIdx.x & 7) * a.kv_per_xcd + (blockIdx.x >> 3);
-  if (logical >= a.kv_nwork) return;
-  const int per_bk = a.ktiles * a.kv_splits;
-  const int bk = __builtin_amdgcn_readfirstlane(logical / per_bk);
-  const int rest = __builtin_amdgcn_readfirstlane(logical - bk * per_bk);
-  const int ktile = rest / a.kv_splits, sp = rest - ktile * a.kv_splits;
+  int bk, item;
+  if (!work_item(a.kv_map, bk, item)) return;
+  const int ktile = item / a.kv_splits, sp = item - ktile * a.kv_splits;
   const int b = bk / a.Hkv, hk = bk - b * a.Hkv;
   const int tid = threadIdx.x, l = tid & 63, h = l >> 5;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -523,14 +513,17 @@ struct BwdPlan {
   size_t stats, parts;  // floats
 };
 
-BwdPlan bwd_plan(int dtype, int B, int H, int Hkv, int64_t Lq, int64_t Lk) {
+// even: neither causal nor lengths.  Workgroups of uneven length balance by number: the
+// rules of the forward, and twice the ranges.
+BwdPlan bwd_plan(int dtype, int B, int H, int Hkv, int64_t Lq, int64_t Lk, bool even) {
   BwdPlan p{};
   const int64_t bh = (int64_t)B * H, bk = (int64_t)B * Hkv, rep = H / Hkv;
-  p.nq = bh * ((Lq + 255) / 256) >= 256 ? 2 : 1;
+  p.nq = bh * ((Lq + 255) / 256) >= (even ? 256 : 768) ? 2 : 1;
   p.qtiles = (Lq + 128 * p.nq - 1) / (128 * p.nq);
-  auto split = [](int64_t blocks, int64_t tiles) {
-    if (blocks >= 256) return 1;
-    const int64_t s = (512 + blocks - 1) / blocks, most = tiles / 4;
+  auto split = [&](int64_t blocks, int64_t tiles) {
+    const int64_t want = even ? 512 : 1024;
+    if (blocks >= want / 2) return 1;
+    const int64_t s = (want + blocks - 1) / blocks, most = tiles / 4;
     return (int)(s < most ? s : (most < 1 ? 1 : most));
   };
   p.dq_splits = split(bh * p.qtiles, (Lk + 63) / 64);
@@ -563,8 +556,12 @@ using namespace sla2h;
 extern "C" size_t sla2h_dense_attn_bwd_workspace_bytes(int dtype, int B, int H, int Hkv,
                                                        int64_t Lq, int64_t Lk) {
   if (!sizes_ok(B, H, Hkv, Lq, Lk)) return 0;
-  const BwdPlan p = bwd_plan(dtype, B, H, Hkv, Lq, Lk);
-  return (p.stats + p.parts) * 4;
+  size_t most = 0;
+  for (bool even : {false, true}) {
+    const BwdPlan p = bwd_plan(dtype, B, H, Hkv, Lq, Lk, even);
+    most = p.parts > most ? p.parts : most;
+  }
+  return (bwd_plan(dtype, B, H, Hkv, Lq, Lk, true).stats + most) * 4;
 }
 
 extern "C" int sla2h_dense_attn_bwd(const void* q, const void* k, const void* v, const void* o,
@@ -585,7 +582,8 @@ extern "C" int sla2h_dense_attn_bwd(const void* q, const void* k, const void* v,
   for (int i : {2, 5, 8, 11, 14, 17, 20, 23}) SLA2H_CHECK_ARG(strides[i] >= kDD);
   // 32-bit byte offsets within a tile of 64 rows
   for (int i : {2, 5, 8, 14}) SLA2H_CHECK_ARG(strides[i] < ((int64_t)1 << 23));
-  const BwdPlan p = bwd_plan(dtype, B, H, Hkv, Lq, Lk);
+  const bool even = !causal && !q_lens && !k_lens;
+  const BwdPlan p = bwd_plan(dtype, B, H, Hkv, Lq, Lk, even);
   SLA2H_CHECK_ARG(p.dq_nwork < ((int64_t)1 << 30) && p.kv_nwork < ((int64_t)1 << 30));
   const int64_t bh = (int64_t)B * H, bk = (int64_t)B * Hkv;
   const int64_t pq = bh * p.nqb, pv = dtype == SLA2H_DTYPE_F16 ? bk * p.nkb : 0;
@@ -625,14 +623,10 @@ extern "C" int sla2h_dense_attn_bwd(const void* q, const void* k, const void* v,
   a.nqb = (int)p.nqb;
   a.nkb = (int)p.nkb;
   a.part = a.nlse + p.stats;
-  a.qtiles = (int)p.qtiles;
+  a.dq_map = work_map(bh, p.qtiles * p.dq_splits, even, causal);
+  a.kv_map = work_map(bk, p.ktiles * p.kv_splits, even, false);  // causal: the first keys' are longest
   a.dq_splits = p.dq_splits;
-  a.dq_nwork = (int)p.dq_nwork;
-  a.dq_per_xcd = (int)((p.dq_nwork + 7) / 8);
-  a.ktiles = (int)p.ktiles;
   a.kv_splits = p.kv_splits;
-  a.kv_nwork = (int)p.kv_nwork;
-  a.kv_per_xcd = (int)((p.kv_nwork + 7) / 8);
   hipStream_t st = static_cast<hipStream_t>(stream);
   auto go = [&](auto tag) -> int {
     using T16 = decltype(tag);
@@ -640,16 +634,16 @@ extern "C" int sla2h_dense_attn_bwd(const void* q, const void* k, const void* v,
     dense_bwd_prep_kernel<T16><<<(unsigned)(pq + pv), 256, 0, st>>>(a, pq);
     if ((err = (int)hipGetLastError())) return err;
     if (p.nq == 2)
-      dense_bwd_dq_kernel<T16, 2><<<8 * a.dq_per_xcd, 256, 0, st>>>(a);
+      dense_bwd_dq_kernel<T16, 2><<<work_grid(a.dq_map), 256, 0, st>>>(a);
     else
-      dense_bwd_dq_kernel<T16, 1><<<8 * a.dq_per_xcd, 256, 0, st>>>(a);
+      dense_bwd_dq_kernel<T16, 1><<<work_grid(a.dq_map), 256, 0, st>>>(a);
     if ((err = (int)hipGetLastError())) return err;
     if (p.dq_splits > 1) {
       dense_bwd_join_kernel<T16, kDD><<<(unsigned)((bh * Lq * kDD / 4 + 255) / 256), 256, 0, st>>>(
           a.part, p.dq_splits, bh * Lq, Lq, H, a.dq, a.dqb, a.dqh, a.dql, nullptr, 0, 0, 0);
       if ((err = (int)hipGetLastError())) return err;
     }
-    dense_bwd_dkdv_kernel<T16, 1><<<8 * a.kv_per_xcd, 256, 0, st>>>(a);
+    dense_bwd_dkdv_kernel<T16, 1><<<work_grid(a.kv_map), 256, 0, st>>>(a);
     if ((err = (int)hipGetLastError()) || p.kv_splits == 1) return err;
     dense_bwd_join_kernel<T16, 2 * kDD>
         <<<(unsigned)((bk * Lk * 2 * kDD / 4 + 255) / 256), 256, 0, st>>>(
