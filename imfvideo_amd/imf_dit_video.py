@@ -307,19 +307,16 @@ class _Situ8Function(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, gate, up, beta, linear_beta):
-        h, g8, u8 = ops.situ8_fwd(gate, up, beta, linear_beta)
-        ctx.args = beta, linear_beta, g8.rows, g8.cols
-        ctx.save_for_backward(g8.codes, g8.scales, u8.codes, u8.scales)
+        h, kept, *shape = ops.situ8_save(gate, up, beta, linear_beta)
+        ctx.args = *shape, beta, linear_beta
+        ctx.save_for_backward(kept)
         return h
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dh):
         _no_batched(dh, "SituAndMul(act8=True)")
-        gc, gs, uc, us = ctx.saved_tensors
-        beta, linear_beta, *shape = ctx.args
-        return (*ops.situ8_bwd(dh, ops.Act8(gc, gs, *shape), ops.Act8(uc, us, *shape), beta,
-                               linear_beta), None, None)
+        return (*ops.situ8_saved_bwd(dh, *ctx.saved_tensors, *ctx.args), None, None)
 
 
 class SituAndMul(nn.Module):
@@ -382,23 +379,22 @@ class _Mlp8Function(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x1, x3, w1, w3, w2, beta, linear_beta):
         h1, h3, h2 = (w.to(x1.dtype) for w in (w1, w3, w2))
-        h, g8, u8 = ops.situ8_fwd(F.linear(x1, h1), F.linear(x1, h3), beta, linear_beta)
-        x8 = ops.act8_pack(x1)
-        ctx.args = beta, linear_beta
-        ctx.shapes = [(a.rows, a.cols) for a in (x8, g8, u8)]
+        h, kept, *shape = ops.situ8_save(F.linear(x1, h1), F.linear(x1, h3), beta, linear_beta)
+        codes, scales, *ctx.x_shape = ops.act8_pack(x1)
+        ctx.args = *shape, beta, linear_beta
         ctx.dtypes = [w.dtype for w in (w1, w3, w2)]
-        ctx.save_for_backward(h1, h3, h2, *(t for a in (x8, g8, u8) for t in a[:2]))
+        ctx.save_for_backward(h1, h3, h2, codes, scales, kept)
         return F.linear(h, h2)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
         _no_batched(dy, "SwiGLUMlp(act8=True)")
-        h1, h3, h2, *ts = ctx.saved_tensors
-        x8, g8, u8 = (ops.Act8(*ts[2 * i:2 * i + 2], *n) for i, n in enumerate(ctx.shapes))
+        h1, h3, h2, codes, scales, kept = ctx.saved_tensors
+        x8 = ops.Act8(codes, scales, *ctx.x_shape)
         n1, n3, nw1, nw3, nw2 = ctx.needs_input_grad[:5]
         d1, d3, d2 = ctx.dtypes
-        dg, du, *h = ops.situ8_bwd(dy @ h2, g8, u8, *ctx.args, with_h=nw2)
+        dg, du, *h = ops.situ8_saved_bwd(dy @ h2, kept, *ctx.args, with_h=nw2)
         return (dg @ h1 if n1 else None, du @ h3 if n3 else None,
                 ops.linear_wgrad8(dg, x8).to(d1) if nw1 else None,
                 ops.linear_wgrad8(du, x8).to(d3) if nw3 else None,

@@ -1741,10 +1741,17 @@ def _gate_args(beta, linear_beta):
     return beta, lb
 
 
-def situ8_fwd(gate, up, beta, linear_beta=None):
-    """situ_mul_fwd that also keeps gate and up in 8 bits -> (h, gate Act8, up Act8).
-    h is computed from the 16-bit inputs."""
-    _need_gpu(gate, up)
+def _situ8_bytes(rows, cols):
+    """(bytes of one operand's codes, of its scales) in a buffer of gate | up codes, scales"""
+    n = -(-rows // E_TILE) * -(-cols // E_TILE)
+    return n * E_TILE * E_TILE, n * 4
+
+
+def situ8_save(gate, up, beta, linear_beta=None):
+    """situ8_fwd with both Act8 in one buffer (for a backward's saved tensors): (h, buffer,
+    rows, cols)."""
+    if not (gate.is_cuda and up.is_cuda):
+        _need_gpu(gate, up)
     if gate.shape != up.shape or gate.dtype != up.dtype or gate.device != up.device:
         raise ValueError("situ8: gate and up must share shape, dtype and device")
     code = _dtype_code(gate)
@@ -1753,34 +1760,66 @@ def situ8_fwd(gate, up, beta, linear_beta=None):
         raise ValueError(f"situ8: nothing to compute in {tuple(gate.shape)}")
     g2, F, sg = _rows_view(gate)
     u2, _, su = _rows_view(up)
-    dev = gate.device
+    rows, dev = g2.shape[0], gate.device
+    nc, ns = _situ8_bytes(rows, F)
     h = torch.empty(gate.shape, device=dev, dtype=gate.dtype)
-    g8, u8 = _act8_empty(g2.shape[0], F, dev), _act8_empty(g2.shape[0], F, dev)
-    _launch(dev, "sla2h_situ8_fwd", g2.data_ptr(), u2.data_ptr(), code, g8.rows, F, sg, su, beta,
-            lb, h.data_ptr(), g8.codes.data_ptr(), g8.scales.data_ptr(), u8.codes.data_ptr(),
-            u8.scales.data_ptr())
-    return h, g8, u8
+    buf = _scratch(2 * (nc + ns), dev)
+    p = buf.data_ptr()
+    _launch(dev, "sla2h_situ8_fwd", g2.data_ptr(), u2.data_ptr(), code, rows, F, sg, su, beta,
+            lb, h.data_ptr(), p, p + 2 * nc, p + nc, p + 2 * nc + ns)
+    return h, buf, rows, F
+
+
+def _situ8_views(buf, rows, cols):
+    nc, ns = _situ8_bytes(rows, cols)
+    rb, cb = -(-rows // E_TILE), -(-cols // E_TILE)
+    codes = buf[:2 * nc].view(torch.int8).view(2, rb, cb, E_TILE, E_TILE)
+    scales = buf[2 * nc:].view(torch.float32).view(2, rb, cb)
+    return Act8(codes[0], scales[0], rows, cols), Act8(codes[1], scales[1], rows, cols)
+
+
+def situ8_fwd(gate, up, beta, linear_beta=None):
+    """situ_mul_fwd that also keeps gate and up in 8 bits -> (h, gate Act8, up Act8).
+    h is computed from the 16-bit inputs."""
+    h, *kept = situ8_save(gate, up, beta, linear_beta)
+    return (h, *_situ8_views(*kept))
+
+
+def _situ8_bwd(dh, g, u, rows, cols, dev, beta, linear_beta, with_h):
+    """g, u: (codes, scales) addresses on dev"""
+    if not dh.is_cuda:
+        _need_gpu(dh)
+    code = _dtype_code(dh)
+    beta, lb = _gate_args(beta, linear_beta)
+    if dh.shape[-1:] != (cols,) or dh.numel() != rows * cols or dh.device != dev:
+        raise ValueError(f"situ8_bwd: dh {tuple(dh.shape)} on {dh.device} does not fit "
+                         f"{rows} x {cols} on {dev}")
+    d2, F, sd = _rows_view(dh)
+    out = [torch.empty(dh.shape, device=dev, dtype=dh.dtype) for _ in range(2 + with_h)]
+    _launch(dev, "sla2h_situ8_bwd", d2.data_ptr(), sd, *g, *u, code, rows, F, beta, lb, F,
+            out[0].data_ptr(), out[1].data_ptr(), out[2].data_ptr() if with_h else None)
+    return tuple(out)
+
+
+def situ8_saved_bwd(dh, buf, rows, cols, beta, linear_beta=None, with_h=False):
+    """situ8_bwd from situ8_save's buffer."""
+    nc, ns = _situ8_bytes(rows, cols)
+    p = buf.data_ptr()
+    return _situ8_bwd(dh, (p, p + 2 * nc), (p + nc, p + 2 * nc + ns), rows, cols, buf.device, beta,
+                      linear_beta, with_h)
 
 
 def situ8_bwd(dh, g8, u8, beta, linear_beta=None, with_h=False):
     """Gradients (dgate, dup) of situ8_fwd for dh (..., cols) at the kept values, in dh's
     dtype and shape; with_h also h of the kept values (the next layer's input again)."""
-    _need_gpu(dh)
-    code = _dtype_code(dh)
-    beta, lb = _gate_args(beta, linear_beta)
     _act8_check(g8, "situ8_bwd gate")
     _act8_check(u8, "situ8_bwd up")
-    if (g8.rows, g8.cols) != (u8.rows, u8.cols) or dh.shape[-1:] != (g8.cols,) or (
-            dh.numel() != g8.rows * g8.cols) or not dh.device == g8.codes.device == u8.codes.device:
-        raise ValueError(f"situ8_bwd: dh {tuple(dh.shape)} on {dh.device} does not fit "
-                         f"{g8.rows} x {g8.cols} and {u8.rows} x {u8.cols} on {g8.codes.device}")
-    d2, F, sd = _rows_view(dh)
-    out = [torch.empty(dh.shape, device=dh.device, dtype=dh.dtype) for _ in range(2 + with_h)]
-    _launch(dh.device, "sla2h_situ8_bwd", d2.data_ptr(), sd, g8.codes.data_ptr(),
-            g8.scales.data_ptr(), u8.codes.data_ptr(), u8.scales.data_ptr(), code, g8.rows, F,
-            beta, lb, F, out[0].data_ptr(), out[1].data_ptr(),
-            out[2].data_ptr() if with_h else None)
-    return tuple(out)
+    if (g8.rows, g8.cols) != (u8.rows, u8.cols) or g8.codes.device != u8.codes.device:
+        raise ValueError(f"situ8_bwd: gate {g8.rows} x {g8.cols} on {g8.codes.device} does not fit "
+                         f"up {u8.rows} x {u8.cols} on {u8.codes.device}")
+    return _situ8_bwd(dh, (g8.codes.data_ptr(), g8.scales.data_ptr()),
+                      (u8.codes.data_ptr(), u8.scales.data_ptr()), g8.rows, g8.cols,
+                      g8.codes.device, beta, linear_beta, with_h)
 
 
 def linear_wgrad8(dy, a):

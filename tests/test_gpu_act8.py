@@ -226,7 +226,7 @@ def test_module_keeps_8_bits_and_its_gradients():
     kept = []
     with torch.autograd.graph.saved_tensors_hooks(lambda t: kept.append(t) or t, lambda t: t):
         h = m(x)
-    assert [t.dtype for t in kept] == [torch.int8, torch.float32] * 2
+    assert sum(t.nbytes for t in kept) == 2 * (2 * 2 * 4096 + 2 * 2 * 4)  # two tiles by two, twice
     g, = torch.autograd.grad(h, x, dh)
     h2, g8, u8 = ops.situ8_fwd(x[..., :96].detach(), x[..., 96:].detach(), 4.0, 25.0)
     assert torch.equal(h, h2)
