@@ -30,6 +30,7 @@ template <>
 struct Range<F16> {
   static constexpr float shift = 9.f, most = 32768.f;
 };
+constexpr int kFineKeys = 512;
 constexpr float kFloor = -1e30f;  // m before the first key (finite: -inf - m stays -inf)
 
 struct DenseFwdArgs {
@@ -87,6 +88,23 @@ __device__ inline float probabilities(const f32x16& s, float c, float m, u32x4 (
   return (r[0] + r[1]) + (r[2] + r[3]);
 }
 
+// What the rounding of a tile's probabilities lost, packed alike.
+template <typename T16>
+__device__ inline void lost_halves(const f32x16& s, float c, float m, const u32x4 (&p)[2],
+                                   u32x4 (&q)[2]) {
+  const float off = Range<T16>::shift - m;
+#pragma unroll
+  for (int t = 0; t < 2; ++t)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int k = 8 * t + 2 * i;
+      const uint32_t w = p[t][i];
+      q[t][i] = pack_pair<T16>(
+          fast_exp2(__builtin_fmaf(s[k], c, off)) - T16::to_f32((uint16_t)(w & 0xffff)),
+          fast_exp2(__builtin_fmaf(s[k + 1], c, off)) - T16::to_f32((uint16_t)(w >> 16)));
+    }
+}
+
 // scores of keys at or past a lane's limit -> -inf; lim counts from the tile's first key
 __device__ inline void mask_tile(f32x16& s, int lim, int h) {
   const int x = lim - 4 * h;
@@ -118,7 +136,12 @@ __device__ inline int key_limit(int i, int qlen, int klen, int causal) {
 // The step of 32 keys is software-pipelined: its scores were computed one step earlier, so
 // that the score products of the next step, which depend on nothing here, run on the matrix
 // cores under this step's exponentials; operands of the step after are read from LDS meanwhile.
-template <typename T16, int NQ>
+// FINE: waves whose rows see at most kFineKeys keys add what the rounding of P lost with a
+// second product.  delta = dO . O of the backward inherits that rounding, and dS = P (dP - delta)
+// shows it where few keys share a row (77 keys: dq and dk 2.6e-3 off against 2.4e-3, of which the
+// roundings of dS and of the result are 2.4e-3); over long rows it averages out.  Without
+// gradients the same, so that both calls give the same output.
+template <typename T16, int NQ, bool FINE>
 __global__ __launch_bounds__(256, 2) void dense_fwd_kernel(DenseFwdArgs a) {
   __shared__ __align__(16) unsigned char k0[kTileB], k1[kTileB], k2[kTileB], k3[kTileB];
   __shared__ __align__(16) unsigned char v0[kTileB], v1[kTileB], v2[kTileB], v3[kTileB];
@@ -240,6 +263,19 @@ __global__ __launch_bounds__(256, 2) void dense_fwd_kernel(DenseFwdArgs a) {
 #pragma unroll
         for (int n = 0; n < NQ; ++n)
           acc[n][mb] = mfma_32x32x16<T16>(vf[s][mb], p[n][s], acc[n][mb]);
+    if (FINE && wany <= kFineKeys) {
+      asm volatile("");
+#pragma unroll
+      for (int n = 0; n < NQ; ++n) {
+        u32x4 q[2];
+        lost_halves<T16>(sc[kb][n], a.c, m[n], p[n], q);
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+          for (int mb = 0; mb < 2; ++mb)
+            acc[n][mb] = mfma_32x32x16<T16>(vf[s][mb], q[s], acc[n][mb]);
+      }
+    }
   };
   // Tile t lives in slot t % 4; tiles past the last one are empty (zeros).  At the top of
   // tile t the tiles up to t + 1 have landed and tile t - 1 is read.
@@ -375,11 +411,17 @@ __global__ __launch_bounds__(256, 2) void dense_fwd_split_kernel(DenseFwdArgs a)
       r = probabilities<T16>(sc, a.c, m, p);
     }
     lsum += r;
+    u32x4 q[2];
+    const bool fine = kmax <= kFineKeys;
+    if (fine) lost_halves<T16>(sc, a.c, m, p, q);
 #pragma unroll
     for (int s = 0; s < 2; ++s)
 #pragma unroll
-      for (int mb = 0; mb < 2; ++mb)
-        acc[mb] = mfma_32x32x16<T16>(col_frag(kv + kUnitB, 16 * s, mb, lo), p[s], acc[mb]);
+      for (int mb = 0; mb < 2; ++mb) {
+        const u32x4 vf = col_frag(kv + kUnitB, 16 * s, mb, lo);
+        acc[mb] = mfma_32x32x16<T16>(vf, p[s], acc[mb]);
+        if (fine) acc[mb] = mfma_32x32x16<T16>(vf, q[s], acc[mb]);
+      }
   };
   int64_t u = u0 + w;
   load_unit(u, kv0[w]);
@@ -621,10 +663,16 @@ extern "C" int sla2h_dense_attn_fwd(const void* q, const void* k, const void* v,
   hipStream_t st = static_cast<hipStream_t>(stream);
   auto go = [&](auto tag) -> int {
     using T16 = decltype(tag);
-    if (p.nq == 2)
-      dense_fwd_kernel<T16, 2><<<work_grid(a.map), 256, 0, st>>>(a);
+    const unsigned grid = work_grid(a.map);
+    const bool fine = Lk <= kFineKeys || causal;
+    if (p.nq == 2 && fine)
+      dense_fwd_kernel<T16, 2, true><<<grid, 256, 0, st>>>(a);
+    else if (p.nq == 2)
+      dense_fwd_kernel<T16, 2, false><<<grid, 256, 0, st>>>(a);
+    else if (p.nq == 1 && fine)
+      dense_fwd_kernel<T16, 1, true><<<grid, 256, 0, st>>>(a);
     else if (p.nq == 1)
-      dense_fwd_kernel<T16, 1><<<work_grid(a.map), 256, 0, st>>>(a);
+      dense_fwd_kernel<T16, 1, false><<<grid, 256, 0, st>>>(a);
     else
       dense_fwd_split_kernel<T16><<<a.nwork, 256, 0, st>>>(a);
     const int err = (int)hipGetLastError();
