@@ -315,14 +315,16 @@ __global__ __launch_bounds__(256, 2) void dense_bwd_dq_kernel(DenseBwdArgs a) {
   }
 }
 
-// dk, dv: workgroup = 4 waves x (32 NK) keys of one key head; the query rows of the heads
-// that read it are streamed through LDS in tiles of 64 with their -lse and -delta,
-// which start the accumulators of S and dP.
-template <typename T16, int NK>
-__global__ __launch_bounds__(256, NK == 1 ? 2 : 1) void dense_bwd_dkdv_kernel(DenseBwdArgs a) {
-  __shared__ __align__(16) unsigned char q0_[kTileB], q1_[kTileB], q2_[kTileB];
-  __shared__ __align__(16) unsigned char g0_[kTileB], g1_[kTileB], g2_[kTileB];
-  __shared__ __align__(16) float s0_[2][64], s1_[2][64], s2_[2][64];
+// dk, dv: workgroup = 4 waves x 32 keys of one key head; the query rows of the heads that
+// read it are streamed through LDS in tiles of 64, three tiles ahead into four slots, with
+// their -lse and -delta, which start the accumulators of S and dP.  The step of 32 rows is
+// software-pipelined as in the forward: S and dP of the next step run on the matrix cores
+// under this step's exponentials.
+template <typename T16, bool CAUSAL>
+__global__ __launch_bounds__(256, 2) void dense_bwd_dkdv_kernel(DenseBwdArgs a) {
+  __shared__ __align__(16) unsigned char q0_[kTileB], q1_[kTileB], q2_[kTileB], q3_[kTileB];
+  __shared__ __align__(16) unsigned char g0_[kTileB], g1_[kTileB], g2_[kTileB], g3_[kTileB];
+  __shared__ __align__(16) float s0_[2][64], s1_[2][64], s2_[2][64], s3_[2][64];
   int bk, item;
   if (!work_item(a.kv_map, bk, item)) return;
   const int ktile = item / a.kv_splits, sp = item - ktile * a.kv_splits;
@@ -332,26 +334,28 @@ __global__ __launch_bounds__(256, NK == 1 ? 2 : 1) void dense_bwd_dkdv_kernel(De
   const LaneOff lo(l);
   const int qlen = seq_len(a.q_lens, b, a.Lq), klen = seq_len(a.k_lens, b, a.Lk);
 
-  const int key0 = ktile * (128 * NK), kw = key0 + w * (32 * NK);
+  const int key0 = ktile * 128, kw = key0 + w * 32;
   // first query that sees a key of the workgroup (causal: i >= j - off)
   const int off = klen - qlen;
   int first = first_query(qlen, klen, a.causal);
-  if (a.causal) first = max(first, key0 - off);
+  if (CAUSAL) first = max(first, key0 - off);
   const int nq = key0 < klen && first < qlen ? (qlen - first + kTileRows - 1) / kTileRows : 0;
   const int total = nq * a.rep;  // (head, query tile) pairs
   const int per = (total + a.kv_splits - 1) / a.kv_splits;
   const int u0 = sp * per, u1 = min(total, u0 + per);
 
   const int64_t qld = a.ql * 2, gld = a.gl * 2;
-  auto load_tile = [&](int u, unsigned char* qt, unsigned char* gt, float (*st)[64]) __attribute__((always_inline)) {
-    const int r = u < u1 ? u / nq : 0;
-    const int hq = hk * a.rep + r;
-    const int row = first + (u - r * nq) * kTileRows;
-    const int64_t n = u < u1 ? (int64_t)qlen - row : 0;
-    const auto rq = rows_rsrc(a.q + b * a.qb + hq * a.qh, row, n, qld);
-    const auto rg = rows_rsrc(a.dout + b * a.gb + hq * a.gh, row, n, gld);
+  // the tile to load next, and the one to compute (their head of the group and first row)
+  int lu = u0, lh = u0 < u1 ? u0 / nq : 0;
+  int lrow = first + (u0 < u1 ? u0 - lh * nq : 0) * kTileRows, crow = lrow;
+  auto load_tile = [&](unsigned char* qt, unsigned char* gt, float (*st)[64])
+      __attribute__((always_inline)) {
+    const int hq = hk * a.rep + lh;
+    const int64_t n = lu < u1 ? (int64_t)qlen - lrow : 0;
+    const auto rq = rows_rsrc(a.q + b * a.qb + hq * a.qh, lrow, n, qld);
+    const auto rg = rows_rsrc(a.dout + b * a.gb + hq * a.gh, lrow, n, gld);
     const float* stat = (w & 1) ? a.ndelta : a.nlse;
-    const auto rs = make_rsrc(stat + ((int64_t)b * a.H + hq) * a.Lq + row,
+    const auto rs = make_rsrc(stat + ((int64_t)b * a.H + hq) * a.Lq + lrow,
                               n <= 0 ? 0 : (n < 64 ? n : 64) * 4);
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
@@ -361,125 +365,122 @@ __global__ __launch_bounds__(256, NK == 1 ? 2 : 1) void dense_bwd_dkdv_kernel(De
     // waves 0 and 2 bring -lse, 1 and 3 -delta (the same values twice)
     __builtin_amdgcn_raw_ptr_buffer_load_lds(
         rs, (__attribute__((address_space(3))) void*)&st[w & 1][0], 4, 4 * l, 0, 0, 0);
+    ++lu;
+    lrow += kTileRows;
+    if (lrow >= qlen && lu < u1) lrow = first, ++lh;
   };
 
   float mul = 1.f;
   if (Shift<T16>::scaled) mul = ds_scale(a, b, hk);
-  u32x4 kf[NK][4], vf[NK][4];
-#pragma unroll
-  for (int n = 0; n < NK; ++n) {
-    const int j = kw + 32 * n + (l & 31);
+  u32x4 kf[4], vf[4];
+  {
+    const int j = kw + (l & 31);
+    const bool live = j < klen;
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
-      const bool live = j < klen;
-      kf[n][s] = live ? *reinterpret_cast<const u32x4*>(a.k + b * a.kb + hk * a.kh + j * a.kl +
-                                                        16 * s + 8 * h)
-                      : u32x4{0, 0, 0, 0};
-      vf[n][s] = live ? *reinterpret_cast<const u32x4*>(a.v + b * a.vb + hk * a.vh + j * a.vl +
-                                                        16 * s + 8 * h)
-                      : u32x4{0, 0, 0, 0};
+      kf[s] = live ? *reinterpret_cast<const u32x4*>(a.k + b * a.kb + hk * a.kh + j * a.kl +
+                                                     16 * s + 8 * h)
+                   : u32x4{0, 0, 0, 0};
+      vf[s] = live ? *reinterpret_cast<const u32x4*>(a.v + b * a.vb + hk * a.vh + j * a.vl +
+                                                     16 * s + 8 * h)
+                   : u32x4{0, 0, 0, 0};
     }
   }
-  f32x16 ak[NK][2], av[NK][2];
-#pragma unroll
-  for (int n = 0; n < NK; ++n) ak[n][0] = ak[n][1] = av[n][0] = av[n][1] = zero16();
+  f32x16 ak[2] = {zero16(), zero16()}, av[2] = {zero16(), zero16()};
+  f32x16 sc[2], dp[2];
 
-  auto compute = [&](int u, const unsigned char* qt, const unsigned char* gt,
-                     const float (*st)[64]) __attribute__((always_inline)) {
-    const int row = first + (u % nq) * kTileRows;
-    if (kw >= klen) return;
+  // S and dP of rows 32 qb .. of a tile
+  auto scores = [&](int qb, const unsigned char* qt, const unsigned char* gt, const float (*st)[64])
+      __attribute__((always_inline)) {
 #pragma unroll
-    for (int qb = 0; qb < 2; ++qb) {
-      u32x4 qa[4], ga[4];
+    for (int g = 0; g < 4; ++g) {
+      const f32x4 x = *reinterpret_cast<const f32x4*>(&st[0][32 * qb + 8 * g + 4 * h]);
+      const f32x4 y = *reinterpret_cast<const f32x4*>(&st[1][32 * qb + 8 * g + 4 * h]);
 #pragma unroll
-      for (int s = 0; s < 4; ++s) {
-        qa[s] = row_frag(qt, 32 * qb, s, lo);
-        ga[s] = row_frag(gt, 32 * qb, s, lo);
+      for (int i = 0; i < 4; ++i) {
+        sc[qb][4 * g + i] = x[i];
+        dp[qb][4 * g + i] = y[i];
       }
-      u32x4 p[NK][2], ds[NK][2];
+    }
 #pragma unroll
-      for (int n = 0; n < NK; ++n) {
-        f32x16 sc, dp;
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          const f32x4 x = *reinterpret_cast<const f32x4*>(&st[0][32 * qb + 8 * g + 4 * h]);
-          const f32x4 y = *reinterpret_cast<const f32x4*>(&st[1][32 * qb + 8 * g + 4 * h]);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            sc[4 * g + i] = x[i];
-            dp[4 * g + i] = y[i];
-          }
-        }
-#pragma unroll
-        for (int s = 0; s < 4; ++s) {
-          sc = mfma_32x32x16<T16>(qa[s], kf[n][s], sc);
-          dp = mfma_32x32x16<T16>(ga[s], vf[n][s], dp);
-        }
-#pragma unroll
-        for (int i = 0; i < 16; ++i) sc[i] = fast_exp2(sc[i] * a.c);
-        if (a.causal && row + 32 * qb < kw + 32 * n + 31 - off) {
-          const int x = kw + 32 * n + (l & 31) - off - row - 32 * qb - 4 * h;
-#pragma unroll
-          for (int i = 0; i < 16; ++i) sc[i] = 8 * (i >> 2) + (i & 3) >= x ? sc[i] : 0.f;
-        }
-#pragma unroll
-        for (int i = 0; i < 16; ++i)
-          dp[i] = (Shift<T16>::scaled ? sc[i] * mul : sc[i]) * dp[i];
-        p[n][0] = pack_step<T16>(sc, 0);
-        p[n][1] = pack_step<T16>(sc, 1);
-        ds[n][0] = pack_step<T16>(dp, 0);
-        ds[n][1] = pack_step<T16>(dp, 1);
-      }
-#pragma unroll
-      for (int s = 0; s < 2; ++s)
-#pragma unroll
-        for (int mb = 0; mb < 2; ++mb) {
-          const u32x4 gc = col_frag(gt, 32 * qb + 16 * s, mb, lo);
-          const u32x4 qc = col_frag(qt, 32 * qb + 16 * s, mb, lo);
-#pragma unroll
-          for (int n = 0; n < NK; ++n) {
-            av[n][mb] = mfma_32x32x16<T16>(gc, p[n][s], av[n][mb]);
-            ak[n][mb] = mfma_32x32x16<T16>(qc, ds[n][s], ak[n][mb]);
-          }
-        }
+    for (int s = 0; s < 4; ++s) {
+      sc[qb] = mfma_32x32x16<T16>(row_frag(qt, 32 * qb, s, lo), kf[s], sc[qb]);
+      dp[qb] = mfma_32x32x16<T16>(row_frag(gt, 32 * qb, s, lo), vf[s], dp[qb]);
     }
   };
-
-  load_tile(u0, q0_, g0_, s0_);
-  load_tile(u0 + 1, q1_, g1_, s1_);
-  for (int u = u0; u < u1; u += 3) {
+  // the step of rows 32 qb of this tile; the next one's are rows 32 (qb ^ 1) of (qn, gn, sn)
+  auto step = [&](int qb, const unsigned char* qt, const unsigned char* gt, const unsigned char* qn,
+                  const unsigned char* gn, const float (*sn)[64]) __attribute__((always_inline)) {
+    scores(qb ^ 1, qn, gn, sn);
+    f32x16 p;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) p[i] = fast_exp2(sc[qb][i] * a.c);
+    if (CAUSAL && crow + 32 * qb < kw + 31 - off) {
+      asm volatile("");
+      const int x = kw + (l & 31) - off - crow - 32 * qb - 4 * h;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) p[i] = 8 * (i >> 2) + (i & 3) >= x ? p[i] : 0.f;
+    }
+    f32x16 d;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) d[i] = (Shift<T16>::scaled ? p[i] * mul : p[i]) * dp[qb][i];
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      const u32x4 pp = pack_step<T16>(p, s), dd = pack_step<T16>(d, s);
+#pragma unroll
+      for (int mb = 0; mb < 2; ++mb) {
+        av[mb] = mfma_32x32x16<T16>(col_frag(gt, 32 * qb + 16 * s, mb, lo), pp, av[mb]);
+        ak[mb] = mfma_32x32x16<T16>(col_frag(qt, 32 * qb + 16 * s, mb, lo), dd, ak[mb]);
+      }
+    }
+  };
+  // Tile i of this range lives in slot i % 4; at its top the tiles up to i + 1 have landed
+  // and tile i - 1 is read.  Tiles past the last one are empty (zeros).
+  auto tile = [&](const unsigned char* qt, const unsigned char* gt, const float (*st)[64],
+                  const unsigned char* qn, const unsigned char* gn, const float (*sn)[64],
+                  unsigned char* ql, unsigned char* gl, float (*sl)[64])
+                  __attribute__((always_inline)) {
     __builtin_amdgcn_s_waitcnt(wait_vm_lgkm0(5));
     __builtin_amdgcn_s_barrier();
-    load_tile(u + 2, q2_, g2_, s2_);
-    compute(u, q0_, g0_, s0_);
+    load_tile(ql, gl, sl);
+    if (kw < klen) {
+      step(0, qt, gt, qt, gt, st);
+      step(1, qt, gt, qn, gn, sn);
+    }
+    if (CAUSAL) {
+      crow += kTileRows;
+      if (crow >= qlen) crow = first;
+    }
+  };
+  load_tile(q0_, g0_, s0_);
+  load_tile(q1_, g1_, s1_);
+  load_tile(q2_, g2_, s2_);
+  __builtin_amdgcn_s_waitcnt(wait_vm_lgkm0(10));
+  __builtin_amdgcn_s_barrier();
+  scores(0, q0_, g0_, s0_);
+  for (int u = u0; u < u1; u += 4) {
+    tile(q0_, g0_, s0_, q1_, g1_, s1_, q3_, g3_, s3_);
     if (u + 1 >= u1) break;
-    __builtin_amdgcn_s_waitcnt(wait_vm_lgkm0(5));
-    __builtin_amdgcn_s_barrier();
-    load_tile(u + 3, q0_, g0_, s0_);
-    compute(u + 1, q1_, g1_, s1_);
+    tile(q1_, g1_, s1_, q2_, g2_, s2_, q0_, g0_, s0_);
     if (u + 2 >= u1) break;
-    __builtin_amdgcn_s_waitcnt(wait_vm_lgkm0(5));
-    __builtin_amdgcn_s_barrier();
-    load_tile(u + 4, q1_, g1_, s1_);
-    compute(u + 2, q2_, g2_, s2_);
+    tile(q2_, g2_, s2_, q3_, g3_, s3_, q1_, g1_, s1_);
+    if (u + 3 >= u1) break;
+    tile(q3_, g3_, s3_, q0_, g0_, s0_, q2_, g2_, s2_);
   }
   __builtin_amdgcn_s_waitcnt(wait_vm_lgkm0(0));
 
   const float fv = Shift<T16>::scaled ? 1.f / 32768.f : 1.f;
   const float fk = Shift<T16>::scaled ? a.scale * (1.f / 32768.f) / mul : a.scale;
-#pragma unroll
-  for (int n = 0; n < NK; ++n) {
-    const int j = kw + 32 * n + (l & 31);
-    if (j >= a.Lk) continue;
-    const bool keep = j < klen;
-    if (a.kv_splits == 1) {
-      store_row<T16>(a.dk + b * a.dkb + hk * a.dkh + j * a.dkl, ak[n], fk, h, keep);
-      store_row<T16>(a.dv + b * a.dvb + hk * a.dvh + j * a.dvl, av[n], fv, h, keep);
-    } else {
-      float* d = a.part + (((int64_t)sp * a.nbk + bk) * a.Lk + j) * (2 * kDD);
-      store_part(d, ak[n], fk, h, keep);
-      store_part(d + kDD, av[n], fv, h, keep);
-    }
+  const int j = kw + (l & 31);
+  if (j >= a.Lk) return;
+  const bool keep = j < klen;
+  if (a.kv_splits == 1) {
+    store_row<T16>(a.dk + b * a.dkb + hk * a.dkh + j * a.dkl, ak, fk, h, keep);
+    store_row<T16>(a.dv + b * a.dvb + hk * a.dvh + j * a.dvl, av, fv, h, keep);
+  } else {
+    float* d = a.part + (((int64_t)sp * a.nbk + bk) * a.Lk + j) * (2 * kDD);
+    store_part(d, ak, fk, h, keep);
+    store_part(d + kDD, av, fv, h, keep);
   }
 }
 
@@ -643,7 +644,10 @@ extern "C" int sla2h_dense_attn_bwd(const void* q, const void* k, const void* v,
           a.part, p.dq_splits, bh * Lq, Lq, H, a.dq, a.dqb, a.dqh, a.dql, nullptr, 0, 0, 0);
       if ((err = (int)hipGetLastError())) return err;
     }
-    dense_bwd_dkdv_kernel<T16, 1><<<work_grid(a.kv_map), 256, 0, st>>>(a);
+    if (causal)
+      dense_bwd_dkdv_kernel<T16, true><<<work_grid(a.kv_map), 256, 0, st>>>(a);
+    else
+      dense_bwd_dkdv_kernel<T16, false><<<work_grid(a.kv_map), 256, 0, st>>>(a);
     if ((err = (int)hipGetLastError()) || p.kv_splits == 1) return err;
     dense_bwd_join_kernel<T16, 2 * kDD>
         <<<(unsigned)((bk * Lk * 2 * kDD / 4 + 255) / 256), 256, 0, st>>>(
