@@ -1685,6 +1685,16 @@ def dense_attn_bwd(do, q, k, v, o, lse, causal=False, q_lens=None, k_lens=None, 
 # ---------------------------------------------------------------------------
 # Activations kept in 8 bits for the backward pass (sla2h_act8_* / situ8 / wgrad8)
 # ---------------------------------------------------------------------------
+def _rows_of(t):
+    """(t or a copy, rows, F, row stride) of t (..., F) as rows, without a view's cost for
+    contiguous tensors."""
+    F = t.shape[-1]
+    if t.is_contiguous():
+        return t, t.numel() // F, F, F
+    v, F, ld = _rows_view(t)
+    return v, v.shape[0], F, ld
+
+
 class Act8(NamedTuple):
     """An activation of `rows` x `cols` kept in 8 bits: int8 codes by 64 x 64 tiles and
     a scale per tile (act8_pack)."""
@@ -1717,8 +1727,8 @@ def act8_pack(x):
     code = _dtype_code(x)
     if x.dim() == 0 or x.numel() == 0:
         raise ValueError(f"act8_pack: nothing to pack in {tuple(x.shape)}")
-    x2, cols, ld = _rows_view(x)
-    a = _act8_empty(x2.shape[0], cols, x.device)
+    x2, rows, cols, ld = _rows_of(x)
+    a = _act8_empty(rows, cols, x.device)
     _launch(x.device, "sla2h_act8_pack", x2.data_ptr(), ld, code, a.rows, cols,
             a.codes.data_ptr(), a.scales.data_ptr())
     return a
@@ -1758,9 +1768,9 @@ def situ8_save(gate, up, beta, linear_beta=None):
     beta, lb = _gate_args(beta, linear_beta)
     if gate.dim() == 0 or gate.numel() == 0:
         raise ValueError(f"situ8: nothing to compute in {tuple(gate.shape)}")
-    g2, F, sg = _rows_view(gate)
-    u2, _, su = _rows_view(up)
-    rows, dev = g2.shape[0], gate.device
+    g2, rows, F, sg = _rows_of(gate)
+    u2, _, _, su = _rows_of(up)
+    dev = gate.device
     nc, ns = _situ8_bytes(rows, F)
     h = torch.empty(gate.shape, device=dev, dtype=gate.dtype)
     buf = _scratch(2 * (nc + ns), dev)
@@ -1794,7 +1804,7 @@ def _situ8_bwd(dh, g, u, rows, cols, dev, beta, linear_beta, with_h):
     if dh.shape[-1:] != (cols,) or dh.numel() != rows * cols or dh.device != dev:
         raise ValueError(f"situ8_bwd: dh {tuple(dh.shape)} on {dh.device} does not fit "
                          f"{rows} x {cols} on {dev}")
-    d2, F, sd = _rows_view(dh)
+    d2, _, F, sd = _rows_of(dh)
     out = [torch.empty(dh.shape, device=dev, dtype=dh.dtype) for _ in range(2 + with_h)]
     _launch(dev, "sla2h_situ8_bwd", d2.data_ptr(), sd, *g, *u, code, rows, F, beta, lb, F,
             out[0].data_ptr(), out[1].data_ptr(), out[2].data_ptr() if with_h else None)
@@ -1832,7 +1842,7 @@ def linear_wgrad8(dy, a):
     if M == 0 or dy.numel() != a.rows * M or dy.device != a.codes.device:
         raise ValueError(f"linear_wgrad8: dy {tuple(dy.shape)} on {dy.device} has not the "
                          f"{a.rows} rows of X on {a.codes.device}")
-    d2, _, ld = _rows_view(dy)
+    d2, _, _, ld = _rows_of(dy)
     if ld >= _ATTN_ROW_SPAN:
         d2 = d2.contiguous()
         ld = M
