@@ -164,10 +164,12 @@ __device__ inline void store_part(float* p, const f32x16 (&x)[2], float f, int h
     }
 }
 
-// dq: workgroup = 4 waves x (32 NQ) query rows; keys and values as in the forward.
-// dQ^T += K^T dS^T with dS^T straight from the score tile's registers.
-template <typename T16, int NQ>
-__global__ __launch_bounds__(256, 2) void dense_bwd_dq_kernel(DenseBwdArgs a) {
+// dq: workgroup = 4 waves x 32 query rows; keys and values in tiles of 64 rows through three
+// LDS slots.  dQ^T += K^T dS^T with dS^T straight from the score tile's registers.  (64 rows per
+// wave halve the LDS reads but spill at two waves per SIMD: the whole backward 6.04 ms against
+// 6.11 at B = 1, H = 8, L = 29,952, 2.96 against 2.93 causal.)
+template <typename T16>
+__global__ __launch_bounds__(256, 3) void dense_bwd_dq_kernel(DenseBwdArgs a) {
   __shared__ __align__(16) unsigned char k0[kTileB], k1[kTileB], k2[kTileB];
   __shared__ __align__(16) unsigned char v0[kTileB], v1[kTileB], v2[kTileB];
   int bh, item;
@@ -179,8 +181,8 @@ __global__ __launch_bounds__(256, 2) void dense_bwd_dq_kernel(DenseBwdArgs a) {
   const LaneOff lo(l);
   const int qlen = seq_len(a.q_lens, b, a.Lq), klen = seq_len(a.k_lens, b, a.Lk);
 
-  const int q0 = qt * (128 * NQ), qw = q0 + w * (32 * NQ);
-  const int qend = min(q0 + 128 * NQ, qlen);
+  const int q0 = qt * 128, qw = q0 + w * 32;
+  const int qend = min(q0 + 128, qlen);
   auto limit = [&](int i) __attribute__((always_inline)) {
     if (i >= qlen) return 0;
     if (!a.causal) return klen;
@@ -208,85 +210,72 @@ __global__ __launch_bounds__(256, 2) void dense_bwd_dq_kernel(DenseBwdArgs a) {
 
   float mul = 1.f;
   if (Shift<T16>::scaled) mul = ds_scale(a, b, hk);
-  u32x4 qf[NQ][4], gf[NQ][4];
-  int lim[NQ];
-  float nl[NQ], nd[NQ];  // shift - lse log2e, -delta (times mul)
+  const int i = qw + (l & 31);
+  const int lim = limit(i);
+  const bool live = lim > 0;
+  // shift - lse log2e, -delta (times mul)
+  const float nl = live ? a.nlse[(int64_t)bh * a.Lq + i] * a.c : -__builtin_inff();
+  const float nd = live ? a.ndelta[(int64_t)bh * a.Lq + i] * mul : 0.f;
+  u32x4 qf[4], gf[4];
   {
-    const uint16_t* qp = a.q + b * a.qb + hq * a.qh;
-    const uint16_t* gp = a.dout + b * a.gb + hq * a.gh;
+    const uint16_t* qp = a.q + b * a.qb + hq * a.qh + i * a.ql + 8 * h;
+    const uint16_t* gp = a.dout + b * a.gb + hq * a.gh + i * a.gl + 8 * h;
 #pragma unroll
-    for (int n = 0; n < NQ; ++n) {
-      const int i = qw + 32 * n + (l & 31);
-      lim[n] = limit(i);
-      const bool live = lim[n] > 0;
-      nl[n] = live ? a.nlse[(int64_t)bh * a.Lq + i] * a.c : -__builtin_inff();
-      nd[n] = live ? a.ndelta[(int64_t)bh * a.Lq + i] * mul : 0.f;
-#pragma unroll
-      for (int s = 0; s < 4; ++s) {
-        qf[n][s] = live ? *reinterpret_cast<const u32x4*>(qp + i * a.ql + 16 * s + 8 * h)
-                        : u32x4{0, 0, 0, 0};
-        gf[n][s] = live ? *reinterpret_cast<const u32x4*>(gp + i * a.gl + 16 * s + 8 * h)
-                        : u32x4{0, 0, 0, 0};
-      }
+    for (int s = 0; s < 4; ++s) {
+      qf[s] = live ? *reinterpret_cast<const u32x4*>(qp + 16 * s) : u32x4{0, 0, 0, 0};
+      gf[s] = live ? *reinterpret_cast<const u32x4*>(gp + 16 * s) : u32x4{0, 0, 0, 0};
     }
   }
-  const int wlast = min(qw + 32 * NQ, qlen) - 1;
+  // keys that any query of the wave sees, and that all of them see
+  const int wlast = min(qw + 32, qlen) - 1;
   const int wany = wlast >= qw ? limit(wlast) : 0;
   const int wall = wlast >= qw ? limit(qw) : 0;
 
-  f32x16 acc[NQ][2];
-#pragma unroll
-  for (int n = 0; n < NQ; ++n) acc[n][0] = acc[n][1] = zero16();
-
-  auto compute = [&](int t, const unsigned char* kt, const unsigned char* vt) __attribute__((always_inline)) {
-    const int base = t * kTileRows;
-    if (base >= wany) return;
+  f32x16 acc[2] = {zero16(), zero16()};
+  auto part = [&](auto masked, int base, const unsigned char* kt, const unsigned char* vt)
+      __attribute__((always_inline)) {
 #pragma unroll
     for (int kb = 0; kb < 2; ++kb) {
-      u32x4 kf[4], vf[4];
+      f32x16 sc = zero16(), dp = zero16();
 #pragma unroll
       for (int s = 0; s < 4; ++s) {
-        kf[s] = row_frag(kt, 32 * kb, s, lo);
-        vf[s] = row_frag(vt, 32 * kb, s, lo);
-      }
-      u32x4 ds[NQ][2];
-#pragma unroll
-      for (int n = 0; n < NQ; ++n) {
-        f32x16 sc = zero16(), dp = zero16();
-#pragma unroll
-        for (int s = 0; s < 4; ++s) {
-          sc = mfma_32x32x16<T16>(kf[s], qf[n][s], sc);
-          dp = mfma_32x32x16<T16>(vf[s], gf[n][s], dp);
-        }
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const float p = fast_exp2(__builtin_fmaf(sc[i], a.c, nl[n]));
-          dp[i] = p * (Shift<T16>::scaled ? __builtin_fmaf(dp[i], mul, nd[n]) : dp[i] + nd[n]);
-        }
-        if (base + kTileRows > wall) {
-          const int x = lim[n] - base - 32 * kb - 4 * h;
-#pragma unroll
-          for (int i = 0; i < 16; ++i) dp[i] = 8 * (i >> 2) + (i & 3) < x ? dp[i] : 0.f;
-        }
-        ds[n][0] = pack_step<T16>(dp, 0);
-        ds[n][1] = pack_step<T16>(dp, 1);
+        sc = mfma_32x32x16<T16>(row_frag(kt, 32 * kb, s, lo), qf[s], sc);
+        dp = mfma_32x32x16<T16>(row_frag(vt, 32 * kb, s, lo), gf[s], dp);
       }
 #pragma unroll
-      for (int s = 0; s < 2; ++s)
+      for (int e = 0; e < 16; ++e) {
+        const float p = fast_exp2(__builtin_fmaf(sc[e], a.c, nl));
+        dp[e] = p * (Shift<T16>::scaled ? __builtin_fmaf(dp[e], mul, nd) : dp[e] + nd);
+      }
+      if (decltype(masked)::value) {
+        const int x = lim - base - 32 * kb - 4 * h;
 #pragma unroll
-        for (int mb = 0; mb < 2; ++mb) {
-          const u32x4 kc = col_frag(kt, 32 * kb + 16 * s, mb, lo);
+        for (int e = 0; e < 16; ++e) dp[e] = 8 * (e >> 2) + (e & 3) < x ? dp[e] : 0.f;
+      }
 #pragma unroll
-          for (int n = 0; n < NQ; ++n) acc[n][mb] = mfma_32x32x16<T16>(kc, ds[n][s], acc[n][mb]);
-        }
+      for (int s = 0; s < 2; ++s) {
+        const u32x4 ds = pack_step<T16>(dp, s);
+#pragma unroll
+        for (int mb = 0; mb < 2; ++mb)
+          acc[mb] = mfma_32x32x16<T16>(col_frag(kt, 32 * kb + 16 * s, mb, lo), ds, acc[mb]);
+      }
     }
+  };
+  // a tile that every query of the wave sees runs without a branch
+  auto compute = [&](int t, const unsigned char* kt, const unsigned char* vt)
+      __attribute__((always_inline)) {
+    const int base = t * kTileRows;
+    if (base + kTileRows <= wall)
+      part(std::false_type{}, base, kt, vt);
+    else if (base < wany)
+      part(std::true_type{}, base, kt, vt);
   };
 
   load_tile(t0, k0, v0);
   load_tile(t0 + 1, k1, v1);
   for (int t = t0; t < nt; t += 3) {
     __builtin_amdgcn_s_waitcnt(wait_vm_lgkm0(4));
-    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_s_barrier();  // tile t has landed, tile t - 1 is read
     load_tile(t + 2, k2, v2);
     compute(t, k0, v0);
     if (t + 1 >= nt) break;
@@ -302,17 +291,12 @@ __global__ __launch_bounds__(256, 2) void dense_bwd_dq_kernel(DenseBwdArgs a) {
   }
   __builtin_amdgcn_s_waitcnt(wait_vm_lgkm0(0));
 
+  if (i >= a.Lq) return;
   const float f = Shift<T16>::scaled ? a.scale * (1.f / 32768.f) / mul : a.scale;
-#pragma unroll
-  for (int n = 0; n < NQ; ++n) {
-    const int i = qw + 32 * n + (l & 31);
-    if (i >= a.Lq) continue;
-    if (a.dq_splits == 1)
-      store_row<T16>(a.dq + b * a.dqb + hq * a.dqh + i * a.dql, acc[n], f, h, lim[n] > 0);
-    else
-      store_part(a.part + (((int64_t)sp * a.nbh + bh) * a.Lq + i) * kDD, acc[n], f, h,
-                 lim[n] > 0);
-  }
+  if (a.dq_splits == 1)
+    store_row<T16>(a.dq + b * a.dqb + hq * a.dqh + i * a.dql, acc, f, h, live);
+  else
+    store_part(a.part + (((int64_t)sp * a.nbh + bh) * a.Lq + i) * kDD, acc, f, h, live);
 }
 
 // dk, dv: workgroup = 4 waves x 32 keys of one key head; the query rows of the heads that
@@ -507,20 +491,18 @@ __global__ __launch_bounds__(256) void dense_bwd_join_kernel(const float* __rest
 }
 
 struct BwdPlan {
-  int nq;  // query rows of a dq workgroup: 128 nq
   int64_t qtiles, dq_nwork, ktiles, kv_nwork;
   int dq_splits, kv_splits;
   int64_t nqb, nkb;
   size_t stats, parts;  // floats
 };
 
-// even: neither causal nor lengths.  Workgroups of uneven length balance by number: the
-// rules of the forward, and twice the ranges.
+// even: neither causal nor lengths.  Workgroups of uneven length balance by number: twice
+// the ranges.
 BwdPlan bwd_plan(int dtype, int B, int H, int Hkv, int64_t Lq, int64_t Lk, bool even) {
   BwdPlan p{};
   const int64_t bh = (int64_t)B * H, bk = (int64_t)B * Hkv, rep = H / Hkv;
-  p.nq = bh * ((Lq + 255) / 256) >= (even ? 256 : 768) ? 2 : 1;
-  p.qtiles = (Lq + 128 * p.nq - 1) / (128 * p.nq);
+  p.qtiles = (Lq + 127) / 128;
   auto split = [&](int64_t blocks, int64_t tiles) {
     const int64_t want = even ? 512 : 1024;
     if (blocks >= want / 2) return 1;
@@ -634,10 +616,7 @@ extern "C" int sla2h_dense_attn_bwd(const void* q, const void* k, const void* v,
     int err;
     dense_bwd_prep_kernel<T16><<<(unsigned)(pq + pv), 256, 0, st>>>(a, pq);
     if ((err = (int)hipGetLastError())) return err;
-    if (p.nq == 2)
-      dense_bwd_dq_kernel<T16, 2><<<work_grid(a.dq_map), 256, 0, st>>>(a);
-    else
-      dense_bwd_dq_kernel<T16, 1><<<work_grid(a.dq_map), 256, 0, st>>>(a);
+    dense_bwd_dq_kernel<T16><<<work_grid(a.dq_map), 256, 0, st>>>(a);
     if ((err = (int)hipGetLastError())) return err;
     if (p.dq_splits > 1) {
       dense_bwd_join_kernel<T16, kDD><<<(unsigned)((bh * Lq * kDD / 4 + 255) / 256), 256, 0, st>>>(
