@@ -315,7 +315,7 @@ __global__ __launch_bounds__(256, 2) void dense_fwd_kernel(DenseFwdArgs a) {
     const int i = qw + 32 * n + (l & 31);
     if (i >= a.Lq) continue;
     const float ls = swap32_sum(lsum[n]);
-    const float inv = ls > 0.f ? 1.f / ls : (ls == 0.f ? 0.f : ls);
+    const float inv = 1.f / ls;  // a row whose scores are all -inf is NaN
 #pragma unroll
     for (int mb = 0; mb < 2; ++mb)
 #pragma unroll

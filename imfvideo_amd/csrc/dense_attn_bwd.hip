@@ -553,7 +553,8 @@ extern "C" int sla2h_dense_attn_bwd(const void* q, const void* k, const void* v,
                                     int B, int H, int Hkv, int64_t Lq, int64_t Lk, int causal,
                                     float scale, void* workspace, void* dq, void* dk, void* dv,
                                     void* stream) {
-  SLA2H_CHECK_ARG(q && k && v && o && dout && lse && strides && workspace && dq && dk && dv);
+  SLA2H_CHECK_ARG(q && k && v && o && dout && lse && strides && workspace);
+  SLA2H_CHECK_ARG((dq || dk) && !dk == !dv);
   SLA2H_CHECK_ARG(dtype == SLA2H_DTYPE_F16 || dtype == SLA2H_DTYPE_BF16);
   SLA2H_CHECK_ARG(sizes_ok(B, H, Hkv, Lq, Lk));
   SLA2H_CHECK_ARG(scale > 0.f && scale < 1e30f);
@@ -616,13 +617,17 @@ extern "C" int sla2h_dense_attn_bwd(const void* q, const void* k, const void* v,
     int err;
     dense_bwd_prep_kernel<T16><<<(unsigned)(pq + pv), 256, 0, st>>>(a, pq);
     if ((err = (int)hipGetLastError())) return err;
-    dense_bwd_dq_kernel<T16><<<work_grid(a.dq_map), 256, 0, st>>>(a);
-    if ((err = (int)hipGetLastError())) return err;
-    if (p.dq_splits > 1) {
-      dense_bwd_join_kernel<T16, kDD><<<(unsigned)((bh * Lq * kDD / 4 + 255) / 256), 256, 0, st>>>(
-          a.part, p.dq_splits, bh * Lq, Lq, H, a.dq, a.dqb, a.dqh, a.dql, nullptr, 0, 0, 0);
+    if (dq) {
+      dense_bwd_dq_kernel<T16><<<work_grid(a.dq_map), 256, 0, st>>>(a);
       if ((err = (int)hipGetLastError())) return err;
+      if (p.dq_splits > 1) {
+        dense_bwd_join_kernel<T16, kDD>
+            <<<(unsigned)((bh * Lq * kDD / 4 + 255) / 256), 256, 0, st>>>(
+                a.part, p.dq_splits, bh * Lq, Lq, H, a.dq, a.dqb, a.dqh, a.dql, nullptr, 0, 0, 0);
+        if ((err = (int)hipGetLastError())) return err;
+      }
     }
+    if (!dk) return 0;
     if (causal)
       dense_bwd_dkdv_kernel<T16, true><<<work_grid(a.kv_map), 256, 0, st>>>(a);
     else

@@ -336,8 +336,6 @@ __global__ __launch_bounds__(256, 2) void wgrad8_kernel(Wgrad8Args a) {
       put_y(ny, yv, ye);
       load_y(s + 2, yv, ye);
     }
-    put_x(nx, xv);
-    load_x(s + 2, xv);
     const float scn = scale_of(s + 1);
     u32x4 fm[2][4];
 #pragma unroll
@@ -358,6 +356,8 @@ __global__ __launch_bounds__(256, 2) void wgrad8_kernel(Wgrad8Args a) {
         for (int e = 0; e < 4; ++e) acc[i][j][e] = __builtin_fmaf(sc, t[e], acc[i][j][e]);
       }
     }
+    put_x(nx, xv);
+    load_x(s + 2, xv);
     sc = scn;
   };
   load_x(0, xv);

@@ -146,8 +146,9 @@ class _DenseAttentionFunction(torch.autograd.Function):
         _no_batched(do, "dense_attention")
         q, k, v, o, lse, o_lo, q_lens, k_lens = ctx.saved_tensors
         causal, scale = ctx.args
-        return (*ops.dense_attn_bwd(do, q, k, v, o, lse, causal, q_lens, k_lens, scale, o_lo,
-                                    True), None, None, None, None)
+        nq, nk, nv = ctx.needs_input_grad[:3]
+        return (*ops.dense_attn_bwd(do, q, k, v, o, lse, causal, q_lens, k_lens, scale, o_lo, True,
+                                    nq, nk or nv), None, None, None, None)
 
 
 def dense_attention(q, k, v, causal=False, q_lens=None, k_lens=None, scale=None):

@@ -1637,11 +1637,11 @@ def dense_attn_fwd(q, k, v, causal=False, q_lens=None, k_lens=None, scale=None, 
 
 
 def dense_attn_bwd(do, q, k, v, o, lse, causal=False, q_lens=None, k_lens=None, scale=None,
-                   o_lo=None, tok=False):
+                   o_lo=None, tok=False, need_q=True, need_kv=True):
     """Gradients (dq, dk, dv) of dense_attn_fwd for the output gradient do, from its
     operands, its output o (with o_lo where it was asked for) and lse, the
     probabilities recomputed; dk and dv summed over the query heads of a key head, zero
-    behind the sequences."""
+    behind the sequences.  Without need_q dq is None, without need_kv dk and dv."""
     q, k, v, p, scale = _attn_operands(q, k, v, scale, tok)
     dev, dtype = q.device, q.dtype
 
@@ -1667,18 +1667,22 @@ def dense_attn_bwd(do, q, k, v, o, lse, causal=False, q_lens=None, k_lens=None, 
         q_lens = attn_lens(q_lens, q, "q_lens")
     if k_lens is not None:
         k_lens = attn_lens(k_lens, q, "k_lens")
-    dq = _attn_empty(p.o_shape, dev, dtype, p.o_flip)
-    ks = p.k_shape
-    kf = (ks[0], ks[2], ks[1], ks[3])
-    dk = _attn_empty(kf if p.k_flip else ks, dev, dtype, p.k_flip)
-    dv = _attn_empty(kf if p.v_flip else ks, dev, dtype, p.v_flip)
+    dq = dk = dv = None
+    if need_q:
+        dq = _attn_empty(p.o_shape, dev, dtype, p.o_flip)
+    if need_kv:
+        ks = p.k_shape
+        kf = (ks[0], ks[2], ks[1], ks[3])
+        dk = _attn_empty(kf if p.k_flip else ks, dev, dtype, p.k_flip)
+        dv = _attn_empty(kf if p.v_flip else ks, dev, dtype, p.v_flip)
     if p.empty:
-        return dq.zero_(), dk.zero_(), dv.zero_()
-    ws = _scratch(p.bwd_ws, dev)
-    _launch(dev, "sla2h_dense_attn_bwd", q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(),
-            _ptr(o_lo), do.data_ptr(), lse.data_ptr(), p.bwd, _ptr(q_lens), _ptr(k_lens),
-            _HALF[dtype], *p.sizes, 1 if causal else 0, scale, ws.data_ptr(), dq.data_ptr(),
-            dk.data_ptr(), dv.data_ptr())
+        return tuple(t if t is None else t.zero_() for t in (dq, dk, dv))
+    if need_q or need_kv:
+        ws = _scratch(p.bwd_ws, dev)
+        _launch(dev, "sla2h_dense_attn_bwd", q.data_ptr(), k.data_ptr(), v.data_ptr(),
+                o.data_ptr(), _ptr(o_lo), do.data_ptr(), lse.data_ptr(), p.bwd, _ptr(q_lens),
+                _ptr(k_lens), _HALF[dtype], *p.sizes, 1 if causal else 0, scale, ws.data_ptr(),
+                _ptr(dq), _ptr(dk), _ptr(dv))
     return dq, dk, dv
 
 

@@ -871,7 +871,7 @@ int sla2h_dense_attn_fwd(const void* q, const void* k, const void* v, const int6
  *   dv = P^T dout, dk and dv summed over the query heads of a key head.
  * q, k, v, lse, lens, sizes, causal and scale as in the forward, o its output (o_lo its
  * second half or NULL), dout like o;
- * dq like q, dk and dv like k.  strides: host array of 24 int64, the (batch, head, row)
+ * dq like q, dk and dv like k; dq, or dk and dv together, may be NULL (not computed).  strides: host array of 24 int64, the (batch, head, row)
  * strides of q, k, v, o, dout, dq, dk, dv in elements (the same conditions; row strides of q, k, v and
  * dout below 2^23).  Gradients of rows behind a sequence and of rows without a key are 0; dout is
  * not read there.  No atomics: results are reproducible bit for bit.

@@ -70,9 +70,9 @@ def test_c_entries_check_their_arguments():
                                         scale, ws, o, lse, lo, None)
 
     def bwd(q=16, lse=4, s=st(), dtype=1, B=1, H=2, Hkv=2, Lq=4, Lk=4, scale=0.125, ws=16,
-            lo=None):
+            lo=None, grads=(16, 16, 16)):
         return lib.sla2h_dense_attn_bwd(q, 16, 16, 16, lo, 16, lse, s, None, None, dtype, B, H, Hkv,
-                                        Lq, Lk, 0, scale, ws, 16, 16, 16, None)
+                                        Lq, Lk, 0, scale, ws, *grads, None)
 
     for f in (fwd, bwd):
         assert f(q=None) == bad and f(q=8) == bad          # missing, unaligned
@@ -84,6 +84,7 @@ def test_c_entries_check_their_arguments():
         assert f(s=st(s2=0)) == bad                              # rows on top of each other
         assert f(lse=2) == bad and f(lo=8) == bad
     assert bwd(lse=None) == bad and bwd(ws=None) == bad
+    assert bwd(grads=(None, None, None)) == bad and bwd(grads=(16, 16, None)) == bad
     # few queries over many keys: the split form needs its workspace
     assert lib.sla2h_dense_attn_fwd_workspace_bytes(1, 1, 1, 1, 100_000) > 0
     assert fwd(H=1, Hkv=1, Lq=1, Lk=100_000) == bad

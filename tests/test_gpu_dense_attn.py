@@ -340,6 +340,79 @@ def test_autograd_entry():
     assert o32.dtype == torch.bfloat16 and torch.equal(o32, dense_attention(q, k, v))
 
 
+def test_only_the_gradients_asked_for():
+    """Frozen keys or queries: the others' gradients are the same bits; an expanded output
+    gradient (of a sum) is taken too."""
+    from imfvideo_amd import ops
+    from imfvideo_amd.imf_dit_video import dense_attention
+    x = [t.cuda().transpose(1, 2).contiguous()
+         for t in inputs(16, 2, 4, 2, 70, 90, torch.float16)[:3]]
+    req = lambda *on: [t.clone().requires_grad_(r) for t, r in zip(x, on)]
+    full = req(True, True, True)
+    want = torch.autograd.grad(dense_attention(*full).sum(), full)
+    for on in ((True, False, False), (False, True, True), (False, True, False), (False, False, True)):
+        a = req(*on)
+        leaves = [t for t, r in zip(a, on) if r]
+        got = torch.autograd.grad(dense_attention(*a).sum(), leaves)
+        for g, w in zip(got, [w for w, r in zip(want, on) if r]):
+            assert torch.equal(g, w), on
+    o, lse = ops.dense_attn_fwd(*x, tok=True)
+    assert ops.dense_attn_bwd(o, *x, o, lse, tok=True, need_kv=False)[1:] == (None, None)
+
+
+def test_autograd_in_a_graph():
+    """Forward and backward of the autograd entry captured together, while an eager graph of
+    other leaves lives; replays on refilled inputs match eager calls."""
+    from imfvideo_amd.imf_dit_video import dense_attention
+    x = [t.cuda().transpose(1, 2).contiguous() for t in inputs(17, 1, 2, 2, 130, 130,
+                                                               torch.bfloat16)]
+
+    def step():
+        leaves = [t.detach().requires_grad_(True) for t in x[:3]]
+        o = dense_attention(*leaves, causal=True)
+        return [o.detach(), *torch.autograd.grad(o, leaves, x[3])]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            step()
+    torch.cuda.current_stream().wait_stream(side)
+    other = x[0].clone().requires_grad_(True)
+    alive = dense_attention(other, x[1], x[2])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    torch.cuda.synchronize()
+    for _ in range(4):
+        for t in x:
+            t.copy_(torch.randn(t.shape, device="cuda"))
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(out, step()):
+            assert torch.equal(a, b)
+        torch.cuda.synchronize()
+    del alive
+
+
+def test_infinite_scores():
+    """A score of +inf makes its row NaN; a row whose scores are all -inf is NaN as the
+    softmax of it is; other rows are not touched."""
+    from imfvideo_amd import ops
+    for L in (40, 300):
+        q, k, v, _ = (t.cuda() for t in inputs(18, 1, 64, 64, L, L, torch.bfloat16))
+        base, _ = ops.dense_attn_fwd(q, k, v)
+        q2, k2 = q.clone(), k.abs()
+        want, _ = ops.dense_attn_fwd(q2, k2, v)
+        q2[:, :, 5] = float("inf")
+        q2[:, :, 7] = float("-inf")
+        o, lse = ops.dense_attn_fwd(q2, k2, v)
+        assert torch.isnan(o[:, :, 5]).all() and torch.isnan(o[:, :, 7]).all()
+        keep = [i for i in range(L) if i not in (5, 7)]
+        assert torch.equal(o[:, :, keep], want[:, :, keep])
+        assert torch.isfinite(base).all()
+
+
 def test_autograd_refusals():
     from imfvideo_amd.imf_dit_video import dense_attention
     x = [torch.randn(1, 8, 2, 64, device="cuda").half().requires_grad_(True) for _ in range(3)]
