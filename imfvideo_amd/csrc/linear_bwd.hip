@@ -277,7 +277,7 @@ __global__ __launch_bounds__(256, 2) void wgrad8_kernel(Wgrad8Args a) {
     }
   };
   // codes: threads 0 .. 127 the first tile's 4 KB, the others the second's, 16 bytes each twice
-  // (always two loads, zeros past the last tile: the loop counts them)
+  // (zeros past the last tile)
   const int ct = n0 / kAct, xi = tid & 127;
   const int xoff = (tid >> 7) * kActBytes + xi * 16;
   auto load_x = [&](int s, u32x4 (&v)[2]) __attribute__((always_inline)) {
@@ -326,10 +326,11 @@ __global__ __launch_bounds__(256, 2) void wgrad8_kernel(Wgrad8Args a) {
   // one stage: everything of stage s + 1 moves into the other slot meanwhile
   auto stage = [&](int s, const unsigned char* ly, const unsigned char* lx, unsigned char* ny,
                    unsigned char* nx) __attribute__((always_inline)) {
-    // this wave's part of stage s is in LDS (the two loads of codes behind it may be
-    // in flight), then everyone's, and stage s - 1 is read
-    __builtin_amdgcn_s_waitcnt(DMA ? 0x0072 : 0xC07F);
+    // this wave's part of stage s is in LDS, then everyone's, and stage s - 1 is read
+    __builtin_amdgcn_s_waitcnt(DMA ? 0x0070 : 0xC07F);
     __builtin_amdgcn_s_barrier();
+    u32x4 xn[2];
+    load_x(s + 2, xn);
     if (DMA) {
       dma_y(s + 1, ny);
     } else {
@@ -357,7 +358,8 @@ __global__ __launch_bounds__(256, 2) void wgrad8_kernel(Wgrad8Args a) {
       }
     }
     put_x(nx, xv);
-    load_x(s + 2, xv);
+    xv[0] = xn[0];
+    xv[1] = xn[1];
     sc = scn;
   };
   load_x(0, xv);
