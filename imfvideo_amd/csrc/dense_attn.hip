@@ -136,6 +136,8 @@ __device__ inline int key_limit(int i, int qlen, int klen, int causal) {
 // The step of 32 keys is software-pipelined: its scores were computed one step earlier, so
 // that the score products of the next step, which depend on nothing here, run on the matrix
 // cores under this step's exponentials; operands of the step after are read from LDS meanwhile.
+// 64 rows per wave at B = 1, H = 8, L = 29,952, bf16: 1.78 ms, 1.03 PFLOP/s (8192^3 matrix product of
+// the library on the same card 1.25); MFMA 48 %, VALU 61 % busy, the clock at the power limit.
 // FINE: waves whose rows see at most kFineKeys keys add what the rounding of P lost with a
 // second product.  delta = dO . O of the backward inherits that rounding, and dS = P (dP - delta)
 // shows it where few keys share a row (77 keys: dq and dk 2.6e-3 off against 2.4e-3, of which the
@@ -342,7 +344,8 @@ __global__ __launch_bounds__(256, 2) void dense_fwd_kernel(DenseFwdArgs a) {
 
 // Few queries: workgroup = 32 rows (of the `rep` query heads that share a key head) over one
 // range of keys; its waves take the 32-key units in turn, each with LDS slots of its own (no
-// barrier in the loop), and their sums are joined in LDS.  With one range the result is final,
+// barrier in the loop), and their sums are joined in LDS: one query over 29,952 and 18,720 keys
+// of 8 heads in 20 us, 5 TB/s.  With one range the result is final,
 // else a second kernel adds the ranges in order.
 template <typename T16>
 __global__ __launch_bounds__(256, 2) void dense_fwd_split_kernel(DenseFwdArgs a) {

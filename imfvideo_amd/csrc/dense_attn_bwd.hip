@@ -60,7 +60,7 @@ __device__ inline int first_query(int qlen, int klen, int causal) {
   return causal && qlen > klen ? qlen - klen : 0;
 }
 
-// delta of 256 rows of a head (8 lanes per row), and for fp16 the largest row norm of
+// delta of 256 rows of a head (8 lanes per row; HBM-bound: 16 us at B = 1, H = 8, L = 29,952), and for fp16 the largest row norm of
 // do; the workgroups behind them take the norms of v.
 template <typename T16>
 __global__ __launch_bounds__(256) void dense_bwd_prep_kernel(DenseBwdArgs a, int64_t nq) {
@@ -303,7 +303,9 @@ __global__ __launch_bounds__(256, 3) void dense_bwd_dq_kernel(DenseBwdArgs a) {
 // read it are streamed through LDS in tiles of 64, three tiles ahead into four slots, with
 // their -lse and -delta, which start the accumulators of S and dP.  The step of 32 rows is
 // software-pipelined as in the forward: S and dP of the next step run on the matrix cores
-// under this step's exponentials.
+// under this step's exponentials.  B = 1, H = 8, L = 29,952, bf16: 3.46 ms, 1.06 PFLOP/s of its
+// four products (dq 2.7 ms, 1.02 of its three), the clock at the power limit; 64 keys per wave,
+// which halves the LDS reads but leaves one wave per SIMD: 3.8.
 template <typename T16, bool CAUSAL>
 __global__ __launch_bounds__(256, 2) void dense_bwd_dkdv_kernel(DenseBwdArgs a) {
   __shared__ __align__(16) unsigned char q0_[kTileB], q1_[kTileB], q2_[kTileB], q3_[kTileB];

@@ -211,7 +211,9 @@ __device__ inline void widen16(u32x4 c, u32x4& lo, u32x4& hi) {
 // LDS slots: dY goes there as it is (DMA: buffer loads straight into LDS, for 16-byte
 // aligned rows; else through registers, as aligned dwords funnelled to the row's start), the
 // codes are widened on their way, and the fragments are read transposed.  A slot is an array
-// of its own: LDS reads of one then need not wait for the loads into the other.
+// of its own: LDS reads of one then need not wait for the loads into the other.  59,904 x 2,048 x 512
+// bf16: 160 us, 785 TFLOP/s (MFMA 30 %, VALU 43 % busy, the rest LDS latency at two waves per
+// SIMD); rows of 2,730 bytes (29,138 x 1,365 x 512): 72 us, element by element 193.
 template <typename T16, bool DMA>
 __global__ __launch_bounds__(256, 2) void wgrad8_kernel(Wgrad8Args a) {
   __shared__ __align__(16) unsigned char ly0[kAStage], ly1[kAStage];
