@@ -245,7 +245,9 @@ bool plan(int64_t rows, int F, int& cb, int64_t& ntile, unsigned& grid) {
   return ntile < ((int64_t)1 << 31);
 }
 
-bool code_ok(const void* c, const void* s) { return c && s && (uintptr_t)c % 16 == 0 && (uintptr_t)s % 4 == 0; }
+bool code_ok(const void* c, const void* s) {
+  return c && s && (uintptr_t)c % 16 == 0 && (uintptr_t)s % 4 == 0;
+}
 bool half_ok(const void* p) { return p && (uintptr_t)p % 2 == 0; }
 bool dtype_ok(int d) { return d == SLA2H_DTYPE_F16 || d == SLA2H_DTYPE_BF16; }
 

@@ -7,9 +7,10 @@
 // row bound in log2 units, the maximum of the first keys.  It moves only when a tile's sums
 // show that its probabilities have outgrown the range set aside for them (a wave-uniform,
 // rarely taken branch computes the tile again and rescales the accumulators): the result
-// does not depend on m beyond rounding, and the common path computes no maximum.  P is rounded to the operands' 16-bit type for the product (an
-// error of half a unit in its last place per term, as the inputs themselves carry); row sums
-// add the fp32 values, so that lse, which the backward builds on, is exact to fp32.
+// does not depend on m beyond rounding, and the common path computes no maximum.  P is
+// rounded to the operands' 16-bit type for the product (an error of half a unit in its last place
+// per term, as the inputs themselves carry); row sums add the fp32 values, so that lse, which
+// the backward builds on, is exact to fp32.
 #include "dense_attn.h"
 
 #include <initializer_list>
@@ -230,7 +231,7 @@ __global__ __launch_bounds__(256, 2) void dense_fwd_kernel(DenseFwdArgs a) {
     for (int n = 0; n < NQ; ++n)
       raise_bound(lane_max(sc[kb][n]), a.c, m[n], lsum[n], acc[n]);
   };
-  // one step: keys 32 kb .. of tile t; kn, kb: the step after next
+  // one step: keys 32 kb .. of tile t; rows 32 kb .. of kn are the step after next
   auto step = [&](int t, int kb, const unsigned char* kt, const unsigned char* vt,
                   const unsigned char* kn) __attribute__((always_inline)) {
     const int base = t * kTileRows + 32 * kb;
@@ -282,7 +283,8 @@ __global__ __launch_bounds__(256, 2) void dense_fwd_kernel(DenseFwdArgs a) {
   // Tile t lives in slot t % 4; tiles past the last one are empty (zeros).  At the top of
   // tile t the tiles up to t + 1 have landed and tile t - 1 is read.
   auto tile = [&](int t, const unsigned char* kt, const unsigned char* vt,
-                  const unsigned char* kt1, unsigned char* kl, unsigned char* vl) __attribute__((always_inline)) {
+                  const unsigned char* kt1, unsigned char* kl, unsigned char* vl)
+      __attribute__((always_inline)) {
     __builtin_amdgcn_s_waitcnt(wait_vm_lgkm0(4));
     __builtin_amdgcn_s_barrier();
     load_tile(t + 3, kl, vl);

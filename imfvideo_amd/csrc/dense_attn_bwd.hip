@@ -60,8 +60,8 @@ __device__ inline int first_query(int qlen, int klen, int causal) {
   return causal && qlen > klen ? qlen - klen : 0;
 }
 
-// delta of 256 rows of a head (8 lanes per row; HBM-bound: 16 us at B = 1, H = 8, L = 29,952), and for fp16 the largest row norm of
-// do; the workgroups behind them take the norms of v.
+// delta of 256 rows of a head (8 lanes per row; HBM-bound: 16 us at B = 1, H = 8, L = 29,952), and
+// for fp16 the largest row norm of do; the workgroups behind them take the norms of v.
 template <typename T16>
 __global__ __launch_bounds__(256) void dense_bwd_prep_kernel(DenseBwdArgs a, int64_t nq) {
   __shared__ float red[4];
@@ -550,8 +550,8 @@ extern "C" size_t sla2h_dense_attn_bwd_workspace_bytes(int dtype, int B, int H, 
 }
 
 extern "C" int sla2h_dense_attn_bwd(const void* q, const void* k, const void* v, const void* o,
-                                    const void* o_lo, const void* dout, const float* lse, const int64_t* strides,
-                                    const int32_t* q_lens, const int32_t* k_lens, int dtype,
+                                    const void* o_lo, const void* dout, const float* lse,
+                                    const int64_t* strides, const int32_t* q_lens, const int32_t* k_lens, int dtype,
                                     int B, int H, int Hkv, int64_t Lq, int64_t Lk, int causal,
                                     float scale, void* workspace, void* dq, void* dk, void* dv,
                                     void* stream) {
@@ -561,7 +561,8 @@ extern "C" int sla2h_dense_attn_bwd(const void* q, const void* k, const void* v,
   SLA2H_CHECK_ARG(sizes_ok(B, H, Hkv, Lq, Lk));
   SLA2H_CHECK_ARG(scale > 0.f && scale < 1e30f);
   SLA2H_CHECK_ARG(((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)o | (uintptr_t)dout |
-                   (uintptr_t)o_lo | (uintptr_t)workspace | (uintptr_t)dq | (uintptr_t)dk | (uintptr_t)dv) % 16 == 0);
+                   (uintptr_t)o_lo | (uintptr_t)workspace | (uintptr_t)dq | (uintptr_t)dk |
+                   (uintptr_t)dv) % 16 == 0);
   SLA2H_CHECK_ARG(((uintptr_t)lse | (uintptr_t)q_lens | (uintptr_t)k_lens) % 4 == 0);
   for (int i = 0; i < 24; ++i) SLA2H_CHECK_ARG(strides[i] >= 0 && strides[i] % 8 == 0);
   // rows apart from each other: the range check of a tile's load tells them by their offset

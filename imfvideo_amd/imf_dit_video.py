@@ -416,8 +416,9 @@ class SwiGLUMlp(nn.Module):
     or 16-bit inputs and weights), keep the input, gate and up in 8 bits for
     the backward and compute the hidden activation again (_Mlp8Function): per token
     in_features + 2 hidden_features bytes instead of 2 in_features + 6
-    hidden_features.  Otherwise (no gradients, CPU tensors, transforms of torch.func,
-    hooked submodules) the same MLP with unpacked activations."""
+    hidden_features.  An input tile with an infinity or a NaN makes the gradients that
+    read it NaN.  Otherwise (no gradients, CPU tensors, hooked or replaced
+    submodules) the layers run one by one, the gate by its own act8."""
 
     def __init__(self, in_features, hidden_features, weight_init_constant=1.0, situ_beta=1.0,
                  situ_linear_beta=None, act8=False):
@@ -444,7 +445,6 @@ class SwiGLUMlp(nn.Module):
         if dt not in half or any(w.dtype not in (half + (torch.float32,) if auto else (dt,))
                                  or w.device != x1.device for w in ws):
             return None
-        from . import ops
         plain = (all(_plain_module(m, _Linear) and m.bias is None
                      for m in (self.w1, self.w3, self.w2))
                  and _plain_module(self.act, SituAndMul) and self.act.act8
