@@ -154,14 +154,15 @@ struct WorkMap {
 inline WorkMap work_map(int64_t heads, int64_t tiles, bool even, bool last) {
   return WorkMap{(int)heads, (int)tiles, (int)(heads * tiles), even, last};
 }
-inline unsigned work_grid(const WorkMap& m) { return m.even ? 8u * ((m.n + 7) / 8) : (unsigned)m.n; }
-__device__ inline bool work_item(const WorkMap& m, int& head, int& tile) {
-  const int blk = blockIdx.x;
+inline unsigned work_grid(const WorkMap& m) { return 8u * ((m.n + 7) / 8); }
+__device__ inline bool work_item(const WorkMap& m, int blk, int& head, int& tile) {
   if (m.even) {
     const int i = (blk & 7) * ((m.n + 7) / 8) + (blk >> 3);
     if (i >= m.n) return false;
     head = i / m.tiles;
     tile = i - head * m.tiles;
+  } else if (blk >= m.n) {
+    return false;
   } else if (m.heads % 8 == 0) {
     const int per = m.heads / 8, i = blk >> 3;
     tile = i / per;

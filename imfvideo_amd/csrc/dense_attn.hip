@@ -149,7 +149,7 @@ __global__ __launch_bounds__(256, 2) void dense_fwd_kernel(DenseFwdArgs a) {
   __shared__ __align__(16) unsigned char k0[kTileB], k1[kTileB], k2[kTileB], k3[kTileB];
   __shared__ __align__(16) unsigned char v0[kTileB], v1[kTileB], v2[kTileB], v3[kTileB];
   int bh, qt;
-  if (!work_item(a.map, bh, qt)) return;
+  if (!work_item(a.map, blockIdx.x, bh, qt)) return;
   const int b = bh / a.H, hq = bh - b * a.H, hk = hq / a.rep;
   const int tid = threadIdx.x, l = tid & 63, h = l >> 5;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);

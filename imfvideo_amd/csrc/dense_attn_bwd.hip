@@ -4,8 +4,8 @@
 //   P_ij = exp(S_ij - lse_i),  delta_i = do_i . o_i,  dP = do v^T,  dS = P (dP - delta),
 //   dq = scale dS k,  dk = scale dS^T q,  dv = P^T do   (summed over a key head's queries).
 //
-// Three kernels: the rows' delta; dq with a workgroup per query block (keys streamed
-// through LDS); dk and dv with a workgroup per key block (queries streamed through LDS).
+// Two kernels: the rows' delta; then dq with a workgroup per query block (keys streamed
+// through LDS) beside dk and dv with a workgroup per key block (queries streamed through LDS).
 // Seven tile products instead of the five of one fused pass, but no sum goes through
 // atomics or memory: the result does not depend on the order of dispatch.
 //
@@ -50,8 +50,9 @@ struct DenseBwdArgs {
   float *gmax, *vmax;    // (B, H, nqb), (B, Hkv, nkb): largest row norms (fp16)
   int nqb, nkb;
   WorkMap dq_map, kv_map;  // tiles x splits of a query head, of a key head
+  int kv_blocks;           // workgroups of dk and dv, before those of dq
   int dq_splits, kv_splits;
-  float* part;
+  float *dq_part, *kv_part;
 };
 
 // Queries [first, qlen) see a key.
@@ -169,11 +170,11 @@ __device__ inline void store_part(float* p, const f32x16 (&x)[2], float f, int h
 // wave halve the LDS reads but spill at two waves per SIMD: the whole backward 6.04 ms against
 // 6.11 at B = 1, H = 8, L = 29,952, 2.96 against 2.93 causal.)
 template <typename T16>
-__global__ __launch_bounds__(256, 3) void dense_bwd_dq_kernel(DenseBwdArgs a) {
-  __shared__ __align__(16) unsigned char k0[kTileB], k1[kTileB], k2[kTileB];
-  __shared__ __align__(16) unsigned char v0[kTileB], v1[kTileB], v2[kTileB];
+__device__ __attribute__((always_inline)) inline void dq_rows(
+    const DenseBwdArgs& a, int blk, unsigned char* k0, unsigned char* k1, unsigned char* k2,
+    unsigned char* v0, unsigned char* v1, unsigned char* v2) {
   int bh, item;
-  if (!work_item(a.dq_map, bh, item)) return;
+  if (!work_item(a.dq_map, blk, bh, item)) return;
   const int qt = item / a.dq_splits, sp = item - qt * a.dq_splits;
   const int b = bh / a.H, hq = bh - b * a.H, hk = hq / a.rep;
   const int tid = threadIdx.x, l = tid & 63, h = l >> 5;
@@ -296,7 +297,7 @@ __global__ __launch_bounds__(256, 3) void dense_bwd_dq_kernel(DenseBwdArgs a) {
   if (a.dq_splits == 1)
     store_row<T16>(a.dq + b * a.dqb + hq * a.dqh + i * a.dql, acc, f, h, live);
   else
-    store_part(a.part + (((int64_t)sp * a.nbh + bh) * a.Lq + i) * kDD, acc, f, h, live);
+    store_part(a.dq_part + (((int64_t)sp * a.nbh + bh) * a.Lq + i) * kDD, acc, f, h, live);
 }
 
 // dk, dv: workgroup = 4 waves x 32 keys of one key head; the query rows of the heads that
@@ -307,12 +308,12 @@ __global__ __launch_bounds__(256, 3) void dense_bwd_dq_kernel(DenseBwdArgs a) {
 // four products (dq 2.7 ms, 1.02 of its three), the clock at the power limit; 64 keys per wave,
 // which halves the LDS reads but leaves one wave per SIMD: 3.8.
 template <typename T16, bool CAUSAL>
-__global__ __launch_bounds__(256, 2) void dense_bwd_dkdv_kernel(DenseBwdArgs a) {
-  __shared__ __align__(16) unsigned char q0_[kTileB], q1_[kTileB], q2_[kTileB], q3_[kTileB];
-  __shared__ __align__(16) unsigned char g0_[kTileB], g1_[kTileB], g2_[kTileB], g3_[kTileB];
-  __shared__ __align__(16) float s0_[2][64], s1_[2][64], s2_[2][64], s3_[2][64];
+__device__ __attribute__((always_inline)) inline void dkdv_rows(
+    const DenseBwdArgs& a, int blk, unsigned char* q0_, unsigned char* q1_, unsigned char* q2_,
+    unsigned char* q3_, unsigned char* g0_, unsigned char* g1_, unsigned char* g2_,
+    unsigned char* g3_, float (*s0_)[64], float (*s1_)[64], float (*s2_)[64], float (*s3_)[64]) {
   int bk, item;
-  if (!work_item(a.kv_map, bk, item)) return;
+  if (!work_item(a.kv_map, blk, bk, item)) return;
   const int ktile = item / a.kv_splits, sp = item - ktile * a.kv_splits;
   const int b = bk / a.Hkv, hk = bk - b * a.Hkv;
   const int tid = threadIdx.x, l = tid & 63, h = l >> 5;
@@ -464,10 +465,25 @@ __global__ __launch_bounds__(256, 2) void dense_bwd_dkdv_kernel(DenseBwdArgs a) 
     store_row<T16>(a.dk + b * a.dkb + hk * a.dkh + j * a.dkl, ak, fk, h, keep);
     store_row<T16>(a.dv + b * a.dvb + hk * a.dvh + j * a.dvl, av, fv, h, keep);
   } else {
-    float* d = a.part + (((int64_t)sp * a.nbk + bk) * a.Lk + j) * (2 * kDD);
+    float* d = a.kv_part + (((int64_t)sp * a.nbk + bk) * a.Lk + j) * (2 * kDD);
     store_part(d, ak, fk, h, keep);
     store_part(d + kDD, av, fv, h, keep);
   }
+}
+
+// Both in one launch, the workgroups of dk and dv first: neither reads what the other writes,
+// so the ones fill the places that the others' last round leaves (and a small call waits for
+// the longer of the two, not for both).
+template <typename T16, bool CAUSAL>
+__global__ __launch_bounds__(256, 2) void dense_bwd_kernel(DenseBwdArgs a) {
+  __shared__ __align__(16) unsigned char a0[kTileB], a1[kTileB], a2[kTileB], a3[kTileB];
+  __shared__ __align__(16) unsigned char b0[kTileB], b1[kTileB], b2[kTileB], b3[kTileB];
+  __shared__ __align__(16) float s0[2][64], s1[2][64], s2[2][64], s3[2][64];
+  const int blk = blockIdx.x;
+  if (blk < a.kv_blocks)
+    dkdv_rows<T16, CAUSAL>(a, blk, a0, a1, a2, a3, b0, b1, b2, b3, s0, s1, s2, s3);
+  else
+    dq_rows<T16>(a, blk - a.kv_blocks, a0, a1, a2, b0, b1, b2);
 }
 
 // Adds the parts of a row of W = 64 (dq) or 128 (dk | dv) channels in order.
@@ -496,7 +512,7 @@ struct BwdPlan {
   int64_t qtiles, dq_nwork, ktiles, kv_nwork;
   int dq_splits, kv_splits;
   int64_t nqb, nkb;
-  size_t stats, parts;  // floats
+  size_t stats, dq_parts, kv_parts;  // floats
 };
 
 // even: neither causal nor lengths.  Workgroups of uneven length balance by number: twice
@@ -520,9 +536,8 @@ BwdPlan bwd_plan(int dtype, int B, int H, int Hkv, int64_t Lq, int64_t Lk, bool 
   p.nkb = (Lk + kNormRows - 1) / kNormRows;
   p.stats = 2 * bh * Lq + (dtype == SLA2H_DTYPE_F16 ? bh * p.nqb + bk * p.nkb : 0);
   p.stats = (p.stats + 3) & ~(size_t)3;
-  const size_t pq = p.dq_splits > 1 ? (size_t)p.dq_splits * bh * Lq * kDD : 0;
-  const size_t pk = p.kv_splits > 1 ? (size_t)p.kv_splits * bk * Lk * 2 * kDD : 0;
-  p.parts = pq > pk ? pq : pk;
+  p.dq_parts = p.dq_splits > 1 ? (size_t)p.dq_splits * bh * Lq * kDD : 0;
+  p.kv_parts = p.kv_splits > 1 ? (size_t)p.kv_splits * bk * Lk * 2 * kDD : 0;
   return p;
 }
 
@@ -544,9 +559,10 @@ extern "C" size_t sla2h_dense_attn_bwd_workspace_bytes(int dtype, int B, int H, 
   size_t most = 0;
   for (bool even : {false, true}) {
     const BwdPlan p = bwd_plan(dtype, B, H, Hkv, Lq, Lk, even);
-    most = p.parts > most ? p.parts : most;
+    const size_t n = p.stats + p.dq_parts + p.kv_parts;
+    most = n > most ? n : most;
   }
-  return (bwd_plan(dtype, B, H, Hkv, Lq, Lk, true).stats + most) * 4;
+  return most * 4;
 }
 
 extern "C" int sla2h_dense_attn_bwd(const void* q, const void* k, const void* v, const void* o,
@@ -609,9 +625,11 @@ extern "C" int sla2h_dense_attn_bwd(const void* q, const void* k, const void* v,
   a.vmax = a.gmax + bh * p.nqb;
   a.nqb = (int)p.nqb;
   a.nkb = (int)p.nkb;
-  a.part = a.nlse + p.stats;
+  a.dq_part = a.nlse + p.stats;
+  a.kv_part = a.dq_part + p.dq_parts;
   a.dq_map = work_map(bh, p.qtiles * p.dq_splits, even, causal);
   a.kv_map = work_map(bk, p.ktiles * p.kv_splits, even, false);  // causal: the first keys' are longest
+  a.kv_blocks = dk ? (int)work_grid(a.kv_map) : 0;
   a.dq_splits = p.dq_splits;
   a.kv_splits = p.kv_splits;
   hipStream_t st = static_cast<hipStream_t>(stream);
@@ -620,26 +638,23 @@ extern "C" int sla2h_dense_attn_bwd(const void* q, const void* k, const void* v,
     int err;
     dense_bwd_prep_kernel<T16><<<(unsigned)(pq + pv), 256, 0, st>>>(a, pq);
     if ((err = (int)hipGetLastError())) return err;
-    if (dq) {
-      dense_bwd_dq_kernel<T16><<<work_grid(a.dq_map), 256, 0, st>>>(a);
-      if ((err = (int)hipGetLastError())) return err;
-      if (p.dq_splits > 1) {
-        dense_bwd_join_kernel<T16, kDD>
-            <<<(unsigned)((bh * Lq * kDD / 4 + 255) / 256), 256, 0, st>>>(
-                a.part, p.dq_splits, bh * Lq, Lq, H, a.dq, a.dqb, a.dqh, a.dql, nullptr, 0, 0, 0);
-        if ((err = (int)hipGetLastError())) return err;
-      }
-    }
-    if (!dk) return 0;
+    const unsigned grid = a.kv_blocks + (dq ? work_grid(a.dq_map) : 0);
     if (causal)
-      dense_bwd_dkdv_kernel<T16, true><<<work_grid(a.kv_map), 256, 0, st>>>(a);
+      dense_bwd_kernel<T16, true><<<grid, 256, 0, st>>>(a);
     else
-      dense_bwd_dkdv_kernel<T16, false><<<work_grid(a.kv_map), 256, 0, st>>>(a);
-    if ((err = (int)hipGetLastError()) || p.kv_splits == 1) return err;
-    dense_bwd_join_kernel<T16, 2 * kDD>
-        <<<(unsigned)((bk * Lk * 2 * kDD / 4 + 255) / 256), 256, 0, st>>>(
-            a.part, p.kv_splits, bk * Lk, Lk, Hkv, a.dk, a.dkb, a.dkh, a.dkl, a.dv, a.dvb, a.dvh,
-            a.dvl);
+      dense_bwd_kernel<T16, false><<<grid, 256, 0, st>>>(a);
+    if ((err = (int)hipGetLastError())) return err;
+    if (dq && p.dq_splits > 1) {
+      dense_bwd_join_kernel<T16, kDD>
+          <<<(unsigned)((bh * Lq * kDD / 4 + 255) / 256), 256, 0, st>>>(
+              a.dq_part, p.dq_splits, bh * Lq, Lq, H, a.dq, a.dqb, a.dqh, a.dql, nullptr, 0, 0, 0);
+      if ((err = (int)hipGetLastError())) return err;
+    }
+    if (dk && p.kv_splits > 1)
+      dense_bwd_join_kernel<T16, 2 * kDD>
+          <<<(unsigned)((bk * Lk * 2 * kDD / 4 + 255) / 256), 256, 0, st>>>(
+              a.kv_part, p.kv_splits, bk * Lk, Lk, Hkv, a.dk, a.dkb, a.dkh, a.dkl, a.dv, a.dvb,
+              a.dvh, a.dvl);
     return (int)hipGetLastError();
   };
   return dtype == SLA2H_DTYPE_BF16 ? go(BF16{}) : go(F16{});
