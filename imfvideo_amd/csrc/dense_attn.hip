@@ -46,10 +46,10 @@ struct DenseFwdArgs {
   float c;  // scale * log2(e)
   WorkMap map;
   int qtiles, nwork;  // split form: query tiles of a key head, workgroups
-  // split form
-  float* part;   // [split][B * H * Lq][64] unnormalised sums
-  float2* ml;    // [split][B * H * Lq] (m, l)
-  int splits, units;  // 32-key units of a split
+  // ranges of keys
+  float* part;   // [range][B * H * Lq][64] unnormalised sums
+  float2* ml;    // [range][B * H * Lq] (m, l)
+  int splits, units;  // split form: 32-key units of a range
   int64_t nrows;      // B * H * Lq
 };
 
@@ -148,8 +148,9 @@ template <typename T16, int NQ, bool FINE>
 __global__ __launch_bounds__(256, 2) void dense_fwd_kernel(DenseFwdArgs a) {
   __shared__ __align__(16) unsigned char k0[kTileB], k1[kTileB], k2[kTileB], k3[kTileB];
   __shared__ __align__(16) unsigned char v0[kTileB], v1[kTileB], v2[kTileB], v3[kTileB];
-  int bh, qt;
-  if (!work_item(a.map, blockIdx.x, bh, qt)) return;
+  int bh, item;
+  if (!work_item(a.map, blockIdx.x, bh, item)) return;
+  const int qt = item / a.splits, sp = item - qt * a.splits;
   const int b = bh / a.H, hq = bh - b * a.H, hk = hq / a.rep;
   const int tid = threadIdx.x, l = tid & 63, h = l >> 5;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -160,7 +161,9 @@ __global__ __launch_bounds__(256, 2) void dense_fwd_kernel(DenseFwdArgs a) {
   const int qw = q0 + w * (32 * NQ);        // ... of the wave
   const int qend = min(q0 + 128 * NQ, qlen);
   const int kmax = qend > q0 ? key_limit(qend - 1, qlen, klen, a.causal) : 0;
-  const int nt = (kmax + kTileRows - 1) / kTileRows;
+  const int ntile = (kmax + kTileRows - 1) / kTileRows;
+  const int per = (ntile + a.splits - 1) / a.splits;
+  const int t0 = sp * per, nt = min(ntile, t0 + per);  // this range's tiles
 
   const uint16_t* kp = a.k + b * a.kb + hk * a.kh;
   const uint16_t* vp = a.v + b * a.vb + hk * a.vh;
@@ -280,7 +283,7 @@ __global__ __launch_bounds__(256, 2) void dense_fwd_kernel(DenseFwdArgs a) {
       }
     }
   };
-  // Tile t lives in slot t % 4; tiles past the last one are empty (zeros).  At the top of
+  // Tile t0 + i lives in slot i % 4; tiles past the sequence are empty (zeros).  At the top of
   // tile t the tiles up to t + 1 have landed and tile t - 1 is read.
   auto tile = [&](int t, const unsigned char* kt, const unsigned char* vt,
                   const unsigned char* kt1, unsigned char* kl, unsigned char* vl)
@@ -292,17 +295,17 @@ __global__ __launch_bounds__(256, 2) void dense_fwd_kernel(DenseFwdArgs a) {
     step(t, 0, kt, vt, kt1);
     step(t, 1, kt, vt, kt1);
   };
-  load_tile(0, k0, v0);
-  load_tile(1, k1, v1);
-  load_tile(2, k2, v2);
+  load_tile(t0, k0, v0);
+  load_tile(t0 + 1, k1, v1);
+  load_tile(t0 + 2, k2, v2);
   __builtin_amdgcn_s_waitcnt(wait_vm_lgkm0(8));
   __builtin_amdgcn_s_barrier();
   read_k(k0, 0);
   scores(0);
-  mask(0, 0);
+  mask(0, t0 * kTileRows);
   raise(0);
   read_k(k0, 1);
-  for (int t = 0; t < nt; t += 4) {
+  for (int t = t0; t < nt; t += 4) {
     tile(t, k0, v0, k1, k3, v3);
     if (t + 1 >= nt) break;
     tile(t + 1, k1, v1, k2, k0, v0);
@@ -319,6 +322,18 @@ __global__ __launch_bounds__(256, 2) void dense_fwd_kernel(DenseFwdArgs a) {
     const int i = qw + 32 * n + (l & 31);
     if (i >= a.Lq) continue;
     const float ls = swap32_sum(lsum[n]);
+    if (a.splits > 1) {
+      const int64_t flat = sp * a.nrows + (int64_t)bh * a.Lq + i;
+#pragma unroll
+      for (int mb = 0; mb < 2; ++mb)
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+          *reinterpret_cast<f32x4*>(a.part + flat * kDD + 32 * mb + 8 * g + 4 * h) =
+              f32x4{acc[n][mb][4 * g], acc[n][mb][4 * g + 1], acc[n][mb][4 * g + 2],
+                    acc[n][mb][4 * g + 3]};
+      if (h == 0) a.ml[flat] = make_float2(m[n], ls);
+      continue;
+    }
     const float inv = 1.f / ls;  // a row whose scores are all -inf is NaN
 #pragma unroll
     for (int mb = 0; mb < 2; ++mb)
@@ -556,11 +571,11 @@ __global__ __launch_bounds__(256) void dense_join_kernel(DenseFwdArgs a) {
     a.lse[flat] = some ? (mm - Range<T16>::shift + __log2f(ll)) * kLn2 : -__builtin_inff();
 }
 
-// The form of a call: query blocks of 256 or 128 rows with all keys, or the split form.
+// The form of a call: query blocks of 256 or 128 rows, or of 32 rows of a key head's group.
 struct FwdPlan {
-  int nq;  // 2, 1: dense_fwd_kernel<NQ>; 0: split form
+  int nq;  // 2, 1: dense_fwd_kernel<NQ>; 0: dense_fwd_split_kernel
   int64_t qtiles, nwork;
-  int splits;
+  int splits;  // ranges of keys
   int64_t units;
 };
 
@@ -581,6 +596,15 @@ FwdPlan fwd_plan(int B, int H, int Hkv, int64_t Lq, int64_t Lk, bool even) {
   p.qtiles = (Lq + 127) / 128;
   p.nwork = bh * p.qtiles;
   if (p.nwork >= 256) return p;
+  // ... with ranges of keys where blocks of 32 rows would read all keys over and over; us, so and
+  // in blocks of 32 rows: 77 queries over 29,952 keys, H = 8, 23 : 39; 300 48 : 91; 2,000, H = 1, 32 : 50; L =
+  // 1,500, H = 4 23 : 24; but L = 2,048, H = 8 (128 workgroups) 41 : 19, where the parts weigh more
+  if (p.nwork <= 64 && Lq > 48 && Lk >= 1024) {
+    const int64_t tiles = (Lk + kTileRows - 1) / kTileRows, most = tiles / 4;
+    const int64_t s = (512 + p.nwork - 1) / p.nwork;
+    p.splits = (int)(s < most ? s : most);
+    return p;
+  }
   p.nq = 0;
   p.qtiles = ((H / Hkv) * Lq + 31) / 32;
   const int64_t blocks = (int64_t)B * Hkv * p.qtiles, units = (Lk + 31) / 32;
@@ -657,7 +681,7 @@ extern "C" int sla2h_dense_attn_fwd(const void* q, const void* k, const void* v,
   a.c = scale * kLog2e;
   a.qtiles = (int)p.qtiles;
   a.nwork = (int)p.nwork;
-  a.map = work_map((int64_t)B * H, p.qtiles, even, causal);
+  a.map = work_map((int64_t)B * H, p.qtiles * (p.nq ? p.splits : 1), even, causal);
   a.splits = p.splits;
   a.units = (int)p.units;
   a.nrows = (int64_t)B * H * Lq;

@@ -41,11 +41,12 @@ def check_all(got, want, case):
 
 
 # B, H, Hkv, Lq, Lk: one row and one key; edges of the 32- and 64-row tiles; odd ones;
-# few queries over many keys (split keys) and many over few (split queries); enough
+# few queries over many keys (split keys, in both forms) and many over few (split queries); enough
 # heads for the 128- and the 256-row forms; grouped key heads
 SHAPES = [(1, 1, 1, 1, 1), (2, 2, 1, 1, 700), (1, 2, 2, 31, 33), (1, 2, 2, 64, 64),
           (2, 3, 3, 65, 63), (1, 4, 4, 274, 274), (2, 4, 2, 7, 1500), (1, 2, 1, 1333, 5),
-          (3, 4, 1, 129, 130), (2, 64, 64, 200, 70), (2, 64, 32, 300, 97), (1, 128, 32, 257, 65)]
+          (1, 2, 2, 70, 1500), (2, 4, 2, 200, 2100), (3, 4, 1, 129, 130), (2, 64, 64, 200, 70),
+          (2, 64, 32, 300, 97), (1, 128, 32, 257, 65)]
 
 
 @pytest.mark.parametrize("dt", DTYPES)
