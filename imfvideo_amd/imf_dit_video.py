@@ -121,6 +121,16 @@ def sdpa_math_attention(q, k, v):
     return o.transpose(1, 2)
 
 
+def _once(backward):
+    """once_differentiable, without its grad-mode bookkeeping in the usual backward (no
+    create_graph), where there is nothing to mark."""
+    marked = once_differentiable(backward)
+
+    def run(ctx, *grads):
+        return (marked if torch.is_grad_enabled() else backward)(ctx, *grads)
+    return run
+
+
 def _no_batched(d, what):
     """RuntimeError for gradients under vmap: the kernels take one at a time."""
     if ops.batched(d):
@@ -141,7 +151,7 @@ class _DenseAttentionFunction(torch.autograd.Function):
         return o
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, do):
         _no_batched(do, "dense_attention")
         q, k, v, o, lse, o_lo, q_lens, k_lens = ctx.saved_tensors
@@ -314,7 +324,7 @@ class _Situ8Function(torch.autograd.Function):
         return h
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, dh):
         _no_batched(dh, "SituAndMul(act8=True)")
         return (*ops.situ8_saved_bwd(dh, *ctx.saved_tensors, *ctx.args), None, None)
@@ -388,7 +398,7 @@ class _Mlp8Function(torch.autograd.Function):
         return F.linear(h, h2)
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, dy):
         _no_batched(dy, "SwiGLUMlp(act8=True)")
         h1, h3, h2, codes, scales, kept = ctx.saved_tensors
