@@ -33,7 +33,7 @@ struct Shift<F16> {
   static constexpr float p = 15.f;
 };
 
-constexpr int kNormRows = 256;  // rows of a partial maximum of the norms
+constexpr int kNormRows = 64;  // rows of a partial maximum of the norms
 
 struct DenseBwdArgs {
   const uint16_t *q, *k, *v, *o, *o_lo, *dout;
@@ -61,7 +61,7 @@ __device__ inline int first_query(int qlen, int klen, int causal) {
   return causal && qlen > klen ? qlen - klen : 0;
 }
 
-// delta of 256 rows of a head (8 lanes per row; HBM-bound: 16 us at B = 1, H = 8, L = 29,952), and
+// delta of 64 rows of a head (8 lanes per row; HBM-bound: 16 us at B = 1, H = 8, L = 29,952), and
 // for fp16 the largest row norm of do; the workgroups behind them take the norms of v.
 template <typename T16>
 __global__ __launch_bounds__(256) void dense_bwd_prep_kernel(DenseBwdArgs a, int64_t nq) {
@@ -76,7 +76,7 @@ __global__ __launch_bounds__(256) void dense_bwd_prep_kernel(DenseBwdArgs a, int
   const int len = is_v ? klen : qlen;
   const int first = is_v ? 0 : first_query(qlen, klen, a.causal);
   float top = 0.f;
-#pragma unroll 2
+#pragma unroll
   for (int j = 0; j < kNormRows / 32; ++j) {
     const int64_t i = (int64_t)t * kNormRows + 32 * j + (tid >> 3);
     float dot = 0.f, nrm = 0.f;
@@ -131,7 +131,9 @@ __device__ inline float ds_scale(const DenseBwdArgs& a, int b, int hk) {
   const float* g = a.gmax + ((int64_t)b * a.H + (int64_t)hk * a.rep) * a.nqb;
   const float* v = a.vmax + ((int64_t)b * a.Hkv + hk) * a.nkb;
   float mg = 0.f, mv = 0.f;
+#pragma unroll 8
   for (int64_t i = l; i < ng; i += 64) mg = fmaxf(mg, g[i]);
+#pragma unroll 8
   for (int i = l; i < a.nkb; i += 64) mv = fmaxf(mv, v[i]);
   const float bound = 2.f * wave_max(mg) * wave_max(mv);
   if (!(bound > 0.f) || !(bound < 1e38f)) return 1.f;
