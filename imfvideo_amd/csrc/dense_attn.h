@@ -119,6 +119,17 @@ __device__ inline u32x4 pack_step(const f32x16& p, int s) {
                pack_pair<T16>(p[8 * s + 6], p[8 * s + 7])};
 }
 
+// What that rounding lost, rounded to 16 bits itself (hi = pack_step(p, s)).
+template <typename T16>
+__device__ inline u32x4 lost_step(const f32x16& p, int s, const u32x4& hi) {
+  u32x4 y;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    y[i] = pack_pair<T16>(p[8 * s + 2 * i] - T16::to_f32((uint16_t)(hi[i] & 0xffff)),
+                          p[8 * s + 2 * i + 1] - T16::to_f32((uint16_t)(hi[i] >> 16)));
+  return y;
+}
+
 __device__ inline float swap32_max(float v) {
   const float2 a = swap32(v);
   return fmaxf(a.x, a.y);

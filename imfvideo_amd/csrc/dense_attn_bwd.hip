@@ -33,6 +33,13 @@ struct Shift<F16> {
   static constexpr float p = 15.f;
 };
 
+// FINE: waves of dq whose rows see at most kFineKeys keys or belong to at most kFineRows queries,
+// and workgroups of dk and dv that see at most kFineRows rows, add what the rounding of dS (and
+// P) lost with a second product.  Few terms do not average the rounding out, and a small call's
+// time is not its products: bf16, the 2-norm of dq's error is 1.7e-3 (its own rounding) instead of
+// 2.4e-3 to 2.8e-3.  Backward, us: two clips of 274, H = 8, 22.3 : 22.5; 8,192 queries x 77 keys
+// 41.8 : 43.7; L = 2,048 47.3 : 53.2; 8,192 x 2,048 157 : 174; causal L = 29,952 2,970 : 3,017.
+constexpr int kFineKeys = 2048, kFineRows = 512;
 constexpr int kNormRows = 64;  // rows of a partial maximum of the norms
 
 struct DenseBwdArgs {
@@ -171,7 +178,7 @@ __device__ inline void store_part(float* p, const f32x16 (&x)[2], float f, int h
 // LDS slots.  dQ^T += K^T dS^T with dS^T straight from the score tile's registers.  (64 rows per
 // wave halve the LDS reads but spill at two waves per SIMD: the whole backward 6.04 ms against
 // 6.11 at B = 1, H = 8, L = 29,952, 2.96 against 2.93 causal.)
-template <typename T16>
+template <typename T16, bool FINE>
 __device__ __attribute__((always_inline)) inline void dq_rows(
     const DenseBwdArgs& a, int blk, unsigned char* k0, unsigned char* k1, unsigned char* k2,
     unsigned char* v0, unsigned char* v1, unsigned char* v2) {
@@ -233,6 +240,7 @@ __device__ __attribute__((always_inline)) inline void dq_rows(
   const int wlast = min(qw + 32, qlen) - 1;
   const int wany = wlast >= qw ? limit(wlast) : 0;
   const int wall = wlast >= qw ? limit(qw) : 0;
+  const bool fine = FINE && (wany <= kFineKeys || qlen <= kFineRows);
 
   f32x16 acc[2] = {zero16(), zero16()};
   auto part = [&](auto masked, int base, const unsigned char* kt, const unsigned char* vt)
@@ -258,9 +266,17 @@ __device__ __attribute__((always_inline)) inline void dq_rows(
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
         const u32x4 ds = pack_step<T16>(dp, s);
+        u32x4 kf[2];
 #pragma unroll
-        for (int mb = 0; mb < 2; ++mb)
-          acc[mb] = mfma_32x32x16<T16>(col_frag(kt, 32 * kb + 16 * s, mb, lo), ds, acc[mb]);
+        for (int mb = 0; mb < 2; ++mb) {
+          kf[mb] = col_frag(kt, 32 * kb + 16 * s, mb, lo);
+          acc[mb] = mfma_32x32x16<T16>(kf[mb], ds, acc[mb]);
+        }
+        if (FINE && fine) {
+          const u32x4 lost = lost_step<T16>(dp, s, ds);
+#pragma unroll
+          for (int mb = 0; mb < 2; ++mb) acc[mb] = mfma_32x32x16<T16>(kf[mb], lost, acc[mb]);
+        }
       }
     }
   };
@@ -295,7 +311,10 @@ __device__ __attribute__((always_inline)) inline void dq_rows(
   __builtin_amdgcn_s_waitcnt(wait_vm_lgkm0(0));
 
   if (i >= a.Lq) return;
-  const float f = Shift<T16>::scaled ? a.scale * (1.f / 32768.f) / mul : a.scale;
+  // (the softmax of one key is constant: its dS is the rounding of dP - delta)
+  const float f = lim == 1             ? 0.f
+                  : Shift<T16>::scaled ? a.scale * (1.f / 32768.f) / mul
+                                       : a.scale;
   if (a.dq_splits == 1)
     store_row<T16>(a.dq + b * a.dqb + hq * a.dqh + i * a.dql, acc, f, h, live);
   else
@@ -309,7 +328,7 @@ __device__ __attribute__((always_inline)) inline void dq_rows(
 // under this step's exponentials.  B = 1, H = 8, L = 29,952, bf16: 3.46 ms, 1.06 PFLOP/s of its
 // four products (dq 2.7 ms, 1.02 of its three), the clock at the power limit; 64 keys per wave,
 // which halves the LDS reads but leaves one wave per SIMD: 3.8.
-template <typename T16, bool CAUSAL>
+template <typename T16, bool CAUSAL, bool FINE>
 __device__ __attribute__((always_inline)) inline void dkdv_rows(
     const DenseBwdArgs& a, int blk, unsigned char* q0_, unsigned char* q1_, unsigned char* q2_,
     unsigned char* q3_, unsigned char* g0_, unsigned char* g1_, unsigned char* g2_,
@@ -330,6 +349,7 @@ __device__ __attribute__((always_inline)) inline void dkdv_rows(
   if (CAUSAL) first = max(first, key0 - off);
   const int nq = key0 < klen && first < qlen ? (qlen - first + kTileRows - 1) / kTileRows : 0;
   const int total = nq * a.rep;  // (head, query tile) pairs
+  const bool fine = FINE && total <= kFineRows / kTileRows;
   const int per = (total + a.kv_splits - 1) / a.kv_splits;
   const int u0 = sp * per, u1 = min(total, u0 + per);
 
@@ -416,10 +436,21 @@ __device__ __attribute__((always_inline)) inline void dkdv_rows(
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
       const u32x4 pp = pack_step<T16>(p, s), dd = pack_step<T16>(d, s);
+      u32x4 gf[2], qf[2];
 #pragma unroll
       for (int mb = 0; mb < 2; ++mb) {
-        av[mb] = mfma_32x32x16<T16>(col_frag(gt, 32 * qb + 16 * s, mb, lo), pp, av[mb]);
-        ak[mb] = mfma_32x32x16<T16>(col_frag(qt, 32 * qb + 16 * s, mb, lo), dd, ak[mb]);
+        gf[mb] = col_frag(gt, 32 * qb + 16 * s, mb, lo);
+        av[mb] = mfma_32x32x16<T16>(gf[mb], pp, av[mb]);
+        qf[mb] = col_frag(qt, 32 * qb + 16 * s, mb, lo);
+        ak[mb] = mfma_32x32x16<T16>(qf[mb], dd, ak[mb]);
+      }
+      if (FINE && fine) {
+        const u32x4 pl = lost_step<T16>(p, s, pp), dl = lost_step<T16>(d, s, dd);
+#pragma unroll
+        for (int mb = 0; mb < 2; ++mb) {
+          av[mb] = mfma_32x32x16<T16>(gf[mb], pl, av[mb]);
+          ak[mb] = mfma_32x32x16<T16>(qf[mb], dl, ak[mb]);
+        }
       }
     }
   };
@@ -459,7 +490,9 @@ __device__ __attribute__((always_inline)) inline void dkdv_rows(
   __builtin_amdgcn_s_waitcnt(wait_vm_lgkm0(0));
 
   const float fv = Shift<T16>::scaled ? 1.f / 32768.f : 1.f;
-  const float fk = Shift<T16>::scaled ? a.scale * (1.f / 32768.f) / mul : a.scale;
+  const float fk = klen == 1            ? 0.f
+                   : Shift<T16>::scaled ? a.scale * (1.f / 32768.f) / mul
+                                        : a.scale;
   const int j = kw + (l & 31);
   if (j >= a.Lk) return;
   const bool keep = j < klen;
@@ -476,16 +509,16 @@ __device__ __attribute__((always_inline)) inline void dkdv_rows(
 // Both in one launch, the workgroups of dk and dv first: neither reads what the other writes,
 // so the ones fill the places that the others' last round leaves (and a small call waits for
 // the longer of the two, not for both).
-template <typename T16, bool CAUSAL>
+template <typename T16, bool CAUSAL, bool FINE>
 __global__ __launch_bounds__(256, 2) void dense_bwd_kernel(DenseBwdArgs a) {
   __shared__ __align__(16) unsigned char a0[kTileB], a1[kTileB], a2[kTileB], a3[kTileB];
   __shared__ __align__(16) unsigned char b0[kTileB], b1[kTileB], b2[kTileB], b3[kTileB];
   __shared__ __align__(16) float s0[2][64], s1[2][64], s2[2][64], s3[2][64];
   const int blk = blockIdx.x;
   if (blk < a.kv_blocks)
-    dkdv_rows<T16, CAUSAL>(a, blk, a0, a1, a2, a3, b0, b1, b2, b3, s0, s1, s2, s3);
+    dkdv_rows<T16, CAUSAL, FINE>(a, blk, a0, a1, a2, a3, b0, b1, b2, b3, s0, s1, s2, s3);
   else
-    dq_rows<T16>(a, blk - a.kv_blocks, a0, a1, a2, b0, b1, b2);
+    dq_rows<T16, FINE>(a, blk - a.kv_blocks, a0, a1, a2, b0, b1, b2);
 }
 
 // Adds the parts of a row of W = 64 (dq) or 128 (dk | dv) channels in order.
@@ -644,9 +677,11 @@ extern "C" int sla2h_dense_attn_bwd(const void* q, const void* k, const void* v,
     if ((err = (int)hipGetLastError())) return err;
     const unsigned grid = a.kv_blocks + (dq ? work_grid(a.dq_map) : 0);
     if (causal)
-      dense_bwd_kernel<T16, true><<<grid, 256, 0, st>>>(a);
+      dense_bwd_kernel<T16, true, true><<<grid, 256, 0, st>>>(a);
+    else if (Lk <= kFineKeys || Lq <= kFineRows)
+      dense_bwd_kernel<T16, false, true><<<grid, 256, 0, st>>>(a);
     else
-      dense_bwd_kernel<T16, false><<<grid, 256, 0, st>>>(a);
+      dense_bwd_kernel<T16, false, false><<<grid, 256, 0, st>>>(a);
     if ((err = (int)hipGetLastError())) return err;
     if (dq && p.dq_splits > 1) {
       dense_bwd_join_kernel<T16, kDD>

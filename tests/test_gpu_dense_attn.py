@@ -87,6 +87,50 @@ def test_what_the_rounding_lost(shape, dt):
             + torch.finfo(dt).smallest_normal).all()
 
 
+@pytest.mark.parametrize("shape", [(1, 2, 2, 70, 90), (2, 4, 2, 7, 500), (1, 2, 1, 250, 33),
+                                   (1, 128, 128, 100, 70)])
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("dt", DTYPES)
+def test_small_gradients_keep_what_rounding_loses(shape, causal, dt):
+    """Few keys and rows: P and dS enter their products with the half that rounding them
+    lost, so an element is off by its own rounding u |x| and second-order terms: dS's
+    u^2 |dS|, and through delta P's u^2 P |v| and the u^2 |o| of the output's second half,
+    each at most u^2 P mag with mag = |dout| . |v_j| + |dout| . P |v|; fp32 arithmetic T32 of
+    the same sums for S, dP and delta."""
+    q, k, v, do = inputs(7 + sum(shape), *shape, dt)
+    B, H, Hkv, Lq, Lk = shape
+    rep = H // Hkv
+    got = run(*[t.cuda() for t in (q, k, v, do)], True, causal=causal)
+    torch.cuda.synchronize()
+    want = R.attention(q, k, v, causal, do=do)
+    u, tiny = torch.finfo(dt).eps / 2, torch.finfo(dt).smallest_normal * torch.finfo(dt).eps
+    see = R.visible(B, Lq, Lk, causal, None, None)[:, None]
+    K, V = (t.double().repeat_interleave(rep, 1) for t in (k, v))
+    s = (q.double() @ K.transpose(-1, -2) / 8).masked_fill(~see, float("-inf"))
+    P = torch.softmax(s, -1).nan_to_num(0.0)
+    g = do.double().abs()
+    mag = g @ V.abs().transpose(-1, -2) + (g * (P @ V.abs())).sum(-1, keepdim=True)
+    E = (4 * u * u + 3 * R.T32) * P * mag + 2.0 ** -36 * see * mag.amax((-1, -2), keepdim=True)
+    heads = lambda t: t.reshape(B, Hkv, rep, Lk, 64).sum(2)
+    more = dict(dq=E @ K.abs() / 8, dk=heads(E.transpose(-1, -2) @ q.double().abs()) / 8,
+                dv=heads(((2 * u * u + R.T32) * P + 2.0 ** -36 * see).transpose(-1, -2) @ g))
+    for n in more:
+        val = want[n][0]
+        R.check(got[n], (val, u * val.abs() + more[n] + tiny), (shape, causal, dt, n))
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+def test_one_key_has_no_score_gradient(dt):
+    """The softmax of one key is 1 whatever its score: dq and dk are zero."""
+    q, k, v, do = [t.cuda() for t in inputs(3, 2, 4, 2, 37, 5, dt)]
+    lens = torch.tensor([1, 5], device="cuda")
+    got = run(q, k, v, do, k_lens=lens)
+    assert not got["dq"][0].any() and not got["dk"][0].any()
+    assert got["dq"][1].any() and got["dk"][1].any()
+    got = run(q, k[:, :, :1], v[:, :, :1], do, causal=True)
+    assert not got["dq"].any() and not got["dk"].any() and got["dv"].any()
+
+
 @pytest.mark.parametrize("dt", DTYPES)
 def test_rows_behind_a_sequence_are_not_used(dt):
     """NaN, infinities and the type's lowest value behind the sequences change nothing,
