@@ -33,13 +33,15 @@ struct Shift<F16> {
   static constexpr float p = 15.f;
 };
 
-// FINE: waves of dq whose rows see at most kFineKeys keys or belong to at most kFineRows queries,
-// and workgroups of dk and dv that see at most kFineRows rows, add what the rounding of dS (and
-// P) lost with a second product.  Few terms do not average the rounding out, and a small call's
-// time is not its products: bf16, the 2-norm of dq's error is 1.7e-3 (its own rounding) instead of
-// 2.4e-3 to 2.8e-3.  Backward, us: two clips of 274, H = 8, 22.3 : 22.5; 8,192 queries x 77 keys
-// 41.8 : 43.7; L = 2,048 47.3 : 53.2; 8,192 x 2,048 157 : 174; causal L = 29,952 2,970 : 3,017.
-constexpr int kFineKeys = 2048, kFineRows = 512;
+// FINE: add what the rounding of P and dS lost with a second product.  Small sums do not
+// average the rounding out, and a small call's time is not its products.  dq: sequences of at
+// most kFineKeys keys or kFineRows queries, and causal waves that see at most kFineRows keys; dk
+// and dv: workgroups that see at most kFineRows rows, and sequences of at most 32 keys (one wave
+// of a workgroup).  bf16, 2-norm of dq's error: 1.7e-3 (its own rounding) to 1.8e-3 instead of
+// 2.4e-3 to 2.8e-3.  Backward, us, without : with, H = 8: two clips of 274 tokens 22.3 : 22.5; two of
+// 8,192 queries x 77 keys 41.8 : 43.5; L = 2,048 47 : 53, 4,096 127 : 144; causal L = 4,096
+// 109 : 122, B = 3 clips of up to 4,159 152 : 159, L = 29,952 2,970 : 3,017.
+constexpr int kFineKeys = 4096, kFineRows = 512;
 constexpr int kNormRows = 64;  // rows of a partial maximum of the norms
 
 struct DenseBwdArgs {
@@ -240,7 +242,7 @@ __device__ __attribute__((always_inline)) inline void dq_rows(
   const int wlast = min(qw + 32, qlen) - 1;
   const int wany = wlast >= qw ? limit(wlast) : 0;
   const int wall = wlast >= qw ? limit(qw) : 0;
-  const bool fine = FINE && (wany <= kFineKeys || qlen <= kFineRows);
+  const bool fine = FINE && (klen <= kFineKeys || wany <= kFineRows || qlen <= kFineRows);
 
   f32x16 acc[2] = {zero16(), zero16()};
   auto part = [&](auto masked, int base, const unsigned char* kt, const unsigned char* vt)
@@ -349,7 +351,7 @@ __device__ __attribute__((always_inline)) inline void dkdv_rows(
   if (CAUSAL) first = max(first, key0 - off);
   const int nq = key0 < klen && first < qlen ? (qlen - first + kTileRows - 1) / kTileRows : 0;
   const int total = nq * a.rep;  // (head, query tile) pairs
-  const bool fine = FINE && total <= kFineRows / kTileRows;
+  const bool fine = FINE && (total <= kFineRows / kTileRows || klen <= 32);
   const int per = (total + a.kv_splits - 1) / a.kv_splits;
   const int u0 = sp * per, u1 = min(total, u0 + per);
 
