@@ -327,9 +327,9 @@ __device__ __attribute__((always_inline)) inline void dq_rows(
 // read it are streamed through LDS in tiles of 64, three tiles ahead into four slots, with
 // their -lse and -delta, which start the accumulators of S and dP.  The step of 32 rows is
 // software-pipelined as in the forward: S and dP of the next step run on the matrix cores
-// under this step's exponentials.  B = 1, H = 8, L = 29,952, bf16: 3.46 ms, 1.06 PFLOP/s of its
-// four products (dq 2.7 ms, 1.02 of its three), the clock at the power limit; 64 keys per wave,
-// which halves the LDS reads but leaves one wave per SIMD: 3.8.
+// under this step's exponentials.  B = 1, H = 8, L = 29,952, bf16, launched alone: 3.46 ms, 1.06
+// PFLOP/s of its four products (dq 2.7 ms, 1.02 of its three), the clock at the power limit;
+// 64 keys per wave, which halves the LDS reads but leaves one wave per SIMD: 3.8.
 template <typename T16, bool CAUSAL, bool FINE>
 __device__ __attribute__((always_inline)) inline void dkdv_rows(
     const DenseBwdArgs& a, int blk, unsigned char* q0_, unsigned char* q1_, unsigned char* q2_,
