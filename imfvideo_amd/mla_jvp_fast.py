@@ -18,10 +18,13 @@ Shapes: h, dh (b, l, d) fp32; H heads, q/kv latent ranks dq/dc, nope / rope /
 value head dims dn = dr = 32, dv = 64.
 """
 
+from functools import partial
+
 import torch
 import torch.nn.functional as F
 
 from . import _lib, ops
+from .imf_dit_video import dense_attention
 from .sla2_cube_qat import sla2_cube_qat_jvp_fused
 from .sla2_mla_jvp import _sla2_mla_jvp, route_blocks, sla2_mla_jvp
 
@@ -191,6 +194,24 @@ def _mlp_sublayer_proj(h, dh, p, w16, eps):
     return F.linear(act, w16["w_down"]).view(2 * B, S, D)
 
 
+def _check_dense_impl(impl):
+    """ValueError for a functools.partial of dense_attention that is another function than
+    the JVP's dense branch (every token sees every token, scale 64^-1/2)."""
+    bound = {}
+    while isinstance(impl, partial):
+        bound = {**impl.keywords, **bound}
+        impl = impl.func
+    if impl is not dense_attention:
+        return
+    other = ["causal"] if bound.get("causal") else []
+    other += [n for n in ("q_lens", "k_lens") if bound.get(n) is not None]
+    if bound.get("scale") not in (None, 64 ** -0.5):
+        other.append("scale")
+    if other:
+        raise ValueError("pack_block: the fast JVP has no form of dense_attention with "
+                         + ", ".join(other))
+
+
 def pack_block(block, tile_major=False):
     """(params, fp16 weight cache) of one TransformerBlock for the fast JVP
     (the inner pack of models/mla_jvp_fast.py:252-300): the block parameters,
@@ -200,7 +221,9 @@ def pack_block(block, tile_major=False):
       cube (SLA2CubeQATAttentionImpl): alpha = sigmoid(alpha_logit) (H, Mb),
         proj_q, proj_k, topk, Np, E, P (prefix tokens), perm, inv and
         pre_permuted = tile_major (the model keeps tokens tile-major);
-      sla2 (SLA2AttentionImpl): alpha (H, Mb), the router projections, topk, bq, bk.
+      sla2 (SLA2AttentionImpl): alpha (H, Mb), the router projections, topk, bq, bk;
+      any other impl is taken for dense softmax attention of every token to every token at
+      scale 64^-1/2 (a partial of dense_attention that is not raises ValueError).
     Rebuild after every optimizer step (the weights change)."""
     p = mla_params_from_block(block)
     for name in ("attn_res_norm", "mlp_res_norm"):
@@ -227,6 +250,8 @@ def pack_block(block, tile_major=False):
             "proj_q": sl.router.proj_q.weight.detach(), "proj_k": sl.router.proj_k.weight.detach(),
             "topk": impl.topk, "bq": impl.bq, "bk": impl.bk,
         }
+    else:
+        _check_dense_impl(impl)
     return p, mla_fp16_cache(p)
 
 

@@ -1,0 +1,39 @@
+"""What dense_attention and the modules around it may be asked for, on the host: calls that the
+kernels cannot answer are refused, and nothing else is."""
+from functools import partial
+
+import pytest
+import torch
+
+from imfvideo_amd.imf_dit_video import TransformerBlock, dense_attention, sdpa_math_attention
+from imfvideo_amd.mla_jvp_fast import pack_block
+
+
+def block(impl):
+    return TransformerBlock(64, 1, 32, 32, 32, 32, 64, attn_impl=impl)
+
+
+@pytest.mark.parametrize("impl", [
+    partial(dense_attention, causal=True),
+    partial(dense_attention, scale=0.25),
+    partial(dense_attention, k_lens=torch.tensor([3])),
+    partial(dense_attention, q_lens=[3]),
+    partial(partial(dense_attention, scale=0.25), causal=False),
+    partial(partial(dense_attention, causal=True), scale=None),
+])
+def test_the_jvp_refuses_attention_that_it_does_not_compute(impl):
+    """The fast JVP's dense branch is bidirectional over all tokens at scale 64^-1/2."""
+    with pytest.raises(ValueError, match="dense_attention"):
+        pack_block(block(impl))
+
+
+@pytest.mark.parametrize("impl", [
+    dense_attention, sdpa_math_attention, partial(dense_attention),
+    partial(dense_attention, causal=False, q_lens=None, k_lens=None, scale=None),
+    partial(dense_attention, scale=64 ** -0.5),
+    partial(partial(dense_attention, causal=True), causal=0),
+    lambda q, k, v: q,
+])
+def test_the_jvp_takes_plain_attention(impl):
+    p, w16 = pack_block(block(impl))
+    assert "cube" not in p and "sla2" not in p and w16["w_out"].dtype == torch.float16
