@@ -179,7 +179,10 @@ def dense_attention(q, k, v, causal=False, q_lens=None, k_lens=None, scale=None)
         q_lens = ops.attn_lens(q_lens, q, "q_lens")
     if k_lens is not None:
         k_lens = ops.attn_lens(k_lens, q, "k_lens")
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+    # a forward-mode tangent and torch.jit.trace see the Function (which refuses the one and is
+    # recorded by the other), and neither of them a raw call
+    if (torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)
+            or torch.autograd.forward_ad._current_level >= 0 or torch.jit.is_tracing()):
         return _DenseAttentionFunction.apply(q, k, v, causal, q_lens, k_lens, scale)
     return ops.dense_attn_fwd(q, k, v, causal, q_lens, k_lens, scale, False, False, True)[0]
 
