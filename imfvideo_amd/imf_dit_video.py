@@ -448,21 +448,22 @@ class SwiGLUMlp(nn.Module):
 
     def _mlp8_dtype(self, x1, x3):
         """The 16-bit dtype in which _Mlp8Function takes this call, or None."""
-        ws = (self.w1.weight, self.w3.weight, self.w2.weight)
+        linears = self.w1, self.w3, self.w2
         if not (self.act8 and x1.is_cuda and x1.numel() and torch.is_grad_enabled()
-                and any(t.requires_grad for t in (x1, x3, *ws)) and x1.is_floating_point()):
+                and x1.is_floating_point()
+                and all(_plain_module(m, _Linear) and m.bias is None for m in linears)
+                and _plain_module(self.act, SituAndMul) and self.act.act8
+                and not nn.modules.module._has_any_global_hook()):
             return None
+        ws = [m.weight for m in linears]
         auto = torch.is_autocast_enabled("cuda")
         dt = torch.get_autocast_dtype("cuda") if auto else x1.dtype
         half = (torch.float16, torch.bfloat16)
-        if dt not in half or any(w.dtype not in (half + (torch.float32,) if auto else (dt,))
-                                 or w.device != x1.device for w in ws):
+        if (dt not in half or not any(t.requires_grad for t in (x1, x3, *ws))
+                or any(w.dtype not in (half + (torch.float32,) if auto else (dt,))
+                       or w.device != x1.device for w in ws)):
             return None
-        plain = (all(_plain_module(m, _Linear) and m.bias is None
-                     for m in (self.w1, self.w3, self.w2))
-                 and _plain_module(self.act, SituAndMul) and self.act.act8
-                 and not nn.modules.module._has_any_global_hook())
-        return dt if plain and ops.plain_eager(x1, x3, *ws) else None
+        return dt if ops.plain_eager(x1, x3, *ws) else None
 
     def _forward(self, x1, x3):
         """The MLP with w1 reading x1 and w3 reading x3 (the same values)."""

@@ -5,7 +5,8 @@ from functools import partial
 import pytest
 import torch
 
-from imfvideo_amd.imf_dit_video import TransformerBlock, dense_attention, sdpa_math_attention
+from imfvideo_amd.imf_dit_video import (SwiGLUMlp, TransformerBlock, dense_attention,
+                                        sdpa_math_attention)
 from imfvideo_amd.mla_jvp_fast import pack_block
 
 
@@ -37,3 +38,15 @@ def test_the_jvp_refuses_attention_that_it_does_not_compute(impl):
 def test_the_jvp_takes_plain_attention(impl):
     p, w16 = pack_block(block(impl))
     assert "cube" not in p and "sla2" not in p and w16["w_out"].dtype == torch.float16
+
+
+@pytest.mark.parametrize("act8", [False, True])
+def test_an_mlp_with_replaced_layers_runs(act8):
+    """Layers that are no plain linears (an adapter around one, two in a row) run one by one."""
+    torch.manual_seed(1)
+    m = SwiGLUMlp(16, 24, act8=act8)
+    x = torch.randn(5, 16, requires_grad=True)
+    want = m(x)
+    for n in ("w1", "w3", "w2"):
+        setattr(m, n, torch.nn.Sequential(getattr(m, n)))
+    assert torch.equal(m(x), want)
