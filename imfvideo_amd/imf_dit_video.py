@@ -344,6 +344,8 @@ class SituAndMul(nn.Module):
     bits for the backward (ops.act8_pack's tiles) instead of the tensors
     themselves; the gradients are those at the kept values."""
 
+    act8 = False  # of modules pickled without it
+
     def __init__(self, beta=1.0, linear_beta=None, act8=False):
         super().__init__()
         self.beta = beta
@@ -432,6 +434,8 @@ class SwiGLUMlp(nn.Module):
     hidden_features.  An input tile with an infinity or a NaN makes the gradients that
     read it NaN.  Otherwise (no gradients, CPU tensors, hooked or replaced
     submodules) the layers run one by one, the gate by its own act8."""
+
+    act8 = False  # of modules pickled without it
 
     def __init__(self, in_features, hidden_features, weight_init_constant=1.0, situ_beta=1.0,
                  situ_linear_beta=None, act8=False):

@@ -1,5 +1,6 @@
 """What dense_attention and the modules around it may be asked for, on the host: calls that the
 kernels cannot answer are refused, and nothing else is."""
+import pickle
 from functools import partial
 
 import pytest
@@ -50,3 +51,13 @@ def test_an_mlp_with_replaced_layers_runs(act8):
     for n in ("w1", "w3", "w2"):
         setattr(m, n, torch.nn.Sequential(getattr(m, n)))
     assert torch.equal(m(x), want)
+
+
+def test_modules_saved_whole_without_act8_run():
+    """A module pickled before act8 existed has no such entry in its __dict__."""
+    m = SwiGLUMlp(16, 24)
+    del m.__dict__["act8"], m.act.__dict__["act8"]
+    x = torch.randn(5, 16, requires_grad=True)
+    m = pickle.loads(pickle.dumps(m))
+    assert not m.act8 and not m.act.act8
+    assert torch.equal(m(x), m.w2(m.act(m.w1(x), m.w3(x))))
