@@ -1587,20 +1587,20 @@ def _attn_empty(shape, dev, dtype, flip):
 
 
 def attn_lens(lens, q, name):
-    """Sequence lengths (whole numbers, one per batch entry of q) as contiguous int32 on
-    q's device, or None."""
+    """Sequence lengths (whole numbers within int64, one per batch entry of q) as contiguous
+    int32 on q's device, or None."""
     if lens is None:
         return None
     lens = torch.as_tensor(lens)
     if (lens.dtype == torch.int32 and lens.shape == q.shape[:1] and lens.device == q.device
             and lens.is_contiguous()):
         return lens
-    if (lens.dtype.is_floating_point or lens.dtype.is_complex or lens.dtype == torch.bool
-            or tuple(lens.shape) != tuple(q.shape[:1])):
+    if (lens.dtype.is_floating_point or lens.dtype.is_complex
+            or lens.dtype in (torch.bool, torch.uint64) or tuple(lens.shape) != tuple(q.shape[:1])):
         raise ValueError(f"{name}: expected {q.shape[0]} whole numbers, got "
                          f"{tuple(lens.shape)} {lens.dtype}")
     if lens.dtype != torch.int32:  # values past 32 bits are past any length
-        lens = lens.clamp(0, 2 ** 31 - 1)
+        lens = lens.to(torch.int64).clamp(0, 2 ** 31 - 1)
     return lens.to(q.device, torch.int32).contiguous()
 
 

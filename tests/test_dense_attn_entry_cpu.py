@@ -6,6 +6,7 @@ from functools import partial
 import pytest
 import torch
 
+from imfvideo_amd import ops
 from imfvideo_amd.imf_dit_video import (SwiGLUMlp, TransformerBlock, dense_attention,
                                         sdpa_math_attention)
 from imfvideo_amd.mla_jvp_fast import pack_block
@@ -61,3 +62,23 @@ def test_modules_saved_whole_without_act8_run():
     m = pickle.loads(pickle.dumps(m))
     assert not m.act8 and not m.act.act8
     assert torch.equal(m(x), m.w2(m.act(m.w1(x), m.w3(x))))
+
+
+@pytest.mark.parametrize("dtype", [torch.uint8, torch.int8, torch.int16, torch.int32, torch.int64,
+                                   torch.uint16, torch.uint32])
+def test_lengths_of_every_whole_number_type(dtype):
+    info = torch.iinfo(dtype)
+    q = torch.zeros(5, 1, 1, 64)
+    vals = [0, 1, 5, info.max, info.min]
+    got = ops.attn_lens(torch.tensor(vals, dtype=dtype), q, "k_lens")
+    assert got.dtype == torch.int32 and got.is_contiguous()
+    # below zero nothing, above 32 bits more than any length has
+    clamped = [min(max(v, -2 ** 31), 2 ** 31 - 1) for v in vals]
+    assert [max(v, 0) for v in got.tolist()] == [max(v, 0) for v in clamped]
+
+
+def test_lengths_that_are_no_whole_numbers_of_int64():
+    q = torch.zeros(1, 1, 1, 64)
+    for bad in ([0.5], [True], torch.tensor([1], dtype=torch.uint64)):
+        with pytest.raises(ValueError, match="k_lens"):
+            ops.attn_lens(bad, q, "k_lens")
