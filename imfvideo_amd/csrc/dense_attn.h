@@ -149,6 +149,15 @@ __device__ inline int seq_len(const int32_t* lens, int b, int64_t L) {
   return n < 0 ? 0 : (n > L ? (int)L : n);
 }
 
+// Sizes that forward and backward take, the same for both: what the forward has answered the
+// backward can answer.  Sizes of sequences fit an int with a tile's room, heads of a batch too (the
+// launches' own bounds are looked at where their grids are known).
+inline bool sizes_ok(int B, int H, int Hkv, int64_t Lq, int64_t Lk) {
+  return B > 0 && H > 0 && Hkv > 0 && H % Hkv == 0 && Lq > 0 && Lk > 0 &&
+         Lq < ((int64_t)1 << 30) && Lk < ((int64_t)1 << 30) &&
+         (int64_t)B * H < ((int64_t)1 << 20) && (H / Hkv) * Lq < ((int64_t)1 << 31);
+}
+
 // Which head and tile a workgroup takes.  Workgroups go to the eight XCDs in turn, each with
 // an L2 of its own.
 //   even tiles (no mask, no lengths): an XCD takes a run of neighbouring tiles, so that those of

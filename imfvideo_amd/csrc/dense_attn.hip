@@ -618,12 +618,6 @@ FwdPlan fwd_plan(int B, int H, int Hkv, int64_t Lq, int64_t Lk, bool even) {
   return p;
 }
 
-bool sizes_ok(int B, int H, int Hkv, int64_t Lq, int64_t Lk) {
-  return B > 0 && H > 0 && Hkv > 0 && H % Hkv == 0 && Lq > 0 && Lk > 0 &&
-         Lq < ((int64_t)1 << 30) && Lk < ((int64_t)1 << 30) &&
-         (int64_t)B * H < ((int64_t)1 << 20) && (H / Hkv) * Lq < ((int64_t)1 << 31);
-}
-
 }  // namespace
 
 }  // namespace sla2h

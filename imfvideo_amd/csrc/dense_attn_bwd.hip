@@ -580,12 +580,6 @@ BwdPlan bwd_plan(int dtype, int B, int H, int Hkv, int64_t Lq, int64_t Lk, bool 
   return p;
 }
 
-bool sizes_ok(int B, int H, int Hkv, int64_t Lq, int64_t Lk) {
-  return B > 0 && H > 0 && Hkv > 0 && H % Hkv == 0 && Lq > 0 && Lk > 0 &&
-         Lq < ((int64_t)1 << 30) && Lk < ((int64_t)1 << 30) && (int64_t)B * H < 65536 &&
-         (H / Hkv) * ((Lq + 63) / 64) < ((int64_t)1 << 30);
-}
-
 }  // namespace
 
 }  // namespace sla2h

@@ -1507,6 +1507,11 @@ class _AttnPlan:
                  "v_flip", "fwd", "bwd", "fwd_ws", "bwd_ws", "lse_shape", "lo_shape")
 
 
+def _attn_too_large(qs, ks):
+    return ValueError(f"too large: {tuple(qs)}, {tuple(ks)} (batch x heads below 2^20, lengths "
+                      "below 2^30, the heads of one row below 2^17 where rows lie apart)")
+
+
 @functools.lru_cache(maxsize=512)
 def _attn_plan(qs, qt, ks, kt, vs, vt, dtype, tok):
     for s, name in ((qs, "q"), (ks, "k"), (vs, "v")):
@@ -1552,6 +1557,10 @@ def _attn_plan(qs, qt, ks, kt, vs, vt, dtype, tok):
         lib = _lib.load()
         p.fwd_ws = lib.sla2h_dense_attn_fwd_workspace_bytes(*p.sizes)
         p.bwd_ws = lib.sla2h_dense_attn_bwd_workspace_bytes(_HALF[dtype], *p.sizes)
+        # (a backward always has a workspace: 0 are sizes that the kernels do not take; operands
+        # that are copied get a plan of their own)
+        if not p.bwd_ws or not any(p.copy) and max(so[2], sk[2], sv[2]) >= _ATTN_ROW_SPAN:
+            raise _attn_too_large(qs, ks)
     return p
 
 
@@ -1574,6 +1583,8 @@ def _attn_operands(q, k, v, scale, tok):
                    for t, c in zip((q, k, v), plan.copy))
         plan = _attn_plan(q.shape, q.stride(), k.shape, k.stride(), v.shape, v.stride(), q.dtype,
                           tok)
+        if any(plan.copy):
+            raise _attn_too_large(q.shape, k.shape)
     if scale is None:
         scale = E_TILE ** -0.5
     elif not 0.0 < scale < 1e30:

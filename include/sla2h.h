@@ -847,7 +847,8 @@ int sla2h_sla2_infer_in(const void* q, const void* k, const void* v, int dtype, 
  *   lse = log sum exp S (natural log).  Rows at or past q_len and rows without a key: o = 0,
  *   lse = -inf.  Whatever memory holds behind a sequence (NaN too) is not used.
  * q (B, H, Lq, 64), k, v (B, Hkv, Lk, 64), o like q, of one 16-bit dtype, H a multiple of
- * Hkv (query head h reads key head h / (H / Hkv)).  strides: host array of 12 int64, the
+ * Hkv (query head h reads key head h / (H / Hkv)); B H < 2^20, Lq and Lk < 2^30, (H / Hkv) Lq <
+ * 2^31 here and in the backward.  strides: host array of 12 int64, the
  * (batch, head, row) strides of q, k, v, o in elements, multiples of 8 (batch and head strides
  * 0 for broadcast inputs; row strides at least 64, k's and v's below 2^23); unit channel stride, 16-byte aligned pointers.  q_lens, k_lens (B)
  * int32 on the device or NULL (all Lq / Lk); values are clamped into [0, Lq] / [0, Lk].

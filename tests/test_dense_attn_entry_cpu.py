@@ -1,12 +1,13 @@
 """What dense_attention and the modules around it may be asked for, on the host: calls that the
 kernels cannot answer are refused, and nothing else is."""
+import ctypes
 import pickle
 from functools import partial
 
 import pytest
 import torch
 
-from imfvideo_amd import ops
+from imfvideo_amd import _lib, ops
 from imfvideo_amd.imf_dit_video import (SwiGLUMlp, TransformerBlock, dense_attention,
                                         sdpa_math_attention)
 from imfvideo_amd.mla_jvp_fast import pack_block
@@ -82,3 +83,41 @@ def test_lengths_that_are_no_whole_numbers_of_int64():
     for bad in ([0.5], [True], torch.tensor([1], dtype=torch.uint64)):
         with pytest.raises(ValueError, match="k_lens"):
             ops.attn_lens(bad, q, "k_lens")
+
+
+class _Gpu(torch.Tensor):
+    """A CPU tensor that says it is on the GPU: the checks run, no launch is reached."""
+    is_cuda = property(lambda self: True)
+
+
+def test_forward_and_backward_take_the_same_sizes():
+    """What the forward answers has a backward: as many heads, lengths and groups."""
+    lib = _lib.load()
+    st = (ctypes.c_int64 * 24)(*[64] * 24)
+    bad, ok = 1, lambda *s: lib.sla2h_dense_attn_bwd_workspace_bytes(1, *s) > 0
+    for sizes, good in (((8200, 8, 8, 3, 3), True), ((1, 65536, 1, 1, 1), True),
+                        ((2 ** 20 - 1, 1, 1, 1, 1), True), ((2 ** 20, 1, 1, 1, 1), False),
+                        ((1, 2, 2, 2 ** 30, 1), False), ((1, 2, 2, 1, 2 ** 30), False),
+                        ((1, 8, 1, 2 ** 28, 1), False), ((1, 3, 2, 4, 4), False)):
+        assert ok(*sizes) == good, sizes
+        if not good:
+            assert lib.sla2h_dense_attn_fwd(16, 16, 16, st, None, None, 1, *sizes, 0, 0.125, 16, 16,
+                                            4, None, None) == bad
+            assert lib.sla2h_dense_attn_bwd(16, 16, 16, 16, None, 16, 4, st, None, None, 1, *sizes,
+                                            0, 0.125, 16, 16, 16, 16, None) == bad
+
+
+@pytest.mark.parametrize("shape", [(2 ** 20, 1, 2, 64), (1, 2 ** 20, 2, 64), (1, 1, 2 ** 30, 64)])
+def test_sizes_past_the_kernels_are_refused_by_name(shape):
+    """The forward refuses what it or its backward could not launch."""
+    shape = torch.Size(shape)
+    strides = (shape[1] * shape[2] * 64, shape[2] * 64, 64, 1)
+    with pytest.raises(ValueError, match="too large"):
+        ops._attn_plan(shape, strides, shape, strides, shape, strides, torch.bfloat16, False)
+
+
+def test_rows_too_far_apart_are_refused_by_name():
+    """2^17 heads of 64 channels side by side: rows past the 32-bit offsets of a tile, in a copy too."""
+    x = torch.zeros(1, 2, 2 ** 17, 64, dtype=torch.bfloat16).as_subclass(_Gpu)
+    with pytest.raises(ValueError, match="too large"):
+        ops.dense_attn_fwd(x, x, x, tok=True)

@@ -42,3 +42,16 @@ def test_a_trace_records_the_call(leaf):
     want = dense_attention(*y, causal=True)
     for _ in range(3):
         assert torch.equal(m(*y), want)
+
+
+def test_many_clips_train():
+    """65,600 heads of three rows: forward and backward."""
+    from imfvideo_amd.imf_dit_video import dense_attention
+    q, k, v, do = operands(4, 8200, 3, 8, 8, 4, torch.bfloat16)
+    x = [t.requires_grad_(True) for t in (q, k, v)]
+    o = dense_attention(*x, causal=True)
+    got = dict(zip(("dq", "dk", "dv"), torch.autograd.grad(o, x, do)), o=o.detach())
+    heads = lambda t: t.detach().transpose(1, 2)
+    want = R.attention(*map(heads, (q, k, v)), causal=True, do=heads(do), dev="cuda", lo=True)
+    for n in ("o", "dq", "dk", "dv"):
+        R.check(heads(got[n]), want[n], n)
