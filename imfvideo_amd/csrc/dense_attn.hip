@@ -687,7 +687,8 @@ extern "C" int sla2h_dense_attn_fwd(const void* q, const void* k, const void* v,
   auto go = [&](auto tag) -> int {
     using T16 = decltype(tag);
     const unsigned grid = work_grid(a.map);
-    const bool fine = Lk <= kFineKeys || causal;
+    // (a wave decides by the keys that its rows see: with causal order or lengths any may be few)
+    const bool fine = Lk <= kFineKeys || causal || k_lens;
     if (p.nq == 2 && fine)
       dense_fwd_kernel<T16, 2, true><<<grid, 256, 0, st>>>(a);
     else if (p.nq == 2)

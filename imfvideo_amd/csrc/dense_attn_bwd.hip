@@ -40,7 +40,9 @@ struct Shift<F16> {
 // of a workgroup).  bf16, 2-norm of dq's error: 1.7e-3 (its own rounding) to 1.8e-3 instead of
 // 2.4e-3 to 2.8e-3.  Backward, us, without : with, H = 8: two clips of 274 tokens 22.3 : 22.5; two of
 // 8,192 queries x 77 keys 41.8 : 43.5; L = 2,048 47 : 53, 4,096 127 : 144; causal L = 4,096
-// 109 : 122, B = 3 clips of up to 4,159 152 : 159, L = 29,952 2,970 : 3,017.
+// 109 : 122, B = 3 clips of up to 4,159 152 : 159, L = 29,952 2,970 : 3,017.  The instance that asks
+// the waves costs padded batches whose sequences are long, too: forward and backward, us, of clips of
+// 4,159, 2,703 and 1,247 tokens, H = 8 over 2, 390 : 417, of 29,952 and 18,720 14,000 : 14,400.
 constexpr int kFineKeys = 4096, kFineRows = 512;
 constexpr int kNormRows = 64;  // rows of a partial maximum of the norms
 
@@ -674,7 +676,7 @@ extern "C" int sla2h_dense_attn_bwd(const void* q, const void* k, const void* v,
     const unsigned grid = a.kv_blocks + (dq ? work_grid(a.dq_map) : 0);
     if (causal)
       dense_bwd_kernel<T16, true, true><<<grid, 256, 0, st>>>(a);
-    else if (Lk <= kFineKeys || Lq <= kFineRows)
+    else if (Lk <= kFineKeys || Lq <= kFineRows || q_lens || k_lens)  // (sequences, not the padding)
       dense_bwd_kernel<T16, false, true><<<grid, 256, 0, st>>>(a);
     else
       dense_bwd_kernel<T16, false, false><<<grid, 256, 0, st>>>(a);

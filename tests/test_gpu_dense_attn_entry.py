@@ -55,3 +55,53 @@ def test_many_clips_train():
     want = R.attention(*map(heads, (q, k, v)), causal=True, do=heads(do), dev="cuda", lo=True)
     for n in ("o", "dq", "dk", "dv"):
         R.check(heads(got[n]), want[n], n)
+
+
+def fine_bounds(q, k, v, do, got, case):
+    """Gradients of operands (1, H, L, 64) whose P and dS enter their products with the half
+    that rounding them lost: an element is off by its own rounding u |x| and second-order terms,
+    each at most u^2 P mag with mag = |dout| . |v_j| + |dout| . P |v| (dS's u^2 |dS|; through
+    delta P's u^2 P |v| and the u^2 |o| of the output's second half), and T32 of the same sums for
+    S, dP and delta in fp32."""
+    dt, (_, H, Lq, _), (Hkv, Lk) = q.dtype, q.shape, k.shape[1:3]
+    rep = H // Hkv
+    want = R.attention(q, k, v, do=do, dev="cuda")
+    u, tiny = torch.finfo(dt).eps / 2, torch.finfo(dt).smallest_normal * torch.finfo(dt).eps
+    K, V = (t.double().repeat_interleave(rep, 1) for t in (k, v))
+    P = torch.softmax(q.double() @ K.transpose(-1, -2).contiguous() / 8, -1)
+    g = do.double().abs()
+    mag = g @ V.abs().transpose(-1, -2).contiguous() + (g * (P @ V.abs())).sum(-1, keepdim=True)
+    E = (4 * u * u + 3 * R.T32) * P * mag + 2.0 ** -36 * mag.amax((-1, -2), keepdim=True)
+    heads = lambda t: t.reshape(1, Hkv, rep, Lk, 64).sum(2)
+    turn = lambda t: t.transpose(-1, -2).contiguous()
+    more = dict(o=(2 * u * u + R.T32) * (P @ V.abs()), dq=E @ K.abs() / 8,
+                dk=heads(turn(E) @ q.double().abs()) / 8,
+                dv=heads(turn((2 * u * u + R.T32) * P + 2.0 ** -36) @ g))
+    for n, m in more.items():
+        val = want[n][0]
+        print("[ratio]", n, round(R.check(got[n], (val, u * val.abs() + m + tiny), (case, n)), 3),
+              flush=True)
+
+
+# B, H, Hkv, Lq, Lk of the padded batch; rows and keys of its first clip, which alone takes each
+# kernel's form for few of them: 128- and 256-row blocks of the forward, the backward's dq and dk/dv
+PADDED = [(2, 128, 128, 130, 700, 130, 200), (8, 64, 32, 300, 700, 200, 97),
+          (2, 4, 2, 700, 4200, 90, 150)]
+
+
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("case", PADDED)
+def test_a_short_clip_keeps_its_accuracy_in_a_padded_batch(case, dt):
+    """The halves that rounding P and dS loses are kept by a sequence's own length, however
+    far its batch is padded."""
+    from imfvideo_amd import ops
+    B, H, Hkv, Lq, Lk, nq, nk = case
+    print("[case]", case, dt, flush=True)
+    q, k, v, do = (t.transpose(1, 2) for t in operands(5, B, Lq, H, Hkv, Lk, dt))
+    ql = torch.tensor([nq] + [Lq] * (B - 1), device="cuda")
+    kl = torch.tensor([nk] + [Lk] * (B - 1), device="cuda")
+    o, lse, lo = ops.dense_attn_fwd(q, k, v, q_lens=ql, k_lens=kl, with_lo=True)
+    grads = ops.dense_attn_bwd(do, q, k, v, o, lse, q_lens=ql, k_lens=kl, o_lo=lo)
+    cut = lambda t, n: t[:1, :, :n]
+    got = dict(o=cut(o, nq), dq=cut(grads[0], nq), dk=cut(grads[1], nk), dv=cut(grads[2], nk))
+    fine_bounds(cut(q, nq), cut(k, nk), cut(v, nk), cut(do, nq), got, (case, dt))
