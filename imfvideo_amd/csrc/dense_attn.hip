@@ -31,7 +31,7 @@ template <>
 struct Range<F16> {
   static constexpr float shift = 9.f, most = 32768.f;
 };
-constexpr int kFineKeys = 512;
+constexpr int kFineKeys = 512, kFewBlocks = 256;
 constexpr float kFloor = -1e30f;  // m before the first key (finite: -inf - m stays -inf)
 
 struct DenseFwdArgs {
@@ -364,7 +364,10 @@ __global__ __launch_bounds__(256, 2) void dense_fwd_kernel(DenseFwdArgs a) {
 // barrier in the loop), and their sums are joined in LDS: one query over 29,952 and 18,720 keys
 // of 8 heads in 20 us, 5 TB/s.  With one range the result is final,
 // else a second kernel adds the ranges in order.
-template <typename T16>
+// What the rounding of P lost is added over any number of keys where at most kFewBlocks blocks
+// of rows leave the matrix cores idle under the loads; us, without : with, H = 8: one query as above 29.2 :
+// 30.2 a call, L = 1,024 (256 blocks) 25.3 : 25.8, but L = 1,500 (376) 37 : 40, 2,048 (512) 22 : 26.
+template <typename T16, bool FEW>
 __global__ __launch_bounds__(256, 2) void dense_fwd_split_kernel(DenseFwdArgs a) {
   constexpr int kUnitB = 32 * kRowB;
   __shared__ __align__(16) unsigned char kv0[4][2 * kUnitB], kv1[4][2 * kUnitB];
@@ -418,6 +421,7 @@ __global__ __launch_bounds__(256, 2) void dense_fwd_split_kernel(DenseFwdArgs a)
   }
   f32x16 acc[2] = {zero16(), zero16()};
   float m = kFloor, lsum = 0.f;
+  const bool fine = FEW || kmax <= kFineKeys;
   auto compute = [&](int64_t u, const unsigned char* kv) __attribute__((always_inline)) {
     f32x16 sc = zero16();
 #pragma unroll
@@ -432,7 +436,6 @@ __global__ __launch_bounds__(256, 2) void dense_fwd_split_kernel(DenseFwdArgs a)
     }
     lsum += r;
     u32x4 q[2];
-    const bool fine = kmax <= kFineKeys;
     if (fine) lost_halves<T16>(sc, a.c, m, p, q);
 #pragma unroll
     for (int s = 0; s < 2; ++s)
@@ -577,6 +580,7 @@ struct FwdPlan {
   int64_t qtiles, nwork;
   int splits;  // ranges of keys
   int64_t units;
+  bool few;  // nq = 0: at most kFewBlocks blocks of rows
 };
 
 // even: neither causal nor lengths
@@ -608,6 +612,7 @@ FwdPlan fwd_plan(int B, int H, int Hkv, int64_t Lq, int64_t Lk, bool even) {
   p.nq = 0;
   p.qtiles = ((H / Hkv) * Lq + 31) / 32;
   const int64_t blocks = (int64_t)B * Hkv * p.qtiles, units = (Lk + 31) / 32;
+  p.few = blocks <= kFewBlocks;
   int64_t s = (512 + blocks - 1) / blocks;
   const int64_t most = units / 8;  // two units per wave and range at least
   s = s < most ? s : most;
@@ -697,8 +702,10 @@ extern "C" int sla2h_dense_attn_fwd(const void* q, const void* k, const void* v,
       dense_fwd_kernel<T16, 1, true><<<grid, 256, 0, st>>>(a);
     else if (p.nq == 1)
       dense_fwd_kernel<T16, 1, false><<<grid, 256, 0, st>>>(a);
+    else if (p.few)
+      dense_fwd_split_kernel<T16, true><<<a.nwork, 256, 0, st>>>(a);
     else
-      dense_fwd_split_kernel<T16><<<a.nwork, 256, 0, st>>>(a);
+      dense_fwd_split_kernel<T16, false><<<a.nwork, 256, 0, st>>>(a);
     const int err = (int)hipGetLastError();
     if (err || p.splits == 1) return err;
     dense_join_kernel<T16><<<(unsigned)a.nrows, 256, 0, st>>>(a);

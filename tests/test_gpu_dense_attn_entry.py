@@ -105,3 +105,23 @@ def test_a_short_clip_keeps_its_accuracy_in_a_padded_batch(case, dt):
     cut = lambda t, n: t[:1, :, :n]
     got = dict(o=cut(o, nq), dq=cut(grads[0], nq), dk=cut(grads[1], nk), dv=cut(grads[2], nk))
     fine_bounds(cut(q, nq), cut(k, nk), cut(v, nk), cut(do, nq), got, (case, dt))
+
+
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("shape", [(1, 2, 2, 1, 29952), (2, 8, 2, 3, 5000), (1, 4, 4, 32, 1100),
+                                   (1, 8, 8, 1000, 1000)])
+def test_few_queries_keep_what_rounding_loses(shape, dt):
+    """The output of calls of at most 256 blocks of 32 rows, over any number of keys: its own
+    rounding, second-order terms and fp32 arithmetic."""
+    from imfvideo_amd import ops
+    B, H, Hkv, Lq, Lk = shape
+    q, k, v, _ = (t.transpose(1, 2) for t in operands(6, B, Lq, H, Hkv, Lk, dt))
+    o, _ = ops.dense_attn_fwd(q, k, v)
+    val, _ = R.attention(q, k, v, dev="cuda")["o"]
+    u, tiny = torch.finfo(dt).eps / 2, torch.finfo(dt).smallest_normal * torch.finfo(dt).eps
+    for b in range(B):
+        x = [t[b:b + 1] for t in (q, k, v.abs())]
+        pv, _ = R.attention(*x, dev="cuda")["o"]  # P |v|
+        val_b = val[b:b + 1]
+        print("[ratio]", round(R.check(o[b:b + 1], (val_b, u * val_b.abs() + (2 * u * u + R.T32) * pv
+                                                    + tiny), (shape, dt)), 3), flush=True)
