@@ -175,9 +175,9 @@ __global__ __launch_bounds__(256) void wgrad_sum_kernel(const f32x4* __restrict_
 // --- dW = dY^T X with X in 8 bits (act8.h) -----------------------------------
 //
 // dW_mn = sum over row tiles t of s_t,n (sum over the tile's rows dY_rm code_rn): the codes are
-// whole numbers up to 127 and exact in either 16-bit type, so the products of a tile of 64 rows
-// are exact in fp32 and the tile's scale is applied to the sum, in fp32.  X is never
-// rounded to 16 bits again.
+// whole numbers up to 127 and exact in either 16-bit type, so each product is exact in fp32.
+// The tile's 64 are added in fp32, which rounds, and its scale is applied to their sum.  X is
+// never rounded to 16 bits again.
 struct Wgrad8Args {
   const uint16_t* dy;
   const int8_t* codes;
@@ -189,6 +189,11 @@ struct Wgrad8Args {
   int64_t per_split;  // row tiles of a range
   int nwork, per_xcd;
 };
+
+// A byte offset past every stage's range (64 rows of at most 2^24 bytes) whose group of eight
+// elements and the dword behind it are offsets too.
+constexpr int kPastEnd = 0x7fffff00;
+static_assert(kPastEnd > (kAct << 24) && kPastEnd + 16 + 4 > kPastEnd);
 
 constexpr int kAStage = kAct * kWT * 2;  // bytes of one operand's stage: 64 rows x 256 B
 
@@ -260,7 +265,7 @@ __global__ __launch_bounds__(256, 2) void wgrad8_kernel(Wgrad8Args a) {
     const int64_t left = a.rows - (t0 + s) * kAct;
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-      const int o = 16 * k + yr < left ? y_off(k) & ~3 : 0x7ffffff0;
+      const int o = 16 * k + yr < left ? y_off(k) & ~3 : kPastEnd;
       v[k] = buf_load16(ry, o, 0);
       x[k] = __builtin_amdgcn_raw_buffer_load_b32(ry, o + 16, 0, 0);
     }
