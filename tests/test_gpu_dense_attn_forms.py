@@ -49,14 +49,16 @@ def test_large_blocks_of_rows(shape, mask, dt):
 
 
 @pytest.mark.parametrize("dt", DTYPES)
-@pytest.mark.parametrize("mask", ["none", "causal", "both"])
+@pytest.mark.parametrize("mask", ["none", "causal", "ragged", "both"])
 @pytest.mark.parametrize("shape", [(1, 2, 2, 700, 4200), (2, 4, 1, 1500, 4300)])
 def test_backward_of_long_sequences(shape, mask, dt):
     """More than 4,096 keys and 512 queries: P and dS without what their rounding lost."""
     print("[case]", shape, mask, dt, flush=True)
     x = [t.cuda() for t in inputs(sum(shape), *shape, dt)]
-    causal = mask != "none"
-    ql, kl = lens(shape[0], shape[3], shape[4], 2) if mask == "both" else (None, None)
+    causal = mask in ("causal", "both")
+    ql = kl = None
+    if mask in ("ragged", "both"):
+        ql, kl = lens(shape[0], shape[3], shape[4], 2)
     got = run(*x, causal=causal, q_lens=ql, k_lens=kl)
     want = R.attention(*x[:3], causal, ql, kl, do=x[3], dev="cuda", lo=True)
     check_all(got, want, (shape, mask, dt))
