@@ -6,8 +6,9 @@
 //   dg = dh sat(u) situ'(g),  du = dh situ(g) sat'(u)   at the restored g and u.
 //
 // HBM-bound by design: 8 bytes per element each way for the gate (10 with 16-bit gate and
-// up in the backward).  59,904 x 2,048 bf16: forward 220 us, backward 212 us, 4.5 TB/s (copy rate
-// 5.2) beside about 75 VALU per element; packing 59,904 x 512 18 us, 5.1 TB/s.
+// up in the backward).  59,904 x 2,048 bf16: both in 421 to 444 us by card, 4.4 to 4.7 TB/s (copy rate
+// 5.2) beside about 75 VALU per element; each alone under the profiler, median (least) of 30: forward
+// 242 (223), backward 254 us (233); packing 59,904 x 512 18 us, 5.1 TB/s.
 //
 // With a = e^(-2|x|), tanh|x| = (1 - a) / (1 + a) and sech^2 x = 4 a / (1 + a)^2: one exp
 // gives both without the cancellation of 1 - tanh^2; 1 - a itself cancels for small |x|, where

@@ -184,7 +184,8 @@ __device__ inline u32x2 lds_read_tr16(const void* p) {
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
-// 2^x on the hardware exp unit (v_exp_f32); inputs here are <= 0 or -inf.
+// 2^x on the hardware exp unit (v_exp_f32): 0 for -inf, +inf from 128 on (dense attention takes
+// that for a bound that has to rise).
 __device__ inline float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // fp32 maximum by integer atomics: positive floats order as int, negative ones

@@ -167,7 +167,8 @@ def dense_attention(q, k, v, causal=False, q_lens=None, k_lens=None, scale=None)
     autocast any floating dtype, cast to it), H a multiple of Hkv; usable as an
     attn_impl.  q_lens, k_lens (b,): the clips' lengths in a padded batch; rows
     behind them, and rows without a key, are zero and take no gradient.  causal:
-    query i sees the keys j <= i + k_len - q_len.  scale: 64^-1/2 by default.
+    query i sees the keys j <= i + k_len - q_len (operands have to be finite
+    within a sequence: what is hidden is weighed with 0).  scale: 64^-1/2 by default.
 
     Memory is linear in l (the probabilities are recomputed in the backward), and
     results do not depend on the order of execution.  GPU tensors only; one

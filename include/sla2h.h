@@ -845,7 +845,9 @@ int sla2h_sla2_infer_in(const void* q, const void* k, const void* v, int dtype, 
  *   S = scale q k^T over the keys j < k_len of a batch's sequence, with causal only
  *   j <= i + k_len - q_len (the last query sees the last key); o = softmax(S) v,
  *   lse = log sum exp S (natural log).  Rows at or past q_len and rows without a key: o = 0,
- *   lse = -inf.  Whatever memory holds behind a sequence (NaN too) is not used.
+ *   lse = -inf.  Whatever memory holds behind a sequence (NaN too) is not used.  Within a sequence
+ *   causal order weighs later keys with 0: an infinity or a NaN in their v (in the backward in k, q
+ *   and dout too) reaches the rows whose tiles of 64 hold them, as in a product with P.
  * q (B, H, Lq, 64), k, v (B, Hkv, Lk, 64), o like q, of one 16-bit dtype, H a multiple of
  * Hkv (query head h reads key head h / (H / Hkv)); B H < 2^20, Lq and Lk < 2^30, (H / Hkv) Lq <
  * 2^31 here and in the backward.  strides: host array of 12 int64, the
