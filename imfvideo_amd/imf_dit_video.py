@@ -21,7 +21,7 @@ from . import ops
 
 __all__ = ["RMSNorm", "SituAndMul", "SwiGLUMlp", "MLAAttention", "TransformerBlock",
            "apply_rotary_pos_emb", "precompute_axial_rope_3d", "scaled_variance_linear",
-           "dense_attention", "sdpa_math_attention"]
+           "dense_attention", "sdpa_math_attention", "residual_norm"]
 
 
 class _CastOf(torch.autograd.Function):
@@ -775,16 +775,94 @@ def _residual(x, a, scale):
     return x + a * scale
 
 
+class _ResidualNormFunction(torch.autograd.Function):
+    """residual_norm on the GPU: one HIP kernel forward, one backward (and one that adds
+    its column sums); saves a and the output y."""
+
+    @staticmethod
+    def forward(ctx, x, a, scale, post, pre, gate, eps, consumers):
+        y, n = ops.residual_norm_fwd(x, a, scale, post, pre, gate, eps)
+        ctx.eps = eps
+        ctx.save_for_backward(y, a, scale, post, pre, gate)
+        ctx.set_materialize_grads(False)
+        return (y,) if n is None else (y, n) + tuple(n.view_as(n) for _ in range(consumers - 1))
+
+    @staticmethod
+    @_once
+    def backward(ctx, dy, *dns):
+        y, a, scale, post, pre, gate = ctx.saved_tensors
+        dns = [d for d in dns if d is not None]
+        if dy is None and not dns:
+            return (None,) * 8
+        _no_batched(dy if dy is not None else dns[0], "residual_norm")
+        dx, da, dscale, dpost, dpre, dgate = ops.residual_norm_bwd(dy, dns, y, a, scale, post, pre,
+                                                                   gate, ctx.eps)
+        if dpre is None and pre is not None:
+            dpre = torch.zeros_like(pre)
+        return dx, da, dscale, dpost, dpre, dgate, None, None
+
+
+def residual_norm(x, a, scale, post_weight, gate=None, pre_weight=None, eps=1e-6, consumers=1):
+    """The residual step between two sublayers, with a norm on both of its sides:
+
+        y = x + scale * gate * (post_weight * a / rms(a)),    n = pre_weight * y / rms(y)
+
+    for the residual stream x (b, l, D), a sublayer's output a of its shape, vectors of D channels
+    and gate (b, D), one row per clip (None: ones); rms = sqrt(mean of squares + eps) of a
+    row.  Returns (y, n, ..., n): n once for each of the `consumers` (1 to 3) that read
+    it, so that their gradients are summed in fp32; (y,) without pre_weight.
+
+    GPU tensors (x fp32, a 16-bit or fp32) run the fused kernels (sla2h_residual_norm_fwd / _bwd):
+    fp32 arithmetic, n rounded once to a's dtype, one reverse-mode derivative.  Anything else
+    (CPU tensors, other dtypes, transforms) runs the eager expression."""
+    if not 1 <= consumers <= 3:
+        raise ValueError(f"residual_norm: 1 to 3 consumers, got {consumers}")
+    given = [t for t in (x, a, scale, post_weight, gate, pre_weight) if t is not None]
+    if gate is not None and (x.dim() < 2 or tuple(gate.shape) != (x.shape[0], x.shape[-1])):
+        raise ValueError(f"residual_norm: expected a gate of {x.shape[0]} rows of {x.shape[-1]}, "
+                         f"got {tuple(gate.shape)}")
+    if (all(t.is_cuda and t.is_floating_point() for t in given) and x.dtype == torch.float32
+            and a.dtype in (torch.float16, torch.bfloat16, torch.float32) and a.shape == x.shape
+            and x.numel() and x.shape[-1] <= ops.RESIDUAL_NORM_MAX
+            and all(tuple(v.shape) == (x.shape[-1],) for v in (scale, post_weight))
+            and (pre_weight is None or tuple(pre_weight.shape) == (x.shape[-1],))
+            and all(t.device == x.device for t in given) and ops.plain_eager(*given)):
+        scale, post, pre, g = (None if t is None else t.float()
+                               for t in (scale, post_weight, pre_weight, gate))
+        return _ResidualNormFunction.apply(x, a, scale, post, pre, g, float(eps), consumers)
+    wide = torch.promote_types(x.dtype, torch.float32)
+    norm = lambda t, w: t * torch.rsqrt(t.pow(2).mean(dim=-1, keepdim=True) + eps) * w
+    step = scale * norm(a.to(wide), post_weight)
+    if gate is not None:
+        step = step * gate.reshape(gate.shape[0], *(1,) * (x.dim() - 2), gate.shape[1])
+    y = (x.to(wide) + step).to(x.dtype)
+    if pre_weight is None:
+        return (y,)
+    return (y,) + (norm(y.to(wide), pre_weight).to(a.dtype),) * consumers
+
+
 class TransformerBlock(nn.Module):
     """x += attn(norm1(x)) * attn_scale;  x += mlp(norm2(x)) * mlp_scale
     (vector gates initialised to zero).  act8: the MLP keeps its activations in 8
-    bits for the backward (SwiGLUMlp)."""
+    bits for the backward (SwiGLUMlp).
+
+    sandwich_norm: a norm behind each sublayer too, x += attn_post_norm(attn(norm1(x))) *
+    attn_scale and the MLP alike, the step from one sublayer's output to the next one's input
+    in one kernel (residual_norm).  forward then takes gates = (attn_gate, mlp_gate), each (b,
+    hidden_size) or None: factors of the two steps, clip by clip."""
+
+    sandwich_norm = False  # of modules pickled without it
 
     def __init__(self, hidden_size, num_heads, q_lora_rank, kv_lora_rank, qk_nope_head_dim,
                  qk_rope_head_dim, v_head_dim, mlp_ratio=8 / 3, weight_init_constant=1.0,
                  norm_eps=1e-6, attn_impl=sdpa_math_attention, use_attn_res=False, situ_beta=4.0,
-                 situ_linear_beta=25.0, mla_use_output_gate=True, act8=False):
+                 situ_linear_beta=25.0, mla_use_output_gate=True, act8=False,
+                 sandwich_norm=False):
         super().__init__()
+        self.sandwich_norm = sandwich_norm
+        if sandwich_norm:
+            self.attn_post_norm = RMSNorm(hidden_size, eps=norm_eps)
+            self.mlp_post_norm = RMSNorm(hidden_size, eps=norm_eps)
         self.norm1 = RMSNorm(hidden_size, eps=norm_eps)
         self.attn = MLAAttention(hidden_size, num_heads=num_heads, q_lora_rank=q_lora_rank,
                                  kv_lora_rank=kv_lora_rank, qk_nope_head_dim=qk_nope_head_dim,
@@ -805,13 +883,22 @@ class TransformerBlock(nn.Module):
             self.mlp_res_proj = scaled_variance_linear(hidden_size, 1, bias=False,
                                                        init_constant=weight_init_constant)
 
-    def forward(self, x, rope_cos, rope_sin):
+    def forward(self, x, rope_cos, rope_sin, gates=None):
+        if gates is not None and not self.sandwich_norm:
+            raise ValueError("TransformerBlock: gates belong to sandwich_norm=True")
         # each norm's output feeds several linears (three in the attention with
         # its output gate, two in the MLP); _norm_fanout hands each its own copy
         na = 3 if self.attn.use_output_gate else 2
         x, *n1 = _norm_fanout(x, self.norm1, na)
         if na == 2:
             n1.append(n1[0])
+        if self.sandwich_norm:
+            attn_gate, mlp_gate = gates or (None, None)
+            a = self.attn._forward(*n1, rope_cos, rope_sin)
+            x, n2a, n2b = residual_norm(x, a, self.attn_scale, self.attn_post_norm.weight,
+                                        attn_gate, self.norm2.weight, self.norm2.eps, 2)
+            return residual_norm(x, self.mlp._forward(n2a, n2b), self.mlp_scale,
+                                 self.mlp_post_norm.weight, mlp_gate, eps=self.norm2.eps)[0]
         x = _residual(x, self.attn._forward(*n1, rope_cos, rope_sin), self.attn_scale)
         x, n2a, n2b = _norm_fanout(x, self.norm2, 2)
         return _residual(x, self.mlp._forward(n2a, n2b), self.mlp_scale)

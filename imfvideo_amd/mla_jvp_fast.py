@@ -224,7 +224,10 @@ def pack_block(block, tile_major=False):
       sla2 (SLA2AttentionImpl): alpha (H, Mb), the router projections, topk, bq, bk;
       any other impl is taken for dense softmax attention of every token to every token at
       scale 64^-1/2 (a partial of dense_attention that is not raises ValueError).
+    A block with norms behind its sublayers (sandwich_norm) raises ValueError.
     Rebuild after every optimizer step (the weights change)."""
+    if getattr(block, "sandwich_norm", False):
+        raise ValueError("pack_block: the fast JVP has no form of a block with sandwich_norm")
     p = mla_params_from_block(block)
     for name in ("attn_res_norm", "mlp_res_norm"):
         if hasattr(block, name):

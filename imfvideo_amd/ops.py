@@ -1868,3 +1868,86 @@ def linear_wgrad8(dy, a):
     _launch(dy.device, "sla2h_linear_wgrad8", d2.data_ptr(), ld, a.codes.data_ptr(),
             a.scales.data_ptr(), code, a.rows, M, a.cols, _ptr(ws), dw.data_ptr())
     return dw
+
+
+# ---------------------------------------------------------------------------
+# DiT block: the residual step with a norm on both sides (sla2h_residual_norm_*)
+# ---------------------------------------------------------------------------
+RESIDUAL_NORM_MAX = 8192  # channels
+_NORM_DTYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
+
+
+def _residual_norm_sizes(x, gate):
+    """(B, L, D): the clips that have gates of their own, or all rows as one clip."""
+    D = x.shape[-1]
+    if gate is None:
+        return 1, x.numel() // D, D
+    return x.shape[0], x.numel() // D // x.shape[0], D
+
+
+def _residual_norm_check(x, a, vectors, gate):
+    _need_gpu(x, a, gate, *vectors)
+    if x.dtype != torch.float32 or a.dtype not in _NORM_DTYPES:
+        raise TypeError("residual_norm: an fp32 residual stream and a 16-bit or fp32 sublayer "
+                        f"output, got {x.dtype} and {a.dtype}")
+    if a.shape != x.shape or x.dim() < 1 or x.numel() == 0 or x.shape[-1] > RESIDUAL_NORM_MAX:
+        raise ValueError(f"residual_norm: expected two tensors of one shape (..., D), D at most "
+                         f"{RESIDUAL_NORM_MAX}, got {tuple(x.shape)} and {tuple(a.shape)}")
+    D = x.shape[-1]
+    for v in vectors:
+        if tuple(v.shape) != (D,) or v.dtype != torch.float32:
+            raise ValueError(f"residual_norm: weights and scale are ({D},) float32, got "
+                             f"{tuple(v.shape)} {v.dtype}")
+    if gate is not None and (x.dim() < 2 or tuple(gate.shape) != (x.shape[0], D)
+                             or gate.dtype != torch.float32):
+        raise ValueError(f"residual_norm: gate is one row of {D} float32 per clip, got "
+                         f"{tuple(gate.shape)} {gate.dtype}")
+    if any(t.device != x.device for t in (a, *vectors) + (() if gate is None else (gate,))):
+        raise ValueError("residual_norm: operands on different devices")
+
+
+def residual_norm_fwd(x, a, scale, post, pre=None, gate=None, eps=1e-6):
+    """(y, n): y = x + scale * post * gate * a / rms(a) in fp32 and n = pre * y / rms(y) in
+    a's dtype (None without pre).  x (..., D) fp32, a (..., D) 16-bit or fp32, scale, post, pre
+    (D,) and gate (x.shape[0], D) fp32."""
+    _residual_norm_check(x, a, [v for v in (scale, post, pre) if v is not None], gate)
+    x, a, scale, post = x.contiguous(), a.contiguous(), scale.contiguous(), post.contiguous()
+    pre = None if pre is None else pre.contiguous()
+    gate = None if gate is None else gate.contiguous()
+    y = torch.empty_like(x)
+    n = None if pre is None else torch.empty_like(a)
+    _launch(x.device, "sla2h_residual_norm_fwd", x.data_ptr(), a.data_ptr(), _NORM_DTYPES[a.dtype],
+            scale.data_ptr(), post.data_ptr(), _ptr(pre), _ptr(gate),
+            *_residual_norm_sizes(x, gate), float(eps), y.data_ptr(), _ptr(n))
+    return y, n
+
+
+def residual_norm_bwd(dy, dns, y, a, scale, post, pre=None, gate=None, eps=1e-6):
+    """(dx, da, dscale, dpost, dpre, dgate) of residual_norm_fwd from its output y for the
+    gradient dy of y (or None) and the gradients dns of n (0 to 3 tensors of a's dtype, summed
+    in fp32); dpre is None without dns, dgate without gate."""
+    _residual_norm_check(y, a, [v for v in (scale, post, pre) if v is not None], gate)
+    if len(dns) > 3 or (dns and pre is None):
+        raise ValueError("residual_norm: up to three gradients of n, and none without pre")
+    for d, like in [(d, a) for d in dns] + ([] if dy is None else [(dy, y)]):
+        if d.shape != like.shape or d.dtype != like.dtype or d.device != like.device:
+            raise ValueError(f"residual_norm: a gradient like {tuple(like.shape)} {like.dtype} on "
+                             f"{like.device}, got {tuple(d.shape)} {d.dtype} on {d.device}")
+    dy = None if dy is None else dy.contiguous()
+    dns = [d.contiguous() for d in dns]
+    y, a, scale, post = y.contiguous(), a.contiguous(), scale.contiguous(), post.contiguous()
+    pre = pre.contiguous() if dns else None
+    gate = None if gate is None else gate.contiguous()
+    sizes = _residual_norm_sizes(y, gate)
+    dx, da = torch.empty_like(y), torch.empty_like(a)
+    dscale, dpost = torch.empty_like(scale), torch.empty_like(post)
+    dpre = torch.empty_like(pre) if dns else None
+    dgate = None if gate is None else torch.empty_like(gate)
+    lib = _lib._LIB or _lib.load()
+    ws = _scratch(lib.sla2h_residual_norm_bwd_workspace_bytes(*sizes), y.device)
+    dn = [d.data_ptr() for d in dns] + [None] * (3 - len(dns))
+    _launch(y.device, "sla2h_residual_norm_bwd", y.data_ptr() if dns else None, a.data_ptr(),
+            _NORM_DTYPES[a.dtype], scale.data_ptr(), post.data_ptr(), _ptr(pre), _ptr(gate),
+            _ptr(dy), *dn, *sizes, float(eps), dx.data_ptr(), da.data_ptr(), dscale.data_ptr(),
+            dpost.data_ptr(), _ptr(dpre), _ptr(dgate), ws.data_ptr())
+    return dx, da, dscale, dpost, dpre, dgate

@@ -925,6 +925,30 @@ int sla2h_linear_wgrad8(const void* dy, int64_t ldy, const int8_t* codes, const 
                         int dtype, int64_t rows, int M, int N, void* workspace, float* dw,
                         void* stream);
 
+/*
+ * The residual step between two sublayers with a norm on both of its sides.  x, y (B, L, D) fp32
+ * contiguous, a (B, L, D) contiguous of dtype (0 fp16, 1 bf16, 2 fp32), scale, post, pre (D,) and gate
+ * (B, D) fp32:
+ *   y = x + scale * post * gate_b * a / rms(a),  n = pre * y / rms(y),  rms = sqrt(mean(.^2) + eps)
+ * gate NULL: ones.  pre NULL: no n (both or neither); n like a.  fp32 arithmetic, n rounded
+ * once.  D <= 8192.
+ * Backward, from y and a: dy (fp32, may be NULL: zero) the gradient of y, dn0 .. dn2 those of n (like
+ * a; the later ones may be NULL, and dn0 with dpre and y where n has no gradient); dx (that of x, fp32), da
+ * (like a), dscale, dpost, dpre (D,), dgate (B, D, exactly where gate is given), all written.
+ * Column sums are added in a fixed order: reproducible.  Workspace, 16-byte aligned, of
+ * sla2h_residual_norm_bwd_workspace_bytes (0: sizes that are not taken).
+ */
+int sla2h_residual_norm_fwd(const float* x, const void* a, int dtype, const float* scale,
+                            const float* post, const float* pre, const float* gate, int64_t B,
+                            int64_t L, int D, float eps, float* y, void* n, void* stream);
+size_t sla2h_residual_norm_bwd_workspace_bytes(int64_t B, int64_t L, int D);
+int sla2h_residual_norm_bwd(const float* y, const void* a, int dtype, const float* scale,
+                            const float* post, const float* pre, const float* gate,
+                            const float* dy, const void* dn0, const void* dn1, const void* dn2,
+                            int64_t B, int64_t L, int D, float eps, float* dx, void* da,
+                            float* dscale, float* dpost, float* dpre, float* dgate,
+                            void* workspace, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
