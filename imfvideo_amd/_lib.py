@@ -171,6 +171,8 @@ SIGNATURES = {
     "sla2h_residual_norm_bwd_workspace_bytes": (ctypes.c_size_t, [_c_i64, _c_i64, _c_int]),
     "sla2h_residual_norm_bwd": (_c_int, [_p, _p, _c_int, _p, _p, _p, _p, _p, _p, _p, _p, _c_i64,
                                          _c_i64, _c_int, _c_f, _p, _p, _p, _p, _p, _p, _p, _p]),
+    "sla2h_orthogonalize_workspace_bytes": (ctypes.c_size_t, [_c_i64, _c_i64, _c_i64]),
+    "sla2h_orthogonalize": (_c_int, [_p, _c_int, _c_i64, _c_i64, _c_i64, _c_int, _p, _p, _p, _p]),
 }
 
 _LIB = None

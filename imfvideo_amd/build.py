@@ -34,6 +34,7 @@ SOURCES = {
     "dense_attn_bwd.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
     "act8.hip": [],
     "residual_norm.hip": [],
+    "ortho.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
     "mla_glue.hip": [],
     "block_train.hip": [],
     "linear_bwd.hip": [],

@@ -1951,3 +1951,53 @@ def residual_norm_bwd(dy, dns, y, a, scale, post, pre=None, gate=None, eps=1e-6)
             _ptr(dy), *dn, *sizes, float(eps), dx.data_ptr(), da.data_ptr(), dscale.data_ptr(),
             dpost.data_ptr(), _ptr(dpre), _ptr(dgate), ws.data_ptr())
     return dx, da, dscale, dpost, dpre, dgate
+
+
+# ---------------------------------------------------------------------------
+# Orthogonalised updates of weight matrices (sla2h_orthogonalize)
+# ---------------------------------------------------------------------------
+NS_COEFFS = (3.4445, -4.7750, 2.0315)  # slope 3.4 at 0, singular values to 0.7 .. 1.2
+
+
+@functools.lru_cache(maxsize=64)
+def _ns_coeffs(steps, coeffs):
+    rows = [coeffs] * steps if not isinstance(coeffs[0], tuple) else list(coeffs)
+    if steps < 1 or steps > 64 or len(rows) != steps or any(len(r) != 3 for r in rows):
+        raise ValueError("orthogonalize: 1 to 64 steps, three coefficients for all of them or for "
+                         f"each, got {steps} and {coeffs}")
+    flat = [float(x) for r in rows for x in r]
+    if not all(map(math.isfinite, flat)):
+        raise ValueError(f"orthogonalize: coefficients have to be finite, got {coeffs}")
+    return (ctypes.c_float * len(flat))(*flat)
+
+
+def ns_rows(steps, coeffs):
+    """coeffs as a tuple that a cache can hold: (a, b, c), or one such row per step."""
+    rows = tuple(coeffs)
+    return tuple(map(tuple, rows)) if rows and not isinstance(rows[0], (int, float)) else rows
+
+
+def orthogonalize(g, steps=5, coeffs=NS_COEFFS):
+    """Newton-Schulz products of each matrix of g (..., R, C), fp32 or 16-bit, in its type:
+    X = g / |g|, then `steps` times X <- a X + (b A + c A^2) X with A = X X^T on the shorter side,
+    coeffs (a, b, c) or such a row for every step.  Singular values go towards 1, singular vectors
+    stay.  Computed to fp32's accuracy whatever the type; zeros stay zeros."""
+    _need_gpu(g)
+    if g.dtype not in _NORM_DTYPES:
+        raise TypeError(f"orthogonalize: fp32 or 16-bit matrices, got {g.dtype}")
+    if g.dim() < 2:
+        raise ValueError(f"orthogonalize: expected (..., R, C), got {tuple(g.shape)}")
+    table = _ns_coeffs(steps, ns_rows(steps, coeffs))
+    out = torch.empty(g.shape, device=g.device, dtype=g.dtype)
+    if g.numel() == 0:
+        return out
+    g = g.contiguous()
+    R, C = g.shape[-2:]
+    n = g.numel() // (R * C)
+    need = (_lib._LIB or _lib.load()).sla2h_orthogonalize_workspace_bytes(n, R, C)
+    if not need:
+        raise ValueError(f"orthogonalize: too large: {tuple(g.shape)} (sides up to 32,768)")
+    ws = _scratch(need, g.device)
+    _launch(g.device, "sla2h_orthogonalize", g.data_ptr(), _NORM_DTYPES[g.dtype], n, R, C, steps,
+            table, ws.data_ptr(), out.data_ptr())
+    return out

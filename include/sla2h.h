@@ -949,6 +949,21 @@ int sla2h_residual_norm_bwd(const float* y, const void* a, int dtype, const floa
                             float* dscale, float* dpost, float* dpre, float* dgate,
                             void* workspace, void* stream);
 
+/*
+ * Orthogonalised updates: each of the n matrices g (n, R, C) contiguous of dtype (0 fp16, 1 bf16, 2
+ * fp32) through `steps` Newton-Schulz steps on its shorter side,
+ *   X = g / |g|_F,  X <- a X + (b A + c A^2) X with A = X X^T,
+ * coeffs: host array of 3 steps floats, (a, b, c) of each; out like g (may be g).  A matrix of zeros
+ * stays zeros; one that is not finite is NaN.  fp32-exact products of pairs of 16-bit numbers: |X| of
+ * the steps below 16, |A| below 16 and |b A + c A^2| below 128 (elementwise), else infinities.  R,
+ * C <= 32768.  Workspace, 16-byte aligned, of sla2h_orthogonalize_workspace_bytes (0: sizes that are
+ * not taken).  Reproducible; a matrix's result does not depend on the others.
+ * The Muon optimiser's step (the reference's moonlight.py).
+ */
+size_t sla2h_orthogonalize_workspace_bytes(int64_t n, int64_t R, int64_t C);
+int sla2h_orthogonalize(const void* g, int dtype, int64_t n, int64_t R, int64_t C, int steps,
+                        const float* coeffs, void* workspace, void* out, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
