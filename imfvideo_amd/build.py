@@ -32,6 +32,8 @@ SOURCES = {
     "attn_bwd.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
     "dense_attn.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
     "dense_attn_bwd.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
+    "diff_attn.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
+    "diff_attn_bwd.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
     "act8.hip": [],
     "residual_norm.hip": [],
     "ortho.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],

@@ -158,6 +158,102 @@ inline bool sizes_ok(int B, int H, int Hkv, int64_t Lq, int64_t Lk) {
          (int64_t)B * H < ((int64_t)1 << 20) && (H / Hkv) * Lq < ((int64_t)1 << 31);
 }
 
+// ---- Softmax in one pass over the keys (forward kernels): see dense_attn.hip.
+
+// Probabilities are held as exp2(S - m + shift); a lane's sum of 16 stays at or below `most`.
+// fp16 spends its exponent range on the small ones (2^-24 to 2^15); bf16 has fp32's range.
+template <typename T16>
+struct Range;
+template <>
+struct Range<BF16> {
+  static constexpr float shift = 0.f, most = 1024.f;
+};
+template <>
+struct Range<F16> {
+  static constexpr float shift = 9.f, most = 32768.f;
+};
+constexpr float kFloor = -1e30f;  // m before the first key (finite: -inf - m stays -inf)
+
+// Largest of a lane's 16 scores.
+__device__ inline float lane_max(const f32x16& s) {
+  float mx = fmaxf(fmaxf(s[0], s[1]), s[2]);
+#pragma unroll
+  for (int i = 3; i < 15; i += 2) mx = fmaxf(fmaxf(mx, s[i]), s[i + 1]);
+  return fmaxf(mx, s[15]);
+}
+
+// Moves the bound of a 32-key x 32-query tile to its maximum and rescales what the old
+// bound weighed.
+template <int MB>
+__device__ inline void raise_bound(float mx, float c, float& m, float& lsum, f32x16 (&acc)[MB]) {
+  const float mn = fmaxf(m, swap32_max(mx) * c);
+  const float f = fast_exp2(m - mn);
+  m = mn;
+  lsum *= f;
+#pragma unroll
+  for (int b = 0; b < MB; ++b)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) acc[b][i] *= f;
+}
+
+// Probabilities of a tile, packed as the operands of the two product steps; their sum.
+template <typename T16>
+__device__ inline float probabilities(const f32x16& s, float c, float m, u32x4 (&p)[2]) {
+  const float off = Range<T16>::shift - m;
+  f32x16 e;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) e[i] = fast_exp2(__builtin_fmaf(s[i], c, off));
+#pragma unroll
+  for (int t = 0; t < 2; ++t) p[t] = pack_step<T16>(e, t);
+  float r[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) r[i] = (e[i] + e[4 + i]) + (e[8 + i] + e[12 + i]);
+  return (r[0] + r[1]) + (r[2] + r[3]);
+}
+
+// What the rounding of a tile's probabilities lost, packed alike.
+template <typename T16>
+__device__ inline void lost_halves(const f32x16& s, float c, float m, const u32x4 (&p)[2],
+                                   u32x4 (&q)[2]) {
+  const float off = Range<T16>::shift - m;
+#pragma unroll
+  for (int t = 0; t < 2; ++t)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int k = 8 * t + 2 * i;
+      const uint32_t w = p[t][i];
+      q[t][i] = pack_pair<T16>(
+          fast_exp2(__builtin_fmaf(s[k], c, off)) - T16::to_f32((uint16_t)(w & 0xffff)),
+          fast_exp2(__builtin_fmaf(s[k + 1], c, off)) - T16::to_f32((uint16_t)(w >> 16)));
+    }
+}
+
+// scores of keys at or past a lane's limit -> -inf; lim counts from the tile's first key
+__device__ inline void mask_tile(f32x16& s, int lim, int h) {
+  const int x = lim - 4 * h;
+#pragma unroll
+  for (int i = 0; i < 16; ++i)
+    s[i] = 8 * (i >> 2) + (i & 3) < x ? s[i] : -__builtin_inff();
+}
+
+// Two values as 16 bits, and what the rounding lost as 16 bits again (0 past the type's range).
+template <typename T16>
+__device__ inline uint32_t round_pair(float x, float y, uint32_t& lost) {
+  const uint32_t p = pack_pair<T16>(x, y);
+  const float ex = x - T16::to_f32((uint16_t)(p & 0xffff)), ey = y - T16::to_f32((uint16_t)(p >> 16));
+  lost = pack_pair<T16>(__builtin_fabsf(ex) < __builtin_inff() ? ex : 0.f,
+                        __builtin_fabsf(ey) < __builtin_inff() ? ey : 0.f);
+  return p;
+}
+
+// Keys that query i sees: [0, limit).
+__device__ inline int key_limit(int i, int qlen, int klen, int causal) {
+  if (i >= qlen) return 0;
+  if (!causal) return klen;
+  const int64_t e = (int64_t)i + klen - qlen + 1;
+  return e < 0 ? 0 : (e < klen ? (int)e : klen);
+}
+
 // Which head and tile a workgroup takes.  Workgroups go to the eight XCDs in turn, each with
 // an L2 of its own.
 //   even tiles (no mask, no lengths): an XCD takes a run of neighbouring tiles, so that those of

@@ -1,0 +1,665 @@
+// Differential attention, forward, gfx950: a pair p of heads (2p, 2p + 1) attends twice with the same
+// 128 value channels (value heads 2p and 2p + 1 side by side),
+//
+//   A_m = softmax(c q_m k_m^T) (m = 1, 2; keys j < k_len, causal: j <= i + k_len - q_len),
+//   o = (A_1 - lam_p A_2) v;   a row without a key is 0.
+//
+// One pass over the keys, each map as in dense_attn.hip: O_m^T += V^T P_m^T with P_m = exp2(S - m)
+// in 16 bits, row sums of the fp32 values, a bound m that moves only when a tile outgrows it.  The two
+// sums meet at the end, when both normalisers are known: six products of 64 channels per (query,
+// key) where a second pass over the scores would make it 2 + 2 + 2 and the exponentials twice.
+// A wave belongs to one map: it holds 128 channels of its rows' sums and reads its own keys and all
+// values; the waves of the other map sit beside it in the workgroup and hand their result over
+// through LDS.  (Both maps in one wave would need both maps' queries and twice the sums for the same rows:
+// half the rows per value operand read from LDS.)
+#include "diff_attn.h"
+
+#include <initializer_list>
+
+namespace sla2h {
+
+namespace {
+
+struct DiffFwdArgs {
+  const uint16_t *q, *k, *v;
+  const float* lam;  // (P)
+  uint16_t* o;       // (B, Lq, H, 64)
+  float* maps;       // (B, Lq, P, 2, 128): A_m v, or null
+  float* lse;        // (B, H, Lq) or null
+  const int32_t *q_lens, *k_lens;
+  int64_t qb, qh, ql, kb, kh, kl, vb, vh, vl;  // strides in elements
+  int64_t Lq, Lk;
+  int P, Pk, rep;  // pairs of query heads, of key heads
+  int causal;
+  float c;  // scale * log2(e)
+  WorkMap map;
+  int qtiles;
+  float* part;   // [range][map][B * P * Lq][128] unnormalised sums
+  float2* ml;    // [range][map][B * P * Lq] (m, l)
+  int splits, units;  // few queries: 32-key units of a range
+  int64_t nrows;      // B * P * Lq
+};
+
+// Element of a row's results: pair bp = b P + p, row i.
+__device__ inline uint16_t* out_row(const DiffFwdArgs& a, int64_t bp, int64_t i) {
+  const int64_t b = bp / a.P, p = bp - b * a.P;
+  return a.o + ((b * a.Lq + i) * a.P + p) * 128;
+}
+
+// Workgroup = 4 waves: two query groups of 32 NQ rows x two maps, of one pair.  Stages of 32 keys
+// (k of both maps, the 128 value channels) three ahead in four LDS slots, one barrier each.  The
+// scores of a wave's first 32 rows are one stage ahead, so that they run on the matrix cores under
+// the exponentials of its other rows, and those of the other rows under the first ones'.
+template <typename T16, int NQ>
+__global__ __launch_bounds__(256, 2) void diff_fwd_kernel(DiffFwdArgs a) {
+  __shared__ __align__(16) unsigned char s0[kStageB], s1[kStageB], s2[kStageB], s3[kStageB],
+      s4[kStageB];
+  int bp, item;
+  if (!work_item(a.map, blockIdx.x, bp, item)) return;
+  const int qt = item / a.splits, sp = item - qt * a.splits;
+  const int b = bp / a.P, p = bp - b * a.P, kp = p / a.rep;
+  const int tid = threadIdx.x, l = tid & 63, h = l >> 5;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6), m = w & 1;
+  const LaneOff lo(l);
+  const int qlen = seq_len(a.q_lens, b, a.Lq), klen = seq_len(a.k_lens, b, a.Lk);
+
+  const int q0 = qt * (64 * NQ);               // first row of the workgroup
+  const int qw = q0 + (w >> 1) * (32 * NQ);    // ... of the wave
+  const int qend = min(q0 + 64 * NQ, qlen);
+  const int kmax = qend > q0 ? key_limit(qend - 1, qlen, klen, a.causal) : 0;
+  const int nunit = (kmax + kUnitRows - 1) / kUnitRows;
+  const int per = (nunit + a.splits - 1) / a.splits;
+  const int t0 = sp * per, nt = min(nunit, t0 + per);  // this range's stages
+
+  // wave w loads the stage's matrix w: k of map 0, of map 1, the lower and the upper value channels
+  const uint16_t* src = w < 2 ? a.k + b * a.kb + (2 * kp + w) * a.kh
+                              : a.v + b * a.vb + (2 * kp + w - 2) * a.vh;
+  const int64_t ld = (w < 2 ? a.kl : a.vl) * 2;
+  auto load = [&](int t, unsigned char* s) __attribute__((always_inline)) {
+    const int64_t row = (int64_t)t * kUnitRows;
+    load_unit(src, row, (int64_t)klen - row, ld, s + w * kUnitB, l);
+  };
+
+  u32x4 qf[NQ][4];
+  int lim[NQ];
+  {
+    const uint16_t* qp = a.q + b * a.qb + (2 * p + m) * a.qh;
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) {
+      const int i = qw + 32 * n + (l & 31);
+      lim[n] = key_limit(i, qlen, klen, a.causal);
+#pragma unroll
+      for (int s = 0; s < 4; ++s)
+        qf[n][s] = i < qlen ? *reinterpret_cast<const u32x4*>(qp + i * a.ql + 16 * s + 8 * h)
+                            : u32x4{0, 0, 0, 0};
+    }
+  }
+  // keys that every query of the wave sees, and that any of them sees
+  const int wlast = min(qw + 32 * NQ, qlen) - 1;
+  const int wany = wlast >= qw ? key_limit(wlast, qlen, klen, a.causal) : 0;
+  const int wall = wlast >= qw ? key_limit(qw, qlen, klen, a.causal) : 0;
+
+  f32x16 acc[NQ][4];
+  float mx[NQ], lsum[NQ];
+#pragma unroll
+  for (int n = 0; n < NQ; ++n) {
+#pragma unroll
+    for (int mb = 0; mb < 4; ++mb) acc[n][mb] = zero16();
+    mx[n] = kFloor;
+    lsum[n] = 0.f;
+  }
+  f32x16 sc[NQ];
+  u32x4 kf[4], pr[NQ][2];
+  auto read_k = [&](const unsigned char* s) __attribute__((always_inline)) {
+#pragma unroll
+    for (int x = 0; x < 4; ++x) kf[x] = row_frag(s + m * kUnitB, 0, x, lo);
+  };
+  auto scores = [&](int n) __attribute__((always_inline)) {
+    sc[n] = zero16();
+#pragma unroll
+    for (int x = 0; x < 4; ++x) sc[n] = mfma_32x32x16<T16>(kf[x], qf[n][x], sc[n]);
+  };
+  auto mask = [&](int n, int base) __attribute__((always_inline)) {
+    if (base + kUnitRows > wall) {
+      asm volatile("");  // a branch: rare, and 16 selects when speculated
+      mask_tile(sc[n], lim[n] - base, h);
+    }
+  };
+  // rows n again under a new bound: `cur` is the stage of their keys, `nxt` what kf holds after it
+  auto again = [&](int n, int base, const unsigned char* cur, const unsigned char* nxt)
+      __attribute__((always_inline)) {
+    f32x16 other;
+    if (NQ == 2) other = sc[n ^ 1];
+    read_k(cur);
+    scores(n);
+    mask(n, base);
+    raise_bound(lane_max(sc[n]), a.c, mx[n], lsum[n], acc[n]);
+    const float r = probabilities<T16>(sc[n], a.c, mx[n], pr[n]);
+    read_k(nxt);
+    if (NQ == 2) sc[n ^ 1] = other;
+    return r;
+  };
+  auto values = [&](int n, const unsigned char* cur) __attribute__((always_inline)) {
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+      for (int mb = 0; mb < 4; ++mb)
+        acc[n][mb] = mfma_32x32x16<T16>(
+            col_frag(cur + (2 + (mb >> 1)) * kUnitB, 16 * s, mb & 1, lo), pr[n][s], acc[n][mb]);
+  };
+  auto stage = [&](int t, const unsigned char* prev, const unsigned char* cur,
+                   const unsigned char* nxt, unsigned char* to) __attribute__((always_inline)) {
+    // the stages up to t + 1 have landed, stage t - 2 is read
+    __builtin_amdgcn_s_waitcnt(wait_vm_lgkm0(4));
+    __builtin_amdgcn_s_barrier();
+    load(t + 3, to);
+    const int base = t * kUnitRows;
+    mask(0, base);
+    if (NQ == 2) {
+      scores(NQ - 1);
+      values(NQ - 1, prev);
+    }
+    float r = probabilities<T16>(sc[0], a.c, mx[0], pr[0]);
+    if (__builtin_amdgcn_ballot_w64(r > Range<T16>::most)) r = again(0, base, cur, cur);
+    lsum[0] += r;
+    if (NQ == 2) mask(NQ - 1, base);
+    read_k(nxt);
+    scores(0);
+    values(0, cur);
+    if (NQ == 2) {
+      r = probabilities<T16>(sc[NQ - 1], a.c, mx[NQ - 1], pr[NQ - 1]);
+      if (__builtin_amdgcn_ballot_w64(r > Range<T16>::most)) r = again(NQ - 1, base, cur, nxt);
+      lsum[NQ - 1] += r;
+    }
+  };
+  load(t0, s0);
+  load(t0 + 1, s1);
+  load(t0 + 2, s2);
+  __builtin_amdgcn_s_waitcnt(wait_vm_lgkm0(8));
+  __builtin_amdgcn_s_barrier();
+  read_k(s0);
+  scores(0);
+#pragma unroll
+  for (int n = 0; n < NQ; ++n) pr[n][0] = pr[n][1] = u32x4{0, 0, 0, 0};
+  // The first stage adds what its own slot holds with probabilities of 0; the other rows of the
+  // last stage that the wave has keys in come behind the loop, and then the waits and loads alone.
+  const int wn = min(nt, (wany + kUnitRows - 1) / kUnitRows);
+  const unsigned char* last = s0;
+  for (int t = t0; t < wn; t += 5) {
+    stage(t, t == t0 ? s0 : s4, s0, s1, s3);
+    last = s0;
+    if (t + 1 >= wn) break;
+    stage(t + 1, s0, s1, s2, s4);
+    last = s1;
+    if (t + 2 >= wn) break;
+    stage(t + 2, s1, s2, s3, s0);
+    last = s2;
+    if (t + 3 >= wn) break;
+    stage(t + 3, s2, s3, s4, s1);
+    last = s3;
+    if (t + 4 >= wn) break;
+    stage(t + 4, s3, s4, s0, s2);
+    last = s4;
+  }
+  if (NQ == 2) values(NQ - 1, last);
+  for (int t = max(wn, t0); t < nt; ++t) {
+    __builtin_amdgcn_s_waitcnt(wait_vm_lgkm0(4));
+    __builtin_amdgcn_s_barrier();
+    const int x = (t + 3 - t0) % 5;
+    load(t + 3, x == 0 ? s0 : x == 1 ? s1 : x == 2 ? s2 : x == 3 ? s3 : s4);
+  }
+  __builtin_amdgcn_s_waitcnt(wait_vm_lgkm0(0));  // no load into this LDS outlives the workgroup
+
+  float inv[NQ];
+#pragma unroll
+  for (int n = 0; n < NQ; ++n) {
+    const int i = qw + 32 * n + (l & 31);
+    const float ls = swap32_sum(lsum[n]);
+    if (a.splits > 1) {
+      if (i >= a.Lq) continue;
+      const int64_t flat = (sp * 2 + m) * a.nrows + (int64_t)bp * a.Lq + i;
+#pragma unroll
+      for (int mb = 0; mb < 4; ++mb)
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+          *reinterpret_cast<f32x4*>(a.part + flat * 128 + 32 * mb + 8 * g + 4 * h) =
+              f32x4{acc[n][mb][4 * g], acc[n][mb][4 * g + 1], acc[n][mb][4 * g + 2],
+                    acc[n][mb][4 * g + 3]};
+      if (h == 0) a.ml[flat] = make_float2(mx[n], ls);
+      continue;
+    }
+    inv[n] = 1.f / ls;  // a row whose scores are all -inf is NaN
+#pragma unroll
+    for (int mb = 0; mb < 4; ++mb)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[n][mb][e] = lim[n] > 0 ? acc[n][mb][e] * inv[n] : 0.f;
+    if (i >= a.Lq) continue;
+    if (a.maps) {
+      float* d = a.maps + ((((int64_t)b * a.Lq + i) * a.P + p) * 2 + m) * 128;
+#pragma unroll
+      for (int mb = 0; mb < 4; ++mb)
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+          *reinterpret_cast<f32x4*>(d + 32 * mb + 8 * g + 4 * h) =
+              f32x4{acc[n][mb][4 * g], acc[n][mb][4 * g + 1], acc[n][mb][4 * g + 2],
+                    acc[n][mb][4 * g + 3]};
+    }
+    if (a.lse && h == 0)
+      a.lse[((int64_t)b * 2 * a.P + 2 * p + m) * a.Lq + i] =
+          lim[n] > 0 ? (mx[n] - Range<T16>::shift + __log2f(ls)) * kLn2 : -__builtin_inff();
+  }
+  if (a.splits > 1) return;
+
+  // map 1's rows through LDS: 16 KB per 32 rows, quads of channels of all rows beside each other
+  __syncthreads();
+  auto slot = [&](int n) __attribute__((always_inline)) {
+    const int x = (w >> 1) * NQ + n;
+    return reinterpret_cast<f32x4*>(x == 0 ? s0 : x == 1 ? s1 : x == 2 ? s2 : s3);
+  };
+  if (m == 1) {
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) {
+      f32x4* x = slot(n);
+#pragma unroll
+      for (int mb = 0; mb < 4; ++mb)
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+          x[(8 * mb + 2 * g + h) * 32 + (l & 31)] = f32x4{acc[n][mb][4 * g], acc[n][mb][4 * g + 1],
+                                                          acc[n][mb][4 * g + 2], acc[n][mb][4 * g + 3]};
+    }
+  }
+  __syncthreads();
+  if (m == 1) return;
+  const float lam = a.lam[p];
+#pragma unroll
+  for (int n = 0; n < NQ; ++n) {
+    const int i = qw + 32 * n + (l & 31);
+    if (i >= a.Lq) continue;
+    const f32x4* x = slot(n);
+    uint16_t* d = out_row(a, bp, i);
+#pragma unroll
+    for (int mb = 0; mb < 4; ++mb)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const f32x4 y = x[(8 * mb + 2 * g + h) * 32 + (l & 31)];
+        float z[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          z[e] = lim[n] > 0 ? __builtin_fmaf(-lam, y[e], acc[n][mb][4 * g + e]) : 0.f;
+        *reinterpret_cast<u32x2*>(d + 32 * mb + 8 * g + 4 * h) =
+            u32x2{pack_pair<T16>(z[0], z[1]), pack_pair<T16>(z[2], z[3])};
+      }
+  }
+}
+
+// Writes eight channels of a finished row: o, and for a backward the maps' rows and log-sum-exps.
+template <typename T16>
+__device__ inline void finish_row(const DiffFwdArgs& a, int64_t bp, int64_t i, int c0, bool some,
+                                  const float (&x)[2][8], const float (&mm)[2],
+                                  const float (&ll)[2]) {
+  const int64_t b = bp / a.P, p = bp - b * a.P;
+  const float lam = a.lam[p];
+  float y[2][8];
+#pragma unroll
+  for (int m = 0; m < 2; ++m) {
+    const float inv = 1.f / ll[m];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) y[m][e] = some ? x[m][e] * inv : 0.f;
+    if (a.maps) {
+      float* d = a.maps + (((b * a.Lq + i) * a.P + p) * 2 + m) * 128 + c0;
+      *reinterpret_cast<f32x4*>(d) = f32x4{y[m][0], y[m][1], y[m][2], y[m][3]};
+      *reinterpret_cast<f32x4*>(d + 4) = f32x4{y[m][4], y[m][5], y[m][6], y[m][7]};
+    }
+    if (a.lse && c0 == 0)
+      a.lse[(b * 2 * a.P + 2 * p + m) * a.Lq + i] =
+          some ? (mm[m] - Range<T16>::shift + __log2f(ll[m])) * kLn2 : -__builtin_inff();
+  }
+  u32x4 z;
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    z[e] = some ? pack_pair<T16>(__builtin_fmaf(-lam, y[1][2 * e], y[0][2 * e]),
+                                 __builtin_fmaf(-lam, y[1][2 * e + 1], y[0][2 * e + 1]))
+                : 0u;
+  *reinterpret_cast<u32x4*>(out_row(a, bp, i) + c0) = z;
+}
+
+// Few queries: workgroup = 32 rows (of the `rep` query pairs that share a key pair) over one range of
+// keys; its waves take the 32-key units in turn, both maps of a unit, each with two LDS slots of its own
+// (no barrier in the loop; 128 KB, one workgroup per CU), and their sums are joined in LDS.  The products
+// wait for the loads here, so what the rounding of P lost is always added by a second one.
+template <typename T16>
+__global__ __launch_bounds__(256, 1) void diff_fwd_split_kernel(DiffFwdArgs a) {
+  __shared__ __align__(16) unsigned char kv[2][4][kStageB];
+  __shared__ float mls[4][2][2][32];  // wave, map, (m, l)
+  const int blk = blockIdx.x / a.splits, sp = blockIdx.x - blk * a.splits;
+  const int bk = __builtin_amdgcn_readfirstlane(blk / a.qtiles);
+  const int qt = __builtin_amdgcn_readfirstlane(blk - bk * a.qtiles);
+  const int b = bk / a.Pk, kp = bk - b * a.Pk;
+  const int tid = threadIdx.x, l = tid & 63, h = l >> 5;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const LaneOff lo(l);
+  const int qlen = seq_len(a.q_lens, b, a.Lq), klen = seq_len(a.k_lens, b, a.Lk);
+
+  // row of the group: pair kp rep + row / Lq, query row % Lq
+  const int64_t row = (int64_t)qt * 32 + (l & 31);
+  const bool live = row < (int64_t)a.rep * a.Lq;
+  const int p = kp * a.rep + (live ? (int)(row / a.Lq) : 0);
+  const int i = live ? (int)(row % a.Lq) : 0;
+  const int lim = live ? key_limit(i, qlen, klen, a.causal) : 0;
+  int kmax = lim, kmin = lim;
+#pragma unroll
+  for (int s = 16; s >= 1; s >>= 1) {
+    kmax = max(kmax, __shfl_xor(kmax, s, 64));
+    kmin = min(kmin, __shfl_xor(kmin, s, 64));
+  }
+  kmax = __builtin_amdgcn_readfirstlane(kmax);
+  kmin = __builtin_amdgcn_readfirstlane(kmin);
+
+  const int64_t u0 = (int64_t)sp * a.units;
+  const int64_t uend = min(u0 + a.units, ((int64_t)kmax + kUnitRows - 1) / kUnitRows);
+  auto load = [&](int64_t u, unsigned char* s) __attribute__((always_inline)) {
+    const int64_t n = u < uend ? (int64_t)klen - u * kUnitRows : 0;
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      load_unit(a.k + b * a.kb + (2 * kp + x) * a.kh, u * kUnitRows, n, a.kl * 2, s + x * kUnitB, l);
+      load_unit(a.v + b * a.vb + (2 * kp + x) * a.vh, u * kUnitRows, n, a.vl * 2,
+                s + (2 + x) * kUnitB, l);
+    }
+  };
+
+  u32x4 qf[2][4];
+#pragma unroll
+  for (int m = 0; m < 2; ++m) {
+    const uint16_t* qp = a.q + b * a.qb + (2 * p + m) * a.qh + i * a.ql;
+#pragma unroll
+    for (int s = 0; s < 4; ++s)
+      qf[m][s] = lim > 0 ? *reinterpret_cast<const u32x4*>(qp + 16 * s + 8 * h) : u32x4{0, 0, 0, 0};
+  }
+  f32x16 acc[2][4];
+  float mx[2], lsum[2];
+#pragma unroll
+  for (int m = 0; m < 2; ++m) {
+#pragma unroll
+    for (int mb = 0; mb < 4; ++mb) acc[m][mb] = zero16();
+    mx[m] = kFloor;
+    lsum[m] = 0.f;
+  }
+  auto compute = [&](int64_t u, const unsigned char* s) __attribute__((always_inline)) {
+    u32x4 pr[2][2], lost[2][2];
+#pragma unroll
+    for (int m = 0; m < 2; ++m) {
+      f32x16 sc = zero16();
+#pragma unroll
+      for (int x = 0; x < 4; ++x)
+        sc = mfma_32x32x16<T16>(row_frag(s + m * kUnitB, 0, x, lo), qf[m][x], sc);
+      if (u * kUnitRows + kUnitRows > kmin) mask_tile(sc, (int)(lim - u * kUnitRows), h);
+      // the wave's first unit sets the bound of the rows that see a key of it
+      float r = probabilities<T16>(sc, a.c, mx[m], pr[m]);
+      if (__builtin_amdgcn_ballot_w64(r > Range<T16>::most)) {
+        raise_bound(lane_max(sc), a.c, mx[m], lsum[m], acc[m]);
+        r = probabilities<T16>(sc, a.c, mx[m], pr[m]);
+      }
+      lsum[m] += r;
+      lost_halves<T16>(sc, a.c, mx[m], pr[m], lost[m]);
+    }
+#pragma unroll
+    for (int x = 0; x < 2; ++x)
+#pragma unroll
+      for (int mb = 0; mb < 4; ++mb) {
+        const u32x4 vf = col_frag(s + (2 + (mb >> 1)) * kUnitB, 16 * x, mb & 1, lo);
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+          acc[m][mb] = mfma_32x32x16<T16>(vf, pr[m][x], acc[m][mb]);
+          acc[m][mb] = mfma_32x32x16<T16>(vf, lost[m][x], acc[m][mb]);
+        }
+      }
+  };
+  int64_t u = u0 + w;
+  load(u, kv[0][w]);
+  for (; u < uend; u += 8) {
+    load(u + 4, kv[1][w]);
+    __builtin_amdgcn_s_waitcnt(wait_vm_lgkm0(16));
+    compute(u, kv[0][w]);
+    if (u + 4 >= uend) break;
+    __builtin_amdgcn_s_waitcnt(wait_vm_lgkm0(16));  // the reads of this slot are done
+    load(u + 8, kv[0][w]);
+    __builtin_amdgcn_s_waitcnt(wait_vm_lgkm0(16));
+    compute(u + 4, kv[1][w]);
+    __builtin_amdgcn_s_waitcnt(wait_vm_lgkm0(16));
+  }
+  __builtin_amdgcn_s_waitcnt(wait_vm_lgkm0(0));
+
+  // join the four waves: fp32 O^T tiles [channel][row] of both maps in the slots' memory
+#pragma unroll
+  for (int m = 0; m < 2; ++m) {
+    const float ls = swap32_sum(lsum[m]);
+    if (h == 0) {
+      mls[w][m][0][l] = mx[m];
+      mls[w][m][1][l] = ls;
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int m = 0; m < 2; ++m) {
+    float* ot = reinterpret_cast<float*>(kv[m][w]);
+#pragma unroll
+    for (int mb = 0; mb < 4; ++mb)
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        ot[(32 * mb + 8 * (r >> 2) + 4 * h + (r & 3)) * 32 + (l & 31)] = acc[m][mb][r];
+  }
+  __syncthreads();
+  // thread: row tid % 32, channels 8 (tid / 32) + 64 k ..
+  const int r = tid & 31;
+  const int64_t orow = (int64_t)qt * 32 + r;
+  if (orow >= (int64_t)a.rep * a.Lq) return;
+  const int64_t op = (int64_t)b * a.P + kp * a.rep + orow / a.Lq, oi = orow % a.Lq;
+  const int64_t flat = op * a.Lq + oi;
+  float mm[2], ll[2], f[2][4];
+#pragma unroll
+  for (int m = 0; m < 2; ++m) {
+    mm[m] = fmaxf(fmaxf(mls[0][m][0][r], mls[1][m][0][r]), fmaxf(mls[2][m][0][r], mls[3][m][0][r]));
+    ll[m] = 0.f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      f[m][j] = fast_exp2(mls[j][m][0][r] - mm[m]);
+      ll[m] += f[m][j] * mls[j][m][1][r];
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const int c0 = 64 * k + (tid >> 5) * 8;
+    float x[2][8];
+#pragma unroll
+    for (int m = 0; m < 2; ++m) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        x[m][e] = 0.f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          x[m][e] += f[m][j] * reinterpret_cast<const float*>(kv[m][j])[(c0 + e) * 32 + r];
+      }
+      if (a.splits > 1) {
+        float* d = a.part + ((sp * 2 + m) * a.nrows + flat) * 128 + c0;
+        *reinterpret_cast<f32x4*>(d) = f32x4{x[m][0], x[m][1], x[m][2], x[m][3]};
+        *reinterpret_cast<f32x4*>(d + 4) = f32x4{x[m][4], x[m][5], x[m][6], x[m][7]};
+        if (c0 == 0) a.ml[(sp * 2 + m) * a.nrows + flat] = make_float2(mm[m], ll[m]);
+      }
+    }
+    if (a.splits == 1)
+      finish_row<T16>(a, op, oi, c0, key_limit((int)oi, qlen, klen, a.causal) > 0, x, mm, ll);
+  }
+}
+
+// Joins the key ranges of a row: 16 groups of 16 lanes (eight channels each) take the ranges in turn,
+// both maps, and their sums are added in order.
+template <typename T16>
+__global__ __launch_bounds__(256) void diff_join_kernel(DiffFwdArgs a) {
+  __shared__ float sm[2][16], sl[2][16];
+  __shared__ f32x4 sx[2][16][32];
+  const int64_t flat = blockIdx.x;
+  const int grp = threadIdx.x >> 4, c0 = (threadIdx.x & 15) * 8;
+  const int64_t bp = flat / a.Lq, i = flat - bp * a.Lq;
+  const int b = (int)(bp / a.P);
+  const int qlen = seq_len(a.q_lens, b, a.Lq), klen = seq_len(a.k_lens, b, a.Lk);
+#pragma unroll
+  for (int m = 0; m < 2; ++m) {
+    float mm = kFloor, ll = 0.f;
+    f32x4 x{0.f, 0.f, 0.f, 0.f}, y = x;
+    for (int s = grp; s < a.splits; s += 16) {
+      const int64_t at = (s * 2 + m) * a.nrows + flat;
+      const float2 ml = a.ml[at];
+      const f32x4* src = reinterpret_cast<const f32x4*>(a.part + at * 128 + c0);
+      const float mn = fmaxf(mm, ml.x), f = fast_exp2(mm - mn), g = fast_exp2(ml.x - mn);
+      mm = mn;
+      ll = ll * f + g * ml.y;
+      x = x * f + g * src[0];
+      y = y * f + g * src[1];
+    }
+    sx[m][grp][c0 / 4] = x;
+    sx[m][grp][c0 / 4 + 1] = y;
+    if (c0 == 0) sm[m][grp] = mm, sl[m][grp] = ll;
+  }
+  __syncthreads();
+  if (grp) return;
+  float mm[2], ll[2], x[2][8];
+#pragma unroll
+  for (int m = 0; m < 2; ++m) {
+    mm[m] = kFloor;
+    ll[m] = 0.f;
+#pragma unroll
+    for (int j = 0; j < 16; ++j) mm[m] = fmaxf(mm[m], sm[m][j]);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[m][e] = 0.f;
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      const float f = fast_exp2(sm[m][j] - mm[m]);
+      ll[m] += f * sl[m][j];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[m][e] += f * sx[m][j][c0 / 4 + (e >> 2)][e & 3];
+    }
+  }
+  finish_row<T16>(a, bp, i, c0, key_limit((int)i, qlen, klen, a.causal) > 0, x, mm, ll);
+}
+
+// The form of a call: query blocks of 128 or 64 rows, or of 32 rows of a key pair's group.
+struct FwdPlan {
+  int nq;  // 2, 1: diff_fwd_kernel<NQ>; 0: diff_fwd_split_kernel
+  int64_t qtiles, nwork;
+  int splits;  // ranges of keys
+  int64_t units;
+};
+
+FwdPlan fwd_plan(int B, int H, int Hkv, int64_t Lq, int64_t Lk) {
+  FwdPlan p{};
+  const int64_t bp = (int64_t)B * H / 2, bk = (int64_t)B * Hkv / 2, rep = H / Hkv;
+  p.splits = 1;
+  p.nq = 2;
+  p.qtiles = (Lq + 127) / 128;
+  p.nwork = bp * p.qtiles;
+  if (p.nwork >= 256) return p;
+  p.nq = 1;
+  p.qtiles = (Lq + 63) / 64;
+  p.nwork = bp * p.qtiles;
+  if (p.nwork >= 256) return p;
+  const int64_t units = (Lk + kUnitRows - 1) / kUnitRows;
+  if (Lq > 48 && Lk >= 1024) {
+    const int64_t most = units / 8, s = (512 + p.nwork - 1) / p.nwork;
+    p.splits = (int)(s < most ? s : most);
+    return p;
+  }
+  p.nq = 0;
+  p.qtiles = (rep * Lq + 31) / 32;
+  const int64_t blocks = bk * p.qtiles;
+  int64_t s = (256 + blocks - 1) / blocks;
+  const int64_t most = units / 8;  // two units per wave and range at least
+  s = s < most ? s : most;
+  p.splits = s < 1 ? 1 : (int)s;
+  p.units = (units + p.splits - 1) / p.splits;
+  p.splits = (int)((units + p.units - 1) / p.units);
+  p.nwork = blocks * p.splits;
+  return p;
+}
+
+}  // namespace
+
+}  // namespace sla2h
+
+using namespace sla2h;
+
+extern "C" size_t sla2h_diff_attn_fwd_workspace_bytes(int B, int H, int Hkv, int64_t Lq,
+                                                      int64_t Lk) {
+  if (!diff_sizes_ok(B, H, Hkv, Lq, Lk)) return 0;
+  const FwdPlan p = fwd_plan(B, H, Hkv, Lq, Lk);
+  return p.splits > 1 ? (size_t)p.splits * B * H * Lq * (128 * 4 + 8) : 0;
+}
+
+extern "C" int sla2h_diff_attn_fwd(const void* q, const void* k, const void* v, const float* lam,
+                                   const int64_t* strides, const int32_t* q_lens,
+                                   const int32_t* k_lens, int dtype, int B, int H, int Hkv,
+                                   int64_t Lq, int64_t Lk, int causal, float scale,
+                                   void* workspace, void* o, float* lse, float* maps,
+                                   void* stream) {
+  SLA2H_CHECK_ARG(q && k && v && lam && strides && o && !lse == !maps);
+  SLA2H_CHECK_ARG(dtype == SLA2H_DTYPE_F16 || dtype == SLA2H_DTYPE_BF16);
+  SLA2H_CHECK_ARG(diff_sizes_ok(B, H, Hkv, Lq, Lk));
+  SLA2H_CHECK_ARG(scale > 0.f && scale < 1e30f);
+  SLA2H_CHECK_ARG(((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)o | (uintptr_t)maps |
+                   (uintptr_t)workspace) % 16 == 0);
+  SLA2H_CHECK_ARG(((uintptr_t)lam | (uintptr_t)lse | (uintptr_t)q_lens | (uintptr_t)k_lens) % 4 == 0);
+  for (int i = 0; i < 9; ++i) SLA2H_CHECK_ARG(strides[i] >= 0 && strides[i] % 8 == 0);
+  // rows apart from each other: the range check of a tile's load tells them by their offset
+  for (int i : {2, 5, 8}) SLA2H_CHECK_ARG(strides[i] >= kDD);
+  // 32-bit byte offsets within a tile
+  SLA2H_CHECK_ARG(strides[5] < ((int64_t)1 << 23) && strides[8] < ((int64_t)1 << 23));
+  const FwdPlan p = fwd_plan(B, H, Hkv, Lq, Lk);
+  SLA2H_CHECK_ARG(p.splits == 1 || workspace);
+  const int64_t nrows = (int64_t)B * (H / 2) * Lq;
+  SLA2H_CHECK_ARG(p.nwork * (p.nq ? p.splits : 1) < ((int64_t)1 << 30));
+  SLA2H_CHECK_ARG(p.splits == 1 || nrows < ((int64_t)1 << 31));
+  DiffFwdArgs a{};
+  a.q = static_cast<const uint16_t*>(q);
+  a.k = static_cast<const uint16_t*>(k);
+  a.v = static_cast<const uint16_t*>(v);
+  a.lam = lam;
+  a.o = static_cast<uint16_t*>(o);
+  a.maps = maps;
+  a.lse = lse;
+  a.q_lens = q_lens;
+  a.k_lens = k_lens;
+  a.qb = strides[0], a.qh = strides[1], a.ql = strides[2];
+  a.kb = strides[3], a.kh = strides[4], a.kl = strides[5];
+  a.vb = strides[6], a.vh = strides[7], a.vl = strides[8];
+  a.Lq = Lq;
+  a.Lk = Lk;
+  a.P = H / 2;
+  a.Pk = Hkv / 2;
+  a.rep = H / Hkv;
+  a.causal = causal != 0;
+  a.c = scale * kLog2e;
+  a.qtiles = (int)p.qtiles;
+  a.map = work_map((int64_t)B * a.P, p.qtiles * (p.nq ? p.splits : 1), !causal && !q_lens && !k_lens,
+                   causal);
+  a.splits = p.splits;
+  a.units = (int)p.units;
+  a.nrows = nrows;
+  if (p.splits > 1) {
+    a.part = static_cast<float*>(workspace);
+    a.ml = reinterpret_cast<float2*>(a.part + (int64_t)p.splits * 2 * a.nrows * 128);
+  }
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  auto go = [&](auto tag) -> int {
+    using T16 = decltype(tag);
+    if (p.nq == 2)
+      diff_fwd_kernel<T16, 2><<<work_grid(a.map), 256, 0, st>>>(a);
+    else if (p.nq == 1)
+      diff_fwd_kernel<T16, 1><<<work_grid(a.map), 256, 0, st>>>(a);
+    else
+      diff_fwd_split_kernel<T16><<<(unsigned)p.nwork, 256, 0, st>>>(a);
+    const int err = (int)hipGetLastError();
+    if (err || p.splits == 1) return err;
+    diff_join_kernel<T16><<<(unsigned)a.nrows, 256, 0, st>>>(a);
+    return (int)hipGetLastError();
+  };
+  return dtype == SLA2H_DTYPE_BF16 ? go(BF16{}) : go(F16{});
+}

@@ -1,0 +1,719 @@
+// Backward of differential attention, gfx950.  The two maps of a pair are recomputed from the
+// rows' log-sum-exps; with the values' 128 channels v and dA = do v^T, delta_m = do . A_m v:
+//
+//   dS_1 = A_1 (dA - delta_1), dS_2 = -lam A_2 (dA - delta_2),
+//   dq_m = scale dS_m k_m,  dk_m = scale dS_m^T q_m,  dv = (A_1 - lam A_2)^T do,
+//   dlam = -sum delta_2     (dk, dv summed over the query pairs of a key pair).
+//
+// Both maps share dA, and the combined map has one product with do: a wave holds both.  Three
+// launches: the rows' delta; dk and dv with a workgroup per key block (queries streamed through
+// LDS); dq with a workgroup per query block (keys streamed) and, in workgroups of its own, the sum of
+// dlam.  14 products of 64 channels per (query, key) where one fused pass has 10, but no sum goes through
+// atomics or memory: the result does not depend on the order of dispatch.
+//
+// fp16 operands: maps (down to 1 / length) and dS would fall below fp16's normal range, so the
+// exponents take + shift, where 2^shift (1 + |lam|) is at most 2^15, and dA - delta a power of two from
+// |dA - delta| <= 2 max|do_i| max|v_j| (row norms, per key pair, times |lam| where that is above
+// one), which brings |dS| below 2^15; both are taken out of the fp32 sums again.  bf16 has
+// fp32's range and needs neither.
+#include "diff_attn.h"
+
+#include <initializer_list>
+
+namespace sla2h {
+
+namespace {
+
+template <typename T16>
+struct Scaled {
+  static constexpr bool value = false;
+};
+template <>
+struct Scaled<F16> {
+  static constexpr bool value = true;
+};
+
+constexpr int kNormRows = 64;  // rows of a partial maximum of the norms and of a partial sum of dlam
+
+struct DiffBwdArgs {
+  const uint16_t *q, *k, *v, *dout;
+  const float *lam, *lse, *maps;
+  uint16_t *dq, *dk, *dv;
+  float* dlam;
+  const int32_t *q_lens, *k_lens;
+  int64_t qb, qh, ql, kb, kh, kl, vb, vh, vl;
+  int64_t Lq, Lk;
+  int B, P, Pk, rep;
+  int causal;
+  float c, inv_c, scale;
+  float* stat;          // [4][B * P * Lq]: (-lse_1, -lse_2) log2e / c, -delta_1, delta_1 - delta_2
+  int64_t nrows;        // B * P * Lq
+  float *gmax, *vmax;   // (B, P, nqb), (B, Pk, nkb): largest row norms (fp16)
+  float* lsum;          // (B, P, nqb): sums of -delta_2
+  int nqb, nkb;
+  WorkMap dq_map, kv_map;  // tiles x splits of a query pair, of a key pair
+  int dq_splits, kv_splits, dq_blocks;
+  float *dq_part, *dk_part, *dv_part;
+};
+
+// Queries [first, qlen) see a key.
+__device__ inline int first_query(int qlen, int klen, int causal) {
+  if (klen == 0) return qlen;
+  return causal && qlen > klen ? qlen - klen : 0;
+}
+
+// delta of 64 rows of a pair (16 lanes per row), the sum of their -delta_2, and for fp16 the
+// largest row norm of do; the workgroups behind them take the norms of v.
+template <typename T16>
+__global__ __launch_bounds__(256) void diff_bwd_prep_kernel(DiffBwdArgs a, int64_t nq) {
+  __shared__ float red[2][4];
+  const int tid = threadIdx.x, c0 = (tid & 15) * 8;
+  const bool is_v = blockIdx.x >= nq;
+  const int64_t blk = is_v ? blockIdx.x - nq : blockIdx.x;
+  const int nb = is_v ? a.nkb : a.nqb, pairs = is_v ? a.Pk : a.P;
+  const int64_t bp = blk / nb;
+  const int t = (int)(blk - bp * nb), b = (int)(bp / pairs), p = (int)(bp - (int64_t)b * pairs);
+  const int qlen = seq_len(a.q_lens, b, a.Lq), klen = seq_len(a.k_lens, b, a.Lk);
+  const int len = is_v ? klen : qlen;
+  const int first = is_v ? 0 : first_query(qlen, klen, a.causal);
+  float top = 0.f, sum = 0.f;
+#pragma unroll
+  for (int j = 0; j < kNormRows / 16; ++j) {
+    const int64_t i = (int64_t)t * kNormRows + 16 * j + (tid >> 4);
+    const bool live = i >= first && i < len;
+    float dot[2] = {0.f, 0.f}, nrm = 0.f;
+    if (live) {
+      const int64_t at = (((int64_t)b * a.Lq + i) * a.P + p) * 128 + c0;
+      const u32x4 g = *reinterpret_cast<const u32x4*>(
+          is_v ? a.v + b * a.vb + (2 * p + (c0 >> 6)) * a.vh + i * a.vl + (c0 & 63) : a.dout + at);
+      f32x4 o[2][2];
+#pragma unroll
+      for (int m = 0; m < 2; ++m)
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+          o[m][x] = is_v ? f32x4{0.f, 0.f, 0.f, 0.f}
+                         : *reinterpret_cast<const f32x4*>(a.maps + 2 * (at - c0) + m * 128 + c0 + 4 * x);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float gv = T16::to_f32((uint16_t)(g[e >> 1] >> (16 * (e & 1))));
+#pragma unroll
+        for (int m = 0; m < 2; ++m) dot[m] += gv * o[m][e >> 2][e & 3];
+        nrm += gv * gv;
+      }
+    }
+#pragma unroll
+    for (int s = 8; s >= 1; s >>= 1) {
+      dot[0] += __shfl_xor(dot[0], s, 64);
+      dot[1] += __shfl_xor(dot[1], s, 64);
+      if (Scaled<T16>::value) nrm += __shfl_xor(nrm, s, 64);
+    }
+    top = fmaxf(top, nrm);
+    if (!is_v && c0 == 0 && i < a.Lq) {
+      const int64_t f = bp * a.Lq + i;
+#pragma unroll
+      for (int m = 0; m < 2; ++m)
+        a.stat[m * a.nrows + f] =
+            live ? -a.lse[((int64_t)b * 2 * a.P + 2 * p + m) * a.Lq + i] * kLog2e * a.inv_c
+                 : -__builtin_inff();
+      a.stat[2 * a.nrows + f] = live ? -dot[0] : 0.f;
+      a.stat[3 * a.nrows + f] = live ? dot[0] - dot[1] : 0.f;
+    }
+    sum += c0 == 0 ? -dot[1] : 0.f;
+  }
+  sum += __shfl_xor(sum, 16, 64);
+  sum += __shfl_xor(sum, 32, 64);
+  if (Scaled<T16>::value) top = wave_max(top);
+  if ((tid & 63) == 0) {
+    red[0][tid >> 6] = top;
+    red[1][tid >> 6] = sum;
+  }
+  __syncthreads();
+  if (tid) return;
+  if (Scaled<T16>::value)
+    (is_v ? a.vmax : a.gmax)[blk] =
+        sqrtf(fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3])));
+  if (!is_v) a.lsum[blk] = (red[1][0] + red[1][1]) + (red[1][2] + red[1][3]);
+}
+
+// fp16: the exponents' shift and the power of two m with 2 max|do| max|v| max(1, |lam|) m <= 1,
+// for a key pair's group.
+struct Powers {
+  float shift, m, back;  // back: 2^-shift
+};
+__device__ inline float power_of_two(int e) { return __builtin_bit_cast(float, (127 + e) << 23); }
+// e with x < 2^e, in [-100, 100]
+__device__ inline int exponent(float x) {
+  int e;
+  (void)frexpf(x, &e);
+  e = e < -100 ? -100 : (e > 100 ? 100 : e);
+  return __builtin_amdgcn_readfirstlane(e);
+}
+__device__ inline Powers powers(const DiffBwdArgs& a, int b, int kp) {
+  const int l = threadIdx.x & 63;
+  const int64_t ng = (int64_t)a.rep * a.nqb;
+  const float* g = a.gmax + ((int64_t)b * a.P + (int64_t)kp * a.rep) * a.nqb;
+  const float* v = a.vmax + ((int64_t)b * a.Pk + kp) * a.nkb;
+  float mg = 0.f, mv = 0.f, ml = 0.f;
+#pragma unroll 8
+  for (int64_t i = l; i < ng; i += 64) mg = fmaxf(mg, g[i]);
+#pragma unroll 8
+  for (int i = l; i < a.nkb; i += 64) mv = fmaxf(mv, v[i]);
+  for (int i = l; i < a.rep; i += 64) ml = fmaxf(ml, __builtin_fabsf(a.lam[kp * a.rep + i]));
+  ml = wave_max(ml);
+  Powers r{15.f, 1.f, power_of_two(-15)};
+  const float most = 1.f + ml;
+  if (most < 1e30f) {
+    // 2^(e - 1) <= 1 + |lam| < 2^e
+    const int e = exponent(most);
+    r.shift = 15.f - (float)e;
+    r.back = power_of_two(e - 15);
+  }
+  const float bound = 2.f * wave_max(mg) * wave_max(mv) * fmaxf(ml, 1.f);
+  if (bound > 0.f && bound < 1e30f) r.m = power_of_two(-exponent(bound));
+  return r;
+}
+
+// A C tile pair ([channel][row]) of a lane's row: 16-bit, or fp32 parts.
+template <typename T16>
+__device__ inline void store_row(uint16_t* p, const f32x16 (&x)[2], float f, int h, bool keep) {
+#pragma unroll
+  for (int mb = 0; mb < 2; ++mb)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const u32x2 y{pack_pair<T16>(x[mb][4 * g] * f, x[mb][4 * g + 1] * f),
+                    pack_pair<T16>(x[mb][4 * g + 2] * f, x[mb][4 * g + 3] * f)};
+      *reinterpret_cast<u32x2*>(p + 32 * mb + 8 * g + 4 * h) = keep ? y : u32x2{0, 0};
+    }
+}
+__device__ inline void store_part(float* p, const f32x16 (&x)[2], float f, int h, bool keep) {
+#pragma unroll
+  for (int mb = 0; mb < 2; ++mb)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      f32x4 y;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) y[i] = keep ? x[mb][4 * g + i] * f : 0.f;
+      *reinterpret_cast<f32x4*>(p + 32 * mb + 8 * g + 4 * h) = y;
+    }
+}
+
+// dq: workgroup = 4 waves x 32 query rows of a pair; keys of both maps and values in stages of 32
+// through four LDS slots, three ahead.  dQ_m^T += K_m^T dS_m^T with dS_m^T straight from the score
+// tile's registers.
+template <typename T16, bool FINE>
+__global__ __launch_bounds__(256, 2) void diff_bwd_dq_kernel(DiffBwdArgs a) {
+  __shared__ __align__(16) unsigned char s0[kStageB], s1[kStageB], s2[kStageB], s3[kStageB];
+  const int tid = threadIdx.x, l = tid & 63, h = l >> 5;
+  if ((int)blockIdx.x >= a.dq_blocks) {  // dlam of a pair: batch by batch, block by block
+    const int p = blockIdx.x - a.dq_blocks;
+    float* red = reinterpret_cast<float*>(s0);
+    float s = 0.f;
+    const int64_t n = (int64_t)a.B * a.nqb;
+    for (int64_t i = tid; i < n; i += 256) {
+      const int64_t b = i / a.nqb;
+      s += a.lsum[(b * a.P + p) * a.nqb + (i - b * a.nqb)];
+    }
+    red[tid] = s;
+    __syncthreads();
+    for (int x = 128; x >= 1; x >>= 1) {
+      if (tid < x) red[tid] += red[tid + x];
+      __syncthreads();
+    }
+    if (tid == 0) a.dlam[p] = red[0];
+    return;
+  }
+  int bp, item;
+  if (!work_item(a.dq_map, blockIdx.x, bp, item)) return;
+  const int qt = item / a.dq_splits, sp = item - qt * a.dq_splits;
+  const int b = bp / a.P, p = bp - b * a.P, kp = p / a.rep;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const LaneOff lo(l);
+  const int qlen = seq_len(a.q_lens, b, a.Lq), klen = seq_len(a.k_lens, b, a.Lk);
+
+  const int q0 = qt * 128, qw = q0 + w * 32;
+  const int qend = min(q0 + 128, qlen);
+  const int kmax = qend > q0 ? key_limit(qend - 1, qlen, klen, a.causal) : 0;
+  const int nunit = (kmax + kUnitRows - 1) / kUnitRows;
+  const int per = (nunit + a.dq_splits - 1) / a.dq_splits;
+  const int t0 = sp * per, nt = min(nunit, t0 + per);
+
+  const uint16_t* src = w < 2 ? a.k + b * a.kb + (2 * kp + w) * a.kh
+                              : a.v + b * a.vb + (2 * kp + w - 2) * a.vh;
+  const int64_t ld = (w < 2 ? a.kl : a.vl) * 2;
+  auto load = [&](int t, unsigned char* s) __attribute__((always_inline)) {
+    const int64_t row = (int64_t)t * kUnitRows;
+    load_unit(src, row, (int64_t)klen - row, ld, s + w * kUnitB, l);
+  };
+
+  Powers pw{0.f, 1.f, 1.f};
+  if (Scaled<T16>::value) pw = powers(a, b, kp);
+  const int i = qw + (l & 31);
+  const int lim = key_limit(i, qlen, klen, a.causal);
+  const bool live = lim > 0;
+  const int64_t flat = (int64_t)bp * a.Lq + i;
+  float nl[2], nd[2];  // shift - lse_m log2e, -delta_m (times m)
+#pragma unroll
+  for (int m = 0; m < 2; ++m)
+    nl[m] = live ? a.stat[m * a.nrows + flat] * a.c + pw.shift : -__builtin_inff();
+  nd[0] = live ? a.stat[2 * a.nrows + flat] * pw.m : 0.f;
+  nd[1] = live ? nd[0] + a.stat[3 * a.nrows + flat] * pw.m : 0.f;
+  u32x4 qf[2][4], gf[2][4];
+#pragma unroll
+  for (int m = 0; m < 2; ++m) {
+    const uint16_t* qp = a.q + b * a.qb + (2 * p + m) * a.qh + i * a.ql + 8 * h;
+    const uint16_t* gp = a.dout + (((int64_t)b * a.Lq + i) * a.P + p) * 128 + 64 * m + 8 * h;
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      qf[m][s] = live ? *reinterpret_cast<const u32x4*>(qp + 16 * s) : u32x4{0, 0, 0, 0};
+      gf[m][s] = live ? *reinterpret_cast<const u32x4*>(gp + 16 * s) : u32x4{0, 0, 0, 0};
+    }
+  }
+  // keys that any query of the wave sees, and that all of them see
+  const int wlast = min(qw + 32, qlen) - 1;
+  const int wany = wlast >= qw ? key_limit(wlast, qlen, klen, a.causal) : 0;
+  const int wall = wlast >= qw ? key_limit(qw, qlen, klen, a.causal) : 0;
+
+  f32x16 acc[2][2];
+#pragma unroll
+  for (int m = 0; m < 2; ++m) acc[m][0] = acc[m][1] = zero16();
+  auto part = [&](auto masked, int base, const unsigned char* s) __attribute__((always_inline)) {
+    f32x16 sc[2] = {zero16(), zero16()}, dp = zero16();
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      sc[0] = mfma_32x32x16<T16>(row_frag(s, 0, x, lo), qf[0][x], sc[0]);
+      dp = mfma_32x32x16<T16>(row_frag(s + 2 * kUnitB, 0, x, lo), gf[0][x], dp);
+      sc[1] = mfma_32x32x16<T16>(row_frag(s + kUnitB, 0, x, lo), qf[1][x], sc[1]);
+      dp = mfma_32x32x16<T16>(row_frag(s + 3 * kUnitB, 0, x, lo), gf[1][x], dp);
+    }
+#pragma unroll
+    for (int m = 0; m < 2; ++m) {
+      f32x16 d;
+#pragma unroll
+      for (int e = 0; e < 16; ++e)
+        d[e] = fast_exp2(__builtin_fmaf(sc[m][e], a.c, nl[m])) *
+               (Scaled<T16>::value ? __builtin_fmaf(dp[e], pw.m, nd[m]) : dp[e] + nd[m]);
+      if (decltype(masked)::value) {
+        const int x = lim - base - 4 * h;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) d[e] = 8 * (e >> 2) + (e & 3) < x ? d[e] : 0.f;
+      }
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const u32x4 ds = pack_step<T16>(d, x);
+        u32x4 kf[2];
+#pragma unroll
+        for (int mb = 0; mb < 2; ++mb) {
+          kf[mb] = col_frag(s + m * kUnitB, 16 * x, mb, lo);
+          acc[m][mb] = mfma_32x32x16<T16>(kf[mb], ds, acc[m][mb]);
+        }
+        if (FINE) {
+          const u32x4 lost = lost_step<T16>(d, x, ds);
+#pragma unroll
+          for (int mb = 0; mb < 2; ++mb)
+            acc[m][mb] = mfma_32x32x16<T16>(kf[mb], lost, acc[m][mb]);
+        }
+      }
+    }
+  };
+  auto stage = [&](int t, const unsigned char* cur, unsigned char* to)
+      __attribute__((always_inline)) {
+    // the stages up to t have landed, stage t - 1 is read
+    __builtin_amdgcn_s_waitcnt(wait_vm_lgkm0(8));
+    __builtin_amdgcn_s_barrier();
+    load(t + 3, to);
+    const int base = t * kUnitRows;
+    if (base + kUnitRows <= wall)  // a stage that every query of the wave sees: no branch inside
+      part(std::false_type{}, base, cur);
+    else if (base < wany)
+      part(std::true_type{}, base, cur);
+  };
+  load(t0, s0);
+  load(t0 + 1, s1);
+  load(t0 + 2, s2);
+  for (int t = t0; t < nt; t += 4) {
+    stage(t, s0, s3);
+    if (t + 1 >= nt) break;
+    stage(t + 1, s1, s0);
+    if (t + 2 >= nt) break;
+    stage(t + 2, s2, s1);
+    if (t + 3 >= nt) break;
+    stage(t + 3, s3, s2);
+  }
+  __builtin_amdgcn_s_waitcnt(wait_vm_lgkm0(0));  // no load into this LDS outlives the workgroup
+
+  if (i >= a.Lq) return;
+  const int64_t orow = ((int64_t)b * a.Lq + i) * a.P + p;
+#pragma unroll
+  for (int m = 0; m < 2; ++m) {
+    // (the softmax of one key is constant: its dS is the rounding of dA - delta)
+    const float f = lim == 1 ? 0.f : (m ? -a.lam[p] : 1.f) * a.scale * pw.back / pw.m;
+    if (a.dq_splits == 1)
+      store_row<T16>(a.dq + orow * 128 + 64 * m, acc[m], f, h, live);
+    else
+      store_part(a.dq_part + ((int64_t)sp * a.nrows + orow) * 128 + 64 * m, acc[m], f, h, live);
+  }
+}
+
+// dk, dv: workgroup = 4 waves x 32 keys of one key pair; the query rows (both maps' queries, the 128
+// channels of do) of the pairs that read it are streamed in stages of 32 rows, with their four
+// statistics, which start the accumulators of S_m and dA.  A wave holds 128 channels of dv, 64
+// of each dk and its keys and values: one wave per SIMD.  The stage is software-pipelined: S_m and dA
+// of the next stage run on the matrix cores under this stage's exponentials.
+template <typename T16, bool CAUSAL, bool FINE>
+__global__ __launch_bounds__(256, 1) void diff_bwd_dkdv_kernel(DiffBwdArgs a) {
+  __shared__ __align__(16) unsigned char r0[kStageB], r1[kStageB], r2[kStageB], r3[kStageB];
+  __shared__ __align__(16) float t0_[4][64], t1_[4][64], t2_[4][64], t3_[4][64];
+  int bk, item;
+  if (!work_item(a.kv_map, blockIdx.x, bk, item)) return;
+  const int ktile = item / a.kv_splits, sp = item - ktile * a.kv_splits;
+  const int b = bk / a.Pk, kp = bk - b * a.Pk;
+  const int tid = threadIdx.x, l = tid & 63, h = l >> 5;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const LaneOff lo(l);
+  const int qlen = seq_len(a.q_lens, b, a.Lq), klen = seq_len(a.k_lens, b, a.Lk);
+
+  const int key0 = ktile * 128, kw = key0 + w * 32;
+  // first query that sees a key of the workgroup (causal: i >= j - off)
+  const int off = klen - qlen;
+  int first = first_query(qlen, klen, a.causal);
+  if (CAUSAL) first = max(first, key0 - off);
+  const int nq = key0 < klen && first < qlen ? (qlen - first + kUnitRows - 1) / kUnitRows : 0;
+  const int total = nq * a.rep;  // (pair, stage)
+  const int per = (total + a.kv_splits - 1) / a.kv_splits;
+  const int u0 = sp * per, u1 = min(total, u0 + per);
+
+  // the stage to load next, and the one to compute (their pair of the group and first row)
+  int lu = u0, lp = u0 < u1 ? u0 / nq : 0;
+  int lrow = first + (u0 < u1 ? u0 - lp * nq : 0) * kUnitRows;
+  int cu = u0, cp = lp, crow = lrow;
+  auto load = [&](unsigned char* s, float (*st)[64]) __attribute__((always_inline)) {
+    const int64_t p = (int64_t)kp * a.rep + lp, n = lu < u1 ? (int64_t)qlen - lrow : 0;
+    if (w < 2)
+      load_unit(a.q + b * a.qb + (2 * p + w) * a.qh, lrow, n, a.ql * 2, s + w * kUnitB, l);
+    else
+      load_unit(a.dout + ((int64_t)b * a.Lq * a.P + p) * 128 + 64 * (w - 2), lrow, n,
+                (int64_t)a.P * 256, s + w * kUnitB, l);
+    const auto rs = make_rsrc(a.stat + w * a.nrows + ((int64_t)b * a.P + p) * a.Lq + lrow,
+                              n <= 0 ? 0 : (n < kUnitRows ? n : kUnitRows) * 4);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(
+        rs, (__attribute__((address_space(3))) void*)&st[w][0], 4, 4 * l, 0, 0, 0);
+    ++lu;
+    lrow += kUnitRows;
+    if (lrow >= qlen && lu < u1) lrow = first, ++lp;
+  };
+
+  Powers pw{0.f, 1.f, 1.f};
+  if (Scaled<T16>::value) pw = powers(a, b, kp);
+  u32x4 kf[2][4], vf[2][4];
+  {
+    const int j = kw + (l & 31);
+    const bool live = j < klen;
+#pragma unroll
+    for (int m = 0; m < 2; ++m)
+#pragma unroll
+      for (int s = 0; s < 4; ++s) {
+        kf[m][s] = live ? *reinterpret_cast<const u32x4*>(a.k + b * a.kb + (2 * kp + m) * a.kh +
+                                                          j * a.kl + 16 * s + 8 * h)
+                        : u32x4{0, 0, 0, 0};
+        vf[m][s] = live ? *reinterpret_cast<const u32x4*>(a.v + b * a.vb + (2 * kp + m) * a.vh +
+                                                          j * a.vl + 16 * s + 8 * h)
+                        : u32x4{0, 0, 0, 0};
+      }
+  }
+  f32x16 ak[2][2], av[4];
+#pragma unroll
+  for (int x = 0; x < 2; ++x) ak[0][x] = ak[1][x] = av[x] = av[2 + x] = zero16();
+  f32x16 sc[2][2], dp[2];
+
+  // S_m and dA - delta_1 of a stage
+  auto scores = [&](int x, const unsigned char* s, const float (*st)[64])
+      __attribute__((always_inline)) {
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const f32x4 y0 = *reinterpret_cast<const f32x4*>(&st[0][8 * g + 4 * h]);
+      const f32x4 y1 = *reinterpret_cast<const f32x4*>(&st[1][8 * g + 4 * h]);
+      const f32x4 y2 = *reinterpret_cast<const f32x4*>(&st[2][8 * g + 4 * h]);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        sc[x][0][4 * g + i] = y0[i];
+        sc[x][1][4 * g + i] = y1[i];
+        dp[x][4 * g + i] = y2[i];
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      sc[x][0] = mfma_32x32x16<T16>(row_frag(s, 0, k, lo), kf[0][k], sc[x][0]);
+      dp[x] = mfma_32x32x16<T16>(row_frag(s + 2 * kUnitB, 0, k, lo), vf[0][k], dp[x]);
+      sc[x][1] = mfma_32x32x16<T16>(row_frag(s + kUnitB, 0, k, lo), kf[1][k], sc[x][1]);
+      dp[x] = mfma_32x32x16<T16>(row_frag(s + 3 * kUnitB, 0, k, lo), vf[1][k], dp[x]);
+    }
+  };
+  auto stage = [&](int x, const unsigned char* s, const float (*st)[64], const unsigned char* sn,
+                   const float (*tn)[64], unsigned char* sl, float (*tl)[64])
+      __attribute__((always_inline)) {
+    // the stages up to the next one have landed, the one before is read
+    __builtin_amdgcn_s_waitcnt(wait_vm_lgkm0(5));
+    __builtin_amdgcn_s_barrier();
+    load(sl, tl);
+    if (kw < klen) {
+      const float lam = a.lam[kp * a.rep + cp];
+      scores(x ^ 1, sn, tn);
+      f32x16 p1, p2, d1, d2;
+      const float sh = pw.shift;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        p1[e] = fast_exp2(Scaled<T16>::value ? __builtin_fmaf(sc[x][0][e], a.c, sh) : sc[x][0][e] * a.c);
+        p2[e] = lam * fast_exp2(Scaled<T16>::value ? __builtin_fmaf(sc[x][1][e], a.c, sh)
+                                                   : sc[x][1][e] * a.c);
+      }
+      if (CAUSAL && crow < kw + 31 - off) {
+        asm volatile("");
+        const int y = kw + (l & 31) - off - crow - 4 * h;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          p1[e] = 8 * (e >> 2) + (e & 3) >= y ? p1[e] : 0.f;
+          p2[e] = 8 * (e >> 2) + (e & 3) >= y ? p2[e] : 0.f;
+        }
+      }
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const f32x4 dd = *reinterpret_cast<const f32x4*>(&st[3][8 * g + 4 * h]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int e = 4 * g + i;
+          d1[e] = (Scaled<T16>::value ? p1[e] * pw.m : p1[e]) * dp[x][e];
+          d2[e] = (Scaled<T16>::value ? p2[e] * pw.m : p2[e]) * (dp[x][e] + dd[i]);
+          p1[e] -= p2[e];
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const u32x4 pp = pack_step<T16>(p1, k), dd1 = pack_step<T16>(d1, k),
+                    dd2 = pack_step<T16>(d2, k);
+        u32x4 gf[4], qf[2][2];
+#pragma unroll
+        for (int mb = 0; mb < 4; ++mb) {
+          gf[mb] = col_frag(s + (2 + (mb >> 1)) * kUnitB, 16 * k, mb & 1, lo);
+          av[mb] = mfma_32x32x16<T16>(gf[mb], pp, av[mb]);
+        }
+#pragma unroll
+        for (int m = 0; m < 2; ++m)
+#pragma unroll
+          for (int mb = 0; mb < 2; ++mb) {
+            qf[m][mb] = col_frag(s + m * kUnitB, 16 * k, mb, lo);
+            ak[m][mb] = mfma_32x32x16<T16>(qf[m][mb], m ? dd2 : dd1, ak[m][mb]);
+          }
+        if (FINE) {
+          const u32x4 pl = lost_step<T16>(p1, k, pp), dl1 = lost_step<T16>(d1, k, dd1),
+                      dl2 = lost_step<T16>(d2, k, dd2);
+#pragma unroll
+          for (int mb = 0; mb < 4; ++mb) av[mb] = mfma_32x32x16<T16>(gf[mb], pl, av[mb]);
+#pragma unroll
+          for (int m = 0; m < 2; ++m)
+#pragma unroll
+            for (int mb = 0; mb < 2; ++mb)
+              ak[m][mb] = mfma_32x32x16<T16>(qf[m][mb], m ? dl2 : dl1, ak[m][mb]);
+        }
+      }
+    }
+    ++cu;
+    crow += kUnitRows;
+    if (crow >= qlen && cu < u1) crow = first, ++cp;
+  };
+  load(r0, t0_);
+  load(r1, t1_);
+  load(r2, t2_);
+  __builtin_amdgcn_s_waitcnt(wait_vm_lgkm0(10));
+  __builtin_amdgcn_s_barrier();
+  scores(0, r0, t0_);
+  for (int u = u0; u < u1; u += 4) {
+    stage(0, r0, t0_, r1, t1_, r3, t3_);
+    if (u + 1 >= u1) break;
+    stage(1, r1, t1_, r2, t2_, r0, t0_);
+    if (u + 2 >= u1) break;
+    stage(0, r2, t2_, r3, t3_, r1, t1_);
+    if (u + 3 >= u1) break;
+    stage(1, r3, t3_, r0, t0_, r2, t2_);
+  }
+  __builtin_amdgcn_s_waitcnt(wait_vm_lgkm0(0));
+
+  const int j = kw + (l & 31);
+  if (j >= a.Lk) return;
+  const bool keep = j < klen;
+  const int64_t orow = ((int64_t)b * a.Lk + j) * a.Pk + kp, n = (int64_t)a.B * a.Lk * a.Pk;
+  const float fk = klen == 1 ? 0.f : a.scale * pw.back / pw.m;
+#pragma unroll
+  for (int m = 0; m < 2; ++m) {
+    const f32x16 y[2] = {av[2 * m], av[2 * m + 1]};
+    if (a.kv_splits == 1) {
+      store_row<T16>(a.dk + orow * 128 + 64 * m, ak[m], m ? -fk : fk, h, keep);
+      store_row<T16>(a.dv + orow * 128 + 64 * m, y, pw.back, h, keep);
+    } else {
+      const int64_t at = (sp * n + orow) * 128 + 64 * m;
+      store_part(a.dk_part + at, ak[m], m ? -fk : fk, h, keep);
+      store_part(a.dv_part + at, y, pw.back, h, keep);
+    }
+  }
+}
+
+// Adds the parts of up to two results in order (blockIdx.y), n values each.
+template <typename T16>
+__global__ __launch_bounds__(256) void diff_bwd_join_kernel(const float* __restrict__ part0,
+                                                            const float* __restrict__ part1,
+                                                            int splits, int64_t n, uint16_t* y0,
+                                                            uint16_t* y1) {
+  const int64_t e = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+  if (e >= n) return;
+  const float* part = blockIdx.y ? part1 : part0;
+  f32x4 x{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int s = 0; s < splits; ++s) x += *reinterpret_cast<const f32x4*>(part + s * n + e);
+  *reinterpret_cast<u32x2*>((blockIdx.y ? y1 : y0) + e) =
+      u32x2{pack_pair<T16>(x[0], x[1]), pack_pair<T16>(x[2], x[3])};
+}
+
+struct BwdPlan {
+  int64_t qtiles, dq_nwork, ktiles, kv_nwork;
+  int dq_splits, kv_splits;
+  int64_t nqb, nkb;
+  size_t stats, dq_parts, kv_parts;  // floats (kv_parts: of dk, and as many of dv)
+};
+
+BwdPlan bwd_plan(int dtype, int B, int H, int Hkv, int64_t Lq, int64_t Lk, bool even) {
+  BwdPlan p{};
+  const int64_t bp = (int64_t)B * H / 2, bk = (int64_t)B * Hkv / 2, rep = H / Hkv;
+  p.qtiles = (Lq + 127) / 128;
+  auto split = [&](int64_t blocks, int64_t units) {
+    const int64_t want = even ? 256 : 512;
+    if (blocks >= want / 2) return 1;
+    const int64_t s = (want + blocks - 1) / blocks, most = units / 8;
+    return (int)(s < most ? s : (most < 1 ? 1 : most));
+  };
+  p.dq_splits = split(bp * p.qtiles, (Lk + 31) / 32);
+  p.dq_nwork = bp * p.qtiles * p.dq_splits;
+  p.ktiles = (Lk + 127) / 128;
+  p.kv_splits = split(bk * p.ktiles, rep * ((Lq + 31) / 32));
+  p.kv_nwork = bk * p.ktiles * p.kv_splits;
+  p.nqb = (Lq + kNormRows - 1) / kNormRows;
+  p.nkb = (Lk + kNormRows - 1) / kNormRows;
+  p.stats = 4 * bp * Lq + bp * p.nqb + (dtype == SLA2H_DTYPE_F16 ? bp * p.nqb + bk * p.nkb : 0);
+  p.stats = (p.stats + 3) & ~(size_t)3;
+  p.dq_parts = p.dq_splits > 1 ? (size_t)p.dq_splits * bp * Lq * 128 : 0;
+  p.kv_parts = p.kv_splits > 1 ? (size_t)p.kv_splits * bk * Lk * 128 : 0;
+  return p;
+}
+
+}  // namespace
+
+}  // namespace sla2h
+
+using namespace sla2h;
+
+extern "C" size_t sla2h_diff_attn_bwd_workspace_bytes(int dtype, int B, int H, int Hkv, int64_t Lq,
+                                                      int64_t Lk) {
+  if (!diff_sizes_ok(B, H, Hkv, Lq, Lk)) return 0;
+  size_t most = 0;
+  for (bool even : {false, true}) {
+    const BwdPlan p = bwd_plan(dtype, B, H, Hkv, Lq, Lk, even);
+    const size_t n = p.stats + p.dq_parts + 2 * p.kv_parts;
+    most = n > most ? n : most;
+  }
+  return most * 4;
+}
+
+extern "C" int sla2h_diff_attn_bwd(const void* q, const void* k, const void* v, const float* lam,
+                                   const void* dout, const float* lse, const float* maps,
+                                   const int64_t* strides, const int32_t* q_lens,
+                                   const int32_t* k_lens, int dtype, int B, int H, int Hkv,
+                                   int64_t Lq, int64_t Lk, int causal, float scale,
+                                   void* workspace, void* dq, void* dk, void* dv, float* dlam,
+                                   void* stream) {
+  SLA2H_CHECK_ARG(q && k && v && lam && dout && lse && maps && strides && workspace && dlam);
+  SLA2H_CHECK_ARG(!dk == !dv);
+  SLA2H_CHECK_ARG(dtype == SLA2H_DTYPE_F16 || dtype == SLA2H_DTYPE_BF16);
+  SLA2H_CHECK_ARG(diff_sizes_ok(B, H, Hkv, Lq, Lk));
+  SLA2H_CHECK_ARG(scale > 0.f && scale < 1e30f);
+  SLA2H_CHECK_ARG(((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)dout | (uintptr_t)maps |
+                   (uintptr_t)workspace | (uintptr_t)dq | (uintptr_t)dk | (uintptr_t)dv) % 16 == 0);
+  SLA2H_CHECK_ARG(((uintptr_t)lam | (uintptr_t)lse | (uintptr_t)dlam | (uintptr_t)q_lens |
+                   (uintptr_t)k_lens) % 4 == 0);
+  for (int i = 0; i < 9; ++i) SLA2H_CHECK_ARG(strides[i] >= 0 && strides[i] % 8 == 0);
+  // rows apart from each other: the range check of a tile's load tells them by their offset; 32-bit
+  // byte offsets within a tile
+  for (int i : {2, 5, 8}) SLA2H_CHECK_ARG(strides[i] >= kDD && strides[i] < ((int64_t)1 << 23));
+  SLA2H_CHECK_ARG((int64_t)H * kDD < ((int64_t)1 << 23));
+  const bool even = !causal && !q_lens && !k_lens;
+  const BwdPlan p = bwd_plan(dtype, B, H, Hkv, Lq, Lk, even);
+  SLA2H_CHECK_ARG(p.dq_nwork < ((int64_t)1 << 30) && p.kv_nwork < ((int64_t)1 << 30));
+  const int64_t bp = (int64_t)B * H / 2, bk = (int64_t)B * Hkv / 2;
+  const int64_t pq = bp * p.nqb, pv = dtype == SLA2H_DTYPE_F16 ? bk * p.nkb : 0;
+  SLA2H_CHECK_ARG(pq + pv < ((int64_t)1 << 31));
+  DiffBwdArgs a{};
+  a.q = static_cast<const uint16_t*>(q);
+  a.k = static_cast<const uint16_t*>(k);
+  a.v = static_cast<const uint16_t*>(v);
+  a.dout = static_cast<const uint16_t*>(dout);
+  a.lam = lam, a.lse = lse, a.maps = maps;
+  a.dq = static_cast<uint16_t*>(dq);
+  a.dk = static_cast<uint16_t*>(dk);
+  a.dv = static_cast<uint16_t*>(dv);
+  a.dlam = dlam;
+  a.q_lens = q_lens;
+  a.k_lens = k_lens;
+  a.qb = strides[0], a.qh = strides[1], a.ql = strides[2];
+  a.kb = strides[3], a.kh = strides[4], a.kl = strides[5];
+  a.vb = strides[6], a.vh = strides[7], a.vl = strides[8];
+  a.Lq = Lq;
+  a.Lk = Lk;
+  a.B = B;
+  a.P = H / 2;
+  a.Pk = Hkv / 2;
+  a.rep = H / Hkv;
+  a.causal = causal != 0;
+  a.c = scale * kLog2e;
+  a.inv_c = 1.f / a.c;
+  a.scale = scale;
+  a.nrows = bp * Lq;
+  a.stat = static_cast<float*>(workspace);
+  a.lsum = a.stat + 4 * a.nrows;
+  a.gmax = a.lsum + bp * p.nqb;
+  a.vmax = a.gmax + bp * p.nqb;
+  a.nqb = (int)p.nqb;
+  a.nkb = (int)p.nkb;
+  a.dq_part = a.stat + p.stats;
+  a.dk_part = a.dq_part + p.dq_parts;
+  a.dv_part = a.dk_part + p.kv_parts;
+  a.dq_map = work_map(bp, p.qtiles * p.dq_splits, even, causal);
+  a.kv_map = work_map(bk, p.ktiles * p.kv_splits, even, false);  // causal: the first keys' are longest
+  a.dq_blocks = dq ? (int)work_grid(a.dq_map) : 0;
+  a.dq_splits = p.dq_splits;
+  a.kv_splits = p.kv_splits;
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  auto go = [&](auto tag) -> int {
+    using T16 = decltype(tag);
+    int err;
+    diff_bwd_prep_kernel<T16><<<(unsigned)(pq + pv), 256, 0, st>>>(a, pq);
+    if ((err = (int)hipGetLastError())) return err;
+    if (dk) {
+      const unsigned grid = work_grid(a.kv_map);
+      if (causal)
+        diff_bwd_dkdv_kernel<T16, true, false><<<grid, 256, 0, st>>>(a);
+      else
+        diff_bwd_dkdv_kernel<T16, false, false><<<grid, 256, 0, st>>>(a);
+      if ((err = (int)hipGetLastError())) return err;
+    }
+    diff_bwd_dq_kernel<T16, false><<<a.dq_blocks + a.P, 256, 0, st>>>(a);
+    if ((err = (int)hipGetLastError())) return err;
+    auto join = [&](int splits, int64_t n, const float* p0, const float* p1, uint16_t* y0,
+                    uint16_t* y1) {
+      diff_bwd_join_kernel<T16><<<dim3((unsigned)((n / 4 + 255) / 256), y1 ? 2 : 1), 256, 0, st>>>(
+          p0, p1, splits, n, y0, y1);
+    };
+    if (dq && p.dq_splits > 1)
+      join(p.dq_splits, a.nrows * 128, a.dq_part, nullptr, a.dq, nullptr);
+    if (dk && p.kv_splits > 1)
+      join(p.kv_splits, bk * Lk * 128, a.dk_part, a.dv_part, a.dk, a.dv);
+    return (int)hipGetLastError();
+  };
+  return dtype == SLA2H_DTYPE_BF16 ? go(BF16{}) : go(F16{});
+}

@@ -21,7 +21,8 @@ from . import ops
 
 __all__ = ["RMSNorm", "SituAndMul", "SwiGLUMlp", "MLAAttention", "TransformerBlock",
            "apply_rotary_pos_emb", "precompute_axial_rope_3d", "scaled_variance_linear",
-           "dense_attention", "sdpa_math_attention", "residual_norm"]
+           "dense_attention", "diff_attention", "DiffAttentionImpl", "sdpa_math_attention",
+           "residual_norm"]
 
 
 class _CastOf(torch.autograd.Function):
@@ -186,6 +187,94 @@ def dense_attention(q, k, v, causal=False, q_lens=None, k_lens=None, scale=None)
             or torch.autograd.forward_ad._current_level >= 0 or torch.jit.is_tracing()):
         return _DenseAttentionFunction.apply(q, k, v, causal, q_lens, k_lens, scale)
     return ops.dense_attn_fwd(q, k, v, causal, q_lens, k_lens, scale, False, False, True)[0]
+
+
+class _DiffAttentionFunction(torch.autograd.Function):
+    """Differential attention of (b, l, H, 64) operands on the HIP kernels; saves the
+    operands, the maps' outputs in fp32 and the rows' log-sum-exps, and recomputes the
+    probabilities."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, lam, causal, q_lens, k_lens, scale):
+        o, lse, maps = ops.diff_attn_fwd(q, k, v, lam, causal, q_lens, k_lens, scale, True)
+        ctx.args = causal, scale
+        ctx.save_for_backward(q, k, v, lam, lse, maps, q_lens, k_lens)
+        return o
+
+    @staticmethod
+    @_once
+    def backward(ctx, do):
+        _no_batched(do, "diff_attention")
+        q, k, v, lam, lse, maps, q_lens, k_lens = ctx.saved_tensors
+        causal, scale = ctx.args
+        nq, nk, nv = ctx.needs_input_grad[:3]
+        *grads, dlam = ops.diff_attn_bwd(do, q, k, v, lam, lse, maps, causal, q_lens, k_lens, scale,
+                                         nq, nk or nv)
+        return (*grads, dlam.to(lam.dtype), None, None, None, None)
+
+
+def diff_attention(q, k, v, lam, causal=False, q_lens=None, k_lens=None, scale=None):
+    """Differential attention on the gfx950 kernels, forward and backward: the difference of two
+    softmax maps with a learned weight, which cancels what the maps have in common.
+
+        o = (softmax(scale q1 k1^T) - lam softmax(scale q2 k2^T)) v
+
+    q (b, l, H, 64) over k, v (b, lk, Hkv, 64) of one 16-bit dtype (under a 16-bit autocast any
+    floating dtype, cast to it), H and Hkv even, H a multiple of Hkv.  The heads 2p and 2p + 1 of
+    q and k are the two maps of pair p, the heads 2p and 2p + 1 of v side by side its 128 value
+    channels, the same heads of o its output: the shapes, and the layers around them, are those of
+    attention with H heads.  lam (H / 2,): a floating-point weight per pair, with a gradient.
+    q_lens, k_lens, causal and scale as in dense_attention, rows without a key too.
+
+    Memory is linear in l (the probabilities are recomputed in the backward), and results do not
+    depend on the order of execution.  GPU tensors only; one reverse-mode derivative (no double
+    backward, forward mode or vmap)."""
+    if torch.is_autocast_enabled("cuda"):
+        dt = torch.get_autocast_dtype("cuda")
+        q, k, v = (t.to(dt) if t.is_floating_point() else t for t in (q, k, v))
+    if q_lens is not None:
+        q_lens = ops.attn_lens(q_lens, q, "q_lens")
+    if k_lens is not None:
+        k_lens = ops.attn_lens(k_lens, q, "k_lens")
+    # (a tangent and a trace see the Function, as in dense_attention)
+    if (torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad
+                                     or lam.requires_grad)
+            or torch.autograd.forward_ad._current_level >= 0 or torch.jit.is_tracing()):
+        return _DiffAttentionFunction.apply(q, k, v, lam, causal, q_lens, k_lens, scale)
+    return ops.diff_attn_fwd(q, k, v, lam, causal, q_lens, k_lens, scale)[0]
+
+
+class DiffAttentionImpl(nn.Module):
+    """Differential attention as an attn_impl of MLAAttention, e.g.
+    ``functools.partial(DiffAttentionImpl, num_heads=H)``: the weight of the second map,
+
+        lam = exp(lambda_q1 . lambda_k1) - exp(lambda_q2 . lambda_k2) + lambda_init,
+
+    is learned and shared by the pairs, and each pair's 128 output channels go through an
+    RMSNorm, times 1 - lambda_init, so that the layer starts at attention's own scale."""
+
+    def __init__(self, head_dim, num_heads, lambda_init=0.8, causal=False, norm_eps=1e-6):
+        super().__init__()
+        if head_dim != ops.E_TILE or num_heads < 2 or num_heads % 2:
+            raise ValueError("DiffAttentionImpl: 64-channel heads in pairs, got "
+                             f"{num_heads} of {head_dim}")
+        self.num_heads, self.lambda_init, self.causal = num_heads, lambda_init, causal
+        for name in ("lambda_q1", "lambda_k1", "lambda_q2", "lambda_k2"):
+            self.register_parameter(name, nn.Parameter(0.1 * torch.randn(head_dim)))
+        self.norm = RMSNorm(2 * head_dim, eps=norm_eps)
+
+    def weight(self):
+        """lam, a scalar."""
+        dot = lambda a, b: torch.exp((a.float() * b.float()).sum())
+        return (dot(self.lambda_q1, self.lambda_k1) - dot(self.lambda_q2, self.lambda_k2)
+                + self.lambda_init)
+
+    def forward(self, q, k, v, q_lens=None, k_lens=None):
+        o = diff_attention(q, k, v, self.weight().expand(self.num_heads // 2), self.causal, q_lens,
+                           k_lens)
+        b, l, H, d = o.shape
+        y = self.norm(o.reshape(b, l, H // 2, 2 * d)) * (1.0 - self.lambda_init)
+        return y.reshape(b, l, H, d).to(o.dtype)
 
 
 class _RMSNormFunction(torch.autograd.Function):

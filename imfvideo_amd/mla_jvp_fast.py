@@ -24,7 +24,7 @@ import torch
 import torch.nn.functional as F
 
 from . import _lib, ops
-from .imf_dit_video import dense_attention
+from .imf_dit_video import DiffAttentionImpl, dense_attention, diff_attention
 from .sla2_cube_qat import sla2_cube_qat_jvp_fused
 from .sla2_mla_jvp import _sla2_mla_jvp, route_blocks, sla2_mla_jvp
 
@@ -196,11 +196,14 @@ def _mlp_sublayer_proj(h, dh, p, w16, eps):
 
 def _check_dense_impl(impl):
     """ValueError for a functools.partial of dense_attention that is another function than
-    the JVP's dense branch (every token sees every token, scale 64^-1/2)."""
+    the JVP's dense branch (every token sees every token, scale 64^-1/2), and for differential
+    attention."""
     bound = {}
     while isinstance(impl, partial):
         bound = {**impl.keywords, **bound}
         impl = impl.func
+    if impl is diff_attention or isinstance(impl, DiffAttentionImpl):
+        raise ValueError("pack_block: the fast JVP has no form of differential attention")
     if impl is not dense_attention:
         return
     other = ["causal"] if bound.get("causal") else []
@@ -223,7 +226,8 @@ def pack_block(block, tile_major=False):
         pre_permuted = tile_major (the model keeps tokens tile-major);
       sla2 (SLA2AttentionImpl): alpha (H, Mb), the router projections, topk, bq, bk;
       any other impl is taken for dense softmax attention of every token to every token at
-      scale 64^-1/2 (a partial of dense_attention that is not raises ValueError).
+      scale 64^-1/2 (a partial of dense_attention that is not, and differential attention, raise
+      ValueError).
     A block with norms behind its sublayers (sandwich_norm) raises ValueError.
     Rebuild after every optimizer step (the weights change)."""
     if getattr(block, "sandwich_norm", False):

@@ -2001,3 +2001,134 @@ def orthogonalize(g, steps=5, coeffs=NS_COEFFS):
     _launch(g.device, "sla2h_orthogonalize", g.data_ptr(), _NORM_DTYPES[g.dtype], n, R, C, steps,
             table, ws.data_ptr(), out.data_ptr())
     return out
+
+
+# ---------------------------------------------------------------------------
+# Differential attention (sla2h_diff_attn_fwd / _bwd)
+# ---------------------------------------------------------------------------
+class _DiffPlan:
+    """What a differential attention call needs of its operands' shapes and strides."""
+    __slots__ = ("sizes", "copy", "empty", "strides", "fwd_ws", "bwd_ws", "lse_shape", "maps_shape")
+
+
+@functools.lru_cache(maxsize=512)
+def _diff_plan(qs, qt, ks, kt, vs, vt, dtype):
+    for s, name in ((qs, "q"), (ks, "k"), (vs, "v")):
+        if len(s) != 4 or s[3] != E_TILE:
+            raise ValueError(f"{name}: expected (B, L, H, 64), got {tuple(s)}")
+    B, Lq, H, _ = qs
+    Lk, Hkv = ks[1:3]
+    if ks != vs or ks[0] != B or H % 2 or Hkv % 2 or (H and (Hkv == 0 or H % Hkv)):
+        raise ValueError("k and v must share their shape, q's batch and an even number of heads that "
+                         f"divides q's: {tuple(qs)}, {tuple(ks)}, {tuple(vs)}")
+    p = _DiffPlan()
+    p.sizes = B, H, Hkv, Lq, Lk
+    p.empty = B * H * Lq * Lk == 0
+    # (batch, head, row): of a size of one 0, of a single row 64
+    ins = [[t[i] if s[i] > 1 else d for i, d in ((0, 0), (2, 0), (1, E_TILE))]
+           for s, t in ((qs, qt), (ks, kt), (vs, vt))]
+    p.copy = [t[3] != 1 or any(x % 8 for x in s) or not E_TILE <= s[2] < _ATTN_ROW_SPAN
+              for s, t in zip(ins, (qt, kt, vt))]
+    p.strides = (ctypes.c_int64 * 9)(*sum(ins, []))
+    p.lse_shape, p.maps_shape = (B, H, Lq), (B, Lq, H // 2, 2, 2 * E_TILE)
+    p.fwd_ws = p.bwd_ws = 0
+    if not p.empty:
+        lib = _lib.load()
+        p.fwd_ws = lib.sla2h_diff_attn_fwd_workspace_bytes(*p.sizes)
+        p.bwd_ws = lib.sla2h_diff_attn_bwd_workspace_bytes(_HALF[dtype], *p.sizes)
+        # (a backward always has a workspace: 0 are sizes that the kernels do not take)
+        if not p.bwd_ws or not any(p.copy) and max(H, Hkv) * E_TILE >= _ATTN_ROW_SPAN:
+            raise _attn_too_large(qs, ks)
+    return p
+
+
+def _diff_operands(q, k, v, lam, scale):
+    """Checks; returns q, k, v (copied where the kernels do not take their strides or
+    alignment), lam in fp32, their plan and the scale."""
+    if not (q.is_cuda and k.is_cuda and v.is_cuda and lam.is_cuda):
+        _need_gpu(q, k, v, lam)
+    if not q.dtype == k.dtype == v.dtype or not q.device == k.device == v.device == lam.device:
+        raise ValueError("q, k and v must share their dtype, and with lam their device: "
+                         f"{q.dtype} {q.device}, {k.dtype} {k.device}, {v.dtype} {v.device}, "
+                         f"{lam.device}")
+    if q.dtype not in _HALF:
+        _dtype_code(q)
+    plan = _diff_plan(q.shape, q.stride(), k.shape, k.stride(), v.shape, v.stride(), q.dtype)
+    if lam.shape != (plan.sizes[1] // 2,) or not lam.is_floating_point():
+        raise ValueError(f"lam: expected {plan.sizes[1] // 2} floating-point numbers, one per pair "
+                         f"of heads, got {tuple(lam.shape)} {lam.dtype}")
+    if any(plan.copy) or (q.data_ptr() | k.data_ptr() | v.data_ptr()) % 16:
+        q, k, v = (t.clone(memory_format=torch.contiguous_format) if c or t.data_ptr() % 16 else t
+                   for t, c in zip((q, k, v), plan.copy))
+        plan = _diff_plan(q.shape, q.stride(), k.shape, k.stride(), v.shape, v.stride(), q.dtype)
+        if any(plan.copy):
+            raise _attn_too_large(q.shape, k.shape)
+    if lam.dtype != torch.float32 or not lam.is_contiguous():
+        lam = lam.to(torch.float32).contiguous()
+    if scale is None:
+        scale = E_TILE ** -0.5
+    elif not 0.0 < scale < 1e30:
+        raise ValueError(f"scale must be positive, got {scale}")
+    return q, k, v, lam, plan, float(scale)
+
+
+def diff_attn_fwd(q, k, v, lam, causal=False, q_lens=None, k_lens=None, scale=None, save=False):
+    """Differential attention of q (B, Lq, H, 64) over k, v (B, Lk, Hkv, 64), 16-bit, any strides
+    with a unit channel stride -> (o (B, Lq, H, 64), lse, maps).  The heads 2p and 2p + 1 are
+    two softmax maps over the same 128 value channels, the value heads 2 kp and 2 kp + 1 side by
+    side with kp = p // (H // Hkv): o = (A_1 - lam[p] A_2) v in the output heads 2p and 2p + 1.
+    lengths, causal order and scale as in dense_attn_fwd.  save: also what the backward
+    reads, lse (B, H, Lq) and maps (B, Lq, H // 2, 2, 128), A_1 v and A_2 v, fp32; else None."""
+    q, k, v, lam, p, scale = _diff_operands(q, k, v, lam, scale)
+    dev = q.device
+    if q_lens is not None:
+        q_lens = attn_lens(q_lens, q, "q_lens")
+    if k_lens is not None:
+        k_lens = attn_lens(k_lens, q, "k_lens")
+    o = torch.empty(q.shape, device=dev, dtype=q.dtype)
+    lse = torch.empty(p.lse_shape, device=dev, dtype=torch.float32) if save else None
+    maps = torch.empty(p.maps_shape, device=dev, dtype=torch.float32) if save else None
+    if p.empty:
+        o.zero_()
+        if save:
+            lse.fill_(float("-inf"))
+            maps.zero_()
+    else:
+        ws = _scratch(p.fwd_ws, dev) if p.fwd_ws else None
+        _launch(dev, "sla2h_diff_attn_fwd", q.data_ptr(), k.data_ptr(), v.data_ptr(),
+                lam.data_ptr(), p.strides, _ptr(q_lens), _ptr(k_lens), _HALF[q.dtype], *p.sizes,
+                1 if causal else 0, scale, _ptr(ws), o.data_ptr(), _ptr(lse), _ptr(maps))
+    return o, lse, maps
+
+
+def diff_attn_bwd(do, q, k, v, lam, lse, maps, causal=False, q_lens=None, k_lens=None, scale=None,
+                  need_q=True, need_kv=True):
+    """Gradients (dq, dk, dv, dlam fp32) of diff_attn_fwd for the output gradient do, from its
+    operands and what it saved, the maps recomputed; dk and dv summed over the query
+    pairs of a key pair, dlam over batch and rows.  Without need_q dq is None, without need_kv dk and dv."""
+    q, k, v, lam, p, scale = _diff_operands(q, k, v, lam, scale)
+    dev, dtype = q.device, q.dtype
+    if do.shape != q.shape or do.dtype != dtype or do.device != dev:
+        raise ValueError(f"do: expected {tuple(q.shape)} {dtype} on {dev}, got "
+                         f"{tuple(do.shape)} {do.dtype} on {do.device}")
+    for t, shape, name in ((lse, p.lse_shape, "lse"), (maps, p.maps_shape, "maps")):
+        if t.shape != shape or t.dtype != torch.float32 or t.device != dev:
+            raise ValueError(f"{name}: expected {shape} float32 on {dev}, got "
+                             f"{tuple(t.shape)} {t.dtype} on {t.device}")
+    do, maps, lse = aligned(do.contiguous(), 16), aligned(maps.contiguous(), 16), lse.contiguous()
+    if q_lens is not None:
+        q_lens = attn_lens(q_lens, q, "q_lens")
+    if k_lens is not None:
+        k_lens = attn_lens(k_lens, q, "k_lens")
+    dq = torch.empty(q.shape, device=dev, dtype=dtype) if need_q else None
+    dk = torch.empty(k.shape, device=dev, dtype=dtype) if need_kv else None
+    dv = torch.empty(v.shape, device=dev, dtype=dtype) if need_kv else None
+    dlam = torch.empty(lam.shape, device=dev, dtype=torch.float32)
+    if p.empty:
+        return tuple(t if t is None else t.zero_() for t in (dq, dk, dv, dlam))
+    ws = _scratch(p.bwd_ws, dev)
+    _launch(dev, "sla2h_diff_attn_bwd", q.data_ptr(), k.data_ptr(), v.data_ptr(), lam.data_ptr(),
+            do.data_ptr(), lse.data_ptr(), maps.data_ptr(), p.strides, _ptr(q_lens), _ptr(k_lens),
+            _HALF[dtype], *p.sizes, 1 if causal else 0, scale, ws.data_ptr(), _ptr(dq), _ptr(dk),
+            _ptr(dv), dlam.data_ptr())
+    return dq, dk, dv, dlam
