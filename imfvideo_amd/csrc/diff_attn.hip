@@ -550,14 +550,15 @@ struct FwdPlan {
   int64_t units;
 };
 
-FwdPlan fwd_plan(int B, int H, int Hkv, int64_t Lq, int64_t Lk) {
+// even: neither causal nor lengths
+FwdPlan fwd_plan(int B, int H, int Hkv, int64_t Lq, int64_t Lk, bool even) {
   FwdPlan p{};
   const int64_t bp = (int64_t)B * H / 2, bk = (int64_t)B * Hkv / 2, rep = H / Hkv;
   p.splits = 1;
   p.nq = 2;
   p.qtiles = (Lq + 127) / 128;
   p.nwork = bp * p.qtiles;
-  if (p.nwork >= 256) return p;
+  if (p.nwork >= (even ? 256 : 768)) return p;
   p.nq = 1;
   p.qtiles = (Lq + 63) / 64;
   p.nwork = bp * p.qtiles;
@@ -590,7 +591,7 @@ using namespace sla2h;
 extern "C" size_t sla2h_diff_attn_fwd_workspace_bytes(int B, int H, int Hkv, int64_t Lq,
                                                       int64_t Lk) {
   if (!diff_sizes_ok(B, H, Hkv, Lq, Lk)) return 0;
-  const FwdPlan p = fwd_plan(B, H, Hkv, Lq, Lk);
+  const FwdPlan p = fwd_plan(B, H, Hkv, Lq, Lk, true);  // the split forms do not depend on it
   return p.splits > 1 ? (size_t)p.splits * B * H * Lq * (128 * 4 + 8) : 0;
 }
 
@@ -612,7 +613,8 @@ extern "C" int sla2h_diff_attn_fwd(const void* q, const void* k, const void* v, 
   for (int i : {2, 5, 8}) SLA2H_CHECK_ARG(strides[i] >= kDD);
   // 32-bit byte offsets within a tile
   SLA2H_CHECK_ARG(strides[5] < ((int64_t)1 << 23) && strides[8] < ((int64_t)1 << 23));
-  const FwdPlan p = fwd_plan(B, H, Hkv, Lq, Lk);
+  const bool even = !causal && !q_lens && !k_lens;
+  const FwdPlan p = fwd_plan(B, H, Hkv, Lq, Lk, even);
   SLA2H_CHECK_ARG(p.splits == 1 || workspace);
   const int64_t nrows = (int64_t)B * (H / 2) * Lq;
   SLA2H_CHECK_ARG(p.nwork * (p.nq ? p.splits : 1) < ((int64_t)1 << 30));
@@ -638,8 +640,7 @@ extern "C" int sla2h_diff_attn_fwd(const void* q, const void* k, const void* v, 
   a.causal = causal != 0;
   a.c = scale * kLog2e;
   a.qtiles = (int)p.qtiles;
-  a.map = work_map((int64_t)B * a.P, p.qtiles * (p.nq ? p.splits : 1), !causal && !q_lens && !k_lens,
-                   causal);
+  a.map = work_map((int64_t)B * a.P, p.qtiles * (p.nq ? p.splits : 1), even, causal);
   a.splits = p.splits;
   a.units = (int)p.units;
   a.nrows = nrows;

@@ -33,6 +33,13 @@ struct Scaled<F16> {
   static constexpr bool value = true;
 };
 
+// What the rounding of dS to 16 bits lost is added by a second product.  dq (its rounding alone would
+// make it 1.5 times as far off as a rounded exact result): in all stages of sequences of at most
+// kFineKeys keys or kFineRows queries and of causal waves that see at most kFineRows keys, else in
+// every second stage (1.25 times; B = 1, H = 8, L = 29,952: 0.4 ms).  dk, dv: calls of at most
+// kFineRows rows per key pair (longer sums average the roundings out).
+constexpr int kFineKeys = 4096, kFineRows = 512;
+constexpr int kKeyRows = 256;  // keys of a workgroup of dk and dv
 constexpr int kNormRows = 64;  // rows of a partial maximum of the norms and of a partial sum of dlam
 
 struct DiffBwdArgs {
@@ -46,7 +53,7 @@ struct DiffBwdArgs {
   int B, P, Pk, rep;
   int causal;
   float c, inv_c, scale;
-  float* stat;          // [4][B * P * Lq]: (-lse_1, -lse_2) log2e / c, -delta_1, delta_1 - delta_2
+  float* stat;          // [4][B * P * Lq]: (shift - lse_m log2e) / c, -delta_m
   int64_t nrows;        // B * P * Lq
   float *gmax, *vmax;   // (B, P, nqb), (B, Pk, nkb): largest row norms (fp16)
   float* lsum;          // (B, P, nqb): sums of -delta_2
@@ -60,6 +67,26 @@ struct DiffBwdArgs {
 __device__ inline int first_query(int qlen, int klen, int causal) {
   if (klen == 0) return qlen;
   return causal && qlen > klen ? qlen - klen : 0;
+}
+
+// fp16: the exponents' shift of a key pair's group, with 2^shift (1 + |lam|) <= 2^15 for its weights.
+__device__ inline float power_of_two(int e) { return __builtin_bit_cast(float, (127 + e) << 23); }
+// e with x < 2^e, in [-100, 100]
+__device__ inline int exponent(float x) {
+  int e;
+  (void)frexpf(x, &e);
+  e = e < -100 ? -100 : (e > 100 ? 100 : e);
+  return __builtin_amdgcn_readfirstlane(e);
+}
+__device__ inline float top_weight(const DiffBwdArgs& a, int kp) {
+  float ml = 0.f;
+  for (int i = threadIdx.x & 63; i < a.rep; i += 64)
+    ml = fmaxf(ml, __builtin_fabsf(a.lam[kp * a.rep + i]));
+  return wave_max(ml);
+}
+__device__ inline int weight_shift(float ml) {
+  const float most = 1.f + ml;
+  return most < 1e30f ? 15 - exponent(most) : 15;  // 2^(e - 1) <= 1 + |lam| < 2^e
 }
 
 // delta of 64 rows of a pair (16 lanes per row), the sum of their -delta_2, and for fp16 the
@@ -77,6 +104,7 @@ __global__ __launch_bounds__(256) void diff_bwd_prep_kernel(DiffBwdArgs a, int64
   const int len = is_v ? klen : qlen;
   const int first = is_v ? 0 : first_query(qlen, klen, a.causal);
   float top = 0.f, sum = 0.f;
+  const float shift = Scaled<T16>::value && !is_v ? (float)weight_shift(top_weight(a, p / a.rep)) : 0.f;
 #pragma unroll
   for (int j = 0; j < kNormRows / 16; ++j) {
     const int64_t i = (int64_t)t * kNormRows + 16 * j + (tid >> 4);
@@ -113,10 +141,10 @@ __global__ __launch_bounds__(256) void diff_bwd_prep_kernel(DiffBwdArgs a, int64
 #pragma unroll
       for (int m = 0; m < 2; ++m)
         a.stat[m * a.nrows + f] =
-            live ? -a.lse[((int64_t)b * 2 * a.P + 2 * p + m) * a.Lq + i] * kLog2e * a.inv_c
+            live ? (shift - a.lse[((int64_t)b * 2 * a.P + 2 * p + m) * a.Lq + i] * kLog2e) * a.inv_c
                  : -__builtin_inff();
       a.stat[2 * a.nrows + f] = live ? -dot[0] : 0.f;
-      a.stat[3 * a.nrows + f] = live ? dot[0] - dot[1] : 0.f;
+      a.stat[3 * a.nrows + f] = live ? -dot[1] : 0.f;
     }
     sum += c0 == 0 ? -dot[1] : 0.f;
   }
@@ -135,42 +163,25 @@ __global__ __launch_bounds__(256) void diff_bwd_prep_kernel(DiffBwdArgs a, int64
   if (!is_v) a.lsum[blk] = (red[1][0] + red[1][1]) + (red[1][2] + red[1][3]);
 }
 
-// fp16: the exponents' shift and the power of two m with 2 max|do| max|v| max(1, |lam|) m <= 1,
-// for a key pair's group.
+// fp16: the power of two m with 2 max|do| max|v| max(1, |lam|) m <= 1 for a key pair's group, and
+// what takes the exponents' shift out again.
 struct Powers {
-  float shift, m, back;  // back: 2^-shift
+  float m, back;
 };
-__device__ inline float power_of_two(int e) { return __builtin_bit_cast(float, (127 + e) << 23); }
-// e with x < 2^e, in [-100, 100]
-__device__ inline int exponent(float x) {
-  int e;
-  (void)frexpf(x, &e);
-  e = e < -100 ? -100 : (e > 100 ? 100 : e);
-  return __builtin_amdgcn_readfirstlane(e);
-}
 __device__ inline Powers powers(const DiffBwdArgs& a, int b, int kp) {
   const int l = threadIdx.x & 63;
   const int64_t ng = (int64_t)a.rep * a.nqb;
   const float* g = a.gmax + ((int64_t)b * a.P + (int64_t)kp * a.rep) * a.nqb;
   const float* v = a.vmax + ((int64_t)b * a.Pk + kp) * a.nkb;
-  float mg = 0.f, mv = 0.f, ml = 0.f;
+  float mg = 0.f, mv = 0.f;
 #pragma unroll 8
   for (int64_t i = l; i < ng; i += 64) mg = fmaxf(mg, g[i]);
 #pragma unroll 8
   for (int i = l; i < a.nkb; i += 64) mv = fmaxf(mv, v[i]);
-  for (int i = l; i < a.rep; i += 64) ml = fmaxf(ml, __builtin_fabsf(a.lam[kp * a.rep + i]));
-  ml = wave_max(ml);
-  Powers r{15.f, 1.f, power_of_two(-15)};
-  const float most = 1.f + ml;
-  if (most < 1e30f) {
-    // 2^(e - 1) <= 1 + |lam| < 2^e
-    const int e = exponent(most);
-    r.shift = 15.f - (float)e;
-    r.back = power_of_two(e - 15);
-  }
+  const float ml = top_weight(a, kp);
   const float bound = 2.f * wave_max(mg) * wave_max(mv) * fmaxf(ml, 1.f);
-  if (bound > 0.f && bound < 1e30f) r.m = power_of_two(-exponent(bound));
-  return r;
+  return Powers{bound > 0.f && bound < 1e30f ? power_of_two(-exponent(bound)) : 1.f,
+                power_of_two(-weight_shift(ml))};
 }
 
 // A C tile pair ([channel][row]) of a lane's row: 16-bit, or fp32 parts.
@@ -200,7 +211,7 @@ __device__ inline void store_part(float* p, const f32x16 (&x)[2], float f, int h
 // dq: workgroup = 4 waves x 32 query rows of a pair; keys of both maps and values in stages of 32
 // through four LDS slots, three ahead.  dQ_m^T += K_m^T dS_m^T with dS_m^T straight from the score
 // tile's registers.
-template <typename T16, bool FINE>
+template <typename T16>
 __global__ __launch_bounds__(256, 2) void diff_bwd_dq_kernel(DiffBwdArgs a) {
   __shared__ __align__(16) unsigned char s0[kStageB], s1[kStageB], s2[kStageB], s3[kStageB];
   const int tid = threadIdx.x, l = tid & 63, h = l >> 5;
@@ -245,7 +256,7 @@ __global__ __launch_bounds__(256, 2) void diff_bwd_dq_kernel(DiffBwdArgs a) {
     load_unit(src, row, (int64_t)klen - row, ld, s + w * kUnitB, l);
   };
 
-  Powers pw{0.f, 1.f, 1.f};
+  Powers pw{1.f, 1.f};
   if (Scaled<T16>::value) pw = powers(a, b, kp);
   const int i = qw + (l & 31);
   const int lim = key_limit(i, qlen, klen, a.causal);
@@ -253,10 +264,10 @@ __global__ __launch_bounds__(256, 2) void diff_bwd_dq_kernel(DiffBwdArgs a) {
   const int64_t flat = (int64_t)bp * a.Lq + i;
   float nl[2], nd[2];  // shift - lse_m log2e, -delta_m (times m)
 #pragma unroll
-  for (int m = 0; m < 2; ++m)
-    nl[m] = live ? a.stat[m * a.nrows + flat] * a.c + pw.shift : -__builtin_inff();
-  nd[0] = live ? a.stat[2 * a.nrows + flat] * pw.m : 0.f;
-  nd[1] = live ? nd[0] + a.stat[3 * a.nrows + flat] * pw.m : 0.f;
+  for (int m = 0; m < 2; ++m) {
+    nl[m] = live ? a.stat[m * a.nrows + flat] * a.c : -__builtin_inff();
+    nd[m] = live ? a.stat[(2 + m) * a.nrows + flat] * pw.m : 0.f;
+  }
   u32x4 qf[2][4], gf[2][4];
 #pragma unroll
   for (int m = 0; m < 2; ++m) {
@@ -272,11 +283,13 @@ __global__ __launch_bounds__(256, 2) void diff_bwd_dq_kernel(DiffBwdArgs a) {
   const int wlast = min(qw + 32, qlen) - 1;
   const int wany = wlast >= qw ? key_limit(wlast, qlen, klen, a.causal) : 0;
   const int wall = wlast >= qw ? key_limit(qw, qlen, klen, a.causal) : 0;
+  const bool few = klen <= kFineKeys || wany <= kFineRows || qlen <= kFineRows;
 
   f32x16 acc[2][2];
 #pragma unroll
   for (int m = 0; m < 2; ++m) acc[m][0] = acc[m][1] = zero16();
-  auto part = [&](auto masked, int base, const unsigned char* s) __attribute__((always_inline)) {
+  auto part = [&](auto masked, bool fine, int base, const unsigned char* s)
+      __attribute__((always_inline)) {
     f32x16 sc[2] = {zero16(), zero16()}, dp = zero16();
 #pragma unroll
     for (int x = 0; x < 4; ++x) {
@@ -306,7 +319,7 @@ __global__ __launch_bounds__(256, 2) void diff_bwd_dq_kernel(DiffBwdArgs a) {
           kf[mb] = col_frag(s + m * kUnitB, 16 * x, mb, lo);
           acc[m][mb] = mfma_32x32x16<T16>(kf[mb], ds, acc[m][mb]);
         }
-        if (FINE) {
+        if (fine) {
           const u32x4 lost = lost_step<T16>(d, x, ds);
 #pragma unroll
           for (int mb = 0; mb < 2; ++mb)
@@ -315,7 +328,7 @@ __global__ __launch_bounds__(256, 2) void diff_bwd_dq_kernel(DiffBwdArgs a) {
       }
     }
   };
-  auto stage = [&](int t, const unsigned char* cur, unsigned char* to)
+  auto stage = [&](int t, bool fine, const unsigned char* cur, unsigned char* to)
       __attribute__((always_inline)) {
     // the stages up to t have landed, stage t - 1 is read
     __builtin_amdgcn_s_waitcnt(wait_vm_lgkm0(8));
@@ -323,21 +336,21 @@ __global__ __launch_bounds__(256, 2) void diff_bwd_dq_kernel(DiffBwdArgs a) {
     load(t + 3, to);
     const int base = t * kUnitRows;
     if (base + kUnitRows <= wall)  // a stage that every query of the wave sees: no branch inside
-      part(std::false_type{}, base, cur);
+      part(std::false_type{}, fine, base, cur);
     else if (base < wany)
-      part(std::true_type{}, base, cur);
+      part(std::true_type{}, true, base, cur);
   };
   load(t0, s0);
   load(t0 + 1, s1);
   load(t0 + 2, s2);
   for (int t = t0; t < nt; t += 4) {
-    stage(t, s0, s3);
+    stage(t, true, s0, s3);
     if (t + 1 >= nt) break;
-    stage(t + 1, s1, s0);
+    stage(t + 1, few, s1, s0);
     if (t + 2 >= nt) break;
-    stage(t + 2, s2, s1);
+    stage(t + 2, true, s2, s1);
     if (t + 3 >= nt) break;
-    stage(t + 3, s3, s2);
+    stage(t + 3, few, s3, s2);
   }
   __builtin_amdgcn_s_waitcnt(wait_vm_lgkm0(0));  // no load into this LDS outlives the workgroup
 
@@ -354,15 +367,30 @@ __global__ __launch_bounds__(256, 2) void diff_bwd_dq_kernel(DiffBwdArgs a) {
   }
 }
 
-// dk, dv: workgroup = 4 waves x 32 keys of one key pair; the query rows (both maps' queries, the 128
-// channels of do) of the pairs that read it are streamed in stages of 32 rows, with their four
-// statistics, which start the accumulators of S_m and dA.  A wave holds 128 channels of dv, 64
-// of each dk and its keys and values: one wave per SIMD.  The stage is software-pipelined: S_m and dA
-// of the next stage run on the matrix cores under this stage's exponentials.
+// The value that the lanes' place e of 16 holds, in all lanes of their row of 16.
+template <int E>
+__device__ inline float row_value(float x) {
+  return __builtin_bit_cast(
+      float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, x), 0x150 + E, 0xf, 0xf, true));
+}
+// x[e] + that value, register e of a C tile
+template <int E = 0>
+__device__ inline void add_rows(f32x16& x, float v) {
+  x[E] += row_value<E>(v);
+  if constexpr (E < 15) add_rows<E + 1>(x, v);
+}
+
+// dk, dv: workgroup = 8 waves x 32 keys of one key pair; the query rows (both maps' queries, the 128
+// channels of do) of the pairs that read it are streamed in stages of 32 rows, three ahead in four
+// LDS slots, with their four statistics.  A wave holds 128 channels of dv, 64 of each dk and its keys
+// in registers; its values lie in LDS, so that two waves fit on a SIMD (with them in registers, and one
+// wave: 6.1 ms at B = 1, H = 8, L = 29,952, bf16).  A row's statistic belongs to one register of a
+// score tile in all lanes of a half: a lane reads one value, and the add takes it from there (DPP).
 template <typename T16, bool CAUSAL, bool FINE>
-__global__ __launch_bounds__(256, 1) void diff_bwd_dkdv_kernel(DiffBwdArgs a) {
+__global__ __launch_bounds__(512, 2) void diff_bwd_dkdv_kernel(DiffBwdArgs a) {
   __shared__ __align__(16) unsigned char r0[kStageB], r1[kStageB], r2[kStageB], r3[kStageB];
   __shared__ __align__(16) float t0_[4][64], t1_[4][64], t2_[4][64], t3_[4][64];
+  __shared__ __align__(16) unsigned char vt[8][2 * kUnitB];
   int bk, item;
   if (!work_item(a.kv_map, blockIdx.x, bk, item)) return;
   const int ktile = item / a.kv_splits, sp = item - ktile * a.kv_splits;
@@ -372,7 +400,7 @@ __global__ __launch_bounds__(256, 1) void diff_bwd_dkdv_kernel(DiffBwdArgs a) {
   const LaneOff lo(l);
   const int qlen = seq_len(a.q_lens, b, a.Lq), klen = seq_len(a.k_lens, b, a.Lk);
 
-  const int key0 = ktile * 128, kw = key0 + w * 32;
+  const int key0 = ktile * kKeyRows, kw = key0 + w * 32;
   // first query that sees a key of the workgroup (causal: i >= j - off)
   const int off = klen - qlen;
   int first = first_query(qlen, klen, a.causal);
@@ -382,137 +410,123 @@ __global__ __launch_bounds__(256, 1) void diff_bwd_dkdv_kernel(DiffBwdArgs a) {
   const int per = (total + a.kv_splits - 1) / a.kv_splits;
   const int u0 = sp * per, u1 = min(total, u0 + per);
 
+  // this wave's values
+#pragma unroll
+  for (int m = 0; m < 2; ++m)
+    load_unit(a.v + b * a.vb + (2 * kp + m) * a.vh, kw, (int64_t)klen - kw, a.vl * 2,
+              vt[w] + m * kUnitB, l);
+
   // the stage to load next, and the one to compute (their pair of the group and first row)
   int lu = u0, lp = u0 < u1 ? u0 / nq : 0;
   int lrow = first + (u0 < u1 ? u0 - lp * nq : 0) * kUnitRows;
   int cu = u0, cp = lp, crow = lrow;
+  // waves 2x and 2x + 1 load matrix x of the stage, 16 rows each, and statistic x (both the same)
+  const int x = w >> 1;
   auto load = [&](unsigned char* s, float (*st)[64]) __attribute__((always_inline)) {
     const int64_t p = (int64_t)kp * a.rep + lp, n = lu < u1 ? (int64_t)qlen - lrow : 0;
-    if (w < 2)
-      load_unit(a.q + b * a.qb + (2 * p + w) * a.qh, lrow, n, a.ql * 2, s + w * kUnitB, l);
-    else
-      load_unit(a.dout + ((int64_t)b * a.Lq * a.P + p) * 128 + 64 * (w - 2), lrow, n,
-                (int64_t)a.P * 256, s + w * kUnitB, l);
-    const auto rs = make_rsrc(a.stat + w * a.nrows + ((int64_t)b * a.P + p) * a.Lq + lrow,
+    const uint16_t* src = x < 2 ? a.q + b * a.qb + (2 * p + x) * a.qh
+                                : a.dout + ((int64_t)b * a.Lq * a.P + p) * 128 + 64 * (x - 2);
+    const int64_t ld = x < 2 ? a.ql * 2 : (int64_t)a.P * 256;
+    const auto rs = rows_rsrc(src, lrow, n < kUnitRows ? n : kUnitRows, ld);
+#pragma unroll
+    for (int j = 0; j < 2; ++j) dma_rows8(rs, s + x * kUnitB, 2 * (w & 1) + j, (int)ld, l);
+    const auto rt = make_rsrc(a.stat + x * a.nrows + ((int64_t)b * a.P + p) * a.Lq + lrow,
                               n <= 0 ? 0 : (n < kUnitRows ? n : kUnitRows) * 4);
     __builtin_amdgcn_raw_ptr_buffer_load_lds(
-        rs, (__attribute__((address_space(3))) void*)&st[w][0], 4, 4 * l, 0, 0, 0);
+        rt, (__attribute__((address_space(3))) void*)&st[x][0], 4, 4 * l, 0, 0, 0);
     ++lu;
     lrow += kUnitRows;
     if (lrow >= qlen && lu < u1) lrow = first, ++lp;
   };
 
-  Powers pw{0.f, 1.f, 1.f};
+  Powers pw{1.f, 1.f};
   if (Scaled<T16>::value) pw = powers(a, b, kp);
-  u32x4 kf[2][4], vf[2][4];
+  u32x4 kf[2][4];
   {
     const int j = kw + (l & 31);
-    const bool live = j < klen;
 #pragma unroll
     for (int m = 0; m < 2; ++m)
 #pragma unroll
-      for (int s = 0; s < 4; ++s) {
-        kf[m][s] = live ? *reinterpret_cast<const u32x4*>(a.k + b * a.kb + (2 * kp + m) * a.kh +
-                                                          j * a.kl + 16 * s + 8 * h)
-                        : u32x4{0, 0, 0, 0};
-        vf[m][s] = live ? *reinterpret_cast<const u32x4*>(a.v + b * a.vb + (2 * kp + m) * a.vh +
-                                                          j * a.vl + 16 * s + 8 * h)
-                        : u32x4{0, 0, 0, 0};
-      }
+      for (int s = 0; s < 4; ++s)
+        kf[m][s] = j < klen ? *reinterpret_cast<const u32x4*>(a.k + b * a.kb + (2 * kp + m) * a.kh +
+                                                              j * a.kl + 16 * s + 8 * h)
+                            : u32x4{0, 0, 0, 0};
   }
   f32x16 ak[2][2], av[4];
 #pragma unroll
-  for (int x = 0; x < 2; ++x) ak[0][x] = ak[1][x] = av[x] = av[2 + x] = zero16();
-  f32x16 sc[2][2], dp[2];
+  for (int y = 0; y < 2; ++y) ak[0][y] = ak[1][y] = av[y] = av[2 + y] = zero16();
+  // register e of a tile is row 8 (e / 4) + 4 h + e % 4: lane e of each 16 reads it
+  const int srow = 8 * ((l & 15) >> 2) + 4 * h + (l & 3);
 
-  // S_m and dA - delta_1 of a stage
-  auto scores = [&](int x, const unsigned char* s, const float (*st)[64])
+  auto stage = [&](const unsigned char* s, const float (*st)[64], unsigned char* sl, float (*tl)[64])
       __attribute__((always_inline)) {
-#pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      const f32x4 y0 = *reinterpret_cast<const f32x4*>(&st[0][8 * g + 4 * h]);
-      const f32x4 y1 = *reinterpret_cast<const f32x4*>(&st[1][8 * g + 4 * h]);
-      const f32x4 y2 = *reinterpret_cast<const f32x4*>(&st[2][8 * g + 4 * h]);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        sc[x][0][4 * g + i] = y0[i];
-        sc[x][1][4 * g + i] = y1[i];
-        dp[x][4 * g + i] = y2[i];
-      }
-    }
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      sc[x][0] = mfma_32x32x16<T16>(row_frag(s, 0, k, lo), kf[0][k], sc[x][0]);
-      dp[x] = mfma_32x32x16<T16>(row_frag(s + 2 * kUnitB, 0, k, lo), vf[0][k], dp[x]);
-      sc[x][1] = mfma_32x32x16<T16>(row_frag(s + kUnitB, 0, k, lo), kf[1][k], sc[x][1]);
-      dp[x] = mfma_32x32x16<T16>(row_frag(s + 3 * kUnitB, 0, k, lo), vf[1][k], dp[x]);
-    }
-  };
-  auto stage = [&](int x, const unsigned char* s, const float (*st)[64], const unsigned char* sn,
-                   const float (*tn)[64], unsigned char* sl, float (*tl)[64])
-      __attribute__((always_inline)) {
-    // the stages up to the next one have landed, the one before is read
-    __builtin_amdgcn_s_waitcnt(wait_vm_lgkm0(5));
+    // the stages up to this one have landed, the one before is read
+    __builtin_amdgcn_s_waitcnt(wait_vm_lgkm0(6));
     __builtin_amdgcn_s_barrier();
     load(sl, tl);
     if (kw < klen) {
       const float lam = a.lam[kp * a.rep + cp];
-      scores(x ^ 1, sn, tn);
-      f32x16 p1, p2, d1, d2;
-      const float sh = pw.shift;
+      const bool hidden = CAUSAL && crow < kw + 31 - off;
+      const int y = kw + (l & 31) - off - crow - 4 * h;
+      float sv[4];
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        p1[e] = fast_exp2(Scaled<T16>::value ? __builtin_fmaf(sc[x][0][e], a.c, sh) : sc[x][0][e] * a.c);
-        p2[e] = lam * fast_exp2(Scaled<T16>::value ? __builtin_fmaf(sc[x][1][e], a.c, sh)
-                                                   : sc[x][1][e] * a.c);
-      }
-      if (CAUSAL && crow < kw + 31 - off) {
-        asm volatile("");
-        const int y = kw + (l & 31) - off - crow - 4 * h;
+      for (int i = 0; i < 4; ++i) sv[i] = st[i][srow];
+      f32x16 dp = zero16(), p[2] = {zero16(), zero16()};
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          p1[e] = 8 * (e >> 2) + (e & 3) >= y ? p1[e] : 0.f;
-          p2[e] = 8 * (e >> 2) + (e & 3) >= y ? p2[e] : 0.f;
-        }
+      for (int k = 0; k < 4; ++k) {
+        p[0] = mfma_32x32x16<T16>(row_frag(s, 0, k, lo), kf[0][k], p[0]);
+        dp = mfma_32x32x16<T16>(row_frag(s + 2 * kUnitB, 0, k, lo), row_frag(vt[w], 0, k, lo), dp);
+        dp = mfma_32x32x16<T16>(row_frag(s + 3 * kUnitB, 0, k, lo),
+                                row_frag(vt[w] + kUnitB, 0, k, lo), dp);
       }
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const f32x4 dd = *reinterpret_cast<const f32x4*>(&st[3][8 * g + 4 * h]);
+      for (int m = 0; m < 2; ++m) {
+        if (m == 1) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int e = 4 * g + i;
-          d1[e] = (Scaled<T16>::value ? p1[e] * pw.m : p1[e]) * dp[x][e];
-          d2[e] = (Scaled<T16>::value ? p2[e] * pw.m : p2[e]) * (dp[x][e] + dd[i]);
-          p1[e] -= p2[e];
+          for (int k = 0; k < 4; ++k)
+            p[1] = mfma_32x32x16<T16>(row_frag(s + kUnitB, 0, k, lo), kf[1][k], p[1]);
         }
-      }
+        add_rows(p[m], sv[m]);
 #pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        const u32x4 pp = pack_step<T16>(p1, k), dd1 = pack_step<T16>(d1, k),
-                    dd2 = pack_step<T16>(d2, k);
-        u32x4 gf[4], qf[2][2];
+        for (int e = 0; e < 16; ++e) p[m][e] = fast_exp2(p[m][e] * a.c);
+        if (m == 1) {
 #pragma unroll
-        for (int mb = 0; mb < 4; ++mb) {
-          gf[mb] = col_frag(s + (2 + (mb >> 1)) * kUnitB, 16 * k, mb & 1, lo);
-          av[mb] = mfma_32x32x16<T16>(gf[mb], pp, av[mb]);
+          for (int e = 0; e < 16; ++e) p[1][e] *= lam;
         }
+        if (hidden) {
+          asm volatile("");
 #pragma unroll
-        for (int m = 0; m < 2; ++m)
+          for (int e = 0; e < 16; ++e) p[m][e] = 8 * (e >> 2) + (e & 3) >= y ? p[m][e] : 0.f;
+        }
+        f32x16 d = dp;
+        add_rows(d, sv[2 + m]);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) d[e] *= Scaled<T16>::value ? p[m][e] * pw.m : p[m][e];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const u32x4 dd = pack_step<T16>(d, k);
+          u32x4 lost;
+          if (FINE) lost = lost_step<T16>(d, k, dd);
 #pragma unroll
           for (int mb = 0; mb < 2; ++mb) {
-            qf[m][mb] = col_frag(s + m * kUnitB, 16 * k, mb, lo);
-            ak[m][mb] = mfma_32x32x16<T16>(qf[m][mb], m ? dd2 : dd1, ak[m][mb]);
+            const u32x4 qf = col_frag(s + m * kUnitB, 16 * k, mb, lo);
+            ak[m][mb] = mfma_32x32x16<T16>(qf, dd, ak[m][mb]);
+            if (FINE) ak[m][mb] = mfma_32x32x16<T16>(qf, lost, ak[m][mb]);
           }
-        if (FINE) {
-          const u32x4 pl = lost_step<T16>(p1, k, pp), dl1 = lost_step<T16>(d1, k, dd1),
-                      dl2 = lost_step<T16>(d2, k, dd2);
+        }
+      }
 #pragma unroll
-          for (int mb = 0; mb < 4; ++mb) av[mb] = mfma_32x32x16<T16>(gf[mb], pl, av[mb]);
+      for (int e = 0; e < 16; ++e) p[0][e] -= p[1][e];
 #pragma unroll
-          for (int m = 0; m < 2; ++m)
+      for (int k = 0; k < 2; ++k) {
+        const u32x4 pp = pack_step<T16>(p[0], k);
+        u32x4 lost;
+        if (FINE) lost = lost_step<T16>(p[0], k, pp);
 #pragma unroll
-            for (int mb = 0; mb < 2; ++mb)
-              ak[m][mb] = mfma_32x32x16<T16>(qf[m][mb], m ? dl2 : dl1, ak[m][mb]);
+        for (int mb = 0; mb < 4; ++mb) {
+          const u32x4 gf = col_frag(s + (2 + (mb >> 1)) * kUnitB, 16 * k, mb & 1, lo);
+          av[mb] = mfma_32x32x16<T16>(gf, pp, av[mb]);
+          if (FINE) av[mb] = mfma_32x32x16<T16>(gf, lost, av[mb]);
         }
       }
     }
@@ -523,17 +537,14 @@ __global__ __launch_bounds__(256, 1) void diff_bwd_dkdv_kernel(DiffBwdArgs a) {
   load(r0, t0_);
   load(r1, t1_);
   load(r2, t2_);
-  __builtin_amdgcn_s_waitcnt(wait_vm_lgkm0(10));
-  __builtin_amdgcn_s_barrier();
-  scores(0, r0, t0_);
   for (int u = u0; u < u1; u += 4) {
-    stage(0, r0, t0_, r1, t1_, r3, t3_);
+    stage(r0, t0_, r3, t3_);
     if (u + 1 >= u1) break;
-    stage(1, r1, t1_, r2, t2_, r0, t0_);
+    stage(r1, t1_, r0, t0_);
     if (u + 2 >= u1) break;
-    stage(0, r2, t2_, r3, t3_, r1, t1_);
+    stage(r2, t2_, r1, t1_);
     if (u + 3 >= u1) break;
-    stage(1, r3, t3_, r0, t0_, r2, t2_);
+    stage(r3, t3_, r2, t2_);
   }
   __builtin_amdgcn_s_waitcnt(wait_vm_lgkm0(0));
 
@@ -583,16 +594,15 @@ BwdPlan bwd_plan(int dtype, int B, int H, int Hkv, int64_t Lq, int64_t Lk, bool 
   BwdPlan p{};
   const int64_t bp = (int64_t)B * H / 2, bk = (int64_t)B * Hkv / 2, rep = H / Hkv;
   p.qtiles = (Lq + 127) / 128;
-  auto split = [&](int64_t blocks, int64_t units) {
-    const int64_t want = even ? 256 : 512;
+  auto split = [&](int64_t blocks, int64_t units, int64_t want) {
     if (blocks >= want / 2) return 1;
     const int64_t s = (want + blocks - 1) / blocks, most = units / 8;
     return (int)(s < most ? s : (most < 1 ? 1 : most));
   };
-  p.dq_splits = split(bp * p.qtiles, (Lk + 31) / 32);
+  p.dq_splits = split(bp * p.qtiles, (Lk + 31) / 32, even ? 256 : 800);
   p.dq_nwork = bp * p.qtiles * p.dq_splits;
-  p.ktiles = (Lk + 127) / 128;
-  p.kv_splits = split(bk * p.ktiles, rep * ((Lq + 31) / 32));
+  p.ktiles = (Lk + kKeyRows - 1) / kKeyRows;
+  p.kv_splits = split(bk * p.ktiles, rep * ((Lq + 31) / 32), even ? 256 : 512);
   p.kv_nwork = bk * p.ktiles * p.kv_splits;
   p.nqb = (Lq + kNormRows - 1) / kNormRows;
   p.nkb = (Lk + kNormRows - 1) / kNormRows;
@@ -696,13 +706,18 @@ extern "C" int sla2h_diff_attn_bwd(const void* q, const void* k, const void* v, 
     if ((err = (int)hipGetLastError())) return err;
     if (dk) {
       const unsigned grid = work_grid(a.kv_map);
-      if (causal)
-        diff_bwd_dkdv_kernel<T16, true, false><<<grid, 256, 0, st>>>(a);
+      const bool few = a.rep * Lq <= kFineRows;
+      if (causal && few)
+        diff_bwd_dkdv_kernel<T16, true, true><<<grid, 512, 0, st>>>(a);
+      else if (causal)
+        diff_bwd_dkdv_kernel<T16, true, false><<<grid, 512, 0, st>>>(a);
+      else if (few)
+        diff_bwd_dkdv_kernel<T16, false, true><<<grid, 512, 0, st>>>(a);
       else
-        diff_bwd_dkdv_kernel<T16, false, false><<<grid, 256, 0, st>>>(a);
+        diff_bwd_dkdv_kernel<T16, false, false><<<grid, 512, 0, st>>>(a);
       if ((err = (int)hipGetLastError())) return err;
     }
-    diff_bwd_dq_kernel<T16, false><<<a.dq_blocks + a.P, 256, 0, st>>>(a);
+    diff_bwd_dq_kernel<T16><<<a.dq_blocks + a.P, 256, 0, st>>>(a);
     if ((err = (int)hipGetLastError())) return err;
     auto join = [&](int splits, int64_t n, const float* p0, const float* p1, uint16_t* y0,
                     uint16_t* y1) {
