@@ -24,12 +24,18 @@ namespace {
 // (singular values of X stay below 1.3 with the usual coefficients) keep hi finite.
 constexpr float kScaleX = 4096.f, kScaleB = 512.f;
 
+// A matrix of pairs: rows of blocks of 32 columns, [32 hi | 32 lo] each, 128 bytes: the row of an LDS
+// tile, so that one load brings both halves.  Element of the block's first half for column j:
+__device__ inline int64_t pair_index(int64_t i, int j, int ld) {
+  return i * 2 * ld + 2 * (j & ~31) + (j & 31);
+}
+
 struct OrthoArgs {
   const void* g;        // (n, R, C)
   void* out;
   double* sums;         // (n, parts) partial sums of squares
-  uint16_t *x, *y;      // (n, 2, rp, mp) hi and lo: the step's X and the next one
-  uint16_t *A, *B;      // (n, 2, rp, rp)
+  uint16_t *x, *y;      // (n, rp, mp) pairs: the step's X and the next one
+  uint16_t *A, *B;      // (n, rp, rp) pairs
   int64_t n, count;     // matrices, elements of one
   int R, C, r, m, rp, mp, parts;
   bool turn;            // rows of X are G's columns
@@ -42,27 +48,50 @@ __device__ inline float load_g(const OrthoArgs& a, int dtype, int64_t i) {
   return dtype == SLA2H_DTYPE_BF16 ? BF16::to_f32(v) : F16::to_f32(v);
 }
 
+__device__ inline double wave_sum(double v) {
+#pragma unroll
+  for (int s = 32; s >= 1; s >>= 1) v += __shfl_xor(v, s, 64);
+  return v;
+}
+
 // Partial sums of squares in double: no overflow of a float's square, and the same sum whatever
-// the launch.  Thread by thread over the part, then a tree.
-__global__ __launch_bounds__(256) void ortho_norm_kernel(OrthoArgs a, int dtype) {
-  __shared__ double red[256];
+// the launch.  Thread by thread over the part (multiples of eight values), then a tree.
+__global__ __launch_bounds__(256) void ortho_norm_kernel(OrthoArgs a, int dtype, int aligned) {
+  __shared__ double red[4];
   const int64_t mat = blockIdx.x / a.parts;
   const int part = (int)(blockIdx.x - mat * a.parts);
-  const int64_t per = (a.count + a.parts - 1) / a.parts;
+  const int64_t per = ((a.count + a.parts - 1) / a.parts + 7) & ~(int64_t)7;
   const int64_t lo = part * per, hi = lo + per < a.count ? lo + per : a.count;
   double s = 0.0;
-#pragma unroll 4
-  for (int64_t i = lo + threadIdx.x; i < hi; i += 256) {
-    const double v = load_g(a, dtype, mat * a.count + i);
-    s += v * v;
+#pragma unroll 2
+  for (int64_t i = lo + 8 * (int)threadIdx.x; i < hi; i += 2048) {
+    float v[8];
+    const int64_t at = mat * a.count + i;
+    if (aligned && i + 8 <= hi) {
+      if (dtype == 2) {
+        const f32x4* q = reinterpret_cast<const f32x4*>(static_cast<const float*>(a.g) + at);
+        const f32x4 x = q[0], y = q[1];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = x[e], v[4 + e] = y[e];
+      } else {
+        const u32x4 x = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(a.g) + at);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const uint16_t u = (uint16_t)(x[e >> 1] >> (16 * (e & 1)));
+          v[e] = dtype == SLA2H_DTYPE_BF16 ? BF16::to_f32(u) : F16::to_f32(u);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = i + e < hi ? load_g(a, dtype, at + e) : 0.f;
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) s += (double)v[e] * (double)v[e];
   }
-  red[threadIdx.x] = s;
+  s = wave_sum(s);
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
   __syncthreads();
-  for (int w = 128; w >= 1; w >>= 1) {
-    if ((int)threadIdx.x < w) red[threadIdx.x] += red[threadIdx.x + w];
-    __syncthreads();
-  }
-  if (threadIdx.x == 0) a.sums[blockIdx.x] = red[0];
+  if (threadIdx.x == 0) a.sums[blockIdx.x] = (red[0] + red[1]) + (red[2] + red[3]);
 }
 
 // hi and lo of a scaled value
@@ -91,8 +120,8 @@ __global__ __launch_bounds__(256) void ortho_split_kernel(OrthoArgs a, int dtype
   const int tm = a.mp / 64, tr = a.rp / 64;
   const int64_t mat = blockIdx.x / (tm * tr);
   const int t = (int)(blockIdx.x - mat * (tm * tr)), i0 = t / tm * 64, j0 = t % tm * 64;
-  double s = 0.0;
-  for (int p = 0; p < a.parts; ++p) s += a.sums[mat * a.parts + p];
+  const int lane = threadIdx.x & 63;  // (at most 64 parts)
+  const double s = wave_sum(lane < a.parts ? a.sums[mat * a.parts + lane] : 0.0);
   const double inv = s == 0.0 ? 0.0 : (double)kScaleX / sqrt(s);
   const int q = threadIdx.x & 63, w = threadIdx.x >> 6;
   // G's rows of the tile, 64 lanes side by side
@@ -105,7 +134,6 @@ __global__ __launch_bounds__(256) void ortho_split_kernel(OrthoArgs a, int dtype
   }
   __syncthreads();
   uint16_t* x = a.x + mat * 2 * a.rp * a.mp;
-  const int64_t plane = (int64_t)a.rp * a.mp;
   const int c = 4 * (threadIdx.x & 15);
   for (int k = threadIdx.x >> 4; k < 64; k += 16) {
     float v[4];
@@ -113,10 +141,22 @@ __global__ __launch_bounds__(256) void ortho_split_kernel(OrthoArgs a, int dtype
     for (int e = 0; e < 4; ++e) v[e] = a.turn ? tile[c + e][k] : tile[k][c + e];
     u32x2 hi, lo;
     split4(v, hi, lo);
-    uint16_t* d = x + (int64_t)(i0 + k) * a.mp + j0 + c;
+    uint16_t* d = x + pair_index(i0 + k, j0 + c, a.mp);
     *reinterpret_cast<u32x2*>(d) = hi;
-    *reinterpret_cast<u32x2*>(d + plane) = lo;
+    *reinterpret_cast<u32x2*>(d + 32) = lo;
   }
+}
+
+// Element (i, j) of the last X (scaled), where G has one, in G's type and layout.
+__device__ inline void store_out(const OrthoArgs& a, int dtype, int64_t mat, int i, int j, float v) {
+  if (i >= a.r || j >= a.m) return;
+  v *= 1.f / kScaleX;
+  const int64_t at = mat * a.count + (a.turn ? (int64_t)j * a.C + i : (int64_t)i * a.C + j);
+  if (dtype == 2)
+    static_cast<float*>(a.out)[at] = v;
+  else
+    static_cast<uint16_t*>(a.out)[at] =
+        dtype == SLA2H_DTYPE_BF16 ? BF16::from_f32(v) : F16::from_f32(v);
 }
 
 enum { kGram, kPoly, kStep, kLast };
@@ -138,17 +178,25 @@ __device__ inline u32x4 turned_frag(const unsigned char* tile, int s, int mb, co
   return u32x4{lo.x, lo.y, hi.x, hi.y};
 }
 
-// One product, T x T tiles, a workgroup of 2 x 2 waves per tile; 64 contracted channels a stage in
-// two LDS slots, hi and lo of both operands (T = 128: 64 KB a slot, one workgroup per CU; T = 64: 32
-// KB, two).  Result element (i, j): j along the registers, i along the lanes, so that four neighbours
-// of a row are stored at once.
+// One product, T x T tiles, a workgroup of 2 x 2 waves per tile.  A stage contracts 32 channels: T rows
+// of 128 bytes, hi and lo, of the operand along the lanes and as much of the other one (kStep: 32 rows
+// of T columns, read transposed); T = 128 two LDS slots of 32 KB, T = 64 four of 16 KB, loaded
+// one and three stages ahead: two workgroups per CU, so that one's first loads and its
+// epilogue run beside the other's products (one workgroup with 64 channels a stage: 24 x 512 x
+// 2048, kStep 174 us).  Result element (i, j): j along the registers, i along the lanes, so that four
+// neighbours of a row are stored at once.
 //   kGram: A = X X^T;  kPoly: B = b A + c A A^T;  kStep: Y = a X + B X;  kLast: that, to G's type
 template <int T, int OP>
-__global__ __launch_bounds__(256, T == 128 ? 1 : 2) void ortho_product_kernel(OrthoArgs a,
-                                                                              int dtype, int work) {
+__global__ __launch_bounds__(256, T == 128 && OP < kStep ? 1 : 2) void ortho_product_kernel(
+    OrthoArgs a, int dtype, int work) {
   constexpr bool STEP = OP >= kStep;
-  constexpr int NT = T / 64;  // 64-row units of an operand; 32 x 32 tiles of a wave: NT x NT
-  __shared__ __align__(16) unsigned char lds[2][4 * NT][kTileB];
+  constexpr int NT = T / 64;      // 32 x 32 tiles of a wave: NT x NT
+  constexpr int NU = T / 32;      // 32-row units (4 KB) of an operand's stage
+  constexpr int kUnit = 32 * kRowB;
+  constexpr bool DEEP = T == 64 || !STEP;  // four slots
+  __shared__ __align__(16) unsigned char s0[2 * NU * kUnit], s1[2 * NU * kUnit];
+  __shared__ __align__(16) unsigned char s2[DEEP ? 2 * NU * kUnit : 16];
+  __shared__ __align__(16) unsigned char s3[DEEP ? 2 * NU * kUnit : 16];
   // neighbouring tiles of a matrix on one XCD
   const int per = (work + 7) / 8, item = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
   if (item >= work) return;
@@ -170,31 +218,25 @@ __global__ __launch_bounds__(256, T == 128 ? 1 : 2) void ortho_product_kernel(Or
   const LaneOff lo(l);
   const ColOff co(l);
 
-  const int64_t px = (int64_t)a.rp * a.mp, pa = (int64_t)a.rp * a.rp;
-  const uint16_t* X = a.x + mat * 2 * px;
-  const uint16_t* A = a.A + mat * 2 * pa;
-  const uint16_t* B = a.B + mat * 2 * pa;
-  const uint16_t* P = OP == kGram ? X : OP == kPoly ? A : B;  // rows i
-  const int ldp = (OP == kGram ? a.mp : a.rp) * 2;
-  const int64_t pp = OP == kGram ? px : pa;
+  const int64_t px = (int64_t)2 * a.rp * a.mp, pa = (int64_t)2 * a.rp * a.rp;
+  const uint16_t* X = a.x + mat * px;
+  const uint16_t* A = a.A + mat * pa;
+  const uint16_t* P = OP == kGram ? X : OP == kPoly ? A : a.B + mat * pa;  // rows i
+  const int ldp = (OP == kGram ? a.mp : a.rp) * 4, ldx = a.mp * 4;         // bytes
   const int K = OP == kGram ? a.mp : a.rp;
 
-  auto load = [&](int k0, unsigned char (*s)[kTileB]) __attribute__((always_inline)) {
+  // unit u of a stage: rows 32 u .. of the operand along the lanes, then the other one's; wave w loads
+  // rows 8 w .. of each (rows and columns past the matrix: zeros)
+  auto load = [&](int k0, unsigned char* s) __attribute__((always_inline)) {
 #pragma unroll
-    for (int pl = 0; pl < 2; ++pl)
-#pragma unroll
-      for (int u = 0; u < NT; ++u) {
-        const int i = it * T + 64 * u, j = jt * T + 64 * u;
-        const auto ri = rows_rsrc(P + pl * pp + k0, i, k0 < K ? a.rp - i : 0, ldp);
-        const auto rj = STEP ? rows_rsrc(X + pl * px + j, k0, j < a.mp ? K - k0 : 0, 2 * a.mp)
-                             : rows_rsrc(P + pl * pp + k0, j, k0 < K ? a.rp - j : 0, ldp);
-        const int ldj = STEP ? 2 * a.mp : ldp;
-#pragma unroll
-        for (int q = 0; q < 2; ++q) {
-          dma_rows8(ri, s[pl * NT + u], 2 * w + q, ldp, l);
-          dma_rows8(rj, s[2 * NT + pl * NT + u], 2 * w + q, ldj, l);
-        }
-      }
+    for (int u = 0; u < NU; ++u) {
+      const int i = it * T + 32 * u, j = jt * T + 32 * u;
+      const auto ri = rows_rsrc(P + 2 * k0, i, k0 < K && i < a.rp ? 32 : 0, ldp);
+      const auto rj = STEP ? rows_rsrc(X + 2 * j, k0, k0 < K && j < a.mp ? 32 : 0, ldx)
+                           : rows_rsrc(P + 2 * k0, j, k0 < K && j < a.rp ? 32 : 0, ldp);
+      dma_rows8(ri, s + u * kUnit, w, ldp, l);
+      dma_rows8(rj, s + (NU + u) * kUnit, w, STEP ? ldx : ldp, l);
+    }
   };
 
   f32x16 acc[NT][NT], low[NT][NT];  // hi hi, and the two cross products
@@ -202,19 +244,18 @@ __global__ __launch_bounds__(256, T == 128 ? 1 : 2) void ortho_product_kernel(Or
   for (int x = 0; x < NT; ++x)
 #pragma unroll
     for (int y = 0; y < NT; ++y) acc[x][y] = low[x][y] = zero16();
-  const int ui = T == 128 ? wi : 0, uj = T == 128 ? wj : 0;  // this wave's units
-  auto compute = [&](const unsigned char (*s)[kTileB]) __attribute__((always_inline)) {
+  auto compute = [&](const unsigned char* s) __attribute__((always_inline)) {
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
+    for (int k = 0; k < 2; ++k) {
       u32x4 fi[2][NT], fj[2][NT];
 #pragma unroll
       for (int pl = 0; pl < 2; ++pl)
 #pragma unroll
         for (int x = 0; x < NT; ++x) {
-          const int r0 = T == 128 ? 32 * x : 32 * wi, c0 = T == 128 ? x : wj;
-          fi[pl][x] = row_frag(s[pl * NT + ui], r0, k, lo);
-          fj[pl][x] = STEP ? turned_frag(s[2 * NT + pl * NT + uj], k, c0, co)
-                           : row_frag(s[2 * NT + pl * NT + uj], 32 * c0, k, lo);
+          const unsigned char* ui = s + (NT * wi + x) * kUnit;
+          const unsigned char* uj = s + (NU + NT * wj + x) * kUnit;
+          fi[pl][x] = row_frag(ui, 0, 2 * pl + k, lo);
+          fj[pl][x] = STEP ? turned_frag(uj, k, pl, co) : row_frag(uj, 0, 2 * pl + k, lo);
         }
 #pragma unroll
       for (int x = 0; x < NT; ++x)
@@ -230,17 +271,37 @@ __global__ __launch_bounds__(256, T == 128 ? 1 : 2) void ortho_product_kernel(Or
         for (int y = 0; y < NT; ++y) low[x][y] = mfma_32x32x16<F16>(fj[0][y], fi[1][x], low[x][y]);
     }
   };
-  load(0, lds[0]);
-  for (int k0 = 0; k0 < K; k0 += 128) {
-    __builtin_amdgcn_s_waitcnt(wait_vm_lgkm0(0));
-    __builtin_amdgcn_s_barrier();  // the stage has landed, the one before is read
-    load(k0 + 64, lds[1]);
-    compute(lds[0]);
-    if (k0 + 64 >= K) break;
-    __builtin_amdgcn_s_waitcnt(wait_vm_lgkm0(0));
-    __builtin_amdgcn_s_barrier();
-    load(k0 + 128, lds[0]);
-    compute(lds[1]);
+  // (K is a multiple of 64; a stage's loads: 2 NU per wave)
+  if (!DEEP) {
+    load(0, s0);
+    for (int k0 = 0; k0 < K; k0 += 64) {
+      __builtin_amdgcn_s_waitcnt(wait_vm_lgkm0(0));
+      __builtin_amdgcn_s_barrier();  // the stage has landed, the one before is read
+      load(k0 + 32, s1);
+      compute(s0);
+      __builtin_amdgcn_s_waitcnt(wait_vm_lgkm0(0));
+      __builtin_amdgcn_s_barrier();
+      load(k0 + 64, s0);
+      compute(s1);
+    }
+  } else {
+    auto stage = [&](int k0, const unsigned char* cur, unsigned char* to)
+        __attribute__((always_inline)) {
+      __builtin_amdgcn_s_waitcnt(wait_vm_lgkm0(4 * NU));
+      __builtin_amdgcn_s_barrier();
+      load(k0 + 96, to);
+      compute(cur);
+    };
+    load(0, s0);
+    load(32, s1);
+    load(64, s2);
+    for (int k0 = 0; k0 < K; k0 += 128) {
+      stage(k0, s0, s3);
+      stage(k0 + 32, s1, s0);
+      if (k0 + 64 >= K) break;
+      stage(k0 + 64, s2, s1);
+      stage(k0 + 96, s3, s2);
+    }
   }
   __builtin_amdgcn_s_waitcnt(wait_vm_lgkm0(0));  // no load into this LDS outlives the workgroup
 
@@ -260,46 +321,35 @@ __global__ __launch_bounds__(256, T == 128 ? 1 : 2) void ortho_product_kernel(Or
 #pragma unroll
           for (int e = 0; e < 4; ++e) v[e] *= 1.f / kScaleX;
         } else if (OP == kPoly) {
-          const uint16_t* s = A + (int64_t)i * a.rp + j;
+          const uint16_t* s = A + pair_index(i, j, a.rp);
           const u32x2 p = *reinterpret_cast<const u32x2*>(s);
-          const u32x2 q = *reinterpret_cast<const u32x2*>(s + pa);
+          const u32x2 q = *reinterpret_cast<const u32x2*>(s + 32);
 #pragma unroll
           for (int e = 0; e < 4; ++e)
             v[e] = a.c * (kScaleB / (kScaleX * kScaleX)) * v[e] +
                    a.b * (kScaleB / kScaleX) * pair_at(p[e >> 1], q[e >> 1], e & 1);
         } else {
-          const uint16_t* s = X + (int64_t)i * a.mp + j;
+          const uint16_t* s = X + pair_index(i, j, a.mp);
           const u32x2 p = *reinterpret_cast<const u32x2*>(s);
-          const u32x2 q = *reinterpret_cast<const u32x2*>(s + px);
+          const u32x2 q = *reinterpret_cast<const u32x2*>(s + 32);
 #pragma unroll
           for (int e = 0; e < 4; ++e)
             v[e] = (1.f / kScaleB) * v[e] + a.a * pair_at(p[e >> 1], q[e >> 1], e & 1);
         }
         if (OP == kLast) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            if (i >= a.r || j + e >= a.m) continue;
-            const float z = v[e] * (1.f / kScaleX);
-            const int64_t at = mat * a.count + (a.turn ? (int64_t)(j + e) * a.C + i
-                                                       : (int64_t)i * a.C + j + e);
-            if (dtype == 2)
-              static_cast<float*>(a.out)[at] = z;
-            else
-              static_cast<uint16_t*>(a.out)[at] =
-                  dtype == SLA2H_DTYPE_BF16 ? BF16::from_f32(z) : F16::from_f32(z);
-          }
+          for (int e = 0; e < 4; ++e) store_out(a, dtype, mat, i, j + e, v[e]);
           continue;
         }
         u32x2 hi, lw;
         split4(v, hi, lw);
-        uint16_t* base = OP == kGram ? a.A + mat * 2 * pa : OP == kPoly ? a.B + mat * 2 * pa
-                                                                        : a.y + mat * 2 * px;
+        uint16_t* base = OP == kGram ? a.A + mat * pa : OP == kPoly ? a.B + mat * pa
+                                                                    : a.y + mat * px;
         const int ld = STEP ? a.mp : a.rp;
-        const int64_t plane = STEP ? px : pa;
-        uint16_t* d = base + (int64_t)i * ld + j;
+        uint16_t* d = base + pair_index(i, j, ld);
         if (STEP || it != jt) {
           *reinterpret_cast<u32x2*>(d) = hi;
-          *reinterpret_cast<u32x2*>(d + plane) = lw;
+          *reinterpret_cast<u32x2*>(d + 32) = lw;
         }
         if (STEP) continue;
         // below the diagonal too (within a tile on it the elements above are the ones kept, so
@@ -309,15 +359,170 @@ __global__ __launch_bounds__(256, T == 128 ? 1 : 2) void ortho_product_kernel(Or
           if (it == jt && j + e < i) continue;
           const uint16_t x0 = (uint16_t)(hi[e >> 1] >> (16 * (e & 1)));
           const uint16_t x1 = (uint16_t)(lw[e >> 1] >> (16 * (e & 1)));
-          uint16_t* d2 = base + (int64_t)(j + e) * ld + i;
+          uint16_t* d2 = base + pair_index(j + e, i, ld);
           d2[0] = x0;
-          d2[plane] = x1;
+          d2[32] = x1;
           if (it == jt) {
             d[e] = x0;
-            d[e + plane] = x1;
+            d[e + 32] = x1;
           }
         }
       }
+}
+
+// Small matrices (r <= 64, m <= 512): all steps of a matrix in one workgroup, X (at most 128 KB) and A,
+// then b A + c A^2 in its place, in LDS as pairs, in tiles of 64 rows x 32 columns, hi and lo.  (A chain of
+// launches waits for first loads, not for products: 64 x 128, five steps, 90 us in fifteen launches.)
+// A and its square: waves 0 .. 3 a 32 x 32 tile each, for A beside waves 4 .. 7 that take every second
+// block of columns; X: a wave takes whole blocks of columns, and replaces them.
+constexpr int kSmallM = 512;
+struct NsTable {
+  float v[3 * 64];
+};
+__global__ __launch_bounds__(512, 2) void ortho_small_kernel(OrthoArgs a, int dtype, int steps,
+                                                             NsTable table) {
+  __shared__ __align__(16) unsigned char xs[kSmallM / 32][kTileB], as[2][kTileB];
+  __shared__ double red[8];
+  const int64_t mat = blockIdx.x;
+  const int tid = threadIdx.x, l = tid & 63, h = l >> 5;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6), grp = w >> 2, wi = (w >> 1) & 1, wj = w & 1;
+  const LaneOff lo(l);
+  const ColOff co(l);
+  const int nb = a.mp / 32;  // blocks of columns
+  // four neighbours of row i: the halves' places in a tile
+  auto place = [&](int i, int j) __attribute__((always_inline)) {
+    return chunk_addr(i, (j & 31) >> 3) + 2 * (j & 7);
+  };
+  auto put = [&](unsigned char* tile, int i, int j, const float (&v)[4])
+      __attribute__((always_inline)) {
+    u32x2 hi, lw;
+    split4(v, hi, lw);
+    const int at = place(i, j);
+    *reinterpret_cast<u32x2*>(tile + at) = hi;
+    *reinterpret_cast<u32x2*>(tile + (at ^ 64)) = lw;  // four chunks further
+  };
+
+  double s = 0.0;
+#pragma unroll 4
+  for (int i = tid; i < (int)a.count; i += 512) {
+    const double v = load_g(a, dtype, mat * a.count + i);
+    s += v * v;
+  }
+  s = wave_sum(s);
+  if (l == 0) red[w] = s;
+  __syncthreads();
+  s = ((red[0] + red[1]) + (red[2] + red[3])) + ((red[4] + red[5]) + (red[6] + red[7]));
+  const double inv = s == 0.0 ? 0.0 : (double)kScaleX / sqrt(s);
+  for (int k = tid; k < 64 * 8 * nb; k += 512) {  // neighbouring threads read neighbours in G
+    const int i = a.turn ? k & 63 : k / (8 * nb), j = 4 * (a.turn ? k >> 6 : k % (8 * nb));
+    float v[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int64_t at = mat * a.count + (a.turn ? (int64_t)(j + e) * a.C + i : (int64_t)i * a.C + j + e);
+      v[e] = i < a.r && j + e < a.m ? (float)((double)load_g(a, dtype, at) * inv) : 0.f;
+    }
+    put(xs[j >> 5], i, j, v);
+  }
+  __syncthreads();
+
+  for (int step = 0; step < steps; ++step) {
+    const float ca = table.v[3 * step], cb = table.v[3 * step + 1], cc = table.v[3 * step + 2];
+    f32x16 acc = zero16(), low = zero16();
+    // rows 32 wj and 32 wi of a block of 32 contracted columns
+    auto block = [&](const unsigned char* tile) __attribute__((always_inline)) {
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const u32x4 ih = row_frag(tile, 32 * wi, k, lo), il = row_frag(tile, 32 * wi, 2 + k, lo);
+        const u32x4 jh = row_frag(tile, 32 * wj, k, lo), jl = row_frag(tile, 32 * wj, 2 + k, lo);
+        low = mfma_32x32x16<F16>(jl, ih, low);
+        acc = mfma_32x32x16<F16>(jh, ih, acc);
+        low = mfma_32x32x16<F16>(jh, il, low);
+      }
+    };
+    for (int c = grp; c < nb; c += 2) block(xs[c]);
+    f32x4* join = reinterpret_cast<f32x4*>(as[0]) + (w & 3) * 256 + l;
+    if (grp) {
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+        join[64 * g] = f32x4{acc[4 * g] + low[4 * g], acc[4 * g + 1] + low[4 * g + 1],
+                             acc[4 * g + 2] + low[4 * g + 2], acc[4 * g + 3] + low[4 * g + 3]};
+    }
+    __syncthreads();
+    float A[16];
+    if (!grp) {
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const f32x4 z = join[64 * g];
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          A[4 * g + e] = (acc[4 * g + e] + low[4 * g + e] + z[e]) * (1.f / kScaleX);
+      }
+    }
+    __syncthreads();
+    const int row = 32 * wi + (l & 31);
+    if (!grp) {
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const float v[4] = {A[4 * g], A[4 * g + 1], A[4 * g + 2], A[4 * g + 3]};
+        put(as[wj], row, 8 * g + 4 * h, v);
+      }
+    }
+    __syncthreads();
+    if (!grp) {
+      acc = low = zero16();
+      block(as[0]);
+      block(as[1]);
+    }
+    __syncthreads();
+    if (!grp) {
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        float v[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          v[e] = cc * (kScaleB / (kScaleX * kScaleX)) * (acc[4 * g + e] + low[4 * g + e]) +
+                 cb * (kScaleB / kScaleX) * A[4 * g + e];
+        put(as[wj], row, 8 * g + 4 * h, v);
+      }
+    }
+    __syncthreads();
+    for (int c = w; c < nb; c += 8) {
+      f32x16 y[2], z[2];
+      y[0] = y[1] = z[0] = z[1] = zero16();
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const u32x4 jh = turned_frag(xs[c], k, 0, co), jl = turned_frag(xs[c], k, 1, co);
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          const u32x4 ih = row_frag(as[k >> 1], 32 * x, k & 1, lo);
+          const u32x4 il = row_frag(as[k >> 1], 32 * x, 2 + (k & 1), lo);
+          z[x] = mfma_32x32x16<F16>(jl, ih, z[x]);
+          y[x] = mfma_32x32x16<F16>(jh, ih, y[x]);
+          z[x] = mfma_32x32x16<F16>(jh, il, z[x]);
+        }
+      }
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const int i = 32 * x + (l & 31), jj = 8 * g + 4 * h, at = place(i, jj);
+          const u32x2 p = *reinterpret_cast<const u32x2*>(xs[c] + at);
+          const u32x2 q = *reinterpret_cast<const u32x2*>(xs[c] + (at ^ 64));
+          float v[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            v[e] = (1.f / kScaleB) * (y[x][4 * g + e] + z[x][4 * g + e]) +
+                   ca * pair_at(p[e >> 1], q[e >> 1], e & 1);
+          if (step + 1 < steps) {
+            put(xs[c], i, jj, v);
+            continue;
+          }
+#pragma unroll
+          for (int e = 0; e < 4; ++e) store_out(a, dtype, mat, i, 32 * c + jj + e, v[e]);
+        }
+    }
+    __syncthreads();
+  }
 }
 
 struct OrthoPlan {
@@ -387,7 +592,15 @@ extern "C" int sla2h_orthogonalize(const void* g, int dtype, int64_t n, int64_t 
   a.turn = R > C;
   hipStream_t st = static_cast<hipStream_t>(stream);
   int err;
-  ortho_norm_kernel<<<(unsigned)(n * p.parts), 256, 0, st>>>(a, dtype);
+  if (p.r <= 64 && p.m <= kSmallM) {
+    NsTable t{};
+    for (int i = 0; i < 3 * steps; ++i) t.v[i] = coeffs[i];
+    ortho_small_kernel<<<(unsigned)n, 512, 0, st>>>(a, dtype, steps, t);
+    return (int)hipGetLastError();
+  }
+  const int size = dtype == 2 ? 4 : 2;
+  ortho_norm_kernel<<<(unsigned)(n * p.parts), 256, 0, st>>>(
+      a, dtype, reinterpret_cast<uintptr_t>(g) % 16 == 0 && a.count * size % 16 == 0);
   if ((err = (int)hipGetLastError())) return err;
   ortho_split_kernel<<<(unsigned)(n * (p.rp / 64) * (p.mp / 64)), 256, 0, st>>>(a, dtype);
   if ((err = (int)hipGetLastError())) return err;
