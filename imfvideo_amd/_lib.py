@@ -175,13 +175,14 @@ SIGNATURES = {
     "sla2h_orthogonalize": (_c_int, [_p, _c_int, _c_i64, _c_i64, _c_i64, _c_int, _p, _p, _p, _p]),
     "sla2h_diff_attn_fwd_workspace_bytes": (ctypes.c_size_t, [_c_int, _c_int, _c_int, _c_i64,
                                                               _c_i64]),
-    "sla2h_diff_attn_fwd": (_c_int, [_p, _p, _p, _p, _p, _p, _p, _c_int, _c_int, _c_int, _c_int,
-                                     _c_i64, _c_i64, _c_int, _c_f, _p, _p, _p, _p, _p]),
+    "sla2h_diff_attn_fwd": (_c_int, [_p, _p, _p, _p, _c_int, _c_i64, _p, _p, _p, _c_int, _c_int,
+                                     _c_int, _c_int, _c_i64, _c_i64, _c_int, _c_f, _p, _p, _p, _p,
+                                     _p]),
     "sla2h_diff_attn_bwd_workspace_bytes": (ctypes.c_size_t, [_c_int, _c_int, _c_int, _c_int,
                                                               _c_i64, _c_i64]),
-    "sla2h_diff_attn_bwd": (_c_int, [_p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _c_int, _c_int,
-                                     _c_int, _c_int, _c_i64, _c_i64, _c_int, _c_f, _p, _p, _p, _p,
-                                     _p, _p]),
+    "sla2h_diff_attn_bwd": (_c_int, [_p, _p, _p, _p, _c_int, _c_i64, _p, _p, _p, _p, _p, _p, _c_int,
+                                     _c_int, _c_int, _c_int, _c_i64, _c_i64, _c_int, _c_f, _p, _p,
+                                     _p, _p, _p, _p]),
 }
 
 _LIB = None

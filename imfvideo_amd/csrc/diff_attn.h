@@ -19,6 +19,22 @@ __device__ inline void load_unit(const uint16_t* base, int64_t row0, int64_t n, 
   for (int j = 0; j < 4; ++j) dma_rows8(rs, unit, j, (int)ld, l);
 }
 
+// The pairs' weights of the second map: fp16, bf16 or fp32 (2), `stride` elements apart (0: one for all).
+struct Weights {
+  const void* p;
+  int dtype;
+  int64_t stride;
+  __device__ float operator[](int64_t i) const {
+    if (dtype == 2) return static_cast<const float*>(p)[i * stride];
+    const uint16_t v = static_cast<const uint16_t*>(p)[i * stride];
+    return dtype == SLA2H_DTYPE_BF16 ? BF16::to_f32(v) : F16::to_f32(v);
+  }
+  bool ok() const {
+    return p && dtype >= 0 && dtype <= 2 && stride >= 0 &&
+           reinterpret_cast<uintptr_t>(p) % (dtype == 2 ? 4 : 2) == 0;
+  }
+};
+
 inline bool diff_sizes_ok(int B, int H, int Hkv, int64_t Lq, int64_t Lk) {
   return sizes_ok(B, H, Hkv, Lq, Lk) && H % 2 == 0 && Hkv % 2 == 0;
 }

@@ -22,7 +22,7 @@ namespace {
 
 struct DiffFwdArgs {
   const uint16_t *q, *k, *v;
-  const float* lam;  // (P)
+  Weights lam;       // (P)
   uint16_t* o;       // (B, Lq, H, 64)
   float* maps;       // (B, Lq, P, 2, 128): A_m v, or null
   float* lse;        // (B, H, Lq) or null
@@ -595,19 +595,20 @@ extern "C" size_t sla2h_diff_attn_fwd_workspace_bytes(int B, int H, int Hkv, int
   return p.splits > 1 ? (size_t)p.splits * B * H * Lq * (128 * 4 + 8) : 0;
 }
 
-extern "C" int sla2h_diff_attn_fwd(const void* q, const void* k, const void* v, const float* lam,
-                                   const int64_t* strides, const int32_t* q_lens,
+extern "C" int sla2h_diff_attn_fwd(const void* q, const void* k, const void* v, const void* lam,
+                                   int lam_dtype, int64_t lam_stride, const int64_t* strides, const int32_t* q_lens,
                                    const int32_t* k_lens, int dtype, int B, int H, int Hkv,
                                    int64_t Lq, int64_t Lk, int causal, float scale,
                                    void* workspace, void* o, float* lse, float* maps,
                                    void* stream) {
-  SLA2H_CHECK_ARG(q && k && v && lam && strides && o && !lse == !maps);
+  const Weights wts{lam, lam_dtype, lam_stride};
+  SLA2H_CHECK_ARG(q && k && v && wts.ok() && strides && o && !lse == !maps);
   SLA2H_CHECK_ARG(dtype == SLA2H_DTYPE_F16 || dtype == SLA2H_DTYPE_BF16);
   SLA2H_CHECK_ARG(diff_sizes_ok(B, H, Hkv, Lq, Lk));
   SLA2H_CHECK_ARG(scale > 0.f && scale < 1e30f);
   SLA2H_CHECK_ARG(((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)o | (uintptr_t)maps |
                    (uintptr_t)workspace) % 16 == 0);
-  SLA2H_CHECK_ARG(((uintptr_t)lam | (uintptr_t)lse | (uintptr_t)q_lens | (uintptr_t)k_lens) % 4 == 0);
+  SLA2H_CHECK_ARG(((uintptr_t)lse | (uintptr_t)q_lens | (uintptr_t)k_lens) % 4 == 0);
   for (int i = 0; i < 9; ++i) SLA2H_CHECK_ARG(strides[i] >= 0 && strides[i] % 8 == 0);
   // rows apart from each other: the range check of a tile's load tells them by their offset
   for (int i : {2, 5, 8}) SLA2H_CHECK_ARG(strides[i] >= kDD);
@@ -623,7 +624,7 @@ extern "C" int sla2h_diff_attn_fwd(const void* q, const void* k, const void* v, 
   a.q = static_cast<const uint16_t*>(q);
   a.k = static_cast<const uint16_t*>(k);
   a.v = static_cast<const uint16_t*>(v);
-  a.lam = lam;
+  a.lam = wts;
   a.o = static_cast<uint16_t*>(o);
   a.maps = maps;
   a.lse = lse;

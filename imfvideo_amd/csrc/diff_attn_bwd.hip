@@ -44,9 +44,11 @@ constexpr int kNormRows = 64;  // rows of a partial maximum of the norms and of 
 
 struct DiffBwdArgs {
   const uint16_t *q, *k, *v, *dout;
-  const float *lam, *lse, *maps;
+  Weights weights;   // (P)
+  float* lam;        // (P): the same in fp32, from the first launch
+  const float *lse, *maps;
   uint16_t *dq, *dk, *dv;
-  float* dlam;
+  void* dlam;        // (P), the weights' type
   const int32_t *q_lens, *k_lens;
   int64_t qb, qh, ql, kb, kh, kl, vb, vh, vl;
   int64_t Lq, Lk;
@@ -81,7 +83,7 @@ __device__ inline int exponent(float x) {
 __device__ inline float top_weight(const DiffBwdArgs& a, int kp) {
   float ml = 0.f;
   for (int i = threadIdx.x & 63; i < a.rep; i += 64)
-    ml = fmaxf(ml, __builtin_fabsf(a.lam[kp * a.rep + i]));
+    ml = fmaxf(ml, __builtin_fabsf(a.weights[kp * a.rep + i]));
   return wave_max(ml);
 }
 __device__ inline int weight_shift(float ml) {
@@ -103,6 +105,8 @@ __global__ __launch_bounds__(256) void diff_bwd_prep_kernel(DiffBwdArgs a, int64
   const int qlen = seq_len(a.q_lens, b, a.Lq), klen = seq_len(a.k_lens, b, a.Lk);
   const int len = is_v ? klen : qlen;
   const int first = is_v ? 0 : first_query(qlen, klen, a.causal);
+  if (blockIdx.x == 0)
+    for (int i = tid; i < a.P; i += 256) a.lam[i] = a.weights[i];
   float top = 0.f, sum = 0.f;
   const float shift = Scaled<T16>::value && !is_v ? (float)weight_shift(top_weight(a, p / a.rep)) : 0.f;
 #pragma unroll
@@ -230,7 +234,12 @@ __global__ __launch_bounds__(256, 2) void diff_bwd_dq_kernel(DiffBwdArgs a) {
       if (tid < x) red[tid] += red[tid + x];
       __syncthreads();
     }
-    if (tid == 0) a.dlam[p] = red[0];
+    if (tid) return;
+    if (a.weights.dtype == 2)
+      static_cast<float*>(a.dlam)[p] = red[0];
+    else
+      static_cast<uint16_t*>(a.dlam)[p] =
+          a.weights.dtype == SLA2H_DTYPE_BF16 ? BF16::from_f32(red[0]) : F16::from_f32(red[0]);
     return;
   }
   int bp, item;
@@ -607,7 +616,7 @@ BwdPlan bwd_plan(int dtype, int B, int H, int Hkv, int64_t Lq, int64_t Lk, bool 
   p.nqb = (Lq + kNormRows - 1) / kNormRows;
   p.nkb = (Lk + kNormRows - 1) / kNormRows;
   p.stats = 4 * bp * Lq + bp * p.nqb + (dtype == SLA2H_DTYPE_F16 ? bp * p.nqb + bk * p.nkb : 0);
-  p.stats = (p.stats + 3) & ~(size_t)3;
+  p.stats = ((p.stats + 3) & ~(size_t)3) + ((H / 2 + 3) & ~3);  // ... and the weights
   p.dq_parts = p.dq_splits > 1 ? (size_t)p.dq_splits * bp * Lq * 128 : 0;
   p.kv_parts = p.kv_splits > 1 ? (size_t)p.kv_splits * bk * Lk * 128 : 0;
   return p;
@@ -631,22 +640,24 @@ extern "C" size_t sla2h_diff_attn_bwd_workspace_bytes(int dtype, int B, int H, i
   return most * 4;
 }
 
-extern "C" int sla2h_diff_attn_bwd(const void* q, const void* k, const void* v, const float* lam,
-                                   const void* dout, const float* lse, const float* maps,
+extern "C" int sla2h_diff_attn_bwd(const void* q, const void* k, const void* v, const void* lam,
+                                   int lam_dtype, int64_t lam_stride, const void* dout,
+                                   const float* lse, const float* maps,
                                    const int64_t* strides, const int32_t* q_lens,
                                    const int32_t* k_lens, int dtype, int B, int H, int Hkv,
                                    int64_t Lq, int64_t Lk, int causal, float scale,
-                                   void* workspace, void* dq, void* dk, void* dv, float* dlam,
+                                   void* workspace, void* dq, void* dk, void* dv, void* dlam,
                                    void* stream) {
-  SLA2H_CHECK_ARG(q && k && v && lam && dout && lse && maps && strides && workspace && dlam);
+  const Weights wts{lam, lam_dtype, lam_stride};
+  SLA2H_CHECK_ARG(q && k && v && wts.ok() && dout && lse && maps && strides && workspace && dlam);
   SLA2H_CHECK_ARG(!dk == !dv);
   SLA2H_CHECK_ARG(dtype == SLA2H_DTYPE_F16 || dtype == SLA2H_DTYPE_BF16);
   SLA2H_CHECK_ARG(diff_sizes_ok(B, H, Hkv, Lq, Lk));
   SLA2H_CHECK_ARG(scale > 0.f && scale < 1e30f);
   SLA2H_CHECK_ARG(((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)dout | (uintptr_t)maps |
                    (uintptr_t)workspace | (uintptr_t)dq | (uintptr_t)dk | (uintptr_t)dv) % 16 == 0);
-  SLA2H_CHECK_ARG(((uintptr_t)lam | (uintptr_t)lse | (uintptr_t)dlam | (uintptr_t)q_lens |
-                   (uintptr_t)k_lens) % 4 == 0);
+  SLA2H_CHECK_ARG(((uintptr_t)lse | (uintptr_t)q_lens | (uintptr_t)k_lens) % 4 == 0 &&
+                  (uintptr_t)dlam % (lam_dtype == 2 ? 4 : 2) == 0);
   for (int i = 0; i < 9; ++i) SLA2H_CHECK_ARG(strides[i] >= 0 && strides[i] % 8 == 0);
   // rows apart from each other: the range check of a tile's load tells them by their offset; 32-bit
   // byte offsets within a tile
@@ -663,7 +674,7 @@ extern "C" int sla2h_diff_attn_bwd(const void* q, const void* k, const void* v, 
   a.k = static_cast<const uint16_t*>(k);
   a.v = static_cast<const uint16_t*>(v);
   a.dout = static_cast<const uint16_t*>(dout);
-  a.lam = lam, a.lse = lse, a.maps = maps;
+  a.weights = wts, a.lse = lse, a.maps = maps;
   a.dq = static_cast<uint16_t*>(dq);
   a.dk = static_cast<uint16_t*>(dk);
   a.dv = static_cast<uint16_t*>(dv);
@@ -688,6 +699,7 @@ extern "C" int sla2h_diff_attn_bwd(const void* q, const void* k, const void* v, 
   a.lsum = a.stat + 4 * a.nrows;
   a.gmax = a.lsum + bp * p.nqb;
   a.vmax = a.gmax + bp * p.nqb;
+  a.lam = a.stat + p.stats - ((a.P + 3) & ~3);
   a.nqb = (int)p.nqb;
   a.nkb = (int)p.nkb;
   a.dq_part = a.stat + p.stats;

@@ -210,7 +210,8 @@ class _DiffAttentionFunction(torch.autograd.Function):
         nq, nk, nv = ctx.needs_input_grad[:3]
         *grads, dlam = ops.diff_attn_bwd(do, q, k, v, lam, lse, maps, causal, q_lens, k_lens, scale,
                                          nq, nk or nv)
-        return (*grads, dlam.to(lam.dtype), None, None, None, None)
+        return (*grads, dlam if dlam.dtype == lam.dtype else dlam.to(lam.dtype), None, None, None,
+                None)
 
 
 def diff_attention(q, k, v, lam, causal=False, q_lens=None, k_lens=None, scale=None):
@@ -870,7 +871,7 @@ class _ResidualNormFunction(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, a, scale, post, pre, gate, eps, consumers):
-        y, n = ops.residual_norm_fwd(x, a, scale, post, pre, gate, eps)
+        y, n = ops._residual_norm_fwd(x, a, scale, post, pre, gate, eps)
         ctx.eps = eps
         ctx.save_for_backward(y, a, scale, post, pre, gate)
         ctx.set_materialize_grads(False)
@@ -884,8 +885,8 @@ class _ResidualNormFunction(torch.autograd.Function):
         if dy is None and not dns:
             return (None,) * 8
         _no_batched(dy if dy is not None else dns[0], "residual_norm")
-        dx, da, dscale, dpost, dpre, dgate = ops.residual_norm_bwd(dy, dns, y, a, scale, post, pre,
-                                                                   gate, ctx.eps)
+        dx, da, dscale, dpost, dpre, dgate = ops._residual_norm_bwd(dy, dns, y, a, scale, post, pre,
+                                                                    gate, ctx.eps)
         if dpre is None and pre is not None:
             dpre = torch.zeros_like(pre)
         return dx, da, dscale, dpost, dpre, dgate, None, None
@@ -906,19 +907,20 @@ def residual_norm(x, a, scale, post_weight, gate=None, pre_weight=None, eps=1e-6
     (CPU tensors, other dtypes, transforms) runs the eager expression."""
     if not 1 <= consumers <= 3:
         raise ValueError(f"residual_norm: 1 to 3 consumers, got {consumers}")
-    given = [t for t in (x, a, scale, post_weight, gate, pre_weight) if t is not None]
     if gate is not None and (x.dim() < 2 or tuple(gate.shape) != (x.shape[0], x.shape[-1])):
         raise ValueError(f"residual_norm: expected a gate of {x.shape[0]} rows of {x.shape[-1]}, "
                          f"got {tuple(gate.shape)}")
-    if (all(t.is_cuda and t.is_floating_point() for t in given) and x.dtype == torch.float32
-            and a.dtype in (torch.float16, torch.bfloat16, torch.float32) and a.shape == x.shape
-            and x.numel() and x.shape[-1] <= ops.RESIDUAL_NORM_MAX
-            and all(tuple(v.shape) == (x.shape[-1],) for v in (scale, post_weight))
-            and (pre_weight is None or tuple(pre_weight.shape) == (x.shape[-1],))
-            and all(t.device == x.device for t in given) and ops.plain_eager(*given)):
-        scale, post, pre, g = (None if t is None else t.float()
-                               for t in (scale, post_weight, pre_weight, gate))
-        return _ResidualNormFunction.apply(x, a, scale, post, pre, g, float(eps), consumers)
+    if x.is_cuda:
+        vecs = (scale, post_weight) if pre_weight is None else (scale, post_weight, pre_weight)
+        vecs = [v.float() if v.is_floating_point() else v for v in vecs]
+        g = gate.float() if gate is not None and gate.is_floating_point() else gate
+        given = (x, a, *vecs) if g is None else (x, a, *vecs, g)
+        if ops.residual_norm_ok(x, a, vecs, g) and ops.plain_eager(*given):
+            pre = None if pre_weight is None else vecs[2]
+            if torch.is_grad_enabled() and any(t.requires_grad for t in given):
+                return _ResidualNormFunction.apply(x, a, *vecs[:2], pre, g, float(eps), consumers)
+            y, n = ops._residual_norm_fwd(x, a, *vecs[:2], pre, g, float(eps))
+            return (y,) if n is None else (y,) + (n,) * consumers
     wide = torch.promote_types(x.dtype, torch.float32)
     norm = lambda t, w: t * torch.rsqrt(t.pow(2).mean(dim=-1, keepdim=True) + eps) * w
     step = scale * norm(a.to(wide), post_weight)

@@ -1906,11 +1906,22 @@ def _residual_norm_check(x, a, vectors, gate):
         raise ValueError("residual_norm: operands on different devices")
 
 
-def residual_norm_fwd(x, a, scale, post, pre=None, gate=None, eps=1e-6):
-    """(y, n): y = x + scale * post * gate * a / rms(a) in fp32 and n = pre * y / rms(y) in
-    a's dtype (None without pre).  x (..., D) fp32, a (..., D) 16-bit or fp32, scale, post, pre
-    (D,) and gate (x.shape[0], D) fp32."""
-    _residual_norm_check(x, a, [v for v in (scale, post, pre) if v is not None], gate)
+def residual_norm_ok(x, a, vectors, gate):
+    """The kernels take these operands (what residual_norm_fwd asks of them)."""
+    D = (x.shape[-1],) if x.dim() else (0,)
+    f32, dev = torch.float32, x.device
+    if not (x.is_cuda and x.dtype == f32 and a.dtype in _NORM_DTYPES and a.shape == x.shape
+            and a.device == dev and x.numel() and D[0] <= RESIDUAL_NORM_MAX):
+        return False
+    for v in vectors:
+        if v.shape != D or v.dtype != f32 or v.device != dev:
+            return False
+    return gate is None or (x.dim() >= 2 and gate.shape == (x.shape[0], *D) and gate.dtype == f32
+                            and gate.device == dev)
+
+
+def _residual_norm_fwd(x, a, scale, post, pre, gate, eps):
+    """residual_norm_fwd of operands that residual_norm_ok takes."""
     x, a, scale, post = x.contiguous(), a.contiguous(), scale.contiguous(), post.contiguous()
     pre = None if pre is None else pre.contiguous()
     gate = None if gate is None else gate.contiguous()
@@ -1918,21 +1929,20 @@ def residual_norm_fwd(x, a, scale, post, pre=None, gate=None, eps=1e-6):
     n = None if pre is None else torch.empty_like(a)
     _launch(x.device, "sla2h_residual_norm_fwd", x.data_ptr(), a.data_ptr(), _NORM_DTYPES[a.dtype],
             scale.data_ptr(), post.data_ptr(), _ptr(pre), _ptr(gate),
-            *_residual_norm_sizes(x, gate), float(eps), y.data_ptr(), _ptr(n))
+            *_residual_norm_sizes(x, gate), eps, y.data_ptr(), _ptr(n))
     return y, n
 
 
-def residual_norm_bwd(dy, dns, y, a, scale, post, pre=None, gate=None, eps=1e-6):
-    """(dx, da, dscale, dpost, dpre, dgate) of residual_norm_fwd from its output y for the
-    gradient dy of y (or None) and the gradients dns of n (0 to 3 tensors of a's dtype, summed
-    in fp32); dpre is None without dns, dgate without gate."""
-    _residual_norm_check(y, a, [v for v in (scale, post, pre) if v is not None], gate)
-    if len(dns) > 3 or (dns and pre is None):
-        raise ValueError("residual_norm: up to three gradients of n, and none without pre")
-    for d, like in [(d, a) for d in dns] + ([] if dy is None else [(dy, y)]):
-        if d.shape != like.shape or d.dtype != like.dtype or d.device != like.device:
-            raise ValueError(f"residual_norm: a gradient like {tuple(like.shape)} {like.dtype} on "
-                             f"{like.device}, got {tuple(d.shape)} {d.dtype} on {d.device}")
+def residual_norm_fwd(x, a, scale, post, pre=None, gate=None, eps=1e-6):
+    """(y, n): y = x + scale * post * gate * a / rms(a) in fp32 and n = pre * y / rms(y) in
+    a's dtype (None without pre).  x (..., D) fp32, a (..., D) 16-bit or fp32, scale, post, pre
+    (D,) and gate (x.shape[0], D) fp32."""
+    _residual_norm_check(x, a, [v for v in (scale, post, pre) if v is not None], gate)
+    return _residual_norm_fwd(x, a, scale, post, pre, gate, float(eps))
+
+
+def _residual_norm_bwd(dy, dns, y, a, scale, post, pre, gate, eps):
+    """residual_norm_bwd of operands and gradients that it takes."""
     dy = None if dy is None else dy.contiguous()
     dns = [d.contiguous() for d in dns]
     y, a, scale, post = y.contiguous(), a.contiguous(), scale.contiguous(), post.contiguous()
@@ -1948,9 +1958,23 @@ def residual_norm_bwd(dy, dns, y, a, scale, post, pre=None, gate=None, eps=1e-6)
     dn = [d.data_ptr() for d in dns] + [None] * (3 - len(dns))
     _launch(y.device, "sla2h_residual_norm_bwd", y.data_ptr() if dns else None, a.data_ptr(),
             _NORM_DTYPES[a.dtype], scale.data_ptr(), post.data_ptr(), _ptr(pre), _ptr(gate),
-            _ptr(dy), *dn, *sizes, float(eps), dx.data_ptr(), da.data_ptr(), dscale.data_ptr(),
+            _ptr(dy), *dn, *sizes, eps, dx.data_ptr(), da.data_ptr(), dscale.data_ptr(),
             dpost.data_ptr(), _ptr(dpre), _ptr(dgate), ws.data_ptr())
     return dx, da, dscale, dpost, dpre, dgate
+
+
+def residual_norm_bwd(dy, dns, y, a, scale, post, pre=None, gate=None, eps=1e-6):
+    """(dx, da, dscale, dpost, dpre, dgate) of residual_norm_fwd from its output y for the
+    gradient dy of y (or None) and the gradients dns of n (0 to 3 tensors of a's dtype, summed
+    in fp32); dpre is None without dns, dgate without gate."""
+    _residual_norm_check(y, a, [v for v in (scale, post, pre) if v is not None], gate)
+    if len(dns) > 3 or (dns and pre is None):
+        raise ValueError("residual_norm: up to three gradients of n, and none without pre")
+    for d, like in [(d, a) for d in dns] + ([] if dy is None else [(dy, y)]):
+        if d.shape != like.shape or d.dtype != like.dtype or d.device != like.device:
+            raise ValueError(f"residual_norm: a gradient like {tuple(like.shape)} {like.dtype} on "
+                             f"{like.device}, got {tuple(d.shape)} {d.dtype} on {d.device}")
+    return _residual_norm_bwd(dy, dns, y, a, scale, post, pre, gate, float(eps))
 
 
 # ---------------------------------------------------------------------------
@@ -2044,7 +2068,7 @@ def _diff_plan(qs, qt, ks, kt, vs, vt, dtype):
 
 def _diff_operands(q, k, v, lam, scale):
     """Checks; returns q, k, v (copied where the kernels do not take their strides or
-    alignment), lam in fp32, their plan and the scale."""
+    alignment), lam (in fp32 where they do not take its type), their plan and the scale."""
     if not (q.is_cuda and k.is_cuda and v.is_cuda and lam.is_cuda):
         _need_gpu(q, k, v, lam)
     if not q.dtype == k.dtype == v.dtype or not q.device == k.device == v.device == lam.device:
@@ -2063,8 +2087,8 @@ def _diff_operands(q, k, v, lam, scale):
         plan = _diff_plan(q.shape, q.stride(), k.shape, k.stride(), v.shape, v.stride(), q.dtype)
         if any(plan.copy):
             raise _attn_too_large(q.shape, k.shape)
-    if lam.dtype != torch.float32 or not lam.is_contiguous():
-        lam = lam.to(torch.float32).contiguous()
+    if lam.dtype not in _NORM_DTYPES:
+        lam = lam.to(torch.float32)
     if scale is None:
         scale = E_TILE ** -0.5
     elif not 0.0 < scale < 1e30:
@@ -2096,14 +2120,15 @@ def diff_attn_fwd(q, k, v, lam, causal=False, q_lens=None, k_lens=None, scale=No
     else:
         ws = _scratch(p.fwd_ws, dev) if p.fwd_ws else None
         _launch(dev, "sla2h_diff_attn_fwd", q.data_ptr(), k.data_ptr(), v.data_ptr(),
-                lam.data_ptr(), p.strides, _ptr(q_lens), _ptr(k_lens), _HALF[q.dtype], *p.sizes,
-                1 if causal else 0, scale, _ptr(ws), o.data_ptr(), _ptr(lse), _ptr(maps))
+                lam.data_ptr(), _NORM_DTYPES[lam.dtype], lam.stride(0), p.strides, _ptr(q_lens),
+                _ptr(k_lens), _HALF[q.dtype], *p.sizes, 1 if causal else 0, scale, _ptr(ws),
+                o.data_ptr(), _ptr(lse), _ptr(maps))
     return o, lse, maps
 
 
 def diff_attn_bwd(do, q, k, v, lam, lse, maps, causal=False, q_lens=None, k_lens=None, scale=None,
                   need_q=True, need_kv=True):
-    """Gradients (dq, dk, dv, dlam fp32) of diff_attn_fwd for the output gradient do, from its
+    """Gradients (dq, dk, dv, dlam) of diff_attn_fwd for the output gradient do, from its
     operands and what it saved, the maps recomputed; dk and dv summed over the query
     pairs of a key pair, dlam over batch and rows.  Without need_q dq is None, without need_kv dk and dv."""
     q, k, v, lam, p, scale = _diff_operands(q, k, v, lam, scale)
@@ -2123,12 +2148,12 @@ def diff_attn_bwd(do, q, k, v, lam, lse, maps, causal=False, q_lens=None, k_lens
     dq = torch.empty(q.shape, device=dev, dtype=dtype) if need_q else None
     dk = torch.empty(k.shape, device=dev, dtype=dtype) if need_kv else None
     dv = torch.empty(v.shape, device=dev, dtype=dtype) if need_kv else None
-    dlam = torch.empty(lam.shape, device=dev, dtype=torch.float32)
+    dlam = torch.empty(lam.shape, device=dev, dtype=lam.dtype)
     if p.empty:
         return tuple(t if t is None else t.zero_() for t in (dq, dk, dv, dlam))
     ws = _scratch(p.bwd_ws, dev)
     _launch(dev, "sla2h_diff_attn_bwd", q.data_ptr(), k.data_ptr(), v.data_ptr(), lam.data_ptr(),
-            do.data_ptr(), lse.data_ptr(), maps.data_ptr(), p.strides, _ptr(q_lens), _ptr(k_lens),
-            _HALF[dtype], *p.sizes, 1 if causal else 0, scale, ws.data_ptr(), _ptr(dq), _ptr(dk),
-            _ptr(dv), dlam.data_ptr())
+            _NORM_DTYPES[lam.dtype], lam.stride(0), do.data_ptr(), lse.data_ptr(), maps.data_ptr(),
+            p.strides, _ptr(q_lens), _ptr(k_lens), _HALF[dtype], *p.sizes, 1 if causal else 0, scale,
+            ws.data_ptr(), _ptr(dq), _ptr(dk), _ptr(dv), dlam.data_ptr())
     return dq, dk, dv, dlam

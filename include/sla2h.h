@@ -972,18 +972,19 @@ int sla2h_orthogonalize(const void* g, int dtype, int64_t n, int64_t R, int64_t 
  *   o = (A_1 - lam_p A_2) v                      (the output heads 2p and 2p + 1)
  * q (B, H, Lq, 64), k, v (B, Hkv, Lk, 64) 16-bit of one dtype, unit channel stride, 16-byte aligned;
  * strides: host array of 9 int64, the (batch, head, row) strides of q, k, v in elements (multiples of
- * 8, rows at least 64 apart, those of k and v below 2^23).  lam (H / 2) fp32.  q_lens, k_lens: device
+ * 8, rows at least 64 apart, those of k and v below 2^23).  lam: H / 2 numbers of lam_dtype (0 fp16, 1 bf16,
+ * 2 fp32), lam_stride elements apart (0: one for all).  q_lens, k_lens: device
  * int32 (B) or NULL, clamped into [0, L].  o (B, Lq, H, 64) contiguous; rows behind q_len and rows
  * without a key are 0.  For the backward, both or neither: lse (B, H, Lq) fp32, each map's log-sum-exp
  * (-inf without a key), and maps (B, Lq, H / 2, 2, 128) fp32, A_1 v and A_2 v.  Workspace of
  * sla2h_diff_attn_fwd_workspace_bytes (0 for most calls).  Reproducible.
  */
 size_t sla2h_diff_attn_fwd_workspace_bytes(int B, int H, int Hkv, int64_t Lq, int64_t Lk);
-int sla2h_diff_attn_fwd(const void* q, const void* k, const void* v, const float* lam,
-                        const int64_t* strides, const int32_t* q_lens, const int32_t* k_lens,
-                        int dtype, int B, int H, int Hkv, int64_t Lq, int64_t Lk, int causal,
-                        float scale, void* workspace, void* o, float* lse, float* maps,
-                        void* stream);
+int sla2h_diff_attn_fwd(const void* q, const void* k, const void* v, const void* lam,
+                        int lam_dtype, int64_t lam_stride, const int64_t* strides,
+                        const int32_t* q_lens, const int32_t* k_lens, int dtype, int B, int H,
+                        int Hkv, int64_t Lq, int64_t Lk, int causal, float scale, void* workspace,
+                        void* o, float* lse, float* maps, void* stream);
 
 /*
  * Its backward, the maps recomputed from lse, with dA = dout v^T over the 128 channels and
@@ -992,18 +993,18 @@ int sla2h_diff_attn_fwd(const void* q, const void* k, const void* v, const float
  *   dk_m = scale dS_m^T q_m, dv = (A_1 - lam A_2)^T dout, dlam_p = -sum delta_2,
  * dk and dv summed over the query pairs of a key pair, dlam over rows and batch.  Operands, lens, sizes,
  * causal, scale, lse and maps as in the forward; dout (B, Lq, H, 64) contiguous.  dq (B, Lq, H,
- * 64), dk, dv (B, Lk, Hkv, 64) contiguous 16-bit, dlam (H / 2) fp32; dq, or dk and dv together, may
+ * 64), dk, dv (B, Lk, Hkv, 64) contiguous 16-bit, dlam (H / 2) of lam_dtype, contiguous; dq, or dk and dv together, may
  * be NULL (not computed).  Gradients of rows behind a sequence and of rows without a key are 0; dout is
  * not read there.  No atomics: reproducible bit for bit.
  */
 size_t sla2h_diff_attn_bwd_workspace_bytes(int dtype, int B, int H, int Hkv, int64_t Lq,
                                            int64_t Lk);
-int sla2h_diff_attn_bwd(const void* q, const void* k, const void* v, const float* lam,
-                        const void* dout, const float* lse, const float* maps,
-                        const int64_t* strides, const int32_t* q_lens, const int32_t* k_lens,
-                        int dtype, int B, int H, int Hkv, int64_t Lq, int64_t Lk, int causal,
-                        float scale, void* workspace, void* dq, void* dk, void* dv, float* dlam,
-                        void* stream);
+int sla2h_diff_attn_bwd(const void* q, const void* k, const void* v, const void* lam,
+                        int lam_dtype, int64_t lam_stride, const void* dout, const float* lse,
+                        const float* maps, const int64_t* strides, const int32_t* q_lens,
+                        const int32_t* k_lens, int dtype, int B, int H, int Hkv, int64_t Lq,
+                        int64_t Lk, int causal, float scale, void* workspace, void* dq, void* dk,
+                        void* dv, void* dlam, void* stream);
 
 #ifdef __cplusplus
 }
