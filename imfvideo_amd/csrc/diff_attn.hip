@@ -324,13 +324,15 @@ __device__ inline void finish_row(const DiffFwdArgs& a, int64_t bp, int64_t i, i
 }
 
 // Few queries: workgroup = 32 rows (of the `rep` query pairs that share a key pair) over one range of
-// keys; its waves take the 32-key units in turn, both maps of a unit, each with two LDS slots of its own
-// (no barrier in the loop; 128 KB, one workgroup per CU), and their sums are joined in LDS.  The products
-// wait for the loads here, so what the rounding of P lost is always added by a second one.
-template <typename T16>
-__global__ __launch_bounds__(256, 1) void diff_fwd_split_kernel(DiffFwdArgs a) {
-  __shared__ __align__(16) unsigned char kv[2][4][kStageB];
-  __shared__ float mls[4][2][2][32];  // wave, map, (m, l)
+// keys; its W waves take the 32-key units in turn, both maps of a unit, each with an LDS slot of its own
+// (no barrier in the loop), and their sums are joined in LDS.  A wave waits for its unit and computes it
+// while the others' units are on their way: W = 4, two workgroups per CU; W = 8, one, where there is
+// at most one for every CU.  The products wait for the loads here, so what the rounding of P lost is
+// always added by a second one.
+template <typename T16, int W>
+__global__ __launch_bounds__(64 * W, 2) void diff_fwd_split_kernel(DiffFwdArgs a) {
+  __shared__ __align__(16) unsigned char kv[W][kStageB];
+  __shared__ float mls[W][2][2][32];  // wave, map, (m, l)
   const int blk = blockIdx.x / a.splits, sp = blockIdx.x - blk * a.splits;
   const int bk = __builtin_amdgcn_readfirstlane(blk / a.qtiles);
   const int qt = __builtin_amdgcn_readfirstlane(blk - bk * a.qtiles);
@@ -341,10 +343,12 @@ __global__ __launch_bounds__(256, 1) void diff_fwd_split_kernel(DiffFwdArgs a) {
   const int qlen = seq_len(a.q_lens, b, a.Lq), klen = seq_len(a.k_lens, b, a.Lk);
 
   // row of the group: pair kp rep + row / Lq, query row % Lq
-  const int64_t row = (int64_t)qt * 32 + (l & 31);
-  const bool live = row < (int64_t)a.rep * a.Lq;
-  const int p = kp * a.rep + (live ? (int)(row / a.Lq) : 0);
-  const int i = live ? (int)(row % a.Lq) : 0;
+  // (fewer than 2^31 of them: 32-bit divisions)
+  const uint32_t lq = (uint32_t)a.Lq, rows = (uint32_t)a.rep * lq;
+  const uint32_t row = (uint32_t)qt * 32 + (l & 31), rq = row / lq;
+  const bool live = row < rows;
+  const int p = kp * a.rep + (live ? (int)rq : 0);
+  const int i = live ? (int)(row - rq * lq) : 0;
   const int lim = live ? key_limit(i, qlen, klen, a.causal) : 0;
   int kmax = lim, kmin = lim;
 #pragma unroll
@@ -357,15 +361,18 @@ __global__ __launch_bounds__(256, 1) void diff_fwd_split_kernel(DiffFwdArgs a) {
 
   const int64_t u0 = (int64_t)sp * a.units;
   const int64_t uend = min(u0 + a.units, ((int64_t)kmax + kUnitRows - 1) / kUnitRows);
-  auto load = [&](int64_t u, unsigned char* s) __attribute__((always_inline)) {
+  auto load = [&](int64_t u) __attribute__((always_inline)) {
     const int64_t n = u < uend ? (int64_t)klen - u * kUnitRows : 0;
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
-      load_unit(a.k + b * a.kb + (2 * kp + x) * a.kh, u * kUnitRows, n, a.kl * 2, s + x * kUnitB, l);
+      load_unit(a.k + b * a.kb + (2 * kp + x) * a.kh, u * kUnitRows, n, a.kl * 2, kv[w] + x * kUnitB,
+                l);
       load_unit(a.v + b * a.vb + (2 * kp + x) * a.vh, u * kUnitRows, n, a.vl * 2,
-                s + (2 + x) * kUnitB, l);
+                kv[w] + (2 + x) * kUnitB, l);
     }
   };
+  int64_t u = u0 + w;
+  load(u);
 
   u32x4 qf[2][4];
 #pragma unroll
@@ -384,8 +391,9 @@ __global__ __launch_bounds__(256, 1) void diff_fwd_split_kernel(DiffFwdArgs a) {
     mx[m] = kFloor;
     lsum[m] = 0.f;
   }
-  auto compute = [&](int64_t u, const unsigned char* s) __attribute__((always_inline)) {
-    u32x4 pr[2][2], lost[2][2];
+  for (; u < uend; u += W) {
+    __builtin_amdgcn_s_waitcnt(wait_vm_lgkm0(0));
+    const unsigned char* s = kv[w];
 #pragma unroll
     for (int m = 0; m < 2; ++m) {
       f32x16 sc = zero16();
@@ -394,42 +402,29 @@ __global__ __launch_bounds__(256, 1) void diff_fwd_split_kernel(DiffFwdArgs a) {
         sc = mfma_32x32x16<T16>(row_frag(s + m * kUnitB, 0, x, lo), qf[m][x], sc);
       if (u * kUnitRows + kUnitRows > kmin) mask_tile(sc, (int)(lim - u * kUnitRows), h);
       // the wave's first unit sets the bound of the rows that see a key of it
-      float r = probabilities<T16>(sc, a.c, mx[m], pr[m]);
+      u32x4 pr[2], lost[2];
+      float r = probabilities<T16>(sc, a.c, mx[m], pr);
       if (__builtin_amdgcn_ballot_w64(r > Range<T16>::most)) {
         raise_bound(lane_max(sc), a.c, mx[m], lsum[m], acc[m]);
-        r = probabilities<T16>(sc, a.c, mx[m], pr[m]);
+        r = probabilities<T16>(sc, a.c, mx[m], pr);
       }
       lsum[m] += r;
-      lost_halves<T16>(sc, a.c, mx[m], pr[m], lost[m]);
-    }
+      lost_halves<T16>(sc, a.c, mx[m], pr, lost);
 #pragma unroll
-    for (int x = 0; x < 2; ++x)
+      for (int x = 0; x < 2; ++x)
 #pragma unroll
-      for (int mb = 0; mb < 4; ++mb) {
-        const u32x4 vf = col_frag(s + (2 + (mb >> 1)) * kUnitB, 16 * x, mb & 1, lo);
-#pragma unroll
-        for (int m = 0; m < 2; ++m) {
-          acc[m][mb] = mfma_32x32x16<T16>(vf, pr[m][x], acc[m][mb]);
-          acc[m][mb] = mfma_32x32x16<T16>(vf, lost[m][x], acc[m][mb]);
+        for (int mb = 0; mb < 4; ++mb) {
+          const u32x4 vf = col_frag(s + (2 + (mb >> 1)) * kUnitB, 16 * x, mb & 1, lo);
+          acc[m][mb] = mfma_32x32x16<T16>(vf, pr[x], acc[m][mb]);
+          acc[m][mb] = mfma_32x32x16<T16>(vf, lost[x], acc[m][mb]);
         }
-      }
-  };
-  int64_t u = u0 + w;
-  load(u, kv[0][w]);
-  for (; u < uend; u += 8) {
-    load(u + 4, kv[1][w]);
-    __builtin_amdgcn_s_waitcnt(wait_vm_lgkm0(16));
-    compute(u, kv[0][w]);
-    if (u + 4 >= uend) break;
-    __builtin_amdgcn_s_waitcnt(wait_vm_lgkm0(16));  // the reads of this slot are done
-    load(u + 8, kv[0][w]);
-    __builtin_amdgcn_s_waitcnt(wait_vm_lgkm0(16));
-    compute(u + 4, kv[1][w]);
-    __builtin_amdgcn_s_waitcnt(wait_vm_lgkm0(16));
+    }
+    __builtin_amdgcn_s_waitcnt(wait_vm_lgkm0(0));  // the reads of this slot are done
+    load(u + W);
   }
   __builtin_amdgcn_s_waitcnt(wait_vm_lgkm0(0));
 
-  // join the four waves: fp32 O^T tiles [channel][row] of both maps in the slots' memory
+  // join the waves, map by map: fp32 O^T tiles [channel][row] in the slots' memory
 #pragma unroll
   for (int m = 0; m < 2; ++m) {
     const float ls = swap32_sum(lsum[m]);
@@ -438,108 +433,125 @@ __global__ __launch_bounds__(256, 1) void diff_fwd_split_kernel(DiffFwdArgs a) {
       mls[w][m][1][l] = ls;
     }
   }
-  __syncthreads();
+  // thread: row tid % 32, channels 8 c8 .., 128 / (2 W) groups of them in turn
+  const int r = tid & 31;
+  // (row r of the tile is lane r's, in every wave)
+  const bool mine = live;
+  const int64_t op = (int64_t)b * a.P + p, oi = i, flat = op * a.Lq + oi;
+  constexpr int NG = 8 / W;  // groups of eight channels of a thread (W = 8: one)
+  float mm[2], ll[2], x[2][NG][8];
 #pragma unroll
   for (int m = 0; m < 2; ++m) {
-    float* ot = reinterpret_cast<float*>(kv[m][w]);
+    if (m) __syncthreads();
+    float* ot = reinterpret_cast<float*>(kv[w]);
 #pragma unroll
     for (int mb = 0; mb < 4; ++mb)
 #pragma unroll
-      for (int r = 0; r < 16; ++r)
-        ot[(32 * mb + 8 * (r >> 2) + 4 * h + (r & 3)) * 32 + (l & 31)] = acc[m][mb][r];
-  }
-  __syncthreads();
-  // thread: row tid % 32, channels 8 (tid / 32) + 64 k ..
-  const int r = tid & 31;
-  const int64_t orow = (int64_t)qt * 32 + r;
-  if (orow >= (int64_t)a.rep * a.Lq) return;
-  const int64_t op = (int64_t)b * a.P + kp * a.rep + orow / a.Lq, oi = orow % a.Lq;
-  const int64_t flat = op * a.Lq + oi;
-  float mm[2], ll[2], f[2][4];
+      for (int e = 0; e < 16; ++e)
+        ot[(32 * mb + 8 * (e >> 2) + 4 * h + (e & 3)) * 32 + (l & 31)] = acc[m][mb][e];
+    __syncthreads();
+    mm[m] = kFloor;
 #pragma unroll
-  for (int m = 0; m < 2; ++m) {
-    mm[m] = fmaxf(fmaxf(mls[0][m][0][r], mls[1][m][0][r]), fmaxf(mls[2][m][0][r], mls[3][m][0][r]));
+    for (int j = 0; j < W; ++j) mm[m] = fmaxf(mm[m], mls[j][m][0][r]);
     ll[m] = 0.f;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      f[m][j] = fast_exp2(mls[j][m][0][r] - mm[m]);
-      ll[m] += f[m][j] * mls[j][m][1][r];
+    for (int g = 0; g < NG; ++g)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[m][g][e] = 0.f;
+#pragma unroll
+    for (int j = 0; j < W; ++j) {
+      const float f = fast_exp2(mls[j][m][0][r] - mm[m]);
+      ll[m] += f * mls[j][m][1][r];
+      const float* src = reinterpret_cast<const float*>(kv[j]);
+#pragma unroll
+      for (int g = 0; g < NG; ++g)
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          x[m][g][e] += f * src[((g * 2 * W + (tid >> 5)) * 8 + e) * 32 + r];
     }
   }
+  if (!mine) return;
 #pragma unroll
-  for (int k = 0; k < 2; ++k) {
-    const int c0 = 64 * k + (tid >> 5) * 8;
-    float x[2][8];
+  for (int g = 0; g < NG; ++g) {
+    const int c0 = (g * 2 * W + (tid >> 5)) * 8;
+    if (a.splits == 1) {
+      const float y[2][8] = {{x[0][g][0], x[0][g][1], x[0][g][2], x[0][g][3], x[0][g][4], x[0][g][5],
+                              x[0][g][6], x[0][g][7]},
+                             {x[1][g][0], x[1][g][1], x[1][g][2], x[1][g][3], x[1][g][4], x[1][g][5],
+                              x[1][g][6], x[1][g][7]}};
+      finish_row<T16>(a, op, oi, c0, key_limit((int)oi, qlen, klen, a.causal) > 0, y, mm, ll);
+      continue;
+    }
 #pragma unroll
     for (int m = 0; m < 2; ++m) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        x[m][e] = 0.f;
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          x[m][e] += f[m][j] * reinterpret_cast<const float*>(kv[m][j])[(c0 + e) * 32 + r];
-      }
-      if (a.splits > 1) {
-        float* d = a.part + ((sp * 2 + m) * a.nrows + flat) * 128 + c0;
-        *reinterpret_cast<f32x4*>(d) = f32x4{x[m][0], x[m][1], x[m][2], x[m][3]};
-        *reinterpret_cast<f32x4*>(d + 4) = f32x4{x[m][4], x[m][5], x[m][6], x[m][7]};
-        if (c0 == 0) a.ml[(sp * 2 + m) * a.nrows + flat] = make_float2(mm[m], ll[m]);
-      }
+      float* d = a.part + ((sp * 2 + m) * a.nrows + flat) * 128 + c0;
+      *reinterpret_cast<f32x4*>(d) = f32x4{x[m][g][0], x[m][g][1], x[m][g][2], x[m][g][3]};
+      *reinterpret_cast<f32x4*>(d + 4) = f32x4{x[m][g][4], x[m][g][5], x[m][g][6], x[m][g][7]};
+      if (c0 == 0) a.ml[(sp * 2 + m) * a.nrows + flat] = make_float2(mm[m], ll[m]);
     }
-    if (a.splits == 1)
-      finish_row<T16>(a, op, oi, c0, key_limit((int)oi, qlen, klen, a.causal) > 0, x, mm, ll);
   }
 }
 
-// Joins the key ranges of a row: 16 groups of 16 lanes (eight channels each) take the ranges in turn,
-// both maps, and their sums are added in order.
+// Joins the key ranges of a row: 64 groups of 16 lanes, 32 for each map (eight channels per lane), take
+// the ranges in turn, and their sums are added in order.
 template <typename T16>
-__global__ __launch_bounds__(256) void diff_join_kernel(DiffFwdArgs a) {
-  __shared__ float sm[2][16], sl[2][16];
-  __shared__ f32x4 sx[2][16][32];
+__global__ __launch_bounds__(1024) void diff_join_kernel(DiffFwdArgs a) {
+  __shared__ float sm[2][32], sl[2][32];
+  __shared__ f32x4 sx[2][32][32];
   const int64_t flat = blockIdx.x;
-  const int grp = threadIdx.x >> 4, c0 = (threadIdx.x & 15) * 8;
+  const int m = threadIdx.x >> 9, grp = (threadIdx.x >> 4) & 31, c0 = (threadIdx.x & 15) * 8;
   const int64_t bp = flat / a.Lq, i = flat - bp * a.Lq;
   const int b = (int)(bp / a.P);
-  const int qlen = seq_len(a.q_lens, b, a.Lq), klen = seq_len(a.k_lens, b, a.Lk);
-#pragma unroll
-  for (int m = 0; m < 2; ++m) {
-    float mm = kFloor, ll = 0.f;
-    f32x4 x{0.f, 0.f, 0.f, 0.f}, y = x;
-    for (int s = grp; s < a.splits; s += 16) {
-      const int64_t at = (s * 2 + m) * a.nrows + flat;
-      const float2 ml = a.ml[at];
-      const f32x4* src = reinterpret_cast<const f32x4*>(a.part + at * 128 + c0);
-      const float mn = fmaxf(mm, ml.x), f = fast_exp2(mm - mn), g = fast_exp2(ml.x - mn);
-      mm = mn;
-      ll = ll * f + g * ml.y;
-      x = x * f + g * src[0];
-      y = y * f + g * src[1];
-    }
-    sx[m][grp][c0 / 4] = x;
-    sx[m][grp][c0 / 4 + 1] = y;
-    if (c0 == 0) sm[m][grp] = mm, sl[m][grp] = ll;
+  float mm = kFloor, ll = 0.f;
+  f32x4 x{0.f, 0.f, 0.f, 0.f}, y = x;
+#pragma unroll 2
+  for (int s = grp; s < a.splits; s += 32) {
+    const int64_t at = (s * 2 + m) * a.nrows + flat;
+    const float2 ml = a.ml[at];
+    const f32x4* src = reinterpret_cast<const f32x4*>(a.part + at * 128 + c0);
+    const f32x4 p0 = src[0], p1 = src[1];
+    const float mn = fmaxf(mm, ml.x), f = fast_exp2(mm - mn), g = fast_exp2(ml.x - mn);
+    mm = mn;
+    ll = ll * f + g * ml.y;
+    x = x * f + g * p0;
+    y = y * f + g * p1;
   }
+  sx[m][grp][c0 / 4] = x;
+  sx[m][grp][c0 / 4 + 1] = y;
+  if (c0 == 0) sm[m][grp] = mm, sl[m][grp] = ll;
   __syncthreads();
-  if (grp) return;
-  float mm[2], ll[2], x[2][8];
+  if (threadIdx.x >= 64) return;  // one wave: lane j of each half the weight of group j
+  const int qlen = seq_len(a.q_lens, b, a.Lq), klen = seq_len(a.k_lens, b, a.Lk);
+  const int k0 = threadIdx.x >> 5, j0 = threadIdx.x & 31;
+  float top = sm[k0][j0];
 #pragma unroll
-  for (int m = 0; m < 2; ++m) {
-    mm[m] = kFloor;
-    ll[m] = 0.f;
+  for (int s = 16; s >= 1; s >>= 1) top = fmaxf(top, __shfl_xor(top, s, 64));
+  const float weight = fast_exp2(sm[k0][j0] - top);
+  float all = weight * sl[k0][j0];
 #pragma unroll
-    for (int j = 0; j < 16; ++j) mm[m] = fmaxf(mm[m], sm[m][j]);
+  for (int s = 16; s >= 1; s >>= 1) all += __shfl_xor(all, s, 64);
+  sm[k0][j0] = weight;
+  __builtin_amdgcn_wave_barrier();  // (read by this wave alone)
+  const float tm[2] = {__shfl(top, 0, 64), __shfl(top, 32, 64)};
+  const float tl[2] = {__shfl(all, 0, 64), __shfl(all, 32, 64)};
+  if (threadIdx.x >= 16) return;
+  float t[2][8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) x[m][e] = 0.f;
+  for (int k = 0; k < 2; ++k) {
 #pragma unroll
-    for (int j = 0; j < 16; ++j) {
-      const float f = fast_exp2(sm[m][j] - mm[m]);
-      ll[m] += f * sl[m][j];
+    for (int e = 0; e < 8; ++e) t[k][e] = 0.f;
+#pragma unroll 8
+    for (int j = 0; j < 32; ++j) {
+      const float f = sm[k][j];
+      const f32x4 p0 = sx[k][j][c0 / 4], p1 = sx[k][j][c0 / 4 + 1];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) x[m][e] += f * sx[m][j][c0 / 4 + (e >> 2)][e & 3];
+      for (int e = 0; e < 4; ++e) {
+        t[k][e] += f * p0[e];
+        t[k][4 + e] += f * p1[e];
+      }
     }
   }
-  finish_row<T16>(a, bp, i, c0, key_limit((int)i, qlen, klen, a.causal) > 0, x, mm, ll);
+  finish_row<T16>(a, bp, i, c0, key_limit((int)i, qlen, klen, a.causal) > 0, t, tm, tl);
 }
 
 // The form of a call: query blocks of 128 or 64 rows, or of 32 rows of a key pair's group.
@@ -548,6 +560,7 @@ struct FwdPlan {
   int64_t qtiles, nwork;
   int splits;  // ranges of keys
   int64_t units;
+  int waves;  // nq = 0
 };
 
 // even: neither causal nor lengths
@@ -572,13 +585,14 @@ FwdPlan fwd_plan(int B, int H, int Hkv, int64_t Lq, int64_t Lk, bool even) {
   p.nq = 0;
   p.qtiles = (rep * Lq + 31) / 32;
   const int64_t blocks = bk * p.qtiles;
-  int64_t s = (256 + blocks - 1) / blocks;
+  int64_t s = (512 + blocks - 1) / blocks;
   const int64_t most = units / 8;  // two units per wave and range at least
   s = s < most ? s : most;
   p.splits = s < 1 ? 1 : (int)s;
   p.units = (units + p.splits - 1) / p.splits;
   p.splits = (int)((units + p.units - 1) / p.units);
   p.nwork = blocks * p.splits;
+  p.waves = p.nwork <= 256 && p.units > 4 ? 8 : 4;
   return p;
 }
 
@@ -656,11 +670,13 @@ extern "C" int sla2h_diff_attn_fwd(const void* q, const void* k, const void* v, 
       diff_fwd_kernel<T16, 2><<<work_grid(a.map), 256, 0, st>>>(a);
     else if (p.nq == 1)
       diff_fwd_kernel<T16, 1><<<work_grid(a.map), 256, 0, st>>>(a);
+    else if (p.waves == 8)
+      diff_fwd_split_kernel<T16, 8><<<(unsigned)p.nwork, 512, 0, st>>>(a);
     else
-      diff_fwd_split_kernel<T16><<<(unsigned)p.nwork, 256, 0, st>>>(a);
+      diff_fwd_split_kernel<T16, 4><<<(unsigned)p.nwork, 256, 0, st>>>(a);
     const int err = (int)hipGetLastError();
     if (err || p.splits == 1) return err;
-    diff_join_kernel<T16><<<(unsigned)a.nrows, 256, 0, st>>>(a);
+    diff_join_kernel<T16><<<(unsigned)a.nrows, 1024, 0, st>>>(a);
     return (int)hipGetLastError();
   };
   return dtype == SLA2H_DTYPE_BF16 ? go(BF16{}) : go(F16{});
