@@ -39,7 +39,7 @@ struct Scaled<F16> {
 // every second stage (1.25 times; B = 1, H = 8, L = 29,952: 0.4 ms).  dk, dv: calls of at most
 // kFineRows rows per key pair (longer sums average the roundings out).
 constexpr int kFineKeys = 4096, kFineRows = 512;
-constexpr int kKeyRows = 256;  // keys of a workgroup of dk and dv
+constexpr int kKeyRows = 128;  // keys of a workgroup of dk and dv
 constexpr int kNormRows = 64;  // rows of a partial maximum of the norms and of a partial sum of dlam
 
 struct DiffBwdArgs {
@@ -396,10 +396,10 @@ __device__ inline void add_rows(f32x16& x, float v) {
 // wave: 6.1 ms at B = 1, H = 8, L = 29,952, bf16).  A row's statistic belongs to one register of a
 // score tile in all lanes of a half: a lane reads one value, and the add takes it from there (DPP).
 template <typename T16, bool CAUSAL, bool FINE>
-__global__ __launch_bounds__(512, 2) void diff_bwd_dkdv_kernel(DiffBwdArgs a) {
-  __shared__ __align__(16) unsigned char r0[kStageB], r1[kStageB], r2[kStageB], r3[kStageB];
-  __shared__ __align__(16) float t0_[4][64], t1_[4][64], t2_[4][64], t3_[4][64];
-  __shared__ __align__(16) unsigned char vt[8][2 * kUnitB];
+__global__ __launch_bounds__(256, 2) void diff_bwd_dkdv_kernel(DiffBwdArgs a) {
+  __shared__ __align__(16) unsigned char r0[kStageB], r1[kStageB];
+  __shared__ __align__(16) float t0_[4][64], t1_[4][64];
+  __shared__ __align__(16) unsigned char vt[4][2 * kUnitB];
   int bk, item;
   if (!work_item(a.kv_map, blockIdx.x, bk, item)) return;
   const int ktile = item / a.kv_splits, sp = item - ktile * a.kv_splits;
@@ -429,16 +429,14 @@ __global__ __launch_bounds__(512, 2) void diff_bwd_dkdv_kernel(DiffBwdArgs a) {
   int lu = u0, lp = u0 < u1 ? u0 / nq : 0;
   int lrow = first + (u0 < u1 ? u0 - lp * nq : 0) * kUnitRows;
   int cu = u0, cp = lp, crow = lrow;
-  // waves 2x and 2x + 1 load matrix x of the stage, 16 rows each, and statistic x (both the same)
-  const int x = w >> 1;
+  // wave x loads matrix x of the stage and statistic x
+  const int x = w;
   auto load = [&](unsigned char* s, float (*st)[64]) __attribute__((always_inline)) {
     const int64_t p = (int64_t)kp * a.rep + lp, n = lu < u1 ? (int64_t)qlen - lrow : 0;
     const uint16_t* src = x < 2 ? a.q + b * a.qb + (2 * p + x) * a.qh
                                 : a.dout + ((int64_t)b * a.Lq * a.P + p) * 128 + 64 * (x - 2);
     const int64_t ld = x < 2 ? a.ql * 2 : (int64_t)a.P * 256;
-    const auto rs = rows_rsrc(src, lrow, n < kUnitRows ? n : kUnitRows, ld);
-#pragma unroll
-    for (int j = 0; j < 2; ++j) dma_rows8(rs, s + x * kUnitB, 2 * (w & 1) + j, (int)ld, l);
+    load_unit(src, lrow, n, ld, s + x * kUnitB, l);
     const auto rt = make_rsrc(a.stat + x * a.nrows + ((int64_t)b * a.P + p) * a.Lq + lrow,
                               n <= 0 ? 0 : (n < kUnitRows ? n : kUnitRows) * 4);
     __builtin_amdgcn_raw_ptr_buffer_load_lds(
@@ -470,7 +468,7 @@ __global__ __launch_bounds__(512, 2) void diff_bwd_dkdv_kernel(DiffBwdArgs a) {
   auto stage = [&](const unsigned char* s, const float (*st)[64], unsigned char* sl, float (*tl)[64])
       __attribute__((always_inline)) {
     // the stages up to this one have landed, the one before is read
-    __builtin_amdgcn_s_waitcnt(wait_vm_lgkm0(6));
+    __builtin_amdgcn_s_waitcnt(wait_vm_lgkm0(0));
     __builtin_amdgcn_s_barrier();
     load(sl, tl);
     if (kw < klen) {
@@ -544,16 +542,10 @@ __global__ __launch_bounds__(512, 2) void diff_bwd_dkdv_kernel(DiffBwdArgs a) {
     if (crow >= qlen && cu < u1) crow = first, ++cp;
   };
   load(r0, t0_);
-  load(r1, t1_);
-  load(r2, t2_);
-  for (int u = u0; u < u1; u += 4) {
-    stage(r0, t0_, r3, t3_);
+  for (int u = u0; u < u1; u += 2) {
+    stage(r0, t0_, r1, t1_);
     if (u + 1 >= u1) break;
     stage(r1, t1_, r0, t0_);
-    if (u + 2 >= u1) break;
-    stage(r2, t2_, r1, t1_);
-    if (u + 3 >= u1) break;
-    stage(r3, t3_, r2, t2_);
   }
   __builtin_amdgcn_s_waitcnt(wait_vm_lgkm0(0));
 
@@ -720,13 +712,13 @@ extern "C" int sla2h_diff_attn_bwd(const void* q, const void* k, const void* v, 
       const unsigned grid = work_grid(a.kv_map);
       const bool few = a.rep * Lq <= kFineRows;
       if (causal && few)
-        diff_bwd_dkdv_kernel<T16, true, true><<<grid, 512, 0, st>>>(a);
+        diff_bwd_dkdv_kernel<T16, true, true><<<grid, 256, 0, st>>>(a);
       else if (causal)
-        diff_bwd_dkdv_kernel<T16, true, false><<<grid, 512, 0, st>>>(a);
+        diff_bwd_dkdv_kernel<T16, true, false><<<grid, 256, 0, st>>>(a);
       else if (few)
-        diff_bwd_dkdv_kernel<T16, false, true><<<grid, 512, 0, st>>>(a);
+        diff_bwd_dkdv_kernel<T16, false, true><<<grid, 256, 0, st>>>(a);
       else
-        diff_bwd_dkdv_kernel<T16, false, false><<<grid, 512, 0, st>>>(a);
+        diff_bwd_dkdv_kernel<T16, false, false><<<grid, 256, 0, st>>>(a);
       if ((err = (int)hipGetLastError())) return err;
     }
     diff_bwd_dq_kernel<T16><<<a.dq_blocks + a.P, 256, 0, st>>>(a);
