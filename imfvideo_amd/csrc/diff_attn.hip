@@ -48,8 +48,8 @@ __device__ inline uint16_t* out_row(const DiffFwdArgs& a, int64_t bp, int64_t i)
 
 // Workgroup = 4 waves: two query groups of 32 NQ rows x two maps, of one pair.  Stages of 32 keys
 // (k of both maps, the 128 value channels) three ahead in four LDS slots, one barrier each.  The
-// scores of a wave's first 32 rows are one stage ahead, so that they run on the matrix cores under
-// the exponentials of its other rows, and those of the other rows under the first ones'.
+// scores of a wave's first 32 rows are one stage ahead, and the products of its last ones with the values
+// one behind: every product has exponentials of other numbers to run under (weave).
 template <typename T16, int NQ>
 __global__ __launch_bounds__(256, 2) void diff_fwd_kernel(DiffFwdArgs a) {
   __shared__ __align__(16) unsigned char s0[kStageB], s1[kStageB], s2[kStageB], s3[kStageB],
@@ -109,15 +109,12 @@ __global__ __launch_bounds__(256, 2) void diff_fwd_kernel(DiffFwdArgs a) {
     lsum[n] = 0.f;
   }
   f32x16 sc[NQ];
-  u32x4 kf[4], pr[NQ][2];
-  auto read_k = [&](const unsigned char* s) __attribute__((always_inline)) {
-#pragma unroll
-    for (int x = 0; x < 4; ++x) kf[x] = row_frag(s + m * kUnitB, 0, x, lo);
-  };
-  auto scores = [&](int n) __attribute__((always_inline)) {
+  u32x4 pr[NQ][2];
+  auto scores = [&](int n, const unsigned char* s) __attribute__((always_inline)) {
     sc[n] = zero16();
 #pragma unroll
-    for (int x = 0; x < 4; ++x) sc[n] = mfma_32x32x16<T16>(kf[x], qf[n][x], sc[n]);
+    for (int x = 0; x < 4; ++x)
+      sc[n] = mfma_32x32x16<T16>(row_frag(s + m * kUnitB, 0, x, lo), qf[n][x], sc[n]);
   };
   auto mask = [&](int n, int base) __attribute__((always_inline)) {
     if (base + kUnitRows > wall) {
@@ -125,28 +122,70 @@ __global__ __launch_bounds__(256, 2) void diff_fwd_kernel(DiffFwdArgs a) {
       mask_tile(sc[n], lim[n] - base, h);
     }
   };
-  // rows n again under a new bound: `cur` is the stage of their keys, `nxt` what kf holds after it
-  auto again = [&](int n, int base, const unsigned char* cur, const unsigned char* nxt)
-      __attribute__((always_inline)) {
-    f32x16 other;
-    if (NQ == 2) other = sc[n ^ 1];
-    read_k(cur);
-    scores(n);
+  // rows n again under a new bound
+  auto again = [&](int n, int base, const unsigned char* cur) __attribute__((always_inline)) {
+    const f32x16 ahead = sc[n];  // (NQ = 1: the next stage's)
+    scores(n, cur);
     mask(n, base);
     raise_bound(lane_max(sc[n]), a.c, mx[n], lsum[n], acc[n]);
     const float r = probabilities<T16>(sc[n], a.c, mx[n], pr[n]);
-    read_k(nxt);
-    if (NQ == 2) sc[n ^ 1] = other;
+    if (NQ == 1) sc[n] = ahead;
     return r;
   };
-  auto values = [&](int n, const unsigned char* cur) __attribute__((always_inline)) {
-#pragma unroll
-    for (int s = 0; s < 2; ++s)
-#pragma unroll
-      for (int mb = 0; mb < 4; ++mb)
-        acc[n][mb] = mfma_32x32x16<T16>(
-            col_frag(cur + (2 + (mb >> 1)) * kUnitB, 16 * s, mb & 1, lo), pr[n][s], acc[n][mb]);
+  auto value = [&](int j, const unsigned char* s) __attribute__((always_inline)) {
+    return col_frag(s + (2 + ((j & 3) >> 1)) * kUnitB, 16 * (j >> 2), j & 1, lo);
   };
+  auto values = [&](int n, const unsigned char* s) __attribute__((always_inline)) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      acc[n][j & 3] = mfma_32x32x16<T16>(value(j, s), pr[n][j >> 2], acc[n][j & 3]);
+  };
+  // Half a stage: rows ns's scores of the keys in `ks`, rows nv's products with the values in `vs`, among
+  // rows ne's exponentials; returns their sum.  Twelve products, their LDS operands read two products
+  // ahead, each beside a share of the exponentials that covers its 32 cycles.  The order is fixed: left
+  // to the compiler the products come first, each behind its operand, and the exponentials after them
+  // (7 % more cycles).
+  auto weave = [&](auto ns_, const unsigned char* ks, auto nv_, const unsigned char* vs, auto ne_)
+      __attribute__((always_inline)) {
+    constexpr int ns = decltype(ns_)::value, nv = decltype(nv_)::value, ne = decltype(ne_)::value;
+    u32x4 f[3], next[2];
+    auto operand = [&](int i) __attribute__((always_inline)) {
+      return i % 3 == 0 ? row_frag(ks + m * kUnitB, 0, i / 3, lo) : value(i / 3 * 2 + i % 3 - 1, vs);
+    };
+    const float off = Range<T16>::shift - mx[ne];
+    float r[2] = {0.f, 0.f};
+    f32x16 z = zero16();
+    f[0] = operand(0);
+    f[1] = operand(1);
+#pragma unroll
+    for (int i = 0; i < 12; ++i) {
+      __builtin_amdgcn_sched_barrier(0);
+      if (i + 2 < 12) f[(i + 2) % 3] = operand(i + 2);
+      if (i % 3 == 0) {
+        z = mfma_32x32x16<T16>(f[i % 3], qf[ns][i / 3], z);
+      } else {
+        const int j = i / 3 * 2 + i % 3 - 1;
+        acc[nv][j & 3] = mfma_32x32x16<T16>(f[i % 3], pr[nv][j >> 2], acc[nv][j & 3]);
+      }
+      if (i % 3 < 2) {  // scores 2 k, 2 k + 1
+        const int k = i / 3 * 2 + i % 3;
+        const float x = fast_exp2(__builtin_fmaf(sc[ne][2 * k], a.c, off));
+        const float y = fast_exp2(__builtin_fmaf(sc[ne][2 * k + 1], a.c, off));
+        uint32_t word = pack_pair<T16>(x, y);
+        r[0] += x;
+        r[1] += y;
+        asm volatile("" : "+v"(word), "+v"(r[0]), "+v"(r[1]));  // here, not behind the products
+        next[k >> 2][k & 3] = word;
+      }
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    sc[ns] = z;
+    pr[ne][0] = next[0];
+    pr[ne][1] = next[1];
+    return r[0] + r[1];
+  };
+  constexpr std::integral_constant<int, 0> first{};
+  constexpr std::integral_constant<int, NQ - 1> other{};
   auto stage = [&](int t, const unsigned char* prev, const unsigned char* cur,
                    const unsigned char* nxt, unsigned char* to) __attribute__((always_inline)) {
     // the stages up to t + 1 have landed, stage t - 2 is read
@@ -155,20 +194,13 @@ __global__ __launch_bounds__(256, 2) void diff_fwd_kernel(DiffFwdArgs a) {
     load(t + 3, to);
     const int base = t * kUnitRows;
     mask(0, base);
-    if (NQ == 2) {
-      scores(NQ - 1);
-      values(NQ - 1, prev);
-    }
-    float r = probabilities<T16>(sc[0], a.c, mx[0], pr[0]);
-    if (__builtin_amdgcn_ballot_w64(r > Range<T16>::most)) r = again(0, base, cur, cur);
+    float r = NQ == 2 ? weave(other, cur, other, prev, first) : weave(first, nxt, first, prev, first);
+    if (__builtin_amdgcn_ballot_w64(r > Range<T16>::most)) r = again(0, base, cur);
     lsum[0] += r;
-    if (NQ == 2) mask(NQ - 1, base);
-    read_k(nxt);
-    scores(0);
-    values(0, cur);
     if (NQ == 2) {
-      r = probabilities<T16>(sc[NQ - 1], a.c, mx[NQ - 1], pr[NQ - 1]);
-      if (__builtin_amdgcn_ballot_w64(r > Range<T16>::most)) r = again(NQ - 1, base, cur, nxt);
+      mask(NQ - 1, base);
+      r = weave(first, nxt, first, cur, other);
+      if (__builtin_amdgcn_ballot_w64(r > Range<T16>::most)) r = again(NQ - 1, base, cur);
       lsum[NQ - 1] += r;
     }
   };
@@ -177,8 +209,7 @@ __global__ __launch_bounds__(256, 2) void diff_fwd_kernel(DiffFwdArgs a) {
   load(t0 + 2, s2);
   __builtin_amdgcn_s_waitcnt(wait_vm_lgkm0(8));
   __builtin_amdgcn_s_barrier();
-  read_k(s0);
-  scores(0);
+  scores(0, s0);
 #pragma unroll
   for (int n = 0; n < NQ; ++n) pr[n][0] = pr[n][1] = u32x4{0, 0, 0, 0};
   // The first stage adds what its own slot holds with probabilities of 0; the other rows of the
@@ -201,7 +232,7 @@ __global__ __launch_bounds__(256, 2) void diff_fwd_kernel(DiffFwdArgs a) {
     stage(t + 4, s3, s4, s0, s2);
     last = s4;
   }
-  if (NQ == 2) values(NQ - 1, last);
+  values(NQ - 1, last);
   for (int t = max(wn, t0); t < nt; ++t) {
     __builtin_amdgcn_s_waitcnt(wait_vm_lgkm0(4));
     __builtin_amdgcn_s_barrier();
