@@ -382,11 +382,18 @@ __device__ inline float row_value(float x) {
   return __builtin_bit_cast(
       float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, x), 0x150 + E, 0xf, 0xf, true));
 }
-// x[e] + that value, register e of a C tile
-template <int E = 0>
-__device__ inline void add_rows(f32x16& x, float v) {
-  x[E] += row_value<E>(v);
-  if constexpr (E < 15) add_rows<E + 1>(x, v);
+__device__ inline float row_value_at(float x, int e) {  // e a constant where it is called
+  switch (e) {
+#define SLA2H_ROW(E) \
+  case E:            \
+    return row_value<E>(x);
+    SLA2H_ROW(0) SLA2H_ROW(1) SLA2H_ROW(2) SLA2H_ROW(3) SLA2H_ROW(4) SLA2H_ROW(5) SLA2H_ROW(6)
+    SLA2H_ROW(7) SLA2H_ROW(8) SLA2H_ROW(9) SLA2H_ROW(10) SLA2H_ROW(11) SLA2H_ROW(12) SLA2H_ROW(13)
+    SLA2H_ROW(14)
+#undef SLA2H_ROW
+    default:
+      return row_value<15>(x);
+  }
 }
 
 // dk, dv: workgroup = 8 waves x 32 keys of one key pair; the query rows (both maps' queries, the 128
@@ -462,84 +469,157 @@ __global__ __launch_bounds__(256, 2) void diff_bwd_dkdv_kernel(DiffBwdArgs a) {
   f32x16 ak[2][2], av[4];
 #pragma unroll
   for (int y = 0; y < 2; ++y) ak[0][y] = ak[1][y] = av[y] = av[2 + y] = zero16();
+  // The weight of the pair at hand: |lam| goes into the exponent, its sign into the packed dS.  (Loaded
+  // where the pair changes only: a load in every stage would wait for the stages on their way.)
+  float log_lam = 0.f;
+  bool minus = false;
+  auto load_weight = [&]() __attribute__((always_inline)) {
+    const float lam = a.lam[kp * a.rep + cp];
+    log_lam = __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(
+                                            int, __log2f(__builtin_fabsf(lam)) * a.inv_c)));
+    minus = __builtin_amdgcn_readfirstlane(lam < 0.f);
+  };
+  load_weight();
   // register e of a tile is row 8 (e / 4) + 4 h + e % 4: lane e of each 16 reads it
   const int srow = 8 * ((l & 15) >> 2) + 4 * h + (l & 3);
 
+  // A stage in four runs of products, each in a fixed order with its LDS operands read ahead (by two
+  // products, by one where the lost halves need the registers) and a share of the
+  // exponentials beside it: S_1 and dA; S_2 under map 1; dk_1 under map 2; dk_2 and dv.
+  constexpr int AHEAD = FINE ? 1 : 2;
   auto stage = [&](const unsigned char* s, const float (*st)[64], unsigned char* sl, float (*tl)[64])
       __attribute__((always_inline)) {
-    // the stages up to this one have landed, the one before is read
+    // this stage has landed, the one before is read
     __builtin_amdgcn_s_waitcnt(wait_vm_lgkm0(0));
     __builtin_amdgcn_s_barrier();
     load(sl, tl);
     if (kw < klen) {
-      const float lam = a.lam[kp * a.rep + cp];
-      const bool hidden = CAUSAL && crow < kw + 31 - off;
-      const int y = kw + (l & 31) - off - crow - 4 * h;
       float sv[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) sv[i] = st[i][srow];
-      f32x16 dp = zero16(), p[2] = {zero16(), zero16()};
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        p[0] = mfma_32x32x16<T16>(row_frag(s, 0, k, lo), kf[0][k], p[0]);
-        dp = mfma_32x32x16<T16>(row_frag(s + 2 * kUnitB, 0, k, lo), row_frag(vt[w], 0, k, lo), dp);
-        dp = mfma_32x32x16<T16>(row_frag(s + 3 * kUnitB, 0, k, lo),
-                                row_frag(vt[w] + kUnitB, 0, k, lo), dp);
-      }
-#pragma unroll
-      for (int m = 0; m < 2; ++m) {
-        if (m == 1) {
-#pragma unroll
-          for (int k = 0; k < 4; ++k)
-            p[1] = mfma_32x32x16<T16>(row_frag(s + kUnitB, 0, k, lo), kf[1][k], p[1]);
-        }
-        add_rows(p[m], sv[m]);
-#pragma unroll
-        for (int e = 0; e < 16; ++e) p[m][e] = fast_exp2(p[m][e] * a.c);
-        if (m == 1) {
-#pragma unroll
-          for (int e = 0; e < 16; ++e) p[1][e] *= lam;
-        }
-        if (hidden) {
+      sv[1] += log_lam;
+      const float sign = minus ? -1.f : 1.f;
+      const uint32_t flip = minus ? 0x80008000u : 0u;
+      auto mask = [&](f32x16& x) __attribute__((always_inline)) {
+        if (CAUSAL && crow < kw + 31 - off) {
           asm volatile("");
+          const int y = kw + (l & 31) - off - crow - 4 * h;
 #pragma unroll
-          for (int e = 0; e < 16; ++e) p[m][e] = 8 * (e >> 2) + (e & 3) >= y ? p[m][e] : 0.f;
+          for (int e = 0; e < 16; ++e)
+            x[e] = 8 * (e >> 2) + (e & 3) >= y ? x[e] : -__builtin_inff();
         }
-        f32x16 d = dp;
-        add_rows(d, sv[2 + m]);
+      };
+      f32x16 dp = zero16(), p[2] = {zero16(), zero16()};
+      int vw = w * 2 * kUnitB;
+      asm volatile("" : "+s"(vw));  // (four addresses held for the whole loop otherwise)
+      {
+        u32x4 fa[AHEAD + 1], fb[AHEAD + 1];
+        auto operands = [&](int i) __attribute__((always_inline)) {
+          const int j = i / 3 * 2 + i % 3 - 1, r = i % (AHEAD + 1);  // j: dA's products
+          fa[r] = i % 3 ? row_frag(s + (2 + (j >> 2)) * kUnitB, 0, j & 3, lo)
+                        : row_frag(s, 0, i / 3, lo);
+          if (i % 3) fb[r] = row_frag(vt[0] + vw + (j >> 2) * kUnitB, 0, j & 3, lo);
+        };
 #pragma unroll
-        for (int e = 0; e < 16; ++e) d[e] *= Scaled<T16>::value ? p[m][e] * pw.m : p[m][e];
+        for (int i = 0; i < AHEAD; ++i) operands(i);
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          const u32x4 dd = pack_step<T16>(d, k);
-          u32x4 lost;
-          if (FINE) lost = lost_step<T16>(d, k, dd);
+        for (int i = 0; i < 12; ++i) {
+          __builtin_amdgcn_sched_barrier(0);
+          if (i + AHEAD < 12) operands(i + AHEAD);
+          const int r = i % (AHEAD + 1);
+          if (i % 3)
+            dp = mfma_32x32x16<T16>(fa[r], fb[r], dp);
+          else
+            p[0] = mfma_32x32x16<T16>(fa[r], kf[0][i / 3], p[0]);
+        }
+      }
+      mask(p[0]);
+      u32x4 dd[2][2], dl[2][2], f[2];
+      // registers 4 g .. 4 g + 3 of map m: probabilities (times |lam|), dS in 16 bits
+      auto elements = [&](int m, int g) __attribute__((always_inline)) {
+        float d[4];
 #pragma unroll
-          for (int mb = 0; mb < 2; ++mb) {
-            const u32x4 qf = col_frag(s + m * kUnitB, 16 * k, mb, lo);
-            ak[m][mb] = mfma_32x32x16<T16>(qf, dd, ak[m][mb]);
-            if (FINE) ak[m][mb] = mfma_32x32x16<T16>(qf, lost, ak[m][mb]);
+        for (int i = 0; i < 4; ++i) {
+          const int e = 4 * g + i;
+          const float y = fast_exp2((p[m][e] + row_value_at(sv[m], e)) * a.c);
+          d[i] = (Scaled<T16>::value ? y * pw.m : y) * (dp[e] + row_value_at(sv[2 + m], e));
+          p[m][e] = y;
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          uint32_t word = pack_pair<T16>(d[2 * i], d[2 * i + 1]);
+          asm volatile("" : "+v"(word));  // here, not behind the products
+          dd[m][g >> 1][2 * (g & 1) + i] = m ? word ^ flip : word;
+          if (FINE) {
+            const uint32_t lost = pack_pair<T16>(d[2 * i] - T16::to_f32((uint16_t)(word & 0xffff)),
+                                                 d[2 * i + 1] - T16::to_f32((uint16_t)(word >> 16)));
+            dl[m][g >> 1][2 * (g & 1) + i] = m ? lost ^ flip : lost;
           }
         }
+      };
+      __builtin_amdgcn_sched_barrier(0);
+      f[0] = row_frag(s + kUnitB, 0, 0, lo);
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        __builtin_amdgcn_sched_barrier(0);
+        if (g < 3) f[(g + 1) & 1] = row_frag(s + kUnitB, 0, g + 1, lo);
+        p[1] = mfma_32x32x16<T16>(f[g & 1], kf[1][g], p[1]);
+        elements(0, g);
       }
+      mask(p[1]);
+      __builtin_amdgcn_sched_barrier(0);
+      f[0] = col_frag(s, 0, 0, lo);
 #pragma unroll
-      for (int e = 0; e < 16; ++e) p[0][e] -= p[1][e];
+      for (int g = 0; g < 4; ++g) {
+        __builtin_amdgcn_sched_barrier(0);
+        if (g < 3) f[(g + 1) & 1] = col_frag(s, 16 * ((g + 1) >> 1), (g + 1) & 1, lo);
+        ak[0][g & 1] = mfma_32x32x16<T16>(f[g & 1], dd[0][g >> 1], ak[0][g & 1]);
+        if (FINE) ak[0][g & 1] = mfma_32x32x16<T16>(f[g & 1], dl[0][g >> 1], ak[0][g & 1]);
+        elements(1, g);
+      }
+      u32x4 pp[2], pl[2], fv[AHEAD + 1];
+      auto value = [&](int j) __attribute__((always_inline)) {
+        return j < 4 ? col_frag(s + kUnitB, 16 * (j >> 1), j & 1, lo)
+                     : col_frag(s + (2 + ((j & 3) >> 1)) * kUnitB, 16 * ((j - 4) >> 2), j & 1, lo);
+      };
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        const u32x4 pp = pack_step<T16>(p[0], k);
-        u32x4 lost;
-        if (FINE) lost = lost_step<T16>(p[0], k, pp);
+      for (int j = 0; j < AHEAD; ++j) fv[j] = value(j);
 #pragma unroll
-        for (int mb = 0; mb < 4; ++mb) {
-          const u32x4 gf = col_frag(s + (2 + (mb >> 1)) * kUnitB, 16 * k, mb & 1, lo);
-          av[mb] = mfma_32x32x16<T16>(gf, pp, av[mb]);
-          if (FINE) av[mb] = mfma_32x32x16<T16>(gf, lost, av[mb]);
+      for (int j = 0; j < 12; ++j) {
+        __builtin_amdgcn_sched_barrier(0);
+        if (j + AHEAD < 12) fv[(j + AHEAD) % (AHEAD + 1)] = value(j + AHEAD);
+        const int r = j % (AHEAD + 1);
+        if (j < 4) {
+          ak[1][j & 1] = mfma_32x32x16<T16>(fv[r], dd[1][j >> 1], ak[1][j & 1]);
+          if (FINE) ak[1][j & 1] = mfma_32x32x16<T16>(fv[r], dl[1][j >> 1], ak[1][j & 1]);
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const int e = 4 * j + 2 * i;
+            const float x = __builtin_fmaf(-sign, p[1][e], p[0][e]);
+            const float y = __builtin_fmaf(-sign, p[1][e + 1], p[0][e + 1]);
+            uint32_t word = pack_pair<T16>(x, y);
+            asm volatile("" : "+v"(word));
+            pp[j >> 1][2 * (j & 1) + i] = word;
+            if (FINE)
+              pl[j >> 1][2 * (j & 1) + i] =
+                  pack_pair<T16>(x - T16::to_f32((uint16_t)(word & 0xffff)),
+                                 y - T16::to_f32((uint16_t)(word >> 16)));
+          }
+        } else {
+          const int k = (j - 4) >> 2;
+          av[j & 3] = mfma_32x32x16<T16>(fv[r], pp[k], av[j & 3]);
+          if (FINE) av[j & 3] = mfma_32x32x16<T16>(fv[r], pl[k], av[j & 3]);
         }
       }
     }
     ++cu;
     crow += kUnitRows;
-    if (crow >= qlen && cu < u1) crow = first, ++cp;
+    if (crow >= qlen && cu < u1) {
+      crow = first;
+      ++cp;
+      load_weight();
+    }
   };
   load(r0, t0_);
   for (int u = u0; u < u1; u += 2) {
