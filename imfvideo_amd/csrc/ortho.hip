@@ -39,6 +39,7 @@ struct OrthoArgs {
   int64_t n, count;     // matrices, elements of one
   int R, C, r, m, rp, mp, parts;
   bool turn;            // rows of X are G's columns
+  bool wide_out;        // eight neighbours of a row of out can be stored at once
   float a, b, c;
 };
 
@@ -120,18 +121,20 @@ __global__ __launch_bounds__(256) void ortho_split_kernel(OrthoArgs a, int dtype
   const int tm = a.mp / 64, tr = a.rp / 64;
   const int64_t mat = blockIdx.x / (tm * tr);
   const int t = (int)(blockIdx.x - mat * (tm * tr)), i0 = t / tm * 64, j0 = t % tm * 64;
-  const int lane = threadIdx.x & 63;  // (at most 64 parts)
-  const double s = wave_sum(lane < a.parts ? a.sums[mat * a.parts + lane] : 0.0);
-  const double inv = s == 0.0 ? 0.0 : (double)kScaleX / sqrt(s);
   const int q = threadIdx.x & 63, w = threadIdx.x >> 6;
-  // G's rows of the tile, 64 lanes side by side
+  // G's rows of the tile, 64 lanes side by side; all of them under way before the sum is needed
   const int g0 = a.turn ? j0 : i0, h0 = a.turn ? i0 : j0;
-#pragma unroll 4
-  for (int k = w; k < 64; k += 4) {
-    const bool in = g0 + k < a.R && h0 + q < a.C;
-    const int64_t at = mat * a.count + (int64_t)(g0 + k) * a.C + h0 + q;
-    tile[k][q] = in ? (float)((double)load_g(a, dtype, at) * inv) : 0.f;
+  float g[16];
+#pragma unroll
+  for (int k = 0; k < 16; ++k) {
+    const int row = g0 + 4 * k + w;
+    const bool in = row < a.R && h0 + q < a.C;
+    g[k] = in ? load_g(a, dtype, mat * a.count + (int64_t)row * a.C + h0 + q) : 0.f;
   }
+  const double s = wave_sum(q < a.parts ? a.sums[mat * a.parts + q] : 0.0);  // (at most 64 parts)
+  const double inv = s == 0.0 ? 0.0 : (double)kScaleX / sqrt(s);
+#pragma unroll
+  for (int k = 0; k < 16; ++k) tile[4 * k + w][q] = (float)((double)g[k] * inv);
   __syncthreads();
   uint16_t* x = a.x + mat * 2 * a.rp * a.mp;
   const int c = 4 * (threadIdx.x & 15);
@@ -157,6 +160,36 @@ __device__ inline void store_out(const OrthoArgs& a, int dtype, int64_t mat, int
   else
     static_cast<uint16_t*>(a.out)[at] =
         dtype == SLA2H_DTYPE_BF16 ? BF16::from_f32(v) : F16::from_f32(v);
+}
+// Eight neighbours of a row of the result (row u of G, columns c on)
+__device__ inline void store_row8(const OrthoArgs& a, int dtype, int64_t mat, int u, int c,
+                                  const float (&v)[8]) {
+  if (u >= a.R || c >= a.C) return;
+  if (!a.wide_out) {  // (a row's end, or an address, off the 16 bytes)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) store_out(a, dtype, mat, a.turn ? c + e : u, a.turn ? u : c + e, v[e]);
+    return;
+  }
+  const int64_t at = mat * a.count + (int64_t)u * a.C + c;
+  if (dtype == 2) {
+    f32x4* d = reinterpret_cast<f32x4*>(static_cast<float*>(a.out) + at);
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      f32x4 x;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[e] = v[4 * q + e] * (1.f / kScaleX);
+      d[q] = x;
+    }
+    return;
+  }
+  u32x4 x;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const float p = v[2 * e] * (1.f / kScaleX), q = v[2 * e + 1] * (1.f / kScaleX);
+    x[e] = dtype == SLA2H_DTYPE_BF16 ? pack2(BF16::from_f32(p), BF16::from_f32(q))
+                                     : pack2(F16::from_f32(p), F16::from_f32(q));
+  }
+  *reinterpret_cast<u32x4*>(static_cast<uint16_t*>(a.out) + at) = x;
 }
 
 enum { kGram, kPoly, kStep, kLast };
@@ -244,31 +277,40 @@ __global__ __launch_bounds__(256, T == 128 && OP < kStep ? 1 : 2) void ortho_pro
   for (int x = 0; x < NT; ++x)
 #pragma unroll
     for (int y = 0; y < NT; ++y) acc[x][y] = low[x][y] = zero16();
+  struct Frags {
+    u32x4 i[2][NT], j[2][NT];
+  };
+  auto read = [&](const unsigned char* s, int k, Frags& f) __attribute__((always_inline)) {
+#pragma unroll
+    for (int pl = 0; pl < 2; ++pl)
+#pragma unroll
+      for (int x = 0; x < NT; ++x) {
+        const unsigned char* ui = s + (NT * wi + x) * kUnit;
+        const unsigned char* uj = s + (NU + NT * wj + x) * kUnit;
+        f.i[pl][x] = row_frag(ui, 0, 2 * pl + k, lo);
+        f.j[pl][x] = STEP ? turned_frag(uj, k, pl, co) : row_frag(uj, 0, 2 * pl + k, lo);
+      }
+  };
+  auto products = [&](const Frags& f) __attribute__((always_inline)) {
+#pragma unroll
+    for (int x = 0; x < NT; ++x)
+#pragma unroll
+      for (int y = 0; y < NT; ++y) low[x][y] = mfma_32x32x16<F16>(f.j[1][y], f.i[0][x], low[x][y]);
+#pragma unroll
+    for (int x = 0; x < NT; ++x)
+#pragma unroll
+      for (int y = 0; y < NT; ++y) acc[x][y] = mfma_32x32x16<F16>(f.j[0][y], f.i[0][x], acc[x][y]);
+#pragma unroll
+    for (int x = 0; x < NT; ++x)
+#pragma unroll
+      for (int y = 0; y < NT; ++y) low[x][y] = mfma_32x32x16<F16>(f.j[0][y], f.i[1][x], low[x][y]);
+  };
   auto compute = [&](const unsigned char* s) __attribute__((always_inline)) {
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
-      u32x4 fi[2][NT], fj[2][NT];
-#pragma unroll
-      for (int pl = 0; pl < 2; ++pl)
-#pragma unroll
-        for (int x = 0; x < NT; ++x) {
-          const unsigned char* ui = s + (NT * wi + x) * kUnit;
-          const unsigned char* uj = s + (NU + NT * wj + x) * kUnit;
-          fi[pl][x] = row_frag(ui, 0, 2 * pl + k, lo);
-          fj[pl][x] = STEP ? turned_frag(uj, k, pl, co) : row_frag(uj, 0, 2 * pl + k, lo);
-        }
-#pragma unroll
-      for (int x = 0; x < NT; ++x)
-#pragma unroll
-        for (int y = 0; y < NT; ++y) low[x][y] = mfma_32x32x16<F16>(fj[1][y], fi[0][x], low[x][y]);
-#pragma unroll
-      for (int x = 0; x < NT; ++x)
-#pragma unroll
-        for (int y = 0; y < NT; ++y) acc[x][y] = mfma_32x32x16<F16>(fj[0][y], fi[0][x], acc[x][y]);
-#pragma unroll
-      for (int x = 0; x < NT; ++x)
-#pragma unroll
-        for (int y = 0; y < NT; ++y) low[x][y] = mfma_32x32x16<F16>(fj[0][y], fi[1][x], low[x][y]);
+      Frags f;
+      read(s, k, f);
+      products(f);
     }
   };
   // (K is a multiple of 64; a stage's loads: 2 NU per wave)
@@ -285,89 +327,148 @@ __global__ __launch_bounds__(256, T == 128 && OP < kStep ? 1 : 2) void ortho_pro
       compute(s1);
     }
   } else {
-    auto stage = [&](int k0, const unsigned char* cur, unsigned char* to)
+    // half a stage ahead: the operands of one half are read while the other's products run; the
+    // barrier between the halves: the next stage has landed, and this one is read
+    Frags f0, f1;
+    auto stage = [&](int k0, const unsigned char* cur, const unsigned char* next, unsigned char* to)
         __attribute__((always_inline)) {
+      load(k0 + 96, to);
+      read(cur, 1, f1);
+      products(f0);
       __builtin_amdgcn_s_waitcnt(wait_vm_lgkm0(4 * NU));
       __builtin_amdgcn_s_barrier();
-      load(k0 + 96, to);
-      compute(cur);
+      read(next, 0, f0);
+      products(f1);
     };
     load(0, s0);
     load(32, s1);
     load(64, s2);
+    __builtin_amdgcn_s_waitcnt(wait_vm_lgkm0(4 * NU));
+    __builtin_amdgcn_s_barrier();
+    read(s0, 0, f0);
     for (int k0 = 0; k0 < K; k0 += 128) {
-      stage(k0, s0, s3);
-      stage(k0 + 32, s1, s0);
+      stage(k0, s0, s1, s3);
+      stage(k0 + 32, s1, s2, s0);
       if (k0 + 64 >= K) break;
-      stage(k0 + 64, s2, s1);
-      stage(k0 + 96, s3, s2);
+      stage(k0 + 64, s2, s3, s1);
+      stage(k0 + 96, s3, s0, s2);
     }
   }
   __builtin_amdgcn_s_waitcnt(wait_vm_lgkm0(0));  // no load into this LDS outlives the workgroup
+  __builtin_amdgcn_s_barrier();
 
+  // The tile in fp32 in LDS, rows i < T / 2 in s0, the others in s1: from there eight neighbours of a
+  // row, or of a column, to a thread.  The 16-byte units of row i are permuted by its number, so
+  // that 16 columns x 4 groups of eight rows, too, are read from 64 banks.
+  auto unit = [&](int i, int u) __attribute__((always_inline)) {
+    return (i & (T / 2 - 1)) * (4 * T) + 16 * (u ^ ((i & 7) ^ (((i >> 3) & 3) << 2)));
+  };
 #pragma unroll
   for (int x = 0; x < NT; ++x)
 #pragma unroll
     for (int y = 0; y < NT; ++y)
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
-        const int i = it * T + (T / 2) * wi + 32 * x + (l & 31);
-        const int j = jt * T + (T / 2) * wj + 32 * y + 8 * g + 4 * h;
-        if (i >= a.rp || j >= (STEP ? a.mp : a.rp)) continue;
-        float v[4];
+        f32x4 v;
 #pragma unroll
         for (int e = 0; e < 4; ++e) v[e] = acc[x][y][4 * g + e] + low[x][y][4 * g + e];
-        if (OP == kGram) {
+        const int i = 32 * x + (l & 31), u = (T / 8) * wj + 8 * y + 2 * g + h;
+        *reinterpret_cast<f32x4*>((wi ? s1 : s0) + unit(i, u)) = v;
+      }
+  __syncthreads();
+  auto one = [&](int i, int j) __attribute__((always_inline)) {
+    return *reinterpret_cast<const float*>((i >= T / 2 ? s1 : s0) + unit(i, j >> 2) + 4 * (j & 3));
+  };
+  // v: products' sums; hi, lo: eight neighbours of the matrix that the epilogue adds.  (The fused
+  // operations are written out: rows, columns and every T round alike.)
+  auto finish = [&](float (&v)[8], const u32x4& hi, const u32x4& lw) __attribute__((always_inline)) {
+    const float cb = a.b * (kScaleB / kScaleX), cc = a.c * (kScaleB / (kScaleX * kScaleX));
 #pragma unroll
-          for (int e = 0; e < 4; ++e) v[e] *= 1.f / kScaleX;
-        } else if (OP == kPoly) {
-          const uint16_t* s = A + pair_index(i, j, a.rp);
-          const u32x2 p = *reinterpret_cast<const u32x2*>(s);
-          const u32x2 q = *reinterpret_cast<const u32x2*>(s + 32);
+    for (int e = 0; e < 8; ++e) {
+      const float p = OP == kGram ? 0.f : pair_at(hi[e >> 1], lw[e >> 1], e & 1);
+      v[e] = OP == kGram   ? v[e] * (1.f / kScaleX)
+             : OP == kPoly ? __builtin_fmaf(cc, v[e], cb * p)
+                           : __builtin_fmaf(a.a, p, (1.f / kScaleB) * v[e]);
+    }
+  };
+  auto store_pairs = [&](uint16_t* d, const float (&v)[8]) __attribute__((always_inline)) {
+    u32x4 hi, lw;
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            v[e] = a.c * (kScaleB / (kScaleX * kScaleX)) * v[e] +
-                   a.b * (kScaleB / kScaleX) * pair_at(p[e >> 1], q[e >> 1], e & 1);
-        } else {
-          const uint16_t* s = X + pair_index(i, j, a.mp);
-          const u32x2 p = *reinterpret_cast<const u32x2*>(s);
-          const u32x2 q = *reinterpret_cast<const u32x2*>(s + 32);
+    for (int e = 0; e < 4; ++e) {
+      uint16_t l0, l1;
+      const uint16_t h0 = split_hi(v[2 * e], l0), h1 = split_hi(v[2 * e + 1], l1);
+      hi[e] = pack2(h0, h1);
+      lw[e] = pack2(l0, l1);
+    }
+    *reinterpret_cast<u32x4*>(d) = hi;
+    *reinterpret_cast<u32x4*>(d + 32) = lw;
+  };
+  uint16_t* base = OP == kGram ? a.A + mat * pa : OP == kPoly ? a.B + mat * pa : a.y + mat * px;
+  const int ld = STEP ? a.mp : a.rp;
+  // rows: T / 8 threads each
+  const bool diagonal = !STEP && it == jt, columns = OP == kLast && a.turn;
+  if (!columns) {
+#pragma unroll 4
+    for (int k = tid; k < T * T / 8; k += 256) {
+      const int il = k / (T / 8), jl = 8 * (k % (T / 8)), i = it * T + il, j = jt * T + jl;
+      if (i >= a.rp || j >= ld) continue;
+      u32x4 hi{}, lw{};
+      if (OP != kGram) {
+        const uint16_t* s = OP == kPoly ? A + pair_index(i, j, ld) : X + pair_index(i, j, ld);
+        hi = *reinterpret_cast<const u32x4*>(s);
+        lw = *reinterpret_cast<const u32x4*>(s + 32);
+      }
+      float v[8];
+      if (diagonal) {  // the elements above the diagonal for both sides: symmetric to the bit
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            v[e] = (1.f / kScaleB) * v[e] + a.a * pair_at(p[e >> 1], q[e >> 1], e & 1);
-        }
-        if (OP == kLast) {
+        for (int e = 0; e < 8; ++e) v[e] = jl + e < il ? one(jl + e, il) : one(il, jl + e);
+      } else {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) store_out(a, dtype, mat, i, j + e, v[e]);
-          continue;
-        }
-        u32x2 hi, lw;
-        split4(v, hi, lw);
-        uint16_t* base = OP == kGram ? a.A + mat * pa : OP == kPoly ? a.B + mat * pa
-                                                                    : a.y + mat * px;
-        const int ld = STEP ? a.mp : a.rp;
-        uint16_t* d = base + pair_index(i, j, ld);
-        if (STEP || it != jt) {
-          *reinterpret_cast<u32x2*>(d) = hi;
-          *reinterpret_cast<u32x2*>(d + 32) = lw;
-        }
-        if (STEP) continue;
-        // below the diagonal too (within a tile on it the elements above are the ones kept, so
-        // that the matrix is symmetric to the bit, whatever the tiles)
+        for (int q = 0; q < 2; ++q) {
+          const f32x4 z = *reinterpret_cast<const f32x4*>((il >= T / 2 ? s1 : s0) + unit(il, jl / 4 + q));
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          if (it == jt && j + e < i) continue;
-          const uint16_t x0 = (uint16_t)(hi[e >> 1] >> (16 * (e & 1)));
-          const uint16_t x1 = (uint16_t)(lw[e >> 1] >> (16 * (e & 1)));
-          uint16_t* d2 = base + pair_index(j + e, i, ld);
-          d2[0] = x0;
-          d2[32] = x1;
-          if (it == jt) {
-            d[e] = x0;
-            d[e + 32] = x1;
-          }
+          for (int e = 0; e < 4; ++e) v[4 * q + e] = z[e];
         }
       }
+      finish(v, hi, lw);
+      if (OP == kLast)
+        store_row8(a, dtype, mat, i, j, v);
+      else
+        store_pairs(base + pair_index(i, j, ld), v);
+    }
+  }
+  // columns, eight rows to a thread, 16 columns x 32 rows to a wave: the tile below the diagonal
+  // (A is symmetric: the same neighbours), or the result of a G whose columns are X's rows
+  if (columns || (!STEP && !diagonal)) {
+#pragma unroll 4
+    for (int k = w; k < T * T / 512; k += 4) {
+      const int il = 32 * (k / (T / 16)) + 8 * (l & 3), jl = 16 * (k % (T / 16)) + (l >> 2);
+      const int i = it * T + il, j = jt * T + jl;
+      if (i >= a.rp || j >= ld) continue;
+      float v[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = one(il + e, jl);
+      u32x4 hi{}, lw{};
+      if (OP == kPoly) {
+        const uint16_t* s = A + pair_index(j, i, ld);
+        hi = *reinterpret_cast<const u32x4*>(s);
+        lw = *reinterpret_cast<const u32x4*>(s + 32);
+      }
+      if (OP == kLast) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const uint16_t* s = X + pair_index(i + e, j, ld);
+          hi[e >> 1] |= (uint32_t)s[0] << (16 * (e & 1));
+          lw[e >> 1] |= (uint32_t)s[32] << (16 * (e & 1));
+        }
+      }
+      finish(v, hi, lw);
+      if (OP == kLast)
+        store_row8(a, dtype, mat, j, i, v);
+      else
+        store_pairs(base + pair_index(j, i, ld), v);
+    }
+  }
 }
 
 // Small matrices (r <= 64, m <= 512): all steps of a matrix in one workgroup, X (at most 128 KB) and A,
@@ -590,6 +691,7 @@ extern "C" int sla2h_orthogonalize(const void* g, int dtype, int64_t n, int64_t 
   a.n = n, a.count = R * C;
   a.R = (int)R, a.C = (int)C, a.r = p.r, a.m = p.m, a.rp = p.rp, a.mp = p.mp, a.parts = p.parts;
   a.turn = R > C;
+  a.wide_out = C % 8 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0;
   hipStream_t st = static_cast<hipStream_t>(stream);
   int err;
   if (p.r <= 64 && p.m <= kSmallM) {
