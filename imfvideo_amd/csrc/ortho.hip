@@ -260,9 +260,9 @@ __global__ __launch_bounds__(256, T == 128 && OP < kStep ? 1 : 2) void ortho_pro
 
   // unit u of a stage: rows 32 u .. of the operand along the lanes, then the other one's; wave w loads
   // rows 8 w .. of each (rows and columns past the matrix: zeros)
-  auto load = [&](int k0, unsigned char* s) __attribute__((always_inline)) {
+  auto load = [&](int k0, unsigned char* s, int u0, int u1) __attribute__((always_inline)) {
 #pragma unroll
-    for (int u = 0; u < NU; ++u) {
+    for (int u = u0; u < u1; ++u) {
       const int i = it * T + 32 * u, j = jt * T + 32 * u;
       const auto ri = rows_rsrc(P + 2 * k0, i, k0 < K && i < a.rp ? 32 : 0, ldp);
       const auto rj = STEP ? rows_rsrc(X + 2 * j, k0, k0 < K && j < a.mp ? 32 : 0, ldx)
@@ -280,50 +280,69 @@ __global__ __launch_bounds__(256, T == 128 && OP < kStep ? 1 : 2) void ortho_pro
   struct Frags {
     u32x4 i[2][NT], j[2][NT];
   };
-  auto read = [&](const unsigned char* s, int k, Frags& f) __attribute__((always_inline)) {
+  auto read_i = [&](const unsigned char* s, int k, int pl, Frags& f) __attribute__((always_inline)) {
 #pragma unroll
-    for (int pl = 0; pl < 2; ++pl)
-#pragma unroll
-      for (int x = 0; x < NT; ++x) {
-        const unsigned char* ui = s + (NT * wi + x) * kUnit;
-        const unsigned char* uj = s + (NU + NT * wj + x) * kUnit;
-        f.i[pl][x] = row_frag(ui, 0, 2 * pl + k, lo);
-        f.j[pl][x] = STEP ? turned_frag(uj, k, pl, co) : row_frag(uj, 0, 2 * pl + k, lo);
-      }
+    for (int x = 0; x < NT; ++x) f.i[pl][x] = row_frag(s + (NT * wi + x) * kUnit, 0, 2 * pl + k, lo);
   };
-  auto products = [&](const Frags& f) __attribute__((always_inline)) {
+  auto read_j = [&](const unsigned char* s, int k, int pl, Frags& f) __attribute__((always_inline)) {
+#pragma unroll
+    for (int x = 0; x < NT; ++x) {
+      const unsigned char* u = s + (NU + NT * wj + x) * kUnit;
+      f.j[pl][x] = STEP ? turned_frag(u, k, pl, co) : row_frag(u, 0, 2 * pl + k, lo);
+    }
+  };
+  auto products = [&](const Frags& f, int pj, int pi, f32x16 (&to)[NT][NT])
+      __attribute__((always_inline)) {
 #pragma unroll
     for (int x = 0; x < NT; ++x)
 #pragma unroll
-      for (int y = 0; y < NT; ++y) low[x][y] = mfma_32x32x16<F16>(f.j[1][y], f.i[0][x], low[x][y]);
-#pragma unroll
-    for (int x = 0; x < NT; ++x)
-#pragma unroll
-      for (int y = 0; y < NT; ++y) acc[x][y] = mfma_32x32x16<F16>(f.j[0][y], f.i[0][x], acc[x][y]);
-#pragma unroll
-    for (int x = 0; x < NT; ++x)
-#pragma unroll
-      for (int y = 0; y < NT; ++y) low[x][y] = mfma_32x32x16<F16>(f.j[0][y], f.i[1][x], low[x][y]);
+      for (int y = 0; y < NT; ++y) to[x][y] = mfma_32x32x16<F16>(f.j[pj][y], f.i[pi][x], to[x][y]);
   };
   auto compute = [&](const unsigned char* s) __attribute__((always_inline)) {
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
       Frags f;
-      read(s, k, f);
-      products(f);
+#pragma unroll
+      for (int pl = 0; pl < 2; ++pl) {
+        read_i(s, k, pl, f);
+        read_j(s, k, pl, f);
+      }
+      products(f, 1, 0, low);
+      products(f, 0, 0, acc);
+      products(f, 0, 1, low);
     }
+  };
+  // the same, while the operands of the next half stage are read (and, where k is 1, a stage's loads
+  // issued): in this order
+  auto half = [&](const Frags& f, const unsigned char* s, int k, Frags& next, int k0,
+                  unsigned char* to) __attribute__((always_inline)) {
+    read_i(s, k, 0, next);
+    read_j(s, k, 1, next);
+    __builtin_amdgcn_sched_barrier(0);
+    products(f, 1, 0, low);
+    __builtin_amdgcn_sched_barrier(0);
+    read_j(s, k, 0, next);
+    if (k) load(k0, to, 0, NU / 2);
+    __builtin_amdgcn_sched_barrier(0);
+    products(f, 0, 0, acc);
+    __builtin_amdgcn_sched_barrier(0);
+    read_i(s, k, 1, next);
+    if (k) load(k0, to, NU / 2, NU);
+    __builtin_amdgcn_sched_barrier(0);
+    products(f, 0, 1, low);
+    __builtin_amdgcn_sched_barrier(0);
   };
   // (K is a multiple of 64; a stage's loads: 2 NU per wave)
   if (!DEEP) {
-    load(0, s0);
+    load(0, s0, 0, NU);
     for (int k0 = 0; k0 < K; k0 += 64) {
       __builtin_amdgcn_s_waitcnt(wait_vm_lgkm0(0));
       __builtin_amdgcn_s_barrier();  // the stage has landed, the one before is read
-      load(k0 + 32, s1);
+      load(k0 + 32, s1, 0, NU);
       compute(s0);
       __builtin_amdgcn_s_waitcnt(wait_vm_lgkm0(0));
       __builtin_amdgcn_s_barrier();
-      load(k0 + 64, s0);
+      load(k0 + 64, s0, 0, NU);
       compute(s1);
     }
   } else {
@@ -332,26 +351,31 @@ __global__ __launch_bounds__(256, T == 128 && OP < kStep ? 1 : 2) void ortho_pro
     Frags f0, f1;
     auto stage = [&](int k0, const unsigned char* cur, const unsigned char* next, unsigned char* to)
         __attribute__((always_inline)) {
-      load(k0 + 96, to);
-      read(cur, 1, f1);
-      products(f0);
+      half(f0, cur, 1, f1, k0 + 96, to);
       __builtin_amdgcn_s_waitcnt(wait_vm_lgkm0(4 * NU));
       __builtin_amdgcn_s_barrier();
-      read(next, 0, f0);
-      products(f1);
+      half(f1, next, 0, f0, 0, to);
     };
-    load(0, s0);
-    load(32, s1);
-    load(64, s2);
+    load(0, s0, 0, NU);
+    load(32, s1, 0, NU);
+    load(64, s2, 0, NU);
     __builtin_amdgcn_s_waitcnt(wait_vm_lgkm0(4 * NU));
     __builtin_amdgcn_s_barrier();
-    read(s0, 0, f0);
-    for (int k0 = 0; k0 < K; k0 += 128) {
+#pragma unroll
+    for (int pl = 0; pl < 2; ++pl) {
+      read_i(s0, 0, pl, f0);
+      read_j(s0, 0, pl, f0);
+    }
+    int k0 = 0;
+    for (; k0 + 64 < K; k0 += 128) {
       stage(k0, s0, s1, s3);
       stage(k0 + 32, s1, s2, s0);
-      if (k0 + 64 >= K) break;
       stage(k0 + 64, s2, s3, s1);
       stage(k0 + 96, s3, s0, s2);
+    }
+    if (k0 < K) {
+      stage(k0, s0, s1, s3);
+      stage(k0 + 32, s1, s2, s0);
     }
   }
   __builtin_amdgcn_s_waitcnt(wait_vm_lgkm0(0));  // no load into this LDS outlives the workgroup
