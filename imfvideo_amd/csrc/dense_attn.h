@@ -51,9 +51,9 @@ __device__ inline f32x16 zero16() {
   return z;
 }
 
-__device__ inline void dma16(__amdgpu_buffer_rsrc_t rs, void* dst, int voff) {
+__device__ inline void dma16(__amdgpu_buffer_rsrc_t rs, void* dst, int voff, int soff = 0) {
   __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (__attribute__((address_space(3))) void*)dst, 16,
-                                           voff, 0, 0, 0);
+                                           voff, soff, 0, 0);
 }
 
 // Rows [row0, row0 + n) of a (rows, 64) 16-bit matrix with row stride `ld` bytes as

@@ -235,7 +235,7 @@ __global__ __launch_bounds__(256, T == 128 && OP < kStep ? 1 : 2) void ortho_pro
   if (item >= work) return;
   const int ti = (a.rp + T - 1) / T, tj = STEP ? (a.mp + T - 1) / T : ti;
   const int tiles = STEP ? ti * tj : ti * (ti + 1) / 2;
-  const int mat = item / tiles;
+  const int mat = __builtin_amdgcn_readfirstlane(item / tiles);
   int t = item - mat * tiles, it = 0, jt;
   if (STEP) {
     it = t % ti;
@@ -258,17 +258,30 @@ __global__ __launch_bounds__(256, T == 128 && OP < kStep ? 1 : 2) void ortho_pro
   const int ldp = (OP == kGram ? a.mp : a.rp) * 4, ldx = a.mp * 4;         // bytes
   const int K = OP == kGram ? a.mp : a.rp;
 
-  // unit u of a stage: rows 32 u .. of the operand along the lanes, then the other one's; wave w loads
-  // rows 8 w .. of each (rows and columns past the matrix: zeros)
+  // Unit u of a stage: rows 32 u .. of the operand along the lanes, then the other one's; wave w loads
+  // rows 8 w .. of each.  Rows past the matrix: zeros; columns past it: what stands there, for results
+  // that are not stored; a stage past K: the last one again, for no product.
+  const int r = 8 * w + (l >> 3), ch = ((l & 7) ^ row_key(r)) << 4;
+  int vi[NU], vj[NU];  // a lane's places in an operand
+#pragma unroll
+  for (int u = 0; u < NU; ++u) {
+    vi[u] = (32 * u + r) * ldp + ch;
+    vj[u] = STEP ? r * ldx + 128 * u + ch : vi[u];
+  }
+  auto rows_of = [&](int t) __attribute__((always_inline)) {
+    const int n = a.rp - t * T < T ? a.rp - t * T : T;
+    return make_rsrc(reinterpret_cast<const char*>(P) + (int64_t)t * T * ldp, (int64_t)n * ldp);
+  };
+  const auto ri = rows_of(it), rk = rows_of(STEP ? it : jt);
   auto load = [&](int k0, unsigned char* s, int u0, int u1) __attribute__((always_inline)) {
+    const int k = k0 < K ? k0 : K - 32;
+    const auto rj = STEP ? make_rsrc(reinterpret_cast<const char*>(X) + (int64_t)k * ldx + 4 * T * jt,
+                                     (int64_t)31 * ldx + 4 * (a.mp - T * jt))
+                         : rk;
 #pragma unroll
     for (int u = u0; u < u1; ++u) {
-      const int i = it * T + 32 * u, j = jt * T + 32 * u;
-      const auto ri = rows_rsrc(P + 2 * k0, i, k0 < K && i < a.rp ? 32 : 0, ldp);
-      const auto rj = STEP ? rows_rsrc(X + 2 * j, k0, k0 < K && j < a.mp ? 32 : 0, ldx)
-                           : rows_rsrc(P + 2 * k0, j, k0 < K && j < a.rp ? 32 : 0, ldp);
-      dma_rows8(ri, s + u * kUnit, w, ldp, l);
-      dma_rows8(rj, s + (NU + u) * kUnit, w, STEP ? ldx : ldp, l);
+      dma16(ri, s + u * kUnit + 8 * w * kRowB, vi[u], 4 * k);
+      dma16(rj, s + (NU + u) * kUnit + 8 * w * kRowB, vj[u], STEP ? 0 : 4 * k);
     }
   };
 
@@ -291,12 +304,11 @@ __global__ __launch_bounds__(256, T == 128 && OP < kStep ? 1 : 2) void ortho_pro
       f.j[pl][x] = STEP ? turned_frag(u, k, pl, co) : row_frag(u, 0, 2 * pl + k, lo);
     }
   };
-  auto products = [&](const Frags& f, int pj, int pi, f32x16 (&to)[NT][NT])
+  // row x of the wave's tiles
+  auto products = [&](const Frags& f, int pj, int pi, int x, f32x16 (&to)[NT][NT])
       __attribute__((always_inline)) {
 #pragma unroll
-    for (int x = 0; x < NT; ++x)
-#pragma unroll
-      for (int y = 0; y < NT; ++y) to[x][y] = mfma_32x32x16<F16>(f.j[pj][y], f.i[pi][x], to[x][y]);
+    for (int y = 0; y < NT; ++y) to[x][y] = mfma_32x32x16<F16>(f.j[pj][y], f.i[pi][x], to[x][y]);
   };
   auto compute = [&](const unsigned char* s) __attribute__((always_inline)) {
 #pragma unroll
@@ -307,30 +319,35 @@ __global__ __launch_bounds__(256, T == 128 && OP < kStep ? 1 : 2) void ortho_pro
         read_i(s, k, pl, f);
         read_j(s, k, pl, f);
       }
-      products(f, 1, 0, low);
-      products(f, 0, 0, acc);
-      products(f, 0, 1, low);
+#pragma unroll
+      for (int x = 0; x < NT; ++x) products(f, 1, 0, x, low);
+#pragma unroll
+      for (int x = 0; x < NT; ++x) products(f, 0, 0, x, acc);
+#pragma unroll
+      for (int x = 0; x < NT; ++x) products(f, 0, 1, x, low);
     }
   };
-  // the same, while the operands of the next half stage are read (and, where k is 1, a stage's loads
-  // issued): in this order
+  // The same, while the operands of the next half stage are read and, where k is 1, a stage's loads
+  // issued: a wave issues in order, so that what stands between two products takes their time unless
+  // it is less than one of them.
   auto half = [&](const Frags& f, const unsigned char* s, int k, Frags& next, int k0,
                   unsigned char* to) __attribute__((always_inline)) {
-    read_i(s, k, 0, next);
-    read_j(s, k, 1, next);
-    __builtin_amdgcn_sched_barrier(0);
-    products(f, 1, 0, low);
-    __builtin_amdgcn_sched_barrier(0);
-    read_j(s, k, 0, next);
-    if (k) load(k0, to, 0, NU / 2);
-    __builtin_amdgcn_sched_barrier(0);
-    products(f, 0, 0, acc);
-    __builtin_amdgcn_sched_barrier(0);
-    read_i(s, k, 1, next);
-    if (k) load(k0, to, NU / 2, NU);
-    __builtin_amdgcn_sched_barrier(0);
-    products(f, 0, 1, low);
-    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int z = 0; z < 3 * NT; ++z) {
+      if (z == 0) read_i(s, k, 0, next);
+      if (z == NT - 1) read_j(s, k, 1, next);
+      if (z == NT) read_j(s, k, 0, next);
+      if (z == 2 * NT - 1 + (NT == 1)) read_i(s, k, 1, next);
+      if (k && z < NU) load(k0, to, z, z + 1);
+      __builtin_amdgcn_sched_barrier(0);
+      if (z < NT)
+        products(f, 1, 0, z, low);
+      else if (z < 2 * NT)
+        products(f, 0, 0, z - NT, acc);
+      else
+        products(f, 0, 1, z - 2 * NT, low);
+      __builtin_amdgcn_sched_barrier(0);
+    }
   };
   // (K is a multiple of 64; a stage's loads: 2 NU per wave)
   if (!DEEP) {
