@@ -95,23 +95,37 @@ __global__ __launch_bounds__(256) void ortho_norm_kernel(OrthoArgs a, int dtype,
   if (threadIdx.x == 0) a.sums[blockIdx.x] = (red[0] + red[1]) + (red[2] + red[3]);
 }
 
-// hi and lo of a scaled value
-__device__ inline uint16_t split_hi(float v, uint16_t& lo) {
-  const uint16_t hi = F16::from_f32(v);
-  lo = F16::from_f32(v - F16::to_f32(hi));
-  return hi;
+// x plus, or minus, half E of a packed pair of fp16 numbers: one instruction that widens as it reads
+template <int E>
+__device__ inline float minus_half(float x, uint32_t p) {
+  float d;
+  if (E)
+    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(d) : "v"(p), "v"(x));
+  else
+    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(d) : "v"(p), "v"(x));
+  return d;
+}
+__device__ inline float pair_at(uint32_t hi, uint32_t lo, int e) {
+  float d;
+  if (e)
+    asm("v_fma_mix_f32 %0, %1, 1.0, %2 op_sel:[1,0,1] op_sel_hi:[1,0,1]" : "=v"(d) : "v"(hi), "v"(lo));
+  else
+    asm("v_fma_mix_f32 %0, %1, 1.0, %2 op_sel_hi:[1,0,1]" : "=v"(d) : "v"(hi), "v"(lo));
+  return d;
+}
+// hi and lo of two scaled values
+__device__ inline void split2(float x, float y, uint32_t& hi, uint32_t& lo) {
+  hi = pack_pair<F16>(x, y);
+  lo = pack_pair<F16>(minus_half<0>(x, hi), minus_half<1>(y, hi));
 }
 __device__ inline void split4(const float (&v)[4], u32x2& hi, u32x2& lo) {
 #pragma unroll
   for (int e = 0; e < 2; ++e) {
-    uint16_t l0, l1;
-    const uint16_t h0 = split_hi(v[2 * e], l0), h1 = split_hi(v[2 * e + 1], l1);
-    hi[e] = pack2(h0, h1);
-    lo[e] = pack2(l0, l1);
+    uint32_t a, b;
+    split2(v[2 * e], v[2 * e + 1], a, b);
+    hi[e] = a;
+    lo[e] = b;
   }
-}
-__device__ inline float pair_at(uint32_t hi, uint32_t lo, int e) {
-  return F16::to_f32((uint16_t)(hi >> (16 * e))) + F16::to_f32((uint16_t)(lo >> (16 * e)));
 }
 
 // X of the first step, zeros up to the padded sizes; a 64 x 64 tile per workgroup, turned through
@@ -125,11 +139,22 @@ __global__ __launch_bounds__(256) void ortho_split_kernel(OrthoArgs a, int dtype
   // G's rows of the tile, 64 lanes side by side; all of them under way before the sum is needed
   const int g0 = a.turn ? j0 : i0, h0 = a.turn ? i0 : j0;
   float g[16];
+  uint16_t raw[16];
+  const int64_t first = mat * a.count + (int64_t)(g0 + w) * a.C + h0 + q;
+  const bool in = h0 + q < a.C;
+  if (dtype == 2) {
 #pragma unroll
-  for (int k = 0; k < 16; ++k) {
-    const int row = g0 + 4 * k + w;
-    const bool in = row < a.R && h0 + q < a.C;
-    g[k] = in ? load_g(a, dtype, mat * a.count + (int64_t)row * a.C + h0 + q) : 0.f;
+    for (int k = 0; k < 16; ++k)
+      g[k] = in && g0 + w + 4 * k < a.R
+                 ? static_cast<const float*>(a.g)[first + (int64_t)(4 * k) * a.C] : 0.f;
+  } else {
+#pragma unroll
+    for (int k = 0; k < 16; ++k)
+      raw[k] = in && g0 + w + 4 * k < a.R
+                   ? static_cast<const uint16_t*>(a.g)[first + (int64_t)(4 * k) * a.C] : (uint16_t)0;
+#pragma unroll
+    for (int k = 0; k < 16; ++k)
+      g[k] = dtype == SLA2H_DTYPE_BF16 ? BF16::to_f32(raw[k]) : F16::to_f32(raw[k]);
   }
   const double s = wave_sum(q < a.parts ? a.sums[mat * a.parts + q] : 0.0);  // (at most 64 parts)
   const double inv = s == 0.0 ? 0.0 : (double)kScaleX / sqrt(s);
@@ -213,11 +238,14 @@ __device__ inline u32x4 turned_frag(const unsigned char* tile, int s, int mb, co
 
 // One product, T x T tiles, a workgroup of 2 x 2 waves per tile.  A stage contracts 32 channels: T rows
 // of 128 bytes, hi and lo, of the operand along the lanes and as much of the other one (kStep: 32 rows
-// of T columns, read transposed); T = 128 two LDS slots of 32 KB, T = 64 four of 16 KB, loaded
-// one and three stages ahead: two workgroups per CU, so that one's first loads and its
-// epilogue run beside the other's products (one workgroup with 64 channels a stage: 24 x 512 x
-// 2048, kStep 174 us).  Result element (i, j): j along the registers, i along the lanes, so that four
-// neighbours of a row are stored at once.
+// of T columns, read transposed).  The steps of T = 128: two LDS slots of 32 KB, one stage ahead, two
+// workgroups per CU, so that one's first loads and its epilogue run beside the other's products (one
+// workgroup with 64 channels a stage: 24 x 512 x 2048, kStep 174 us for 84).  The others: four slots,
+// three stages ahead, the operands of half a stage read beside the products of the half before (left to
+// the compiler's order: 24 x 512 x 2048, kGram 63 us for 48).  Result element (i, j): j along the
+// registers, i along the lanes; it goes through LDS, so that whole rows are stored (from the registers,
+// eight bytes to a row: kStep 105 us, kGram 65).  24 x 512 x 2048: kGram 1.0, kStep 0.92 PFLOP/s of
+// 16-bit products, with 200 MB read and written beside kStep's.
 //   kGram: A = X X^T;  kPoly: B = b A + c A A^T;  kStep: Y = a X + B X;  kLast: that, to G's type
 template <int T, int OP>
 __global__ __launch_bounds__(256, T == 128 && OP < kStep ? 1 : 2) void ortho_product_kernel(
@@ -284,6 +312,26 @@ __global__ __launch_bounds__(256, T == 128 && OP < kStep ? 1 : 2) void ortho_pro
       dma16(rj, s + (NU + u) * kUnit + 8 * w * kRowB, vj[u], STEP ? 0 : 4 * k);
     }
   };
+
+  // The epilogue's share of a thread: rows, T / 8 threads each, kPass of them at once.  The matrix that
+  // is added is on its way while something else is done (T = 64: from the start).
+  constexpr int kRows = 2048 / T, kPass = T == 64 ? 2 : 4;
+  const int ld = STEP ? a.mp : a.rp;
+  const int ni = a.rp - it * T < T ? a.rp - it * T : T, nj = ld - jt * T < T ? ld - jt * T : T;
+  const bool diagonal = !STEP && it == jt, columns = OP == kLast && a.turn;
+  const int il = tid / (T / 8), jl = 8 * (tid % (T / 8));
+  u32x4 ph[kPass]{}, pl[kPass]{};
+  auto fetch = [&](int p0) __attribute__((always_inline)) {
+    if (OP == kGram || p0 * kRows >= ni || jl >= nj) return;
+#pragma unroll
+    for (int p = 0; p < kPass; ++p) {
+      const uint16_t* s = (OP == kPoly ? A : X) +
+                          pair_index(it * T + il + (p0 + p) * kRows, jt * T + jl, ld);
+      ph[p] = *reinterpret_cast<const u32x4*>(s);
+      pl[p] = *reinterpret_cast<const u32x4*>(s + 32);
+    }
+  };
+  if (T == 64) fetch(0);
 
   f32x16 acc[NT][NT], low[NT][NT];  // hi hi, and the two cross products
 #pragma unroll
@@ -404,6 +452,10 @@ __global__ __launch_bounds__(256, T == 128 && OP < kStep ? 1 : 2) void ortho_pro
   auto unit = [&](int i, int u) __attribute__((always_inline)) {
     return (i & (T / 2 - 1)) * (4 * T) + 16 * (u ^ ((i & 7) ^ (((i >> 3) & 3) << 2)));
   };
+  auto one = [&](int i, int j) __attribute__((always_inline)) {
+    return reinterpret_cast<float*>((i >= T / 2 ? s1 : s0) + unit(i, j >> 2) + 4 * (j & 3));
+  };
+  if (T == 128) fetch(0);
 #pragma unroll
   for (int x = 0; x < NT; ++x)
 #pragma unroll
@@ -413,13 +465,20 @@ __global__ __launch_bounds__(256, T == 128 && OP < kStep ? 1 : 2) void ortho_pro
         f32x4 v;
 #pragma unroll
         for (int e = 0; e < 4; ++e) v[e] = acc[x][y][4 * g + e] + low[x][y][4 * g + e];
-        const int i = 32 * x + (l & 31), u = (T / 8) * wj + 8 * y + 2 * g + h;
-        *reinterpret_cast<f32x4*>((wi ? s1 : s0) + unit(i, u)) = v;
+        const int i = (T / 2) * wi + 32 * x + (l & 31), j = (T / 2) * wj + 32 * y + 8 * g + 4 * h;
+        if (!diagonal) {
+          *reinterpret_cast<f32x4*>(one(i, j)) = v;
+          continue;
+        }
+        // the elements above the diagonal for both sides: symmetric to the bit
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (i <= j + e) {
+            *one(i, j + e) = v[e];
+            *one(j + e, i) = v[e];
+          }
       }
   __syncthreads();
-  auto one = [&](int i, int j) __attribute__((always_inline)) {
-    return *reinterpret_cast<const float*>((i >= T / 2 ? s1 : s0) + unit(i, j >> 2) + 4 * (j & 3));
-  };
   // v: products' sums; hi, lo: eight neighbours of the matrix that the epilogue adds.  (The fused
   // operations are written out: rows, columns and every T round alike.)
   auto finish = [&](float (&v)[8], const u32x4& hi, const u32x4& lw) __attribute__((always_inline)) {
@@ -436,80 +495,71 @@ __global__ __launch_bounds__(256, T == 128 && OP < kStep ? 1 : 2) void ortho_pro
     u32x4 hi, lw;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      uint16_t l0, l1;
-      const uint16_t h0 = split_hi(v[2 * e], l0), h1 = split_hi(v[2 * e + 1], l1);
-      hi[e] = pack2(h0, h1);
-      lw[e] = pack2(l0, l1);
+      uint32_t x, y;
+      split2(v[2 * e], v[2 * e + 1], x, y);
+      hi[e] = x;
+      lw[e] = y;
     }
     *reinterpret_cast<u32x4*>(d) = hi;
     *reinterpret_cast<u32x4*>(d + 32) = lw;
   };
   uint16_t* base = OP == kGram ? a.A + mat * pa : OP == kPoly ? a.B + mat * pa : a.y + mat * px;
-  const int ld = STEP ? a.mp : a.rp;
-  // rows: T / 8 threads each
-  const bool diagonal = !STEP && it == jt, columns = OP == kLast && a.turn;
-  if (!columns) {
-#pragma unroll 4
-    for (int k = tid; k < T * T / 8; k += 256) {
-      const int il = k / (T / 8), jl = 8 * (k % (T / 8)), i = it * T + il, j = jt * T + jl;
-      if (i >= a.rp || j >= ld) continue;
-      u32x4 hi{}, lw{};
-      if (OP != kGram) {
-        const uint16_t* s = OP == kPoly ? A + pair_index(i, j, ld) : X + pair_index(i, j, ld);
-        hi = *reinterpret_cast<const u32x4*>(s);
-        lw = *reinterpret_cast<const u32x4*>(s + 32);
-      }
-      float v[8];
-      if (diagonal) {  // the elements above the diagonal for both sides: symmetric to the bit
+  if (jl < nj)
+    for (int p0 = 0; p0 * kRows < ni; p0 += kPass) {
+      float v[kPass][8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = jl + e < il ? one(jl + e, il) : one(il, jl + e);
-      } else {
+      for (int p = 0; p < kPass; ++p) {
 #pragma unroll
         for (int q = 0; q < 2; ++q) {
-          const f32x4 z = *reinterpret_cast<const f32x4*>((il >= T / 2 ? s1 : s0) + unit(il, jl / 4 + q));
+          const f32x4 z = *reinterpret_cast<const f32x4*>(one(il + (p0 + p) * kRows, jl + 4 * q));
 #pragma unroll
-          for (int e = 0; e < 4; ++e) v[4 * q + e] = z[e];
+          for (int e = 0; e < 4; ++e) v[p][4 * q + e] = z[e];
         }
       }
-      finish(v, hi, lw);
-      if (OP == kLast)
-        store_row8(a, dtype, mat, i, j, v);
-      else
-        store_pairs(base + pair_index(i, j, ld), v);
+#pragma unroll
+      for (int p = 0; p < kPass; ++p) finish(v[p], ph[p], pl[p]);
+      fetch(p0 + kPass);
+#pragma unroll
+      for (int p = 0; p < kPass; ++p) {
+        const int i = it * T + il + (p0 + p) * kRows, j = jt * T + jl;
+        if (columns) {  // back to its place
+#pragma unroll
+          for (int q = 0; q < 2; ++q)
+            *reinterpret_cast<f32x4*>(one(il + (p0 + p) * kRows, jl + 4 * q)) =
+                f32x4{v[p][4 * q], v[p][4 * q + 1], v[p][4 * q + 2], v[p][4 * q + 3]};
+        } else if (OP == kLast) {
+          store_row8(a, dtype, mat, i, j, v[p]);
+        } else {
+          store_pairs(base + pair_index(i, j, ld), v[p]);
+        }
+      }
     }
-  }
+  if (columns) __syncthreads();
   // columns, eight rows to a thread, 16 columns x 32 rows to a wave: the tile below the diagonal
   // (A is symmetric: the same neighbours), or the result of a G whose columns are X's rows
-  if (columns || (!STEP && !diagonal)) {
-#pragma unroll 4
-    for (int k = w; k < T * T / 512; k += 4) {
-      const int il = 32 * (k / (T / 16)) + 8 * (l & 3), jl = 16 * (k % (T / 16)) + (l >> 2);
-      const int i = it * T + il, j = jt * T + jl;
-      if (i >= a.rp || j >= ld) continue;
-      float v[8];
+  if (columns || (!STEP && !diagonal))
+    for (int i0 = 0; i0 < ni; i0 += 32)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = one(il + e, jl);
-      u32x4 hi{}, lw{};
-      if (OP == kPoly) {
-        const uint16_t* s = A + pair_index(j, i, ld);
-        hi = *reinterpret_cast<const u32x4*>(s);
-        lw = *reinterpret_cast<const u32x4*>(s + 32);
-      }
-      if (OP == kLast) {
+      for (int p = 0; p < T / 64; ++p) {
+        const int j0 = 16 * w + 64 * p;
+        if (j0 >= nj) continue;
+        const int ic = i0 + 8 * (l & 3), jc = j0 + (l >> 2), i = it * T + ic, j = jt * T + jc;
+        u32x4 hi{}, lw{};
+        if (OP == kPoly) {
+          const uint16_t* s = A + pair_index(j, i, ld);
+          hi = *reinterpret_cast<const u32x4*>(s);
+          lw = *reinterpret_cast<const u32x4*>(s + 32);
+        }
+        float v[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const uint16_t* s = X + pair_index(i + e, j, ld);
-          hi[e >> 1] |= (uint32_t)s[0] << (16 * (e & 1));
-          lw[e >> 1] |= (uint32_t)s[32] << (16 * (e & 1));
+        for (int e = 0; e < 8; ++e) v[e] = *one(ic + e, jc);
+        if (OP == kLast) {
+          store_row8(a, dtype, mat, j, i, v);
+        } else {
+          finish(v, hi, lw);
+          store_pairs(base + pair_index(j, i, ld), v);
         }
       }
-      finish(v, hi, lw);
-      if (OP == kLast)
-        store_row8(a, dtype, mat, j, i, v);
-      else
-        store_pairs(base + pair_index(j, i, ld), v);
-    }
-  }
 }
 
 // Small matrices (r <= 64, m <= 512): all steps of a matrix in one workgroup, X (at most 128 KB) and A,
@@ -693,7 +743,13 @@ int ortho_product(const OrthoArgs& a, int dtype, hipStream_t st) {
     const int64_t ti = (a.rp + t - 1) / t, tj = (a.mp + t - 1) / t;
     return a.n * (OP >= kStep ? ti * tj : ti * (ti + 1) / 2);
   };
-  const bool wide = tiles(128) >= 200;
+  // Tiles of 128 read half the bytes per product, tiles of 64 take half as long to begin and end, and are
+  // four times as many.  us, 128 / 64, at the number of tiles of 128 and the length that is contracted:
+  // step 224, 512: 22 / 19; 384, 512: 26 / 28; 1024, 256: 37 / 47; 1536, 512: 84 / 101; 256, 1024: 37 / 33;
+  // 256, 2048: 64 / 76; Gram and square 240, 512: 19 / 19; 400, 512: 33 / 27; 480, 512: 39 / 35; 72, 2048:
+  // 36 / 27; 136, 2048: 40 / 44; 240, 2048: 48 / 53; 528, 4096: 230 / 330.
+  const bool deep = (OP == kGram ? a.mp : a.rp) >= 2048;
+  const bool wide = OP >= kStep ? tiles(128) >= (deep ? 200 : 300) : deep && tiles(128) >= 130;
   const int64_t work = tiles(wide ? 128 : 64);
   const unsigned grid = 8u * (unsigned)((work + 7) / 8);
   if (wide)
