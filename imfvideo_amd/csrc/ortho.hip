@@ -244,7 +244,7 @@ __device__ inline u32x4 turned_frag(const unsigned char* tile, int s, int mb, co
 // three stages ahead, the operands of half a stage read beside the products of the half before (left to
 // the compiler's order: 24 x 512 x 2048, kGram 63 us for 48).  Result element (i, j): j along the
 // registers, i along the lanes; it goes through LDS, so that whole rows are stored (from the registers,
-// eight bytes to a row: kStep 105 us, kGram 65).  24 x 512 x 2048: kGram 1.0, kStep 0.92 PFLOP/s of
+// eight bytes to a row: kStep 105 us for 91, kGram 65 for 58).  24 x 512 x 2048: kGram 1.0, kStep 0.92 PFLOP/s of
 // 16-bit products, with 200 MB read and written beside kStep's.
 //   kGram: A = X X^T;  kPoly: B = b A + c A A^T;  kStep: Y = a X + B X;  kLast: that, to G's type
 template <int T, int OP>

@@ -20,8 +20,8 @@ __all__ = ["Muon", "matrix_parameters", "newton_schulz"]
 
 
 def newton_schulz(g, steps=5, coeffs=ops.NS_COEFFS):
-    """ops.orthogonalize; CPU tensors run the products one by one, in float32 or wider."""
-    if g.is_cuda:
+    """ops.orthogonalize; CPU and float64 tensors run the products one by one, in float32 or wider."""
+    if g.is_cuda and g.dtype != torch.float64:
         return ops.orthogonalize(g, steps, coeffs)
     ops._ns_coeffs(steps, ops.ns_rows(steps, coeffs))  # its checks
     x = g.to(torch.promote_types(g.dtype, torch.float32))
@@ -63,9 +63,10 @@ class Muon(torch.optim.Optimizer):
     def add_param_group(self, group):
         super().add_param_group(group)
         for p in self.param_groups[-1]["params"]:
-            if p.dim() != 2 or not p.is_floating_point():
+            if p.dim() != 2 or not p.is_floating_point() or max(p.shape) > 32768:
                 self.param_groups.pop()
-                raise ValueError(f"Muon: matrices only, got {tuple(p.shape)} {p.dtype}")
+                raise ValueError("Muon: matrices only, sides up to 32,768, got "
+                                 f"{tuple(p.shape)} {p.dtype}")
 
     def load_state_dict(self, state_dict):
         super().load_state_dict(state_dict)
@@ -112,9 +113,10 @@ class Muon(torch.optim.Optimizer):
         u = torch.stack(torch._foreach_add(grads, bufs, alpha=mu) if group["nesterov"] else bufs)
         x = newton_schulz(u, group["ns_steps"], group["ns_coeffs"])
         R, C = ps[0].shape
-        step = -group["lr"] * group["rms"] * math.sqrt(max(R, C))
+        lr = float(group["lr"])
+        step = -lr * group["rms"] * math.sqrt(max(R, C))
         if group["weight_decay"]:
-            torch._foreach_mul_(ps, 1.0 - group["lr"] * group["weight_decay"])
+            torch._foreach_mul_(ps, 1.0 - lr * group["weight_decay"])
         if ps[0].dtype == wide:
             torch._foreach_add_(ps, list(x), alpha=step)
         else:  # (16-bit weights: the sum in fp32, rounded once)

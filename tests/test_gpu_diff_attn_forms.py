@@ -1,0 +1,183 @@
+"""diff_attention's entry on the GPU: what it hands to autograd, tracing and forward mode, offsets
+past 32 bits, many clips, calls on two streams and in graphs, its kernels' other forms."""
+import pytest
+import torch
+
+from tests import diff_attn_ref as R
+from tests.test_gpu_diff_attn import call, compare, operands
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("leaf", [False, True])
+def test_a_tangent_is_refused_and_never_dropped(leaf):
+    import torch.autograd.forward_ad as fw
+    from imfvideo_amd.imf_dit_video import diff_attention
+    x, lam, _ = operands(1, 1, 8, 2)
+    want = diff_attention(*x, lam)
+    with fw.dual_level():
+        for i in range(4):
+            t = [*x, lam]
+            t[i] = fw.make_dual(t[i].clone().requires_grad_(leaf), torch.ones_like(t[i]))
+            with pytest.raises(NotImplementedError, match="forward mode"):
+                diff_attention(*t)
+        assert torch.equal(diff_attention(*x, lam), want)
+
+
+def test_one_reverse_mode_derivative():
+    from imfvideo_amd.imf_dit_video import diff_attention
+    x, lam, do = operands(2, 1, 40, 2)
+    q = x[0].requires_grad_(True)
+    o = diff_attention(q, x[1], x[2], lam)
+    with pytest.raises(RuntimeError, match="one gradient at a time"):
+        torch.autograd.grad(o, q, torch.stack([do, do]), is_grads_batched=True, retain_graph=True)
+    d, = torch.autograd.grad(o, q, do, create_graph=True)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(d.float().sum(), q)
+    with pytest.raises(RuntimeError):
+        torch.func.vmap(lambda a: diff_attention(a, x[1], x[2], lam))(torch.stack([q] * 2))
+    with pytest.raises(RuntimeError), torch.no_grad():
+        torch.func.vmap(lambda a: diff_attention(a, x[1], x[2], lam))(torch.stack([q] * 2))
+
+
+@pytest.mark.filterwarnings("ignore")
+@pytest.mark.parametrize("leaf", [False, True])
+def test_a_trace_records_the_call(leaf):
+    from imfvideo_amd.imf_dit_video import diff_attention
+    x, lam, _ = operands(3, 1, 8, 2)
+    m = torch.jit.trace(lambda a, b, c, w: diff_attention(a, b, c, w, causal=True),
+                        [t.requires_grad_(leaf) for t in (*x, lam)], check_trace=False)
+    y, lam2, _ = operands(4, 1, 8, 2)
+    want = diff_attention(*y, lam2, causal=True)
+    for _ in range(3):
+        assert torch.equal(m(*y, lam2), want)
+
+
+def test_many_clips_train():
+    """65,600 heads of three rows: forward and backward, each clip as it is alone."""
+    x, lam, do = operands(5, 8200, 3, 8, Lk=4)
+    got = call(x, lam, do, causal=True)
+    want = R.attention(*x, lam, causal=True, do=do, dev="cuda")
+    for n in ("o", "dq", "dk", "dv", "dlam"):
+        R.check(got[n], want[n], n)
+
+
+@pytest.mark.parametrize("which", ["batch", "heads", "rows"])
+def test_offsets_past_32_bits(which):
+    """Operands as views of buffers of more than 2^32 bytes, strides past 2^31 elements between clips
+    or heads, and 300 rows of 2^23 - 8 elements."""
+    x, lam, do = operands(6, 2, 300, 2, dt=torch.float16)
+    want = call(x, lam, do)
+    far = 2 ** 31 + 128
+    strides = {"batch": (far, 300, 64), "heads": (300 * 64, 64, far),
+               "rows": (64, 2 ** 23 - 8, 128)}[which]
+    if which == "batch":
+        strides = (far, 128, 64)
+    views = []
+    for t in x:
+        size = sum((n - 1) * s for n, s in zip((2, 300, 2), strides)) + 64
+        buf = torch.empty(size, device="cuda", dtype=t.dtype)
+        view = buf.as_strided(t.shape, (*strides, 1))
+        view.copy_(t)
+        views.append(view)
+    if which == "rows":  # (clip 1 begins 64 elements behind clip 0, its rows between those)
+        assert torch.equal(views[0], x[0])
+    got = call(views, lam, do)
+    for n in want:
+        assert torch.equal(got[n], want[n]), n
+
+
+def test_two_streams_at_once():
+    """Calls of both forms interleaved on two streams, with workspaces of their own."""
+    sets = [operands(7, 1, 1, 4, Lk=9000), operands(8, 2, 700, 4), operands(9, 1, 64, 4, Lk=5000)]
+    want = [call(*s) for s in sets]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = []
+    torch.cuda.synchronize()
+    for r in range(4):
+        for i, s in enumerate(sets):
+            with torch.cuda.stream(streams[(r + i) % 2]):
+                got.append((i, call(*s)))
+    torch.cuda.synchronize()
+    for i, g in got:
+        for n in want[i]:
+            assert torch.equal(g[n], want[i][n]), (i, n)
+
+
+def test_two_graphs_and_eager_calls_between_their_replays():
+    """Captured forward and backward, a graph each for few and for many queries, replayed in turn on
+    refilled operands, an eager graph of other leaves alive."""
+    from imfvideo_amd.imf_dit_video import diff_attention
+    sets = [operands(10, 1, 2, 4, Lk=6000), operands(11, 2, 300, 4)]
+    for s in sets:
+        call(*s)
+    other = sets[0][0][0].clone().requires_grad_(True)
+    alive = diff_attention(other, *sets[0][0][1:], sets[0][1])
+    graphs, kept = [], []
+    for s in sets:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            kept.append(call(*s, causal=True))
+        graphs.append(g)
+    for r in range(4):
+        for s in sets:
+            for t in (*s[0], s[2]):
+                t.copy_(torch.randn(t.shape, device="cuda"))
+        for i in (0, 1, 0):
+            graphs[i].replay()
+            torch.cuda.synchronize()
+            want = call(*sets[i], causal=True)
+            torch.cuda.synchronize()
+            for n in want:
+                assert torch.equal(kept[i][n], want[n]), (r, i, n)
+    del alive
+
+
+def test_the_least_and_most_gradients_of_an_expanded_output():
+    """An output gradient that is one number for all, and operands that share memory."""
+    from imfvideo_amd.imf_dit_video import diff_attention
+    x, lam, _ = operands(12, 2, 70, 4)
+    q = x[0]
+    leaves = [t.clone().requires_grad_(True) for t in (q, lam)]
+    o = diff_attention(leaves[0], leaves[0], leaves[0], leaves[1])
+    dq, dlam = torch.autograd.grad(o.sum(), leaves)
+    want = call([q, q, q], lam, torch.ones_like(q))
+    assert torch.equal(dlam, want["dlam"])
+    # the three gradients of the one leaf, added by autograd in the operands' type: two roundings
+    total = sum(want[n].double() for n in ("dq", "dk", "dv"))
+    size = sum(want[n].double().abs() for n in ("dq", "dk", "dv"))
+    assert ((dq.double() - total).abs() <= 2 * 2.0 ** -8 * size).all()
+
+
+@pytest.mark.parametrize("Hkv", [2, 8])
+@pytest.mark.parametrize("Lq,Lk,causal", [(600, 40, False), (520, 520, True), (40, 9000, False),
+                                          (130, 4100, True), (1500, 1500, False)])
+def test_other_forms(Lq, Lk, causal, Hkv):
+    """Sizes on both sides of the rules for tiles, splits and lost halves."""
+    compare(*operands(13, 1, Lq, 8, Hkv, Lk), "forms", causal=causal)
+
+
+@pytest.mark.parametrize("ql,kl", [([-3, 400], [400, 2 ** 31 - 1]), ([401, 0], [0, 17])])
+def test_lengths_are_clamped(ql, kl):
+    x, lam, do = operands(14, 2, 400, 2)
+    n = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")
+    clamp = lambda v: n([min(max(i, 0), 400) for i in v])
+    got = call(x, lam, do, q_lens=n(ql), k_lens=n(kl))
+    want = call(x, lam, do, q_lens=clamp(ql), k_lens=clamp(kl))
+    for name in want:
+        assert torch.equal(got[name], want[name]), name
+
+
+def test_what_stands_behind_a_sequence_is_not_read():
+    """NaN in the rows behind q_len and k_len, of the output gradient too, reaches no result."""
+    x, lam, do = operands(15, 2, 400, 4)
+    kw = dict(q_lens=[130, 400], k_lens=[77, 331])
+    want = call(x, lam, do, **kw)
+    for t, lens in ((x[0], kw["q_lens"]), (x[1], kw["k_lens"]), (x[2], kw["k_lens"]),
+                    (do, kw["q_lens"])):
+        for b in range(2):
+            t[b, lens[b]:] = float("nan")
+    got = call(x, lam, do, **kw)
+    for n in want:
+        assert torch.equal(got[n], want[n]), n
+        assert torch.isfinite(got[n]).all(), n

@@ -179,3 +179,38 @@ def test_muon_steps_as_its_formula(dt, nesterov):
             tol[i] += 2 * u * (w[i].abs() + d.abs()) + 1e-4 * d.abs().max() + 2.0 ** -23 * w[i].abs()
     for i, p in enumerate(ps):
         assert ((p.detach().double().cpu() - w[i]).abs() <= tol[i]).all(), i
+
+
+def test_offsets_past_32_bits():
+    """66 matrices of 2^24 elements, 4.4 GB: each is as it is alone."""
+    from imfvideo_amd import ops
+    g = torch.empty(66, 4096, 4096, device="cuda")
+    for i in (0, 63, 64, 65):
+        g[i] = torch.randn(4096, 4096, device="cuda")
+    g[1:63] = g[0]
+    x = ops.orthogonalize(g, steps=1)
+    for i in (0, 62, 63, 65):
+        assert torch.equal(ops.orthogonalize(g[i], steps=1), x[i]), i
+
+
+def test_float64_weights_take_the_eager_products():
+    from imfvideo_amd.muon import Muon
+    p = torch.nn.Parameter(torch.randn(20, 30, device="cuda", dtype=torch.float64))
+    w, g = p.detach().clone(), torch.randn_like(p)
+    p.grad = g
+    Muon([p], lr=0.1, nesterov=False).step()
+    want = w.cpu() - 0.1 * 0.2 * 30 ** 0.5 * exact(g.cpu())
+    assert (p.detach().cpu() - want).abs().max() < 1e-9
+
+
+@pytest.mark.parametrize("n,R,C", [(3, 130, 2100), (40, 512, 512), (2, 2050, 2049), (1, 192, 5000),
+                                   (9, 320, 1000)])
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16])
+def test_forms_on_both_sides_of_the_tile_rule(n, R, C, dt):
+    from imfvideo_amd import ops
+    g = matrices(n, n, R, C).to(dt)
+    check(ops.orthogonalize(g, steps=2), g, (n, R, C, dt), steps=2)
+    if R != C:  # (of a square matrix the rows are contracted whichever way it stands)
+        t = g.transpose(-1, -2).contiguous()
+        assert torch.equal(ops.orthogonalize(t, steps=2),
+                           ops.orthogonalize(g, steps=2).transpose(-1, -2))
