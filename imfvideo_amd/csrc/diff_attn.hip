@@ -354,13 +354,14 @@ __device__ inline void finish_row(const DiffFwdArgs& a, int64_t bp, int64_t i, i
   *reinterpret_cast<u32x4*>(out_row(a, bp, i) + c0) = z;
 }
 
-// Few queries: workgroup = 32 rows (of the `rep` query pairs that share a key pair) over one range of
-// keys; its W waves take the 32-key units in turn, both maps of a unit, each with an LDS slot of its own
-// (no barrier in the loop), and their sums are joined in LDS.  A wave waits for its unit and computes it
-// while the others' units are on their way: W = 4, two workgroups per CU; W = 8, one, where there is
-// at most one for every CU.  The products wait for the loads here, so what the rounding of P lost is
-// always added by a second one.
-template <typename T16, int W>
+// Few queries of grouped heads, or few keys: workgroup = 32 rows of the `rep` query pairs that share a key pair, over
+// one range of keys; its four waves take the 32-key units in turn, both maps of a unit, each with an LDS
+// slot of its own (no barrier in the loop), and their sums are joined in LDS.  A wave waits for its unit
+// and computes it while the others' units are on their way (eight waves, one workgroup per CU: no
+// faster).  The products wait for the loads here, so what the rounding of P lost is always added by
+// a second one.
+constexpr int W = 4;  // waves
+template <typename T16>
 __global__ __launch_bounds__(64 * W, 2) void diff_fwd_split_kernel(DiffFwdArgs a) {
   __shared__ __align__(16) unsigned char kv[W][kStageB];
   __shared__ float mls[W][2][2][32];  // wave, map, (m, l)
@@ -469,7 +470,7 @@ __global__ __launch_bounds__(64 * W, 2) void diff_fwd_split_kernel(DiffFwdArgs a
   // (row r of the tile is lane r's, in every wave)
   const bool mine = live;
   const int64_t op = (int64_t)b * a.P + p, oi = i, flat = op * a.Lq + oi;
-  constexpr int NG = 8 / W;  // groups of eight channels of a thread (W = 8: one)
+  constexpr int NG = 8 / W;  // groups of eight channels of a thread
   float mm[2], ll[2], x[2][NG][8];
 #pragma unroll
   for (int m = 0; m < 2; ++m) {
@@ -523,8 +524,51 @@ __global__ __launch_bounds__(64 * W, 2) void diff_fwd_split_kernel(DiffFwdArgs a
   }
 }
 
-// Joins the key ranges of a row: 64 groups of 16 lanes, 32 for each map (eight channels per lane), take
-// the ranges in turn, and their sums are added in order.
+// Joins the key ranges of a row, many rows: 16 lanes for each map (eight channels per lane) take the
+// ranges one after the other, eight rows per workgroup.
+template <typename T16>
+__global__ __launch_bounds__(256) void diff_join_rows_kernel(DiffFwdArgs a) {
+  const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  const int64_t flat = row < a.nrows ? row : a.nrows - 1;
+  const int m = (threadIdx.x >> 4) & 1, c0 = (threadIdx.x & 15) * 8;
+  float t[2][8], mm[2], ll[2];
+  float top = kFloor, sum = 0.f;
+  f32x4 x{0.f, 0.f, 0.f, 0.f}, y = x;
+#pragma unroll 4
+  for (int s = 0; s < a.splits; ++s) {
+    const int64_t at = (s * 2 + m) * a.nrows + flat;
+    const float2 ml = a.ml[at];
+    const f32x4* src = reinterpret_cast<const f32x4*>(a.part + at * 128 + c0);
+    const f32x4 p0 = src[0], p1 = src[1];
+    const float mn = fmaxf(top, ml.x), f = fast_exp2(top - mn), g = fast_exp2(ml.x - mn);
+    top = mn;
+    sum = sum * f + g * ml.y;
+    x = x * f + g * p0;
+    y = y * f + g * p1;
+  }
+  // the second map's lanes hand theirs over
+  mm[0] = top, ll[0] = sum;
+  mm[1] = __shfl_xor(top, 16, 64);
+  ll[1] = __shfl_xor(sum, 16, 64);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    t[0][e] = e < 4 ? x[e & 3] : y[e & 3];
+    t[1][e] = __shfl_xor(t[0][e], 16, 64);
+  }
+  if (m || row >= a.nrows) return;
+  const int64_t bp = flat / a.Lq, i = flat - bp * a.Lq;
+  const int b = (int)(bp / a.P);
+  // (the halves of a wave may be of two clips: seq_len would take the first one's)
+  auto len = [&](const int32_t* lens, int64_t L) {
+    const int n = lens ? lens[b] : (int)L;
+    return n < 0 ? 0 : (n > L ? (int)L : n);
+  };
+  finish_row<T16>(a, bp, i, c0,
+                  key_limit((int)i, len(a.q_lens, a.Lq), len(a.k_lens, a.Lk), a.causal) > 0, t, mm, ll);
+}
+
+// Few rows and many ranges: a workgroup per row, 64 groups of 16 lanes, 32 for each map, take the
+// ranges in turn, and their sums are added in order.
 template <typename T16>
 __global__ __launch_bounds__(1024) void diff_join_kernel(DiffFwdArgs a) {
   __shared__ float sm[2][32], sl[2][32];
@@ -585,45 +629,46 @@ __global__ __launch_bounds__(1024) void diff_join_kernel(DiffFwdArgs a) {
   finish_row<T16>(a, bp, i, c0, key_limit((int)i, qlen, klen, a.causal) > 0, t, tm, tl);
 }
 
-// The form of a call: query blocks of 128 or 64 rows, or of 32 rows of a key pair's group.
+// The form of a call: query blocks of 128 or 64 rows, over all keys or ranges of them; or the one tile
+// of 32 rows of a key pair's group.
 struct FwdPlan {
   int nq;  // 2, 1: diff_fwd_kernel<NQ>; 0: diff_fwd_split_kernel
   int64_t qtiles, nwork;
   int splits;  // ranges of keys
-  int64_t units;
-  int waves;  // nq = 0
+  int64_t units;  // nq = 0: 32-key units of a range
 };
 
 // even: neither causal nor lengths
 FwdPlan fwd_plan(int B, int H, int Hkv, int64_t Lq, int64_t Lk, bool even) {
   FwdPlan p{};
   const int64_t bp = (int64_t)B * H / 2, bk = (int64_t)B * Hkv / 2, rep = H / Hkv;
-  p.splits = 1;
-  p.nq = 2;
-  p.qtiles = (Lq + 127) / 128;
-  p.nwork = bp * p.qtiles;
-  if (p.nwork >= (even ? 256 : 768)) return p;
-  p.nq = 1;
-  p.qtiles = (Lq + 63) / 64;
-  p.nwork = bp * p.qtiles;
-  if (p.nwork >= 256) return p;
   const int64_t units = (Lk + kUnitRows - 1) / kUnitRows;
-  if (Lq > 48 && Lk >= 1024) {
-    const int64_t most = units / 8, s = (512 + p.nwork - 1) / p.nwork;
-    p.splits = (int)(s < most ? s : most);
+  // A group's rows in one tile read their keys once (us, in this form / in query blocks: 64 clips, H = 16,
+  // Hkv = 2, 1 query, 2,000 keys 23 / 64; 1 clip, 29,952 keys 18 / 27; 32 clips, 32, 4, 4 queries
+  // 27 / 48; in two tiles and more: 8 clips, 16, 2, 16 queries 20 / 18).  A row of few keys needs the second
+  // product: the rounding of P_m is a part of delta_m, and of dA - delta_m, which then nearly cancel (2
+  // keys: dq and dk six times as far off; 100 of 100 keys 10 / 8 us).
+  if (units <= 4 || (rep > 1 && rep * Lq <= 32)) {
+    p.qtiles = (rep * Lq + 31) / 32;
+    const int64_t blocks = bk * p.qtiles;
+    const int64_t s = 512 / blocks, most = units / 8;  // two units per wave and range at least
+    p.splits = (int)(s < 1 || most < 1 ? 1 : (s < most ? s : most));
+    p.units = (units + p.splits - 1) / p.splits;
+    p.splits = (int)((units + p.units - 1) / p.units);
+    p.nwork = blocks * p.splits;
     return p;
   }
-  p.nq = 0;
-  p.qtiles = (rep * Lq + 31) / 32;
-  const int64_t blocks = bk * p.qtiles;
-  int64_t s = (512 + blocks - 1) / blocks;
-  const int64_t most = units / 8;  // two units per wave and range at least
-  s = s < most ? s : most;
-  p.splits = s < 1 ? 1 : (int)s;
-  p.units = (units + p.splits - 1) / p.splits;
-  p.splits = (int)((units + p.units - 1) / p.units);
-  p.nwork = blocks * p.splits;
-  p.waves = p.nwork <= 256 && p.units > 4 ? 8 : 4;
+  // 128 rows (no ranges) or 64, by what a stage takes (SplitCost) with one and two workgroups per CU.  us,
+  // 128 / 64, H = 8: 1 clip of 8,192 231 / 208, of 12,000 476 / 479, of 16,384 738 / 809, 4 clips of
+  // 2,048, H = 16, 106 / 113; causal 12,000 334 / 244, 24,000 831 / 870.
+  const int64_t q2 = (Lq + 127) / 128, q1 = (Lq + 63) / 64;
+  const SplitCost c2{0.88f, 1.43f, 0.f, 0}, c1{0.53f, 0.74f, 0.033f, 4};
+  float t1;
+  p.splits = best_split(bp * q1, units, even, c1, t1);
+  p.nq = c2.time(bp * q2, units, 1, even) < t1 ? 2 : 1;
+  if (p.nq == 2) p.splits = 1;
+  p.qtiles = p.nq == 2 ? q2 : q1;
+  p.nwork = bp * p.qtiles;
   return p;
 }
 
@@ -636,8 +681,13 @@ using namespace sla2h;
 extern "C" size_t sla2h_diff_attn_fwd_workspace_bytes(int B, int H, int Hkv, int64_t Lq,
                                                       int64_t Lk) {
   if (!diff_sizes_ok(B, H, Hkv, Lq, Lk)) return 0;
-  const FwdPlan p = fwd_plan(B, H, Hkv, Lq, Lk, true);  // the split forms do not depend on it
-  return p.splits > 1 ? (size_t)p.splits * B * H * Lq * (128 * 4 + 8) : 0;
+  size_t most = 0;
+  for (bool even : {false, true}) {
+    const FwdPlan p = fwd_plan(B, H, Hkv, Lq, Lk, even);
+    const size_t n = p.splits > 1 ? (size_t)p.splits * B * H * Lq * (128 * 4 + 8) : 0;
+    most = n > most ? n : most;
+  }
+  return most;
 }
 
 extern "C" int sla2h_diff_attn_fwd(const void* q, const void* k, const void* v, const void* lam,
@@ -701,13 +751,15 @@ extern "C" int sla2h_diff_attn_fwd(const void* q, const void* k, const void* v, 
       diff_fwd_kernel<T16, 2><<<work_grid(a.map), 256, 0, st>>>(a);
     else if (p.nq == 1)
       diff_fwd_kernel<T16, 1><<<work_grid(a.map), 256, 0, st>>>(a);
-    else if (p.waves == 8)
-      diff_fwd_split_kernel<T16, 8><<<(unsigned)p.nwork, 512, 0, st>>>(a);
     else
-      diff_fwd_split_kernel<T16, 4><<<(unsigned)p.nwork, 256, 0, st>>>(a);
+      diff_fwd_split_kernel<T16><<<(unsigned)p.nwork, 256, 0, st>>>(a);
     const int err = (int)hipGetLastError();
     if (err || p.splits == 1) return err;
-    diff_join_kernel<T16><<<(unsigned)a.nrows, 1024, 0, st>>>(a);
+    // (us: 4 rows, 64 ranges 14 / 4; 2,000 rows of 4 pairs, 2 ranges 10 / 40)
+    if (a.nrows >= 512 || p.splits <= 8)
+      diff_join_rows_kernel<T16><<<(unsigned)((a.nrows + 7) / 8), 256, 0, st>>>(a);
+    else
+      diff_join_kernel<T16><<<(unsigned)a.nrows, 1024, 0, st>>>(a);
     return (int)hipGetLastError();
   };
   return dtype == SLA2H_DTYPE_BF16 ? go(BF16{}) : go(F16{});

@@ -37,7 +37,8 @@ struct Scaled<F16> {
 // make it 1.5 times as far off as a rounded exact result): in all stages of sequences of at most
 // kFineKeys keys or kFineRows queries and of causal waves that see at most kFineRows keys, else in
 // every second stage (1.25 times; B = 1, H = 8, L = 29,952: 0.4 ms).  dk, dv: calls of at most
-// kFineRows rows per key pair (longer sums average the roundings out).
+// kFineRows rows per key pair, or of one block of keys, whose few large probabilities round alike in
+// row after row (longer sums average the roundings out).
 constexpr int kFineKeys = 4096, kFineRows = 512;
 constexpr int kKeyRows = 128;  // keys of a workgroup of dk and dv
 constexpr int kNormRows = 64;  // rows of a partial maximum of the norms and of a partial sum of dlam
@@ -396,12 +397,14 @@ __device__ inline float row_value_at(float x, int e) {  // e a constant where it
   }
 }
 
-// dk, dv: workgroup = 8 waves x 32 keys of one key pair; the query rows (both maps' queries, the 128
-// channels of do) of the pairs that read it are streamed in stages of 32 rows, three ahead in four
-// LDS slots, with their four statistics.  A wave holds 128 channels of dv, 64 of each dk and its keys
-// in registers; its values lie in LDS, so that two waves fit on a SIMD (with them in registers, and one
-// wave: 6.1 ms at B = 1, H = 8, L = 29,952, bf16).  A row's statistic belongs to one register of a
-// score tile in all lanes of a half: a lane reads one value, and the add takes it from there (DPP).
+// dk, dv: workgroup = 4 waves x 32 keys of one key pair; the query rows (both maps' queries, the 128
+// channels of do) of the pairs that read it are streamed in stages of 32 rows through two LDS slots, one
+// ahead, with their four statistics.  A wave holds 128 channels of dv, 64 of each dk and its keys in
+// registers; its values lie in LDS, so that two workgroups fit on a CU and one computes while the other
+// waits (with the values in registers, one wave per SIMD: 6.1 ms at B = 1, H = 8, L = 29,952, bf16; eight
+// waves in one workgroup: 4.1; this form 3.75, 0.98 PFLOP/s, at the card's power limit).  A row's
+// statistic belongs to one register of a score tile in all lanes of a half: a lane reads one value, and
+// the add takes it from there (DPP).
 template <typename T16, bool CAUSAL, bool FINE>
 __global__ __launch_bounds__(256, 2) void diff_bwd_dkdv_kernel(DiffBwdArgs a) {
   __shared__ __align__(16) unsigned char r0[kStageB], r1[kStageB];
@@ -675,15 +678,14 @@ BwdPlan bwd_plan(int dtype, int B, int H, int Hkv, int64_t Lq, int64_t Lk, bool 
   BwdPlan p{};
   const int64_t bp = (int64_t)B * H / 2, bk = (int64_t)B * Hkv / 2, rep = H / Hkv;
   p.qtiles = (Lq + 127) / 128;
-  auto split = [&](int64_t blocks, int64_t units, int64_t want) {
-    if (blocks >= want / 2) return 1;
-    const int64_t s = (want + blocks - 1) / blocks, most = units / 8;
-    return (int)(s < most ? s : (most < 1 ? 1 : most));
-  };
-  p.dq_splits = split(bp * p.qtiles, (Lk + 31) / 32, even ? 256 : 800);
+  // (us, unsplit / split, B x H x L: 2 x 8 x 2,048 dq 87 / 63, dk and dv 90 / 69; 1 x 8 x 6,000 204 / 164,
+  // 230 / 194; causal 1 x 8 x 12,000 417 / 283, 488 / 339)
+  float t;
+  p.dq_splits = best_split(bp * p.qtiles, (Lk + 31) / 32, even, SplitCost{1.15f, 2.f, 0.033f, 8}, t);
   p.dq_nwork = bp * p.qtiles * p.dq_splits;
   p.ktiles = (Lk + kKeyRows - 1) / kKeyRows;
-  p.kv_splits = split(bk * p.ktiles, rep * ((Lq + 31) / 32), even ? 256 : 512);
+  p.kv_splits = best_split(bk * p.ktiles, rep * ((Lq + 31) / 32), even,
+                           SplitCost{1.2f, 2.1f, 0.066f, 8}, t);
   p.kv_nwork = bk * p.ktiles * p.kv_splits;
   p.nqb = (Lq + kNormRows - 1) / kNormRows;
   p.nkb = (Lk + kNormRows - 1) / kNormRows;
@@ -790,7 +792,7 @@ extern "C" int sla2h_diff_attn_bwd(const void* q, const void* k, const void* v, 
     if ((err = (int)hipGetLastError())) return err;
     if (dk) {
       const unsigned grid = work_grid(a.kv_map);
-      const bool few = a.rep * Lq <= kFineRows;
+      const bool few = a.rep * Lq <= kFineRows || Lk <= kKeyRows;
       if (causal && few)
         diff_bwd_dkdv_kernel<T16, true, true><<<grid, 256, 0, st>>>(a);
       else if (causal)

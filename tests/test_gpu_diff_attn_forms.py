@@ -157,6 +157,38 @@ def test_other_forms(Lq, Lk, causal, Hkv):
     compare(*operands(13, 1, Lq, 8, Hkv, Lk), "forms", causal=causal)
 
 
+@pytest.mark.parametrize("B,H,Lq,Lk,ql,kl", [
+    (3, 2, 1, 405, [1, 0, 1], [405, 263, 121]), (2, 6, 37, 928, [37, 0], [928, 928]),
+    (2, 6, 37, 928, [0, 37], [928, 0]), (3, 2, 5, 3000, [5, 0, 2], [64, 3000, 2999]),
+    (3, 2, 1893, 1893, [1893, 0, 700], [1893, 0, 700])])
+@pytest.mark.parametrize("causal", [False, True])
+def test_ranges_of_keys_in_a_padded_batch(B, H, Lq, Lk, ql, kl, causal):
+    """Rows of two clips in one wave of the join, ranges without a key, clips without any."""
+    x, lam, do = operands(16, B, Lq, H, Lk=Lk)
+    n = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")
+    got = compare(x, lam, do, "ranges", ql=n(ql), kl=n(kl), causal=causal)
+    for b in range(B):
+        dead = ql[b] if kl[b] else 0
+        assert (got["o"][b, dead:] == 0).all() and (got["dq"][b, dead:] == 0).all()
+
+
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("Lq,Lk,causal", [(1267, 2, True), (2500, 2, False), (64, 3, False),
+                                          (2, 2, True), (3000, 100, True), (1500, 1, False)])
+def test_few_keys_keep_the_gradients_accuracy(Lq, Lk, causal, dt):
+    """Rows that see few keys: dA - delta nearly cancels, and what the rounding of the maps lost would
+    show in it.  As far off as roundings of the exact result and of its last operand are, in norm:
+    sqrt(2) of one rounding's u / sqrt(3), and half as much again for the others."""
+    x, lam, do = operands(17, 2, Lq, 4, Lk=Lk, dt=dt)
+    got = call(x, lam, do, causal=causal)
+    want = R.attention(*x, lam, causal=causal, do=do, dev="cuda")
+    u = torch.finfo(dt).eps / 2
+    for n in ("o", "dq", "dk", "dv"):
+        err = (got[n].double() - want[n][0]).norm().item()
+        print("[ratio]", n, err / max(want[n][0].norm().item() * u, 1e-300), flush=True)
+        assert err <= 1.5 * 2 ** 0.5 * u / 3 ** 0.5 * want[n][0].norm().item(), n
+
+
 @pytest.mark.parametrize("ql,kl", [([-3, 400], [400, 2 ** 31 - 1]), ([401, 0], [0, 17])])
 def test_lengths_are_clamped(ql, kl):
     x, lam, do = operands(14, 2, 400, 2)
