@@ -41,26 +41,28 @@ inline bool diff_sizes_ok(int B, int H, int Hkv, int64_t Lq, int64_t Lk) {
 
 // What a launch of workgroups, two of which fit on a CU, takes (us on this card, without launching): per
 // stage `two` for every full round of 512 and, for the rest, `one` while each has a CU of its own.  Work
-// that is not even (causal, lengths) is half as much on average and has no rounds, but no less than its longest
-// workgroup.  Ranges of a long axis: `join` more per workgroup for its partial sums' way through
-// memory, and the launch that adds them.
+// of unequal workgroups (share below 1: what is left of all of it on average) has no rounds, but takes no less
+// than its longest one, a fifth more for its neighbours.  Ranges of a long axis: `join` more per
+// workgroup for its partial sums' way through memory, and the launch that adds them.
 struct SplitCost {
   float one, two, join;
   int least;  // stages of a range
-  float time(int64_t blocks, int64_t stages, int64_t s, bool even) const {
+  float time(int64_t blocks, int64_t stages, int64_t s, float share) const {
     const int64_t w = blocks * s, n = (stages + s - 1) / s, rest = w % 512;
-    const float full = two * (float)w / 1024.f;
-    const float stage = even ? (float)(w / 512) * two + (rest == 0 ? 0.f : (rest <= 256 ? one : two))
-                             : (full > one ? full : one);
+    const float full = two * (float)w * share / 512.f, longest = 1.2f * one;
+    const float stage = share == 1.f
+                            ? (float)(w / 512) * two + (rest == 0 ? 0.f : (rest <= 256 ? one : two))
+                            : (full > longest ? full : longest);
     return (float)n * stage + (s > 1 ? 3.f + join * (float)w : 0.f);
   }
 };
+constexpr float kShares[2][2] = {{1.f, 0.7f}, {0.5f, 0.35f}};  // causal, lengths
 // The number of ranges that takes least.
-inline int best_split(int64_t blocks, int64_t stages, bool even, const SplitCost& c, float& least) {
+inline int best_split(int64_t blocks, int64_t stages, float share, const SplitCost& c, float& least) {
   int best = 1;
-  least = c.time(blocks, stages, 1, even);
-  for (int64_t s = 2; blocks * s <= 1024 && stages >= s * c.least; ++s) {
-    const float t = c.time(blocks, stages, s, even);
+  least = c.time(blocks, stages, 1, share);
+  for (int64_t s = 2; blocks * s <= 1280 && stages >= s * c.least; ++s) {
+    const float t = c.time(blocks, stages, s, share);
     if (t < least) least = t, best = (int)s;
   }
   return best;

@@ -638,8 +638,7 @@ struct FwdPlan {
   int64_t units;  // nq = 0: 32-key units of a range
 };
 
-// even: neither causal nor lengths
-FwdPlan fwd_plan(int B, int H, int Hkv, int64_t Lq, int64_t Lk, bool even) {
+FwdPlan fwd_plan(int B, int H, int Hkv, int64_t Lq, int64_t Lk, float share) {
   FwdPlan p{};
   const int64_t bp = (int64_t)B * H / 2, bk = (int64_t)B * Hkv / 2, rep = H / Hkv;
   const int64_t units = (Lk + kUnitRows - 1) / kUnitRows;
@@ -664,8 +663,8 @@ FwdPlan fwd_plan(int B, int H, int Hkv, int64_t Lq, int64_t Lk, bool even) {
   const int64_t q2 = (Lq + 127) / 128, q1 = (Lq + 63) / 64;
   const SplitCost c2{0.88f, 1.43f, 0.f, 0}, c1{0.53f, 0.74f, 0.033f, 4};
   float t1;
-  p.splits = best_split(bp * q1, units, even, c1, t1);
-  p.nq = c2.time(bp * q2, units, 1, even) < t1 ? 2 : 1;
+  p.splits = best_split(bp * q1, units, share, c1, t1);
+  p.nq = c2.time(bp * q2, units, 1, share) < t1 ? 2 : 1;
   if (p.nq == 2) p.splits = 1;
   p.qtiles = p.nq == 2 ? q2 : q1;
   p.nwork = bp * p.qtiles;
@@ -682,8 +681,8 @@ extern "C" size_t sla2h_diff_attn_fwd_workspace_bytes(int B, int H, int Hkv, int
                                                       int64_t Lk) {
   if (!diff_sizes_ok(B, H, Hkv, Lq, Lk)) return 0;
   size_t most = 0;
-  for (bool even : {false, true}) {
-    const FwdPlan p = fwd_plan(B, H, Hkv, Lq, Lk, even);
+  for (const auto& lens : kShares) for (float share : lens) {
+    const FwdPlan p = fwd_plan(B, H, Hkv, Lq, Lk, share);
     const size_t n = p.splits > 1 ? (size_t)p.splits * B * H * Lq * (128 * 4 + 8) : 0;
     most = n > most ? n : most;
   }
@@ -710,7 +709,7 @@ extern "C" int sla2h_diff_attn_fwd(const void* q, const void* k, const void* v, 
   // 32-bit byte offsets within a tile
   SLA2H_CHECK_ARG(strides[5] < ((int64_t)1 << 23) && strides[8] < ((int64_t)1 << 23));
   const bool even = !causal && !q_lens && !k_lens;
-  const FwdPlan p = fwd_plan(B, H, Hkv, Lq, Lk, even);
+  const FwdPlan p = fwd_plan(B, H, Hkv, Lq, Lk, kShares[causal != 0][q_lens || k_lens]);
   SLA2H_CHECK_ARG(p.splits == 1 || workspace);
   const int64_t nrows = (int64_t)B * (H / 2) * Lq;
   SLA2H_CHECK_ARG(p.nwork * (p.nq ? p.splits : 1) < ((int64_t)1 << 30));

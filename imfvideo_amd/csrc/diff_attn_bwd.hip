@@ -674,17 +674,17 @@ struct BwdPlan {
   size_t stats, dq_parts, kv_parts;  // floats (kv_parts: of dk, and as many of dv)
 };
 
-BwdPlan bwd_plan(int dtype, int B, int H, int Hkv, int64_t Lq, int64_t Lk, bool even) {
+BwdPlan bwd_plan(int dtype, int B, int H, int Hkv, int64_t Lq, int64_t Lk, float share) {
   BwdPlan p{};
   const int64_t bp = (int64_t)B * H / 2, bk = (int64_t)B * Hkv / 2, rep = H / Hkv;
   p.qtiles = (Lq + 127) / 128;
   // (us, unsplit / split, B x H x L: 2 x 8 x 2,048 dq 87 / 63, dk and dv 90 / 69; 1 x 8 x 6,000 204 / 164,
   // 230 / 194; causal 1 x 8 x 12,000 417 / 283, 488 / 339)
   float t;
-  p.dq_splits = best_split(bp * p.qtiles, (Lk + 31) / 32, even, SplitCost{1.15f, 2.f, 0.033f, 8}, t);
+  p.dq_splits = best_split(bp * p.qtiles, (Lk + 31) / 32, share, SplitCost{1.15f, 2.f, 0.033f, 8}, t);
   p.dq_nwork = bp * p.qtiles * p.dq_splits;
   p.ktiles = (Lk + kKeyRows - 1) / kKeyRows;
-  p.kv_splits = best_split(bk * p.ktiles, rep * ((Lq + 31) / 32), even,
+  p.kv_splits = best_split(bk * p.ktiles, rep * ((Lq + 31) / 32), share,
                            SplitCost{1.2f, 2.1f, 0.066f, 8}, t);
   p.kv_nwork = bk * p.ktiles * p.kv_splits;
   p.nqb = (Lq + kNormRows - 1) / kNormRows;
@@ -706,8 +706,8 @@ extern "C" size_t sla2h_diff_attn_bwd_workspace_bytes(int dtype, int B, int H, i
                                                       int64_t Lk) {
   if (!diff_sizes_ok(B, H, Hkv, Lq, Lk)) return 0;
   size_t most = 0;
-  for (bool even : {false, true}) {
-    const BwdPlan p = bwd_plan(dtype, B, H, Hkv, Lq, Lk, even);
+  for (const auto& lens : kShares) for (float share : lens) {
+    const BwdPlan p = bwd_plan(dtype, B, H, Hkv, Lq, Lk, share);
     const size_t n = p.stats + p.dq_parts + 2 * p.kv_parts;
     most = n > most ? n : most;
   }
@@ -738,7 +738,7 @@ extern "C" int sla2h_diff_attn_bwd(const void* q, const void* k, const void* v, 
   for (int i : {2, 5, 8}) SLA2H_CHECK_ARG(strides[i] >= kDD && strides[i] < ((int64_t)1 << 23));
   SLA2H_CHECK_ARG((int64_t)H * kDD < ((int64_t)1 << 23));
   const bool even = !causal && !q_lens && !k_lens;
-  const BwdPlan p = bwd_plan(dtype, B, H, Hkv, Lq, Lk, even);
+  const BwdPlan p = bwd_plan(dtype, B, H, Hkv, Lq, Lk, kShares[causal != 0][q_lens || k_lens]);
   SLA2H_CHECK_ARG(p.dq_nwork < ((int64_t)1 << 30) && p.kv_nwork < ((int64_t)1 << 30));
   const int64_t bp = (int64_t)B * H / 2, bk = (int64_t)B * Hkv / 2;
   const int64_t pq = bp * p.nqb, pv = dtype == SLA2H_DTYPE_F16 ? bk * p.nkb : 0;
