@@ -20,6 +20,9 @@ namespace sla2h {
 
 namespace {
 
+// Sequences of so many units of keys take what the rounding of P lost with a second product.
+constexpr int kFewUnits = 4;
+
 struct DiffFwdArgs {
   const uint16_t *q, *k, *v;
   Weights lam;       // (P)
@@ -216,7 +219,31 @@ __global__ __launch_bounds__(256, 2) void diff_fwd_kernel(DiffFwdArgs a) {
   // last stage that the wave has keys in come behind the loop, and then the waits and loads alone.
   const int wn = min(nt, (wany + kUnitRows - 1) / kUnitRows);
   const unsigned char* last = s0;
-  for (int t = t0; t < wn; t += 5) {
+  int tm = t0;
+  if (NQ == 1 && klen <= kFewUnits * kUnitRows) {  // a short clip in a padded batch: the second product too
+    load(t0 + 3, s3);
+    __builtin_amdgcn_s_waitcnt(wait_vm_lgkm0(0));
+    __builtin_amdgcn_s_barrier();
+    for (; tm < wn; ++tm) {
+      const int x = tm - t0;
+      const unsigned char* s = x == 0 ? s0 : x == 1 ? s1 : x == 2 ? s2 : s3;
+#pragma unroll
+      for (int n = 0; n < NQ; ++n) {
+        u32x4 lost[2];
+        scores(n, s);
+        mask_tile(sc[n], lim[n] - tm * kUnitRows, h);
+        raise_bound(lane_max(sc[n]), a.c, mx[n], lsum[n], acc[n]);
+        lsum[n] += probabilities<T16>(sc[n], a.c, mx[n], pr[n]);
+        lost_halves<T16>(sc[n], a.c, mx[n], pr[n], lost);
+        values(n, s);
+        pr[n][0] = lost[0], pr[n][1] = lost[1];
+        values(n, s);
+        pr[n][0] = pr[n][1] = u32x4{0, 0, 0, 0};
+      }
+    }
+    tm = nt;
+  }
+  for (int t = tm; t < wn; t += 5) {
     stage(t, t == t0 ? s0 : s4, s0, s1, s3);
     last = s0;
     if (t + 1 >= wn) break;
@@ -233,7 +260,7 @@ __global__ __launch_bounds__(256, 2) void diff_fwd_kernel(DiffFwdArgs a) {
     last = s4;
   }
   values(NQ - 1, last);
-  for (int t = max(wn, t0); t < nt; ++t) {
+  for (int t = max(wn, tm); t < nt; ++t) {
     __builtin_amdgcn_s_waitcnt(wait_vm_lgkm0(4));
     __builtin_amdgcn_s_barrier();
     const int x = (t + 3 - t0) % 5;
@@ -638,16 +665,17 @@ struct FwdPlan {
   int64_t units;  // nq = 0: 32-key units of a range
 };
 
-FwdPlan fwd_plan(int B, int H, int Hkv, int64_t Lq, int64_t Lk, float share) {
+FwdPlan fwd_plan(int B, int H, int Hkv, int64_t Lq, int64_t Lk, bool causal, bool lens) {
   FwdPlan p{};
   const int64_t bp = (int64_t)B * H / 2, bk = (int64_t)B * Hkv / 2, rep = H / Hkv;
   const int64_t units = (Lk + kUnitRows - 1) / kUnitRows;
+  const float share = kShares[causal][lens];
   // A group's rows in one tile read their keys once (us, in this form / in query blocks: 64 clips, H = 16,
   // Hkv = 2, 1 query, 2,000 keys 23 / 64; 1 clip, 29,952 keys 18 / 27; 32 clips, 32, 4, 4 queries
   // 27 / 48; in two tiles and more: 8 clips, 16, 2, 16 queries 20 / 18).  A row of few keys needs the second
   // product: the rounding of P_m is a part of delta_m, and of dA - delta_m, which then nearly cancel (2
   // keys: dq and dk six times as far off; 100 of 100 keys 10 / 8 us).
-  if (units <= 4 || (rep > 1 && rep * Lq <= 32)) {
+  if (units <= kFewUnits || (rep > 1 && rep * Lq <= 32)) {
     p.qtiles = (rep * Lq + 31) / 32;
     const int64_t blocks = bk * p.qtiles;
     const int64_t s = 512 / blocks, most = units / 8;  // two units per wave and range at least
@@ -657,14 +685,14 @@ FwdPlan fwd_plan(int B, int H, int Hkv, int64_t Lq, int64_t Lk, float share) {
     p.nwork = blocks * p.splits;
     return p;
   }
-  // 128 rows (no ranges) or 64, by what a stage takes (SplitCost) with one and two workgroups per CU.  us,
+  // 128 rows (no ranges; not where lengths may leave few keys) or 64, by what a stage takes (SplitCost) with one and two workgroups per CU.  us,
   // 128 / 64, H = 8: 1 clip of 8,192 231 / 208, of 12,000 476 / 479, of 16,384 738 / 809, 4 clips of
   // 2,048, H = 16, 106 / 113; causal 12,000 334 / 244, 24,000 831 / 870.
   const int64_t q2 = (Lq + 127) / 128, q1 = (Lq + 63) / 64;
   const SplitCost c2{0.88f, 1.43f, 0.f, 0}, c1{0.53f, 0.74f, 0.033f, 4};
   float t1;
   p.splits = best_split(bp * q1, units, share, c1, t1);
-  p.nq = c2.time(bp * q2, units, 1, share) < t1 ? 2 : 1;
+  p.nq = !lens && c2.time(bp * q2, units, 1, share) < t1 ? 2 : 1;
   if (p.nq == 2) p.splits = 1;
   p.qtiles = p.nq == 2 ? q2 : q1;
   p.nwork = bp * p.qtiles;
@@ -681,8 +709,8 @@ extern "C" size_t sla2h_diff_attn_fwd_workspace_bytes(int B, int H, int Hkv, int
                                                       int64_t Lk) {
   if (!diff_sizes_ok(B, H, Hkv, Lq, Lk)) return 0;
   size_t most = 0;
-  for (const auto& lens : kShares) for (float share : lens) {
-    const FwdPlan p = fwd_plan(B, H, Hkv, Lq, Lk, share);
+  for (int i = 0; i < 4; ++i) {
+    const FwdPlan p = fwd_plan(B, H, Hkv, Lq, Lk, i & 1, i & 2);
     const size_t n = p.splits > 1 ? (size_t)p.splits * B * H * Lq * (128 * 4 + 8) : 0;
     most = n > most ? n : most;
   }
@@ -709,7 +737,7 @@ extern "C" int sla2h_diff_attn_fwd(const void* q, const void* k, const void* v, 
   // 32-bit byte offsets within a tile
   SLA2H_CHECK_ARG(strides[5] < ((int64_t)1 << 23) && strides[8] < ((int64_t)1 << 23));
   const bool even = !causal && !q_lens && !k_lens;
-  const FwdPlan p = fwd_plan(B, H, Hkv, Lq, Lk, kShares[causal != 0][q_lens || k_lens]);
+  const FwdPlan p = fwd_plan(B, H, Hkv, Lq, Lk, causal != 0, q_lens || k_lens);
   SLA2H_CHECK_ARG(p.splits == 1 || workspace);
   const int64_t nrows = (int64_t)B * (H / 2) * Lq;
   SLA2H_CHECK_ARG(p.nwork * (p.nq ? p.splits : 1) < ((int64_t)1 << 30));

@@ -706,7 +706,8 @@ extern "C" size_t sla2h_diff_attn_bwd_workspace_bytes(int dtype, int B, int H, i
                                                       int64_t Lk) {
   if (!diff_sizes_ok(B, H, Hkv, Lq, Lk)) return 0;
   size_t most = 0;
-  for (const auto& lens : kShares) for (float share : lens) {
+  for (int i = 0; i < 4; ++i) {
+    const float share = kShares[i & 1][i >> 1];
     const BwdPlan p = bwd_plan(dtype, B, H, Hkv, Lq, Lk, share);
     const size_t n = p.stats + p.dq_parts + 2 * p.kv_parts;
     most = n > most ? n : most;

@@ -189,6 +189,21 @@ def test_few_keys_keep_the_gradients_accuracy(Lq, Lk, causal, dt):
         assert err <= 1.5 * 2 ** 0.5 * u / 3 ** 0.5 * want[n][0].norm().item(), n
 
 
+@pytest.mark.parametrize("B,H,L", [(2, 4, 900), (3, 8, 5000)])
+def test_a_short_clip_keeps_its_accuracy_in_a_padded_batch(B, H, L):
+    """The clip's gradients are as far off as roundings in norm are (as above), among long ones."""
+    x, lam, do = operands(18, B, L, H, dt=torch.float16)
+    lens = [L, 3, 100][:B]
+    got = call(x, lam, do, q_lens=lens, k_lens=lens)
+    want = R.attention(*x, lam, ql=lens, kl=lens, do=do, dev="cuda")
+    for b in range(1, B):
+        for n in ("o", "dq", "dk", "dv"):
+            w = want[n][0][b]
+            err = (got[n][b].double() - w).norm().item()
+            print("[ratio]", b, n, err / w.norm().item() * 2 ** 11, flush=True)
+            assert err <= 1.5 * 2 ** 0.5 * 2 ** -11 / 3 ** 0.5 * w.norm().item(), (b, n)
+
+
 @pytest.mark.parametrize("ql,kl", [([-3, 400], [400, 2 ** 31 - 1]), ([401, 0], [0, 17])])
 def test_lengths_are_clamped(ql, kl):
     x, lam, do = operands(14, 2, 400, 2)
