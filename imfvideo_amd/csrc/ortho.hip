@@ -10,8 +10,8 @@
 // be 1e-2 off.  Every intermediate is therefore a pair of fp16 numbers hi + lo, 22 bits of a value
 // scaled by a power of two that keeps lo a normal number (absolute resolution 2^-25 of a unit), and a
 // product of two pairs is three products of the matrix cores, hi hi + hi lo + lo hi, summed in fp32:
-// lo lo, below 2^-24 of the product, is what fp32 arithmetic rounds off too.  (In A^2, where the squares of
-// the diagonal's lo add up, it is the fourth: 0.7e-6 of the result otherwise for 20 rows.)  The result
+// lo lo, below 2^-24 of the product, is what fp32 arithmetic rounds off too.  (In A^2 of up to 128 rows,
+// where the squares of the diagonal's lo show, it is the fourth: 20 rows 0.7e-6 off otherwise.)  The result
 // is as exact as with fp32 products, at three times the 16-bit rate's cost.
 #include "dense_attn.h"
 
@@ -218,7 +218,7 @@ __device__ inline void store_row8(const OrthoArgs& a, int dtype, int64_t mat, in
   *reinterpret_cast<u32x4*>(static_cast<uint16_t*>(a.out) + at) = x;
 }
 
-enum { kGram, kPoly, kStep, kLast };
+enum { kGram, kPoly, kPolyFew, kStep, kLast };
 
 // Offsets of the transposed operand whose slots follow row_frag's order: rows 8 h + 4 x + 0 .. 3.
 // (Channels 32 mb on: four chunks further, a bit of the address that no swizzle carries into.)
@@ -247,11 +247,11 @@ __device__ inline u32x4 turned_frag(const unsigned char* tile, int s, int mb, co
 // registers, i along the lanes; it goes through LDS, so that whole rows are stored (from the registers,
 // eight bytes to a row: kStep 105 us for 91, kGram 65 for 58).  24 x 512 x 2048: kGram 1.0, kStep 0.92 PFLOP/s of
 // 16-bit products, with 200 MB read and written beside kStep's.
-//   kGram: A = X X^T;  kPoly: B = b A + c A A^T;  kStep: Y = a X + B X;  kLast: that, to G's type
+//   kGram: A = X X^T;  kPoly: B = b A + c A A^T (kPolyFew: with lo lo);  kStep: Y = a X + B X;  kLast: that, to G's type
 template <int T, int OP>
 __global__ __launch_bounds__(256, T == 128 && OP < kStep ? 1 : 2) void ortho_product_kernel(
     OrthoArgs a, int dtype, int work) {
-  constexpr bool STEP = OP >= kStep;
+  constexpr bool STEP = OP >= kStep, POLY = OP == kPoly || OP == kPolyFew;
   constexpr int NT = T / 64;      // 32 x 32 tiles of a wave: NT x NT
   constexpr int NU = T / 32;      // 32-row units (4 KB) of an operand's stage
   constexpr int kUnit = 32 * kRowB;
@@ -283,7 +283,7 @@ __global__ __launch_bounds__(256, T == 128 && OP < kStep ? 1 : 2) void ortho_pro
   const int64_t px = (int64_t)2 * a.rp * a.mp, pa = (int64_t)2 * a.rp * a.rp;
   const uint16_t* X = a.x + mat * px;
   const uint16_t* A = a.A + mat * pa;
-  const uint16_t* P = OP == kGram ? X : OP == kPoly ? A : a.B + mat * pa;  // rows i
+  const uint16_t* P = OP == kGram ? X : POLY ? A : a.B + mat * pa;  // rows i
   const int ldp = (OP == kGram ? a.mp : a.rp) * 4, ldx = a.mp * 4;         // bytes
   const int K = OP == kGram ? a.mp : a.rp;
 
@@ -326,7 +326,7 @@ __global__ __launch_bounds__(256, T == 128 && OP < kStep ? 1 : 2) void ortho_pro
     if (OP == kGram || p0 * kRows >= ni || jl >= nj) return;
 #pragma unroll
     for (int p = 0; p < kPass; ++p) {
-      const uint16_t* s = (OP == kPoly ? A : X) +
+      const uint16_t* s = (POLY ? A : X) +
                           pair_index(it * T + il + (p0 + p) * kRows, jt * T + jl, ld);
       ph[p] = *reinterpret_cast<const u32x4*>(s);
       pl[p] = *reinterpret_cast<const u32x4*>(s + 32);
@@ -395,7 +395,7 @@ __global__ __launch_bounds__(256, T == 128 && OP < kStep ? 1 : 2) void ortho_pro
         products(f, 0, 0, z - NT, acc);
       else
         products(f, 0, 1, z - 2 * NT, low);
-      if (OP == kPoly && z >= 2 * NT) products(f, 1, 1, z - 2 * NT, low);
+      if (OP == kPolyFew && z >= 2 * NT) products(f, 1, 1, z - 2 * NT, low);
       __builtin_amdgcn_sched_barrier(0);
     }
   };
@@ -489,7 +489,7 @@ __global__ __launch_bounds__(256, T == 128 && OP < kStep ? 1 : 2) void ortho_pro
     for (int e = 0; e < 8; ++e) {
       const float p = OP == kGram ? 0.f : pair_at(hi[e >> 1], lw[e >> 1], e & 1);
       v[e] = OP == kGram   ? v[e] * (1.f / kScaleX)
-             : OP == kPoly ? __builtin_fmaf(cc, v[e], cb * p)
+             : POLY ? __builtin_fmaf(cc, v[e], cb * p)
                            : __builtin_fmaf(a.a, p, (1.f / kScaleB) * v[e]);
     }
   };
@@ -505,7 +505,7 @@ __global__ __launch_bounds__(256, T == 128 && OP < kStep ? 1 : 2) void ortho_pro
     *reinterpret_cast<u32x4*>(d) = hi;
     *reinterpret_cast<u32x4*>(d + 32) = lw;
   };
-  uint16_t* base = OP == kGram ? a.A + mat * pa : OP == kPoly ? a.B + mat * pa : a.y + mat * px;
+  uint16_t* base = OP == kGram ? a.A + mat * pa : POLY ? a.B + mat * pa : a.y + mat * px;
   if (jl < nj)
     for (int p0 = 0; p0 * kRows < ni; p0 += kPass) {
       float v[kPass][8];
@@ -547,7 +547,7 @@ __global__ __launch_bounds__(256, T == 128 && OP < kStep ? 1 : 2) void ortho_pro
         if (j0 >= nj) continue;
         const int ic = i0 + 8 * (l & 3), jc = j0 + (l >> 2), i = it * T + ic, j = jt * T + jc;
         u32x4 hi{}, lw{};
-        if (OP == kPoly) {
+        if (POLY) {
           const uint16_t* s = A + pair_index(j, i, ld);
           hi = *reinterpret_cast<const u32x4*>(s);
           lw = *reinterpret_cast<const u32x4*>(s + 32);
@@ -752,11 +752,11 @@ int ortho_product(const OrthoArgs& a, int dtype, hipStream_t st) {
   // 256, 2048: 64 / 76; Gram and square 240, 512: 19 / 19; 400, 512: 33 / 27; 480, 512: 39 / 35; 72, 2048:
   // 36 / 27; 136, 2048: 40 / 44; 240, 2048: 48 / 53; 528, 4096: 230 / 330.
   const bool deep = (OP == kGram ? a.mp : a.rp) >= 2048;
-  const bool wide = OP >= kStep ? tiles(128) >= (deep ? 200 : 300) : deep && tiles(128) >= 130;
+  const bool wide = OP == kPolyFew ? false : OP >= kStep ? tiles(128) >= (deep ? 200 : 300) : deep && tiles(128) >= 130;
   const int64_t work = tiles(wide ? 128 : 64);
   const unsigned grid = 8u * (unsigned)((work + 7) / 8);
   if (wide)
-    ortho_product_kernel<128, OP><<<grid, 256, 0, st>>>(a, dtype, (int)work);
+    ortho_product_kernel<OP == kPolyFew ? 64 : 128, OP><<<grid, 256, 0, st>>>(a, dtype, (int)work);
   else
     ortho_product_kernel<64, OP><<<grid, 256, 0, st>>>(a, dtype, (int)work);
   return (int)hipGetLastError();
@@ -809,7 +809,9 @@ extern "C" int sla2h_orthogonalize(const void* g, int dtype, int64_t n, int64_t 
   for (int s = 0; s < steps; ++s) {
     a.a = coeffs[3 * s], a.b = coeffs[3 * s + 1], a.c = coeffs[3 * s + 2];
     if ((err = ortho_product<kGram>(a, dtype, st))) return err;
-    if ((err = ortho_product<kPoly>(a, dtype, st))) return err;
+    // (few rows: 8 x 448 x 448 would take 175 us for 150 with the fourth product, and gain nothing)
+    err = a.rp <= 128 ? ortho_product<kPolyFew>(a, dtype, st) : ortho_product<kPoly>(a, dtype, st);
+    if (err) return err;
     if ((err = s + 1 < steps ? ortho_product<kStep>(a, dtype, st)
                              : ortho_product<kLast>(a, dtype, st)))
       return err;
