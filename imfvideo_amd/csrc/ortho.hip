@@ -378,7 +378,9 @@ __global__ __launch_bounds__(256, T == 128 && OP < kStep ? 1 : 2) void ortho_pro
   };
   // The same, while the operands of the next half stage are read and, where k is 1, a stage's loads
   // issued: a wave issues in order, so that what stands between two products takes their time unless
-  // it is less than one of them.
+  // it is less than one of them.  The order is fixed for T = 128.  T = 64, whose workgroups run in step,
+  // is left to the compiler: with the fixed order its bursts make some cards lower their clock (8 x 512 x
+  // 512, one call after another: 238 us for 176; zeros, which draw less, 148 for 154).
   auto half = [&](const Frags& f, const unsigned char* s, int k, Frags& next, int k0,
                   unsigned char* to) __attribute__((always_inline)) {
 #pragma unroll
@@ -388,7 +390,7 @@ __global__ __launch_bounds__(256, T == 128 && OP < kStep ? 1 : 2) void ortho_pro
       if (z == NT) read_j(s, k, 0, next);
       if (z == 2 * NT - 1 + (NT == 1)) read_i(s, k, 1, next);
       if (k && z < NU) load(k0, to, z, z + 1);
-      __builtin_amdgcn_sched_barrier(0);
+      if (T == 128) __builtin_amdgcn_sched_barrier(0);
       if (z < NT)
         products(f, 1, 0, z, low);
       else if (z < 2 * NT)
@@ -396,7 +398,7 @@ __global__ __launch_bounds__(256, T == 128 && OP < kStep ? 1 : 2) void ortho_pro
       else
         products(f, 0, 1, z - 2 * NT, low);
       if (OP == kPolyFew && z >= 2 * NT) products(f, 1, 1, z - 2 * NT, low);
-      __builtin_amdgcn_sched_barrier(0);
+      if (T == 128) __builtin_amdgcn_sched_barrier(0);
     }
   };
   // (K is a multiple of 64; a stage's loads: 2 NU per wave)
