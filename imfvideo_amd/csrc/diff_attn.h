@@ -39,11 +39,11 @@ inline bool diff_sizes_ok(int B, int H, int Hkv, int64_t Lq, int64_t Lk) {
   return sizes_ok(B, H, Hkv, Lq, Lk) && H % 2 == 0 && Hkv % 2 == 0;
 }
 
-// What a launch of workgroups, two of which fit on a CU, takes (us on this card, without launching): per
-// stage `two` for every full round of 512 and, for the rest, `one` while each has a CU of its own.  Work
-// of unequal workgroups (share below 1: what is left of all of it on average) has no rounds, but takes no less
-// than its longest one, a fifth more for its neighbours.  Ranges of a long axis: `join` more per
-// workgroup for its partial sums' way through memory, and the launch that adds them.
+// What a launch of workgroups, two of which fit on a CU, takes (us on this card, without launching):
+// per stage `two` for every full round of 512 and, for the rest, `one` while each has a CU of its own.
+// Work of unequal workgroups (share below 1: what is left of all of it on average) has no rounds, but
+// takes no less than its longest one, a fifth more for its neighbours.  Ranges of a long axis: `join`
+// more per workgroup for its partial sums' way through memory, and the launch that adds them.
 struct SplitCost {
   float one, two, join;
   int least;  // stages of a range
@@ -57,11 +57,11 @@ struct SplitCost {
   }
 };
 constexpr float kShares[2][2] = {{1.f, 0.7f}, {0.5f, 0.35f}};  // causal, lengths
-// The number of ranges that takes least.
+// The number of ranges that takes least (of many, every eighth part more is tried).
 inline int best_split(int64_t blocks, int64_t stages, float share, const SplitCost& c, float& least) {
   int best = 1;
   least = c.time(blocks, stages, 1, share);
-  for (int64_t s = 2; blocks * s <= 1280 && stages >= s * c.least; ++s) {
+  for (int64_t s = 2; blocks * s <= 1280 && stages >= s * c.least; s += s < 16 ? 1 : s / 8) {
     const float t = c.time(blocks, stages, s, share);
     if (t < least) least = t, best = (int)s;
   }

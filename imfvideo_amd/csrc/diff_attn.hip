@@ -381,12 +381,12 @@ __device__ inline void finish_row(const DiffFwdArgs& a, int64_t bp, int64_t i, i
   *reinterpret_cast<u32x4*>(out_row(a, bp, i) + c0) = z;
 }
 
-// Few queries of grouped heads, or few keys: workgroup = 32 rows of the `rep` query pairs that share a key pair, over
-// one range of keys; its four waves take the 32-key units in turn, both maps of a unit, each with an LDS
-// slot of its own (no barrier in the loop), and their sums are joined in LDS.  A wave waits for its unit
-// and computes it while the others' units are on their way (eight waves, one workgroup per CU: no
-// faster).  The products wait for the loads here, so what the rounding of P lost is always added by
-// a second one.
+// Few queries of grouped heads, or few keys: workgroup = 32 rows of the `rep` query pairs that share a
+// key pair, over one range of keys; its four waves take the 32-key units in turn, both maps of a unit,
+// each with an LDS slot of its own (no barrier in the loop), and their sums are joined in LDS.  A wave
+// waits for its unit and computes it while the others' units are on their way (eight waves, one
+// workgroup per CU: no faster).  The products wait for the loads here, so what the rounding of P lost
+// is always added by a second one.
 constexpr int W = 4;  // waves
 template <typename T16>
 __global__ __launch_bounds__(64 * W, 2) void diff_fwd_split_kernel(DiffFwdArgs a) {
@@ -685,8 +685,8 @@ FwdPlan fwd_plan(int B, int H, int Hkv, int64_t Lq, int64_t Lk, bool causal, boo
     p.nwork = blocks * p.splits;
     return p;
   }
-  // 128 rows (no ranges; not where lengths may leave few keys) or 64, by what a stage takes (SplitCost) with one and two workgroups per CU.  us,
-  // 128 / 64, H = 8: 1 clip of 8,192 231 / 208, of 12,000 476 / 479, of 16,384 738 / 809, 4 clips of
+  // 128 rows (no ranges; not where lengths may leave few keys) or 64, by what a stage takes (SplitCost)
+  // with one and two workgroups per CU.  us, 128 / 64, H = 8: 1 clip of 8,192 231 / 208, of 12,000 476 / 479, of 16,384 738 / 809, 4 clips of
   // 2,048, H = 16, 106 / 113; causal 12,000 334 / 244, 24,000 831 / 870.
   const int64_t q2 = (Lq + 127) / 128, q1 = (Lq + 63) / 64;
   const SplitCost c2{0.88f, 1.43f, 0.f, 0}, c1{0.53f, 0.74f, 0.033f, 4};
@@ -718,8 +718,8 @@ extern "C" size_t sla2h_diff_attn_fwd_workspace_bytes(int B, int H, int Hkv, int
 }
 
 extern "C" int sla2h_diff_attn_fwd(const void* q, const void* k, const void* v, const void* lam,
-                                   int lam_dtype, int64_t lam_stride, const int64_t* strides, const int32_t* q_lens,
-                                   const int32_t* k_lens, int dtype, int B, int H, int Hkv,
+                                   int lam_dtype, int64_t lam_stride, const int64_t* strides,
+                                   const int32_t* q_lens, const int32_t* k_lens, int dtype, int B, int H, int Hkv,
                                    int64_t Lq, int64_t Lk, int causal, float scale,
                                    void* workspace, void* o, float* lse, float* maps,
                                    void* stream) {

@@ -245,9 +245,10 @@ __device__ inline u32x4 turned_frag(const unsigned char* tile, int s, int mb, co
 // three stages ahead, the operands of half a stage read beside the products of the half before (left to
 // the compiler's order: 24 x 512 x 2048, kGram 63 us for 48).  Result element (i, j): j along the
 // registers, i along the lanes; it goes through LDS, so that whole rows are stored (from the registers,
-// eight bytes to a row: kStep 105 us for 91, kGram 65 for 58).  24 x 512 x 2048: kGram 1.0, kStep 0.92 PFLOP/s of
-// 16-bit products, with 200 MB read and written beside kStep's.
-//   kGram: A = X X^T;  kPoly: B = b A + c A A^T (kPolyFew: with lo lo);  kStep: Y = a X + B X;  kLast: that, to G's type
+// eight bytes to a row: kStep 105 us for 91, kGram 65 for 58).  24 x 512 x 2048: kGram 1.0, kStep 0.92
+// PFLOP/s of 16-bit products, with 200 MB read and written beside kStep's.
+//   kGram: A = X X^T;  kPoly: B = b A + c A A^T (kPolyFew: with lo lo);  kStep: Y = a X + B X;
+//   kLast: that, to G's type
 template <int T, int OP>
 __global__ __launch_bounds__(256, T == 128 && OP < kStep ? 1 : 2) void ortho_product_kernel(
     OrthoArgs a, int dtype, int work) {
@@ -724,12 +725,14 @@ __global__ __launch_bounds__(512, 2) void ortho_small_kernel(OrthoArgs a, int dt
 
 struct OrthoPlan {
   int r, m, rp, mp, parts;
+  bool small;     // one launch, no workspace
   size_t sums, x, A;  // bytes of the sums, of X, of A
 };
 bool ortho_plan(int64_t n, int64_t R, int64_t C, OrthoPlan& p) {
   if (n <= 0 || R <= 0 || C <= 0 || R > 32768 || C > 32768) return false;
   p.r = (int)(R < C ? R : C);
   p.m = (int)(R < C ? C : R);
+  p.small = p.r <= 64 && p.m <= kSmallM;
   p.rp = (p.r + 63) & ~63;
   p.mp = (p.m + 63) & ~63;
   // (numbers of workgroups and bytes of all matrices)
@@ -754,7 +757,9 @@ int ortho_product(const OrthoArgs& a, int dtype, hipStream_t st) {
   // 256, 2048: 64 / 76; Gram and square 240, 512: 19 / 19; 400, 512: 33 / 27; 480, 512: 39 / 35; 72, 2048:
   // 36 / 27; 136, 2048: 40 / 44; 240, 2048: 48 / 53; 528, 4096: 230 / 330.
   const bool deep = (OP == kGram ? a.mp : a.rp) >= 2048;
-  const bool wide = OP == kPolyFew ? false : OP >= kStep ? tiles(128) >= (deep ? 200 : 300) : deep && tiles(128) >= 130;
+  const bool wide = OP == kPolyFew ? false
+                    : OP >= kStep  ? tiles(128) >= (deep ? 200 : 300)
+                                   : deep && tiles(128) >= 130;
   const int64_t work = tiles(wide ? 128 : 64);
   const unsigned grid = 8u * (unsigned)((work + 7) / 8);
   if (wide)
@@ -772,7 +777,8 @@ using namespace sla2h;
 
 extern "C" size_t sla2h_orthogonalize_workspace_bytes(int64_t n, int64_t R, int64_t C) {
   OrthoPlan p;
-  return ortho_plan(n, R, C, p) ? p.sums + 2 * p.x + 2 * p.A : 0;
+  if (!ortho_plan(n, R, C, p)) return 0;
+  return p.small ? 256 : p.sums + 2 * p.x + 2 * p.A;
 }
 
 extern "C" int sla2h_orthogonalize(const void* g, int dtype, int64_t n, int64_t R, int64_t C,
@@ -796,7 +802,7 @@ extern "C" int sla2h_orthogonalize(const void* g, int dtype, int64_t n, int64_t 
   a.wide_out = C % 8 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0;
   hipStream_t st = static_cast<hipStream_t>(stream);
   int err;
-  if (p.r <= 64 && p.m <= kSmallM) {
+  if (p.small) {
     NsTable t{};
     for (int i = 0; i < 3 * steps; ++i) t.v[i] = coeffs[i];
     ortho_small_kernel<<<(unsigned)n, 512, 0, st>>>(a, dtype, steps, t);

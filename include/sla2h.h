@@ -993,8 +993,8 @@ int sla2h_diff_attn_fwd(const void* q, const void* k, const void* v, const void*
  *   dk_m = scale dS_m^T q_m, dv = (A_1 - lam A_2)^T dout, dlam_p = -sum delta_2,
  * dk and dv summed over the query pairs of a key pair, dlam over rows and batch.  Operands, lens, sizes,
  * causal, scale, lse and maps as in the forward; dout (B, Lq, H, 64) contiguous.  dq (B, Lq, H,
- * 64), dk, dv (B, Lk, Hkv, 64) contiguous 16-bit, dlam (H / 2) of lam_dtype, contiguous; dq, or dk and dv together, may
- * be NULL (not computed).  Gradients of rows behind a sequence and of rows without a key are 0; dout is
+ * 64), dk, dv (B, Lk, Hkv, 64) contiguous 16-bit, dlam (H / 2) of lam_dtype, contiguous; dq, or dk and
+ * dv together, may be NULL (not computed).  Gradients of rows behind a sequence and of rows without a key are 0; dout is
  * not read there.  No atomics: reproducible bit for bit.
  */
 size_t sla2h_diff_attn_bwd_workspace_bytes(int dtype, int B, int H, int Hkv, int64_t Lq,

@@ -111,3 +111,14 @@ def test_operands_that_the_kernels_do_not_take():
     for dtype, steps, ws in ((3, 1, 16), (2, 0, 16), (2, 65, 16), (2, 1, 8), (2, 1, None)):
         assert lib.sla2h_orthogonalize(16, dtype, 1, 4, 4, steps, ops._ns_coeffs(1, ops.NS_COEFFS),
                                        ws, 16, None) == 1
+
+
+def test_sides_past_the_kernels():
+    with pytest.raises(ValueError, match="32,768"):
+        Muon([torch.nn.Parameter(torch.zeros(32769, 1))])
+    Muon([torch.nn.Parameter(torch.zeros(32768, 1))])
+    lib = ops._lib.load()
+    size = lib.sla2h_orthogonalize_workspace_bytes
+    assert size(1, 32768, 32768) > 0 and size(1, 32769, 1) == 0 and size(0, 1, 1) == 0
+    # matrices that one workgroup holds need none
+    assert size(1 << 20, 64, 512) == size(1, 1, 1) < 1024 < size(1, 65, 512)
