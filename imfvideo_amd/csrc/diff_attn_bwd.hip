@@ -5,10 +5,10 @@
 //   dq_m = scale dS_m k_m,  dk_m = scale dS_m^T q_m,  dv = (A_1 - lam A_2)^T do,
 //   dlam = -sum delta_2     (dk, dv summed over the query pairs of a key pair).
 //
-// Both maps share dA, and the combined map has one product with do: a wave holds both.  Three
+// Both maps share dA, and the combined map has one product with do: a wave holds both.  The
 // launches: the rows' delta; dk and dv with a workgroup per key block (queries streamed through
 // LDS); dq with a workgroup per query block (keys streamed) and, in workgroups of its own, the sum of
-// dlam.  14 products of 64 channels per (query, key) where one fused pass has 10, but no sum goes through
+// dlam; where ranges of an axis are computed apart, their sum.  14 products of 64 channels per (query, key) where one fused pass has 10, but no sum goes through
 // atomics or memory: the result does not depend on the order of dispatch.
 //
 // fp16 operands: maps (down to 1 / length) and dS would fall below fp16's normal range, so the
@@ -62,7 +62,7 @@ struct DiffBwdArgs {
   float* lsum;          // (B, P, nqb): sums of -delta_2
   int nqb, nkb;
   WorkMap dq_map, kv_map;  // tiles x splits of a query pair, of a key pair
-  int dq_splits, kv_splits, dq_blocks;
+  int dq_splits, kv_splits, dq_blocks, kv_blocks;
   float *dq_part, *dk_part, *dv_part;
 };
 
@@ -217,11 +217,12 @@ __device__ inline void store_part(float* p, const f32x16 (&x)[2], float f, int h
 // through four LDS slots, three ahead.  dQ_m^T += K_m^T dS_m^T with dS_m^T straight from the score
 // tile's registers.
 template <typename T16>
-__global__ __launch_bounds__(256, 2) void diff_bwd_dq_kernel(DiffBwdArgs a) {
-  __shared__ __align__(16) unsigned char s0[kStageB], s1[kStageB], s2[kStageB], s3[kStageB];
+__device__ inline __attribute__((always_inline)) void dq_of(const DiffBwdArgs& a, int blk,
+                                                            unsigned char* s0, unsigned char* s1,
+                                                            unsigned char* s2, unsigned char* s3) {
   const int tid = threadIdx.x, l = tid & 63, h = l >> 5;
-  if ((int)blockIdx.x >= a.dq_blocks) {  // dlam of a pair: batch by batch, block by block
-    const int p = blockIdx.x - a.dq_blocks;
+  if (blk >= a.dq_blocks) {  // dlam of a pair: batch by batch, block by block
+    const int p = blk - a.dq_blocks;
     float* red = reinterpret_cast<float*>(s0);
     float s = 0.f;
     const int64_t n = (int64_t)a.B * a.nqb;
@@ -244,7 +245,7 @@ __global__ __launch_bounds__(256, 2) void diff_bwd_dq_kernel(DiffBwdArgs a) {
     return;
   }
   int bp, item;
-  if (!work_item(a.dq_map, blockIdx.x, bp, item)) return;
+  if (!work_item(a.dq_map, blk, bp, item)) return;
   const int qt = item / a.dq_splits, sp = item - qt * a.dq_splits;
   const int b = bp / a.P, p = bp - b * a.P, kp = p / a.rep;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -406,12 +407,12 @@ __device__ inline float row_value_at(float x, int e) {  // e a constant where it
 // statistic belongs to one register of a score tile in all lanes of a half: a lane reads one value, and
 // the add takes it from there (DPP).
 template <typename T16, bool CAUSAL, bool FINE>
-__global__ __launch_bounds__(256, 2) void diff_bwd_dkdv_kernel(DiffBwdArgs a) {
-  __shared__ __align__(16) unsigned char r0[kStageB], r1[kStageB];
-  __shared__ __align__(16) float t0_[4][64], t1_[4][64];
-  __shared__ __align__(16) unsigned char vt[4][2 * kUnitB];
+__device__ inline __attribute__((always_inline)) void dkdv_of(const DiffBwdArgs& a, int blk,
+                                                              unsigned char* r0, unsigned char* r1,
+                                                              float (*t0_)[64], float (*t1_)[64],
+                                                              unsigned char* vt) {
   int bk, item;
-  if (!work_item(a.kv_map, blockIdx.x, bk, item)) return;
+  if (!work_item(a.kv_map, blk, bk, item)) return;
   const int ktile = item / a.kv_splits, sp = item - ktile * a.kv_splits;
   const int b = bk / a.Pk, kp = bk - b * a.Pk;
   const int tid = threadIdx.x, l = tid & 63, h = l >> 5;
@@ -433,7 +434,7 @@ __global__ __launch_bounds__(256, 2) void diff_bwd_dkdv_kernel(DiffBwdArgs a) {
 #pragma unroll
   for (int m = 0; m < 2; ++m)
     load_unit(a.v + b * a.vb + (2 * kp + m) * a.vh, kw, (int64_t)klen - kw, a.vl * 2,
-              vt[w] + m * kUnitB, l);
+              vt + (2 * w + m) * kUnitB, l);
 
   // the stage to load next, and the one to compute (their pair of the group and first row)
   int lu = u0, lp = u0 < u1 ? u0 / nq : 0;
@@ -521,7 +522,7 @@ __global__ __launch_bounds__(256, 2) void diff_bwd_dkdv_kernel(DiffBwdArgs a) {
           const int j = i / 3 * 2 + i % 3 - 1, r = i % (AHEAD + 1);  // j: dA's products
           fa[r] = i % 3 ? row_frag(s + (2 + (j >> 2)) * kUnitB, 0, j & 3, lo)
                         : row_frag(s, 0, i / 3, lo);
-          if (i % 3) fb[r] = row_frag(vt[0] + vw + (j >> 2) * kUnitB, 0, j & 3, lo);
+          if (i % 3) fb[r] = row_frag(vt + vw + (j >> 2) * kUnitB, 0, j & 3, lo);
         };
 #pragma unroll
         for (int i = 0; i < AHEAD; ++i) operands(i);
@@ -651,19 +652,48 @@ __global__ __launch_bounds__(256, 2) void diff_bwd_dkdv_kernel(DiffBwdArgs a) {
   }
 }
 
-// Adds the parts of up to two results in order (blockIdx.y), n values each.
+// The launches.  Calls that take the lost halves everywhere are small: both in one, side by side (2 x 4
+// x 274 tokens 27 us, one after the other 45).  Of others the two bodies under one allocation spill 20
+// registers (29,952 tokens: 7.65 ms, one after the other 7.2).
+template <typename T16, bool CAUSAL>
+__global__ __launch_bounds__(256, 2) void diff_bwd_few_kernel(DiffBwdArgs a) {
+  __shared__ __align__(16) unsigned char s0[kStageB], s1[kStageB], v[2 * kStageB];
+  __shared__ __align__(16) float t0_[4][64], t1_[4][64];
+  const int blk = blockIdx.x;
+  if (blk < a.kv_blocks)
+    dkdv_of<T16, CAUSAL, true>(a, blk, s0, s1, t0_, t1_, v);
+  else
+    dq_of<T16>(a, blk - a.kv_blocks, s0, s1, v, v + kStageB);
+}
+template <typename T16, bool CAUSAL>
+__global__ __launch_bounds__(256, 2) void diff_bwd_dkdv_kernel(DiffBwdArgs a) {
+  __shared__ __align__(16) unsigned char s0[kStageB], s1[kStageB], v[2 * kStageB];
+  __shared__ __align__(16) float t0_[4][64], t1_[4][64];
+  dkdv_of<T16, CAUSAL, false>(a, blockIdx.x, s0, s1, t0_, t1_, v);
+}
 template <typename T16>
-__global__ __launch_bounds__(256) void diff_bwd_join_kernel(const float* __restrict__ part0,
-                                                            const float* __restrict__ part1,
-                                                            int splits, int64_t n, uint16_t* y0,
-                                                            uint16_t* y1) {
-  const int64_t e = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+__global__ __launch_bounds__(256, 2) void diff_bwd_dq_kernel(DiffBwdArgs a) {
+  __shared__ __align__(16) unsigned char s0[kStageB], s1[kStageB], s2[kStageB], s3[kStageB];
+  dq_of<T16>(a, blockIdx.x, s0, s1, s2, s3);
+}
+
+// Adds the parts of a result in order; blockIdx.y: which.
+struct JoinArgs {
+  const float* part[3];
+  uint16_t* y[3];
+  int64_t n[3];
+  int splits[3];
+};
+template <typename T16>
+__global__ __launch_bounds__(256) void diff_bwd_join_kernel(JoinArgs a) {
+  const int64_t e = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4, n = a.n[blockIdx.y];
   if (e >= n) return;
-  const float* part = blockIdx.y ? part1 : part0;
+  const float* part = a.part[blockIdx.y] + e;
+  const int splits = a.splits[blockIdx.y];
   f32x4 x{0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
-  for (int s = 0; s < splits; ++s) x += *reinterpret_cast<const f32x4*>(part + s * n + e);
-  *reinterpret_cast<u32x2*>((blockIdx.y ? y1 : y0) + e) =
+  for (int s = 0; s < splits; ++s) x += *reinterpret_cast<const f32x4*>(part + s * n);
+  *reinterpret_cast<u32x2*>(a.y[blockIdx.y] + e) =
       u32x2{pack_pair<T16>(x[0], x[1]), pack_pair<T16>(x[2], x[3])};
 }
 
@@ -783,6 +813,7 @@ extern "C" int sla2h_diff_attn_bwd(const void* q, const void* k, const void* v, 
   a.dq_map = work_map(bp, p.qtiles * p.dq_splits, even, causal);
   a.kv_map = work_map(bk, p.ktiles * p.kv_splits, even, false);  // causal: the first keys' are longest
   a.dq_blocks = dq ? (int)work_grid(a.dq_map) : 0;
+  a.kv_blocks = dk ? (int)work_grid(a.kv_map) : 0;
   a.dq_splits = p.dq_splits;
   a.kv_splits = p.kv_splits;
   hipStream_t st = static_cast<hipStream_t>(stream);
@@ -791,30 +822,33 @@ extern "C" int sla2h_diff_attn_bwd(const void* q, const void* k, const void* v, 
     int err;
     diff_bwd_prep_kernel<T16><<<(unsigned)(pq + pv), 256, 0, st>>>(a, pq);
     if ((err = (int)hipGetLastError())) return err;
-    if (dk) {
-      const unsigned grid = work_grid(a.kv_map);
-      const bool few = a.rep * Lq <= kFineRows || Lk <= kKeyRows;
-      if (causal && few)
-        diff_bwd_dkdv_kernel<T16, true, true><<<grid, 256, 0, st>>>(a);
-      else if (causal)
-        diff_bwd_dkdv_kernel<T16, true, false><<<grid, 256, 0, st>>>(a);
-      else if (few)
-        diff_bwd_dkdv_kernel<T16, false, true><<<grid, 256, 0, st>>>(a);
+    const unsigned nq = (unsigned)(a.dq_blocks + a.P), nk = (unsigned)a.kv_blocks;
+    if (a.rep * Lq <= kFineRows || Lk <= kKeyRows) {
+      if (causal)
+        diff_bwd_few_kernel<T16, true><<<nk + nq, 256, 0, st>>>(a);
       else
-        diff_bwd_dkdv_kernel<T16, false, false><<<grid, 256, 0, st>>>(a);
+        diff_bwd_few_kernel<T16, false><<<nk + nq, 256, 0, st>>>(a);
+    } else {
+      if (dk && causal) diff_bwd_dkdv_kernel<T16, true><<<nk, 256, 0, st>>>(a);
+      if (dk && !causal) diff_bwd_dkdv_kernel<T16, false><<<nk, 256, 0, st>>>(a);
       if ((err = (int)hipGetLastError())) return err;
+      diff_bwd_dq_kernel<T16><<<nq, 256, 0, st>>>(a);
     }
-    diff_bwd_dq_kernel<T16><<<a.dq_blocks + a.P, 256, 0, st>>>(a);
     if ((err = (int)hipGetLastError())) return err;
-    auto join = [&](int splits, int64_t n, const float* p0, const float* p1, uint16_t* y0,
-                    uint16_t* y1) {
-      diff_bwd_join_kernel<T16><<<dim3((unsigned)((n / 4 + 255) / 256), y1 ? 2 : 1), 256, 0, st>>>(
-          p0, p1, splits, n, y0, y1);
+    JoinArgs j{};
+    int joins = 0;
+    int64_t most = 0;
+    auto join = [&](const float* part, uint16_t* y, int64_t n, int splits) {
+      if (!y || splits == 1) return;
+      j.part[joins] = part, j.y[joins] = y, j.n[joins] = n, j.splits[joins] = splits;
+      most = n > most ? n : most;
+      ++joins;
     };
-    if (dq && p.dq_splits > 1)
-      join(p.dq_splits, a.nrows * 128, a.dq_part, nullptr, a.dq, nullptr);
-    if (dk && p.kv_splits > 1)
-      join(p.kv_splits, bk * Lk * 128, a.dk_part, a.dv_part, a.dk, a.dv);
+    join(a.dq_part, a.dq, a.nrows * 128, p.dq_splits);
+    join(a.dk_part, a.dk, bk * Lk * 128, p.kv_splits);
+    join(a.dv_part, a.dv, bk * Lk * 128, p.kv_splits);
+    if (joins)
+      diff_bwd_join_kernel<T16><<<dim3((unsigned)((most / 4 + 255) / 256), joins), 256, 0, st>>>(j);
     return (int)hipGetLastError();
   };
   return dtype == SLA2H_DTYPE_BF16 ? go(BF16{}) : go(F16{});
