@@ -218,7 +218,7 @@ __device__ inline void store_row8(const OrthoArgs& a, int dtype, int64_t mat, in
   *reinterpret_cast<u32x4*>(static_cast<uint16_t*>(a.out) + at) = x;
 }
 
-enum { kGram, kPoly, kPolyFew, kStep, kLast };
+enum { kGram, kGramFew, kPoly, kPolyFew, kStep, kLast };
 
 // Offsets of the transposed operand whose slots follow row_frag's order: rows 8 h + 4 x + 0 .. 3.
 // (Channels 32 mb on: four chunks further, a bit of the address that no swizzle carries into.)
@@ -247,12 +247,13 @@ __device__ inline u32x4 turned_frag(const unsigned char* tile, int s, int mb, co
 // registers, i along the lanes; it goes through LDS, so that whole rows are stored (from the registers,
 // eight bytes to a row: kStep 105 us for 91, kGram 65 for 58).  24 x 512 x 2048: kGram 1.0, kStep 0.92
 // PFLOP/s of 16-bit products, with 200 MB read and written beside kStep's.
-//   kGram: A = X X^T;  kPoly: B = b A + c A A^T (kPolyFew: with lo lo);  kStep: Y = a X + B X;
+//   kGram, kGramFew: A = X X^T;  kPoly, kPolyFew (with lo lo): B = b A + c A A^T;  kStep: Y = a X + B X;
 //   kLast: that, to G's type
 template <int T, int OP>
 __global__ __launch_bounds__(256, T == 128 && OP < kStep ? 1 : 2) void ortho_product_kernel(
     OrthoArgs a, int dtype, int work) {
-  constexpr bool STEP = OP >= kStep, POLY = OP == kPoly || OP == kPolyFew;
+  constexpr bool STEP = OP >= kStep, POLY = OP == kPoly || OP == kPolyFew,
+                 GRAM = OP == kGram || OP == kGramFew;
   constexpr int NT = T / 64;      // 32 x 32 tiles of a wave: NT x NT
   constexpr int NU = T / 32;      // 32-row units (4 KB) of an operand's stage
   constexpr int kUnit = 32 * kRowB;
@@ -284,9 +285,9 @@ __global__ __launch_bounds__(256, T == 128 && OP < kStep ? 1 : 2) void ortho_pro
   const int64_t px = (int64_t)2 * a.rp * a.mp, pa = (int64_t)2 * a.rp * a.rp;
   const uint16_t* X = a.x + mat * px;
   const uint16_t* A = a.A + mat * pa;
-  const uint16_t* P = OP == kGram ? X : POLY ? A : a.B + mat * pa;  // rows i
-  const int ldp = (OP == kGram ? a.mp : a.rp) * 4, ldx = a.mp * 4;         // bytes
-  const int K = OP == kGram ? a.mp : a.rp;
+  const uint16_t* P = GRAM ? X : POLY ? A : a.B + mat * pa;  // rows i
+  const int ldp = (GRAM ? a.mp : a.rp) * 4, ldx = a.mp * 4;         // bytes
+  const int K = GRAM ? a.mp : a.rp;
 
   // Unit u of a stage: rows 32 u .. of the operand along the lanes, then the other one's; wave w loads
   // rows 8 w .. of each.  Rows past the matrix: zeros; columns past it: what stands there, for results
@@ -324,7 +325,7 @@ __global__ __launch_bounds__(256, T == 128 && OP < kStep ? 1 : 2) void ortho_pro
   const int il = tid / (T / 8), jl = 8 * (tid % (T / 8));
   u32x4 ph[kPass]{}, pl[kPass]{};
   auto fetch = [&](int p0) __attribute__((always_inline)) {
-    if (OP == kGram || p0 * kRows >= ni || jl >= nj) return;
+    if (GRAM || p0 * kRows >= ni || jl >= nj) return;
 #pragma unroll
     for (int p = 0; p < kPass; ++p) {
       const uint16_t* s = (POLY ? A : X) +
@@ -335,11 +336,14 @@ __global__ __launch_bounds__(256, T == 128 && OP < kStep ? 1 : 2) void ortho_pro
   };
   if (T == 64) fetch(0);
 
-  f32x16 acc[NT][NT], low[NT][NT];  // hi hi, and the two cross products
+  // hi hi, and the two cross products; of few rows the second halves of the stages apart: half as long a
+  // chain of additions (20 rows of 1,500: 1.5 to 1.9 times fp32's error otherwise)
+  f32x16 acc[NT][NT], low[NT][NT], acc2[NT][NT], low2[NT][NT];
 #pragma unroll
   for (int x = 0; x < NT; ++x)
 #pragma unroll
-    for (int y = 0; y < NT; ++y) acc[x][y] = low[x][y] = zero16();
+    for (int y = 0; y < NT; ++y)
+      acc[x][y] = low[x][y] = acc2[x][y] = low2[x][y] = zero16();
   struct Frags {
     u32x4 i[2][NT], j[2][NT];
   };
@@ -383,7 +387,8 @@ __global__ __launch_bounds__(256, T == 128 && OP < kStep ? 1 : 2) void ortho_pro
   // is left to the compiler: with the fixed order its bursts make some cards lower their clock (8 x 512 x
   // 512, one call after another: 238 us for 176; zeros, which draw less, 148 for 154).
   auto half = [&](const Frags& f, const unsigned char* s, int k, Frags& next, int k0,
-                  unsigned char* to) __attribute__((always_inline)) {
+                  unsigned char* to, f32x16 (&acc)[NT][NT], f32x16 (&low)[NT][NT])
+      __attribute__((always_inline)) {
 #pragma unroll
     for (int z = 0; z < 3 * NT; ++z) {
       if (z == 0) read_i(s, k, 0, next);
@@ -421,10 +426,13 @@ __global__ __launch_bounds__(256, T == 128 && OP < kStep ? 1 : 2) void ortho_pro
     Frags f0, f1;
     auto stage = [&](int k0, const unsigned char* cur, const unsigned char* next, unsigned char* to)
         __attribute__((always_inline)) {
-      half(f0, cur, 1, f1, k0 + 96, to);
+      half(f0, cur, 1, f1, k0 + 96, to, acc, low);
       __builtin_amdgcn_s_waitcnt(wait_vm_lgkm0(4 * NU));
       __builtin_amdgcn_s_barrier();
-      half(f1, next, 0, f0, 0, to);
+      if (OP == kGramFew)
+        half(f1, next, 0, f0, 0, to, acc2, low2);
+      else
+        half(f1, next, 0, f0, 0, to, acc, low);
     };
     load(0, s0, 0, NU);
     load(32, s1, 0, NU);
@@ -469,7 +477,11 @@ __global__ __launch_bounds__(256, T == 128 && OP < kStep ? 1 : 2) void ortho_pro
       for (int g = 0; g < 4; ++g) {
         f32x4 v;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = acc[x][y][4 * g + e] + low[x][y][4 * g + e];
+        for (int e = 0; e < 4; ++e) {
+          const int r = 4 * g + e;
+          v[e] = acc[x][y][r] + low[x][y][r];
+          if (OP == kGramFew) v[e] = (acc[x][y][r] + acc2[x][y][r]) + (low[x][y][r] + low2[x][y][r]);
+        }
         const int i = (T / 2) * wi + 32 * x + (l & 31), j = (T / 2) * wj + 32 * y + 8 * g + 4 * h;
         if (!diagonal) {
           *reinterpret_cast<f32x4*>(one(i, j)) = v;
@@ -490,8 +502,8 @@ __global__ __launch_bounds__(256, T == 128 && OP < kStep ? 1 : 2) void ortho_pro
     const float cb = a.b * (kScaleB / kScaleX), cc = a.c * (kScaleB / (kScaleX * kScaleX));
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const float p = OP == kGram ? 0.f : pair_at(hi[e >> 1], lw[e >> 1], e & 1);
-      v[e] = OP == kGram   ? v[e] * (1.f / kScaleX)
+      const float p = GRAM ? 0.f : pair_at(hi[e >> 1], lw[e >> 1], e & 1);
+      v[e] = GRAM   ? v[e] * (1.f / kScaleX)
              : POLY ? __builtin_fmaf(cc, v[e], cb * p)
                            : __builtin_fmaf(a.a, p, (1.f / kScaleB) * v[e]);
     }
@@ -508,7 +520,7 @@ __global__ __launch_bounds__(256, T == 128 && OP < kStep ? 1 : 2) void ortho_pro
     *reinterpret_cast<u32x4*>(d) = hi;
     *reinterpret_cast<u32x4*>(d + 32) = lw;
   };
-  uint16_t* base = OP == kGram ? a.A + mat * pa : POLY ? a.B + mat * pa : a.y + mat * px;
+  uint16_t* base = GRAM ? a.A + mat * pa : POLY ? a.B + mat * pa : a.y + mat * px;
   if (jl < nj)
     for (int p0 = 0; p0 * kRows < ni; p0 += kPass) {
       float v[kPass][8];
@@ -757,13 +769,14 @@ int ortho_product(const OrthoArgs& a, int dtype, hipStream_t st) {
   // 256, 2048: 64 / 76; Gram and square 240, 512: 19 / 19; 400, 512: 33 / 27; 480, 512: 39 / 35; 72, 2048:
   // 36 / 27; 136, 2048: 40 / 44; 240, 2048: 48 / 53; 528, 4096: 230 / 330.
   const bool deep = (OP == kGram ? a.mp : a.rp) >= 2048;
-  const bool wide = OP == kPolyFew ? false
+  constexpr bool few = OP == kGramFew || OP == kPolyFew;
+  const bool wide = few ? false
                     : OP >= kStep  ? tiles(128) >= (deep ? 200 : 300)
                                    : deep && tiles(128) >= 130;
   const int64_t work = tiles(wide ? 128 : 64);
   const unsigned grid = 8u * (unsigned)((work + 7) / 8);
   if (wide)
-    ortho_product_kernel<OP == kPolyFew ? 64 : 128, OP><<<grid, 256, 0, st>>>(a, dtype, (int)work);
+    ortho_product_kernel<few ? 64 : 128, OP><<<grid, 256, 0, st>>>(a, dtype, (int)work);
   else
     ortho_product_kernel<64, OP><<<grid, 256, 0, st>>>(a, dtype, (int)work);
   return (int)hipGetLastError();
@@ -816,9 +829,11 @@ extern "C" int sla2h_orthogonalize(const void* g, int dtype, int64_t n, int64_t 
   if ((err = (int)hipGetLastError())) return err;
   for (int s = 0; s < steps; ++s) {
     a.a = coeffs[3 * s], a.b = coeffs[3 * s + 1], a.c = coeffs[3 * s + 2];
-    if ((err = ortho_product<kGram>(a, dtype, st))) return err;
+    const bool few = a.rp <= 128;
+    err = few ? ortho_product<kGramFew>(a, dtype, st) : ortho_product<kGram>(a, dtype, st);
+    if (err) return err;
     // (few rows: 8 x 448 x 448 would take 175 us for 150 with the fourth product, and gain nothing)
-    err = a.rp <= 128 ? ortho_product<kPolyFew>(a, dtype, st) : ortho_product<kPoly>(a, dtype, st);
+    err = few ? ortho_product<kPolyFew>(a, dtype, st) : ortho_product<kPoly>(a, dtype, st);
     if (err) return err;
     if ((err = s + 1 < steps ? ortho_product<kStep>(a, dtype, st)
                              : ortho_product<kLast>(a, dtype, st)))
