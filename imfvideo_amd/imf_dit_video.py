@@ -907,6 +907,8 @@ def residual_norm(x, a, scale, post_weight, gate=None, pre_weight=None, eps=1e-6
     (CPU tensors, other dtypes, transforms) runs the eager expression."""
     if not 1 <= consumers <= 3:
         raise ValueError(f"residual_norm: 1 to 3 consumers, got {consumers}")
+    if not eps > 0.0:
+        raise ValueError(f"residual_norm: eps has to be above 0, got {eps}")
     if gate is not None and (x.dim() < 2 or tuple(gate.shape) != (x.shape[0], x.shape[-1])):
         raise ValueError(f"residual_norm: expected a gate of {x.shape[0]} rows of {x.shape[-1]}, "
                          f"got {tuple(gate.shape)}")

@@ -1983,6 +1983,27 @@ def residual_norm_bwd(dy, dns, y, a, scale, post, pre=None, gate=None, eps=1e-6)
 NS_COEFFS = (3.4445, -4.7750, 2.0315)  # slope 3.4 at 0, singular values to 0.7 .. 1.2
 
 
+def _ns_bounds(flat):
+    """ValueError where the steps may leave what the kernels' scaled pairs hold: singular values up to
+    4 (A below 16) and |b A + c A^2| below 128."""
+    def largest(f, top, at):  # |f| on [0, top], f's extrema in `at`
+        return max(abs(f(min(max(x, 0.0), top))) for x in (top, *at))
+    def roots(a, b, c):  # of a + b t + c t^2
+        if c == 0.0:
+            return (-a / b,) if b else ()
+        d = b * b - 4 * a * c
+        return () if d < 0 else tuple((-b + s * math.sqrt(d)) / (2 * c) for s in (1, -1))
+    top = 1.0
+    for i in range(0, len(flat), 3):
+        a, b, c = flat[i:i + 3]
+        gain = largest(lambda t: b * t + c * t * t, top * top, roots(b, 2 * c, 0.0))
+        if top > 4.0 or gain >= 127.0:
+            raise ValueError(f"orthogonalize: step {i // 3 + 1} of these coefficients takes singular "
+                             f"values up to {top:.3g}, and factors up to {gain:.3g}: at most 4 and 127")
+        top = largest(lambda x: x * (a + x * x * (b + c * x * x)), top,
+                      [math.sqrt(t) for t in roots(a, 3 * b, 5 * c) if t > 0])
+
+
 @functools.lru_cache(maxsize=64)
 def _ns_coeffs(steps, coeffs):
     rows = [coeffs] * steps if not isinstance(coeffs[0], tuple) else list(coeffs)
@@ -1992,6 +2013,7 @@ def _ns_coeffs(steps, coeffs):
     flat = [float(x) for r in rows for x in r]
     if not all(map(math.isfinite, flat)):
         raise ValueError(f"orthogonalize: coefficients have to be finite, got {coeffs}")
+    _ns_bounds(flat)
     return (ctypes.c_float * len(flat))(*flat)
 
 
@@ -2004,7 +2026,7 @@ def ns_rows(steps, coeffs):
 def orthogonalize(g, steps=5, coeffs=NS_COEFFS):
     """Newton-Schulz products of each matrix of g (..., R, C), fp32 or 16-bit, in its type:
     X = g / |g|, then `steps` times X <- a X + (b A + c A^2) X with A = X X^T on the shorter side,
-    coeffs (a, b, c) or such a row for every step.  Singular values go towards 1, singular vectors
+    coeffs (a, b, c) or such a row for every step (that keep singular values up to 4).  Singular values go towards 1, singular vectors
     stay.  Computed to fp32's accuracy whatever the type; zeros stay zeros."""
     _need_gpu(g)
     if g.dtype not in _NORM_DTYPES:

@@ -122,3 +122,26 @@ def test_sides_past_the_kernels():
     assert size(1, 32768, 32768) > 0 and size(1, 32769, 1) == 0 and size(0, 1, 1) == 0
     # matrices that one workgroup holds need none
     assert size(1 << 20, 64, 512) == size(1, 1, 1) < 1024 < size(1, 65, 512)
+
+
+@pytest.mark.parametrize("steps,coeffs,ok", [
+    (5, ops.NS_COEFFS, True), (30, ops.NS_COEFFS, True), (6, (1.5, -0.5, 0.0), True),
+    (5, (2.0, -1.5, 0.5), True), (1, (10.0, 0.0, 0.0), True), (2, (10.0, 0.0, 0.0), False),
+    (1, (1.0, 100.0, 50.0), False), (2, [(3.9, 0.0, 0.0), (1.0, -1.0, 0.0)], True),
+    (2, [(4.1, 0.0, 0.0), (1.0, -1.0, 0.0)], False), (64, (1.0, 0.0, 0.0), True),
+    (3, (3.0, -3.0, 1.0), True), (2, (0.0, 0.0, -5.0), False)])
+def test_coefficients_that_leave_the_kernels_range(steps, coeffs, ok):
+    """The bound is the largest value that the polynomials reach from [0, 1], step by step."""
+    rows = [coeffs] * steps if not isinstance(coeffs[0], tuple) else coeffs
+    top, fits = 1.0, True
+    for a, b, c in rows:
+        t = torch.linspace(0, top, 100001, dtype=torch.float64)
+        fits &= top <= 4.0 and (b * t ** 2 + c * t ** 4).abs().max().item() < 127.0
+        top = (a * t + b * t ** 3 + c * t ** 5).abs().max().item()
+    assert fits == ok
+    call = lambda: ops._ns_coeffs(steps, ops.ns_rows(steps, coeffs))
+    if ok:
+        call()
+    else:
+        with pytest.raises(ValueError, match="singular values"):
+            call()

@@ -115,3 +115,9 @@ def test_the_block_on_the_host():
     y = x + m.attn_scale * g[0][:, None] * m.attn_post_norm(m.attn(m.norm1(x), cos, sin))
     y = y + m.mlp_scale * g[1][:, None] * m.mlp_post_norm(m.mlp(m.norm2(y)))
     assert torch.allclose(m(x, cos, sin, g), y, rtol=1e-5, atol=1e-5)
+
+
+@pytest.mark.parametrize("eps", [0.0, -1e-6, float("nan")])
+def test_an_eps_that_is_not_above_zero(eps):
+    with pytest.raises(ValueError, match="eps"):
+        residual_norm(**operands(), eps=eps)
