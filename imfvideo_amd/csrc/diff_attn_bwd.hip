@@ -38,7 +38,7 @@ struct Scaled<F16> {
 // kFineKeys keys or kFineRows queries and of causal waves that see at most kFineRows keys, else in
 // every second stage (1.25 times; B = 1, H = 8, L = 29,952: 0.4 ms).  dk, dv: calls of at most
 // kFineRows rows per key pair, or of one block of keys, whose few large probabilities round alike in
-// row after row (longer sums average the roundings out).
+// row after row, and others that are one small launch (longer sums average the roundings out).
 constexpr int kFineKeys = 4096, kFineRows = 512;
 constexpr int kKeyRows = 128;  // keys of a workgroup of dk and dv
 constexpr int kNormRows = 64;  // rows of a partial maximum of the norms and of a partial sum of dlam
@@ -652,9 +652,11 @@ __device__ inline __attribute__((always_inline)) void dkdv_of(const DiffBwdArgs&
   }
 }
 
-// The launches.  Calls that take the lost halves everywhere are small: both in one, side by side (2 x 4
-// x 274 tokens 27 us, one after the other 45).  Of others the two bodies under one allocation spill 20
-// registers (29,952 tokens: 7.65 ms, one after the other 7.2).
+// The launches.  Calls that take the lost halves everywhere and those whose workgroups are all resident
+// at once: both in one, side by side, with the lost halves (us for the backward of 8 heads, in one / one
+// after the other: 600 tokens 36 / 48, 1,000 43 / 55, causal 44 / 52, 2,000 75 / 78; 600 queries of 5,000
+// keys 58 / 68).  Of others the two bodies under one allocation spill 20 registers (29,952 tokens: 7.65
+// ms, one after the other 7.2).
 template <typename T16, bool CAUSAL>
 __global__ __launch_bounds__(256, 2) void diff_bwd_few_kernel(DiffBwdArgs a) {
   __shared__ __align__(16) unsigned char s0[kStageB], s1[kStageB], v[2 * kStageB];
@@ -823,7 +825,9 @@ extern "C" int sla2h_diff_attn_bwd(const void* q, const void* k, const void* v, 
     diff_bwd_prep_kernel<T16><<<(unsigned)(pq + pv), 256, 0, st>>>(a, pq);
     if ((err = (int)hipGetLastError())) return err;
     const unsigned nq = (unsigned)(a.dq_blocks + a.P), nk = (unsigned)a.kv_blocks;
-    if (a.rep * Lq <= kFineRows || Lk <= kKeyRows) {
+    // (whether or not both are asked for: a gradient does not depend on the others)
+    const bool together = work_grid(a.kv_map) + work_grid(a.dq_map) <= 512;
+    if (a.rep * Lq <= kFineRows || Lk <= kKeyRows || together) {
       if (causal)
         diff_bwd_few_kernel<T16, true><<<nk + nq, 256, 0, st>>>(a);
       else

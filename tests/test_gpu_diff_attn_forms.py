@@ -87,6 +87,18 @@ def test_offsets_past_32_bits(which):
         assert torch.equal(got[n], want[n]), n
 
 
+@pytest.mark.parametrize("L", [274, 700, 1500, 2500])
+def test_a_gradient_does_not_depend_on_the_others(L):
+    from imfvideo_amd.imf_dit_video import diff_attention
+    x, lam, do = operands(19, 1, L, 8)
+    want = call(x, lam, do)
+    for i, n in enumerate(("dq", "dk", "dv", "dlam")):
+        t = [*x, lam]
+        t[i] = t[i].clone().requires_grad_(True)
+        got, = torch.autograd.grad(diff_attention(*t), t[i], do)
+        assert torch.equal(got, want[n]), n
+
+
 def test_two_streams_at_once():
     """Calls of both forms interleaved on two streams, with workspaces of their own."""
     sets = [operands(7, 1, 1, 4, Lk=9000), operands(8, 2, 700, 4), operands(9, 1, 64, 4, Lk=5000)]
