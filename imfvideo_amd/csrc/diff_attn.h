@@ -46,7 +46,8 @@ inline bool diff_sizes_ok(int B, int H, int Hkv, int64_t Lq, int64_t Lk) {
 // more per workgroup for its partial sums' way through memory, and the launch that adds them.
 struct SplitCost {
   float one, two, join;
-  int least;  // stages of a range
+  int least;         // stages of a range
+  int64_t most = 1280;  // workgroups
   float time(int64_t blocks, int64_t stages, int64_t s, float share) const {
     const int64_t w = blocks * s, n = (stages + s - 1) / s, rest = w % 512;
     const float full = two * (float)w * share / 512.f, longest = 1.2f * one;
@@ -61,7 +62,7 @@ constexpr float kShares[2][2] = {{1.f, 0.7f}, {0.5f, 0.35f}};  // causal, length
 inline int best_split(int64_t blocks, int64_t stages, float share, const SplitCost& c, float& least) {
   int best = 1;
   least = c.time(blocks, stages, 1, share);
-  for (int64_t s = 2; blocks * s <= 1280 && stages >= s * c.least; s += s < 16 ? 1 : s / 8) {
+  for (int64_t s = 2; blocks * s <= c.most && stages >= s * c.least; s += s < 16 ? 1 : s / 8) {
     const float t = c.time(blocks, stages, s, share);
     if (t < least) least = t, best = (int)s;
   }

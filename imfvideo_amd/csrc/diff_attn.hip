@@ -689,7 +689,15 @@ FwdPlan fwd_plan(int B, int H, int Hkv, int64_t Lq, int64_t Lk, bool causal, boo
   // with one and two workgroups per CU.  us, 128 / 64, H = 8: 1 clip of 8,192 231 / 208, of 12,000 476 / 479, of 16,384 738 / 809, 4 clips of
   // 2,048, H = 16, 106 / 113; causal 12,000 334 / 244, 24,000 831 / 870.
   const int64_t q2 = (Lq + 127) / 128, q1 = (Lq + 63) / 64;
-  const SplitCost c2{0.88f, 1.43f, 0.f, 0}, c1{0.53f, 0.74f, 0.033f, 4};
+  const SplitCost c2{0.88f, 1.43f, 0.f, 0};
+  SplitCost c1{0.53f, 0.74f, 0.033f, 4};
+  if (q1 == 1) {
+    // One block of queries reads every key from memory, and 256 workgroups are all that it feeds (us for 2
+    // clips, H = 8, 1 query, 29,952 keys and fewer: 192 27, 256 25, 320 to 512 26 to 28, more 30 to 34);
+    // its partial sums are few.
+    c1.most = 256;
+    c1.join *= (float)Lq / 64.f;
+  }
   float t1;
   p.splits = best_split(bp * q1, units, share, c1, t1);
   p.nq = !lens && c2.time(bp * q2, units, 1, share) < t1 ? 2 : 1;
