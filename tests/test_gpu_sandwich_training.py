@@ -99,9 +99,7 @@ def test_a_block_is_its_operators_one_after_the_other():
                              pre_weight=b.norm2.weight, eps=b.norm2.eps)
         want, = residual_norm(y, b.mlp(n), b.mlp_scale, b.mlp_post_norm.weight, gate=gates[1],
                               eps=b.mlp_post_norm.eps)
-    # (the first norm's rounding may be inside or outside of a kernel: one step of bf16 on the
-    # attention's input, which its layers pass on)
-    assert (got - want).abs().max() <= 0.05 * want.abs().max()
+    assert torch.equal(got, want)
 
 
 def test_gradients_of_the_block_are_the_differences():
