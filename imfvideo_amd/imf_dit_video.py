@@ -196,8 +196,10 @@ class _DiffAttentionFunction(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, v, lam, causal, q_lens, k_lens, scale):
-        o, lse, maps = ops.diff_attn_fwd(q, k, v, lam, causal, q_lens, k_lens, scale, True)
-        ctx.args = causal, scale
+        ctx.lam_dtype = lam.dtype
+        q, k, v, lam, *ctx.plan = ops._diff_operands(q, k, v, lam, scale)
+        ctx.causal = causal
+        o, lse, maps = ops._diff_fwd(q, k, v, lam, *ctx.plan, causal, q_lens, k_lens, True)
         ctx.save_for_backward(q, k, v, lam, lse, maps, q_lens, k_lens)
         return o
 
@@ -206,12 +208,14 @@ class _DiffAttentionFunction(torch.autograd.Function):
     def backward(ctx, do):
         _no_batched(do, "diff_attention")
         q, k, v, lam, lse, maps, q_lens, k_lens = ctx.saved_tensors
-        causal, scale = ctx.args
+        plan, scale = ctx.plan
+        if not plan.fits(q, k, v):  # (saved tensors that a hook brought back)
+            q, k, v, lam, plan, scale = ops._diff_operands(q, k, v, lam, scale)
         nq, nk, nv = ctx.needs_input_grad[:3]
-        *grads, dlam = ops.diff_attn_bwd(do, q, k, v, lam, lse, maps, causal, q_lens, k_lens, scale,
-                                         nq, nk or nv)
-        return (*grads, dlam if dlam.dtype == lam.dtype else dlam.to(lam.dtype), None, None, None,
-                None)
+        *grads, dlam = ops._diff_bwd(do, q, k, v, lam, lse, maps, plan, scale, ctx.causal, q_lens,
+                                     k_lens, nq, nk or nv)
+        return (*grads, dlam if dlam.dtype == ctx.lam_dtype else dlam.to(ctx.lam_dtype), None, None,
+                None, None)
 
 
 def diff_attention(q, k, v, lam, causal=False, q_lens=None, k_lens=None, scale=None):

@@ -2054,7 +2054,13 @@ def orthogonalize(g, steps=5, coeffs=NS_COEFFS):
 # ---------------------------------------------------------------------------
 class _DiffPlan:
     """What a differential attention call needs of its operands' shapes and strides."""
-    __slots__ = ("sizes", "copy", "empty", "strides", "fwd_ws", "bwd_ws", "lse_shape", "maps_shape")
+    __slots__ = ("sizes", "copy", "empty", "given", "strides", "fwd_ws", "bwd_ws", "lse_shape",
+                 "maps_shape")
+
+    def fits(self, q, k, v):
+        """The operands are laid out as those that it was made of."""
+        return ((q.stride(), k.stride(), v.stride()) == self.given
+                and not (q.data_ptr() | k.data_ptr() | v.data_ptr()) % 16)
 
 
 @functools.lru_cache(maxsize=512)
@@ -2076,6 +2082,7 @@ def _diff_plan(qs, qt, ks, kt, vs, vt, dtype):
     p.copy = [t[3] != 1 or any(x % 8 for x in s) or not E_TILE <= s[2] < _ATTN_ROW_SPAN
               for s, t in zip(ins, (qt, kt, vt))]
     p.strides = (ctypes.c_int64 * 9)(*sum(ins, []))
+    p.given = qt, kt, vt
     p.lse_shape, p.maps_shape = (B, H, Lq), (B, Lq, H // 2, 2, 2 * E_TILE)
     p.fwd_ws = p.bwd_ws = 0
     if not p.empty:
@@ -2118,19 +2125,9 @@ def _diff_operands(q, k, v, lam, scale):
     return q, k, v, lam, plan, float(scale)
 
 
-def diff_attn_fwd(q, k, v, lam, causal=False, q_lens=None, k_lens=None, scale=None, save=False):
-    """Differential attention of q (B, Lq, H, 64) over k, v (B, Lk, Hkv, 64), 16-bit, any strides
-    with a unit channel stride -> (o (B, Lq, H, 64), lse, maps).  The heads 2p and 2p + 1 are
-    two softmax maps over the same 128 value channels, the value heads 2 kp and 2 kp + 1 side by
-    side with kp = p // (H // Hkv): o = (A_1 - lam[p] A_2) v in the output heads 2p and 2p + 1.
-    lengths, causal order and scale as in dense_attn_fwd.  save: also what the backward
-    reads, lse (B, H, Lq) and maps (B, Lq, H // 2, 2, 128), A_1 v and A_2 v, fp32; else None."""
-    q, k, v, lam, p, scale = _diff_operands(q, k, v, lam, scale)
+def _diff_fwd(q, k, v, lam, p, scale, causal, q_lens, k_lens, save):
+    """diff_attn_fwd of what _diff_operands and attn_lens return."""
     dev = q.device
-    if q_lens is not None:
-        q_lens = attn_lens(q_lens, q, "q_lens")
-    if k_lens is not None:
-        k_lens = attn_lens(k_lens, q, "k_lens")
     o = torch.empty(q.shape, device=dev, dtype=q.dtype)
     lse = torch.empty(p.lse_shape, device=dev, dtype=torch.float32) if save else None
     maps = torch.empty(p.maps_shape, device=dev, dtype=torch.float32) if save else None
@@ -2148,6 +2145,35 @@ def diff_attn_fwd(q, k, v, lam, causal=False, q_lens=None, k_lens=None, scale=No
     return o, lse, maps
 
 
+def diff_attn_fwd(q, k, v, lam, causal=False, q_lens=None, k_lens=None, scale=None, save=False):
+    """Differential attention of q (B, Lq, H, 64) over k, v (B, Lk, Hkv, 64), 16-bit, any strides
+    with a unit channel stride -> (o (B, Lq, H, 64), lse, maps).  The heads 2p and 2p + 1 are
+    two softmax maps over the same 128 value channels, the value heads 2 kp and 2 kp + 1 side by
+    side with kp = p // (H // Hkv): o = (A_1 - lam[p] A_2) v in the output heads 2p and 2p + 1.
+    lengths, causal order and scale as in dense_attn_fwd.  save: also what the backward
+    reads, lse (B, H, Lq) and maps (B, Lq, H // 2, 2, 128), A_1 v and A_2 v, fp32; else None."""
+    x = _diff_operands(q, k, v, lam, scale)
+    return _diff_fwd(*x, causal, attn_lens(q_lens, q, "q_lens"), attn_lens(k_lens, q, "k_lens"), save)
+
+
+def _diff_bwd(do, q, k, v, lam, lse, maps, p, scale, causal, q_lens, k_lens, need_q, need_kv):
+    """diff_attn_bwd of what _diff_operands and attn_lens return, lse and maps as _diff_fwd does."""
+    dev, dtype = q.device, q.dtype
+    do = aligned(do.contiguous(), 16)
+    dq = torch.empty(q.shape, device=dev, dtype=dtype) if need_q else None
+    dk = torch.empty(k.shape, device=dev, dtype=dtype) if need_kv else None
+    dv = torch.empty(v.shape, device=dev, dtype=dtype) if need_kv else None
+    dlam = torch.empty(lam.shape, device=dev, dtype=lam.dtype)
+    if p.empty:
+        return tuple(t if t is None else t.zero_() for t in (dq, dk, dv, dlam))
+    ws = _scratch(p.bwd_ws, dev)
+    _launch(dev, "sla2h_diff_attn_bwd", q.data_ptr(), k.data_ptr(), v.data_ptr(), lam.data_ptr(),
+            _NORM_DTYPES[lam.dtype], lam.stride(0), do.data_ptr(), lse.data_ptr(), maps.data_ptr(),
+            p.strides, _ptr(q_lens), _ptr(k_lens), _HALF[dtype], *p.sizes, 1 if causal else 0, scale,
+            ws.data_ptr(), _ptr(dq), _ptr(dk), _ptr(dv), dlam.data_ptr())
+    return dq, dk, dv, dlam
+
+
 def diff_attn_bwd(do, q, k, v, lam, lse, maps, causal=False, q_lens=None, k_lens=None, scale=None,
                   need_q=True, need_kv=True):
     """Gradients (dq, dk, dv, dlam) of diff_attn_fwd for the output gradient do, from its
@@ -2162,20 +2188,6 @@ def diff_attn_bwd(do, q, k, v, lam, lse, maps, causal=False, q_lens=None, k_lens
         if t.shape != shape or t.dtype != torch.float32 or t.device != dev:
             raise ValueError(f"{name}: expected {shape} float32 on {dev}, got "
                              f"{tuple(t.shape)} {t.dtype} on {t.device}")
-    do, maps, lse = aligned(do.contiguous(), 16), aligned(maps.contiguous(), 16), lse.contiguous()
-    if q_lens is not None:
-        q_lens = attn_lens(q_lens, q, "q_lens")
-    if k_lens is not None:
-        k_lens = attn_lens(k_lens, q, "k_lens")
-    dq = torch.empty(q.shape, device=dev, dtype=dtype) if need_q else None
-    dk = torch.empty(k.shape, device=dev, dtype=dtype) if need_kv else None
-    dv = torch.empty(v.shape, device=dev, dtype=dtype) if need_kv else None
-    dlam = torch.empty(lam.shape, device=dev, dtype=lam.dtype)
-    if p.empty:
-        return tuple(t if t is None else t.zero_() for t in (dq, dk, dv, dlam))
-    ws = _scratch(p.bwd_ws, dev)
-    _launch(dev, "sla2h_diff_attn_bwd", q.data_ptr(), k.data_ptr(), v.data_ptr(), lam.data_ptr(),
-            _NORM_DTYPES[lam.dtype], lam.stride(0), do.data_ptr(), lse.data_ptr(), maps.data_ptr(),
-            p.strides, _ptr(q_lens), _ptr(k_lens), _HALF[dtype], *p.sizes, 1 if causal else 0, scale,
-            ws.data_ptr(), _ptr(dq), _ptr(dk), _ptr(dv), dlam.data_ptr())
-    return dq, dk, dv, dlam
+    return _diff_bwd(do, q, k, v, lam, lse.contiguous(), aligned(maps.contiguous(), 16), p, scale,
+                     causal, attn_lens(q_lens, q, "q_lens"), attn_lens(k_lens, q, "k_lens"), need_q,
+                     need_kv)

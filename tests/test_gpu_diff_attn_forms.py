@@ -99,6 +99,21 @@ def test_a_gradient_does_not_depend_on_the_others(L):
         assert torch.equal(got, want[n]), n
 
 
+def test_saved_tensors_that_went_to_the_host_and_back():
+    """Views come back contiguous: their strides are not the forward's."""
+    from imfvideo_amd.imf_dit_video import diff_attention
+    x, lam, do = operands(20, 2, 130, 4)
+    want = call(x, lam, do, k_lens=[130, 77])
+    wide = torch.stack([t.flatten(2) for t in x], 2).reshape(2, 130, 3, 4, 64).requires_grad_(True)
+    w = lam.clone().requires_grad_(True)
+    with torch.autograd.graph.save_on_cpu():
+        o = diff_attention(*wide.unbind(2), w, k_lens=[130, 77])
+    dx, dlam = torch.autograd.grad(o, (wide, w), do)
+    assert torch.equal(o, want["o"]) and torch.equal(dlam, want["dlam"])
+    for i, n in enumerate(("dq", "dk", "dv")):
+        assert torch.equal(dx[:, :, i], want[n]), n
+
+
 def test_two_streams_at_once():
     """Calls of both forms interleaved on two streams, with workspaces of their own."""
     sets = [operands(7, 1, 1, 4, Lk=9000), operands(8, 2, 700, 4), operands(9, 1, 64, 4, Lk=5000)]
