@@ -115,10 +115,11 @@ class Muon(torch.optim.Optimizer):
         R, C = ps[0].shape
         lr = float(group["lr"])
         step = -lr * group["rms"] * math.sqrt(max(R, C))
-        if group["weight_decay"]:
-            torch._foreach_mul_(ps, 1.0 - lr * group["weight_decay"])
+        keep = 1.0 - lr * group["weight_decay"]
         if ps[0].dtype == wide:
+            if keep != 1.0:
+                torch._foreach_mul_(ps, keep)
             torch._foreach_add_(ps, list(x), alpha=step)
-        else:  # (16-bit weights: the sum in fp32, rounded once)
+        else:  # (16-bit weights: decay and update in fp32, rounded once)
             for p, d in zip(ps, x):
-                p.copy_(torch.add(p.to(wide), d, alpha=step))
+                p.copy_(p.to(wide).mul_(keep).add_(d, alpha=step))
