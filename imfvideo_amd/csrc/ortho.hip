@@ -21,8 +21,8 @@ namespace sla2h {
 
 namespace {
 
-// Powers of two that the planes are scaled with: |X| below 16, |A| below 16, |b A + c A^2| below 128
-// (singular values of X stay below 1.3 with the usual coefficients) keep hi finite.
+// Powers of two that the planes are scaled with: |X| and |A| below 15.99, |b A + c A^2| below 127.9
+// (singular values of X stay below 1.3 with the usual coefficients) keep hi, an fp16 number, finite.
 constexpr float kScaleX = 4096.f, kScaleB = 512.f;
 
 // A matrix of pairs: rows of blocks of 32 columns, [32 hi | 32 lo] each, 128 bytes: the row of an LDS

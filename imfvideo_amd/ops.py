@@ -1984,8 +1984,9 @@ NS_COEFFS = (3.4445, -4.7750, 2.0315)  # slope 3.4 at 0, singular values to 0.7 
 
 
 def _ns_bounds(flat):
-    """ValueError where the steps may leave what the kernels' scaled pairs hold: singular values up to
-    4 (A below 16) and |b A + c A^2| below 128."""
+    """ValueError where the steps may leave what the kernels' scaled pairs hold, fp16 numbers of 4,096 A and
+    512 (b A + c A^2): singular values below 3.99 (A below 15.93; from 65,520 / 4,096 = 15.996 it is
+    infinite) and |b A + c A^2| below 127."""
     def largest(f, top, at):  # |f| on [0, top], f's extrema in `at`
         return max(abs(f(min(max(x, 0.0), top))) for x in (top, *at))
     def roots(a, b, c):  # of a + b t + c t^2
@@ -1997,9 +1998,9 @@ def _ns_bounds(flat):
     for i in range(0, len(flat), 3):
         a, b, c = flat[i:i + 3]
         gain = largest(lambda t: b * t + c * t * t, top * top, roots(b, 2 * c, 0.0))
-        if top > 4.0 or gain >= 127.0:
+        if top >= 3.99 or gain >= 127.0:
             raise ValueError(f"orthogonalize: step {i // 3 + 1} of these coefficients takes singular "
-                             f"values up to {top:.3g}, and factors up to {gain:.3g}: at most 4 and 127")
+                             f"values up to {top:.4g}, and factors up to {gain:.4g}: below 3.99 and 127")
         top = largest(lambda x: x * (a + x * x * (b + c * x * x)), top,
                       [math.sqrt(t) for t in roots(a, 3 * b, 5 * c) if t > 0])
 
@@ -2026,8 +2027,9 @@ def ns_rows(steps, coeffs):
 def orthogonalize(g, steps=5, coeffs=NS_COEFFS):
     """Newton-Schulz products of each matrix of g (..., R, C), fp32 or 16-bit, in its type:
     X = g / |g|, then `steps` times X <- a X + (b A + c A^2) X with A = X X^T on the shorter side,
-    coeffs (a, b, c) or such a row for every step (that keep singular values up to 4).  Singular values go towards 1, singular vectors
-    stay.  Computed to fp32's accuracy whatever the type; zeros stay zeros."""
+    coeffs (a, b, c) or such a row for every step (that keep singular values below 3.99).  Singular
+    values go towards 1, singular vectors stay.  Computed to fp32's accuracy whatever the type; zeros
+    stay zeros."""
     _need_gpu(g)
     if g.dtype not in _NORM_DTYPES:
         raise TypeError(f"orthogonalize: fp32 or 16-bit matrices, got {g.dtype}")

@@ -955,7 +955,7 @@ int sla2h_residual_norm_bwd(const float* y, const void* a, int dtype, const floa
  *   X = g / |g|_F,  X <- a X + (b A + c A^2) X with A = X X^T,
  * coeffs: host array of 3 steps floats, (a, b, c) of each; out like g (may be g).  A matrix of zeros
  * stays zeros; one that is not finite is NaN.  fp32-exact products of pairs of 16-bit numbers: |X| of
- * the steps below 16, |A| below 16 and |b A + c A^2| below 128 (elementwise), else infinities.  R,
+ * the steps and |A| below 15.99 and |b A + c A^2| below 127.9 (elementwise), else infinities and NaN.  R,
  * C <= 32768.  Workspace, 16-byte aligned, of sla2h_orthogonalize_workspace_bytes (0: sizes that are
  * not taken).  Reproducible; a matrix's result does not depend on the others.
  * The Muon optimiser's step (the reference's moonlight.py).
