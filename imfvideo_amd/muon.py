@@ -20,8 +20,10 @@ __all__ = ["Muon", "matrix_parameters", "newton_schulz"]
 
 
 def newton_schulz(g, steps=5, coeffs=ops.NS_COEFFS):
-    """ops.orthogonalize; CPU and float64 tensors run the products one by one, in float32 or wider."""
-    if g.is_cuda and g.dtype != torch.float64:
+    """ops.orthogonalize; CPU and float64 tensors, and those with a gradient or a tangent to carry, run the
+    products one by one, in float32 or wider."""
+    if (g.is_cuda and g.dtype != torch.float64 and ops.plain_eager(g)
+            and not (g.requires_grad and torch.is_grad_enabled())):
         return ops.orthogonalize(g, steps, coeffs)
     ops._ns_coeffs(steps, ops.ns_rows(steps, coeffs))  # its checks
     x = g.to(torch.promote_types(g.dtype, torch.float32))

@@ -2029,7 +2029,7 @@ def orthogonalize(g, steps=5, coeffs=NS_COEFFS):
     X = g / |g|, then `steps` times X <- a X + (b A + c A^2) X with A = X X^T on the shorter side,
     coeffs (a, b, c) or such a row for every step (that keep singular values below 3.99).  Singular
     values go towards 1, singular vectors stay.  Computed to fp32's accuracy whatever the type; zeros
-    stay zeros."""
+    stay zeros.  The kernels alone: no derivative is recorded (muon.newton_schulz keeps them)."""
     _need_gpu(g)
     if g.dtype not in _NORM_DTYPES:
         raise TypeError(f"orthogonalize: fp32 or 16-bit matrices, got {g.dtype}")
