@@ -20,8 +20,16 @@ namespace sla2h {
 
 namespace {
 
-// Sequences of so many units of keys take what the rounding of P lost with a second product.
-constexpr int kFewUnits = 4;
+// What the rounding of P lost is added by a second product for clips of so many units of keys: their rows'
+// few large probabilities make delta_m of the backward, and dA - delta_m, which then nearly cancel (2
+// keys: dq and dk six times as far off).  And for clips of a few rows of not many keys, whose few
+// roundings do not average out in any sum over the rows (two rows of 146 and 248 keys: o 1.5 times as far
+// off as its own rounding, 1.05 so; 17 rows of 1,000 keys or 16 of 1,100: 1.04).  The clip's own lengths
+// decide, not those that its batch is padded to.
+constexpr int kFewUnits = 4, kFineRows = 16, kFineUnits = 32;
+__host__ __device__ inline bool fine_clip(int64_t qlen, int64_t klen) {
+  return klen <= kFewUnits * kUnitRows || (qlen <= kFineRows && klen <= kFineUnits * kUnitRows);
+}
 
 struct DiffFwdArgs {
   const uint16_t *q, *k, *v;
@@ -247,53 +255,49 @@ __global__ __launch_bounds__(256, 2) void diff_fwd_kernel(DiffFwdArgs a) {
   // last stage that the wave has keys in come behind the loop, and then the waits and loads alone.
   const int wn = min(nt, (wany + kUnitRows - 1) / kUnitRows);
   const unsigned char* last = s0;
-  int tm = t0;
-  if (NQ == 1 && klen <= kFewUnits * kUnitRows) {  // a short clip in a padded batch: the second product too
-    load(t0 + 3, s3);
-    __builtin_amdgcn_s_waitcnt(wait_vm_lgkm0(0));
-    __builtin_amdgcn_s_barrier();
-    for (; tm < wn; ++tm) {
-      const int x = tm - t0;
-      const unsigned char* s = x == 0 ? s0 : x == 1 ? s1 : x == 2 ? s2 : s3;
-#pragma unroll
-      for (int n = 0; n < NQ; ++n) {
-        scores(n, s);
-        mask_tile(sc[n], lim[n] - tm * kUnitRows, h);
-        raise_bound(lane_max(sc[n]), a.c, mx[n], lsum[n], acc[n]);
-        lsum[n] += probabilities<T16>(sc[n], a.c, mx[n], pr[n]);
-        lost_halves<T16>(sc[n], a.c, mx[n], pr[n], lo_);
-        values(n, s);
-        if (!FINE) {
-          pr[n][0] = lo_[0], pr[n][1] = lo_[1];
-          values(n, s);
-        }
-        pr[n][0] = pr[n][1] = lo_[0] = lo_[1] = u32x4{0, 0, 0, 0};
-      }
+  auto slot_of = [&](int t) __attribute__((always_inline)) {
+    const int x = (t - t0) % 5;
+    return x == 0 ? s0 : x == 1 ? s1 : x == 2 ? s2 : x == 3 ? s3 : s4;
+  };
+  if (NQ == 1 && !FINE && fine_clip(qlen, klen)) {  // a short clip in a padded batch, stage after stage
+    for (int t = t0; t < nt; ++t) {
+      __builtin_amdgcn_s_waitcnt(wait_vm_lgkm0(4));
+      __builtin_amdgcn_s_barrier();
+      load(t + 3, slot_of(t + 3));
+      if (t >= wn) continue;
+      const unsigned char* s = slot_of(t);
+      scores(0, s);
+      mask_tile(sc[0], lim[0] - t * kUnitRows, h);
+      raise_bound(lane_max(sc[0]), a.c, mx[0], lsum[0], acc[0]);
+      lsum[0] += probabilities<T16>(sc[0], a.c, mx[0], pr[0]);
+      lost_halves<T16>(sc[0], a.c, mx[0], pr[0], lo_);
+      values(0, s);
+      pr[0][0] = lo_[0], pr[0][1] = lo_[1];
+      values(0, s);
     }
-    tm = nt;
-  }
-  for (int t = tm; t < wn; t += 5) {
-    stage(t, t == t0 ? s0 : s4, s0, s1, s3);
-    last = s0;
-    if (t + 1 >= wn) break;
-    stage(t + 1, s0, s1, s2, s4);
-    last = s1;
-    if (t + 2 >= wn) break;
-    stage(t + 2, s1, s2, s3, s0);
-    last = s2;
-    if (t + 3 >= wn) break;
-    stage(t + 3, s2, s3, s4, s1);
-    last = s3;
-    if (t + 4 >= wn) break;
-    stage(t + 4, s3, s4, s0, s2);
-    last = s4;
-  }
-  values(NQ - 1, last);
-  for (int t = max(wn, tm); t < nt; ++t) {
-    __builtin_amdgcn_s_waitcnt(wait_vm_lgkm0(4));
-    __builtin_amdgcn_s_barrier();
-    const int x = (t + 3 - t0) % 5;
-    load(t + 3, x == 0 ? s0 : x == 1 ? s1 : x == 2 ? s2 : x == 3 ? s3 : s4);
+  } else {
+    for (int t = t0; t < wn; t += 5) {
+      stage(t, t == t0 ? s0 : s4, s0, s1, s3);
+      last = s0;
+      if (t + 1 >= wn) break;
+      stage(t + 1, s0, s1, s2, s4);
+      last = s1;
+      if (t + 2 >= wn) break;
+      stage(t + 2, s1, s2, s3, s0);
+      last = s2;
+      if (t + 3 >= wn) break;
+      stage(t + 3, s2, s3, s4, s1);
+      last = s3;
+      if (t + 4 >= wn) break;
+      stage(t + 4, s3, s4, s0, s2);
+      last = s4;
+    }
+    values(NQ - 1, last);
+    for (int t = max(wn, t0); t < nt; ++t) {
+      __builtin_amdgcn_s_waitcnt(wait_vm_lgkm0(4));
+      __builtin_amdgcn_s_barrier();
+      load(t + 3, slot_of(t + 3));
+    }
   }
   __builtin_amdgcn_s_waitcnt(wait_vm_lgkm0(0));  // no load into this LDS outlives the workgroup
 
@@ -702,9 +706,8 @@ FwdPlan fwd_plan(int B, int H, int Hkv, int64_t Lq, int64_t Lk, bool causal, boo
   const float share = kShares[causal][lens];
   // A group's rows in one tile read their keys once (us, in this form / in query blocks: 64 clips, H = 16,
   // Hkv = 2, 1 query, 2,000 keys 23 / 64; 1 clip, 29,952 keys 18 / 27; 32 clips, 32, 4, 4 queries
-  // 27 / 48; in two tiles and more: 8 clips, 16, 2, 16 queries 20 / 18).  A row of few keys needs the second
-  // product: the rounding of P_m is a part of delta_m, and of dA - delta_m, which then nearly cancel (2
-  // keys: dq and dk six times as far off; 100 of 100 keys 10 / 8 us).
+  // 27 / 48; in two tiles and more: 8 clips, 16, 2, 16 queries 20 / 18), and so do calls of few keys, with
+  // their second product (100 of 100 keys 10 / 8 us without it).
   if (units <= kFewUnits || (rep > 1 && rep * Lq <= 32)) {
     p.qtiles = (rep * Lq + 31) / 32;
     const int64_t blocks = bk * p.qtiles;
@@ -734,10 +737,9 @@ FwdPlan fwd_plan(int B, int H, int Hkv, int64_t Lq, int64_t Lk, bool causal, boo
   if (p.nq == 2) p.splits = 1;
   p.qtiles = p.nq == 2 ? q2 : q1;
   p.nwork = bp * p.qtiles;
-  // A few rows of not many keys have few roundings to average out (two rows of 146 and 248 keys: o 1.5
-  // times as far off as its own rounding, 1.05 with the second products).  us without / with, 8 heads, 1
-  // query: 1,000 keys 10.1 / 10.8, 64 clips of 1,000 26.3 / 28.7; of 29,952 keys it would be 19.8 / 21.8.
-  p.fine = p.nq == 1 && Lq <= 16 && units <= 32;
+  // (all clips of the call: one body for it.  us without / with the second products, 8 heads, 1 query:
+  // 1,000 keys 10.1 / 10.8, 64 clips of 1,000 26.3 / 28.7; of 29,952 keys it would be 19.8 / 21.8)
+  p.fine = p.nq == 1 && fine_clip(Lq, Lk);
   return p;
 }
 
