@@ -36,11 +36,17 @@ struct Scaled<F16> {
 // What the rounding of dS to 16 bits lost is added by a second product.  dq (its rounding alone would
 // make it 1.5 times as far off as a rounded exact result): in all stages of sequences of at most
 // kFineKeys keys or kFineRows queries and of causal waves that see at most kFineRows keys, else in
-// every second stage (1.25 times; B = 1, H = 8, L = 29,952: 0.4 ms).  dk, dv: calls of at most
-// kFineRows rows per key pair, or of one block of keys, whose few large probabilities round alike in
-// row after row, and others that are one small launch (longer sums average the roundings out).
-constexpr int kFineKeys = 4096, kFineRows = 512;
+// every second stage (1.25 times; B = 1, H = 8, L = 29,952: 0.4 ms).  dk, dv: clips of at most
+// kFineSums rows per key pair, or of one block of keys, whose few large probabilities round alike in
+// row after row; longer sums average the roundings out (dk without them, in units of its own rounding, not
+// causal / causal: 130 rows 1.37 / 1.42, 600 1.27 / 1.34, 2,000 1.13 / 1.23, with them 1.00 to 1.04).  A
+// clip's own lengths decide, whatever its batch is padded to.  us for the backward of 8 heads without / with
+// them: 1,000 tokens 36 / 41, 16 clips of 1,000 176 / 199, eight of 100 to 2,000 250 / 293.
+constexpr int kFineKeys = 4096, kFineRows = 512, kFineSums = 2048;
 constexpr int kKeyRows = 128;  // keys of a workgroup of dk and dv
+__host__ __device__ inline bool fine_clip(int64_t rep, int64_t qlen, int64_t klen) {
+  return rep * qlen <= kFineSums || klen <= kKeyRows;
+}
 constexpr int kNormRows = 64;  // rows of a partial maximum of the norms and of a partial sum of dlam
 
 struct DiffBwdArgs {
@@ -407,10 +413,10 @@ __device__ inline float row_value_at(float x, int e) {  // e a constant where it
 // statistic belongs to one register of a score tile in all lanes of a half: a lane reads one value, and
 // the add takes it from there (DPP).
 template <typename T16, bool CAUSAL, bool FINE>
-__device__ inline __attribute__((always_inline)) void dkdv_of(const DiffBwdArgs& a, int blk,
-                                                              unsigned char* r0, unsigned char* r1,
-                                                              float (*t0_)[64], float (*t1_)[64],
-                                                              unsigned char* vt) {
+__device__ inline __attribute__((always_inline)) void dkdv_body(const DiffBwdArgs& a, int blk,
+                                                                unsigned char* r0, unsigned char* r1,
+                                                                float (*t0_)[64], float (*t1_)[64],
+                                                                unsigned char* vt) {
   int bk, item;
   if (!work_item(a.kv_map, blk, bk, item)) return;
   const int ktile = item / a.kv_splits, sp = item - ktile * a.kv_splits;
@@ -652,26 +658,49 @@ __device__ inline __attribute__((always_inline)) void dkdv_of(const DiffBwdArgs&
   }
 }
 
-// The launches.  Calls that take the lost halves everywhere and those whose workgroups are all resident
-// at once: both in one, side by side, with the lost halves (us for the backward of 8 heads, in one / one
-// after the other: 600 tokens 36 / 48, 1,000 43 / 55, causal 44 / 52, 2,000 75 / 78; 600 queries of 5,000
-// keys 58 / 68).  Of others the two bodies under one allocation spill 20 registers (29,952 tokens: 7.65
-// ms, one after the other 7.2).
-template <typename T16, bool CAUSAL>
+// The launches.  dk and dv with the lost halves in all clips (fine_clip), in none, or in those whose own
+// lengths ask for them: both bodies, a workgroup takes one (clips of 4,159, 2,703 and 1,247 tokens, which
+// take none, causal: 226 us for 230).
+enum { kNone, kAll, kByClip };
+template <typename T16, bool CAUSAL, int LOST>
+__device__ inline __attribute__((always_inline)) void dkdv_of(const DiffBwdArgs& a, int blk,
+                                                              unsigned char* r0, unsigned char* r1,
+                                                              float (*t0_)[64], float (*t1_)[64],
+                                                              unsigned char* vt) {
+  bool fine = LOST == kAll;
+  if (LOST == kByClip) {
+    int bk, item;
+    if (!work_item(a.kv_map, blk, bk, item)) return;
+    const int b = bk / a.Pk;
+    fine = fine_clip(a.rep, seq_len(a.q_lens, b, a.Lq), seq_len(a.k_lens, b, a.Lk));
+  }
+  if (fine)
+    dkdv_body<T16, CAUSAL, true>(a, blk, r0, r1, t0_, t1_, vt);
+  else
+    dkdv_body<T16, CAUSAL, false>(a, blk, r0, r1, t0_, t1_, vt);
+}
+
+// Calls whose clips all take the lost halves and those whose workgroups are all resident at once: both in
+// one launch, side by side (us for the backward of 8 heads, in one / one after the other: 600 tokens 36 /
+// 48, 1,000 41 / 54, causal 44 / 52, 2,500 90 / 104; 600 queries of 5,000 keys 58 / 68).  Of others the
+// two bodies under one allocation spill 20 registers (29,952 tokens: 7.65 ms, one after the other 7.2).
+// Spilled in what is kept: 12 to 47 registers in one launch, 4 to 27 with both bodies of dk and dv, 9 to
+// 12 in dq's own; none in dk and dv's without the lost halves.
+template <typename T16, bool CAUSAL, int LOST>
 __global__ __launch_bounds__(256, 2) void diff_bwd_few_kernel(DiffBwdArgs a) {
   __shared__ __align__(16) unsigned char s0[kStageB], s1[kStageB], v[2 * kStageB];
   __shared__ __align__(16) float t0_[4][64], t1_[4][64];
   const int blk = blockIdx.x;
   if (blk < a.kv_blocks)
-    dkdv_of<T16, CAUSAL, true>(a, blk, s0, s1, t0_, t1_, v);
+    dkdv_of<T16, CAUSAL, LOST>(a, blk, s0, s1, t0_, t1_, v);
   else
     dq_of<T16>(a, blk - a.kv_blocks, s0, s1, v, v + kStageB);
 }
-template <typename T16, bool CAUSAL>
+template <typename T16, bool CAUSAL, int LOST>
 __global__ __launch_bounds__(256, 2) void diff_bwd_dkdv_kernel(DiffBwdArgs a) {
   __shared__ __align__(16) unsigned char s0[kStageB], s1[kStageB], v[2 * kStageB];
   __shared__ __align__(16) float t0_[4][64], t1_[4][64];
-  dkdv_of<T16, CAUSAL, false>(a, blockIdx.x, s0, s1, t0_, t1_, v);
+  dkdv_of<T16, CAUSAL, LOST>(a, blockIdx.x, s0, s1, t0_, t1_, v);
 }
 template <typename T16>
 __global__ __launch_bounds__(256, 2) void diff_bwd_dq_kernel(DiffBwdArgs a) {
@@ -825,16 +854,31 @@ extern "C" int sla2h_diff_attn_bwd(const void* q, const void* k, const void* v, 
     diff_bwd_prep_kernel<T16><<<(unsigned)(pq + pv), 256, 0, st>>>(a, pq);
     if ((err = (int)hipGetLastError())) return err;
     const unsigned nq = (unsigned)(a.dq_blocks + a.P), nk = (unsigned)a.kv_blocks;
+    const bool all = fine_clip(a.rep, Lq, Lk);
     // (whether or not both are asked for: a gradient does not depend on the others)
-    const bool together = work_grid(a.kv_map) + work_grid(a.dq_map) <= 512;
-    if (a.rep * Lq <= kFineRows || Lk <= kKeyRows || together) {
-      if (causal)
-        diff_bwd_few_kernel<T16, true><<<nk + nq, 256, 0, st>>>(a);
+    const bool one = all || work_grid(a.kv_map) + work_grid(a.dq_map) <= 512;
+    using std::integral_constant;
+    auto launch = [&](auto causal_, auto lost) {
+      constexpr bool CAUSAL = decltype(causal_)::value;
+      constexpr int LOST = decltype(lost)::value;
+      if (one)
+        diff_bwd_few_kernel<T16, CAUSAL, LOST><<<nk + nq, 256, 0, st>>>(a);
+      else if constexpr (LOST != kAll)
+        if (dk) diff_bwd_dkdv_kernel<T16, CAUSAL, LOST><<<nk, 256, 0, st>>>(a);
+    };
+    auto lost = [&](auto causal_) {
+      if (all)
+        launch(causal_, integral_constant<int, kAll>{});
+      else if (q_lens || k_lens)
+        launch(causal_, integral_constant<int, kByClip>{});
       else
-        diff_bwd_few_kernel<T16, false><<<nk + nq, 256, 0, st>>>(a);
-    } else {
-      if (dk && causal) diff_bwd_dkdv_kernel<T16, true><<<nk, 256, 0, st>>>(a);
-      if (dk && !causal) diff_bwd_dkdv_kernel<T16, false><<<nk, 256, 0, st>>>(a);
+        launch(causal_, integral_constant<int, kNone>{});
+    };
+    if (causal)
+      lost(std::true_type{});
+    else
+      lost(std::false_type{});
+    if (!one) {
       if ((err = (int)hipGetLastError())) return err;
       diff_bwd_dq_kernel<T16><<<nq, 256, 0, st>>>(a);
     }
