@@ -26,6 +26,12 @@ def newton_schulz(g, steps=5, coeffs=ops.NS_COEFFS):
             and not (g.requires_grad and torch.is_grad_enabled())):
         return ops.orthogonalize(g, steps, coeffs)
     ops._ns_coeffs(steps, ops.ns_rows(steps, coeffs))  # its checks
+    # (autocast would make the products 16-bit ones)
+    with torch.autocast("cuda" if g.is_cuda else "cpu", enabled=False):
+        return _products(g, steps, coeffs)
+
+
+def _products(g, steps, coeffs):
     x = g.to(torch.promote_types(g.dtype, torch.float32))
     if g.shape[-2] > g.shape[-1]:
         x = x.transpose(-1, -2)
